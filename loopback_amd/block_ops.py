@@ -1,0 +1,318 @@
+"""Operators of a transformer block's training step on the HIP kernels of libloopback_block.so (include/loopback_block.h):
+
+  * `block_join(x, y, ...)`: a block's output y back on the residual stream x, with the norm after the block, a gate, a
+    residual scale and dropout before the add, and the next block's norm after it;
+  * `dropout(x, p, rng, site)`: dropout whose mask comes from a counter-based generator and is never stored.
+
+The kernels take plain fp32, bf16 and fp16 tensors of the current GPU where nothing has to see torch operations (lm_ops.native
+says what does); everything else -- the CPU, other types, tracers, transforms -- runs the torch form of the same operator:
+the same formulas and the same masks. A backward that is itself differentiated, or watched, runs the torch form too. Tensors
+of any strides are taken (the kernels work on contiguous rows; others are copied).
+
+Dropout's generator: `rng` is an int64 tensor (seed, step) on the inputs' device, read when a kernel runs: a captured graph
+draws a new mask when the program has changed it, and a backward reads it again, so the program changes a copy, not the
+tensor that a forward took, before that forward's backward (autograd refuses it otherwise). `site`, 0 to 2^32 - 1, tells the
+places of one step apart. The mask depends on (seed, step, site, row, column) alone.
+"""
+from __future__ import annotations
+
+import ctypes
+import os
+
+import torch
+
+from . import build as _build
+from .lm_ops import _again, _launchable, _stream, _watched, native
+
+ABI_VERSION = 1
+JOIN_MAX_WIDTH = 8192
+MAX_ROWS = 2 ** 31 - 1
+_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+_p, _i64, _i32, _u32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint32, ctypes.c_float
+# name -> (restype, argtypes); one line per declaration of include/loopback_block.h
+SIGNATURES = {
+    "lbk_abi_version": (_i32, []),
+    "lbk_dropout": (_i32, [_p, _p, _u32, _i32, _p, _i64, _i64, _i32, _p]),
+    "lbk_join_fwd": (_i32, [_p, _p, _p, _p, _i64, _p, _p, _u32, _i32, _f32, _f32, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
+    "lbk_join_scratch": (_i64, [_i64, _i64, _i64]),
+    "lbk_join_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _u32, _i32, _f32, _p, _p, _p, _p, _p, _p, _i64,
+                            _i64, _i32, _p]),
+}
+
+
+def _load() -> ctypes.CDLL:
+    path = _build.BLOCK_LIB
+    if not os.path.exists(path):
+        raise ImportError(f"loopback_block: {path} is not built (run `python -m loopback_amd.build`)")
+    lib = ctypes.CDLL(path)
+    for name, (res, args) in SIGNATURES.items():
+        fn = getattr(lib, name)          # AttributeError -> the library is stale
+        fn.restype, fn.argtypes = res, args
+    if lib.lbk_abi_version() != ABI_VERSION:
+        raise ImportError(f"loopback_block: {path} has ABI {lib.lbk_abi_version()}, expected {ABI_VERSION}; rebuild")
+    return lib
+
+
+LIB = _load()
+_FN = {name: getattr(LIB, name) for name in SIGNATURES}
+
+
+def _run(name: str, *args) -> None:
+    code = _FN[name](*args)
+    if code:
+        raise RuntimeError(f"{name}: refused or failed to launch (code {code})")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _upcast(t: torch.Tensor) -> torch.Tensor:
+    return t.float() if t.dtype in (torch.bfloat16, torch.float16) else t
+
+
+def _plain_rows(*tensors):
+    return [t if t is None or t.is_contiguous() else t.contiguous() for t in tensors]
+
+
+def _records(*tensors) -> bool:
+    """Whether a call on these records a backward."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# dropout
+# ---------------------------------------------------------------------------------------------------------------
+def _drop_of(p: float, rng, x, site) -> int:
+    """The probability's 65536ths, after the checks of dropout's arguments."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"a dropout probability lies in [0, 1], got {p}")
+    if not 0 <= site < 2 ** 32:
+        raise ValueError(f"site lies in [0, 2^32), got {site}")
+    drop = round(65536 * p)
+    if drop:
+        if not isinstance(rng, torch.Tensor) or rng.dtype is not torch.int64 or rng.shape != (2,):
+            raise ValueError("dropout needs rng, an int64 tensor (seed, step)")
+        if rng.device != x.device:
+            raise ValueError(f"rng is on {rng.device}, the input on {x.device}")
+    return drop
+
+
+def keep_mask(shape, p: float, rng: torch.Tensor, site: int = 0) -> torch.Tensor:
+    """The kept elements (bool, `shape`) of dropout(x, p, rng, site) for an x of this shape, in torch operations."""
+    shape = torch.Size(shape)
+    drop = _drop_of(p, rng, rng, site)
+    d = shape[-1] if shape else 1
+    rows = shape[:-1].numel()
+    return _mask(drop, rng, site, rows, d).view(shape)
+
+
+def _mask(drop: int, rng, site: int, rows: int, d: int) -> torch.Tensor:
+    """Philox-4x32-10 (Salmon et al., 2011) in 64-bit integers, a counter per row and eight columns, 16 bits a column."""
+    nb, low, dev = (d + 7) // 8, 0xFFFFFFFF, rng.device
+    c0 = torch.arange(nb, device=dev).expand(rows, nb)
+    c1 = torch.arange(rows, device=dev).unsqueeze(1).expand(rows, nb)
+    c2 = torch.full((rows, nb), site, device=dev, dtype=torch.int64)
+    c3 = (rng[1] & low).expand(rows, nb)
+    k0, k1 = rng[0] & low, (rng[0] >> 32) & low
+    for _ in range(10):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57      # modulo 2^64: the shifts below take the bits that are right
+        c0, c1, c2, c3 = ((b >> 32) & low) ^ c1 ^ k0, b & low, ((a >> 32) & low) ^ c3 ^ k1, a & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    w = torch.stack((c0, c1, c2, c3), -1)
+    return (torch.stack((w & 0xFFFF, w >> 16), -1).reshape(rows, 8 * nb)[:, :d] >= drop)
+
+
+def _dropout_torch(x, rng, site, drop):
+    d = x.shape[-1] if x.dim() else 1
+    keep = _mask(drop, rng, site, x.shape[:-1].numel(), d).view(x.shape)
+    s = 65536.0 / (65536 - drop) if drop < 65536 else 0.0
+    return torch.where(keep, _upcast(x) * s, 0.0).to(x.dtype)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, rng, site, drop):
+        ctx.site, ctx.drop = site, drop
+        ctx.save_for_backward(rng)
+        return _dropout_launch(x, rng, site, drop)
+
+    @staticmethod
+    def backward(ctx, dy):
+        rng, = ctx.saved_tensors
+        if _launchable(dy) and _dropout_native(dy, rng):
+            return _dropout_launch(dy.contiguous(), rng, ctx.site, ctx.drop), None, None, None
+        return _dropout_torch(dy, rng, ctx.site, ctx.drop), None, None, None
+
+
+def _dropout_native(x, rng) -> bool:
+    # autocast changes nothing here: the operation keeps its input's type
+    return ((native(x, codes=_CODES) or _autocast_only(x)) and x.dim() > 0 and x.numel() > 0
+            and x.shape[:-1].numel() <= MAX_ROWS and type(rng) is torch.Tensor and rng.is_contiguous())
+
+
+def _autocast_only(x) -> bool:
+    if _watched() or not x.is_cuda or not torch.is_autocast_enabled("cuda"):
+        return False
+    with torch.autocast("cuda", enabled=False):
+        return native(x, codes=_CODES)
+
+
+def _dropout_launch(x, rng, site, drop):
+    out = torch.empty_like(x)
+    d = x.shape[-1]
+    _run("lbk_dropout", x.data_ptr(), rng.data_ptr(), site, drop, out.data_ptr(), x.numel() // d, d, _CODES[x.dtype],
+         _stream(x))
+    return out
+
+
+def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0) -> torch.Tensor:
+    """x with each element dropped with probability p (to its 65536ths; 0 returns x) and the others multiplied by 1 / (1 - p);
+    what is dropped is 0, also where x is not finite. The rows of the generator are those of x's last dimension."""
+    if not x.is_floating_point():
+        raise ValueError(f"dropout takes floating point tensors, got {x.dtype}")
+    drop = _drop_of(p, rng, x, site)
+    if drop == 0:
+        return x
+    if not _dropout_native(x, rng):
+        return _dropout_torch(x, rng, site, drop)
+    x = x.contiguous()
+    return _Dropout.apply(x, rng, site, drop) if _records(x) else _dropout_launch(x, rng, site, drop)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# block join
+# ---------------------------------------------------------------------------------------------------------------
+def _rms_torch(x, w, eps):
+    """rms_norm of unrounded rows (fp32, or fp64 where those are given)."""
+    return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * _upcast(w)
+
+
+def _branch_torch(y, post, gate, rng, site, drop, scale, eps):
+    """What is added to the residual stream, unrounded."""
+    z = _upcast(y)
+    if post is not None:
+        z = _rms_torch(z, post, eps)
+    if gate is not None:
+        z = z * _upcast(gate)
+    z = z * scale
+    return _dropout_torch(z, rng, site, drop) if drop else z
+
+
+def _join_torch(x, y, post, gate, pre, rng, site, drop, scale, eps):
+    h = _upcast(x) + _branch_torch(y, post, gate, rng, site, drop, scale, eps)
+    return h.to(x.dtype), None if pre is None else _rms_torch(h, pre, eps).to(x.dtype)
+
+
+def _join_launch(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, keep):
+    """h, n and, with `keep`, the rows' scales for a backward. Contiguous tensors."""
+    d = x.shape[-1]
+    rows = x.numel() // d
+    h = torch.empty_like(x)
+    n = None if pre is None else torch.empty_like(x)
+    r_post = torch.empty(rows, device=x.device, dtype=torch.float32) if keep and post is not None else None
+    r_pre = torch.empty(rows, device=x.device, dtype=torch.float32) if keep and pre is not None else None
+    _run("lbk_join_fwd", x.data_ptr(), y.data_ptr(), _ptr(post), _ptr(gate), gate_rows, _ptr(pre),
+         rng.data_ptr() if drop else None, site, drop, scale, eps, h.data_ptr(), _ptr(n), _ptr(r_post), _ptr(r_pre), rows, d,
+         _CODES[x.dtype], _stream(x))
+    return h, n, r_post, r_pre
+
+
+class _Join(torch.autograd.Function):
+    """(h, n): the two take their gradients into one kernel. Saves h, y and the rows' scales."""
+
+    @staticmethod
+    def forward(ctx, x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps):
+        h, n, r_post, r_pre = _join_launch(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, True)
+        ctx.args = gate_rows, site, drop, scale, eps
+        ctx.save_for_backward(h if pre is not None else None, y, post, gate, pre, r_post, r_pre, rng if drop else None)
+        ctx.set_materialize_grads(False)
+        return h, n
+
+    @staticmethod
+    def backward(ctx, dh, dn):
+        gate_rows, site, drop, scale, eps = ctx.args
+        # a saved-tensor hook may give a tensor back with other strides than it was saved with
+        h, y, post, gate, pre, r_post, r_pre, rng = _plain_rows(*ctx.saved_tensors)
+        need = ctx.needs_input_grad
+        nx, ny, npost, ngate, npre = need[0], need[1], need[2], need[3], need[5] and dn is not None
+        out = [None] * 11
+        if dh is None and dn is None:
+            return tuple(out)
+        if not _launchable(dh, dn):
+            g = dh
+            if dn is not None:
+                gh, out[5] = _again(lambda h, w: _rms_torch(_upcast(h), w, eps).to(h.dtype), [h, pre], [True, npre], dn)
+                g = gh if dh is None else dh + gh
+            out[0] = g if nx else None
+            inputs = [t for t in (y, post, gate) if t is not None]
+            asked = [n for n, t in ((ny, y), (npost, post), (ngate, gate)) if t is not None]
+
+            def branch(*ts):
+                it = iter(ts)
+                return _branch_torch(next(it), None if post is None else next(it), None if gate is None else next(it), rng,
+                                     site, drop, scale, eps).to(g.dtype)
+
+            got = iter(_again(branch, inputs, asked, g))
+            out[1] = next(got)
+            out[2] = None if post is None else next(got)
+            out[3] = None if gate is None else next(got)
+            return tuple(out)
+        d = y.shape[-1]
+        rows = y.numel() // d
+        dh, dn = _plain_rows(None if dh is None else dh.to(y.dtype), None if dn is None else dn.to(y.dtype))
+        new = lambda wanted, like: torch.empty_like(like) if wanted else None
+        dx, dy, dpost, dgate, dpre = new(nx, y), new(ny, y), new(npost, post), new(ngate, gate), new(npre, pre)
+        scratch = None
+        if npost or ngate or npre:
+            scratch = torch.empty(LIB.lbk_join_scratch(rows, d, gate_rows), device=y.device, dtype=torch.float32)
+        if nx or ny or scratch is not None:
+            _run("lbk_join_bwd", _ptr(dh), _ptr(dn), _ptr(h), y.data_ptr(), _ptr(post), _ptr(gate), gate_rows, _ptr(pre),
+                 _ptr(r_post), _ptr(r_pre), _ptr(rng), site, drop, scale, _ptr(dx), _ptr(dy), _ptr(dpost), _ptr(dgate),
+                 _ptr(dpre), _ptr(scratch), rows, d, _CODES[y.dtype], _stream(y))
+        out[0], out[1], out[2], out[3], out[5] = dx, dy, dpost, dgate, dpre
+        return tuple(out)
+
+
+def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
+    """The consecutive rows of x that share a row of the gate: (d,), or x's dimensions with the last leading ones 1."""
+    lead, gl = x.shape[:-1], gate.shape[:-1]
+    if gate.dim() >= 1 and gate.shape[-1] == x.shape[-1]:
+        if gate.dim() == 1:
+            return max(1, lead.numel())
+        if len(gl) == len(lead):
+            for k in range(len(lead) + 1):
+                if gl[:k] == lead[:k] and all(s == 1 for s in gl[k:]):
+                    return max(1, lead[k:].numel())
+    raise ValueError(f"a gate for {tuple(x.shape)} is ({x.shape[-1]},) or has x's dimensions, the last of those before the "
+                     f"width 1: got {tuple(gate.shape)}")
+
+
+def block_join(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor | None = None,
+               gate: torch.Tensor | None = None, scale: float = 1.0, dropout: float = 0.0,
+               rng: torch.Tensor | None = None, site: int = 0, pre_weight: torch.Tensor | None = None, eps: float = 1e-6):
+    """(h, n) of a residual stream x and a block's output y of one shape (..., d):
+
+        h = x + drop(scale * gate * rms_norm(y) post_weight),   n = rms_norm(h) pre_weight
+
+    Each of post_weight (d,), gate, dropout and pre_weight may be left out (n is then None, for pre_weight). The gate is one
+    row (d,), a row for each of the leading dimensions ((b, 1, d) for (b, t, d): one per sequence), or x's shape. h and n are
+    each rounded once, n from the unrounded sum. Differentiable in x, y, post_weight, gate and pre_weight."""
+    if y.shape != x.shape or not x.is_floating_point() or x.dim() < 1:
+        raise ValueError(f"block_join takes two floating point tensors of one shape, got {tuple(x.shape)} and {tuple(y.shape)}")
+    d = x.shape[-1]
+    for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if w is not None and w.shape != (d,):
+            raise ValueError(f"{name} has the width's shape ({d},), got {tuple(w.shape)}")
+    gate_rows = 1 if gate is None else _gate_rows(gate, x)
+    drop = _drop_of(dropout, rng, x, site)
+    scale, eps = float(scale), float(eps)
+    ts = [t for t in (x, y, post_weight, gate, pre_weight) if t is not None]
+    if not (native(*ts, codes=_CODES) and x.numel() > 0 and d <= JOIN_MAX_WIDTH and x.numel() // d <= MAX_ROWS
+            and (not drop or (type(rng) is torch.Tensor and rng.is_contiguous()))):
+        return _join_torch(x, y, post_weight, gate, pre_weight, rng, site, drop, scale, eps)
+    x, y, post_weight, gate, pre_weight = _plain_rows(x, y, post_weight, gate, pre_weight)   # recorded, where they copy
+    if _records(*ts):
+        return _Join.apply(x, y, post_weight, gate, gate_rows, pre_weight, rng, site, drop, scale, eps)
+    return _join_launch(x, y, post_weight, gate, gate_rows, pre_weight, rng, site, drop, scale, eps, False)[:2]

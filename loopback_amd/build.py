@@ -1,5 +1,5 @@
-"""Build libloopback_read.so (the read's kernels and C ABI) and libloopback_lm.so (the language model's) in-tree with
-hipcc for gfx950 (MI355X), and _host.so, the Python module's launch path, with g++ against torch's headers.
+"""Build libloopback_read.so (the read's kernels and C ABI), libloopback_lm.so (the language model's) and
+libloopback_block.so (a block's feed-forward, join and dropout) in-tree with hipcc for gfx950 (MI355X), and _host.so, the Python module's launch path, with g++ against torch's headers.
 
     python -m loopback_amd.build                          # compile, print the commands
     python -m loopback_amd.build -D LDR_RF_GRID=768 ...   # with launch settings other than the measured defaults
@@ -26,6 +26,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "libloopback_read.so")
 LM_SRC = os.path.join(HERE, "csrc", "loopback_lm.hip")
 LM_LIB = os.path.join(HERE, "libloopback_lm.so")
+BLOCK_SRC = os.path.join(HERE, "csrc", "loopback_block.hip")
+BLOCK_LIB = os.path.join(HERE, "libloopback_block.so")
 HOST_SRC = os.path.join(HERE, "csrc", "host.cpp")
 HOST_LIB = os.path.join(HERE, "_host.so")
 # A test fixture: the same source built with the alternative kernel shapes -- the write in the matrix cores' layout
@@ -128,14 +130,15 @@ def build(verbose: bool = True, defines=None, fixtures: bool = True) -> str:
     path. Every compile started is waited for before any error is raised. A library's failure raises; a test
     fixture's is reported on stderr and does not fail the library's build (the GPU tests that load the fixture then
     fail on its absence). defines: NAME=VALUE launch settings (see the module docstring)."""
-    jobs = [_start(SRC, LIB, verbose, defines), _start(LM_SRC, LM_LIB, verbose, []), _start_host(verbose)]
+    jobs = [_start(SRC, LIB, verbose, defines), _start(LM_SRC, LM_LIB, verbose, []),
+            _start(BLOCK_SRC, BLOCK_LIB, verbose, []), _start_host(verbose)]
     if fixtures:
         jobs.append(_start(SRC, TEST_LIB_ALT, verbose, list(defines or []) + ALT_DEFINES))
     errors = [_wait(job) for job in jobs]
-    for e in errors[:3]:
+    for e in errors[:4]:
         if e is not None:
             raise RuntimeError(e)
-    fixture_errors = [e for e in errors[3:] if e is not None]
+    fixture_errors = [e for e in errors[4:] if e is not None]
     if fixtures and not fixture_errors:
         try:
             build_abi_smoke(verbose)

@@ -84,7 +84,7 @@ def _watched() -> bool:
             or _transform() is not None)
 
 
-def native(*tensors) -> bool:
+def native(*tensors, codes=_CODES) -> bool:
     # what watches the call first, then what the arguments are: a tracer's arguments (fake tensors, proxies) are not
     # asked for a device, and a compiler meets no query of the GPU
     if _watched():
@@ -93,7 +93,7 @@ def native(*tensors) -> bool:
     for t in tensors:
         if type(t) is not _Tensor and type(t) is not _Parameter:
             return False
-    if not first.is_cuda or first.dtype not in _CODES or first.device.index != torch._C._cuda_getDevice():
+    if not first.is_cuda or first.dtype not in codes or first.device.index != torch._C._cuda_getDevice():
         return False
     for t in tensors[1:]:
         if t.dtype is not first.dtype or t.device != first.device:

@@ -1,0 +1,148 @@
+"""block_ops on the CPU: the library and its refusals, the generator's published test vectors, the torch forms against the
+formulas in fp64 and against differences, the checks of arguments."""
+import os
+import re
+
+import pytest
+import torch
+
+from loopback_amd import block_ops as ops
+from loopback_amd import rocprof_summary as RS
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def rnd(shape, seed, dtype=torch.float64):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64).to(dtype)
+
+
+def test_library():
+    """The library exports what include/loopback_block.h declares and the binding's table is the header's."""
+    with open(os.path.join(ROOT, "include", "loopback_block.h")) as f:
+        text = f.read()
+    names = set(re.findall(r"\b(lbk_\w+)\s*\(", re.sub(r"/\*.*?\*/", "", text, flags=re.S)))
+    assert names == set(ops.SIGNATURES) and all(hasattr(ops.LIB, n) for n in names)
+    define = lambda n: int(re.search(rf"#define {n} (\d+)", text).group(1))
+    assert define("LBK_ABI_VERSION") == ops.ABI_VERSION and define("LBK_JOIN_MAX_WIDTH") == ops.JOIN_MAX_WIDTH
+
+
+def test_row_kernels_refuse():
+    """Calls whose operands the kernels do not take are refused before any launch; empty ones return at once."""
+    L, p, null = ops.LIB, 4096, None
+    drop = lambda x=p, rng=p, d=16, rows=4, drop=100, dt=1: L.lbk_dropout(x, rng, 0, drop, p, rows, d, dt, null)
+    assert drop(dt=3) == -4 and drop(rows=-1) == -1 and drop(d=0) == -1 and drop(drop=65537) == -1 and drop(drop=-1) == -1
+    assert drop(rows=2 ** 31) == -2 and drop(x=null) == -1 and drop(rng=null) == -1 and drop(x=4097) == -3
+    assert drop(rng=4100) == -3 and drop(rows=0) == 0 and drop(x=4098, dt=0) == -3
+    fwd = lambda x=p, n=p, gate=null, gr=1, pre=p, rng=null, dr=0, rows=4, d=64, dt=1, h=p: L.lbk_join_fwd(
+        x, p, p, gate, gr, pre, rng, 0, dr, 1.0, 1e-6, h, n, p, p, rows, d, dt, null)
+    assert fwd(dt=7) == -4 and fwd(d=0) == -1 and fwd(rows=-1) == -1 and fwd(d=8193) == -2 and fwd(rows=2 ** 31) == -2
+    assert fwd(x=null) == -1 and fwd(n=null) == -1 and fwd(h=null) == -1 and fwd(gate=p, gr=0) == -1 and fwd(dr=5) == -1
+    assert fwd(x=4097) == -3 and fwd(rng=4100, dr=5) == -3 and fwd(rows=0, x=null) == 0
+    bwd = lambda dh=p, dn=p, h=p, y=p, pre=p, post=p, rpo=p, gate=null, dgate=null, s=p, rows=4: L.lbk_join_bwd(
+        dh, dn, h, y, post, gate, 1, pre, rpo, p, null, 0, 0, 1.0, p, p, p, dgate, p, s, rows, 64, 1, null)
+    assert bwd(dh=null, dn=null) == -1 and bwd(h=null) == -1 and bwd(y=null) == -1 and bwd(pre=null) == -1
+    assert bwd(rpo=null) == -1 and bwd(post=null) == -1 and bwd(dgate=p) == -1 and bwd(s=null) == -1 and bwd(rows=0) == 0
+    assert bwd(dn=null) == -1 and bwd(dh=4097) == -3 and bwd(s=4098) == -3   # dpre without dn
+    assert L.lbk_join_scratch(0, 64, 1) == 0 and L.lbk_join_scratch(4, 9000, 1) == 0
+    assert L.lbk_join_scratch(1, 64, 1) == 4 * 64
+
+
+def test_generator_vectors():
+    """Philox-4x32-10's published known answers, as the halves of its words: counters and keys of zeros and of ones."""
+    def bits(seed, step, site, row, block):
+        lo, hi = torch.zeros(8, dtype=torch.int64), torch.full((8,), 65537)
+        rng = torch.tensor([seed, step])
+        while (hi - lo > 1).any():   # the largest `drop` at which an element is kept is its 16 bits
+            mid = (lo + hi) // 2
+            keep = torch.stack([ops._mask(int(m), rng, site, row + 1, 8 * block + 8)[row, 8 * block + k] for k, m in enumerate(mid)])
+            lo, hi = torch.where(keep, mid, lo), torch.where(keep, hi, mid)
+        return [int(a) + (int(b) << 16) for a, b in zip(lo[::2], lo[1::2])]
+
+    assert bits(0, 0, 0, 0, 0) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    # counter (block, row, site, step) and key halves beyond 2^31: signs of 64-bit products
+    import numpy as np
+
+    def numpy_words(c, k):
+        u, m = np.uint64, np.uint64(0xFFFFFFFF)
+        c, k = [u(v) for v in c], [u(v) for v in k]
+        for _ in range(10):
+            a, b = c[0] * u(0xD2511F53), c[2] * u(0xCD9E8D57)
+            c = [(b >> u(32)) ^ c[1] ^ k[0], b & m, (a >> u(32)) ^ c[3] ^ k[1], a & m]
+            k = [(k[0] + u(0x9E3779B9)) & m, (k[1] + u(0xBB67AE85)) & m]
+        return [int(v) for v in c]
+
+    assert numpy_words([0xFFFFFFFF] * 4, [0xFFFFFFFF] * 2) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert numpy_words([0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344], [0xA4093822, 0x299F31D0]) == \
+        [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+    for seed, step, site, row, block in ((-1, 2 ** 32 - 1, 2 ** 32 - 1, 5, 3), (-2 ** 63, 7, 2 ** 31, 0, 1),
+                                         (0x299F31D0A4093822, 0x03707344, 0x13198A2E, 2, 2)):
+        assert bits(seed, step, site, row, block) == numpy_words([block, row, site, step & 0xFFFFFFFF],
+                                                                 [seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF])
+
+
+def test_dropout_form():
+    """The share that is kept, its scale, the mask's independence of type and strides, and of other places and steps."""
+    x, rng = torch.ones(300, 1001), torch.tensor([5, 1])
+    y = ops.dropout(x, 0.1, rng, site=2)
+    keep = ops.keep_mask((300, 1001), 0.1, rng, site=2)
+    s = 65536 / (65536 - round(65536 * 0.1))
+    assert torch.equal(y, keep * torch.tensor(s)) and abs(keep.double().mean() - 1 / s) < 4 * (0.09 / 300300) ** 0.5
+    assert torch.equal(ops.dropout(x.t().contiguous().t().double(), 0.1, rng, site=2), keep.double() * s)
+    for other in (ops.keep_mask((300, 1001), 0.1, torch.tensor([5, 2]), 2), ops.keep_mask((300, 1001), 0.1, rng, 3),
+                  ops.keep_mask((300, 1001), 0.1, torch.tensor([6, 1]), 2)):
+        agree = (other == keep).double().mean()
+        assert abs(agree - 0.82) < 4 * (0.82 * 0.18 / 300300) ** 0.5
+    assert ops.dropout(x, 0.0, None) is x and not ops.dropout(x, 1.0, rng).any()
+    assert torch.equal(ops.dropout(x.bfloat16(), 0.1, rng, site=2), y.bfloat16())
+    assert ops.dropout(torch.ones(()), 0.5, rng).shape == () and ops.dropout(torch.ones(0, 4), 0.5, rng).shape == (0, 4)
+
+
+@pytest.mark.parametrize("gate", [None, (6,), (2, 1, 6), (2, 3, 6)])
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("pre", [True, False])
+def test_join_form_against_differences(gate, post, pre):
+    """The torch form's gradients against central differences in fp64."""
+    rng = torch.tensor([3, 4])
+    args = [rnd((2, 3, 6), 1), rnd((2, 3, 6), 2), *([rnd((6,), 3)] if post else []), *([rnd(gate, 4)] if gate else []),
+            *([rnd((6,), 5)] if pre else [])]
+
+    def fn(x, y, *rest):
+        it = iter(rest)
+        h, n = ops.block_join(x, y, post_weight=next(it) if post else None, gate=next(it) if gate else None, scale=0.6,
+                              dropout=0.3, rng=rng, site=1, pre_weight=next(it) if pre else None)
+        return (h,) if n is None else (h, n)
+
+    assert torch.autograd.gradcheck(fn, [a.requires_grad_() for a in args])
+
+
+def test_join_form_values():
+    x, y, w, g, v = rnd((4, 10), 1), rnd((4, 10), 2), rnd((10,), 3), rnd((4, 10), 4), rnd((10,), 5)
+    h, n = ops.block_join(x, y, post_weight=w, gate=g, scale=-2.0, pre_weight=v, eps=0.1)
+    z = torch.nn.functional.rms_norm(y, (10,), w, 0.1) * g * -2.0
+    assert torch.allclose(h, x + z, atol=1e-12) and torch.allclose(n, torch.nn.functional.rms_norm(x + z, (10,), v, 0.1), atol=1e-12)
+    h, n = ops.block_join(x.bfloat16(), y.bfloat16())
+    assert n is None and torch.equal(h, (x.bfloat16().float() + y.bfloat16().float()).bfloat16())
+
+
+def test_arguments():
+    x, w, rng = torch.zeros(2, 3, 8), torch.ones(8), torch.tensor([1, 2])
+    for bad in (lambda: ops.dropout(x, 1.5, rng), lambda: ops.dropout(x, -0.1, rng), lambda: ops.dropout(x, float("nan"), rng),
+                lambda: ops.dropout(x, 0.5, None), lambda: ops.dropout(x, 0.5, rng.int()), lambda: ops.dropout(x, 0.5, rng[:1]),
+                lambda: ops.dropout(x, 0.5, rng, site=-1), lambda: ops.dropout(x, 0.5, rng, site=2 ** 32),
+                lambda: ops.dropout(x.long(), 0.5, rng), lambda: ops.block_join(x, x[:1]), lambda: ops.block_join(x, x.view(6, 8)),
+                lambda: ops.block_join(x, x, post_weight=w[:4]), lambda: ops.block_join(x, x, pre_weight=w.view(1, 8)),
+                lambda: ops.block_join(x, x, gate=torch.ones(3, 8)), lambda: ops.block_join(x, x, gate=torch.ones(1, 3, 8)),
+                lambda: ops.block_join(x, x, gate=torch.ones(2, 3, 1)), lambda: ops.block_join(x, x, gate=torch.ones(())),
+                lambda: ops.block_join(x, x, dropout=0.1)):
+        with pytest.raises(ValueError):
+            bad()
+    assert [ops._gate_rows(torch.empty(s), x) for s in ((8,), (1, 1, 8), (2, 1, 8), (2, 3, 8))] == [6, 6, 3, 1]
+
+
+def test_every_kernel_has_a_family():
+    names = set()
+    for src in ("loopback_block.hip",):
+        with open(os.path.join(ROOT, "loopback_amd", "csrc", src)) as f:
+            names |= set(re.findall(r"__global__[^;{]*?\bvoid\s+(k_\w+)\s*\(", f.read(), flags=re.S))
+    assert {"k_dropout", "k_join_fwd", "k_join_bwd", "k_join_sum"} <= names
+    assert all(RS.family(f"void (anonymous namespace)::{n}<float, 1>(...)") != "torch / runtime" for n in names)
