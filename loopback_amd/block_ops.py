@@ -1,10 +1,12 @@
 """Operators of a transformer block's training step on the HIP kernels of libloopback_block.so (include/loopback_block.h):
 
+  * `gated_ffn(x, w_gate_up, w_down)`: the gated feed-forward block, both projections, the activation and the product in
+    one kernel, the activation's gradient in the one that forms it (bf16 and fp16);
   * `block_join(x, y, ...)`: a block's output y back on the residual stream x, with the norm after the block, a gate, a
     residual scale and dropout before the add, and the next block's norm after it;
   * `dropout(x, p, rng, site)`: dropout whose mask comes from a counter-based generator and is never stored.
 
-The kernels take plain fp32, bf16 and fp16 tensors of the current GPU where nothing has to see torch operations (lm_ops.native
+The row kernels take plain fp32, bf16 and fp16 tensors of the current GPU where nothing has to see torch operations (lm_ops.native
 says what does); everything else -- the CPU, other types, tracers, transforms -- runs the torch form of the same operator:
 the same formulas and the same masks. A backward that is itself differentiated, or watched, runs the torch form too. Tensors
 of any strides are taken (the kernels work on contiguous rows; others are copied).
@@ -20,6 +22,7 @@ import ctypes
 import os
 
 import torch
+import torch.nn.functional as F
 
 from . import build as _build
 from .lm_ops import _again, _launchable, _stream, _watched, native
@@ -38,6 +41,13 @@ SIGNATURES = {
     "lbk_join_scratch": (_i64, [_i64, _i64, _i64]),
     "lbk_join_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _u32, _i32, _f32, _p, _p, _p, _p, _p, _p, _i64,
                             _i64, _i32, _p]),
+    "lbk_ffn_saved_bytes": (_i64, [_i64, _i64]),
+    "lbk_ffn_gate_up": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _p]),
+    "lbk_ffn_dgate_up": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "lbk_linear_fwd": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "lbk_linear_dx": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "lbk_linear_dw_scratch": (_i64, [_i64, _i64, _i64]),
+    "lbk_linear_dw": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
 }
 
 
@@ -316,3 +326,92 @@ def block_join(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor | 
     if _records(*ts):
         return _Join.apply(x, y, post_weight, gate, gate_rows, pre_weight, rng, site, drop, scale, eps)
     return _join_launch(x, y, post_weight, gate, gate_rows, pre_weight, rng, site, drop, scale, eps, False)[:2]
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# gated feed-forward block
+# ---------------------------------------------------------------------------------------------------------------
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _ffn_torch(x, w_gate_up, w_down, activation):
+    g, u = F.linear(x, w_gate_up).chunk(2, dim=-1)
+    a = F.silu(g) if activation == 0 else F.gelu(g, approximate="tanh")
+    return F.linear(a * u, w_down)
+
+
+def _ffn_forward(x, w_gate_up, w_down, activation, keep):
+    """y, and what the backward needs: the activations and the projections' saved values."""
+    t, d = x.numel() // x.shape[-1], x.shape[-1]
+    n, m, code, st = w_down.shape[1], w_down.shape[0], _CODES[x.dtype], _stream(x)
+    act = torch.empty((t, n), device=x.device, dtype=x.dtype)
+    saved = torch.empty(LIB.lbk_ffn_saved_bytes(t, n), device=x.device, dtype=torch.uint8) if keep else None
+    _run("lbk_ffn_gate_up", x.data_ptr(), w_gate_up.data_ptr(), act.data_ptr(), _ptr(saved), t, d, n, activation, code, st)
+    y = torch.empty((*x.shape[:-1], m), device=x.device, dtype=x.dtype)
+    _run("lbk_linear_fwd", act.data_ptr(), w_down.data_ptr(), y.data_ptr(), t, n, m, code, st)
+    return y, act, saved
+
+
+def _linear_dw(dy, x, w, t, code, st):
+    dw = torch.empty_like(w)
+    size = LIB.lbk_linear_dw_scratch(t, *w.shape)
+    scratch = torch.empty(size, device=w.device, dtype=torch.float32) if size else None
+    _run("lbk_linear_dw", dy.data_ptr(), x.data_ptr(), _ptr(scratch), dw.data_ptr(), t, *w.shape, code, st)
+    return dw
+
+
+class _GatedFfn(torch.autograd.Function):
+    """Saves x, the weights, the activations and (saved) u a'(g) and a(g) of the projections."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate_up, w_down, activation):
+        need = ctx.needs_input_grad
+        y, act, saved = _ffn_forward(x, w_gate_up, w_down, activation, need[0] or need[1])
+        ctx.activation = activation
+        ctx.save_for_backward(x, w_gate_up, w_down, act if need[2] else None, saved)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w_gate_up, w_down, act, saved = _plain_rows(*ctx.saved_tensors)
+        need = ctx.needs_input_grad
+        if not _launchable(dy):
+            fn = lambda x, g, d: _ffn_torch(x, g, d, ctx.activation)
+            return *_again(fn, [x, w_gate_up, w_down], need[:3], dy), None
+        dy = dy.to(x.dtype).contiguous()
+        t, d = x.numel() // x.shape[-1], x.shape[-1]
+        (m, n), code, st = w_down.shape, _CODES[x.dtype], _stream(x)
+        dx = dw_gate_up = dw_down = None
+        if need[0] or need[1]:
+            if saved.data_ptr() % 16:
+                saved = saved.clone()   # a saved-tensor hook's
+            dgu = torch.empty((t, 2 * n), device=x.device, dtype=x.dtype)
+            _run("lbk_ffn_dgate_up", dy.data_ptr(), w_down.data_ptr(), saved.data_ptr(), dgu.data_ptr(), t, n, m, code, st)
+            if need[0]:
+                dx = torch.empty_like(x)
+                _run("lbk_linear_dx", dgu.data_ptr(), w_gate_up.data_ptr(), dx.data_ptr(), t, 2 * n, d, code, st)
+            if need[1]:
+                dw_gate_up = _linear_dw(dgu, x, w_gate_up, t, code, st)
+        if need[2]:
+            dw_down = _linear_dw(dy, act, w_down, t, code, st)
+        return dx, dw_gate_up, dw_down, None
+
+
+def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """(a(x Wg^T) * (x Wu^T)) Wd^T of x (..., d), w_gate_up (2 n, d) = [Wg; Wu] and w_down (m, n); a is "silu" or "gelu" (its
+    tanh form). On the kernels the projections, the activation and their product are one fp32 value rounded once, and the
+    backward's gradients of the two projections are formed from 24 bits of them."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    if w_gate_up.dim() != 2 or w_down.dim() != 2 or x.dim() < 1 or w_gate_up.shape[1] != x.shape[-1] \
+            or w_gate_up.shape[0] != 2 * w_down.shape[1]:
+        raise ValueError(f"gated_ffn takes x (..., d), w_gate_up (2 n, d) and w_down (m, n), got {tuple(x.shape)}, "
+                         f"{tuple(w_gate_up.shape)} and {tuple(w_down.shape)}")
+    code = ACTIVATIONS[activation]
+    if not (native(x, w_gate_up, w_down) and x.numel() > 0 and w_down.numel() > 0
+            and max(x.numel() // x.shape[-1], *w_gate_up.shape, *w_down.shape) <= MAX_ROWS):
+        return _ffn_torch(x, w_gate_up, w_down, code)
+    x, w_gate_up, w_down = _plain_rows(x, w_gate_up, w_down)   # recorded, where they copy
+    if _records(x, w_gate_up, w_down):
+        return _GatedFfn.apply(x, w_gate_up, w_down, code)
+    return _ffn_forward(x, w_gate_up, w_down, code, False)[0]

@@ -26,7 +26,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "libloopback_read.so")
 LM_SRC = os.path.join(HERE, "csrc", "loopback_lm.hip")
 LM_LIB = os.path.join(HERE, "libloopback_lm.so")
-BLOCK_SRC = os.path.join(HERE, "csrc", "loopback_block.hip")
+BLOCK_SRC = [os.path.join(HERE, "csrc", f) for f in ("loopback_block.hip", "loopback_ffn.hip")]
 BLOCK_LIB = os.path.join(HERE, "libloopback_block.so")
 HOST_SRC = os.path.join(HERE, "csrc", "host.cpp")
 HOST_LIB = os.path.join(HERE, "_host.so")
@@ -65,9 +65,10 @@ def _defines(defines) -> list[str]:
     return [f"-D{w}" for w in words]
 
 
-def _start(src: str, lib: str, verbose: bool, defines) -> tuple:
+def _start(src, lib: str, verbose: bool, defines) -> tuple:
     tmp = lib + ".tmp"
-    cmd = [hipcc(), *FLAGS, *_defines(defines), f"-I{INCLUDE}", "-o", tmp, src]
+    srcs = [src] if isinstance(src, str) else src
+    cmd = [hipcc(), *FLAGS, *_defines(defines), f"-I{INCLUDE}", f"-parallel-jobs={len(srcs)}", "-o", tmp, *srcs]
     if verbose:
         print(" ".join(cmd), flush=True)
     return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True), tmp, lib

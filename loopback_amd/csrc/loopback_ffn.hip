@@ -1,0 +1,534 @@
+// loopback_ffn.hip -- MI355X (gfx950, CDNA4) kernels of the gated feed-forward block on the matrix cores: one tiled product
+// with the block's epilogues.
+//
+// A product is C[q][p] = sum_k P(p, k) Q(q, k): p the contiguous dimension of the result, q its rows (tokens, or a weight's
+// output rows). Each operand lies in memory either by rows of k ("ROW": index i at i * ld, k contiguous) or by rows of the
+// index ("COL": k at k * ld, the index contiguous), so the forward (x W^T), the input gradient (dy W) and the weight
+// gradient (dy^T x) are the same kernel without a transposed copy of anything.
+//
+// Operands go through v_mfma_f32_32x32x16 (bf16 or fp16): lane l holds row (P) or column (Q) l mod 32 at k = 8 (l / 32) .. + 8;
+// of the 32 x 32 result it holds column l mod 32 and, in register r, row 4 (l / 32) + r mod 4 + 8 (r / 4): four consecutive p of
+// one q, which one exchange of lane halves makes eight (a 16-byte store). Tiles of 64 k sit in LDS twice, the next one filled
+// by direct global -> LDS loads while one is worked on. Such loads write 64 lanes' 16 bytes in order, so the tiles have no
+// padding; instead the 16-byte pieces of a row are permuted: ROW tiles (128-byte rows) by (row / 2) mod 8, so that 16 rows at
+// one k cover the 64 banks once, COL tiles (rows of the tile's width) by 4 (k mod 4), so that the four rows a transposing read
+// (ds_read_b64_tr_b16) takes together do.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "loopback_block.h"
+#include "loopback_read.h"
+#include "device_io.h"
+
+namespace {
+
+constexpr int BK = 64;             // k per tile
+enum Kind { ROW, COL };
+enum Epi { STORE, PARTIAL, GATED, DGATED };
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+__device__ __forceinline__ f32x16 mfma(bf16_t, uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(_Float16, uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename T> struct CvtOf { typedef Bf16Cvt type; };
+template <> struct CvtOf<_Float16> { typedef F16Cvt type; };
+
+// ---------------------------------------------------------------------------------------------------------------
+// one operand: where it lies, and its tile of ROWS indices (ROW) or columns (COL) x 64 k
+// ---------------------------------------------------------------------------------------------------------------
+struct Operand {
+  const void* base;
+  int64_t ld;      // elements between rows of memory
+  int64_t size;    // indices
+  int64_t half;    // GATED: indices per half (tile indices past its middle are those of the second half); else 0
+};
+
+template <typename T, Kind KIND, int ROWS, int LANES> struct Tile {
+  static constexpr int PER = KIND == ROW ? 8 : ROWS / 8;   // 16-byte pieces per row of the tile
+  static constexpr int PASSES = ROWS * 8 / LANES, STEP = LANES / PER;
+  static_assert(ROWS * 8 % LANES == 0 && STEP % 16 == 0 && (KIND == ROW || ROWS >= 128), "tile shape");
+
+  // this lane's piece of pass i: row i STEP + tid / PER, stored as piece tid % PER, which is piece `piece()` of memory's row
+  static __device__ __forceinline__ int row(int i) { return i * STEP + (int)threadIdx.x / PER; }
+  static __device__ __forceinline__ int piece() {
+    const int r = (int)threadIdx.x / PER, c = (int)threadIdx.x % PER;
+    return KIND == ROW ? c ^ ((r >> 1) & 7) : c ^ (4 * (r & 3));
+  }
+  // the operand's index of tile row r (ROW) from the tile's first index i0; past the end: the last one
+  static __device__ __forceinline__ int64_t index(const Operand& o, int64_t i0, int r) {
+    if (o.half) return r < ROWS / 2 ? min(i0 + r, o.half - 1) : o.half + min(i0 + r - ROWS / 2, o.half - 1);
+    return min(i0 + r, o.size - 1);
+  }
+
+  const T* src[PASSES];
+  int64_t step;
+  // aligned operands (rows of a multiple of 8 elements, 16-byte aligned), whole tiles of k from k0 on
+  __device__ __forceinline__ void start(const Operand& o, int64_t i0, int64_t k0) {
+    const T* base = static_cast<const T*>(o.base);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+      src[i] = KIND == ROW ? base + index(o, i0, row(i)) * o.ld + k0 + 8 * piece()
+                           : base + (k0 + row(i)) * o.ld + min(i0 + 8 * piece(), o.size - 8);
+    step = KIND == ROW ? BK : BK * o.ld;
+  }
+  __device__ __forceinline__ void fetch(T* lds) {   // asynchronous: done when vmcnt says so
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      __builtin_amdgcn_global_load_lds((global_void*)src[i], (lds_void*)(lds + 8 * (i * LANES + wave * 64)), 16, 0, 0);
+      src[i] += step;
+    }
+  }
+  // any alignment, k from k0 to k1 (at most BK of them): zeros past k1 and past the operand's indices
+  static __device__ __forceinline__ void copy(const Operand& o, int64_t i0, int64_t k0, int64_t k1, T* lds) {
+    const T* base = static_cast<const T*>(o.base);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const T* p;
+      int64_t left;   // elements of this piece that exist
+      if (KIND == ROW) {
+        p = base + index(o, i0, row(i)) * o.ld + k0 + 8 * piece();
+        left = k1 - k0 - 8 * piece();
+      } else {
+        p = base + (k0 + row(i)) * o.ld + i0 + 8 * piece();
+        left = k0 + row(i) < k1 ? o.size - i0 - 8 * piece() : 0;
+      }
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (left >= 8) {
+        v = UIO<T>::raw(p).u;
+      } else if (left > 0) {
+        struct { T e[8]; } e;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e.e[k] = k < left ? p[k] : (T)0;
+        v = __builtin_bit_cast(uint4, e);
+      }
+      *reinterpret_cast<uint4*>(lds + 8 * (i * LANES + (int)threadIdx.x)) = v;
+    }
+  }
+  // the matrix cores' operand: indices r0 .. r0 + 31 (r0 a multiple of 32) at k = 16 s .. 16 s + 15
+  static __device__ __forceinline__ uint4 frag(const T* lds, int r0, int s) {
+    const int lane = (int)threadIdx.x & 63, h = lane >> 5;
+    if constexpr (KIND == ROW) {
+      const int r = lane & 31;
+      return *reinterpret_cast<const uint4*>(lds + (r0 + r) * BK + 8 * ((2 * s + h) ^ ((r >> 1) & 7)));
+    } else {
+      typedef __attribute__((address_space(3))) s16x4* lds4;
+      const int j = lane & 15, kr = j >> 2;
+      const int col = 32 * ((r0 >> 5) ^ kr) + (lane & 16) + 4 * (j & 3);
+      const T* p = lds + (16 * s + 8 * h + kr) * ROWS + col;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(const_cast<T*>(p)));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(const_cast<T*>(p + 4 * ROWS)));
+      const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
+      return make_uint4(ua.x, ua.y, ub.x, ub.y);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// what the backward needs of the gate and up projections: (u a'(g), a(g)) of each (token, inner column), which the
+// activation's gradient is multiplied by. Kept as the upper 24 bits of their fp32 values: 16 would double the input and
+// gate/up weight gradients' squared error (three roundings of 2^-9 instead of two). In blocks of 32 tokens x 32 columns in the
+// matrix cores' own order, so both kernels move them as whole vectors: 64 lanes x 16 values, upper 16 bits as two planes of
+// eight values a lane, then the next eight bits: 3072 bytes for each of the two.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int64_t SAVED_BLOCK = 6144;
+struct Saved {
+  static __device__ __forceinline__ unsigned hi2(float a, float b) {   // upper halves of two words
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  }
+  static __device__ __forceinline__ void put(char* block, const f32x16& v) {
+    const int lane = (int)threadIdx.x & 63;
+    unsigned lo[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      lo[q] = ((__float_as_uint(v[4 * q]) >> 8) & 0xffu) | (__float_as_uint(v[4 * q + 1]) & 0xff00u) |
+              ((__float_as_uint(v[4 * q + 2]) & 0xff00u) << 8) | ((__float_as_uint(v[4 * q + 3]) & 0xff00u) << 16);
+    uint4* p = reinterpret_cast<uint4*>(block) + lane;
+    p[0] = make_uint4(hi2(v[0], v[1]), hi2(v[2], v[3]), hi2(v[4], v[5]), hi2(v[6], v[7]));
+    p[64] = make_uint4(hi2(v[8], v[9]), hi2(v[10], v[11]), hi2(v[12], v[13]), hi2(v[14], v[15]));
+    p[128] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+  static __device__ __forceinline__ void get(const char* block, float (&v)[16]) {
+    const uint4* p = reinterpret_cast<const uint4*>(block) + ((int)threadIdx.x & 63);
+    const uint4 a = p[0], b = p[64], c = p[128];
+    const unsigned hi[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, lo[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const unsigned h = r & 1 ? hi[r >> 1] & 0xffff0000u : hi[r >> 1] << 16;
+      const unsigned l = (r & 3) == 0 ? (lo[r >> 2] & 0xffu) << 8 : (r & 3) == 1 ? lo[r >> 2] & 0xff00u
+                       : (r & 3) == 2 ? (lo[r >> 2] >> 8) & 0xff00u : (lo[r >> 2] >> 16) & 0xff00u;
+      v[r] = __uint_as_float(h | l);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// the product
+// ---------------------------------------------------------------------------------------------------------------
+struct Product {
+  Operand p, q;
+  int64_t k, run;          // k in all, and per split (a multiple of BK)
+  void* out;               // [q][ldo]; PARTIAL: fp32 [split][q][ldo]
+  int64_t ldo;
+  void* saved;             // GATED: written (NULL: not wanted); DGATED: read
+  int64_t saved_cols;      // its blocks of columns
+  int tiles_p, tiles, splits, per;
+  int act;                 // 0 silu, 1 gelu (tanh form)
+};
+
+// 16 registers of a result tile (column q = this lane's, rows p0 + 4 h + r mod 4 + 8 (r / 4)) to out[p0 ..], rounded:
+// exchanged between the lane halves so that each lane has eight consecutive p, twice
+template <typename T, bool AL>
+__device__ __forceinline__ void store_tile(T* row, int64_t p0, int64_t np, bool ok, const f32x16& v) {
+  typedef typename CvtOf<T>::type Cvt;
+  const int h = ((int)threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    unsigned u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = Cvt::pack2(v[8 * g + 2 * e], v[8 * g + 2 * e + 1]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const auto sw = __builtin_amdgcn_permlane32_swap(u[e], u[2 + e], false, false);
+      u[e] = (unsigned)sw[0];
+      u[2 + e] = (unsigned)sw[1];
+    }
+    const int64_t p = p0 + 16 * g + 8 * h;
+    if (ok) {
+      if (AL ? p < np : p + 8 <= np) {
+        if (AL) *reinterpret_cast<uint4*>(row + p) = make_uint4(u[0], u[1], u[2], u[3]);
+        else *reinterpret_cast<u32x4_u16*>(row + p) = u32x4{u[0], u[1], u[2], u[3]};
+      } else if (!AL && p < np) {
+        struct { T e[8]; } e = __builtin_bit_cast(decltype(e), make_uint4(u[0], u[1], u[2], u[3]));
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (p + k < np) row[p + k] = e.e[k];
+      }
+    }
+  }
+}
+
+// a(g) and a'(g): silu, or gelu in its tanh form, g s(2 sqrt(2/pi) (g + 0.044715 g^3)) (the fast exponential's error, some
+// 2^-24 of its argument, is far below the results' rounding; where the argument is large the sigmoid is 0 or 1)
+__device__ __forceinline__ void activation(float g, int act, float& a, float& da) {
+  const float g2 = g * g;
+  const float q = act ? g * __builtin_fmaf(0.07135481282553433f, g2, 1.5957691216057308f) : g;
+  const float dq = act ? __builtin_fmaf(0.21406443847660298f, g2, 1.5957691216057308f) : 1.f;
+  const float s = 1.f / (1.f + __expf(-q));
+  a = g * s;
+  da = s + a * dq * (1.f - s);
+  if (act && !(g2 < 1e4f)) da = g != g ? g : s;   // far out, where q' overflows: a is 0 or g
+}
+
+template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI, bool AL>
+__global__ __launch_bounds__(WP * WQ * 64) void k_product(const Product a) {
+  constexpr int LANES = WP * WQ * 64, TP = WP * FP * 32, TQ = WQ * FQ * 32;
+  typedef Tile<T, KP, TP, LANES> PT;
+  typedef Tile<T, KQ, TQ, LANES> QT;
+  __shared__ __align__(16) T sp0[TP * BK], sq0[TQ * BK], sp1[TP * BK], sq1[TQ * BK];
+  // XCD x (workgroups go to XCDs in turn) takes `per` consecutive tiles, in groups of eight rows of tiles: the tiles worked
+  // on at a time then share their operands' rows in that XCD's L2
+  const int id = ((int)blockIdx.x & 7) * a.per + ((int)blockIdx.x >> 3);
+  if (id >= a.tiles * a.splits || ((int)blockIdx.x >> 3) >= a.per) return;
+  const int split = id / a.tiles, tile = id - split * a.tiles;
+  const int tiles_q = a.tiles / a.tiles_p, group = tile / (8 * a.tiles_p), first = 8 * group, rows = min(8, tiles_q - first);
+  const int in = tile - first * a.tiles_p, tp = in / rows, tq = first + in - tp * rows;
+  const int64_t p0 = (int64_t)tp * (EPI == GATED ? TP / 2 : TP), q0 = (int64_t)tq * TQ;
+  const int64_t k0 = split * a.run, k1 = min(a.k, k0 + a.run);
+  const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wp = wave % WP, wq = wave / WP;
+  // GATED: a wave's two P tiles are the gate's and the up projection's of the same columns
+  auto p_row = [&](int i) { return EPI == GATED ? i * (TP / 2) + 32 * wp : 32 * (wp * FP + i); };
+
+  f32x16 acc[FP][FQ];
+#pragma unroll
+  for (int i = 0; i < FP; ++i)
+#pragma unroll
+    for (int j = 0; j < FQ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  auto work = [&](const T* sp, const T* sq) {
+#pragma unroll
+    for (int s = 0; s < BK / 16; ++s) {
+      uint4 fp[FP], fq[FQ];
+#pragma unroll
+      for (int i = 0; i < FP; ++i) fp[i] = PT::frag(sp, p_row(i), s);
+#pragma unroll
+      for (int j = 0; j < FQ; ++j) fq[j] = QT::frag(sq, 32 * (wq * FQ + j), s);
+#pragma unroll
+      for (int i = 0; i < FP; ++i)
+#pragma unroll
+        for (int j = 0; j < FQ; ++j) acc[i][j] = mfma(T{}, fp[i], fq[j], acc[i][j]);
+    }
+  };
+
+  const int64_t whole = AL ? (k1 - k0) / BK : 0;
+  for (int64_t k = k0 + whole * BK; k < k1; k += BK) {   // AL: what is left of k past the whole tiles
+    __syncthreads();
+    PT::copy(a.p, p0, k, k1, sp1);
+    QT::copy(a.q, q0, k, k1, sq1);
+    __syncthreads();
+    work(sp1, sq1);
+  }
+  if constexpr (AL) {
+    if (whole) {
+      PT pt;
+      QT qt;
+      pt.start(a.p, p0, k0);
+      qt.start(a.q, q0, k0);
+      pt.fetch(sp0);
+      qt.fetch(sq0);
+      // a tile's loads are waited for, then every wave is past its reads of the other buffer and its loads are here
+      auto ready = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+        __syncthreads();
+      };
+      for (int64_t t = 0;;) {
+        ready();
+        if (t + 1 < whole) {
+          pt.fetch(sp1);
+          qt.fetch(sq1);
+        }
+        work(sp0, sq0);
+        if (++t == whole) break;
+        ready();
+        if (t + 1 < whole) {
+          pt.fetch(sp0);
+          qt.fetch(sq0);
+        }
+        work(sp1, sq1);
+        if (++t == whole) break;
+      }
+    }
+  }
+
+  const int64_t np = EPI == GATED ? a.p.half : a.p.size;
+#pragma unroll
+  for (int j = 0; j < FQ; ++j) {
+    const int64_t qt = q0 + 32 * (wq * FQ + j), q = qt + (lane & 31);
+    const bool ok = q < a.q.size;
+    if constexpr (EPI == GATED) {
+      const int64_t p = p0 + 32 * wp;
+      if (qt < a.q.size && p < np) {
+        f32x16 x, y, z;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float av, da;
+          activation(acc[0][j][r], a.act, av, da);
+          z[r] = av * acc[1][j][r];
+          x[r] = acc[1][j][r] * da;
+          y[r] = av;
+        }
+        store_tile<T, AL>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, z);
+        if (a.saved) {
+          char* block = static_cast<char*>(a.saved) + ((qt >> 5) * a.saved_cols + (p >> 5)) * SAVED_BLOCK;
+          Saved::put(block, x);
+          Saved::put(block + SAVED_BLOCK / 2, y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < FP; ++i) {
+        const int64_t p = p0 + p_row(i);
+        if (qt >= a.q.size || p >= np) continue;   // wave-uniform
+        if constexpr (EPI == STORE) {
+          store_tile<T, AL>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, acc[i][j]);
+        } else if constexpr (EPI == DGATED) {
+          const char* block = static_cast<const char*>(a.saved) + ((qt >> 5) * a.saved_cols + (p >> 5)) * SAVED_BLOCK;
+          float m[16];
+          f32x16 o;
+          T* row = static_cast<T*>(a.out) + q * a.ldo;
+          Saved::get(block, m);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[r] = acc[i][j][r] * m[r];
+          store_tile<T, AL>(row, p, np, ok, o);
+          Saved::get(block + SAVED_BLOCK / 2, m);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[r] = acc[i][j][r] * m[r];
+          store_tile<T, AL>(row + np, p, np, ok, o);
+        } else {
+          float* row = static_cast<float*>(a.out) + ((int64_t)split * a.q.size + q) * a.ldo;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int64_t pp = p + 8 * g + 4 * (lane >> 5);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (ok && pp + r < np) row[pp + r] = acc[i][j][4 * g + r];
+          }
+        }
+      }
+    }
+  }
+}
+
+// out = round(sum of the splits' products, in order)
+template <typename T>
+__global__ __launch_bounds__(256) void k_split_sum(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ out) {
+  for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n; i += 4 * (int64_t)gridDim.x * 256) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const int left = (int)min((int64_t)4, n - i);
+    for (int s = 0; s < splits; ++s)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += k < left ? part[s * n + i + k] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < left) st1(out + i + k, acc[k]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------
+inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool al2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
+inline int launched() { return (int)hipGetLastError(); }
+constexpr int64_t MAX_SIZE = 0x7fffffff;   // of one dimension
+
+template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI, bool AL>
+int launch_tiles(Product a, hipStream_t st) {
+  constexpr int TP = (EPI == GATED ? WP * FP * 16 : WP * FP * 32), TQ = WQ * FQ * 32;
+  const int64_t np = EPI == GATED ? a.p.half : a.p.size;
+  const int64_t tp = (np + TP - 1) / TP, tq = (a.q.size + TQ - 1) / TQ, tiles = tp * tq;
+  if (tiles * a.splits > 0xfffffff) return LDR_E_SHAPE;
+  a.tiles_p = (int)tp;
+  a.tiles = (int)tiles;
+  a.per = (int)((tiles * a.splits + 7) / 8);
+  hipLaunchKernelGGL((k_product<T, KP, KQ, WP, WQ, FP, FQ, EPI, AL>), dim3((unsigned)(8 * a.per)), dim3(WP * WQ * 64), 0, st, a);
+  return launched();
+}
+
+// 256 x 256 tiles by eight waves where they give every CU one; 128 x 128 by four waves else
+constexpr int64_t CUS = 256;
+inline int64_t tiles_of(int64_t np, int64_t nq, int64_t t) { return ((np + t - 1) / t) * ((nq + t - 1) / t); }
+
+template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, bool al, hipStream_t st) {
+  if (!al) return launch_tiles<T, KP, KQ, 2, 2, 2, 2, EPI, false>(a, st);
+  const int64_t np = a.p.half ? 2 * a.p.half : a.p.size;
+  if (tiles_of(np, a.q.size, 256) * a.splits >= CUS / 2) return launch_tiles<T, KP, KQ, 4, 2, 2, 4, EPI, true>(a, st);
+  return launch_tiles<T, KP, KQ, 2, 2, 2, 2, EPI, true>(a, st);
+}
+
+#define FFN_TYPE_SWITCH(DT, ...)                                 \
+  if ((DT) == LDR_BF16) { typedef bf16_t T; __VA_ARGS__; }       \
+  else { typedef _Float16 T; __VA_ARGS__; }
+
+inline int sizes(int64_t a, int64_t b, int64_t c, int dtype) {
+  if (dtype != LDR_BF16 && dtype != LDR_F16) return LDR_E_DTYPE;
+  if (a < 0 || b < 1 || c < 1) return LDR_E_ARG;
+  return a > MAX_SIZE || b > MAX_SIZE || c > MAX_SIZE ? LDR_E_SHAPE : LDR_OK;
+}
+inline Product product(Operand p, Operand q, int64_t k, void* out, int64_t ldo) {
+  return Product{p, q, k, (k + BK - 1) / BK * BK, out, ldo, nullptr, 0, 0, 0, 1, 0, 0};
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t lbk_ffn_saved_bytes(int64_t t, int64_t n) {
+  return t < 1 || n < 1 ? 0 : ((t + 31) / 32) * ((n + 31) / 32) * SAVED_BLOCK;
+}
+
+int lbk_ffn_gate_up(const void* x, const void* w, void* act, void* saved, int64_t t, int64_t d, int64_t n, int activation,
+                    int dtype, void* stream) {
+  const int e = sizes(t, d, n, dtype);
+  if (e) return e;
+  if (activation != 0 && activation != 1) return LDR_E_ARG;
+  if (t == 0) return LDR_OK;
+  if (!x || !w || !act) return LDR_E_ARG;
+  if (!al2(x) || !al2(w) || !al2(act) || !al16(saved)) return LDR_E_ALIGN;
+  const bool al = d % 8 == 0 && n % 8 == 0 && al16(x) && al16(w) && al16(act);
+  Product a = product({w, d, 2 * n, n}, {x, d, t, 0}, d, act, n);
+  a.saved = saved;
+  a.saved_cols = (n + 31) / 32;
+  a.act = activation;
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, GATED>(a, al, static_cast<hipStream_t>(stream))))
+}
+
+int lbk_ffn_dgate_up(const void* dy, const void* w_down, const void* saved, void* dgate_up, int64_t t, int64_t n, int64_t d,
+                     int dtype, void* stream) {
+  const int e = sizes(t, d, n, dtype);
+  if (e) return e;
+  if (t == 0) return LDR_OK;
+  if (!dy || !w_down || !saved || !dgate_up) return LDR_E_ARG;
+  if (!al2(dy) || !al2(w_down) || !al2(dgate_up) || !al16(saved)) return LDR_E_ALIGN;
+  const bool al = d % 8 == 0 && n % 8 == 0 && al16(dy) && al16(w_down) && al16(dgate_up);
+  Product a = product({w_down, n, n, 0}, {dy, d, t, 0}, d, dgate_up, 2 * n);
+  a.saved = const_cast<void*>(saved);
+  a.saved_cols = (n + 31) / 32;
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, DGATED>(a, al, static_cast<hipStream_t>(stream))))
+}
+
+int lbk_linear_fwd(const void* x, const void* w, void* y, int64_t t, int64_t k, int64_t n, int dtype, void* stream) {
+  const int e = sizes(t, k, n, dtype);
+  if (e || t == 0) return e;
+  if (!x || !w || !y) return LDR_E_ARG;
+  if (!al2(x) || !al2(w) || !al2(y)) return LDR_E_ALIGN;
+  const bool al = k % 8 == 0 && n % 8 == 0 && al16(x) && al16(w) && al16(y);
+  const Product a = product({w, k, n, 0}, {x, k, t, 0}, k, y, n);
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, STORE>(a, al, static_cast<hipStream_t>(stream))))
+}
+
+int lbk_linear_dx(const void* dy, const void* w, void* dx, int64_t t, int64_t n, int64_t k, int dtype, void* stream) {
+  const int e = sizes(t, k, n, dtype);
+  if (e || t == 0) return e;
+  if (!dy || !w || !dx) return LDR_E_ARG;
+  if (!al2(dy) || !al2(w) || !al2(dx)) return LDR_E_ALIGN;
+  const bool al = k % 8 == 0 && n % 8 == 0 && al16(dy) && al16(w) && al16(dx);
+  const Product a = product({w, k, k, 0}, {dy, n, t, 0}, n, dx, k);
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, STORE>(a, al, static_cast<hipStream_t>(stream))))
+}
+
+static int64_t dw_splits(int64_t t, int64_t n, int64_t k) {
+  const int64_t tiles = tiles_of(n, k, 256), fill = CUS / tiles, most = t / 512;
+  const int64_t s = fill < most ? fill : most;
+  return s < 1 ? 1 : s;
+}
+
+int64_t lbk_linear_dw_scratch(int64_t t, int64_t n, int64_t k) {
+  if (t < 1 || n < 1 || k < 1) return 0;
+  const int64_t s = dw_splits(t, n, k);
+  return s > 1 ? s * n * k : 0;
+}
+
+int lbk_linear_dw(const void* dy, const void* x, float* scratch, void* dw, int64_t t, int64_t n, int64_t k, int dtype,
+                  void* stream) {
+  const int e = sizes(t, k, n, dtype);
+  if (e) return e;
+  if (!dw || (t > 0 && (!dy || !x))) return LDR_E_ARG;
+  if (!al2(dy) || !al2(x) || !al2(dw) || !al16(scratch)) return LDR_E_ALIGN;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t splits = t < 1 ? 1 : dw_splits(t, n, k);
+  if (splits > 1 && !scratch) return LDR_E_ARG;
+  const bool al = k % 8 == 0 && n % 8 == 0 && al16(dy) && al16(x) && al16(dw);
+  Product a = product({x, k, k, 0}, {dy, n, n, 0}, t, dw, k);
+  if (splits == 1) {
+    FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, COL, STORE>(a, al, st)))
+  }
+  a.run = ((t + splits - 1) / splits + BK - 1) / BK * BK;
+  a.splits = (int)((t + a.run - 1) / a.run);
+  a.out = scratch;
+  FFN_TYPE_SWITCH(dtype, {
+    const int err = launch_product<T, COL, COL, PARTIAL>(a, al, st);
+    if (err) return err;
+    const int64_t blocks = (n * k / 4 + 255) / 256 + 1;
+    hipLaunchKernelGGL(k_split_sum<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, scratch, a.splits,
+                       n * k, static_cast<T*>(dw));
+  })
+  return launched();
+}
+
+}  // extern "C"

@@ -47,6 +47,35 @@ def test_row_kernels_refuse():
     assert L.lbk_join_scratch(1, 64, 1) == 4 * 64
 
 
+def test_products_refuse():
+    L, p, null = ops.LIB, 4096, None
+    up = lambda x=p, w=p, act=p, saved=p, t=4, d=8, n=8, a=0, dt=1: L.lbk_ffn_gate_up(x, w, act, saved, t, d, n, a, dt, null)
+    assert up(dt=0) == -4 and up(dt=3) == -4 and up(t=-1) == -1 and up(d=0) == -1 and up(n=0) == -1 and up(a=2) == -1
+    assert up(x=null) == -1 and up(w=null) == -1 and up(act=null) == -1 and up(x=4097) == -3 and up(saved=4098) == -3
+    assert up(t=2 ** 31) == -2 and up(d=2 ** 31) == -2 and up(n=2 ** 31) == -2 and up(t=0, x=null) == 0
+    dn = lambda dy=p, w=p, saved=p, out=p, t=4, dt=2: L.lbk_ffn_dgate_up(dy, w, saved, out, t, 8, 8, dt, null)
+    assert dn(dt=0) == -4 and dn(dy=null) == -1 and dn(w=null) == -1 and dn(saved=null) == -1 and dn(out=null) == -1
+    assert dn(saved=4098) == -3 and dn(out=4097) == -3 and dn(t=0) == 0
+    for fn in (L.lbk_linear_fwd, L.lbk_linear_dx):
+        assert fn(p, p, p, 4, 8, 8, 0, null) == -4 and fn(null, p, p, 4, 8, 8, 1, null) == -1
+        assert fn(p, p, 4097, 4, 8, 8, 1, null) == -3 and fn(p, p, p, 4, 0, 8, 1, null) == -1 and fn(p, p, p, 0, 8, 8, 1, null) == 0
+    dw = lambda dy=p, s=p, out=p, t=4: L.lbk_linear_dw(dy, p, s, out, t, 8, 8, 1, null)
+    assert dw(dy=null) == -1 and dw(out=null) == -1 and dw(s=null, t=1 << 20) == -1 and dw(s=4100) == -3 and dw(t=-1) == -1
+    assert L.lbk_linear_dw_scratch(0, 8, 8) == 0 and L.lbk_linear_dw_scratch(100, 768, 768) == 0
+    assert L.lbk_linear_dw_scratch(1 << 20, 8, 8) > 0 and L.lbk_ffn_saved_bytes(33, 1) == 2 * 6144
+
+
+def test_ffn_form():
+    """The torch form: its values by their formula and its gradients against differences, in fp64."""
+    args = [rnd((3, 5), 1).requires_grad_(), rnd((8, 5), 2).requires_grad_(), rnd((6, 4), 3).requires_grad_()]
+    for act in ("silu", "gelu"):
+        assert torch.autograd.gradcheck(lambda *a: ops.gated_ffn(*a, activation=act), args)
+        g, u = (args[0] @ args[1].t()).chunk(2, -1)
+        q = g if act == "silu" else 2 * (2 / torch.pi) ** 0.5 * (g + 0.044715 * g ** 3)
+        assert torch.allclose(ops.gated_ffn(*args, activation=act), (g * torch.sigmoid(q) * u) @ args[2].t(), atol=1e-12)
+    assert ops.gated_ffn(args[0][:0], *args[1:]).shape == (0, 6)
+
+
 def test_generator_vectors():
     """Philox-4x32-10's published known answers, as the halves of its words: counters and keys of zeros and of ones."""
     def bits(seed, step, site, row, block):
@@ -133,7 +162,9 @@ def test_arguments():
                 lambda: ops.block_join(x, x, post_weight=w[:4]), lambda: ops.block_join(x, x, pre_weight=w.view(1, 8)),
                 lambda: ops.block_join(x, x, gate=torch.ones(3, 8)), lambda: ops.block_join(x, x, gate=torch.ones(1, 3, 8)),
                 lambda: ops.block_join(x, x, gate=torch.ones(2, 3, 1)), lambda: ops.block_join(x, x, gate=torch.ones(())),
-                lambda: ops.block_join(x, x, dropout=0.1)):
+                lambda: ops.block_join(x, x, dropout=0.1),
+                lambda: ops.gated_ffn(x, torch.ones(4, 8), torch.ones(8, 3)), lambda: ops.gated_ffn(x, torch.ones(4, 7), torch.ones(8, 2)),
+                lambda: ops.gated_ffn(x, torch.ones(4, 8), torch.ones(8, 2), "relu"), lambda: ops.gated_ffn(x, w, w)):
         with pytest.raises(ValueError):
             bad()
     assert [ops._gate_rows(torch.empty(s), x) for s in ((8,), (1, 1, 8), (2, 1, 8), (2, 3, 8))] == [6, 6, 3, 1]
@@ -141,8 +172,8 @@ def test_arguments():
 
 def test_every_kernel_has_a_family():
     names = set()
-    for src in ("loopback_block.hip",):
+    for src in ("loopback_block.hip", "loopback_ffn.hip"):
         with open(os.path.join(ROOT, "loopback_amd", "csrc", src)) as f:
             names |= set(re.findall(r"__global__[^;{]*?\bvoid\s+(k_\w+)\s*\(", f.read(), flags=re.S))
-    assert {"k_dropout", "k_join_fwd", "k_join_bwd", "k_join_sum"} <= names
+    assert {"k_dropout", "k_join_fwd", "k_join_bwd", "k_join_sum", "k_product", "k_split_sum"} <= names
     assert all(RS.family(f"void (anonymous namespace)::{n}<float, 1>(...)") != "torch / runtime" for n in names)
