@@ -55,7 +55,7 @@ struct Operand {
   int64_t half;    // GATED: indices per half (tile indices past its middle are those of the second half); else 0
 };
 
-template <typename T, Kind KIND, int ROWS, int LANES> struct Tile {
+template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile {
   static constexpr int PER = KIND == ROW ? 8 : ROWS / 8;   // 16-byte pieces per row of the tile
   static constexpr int PASSES = ROWS * 8 / LANES, STEP = LANES / PER;
   static_assert(ROWS * 8 % LANES == 0 && STEP % 16 == 0 && (KIND == ROW || ROWS >= 128), "tile shape");
@@ -72,24 +72,40 @@ template <typename T, Kind KIND, int ROWS, int LANES> struct Tile {
     return min(i0 + r, o.size - 1);
   }
 
-  const T* src[PASSES];
+  // aligned operands (rows of a multiple of 8 elements, 16-byte aligned), whole tiles of k from k0 on: a base that all lanes
+  // share and moves on by a tile, and each lane's byte offsets from it
+  const T *base, *base2;   // GATED: of the first and the second half's indices
+  uint32_t off[PASSES];
   int64_t step;
-  // aligned operands (rows of a multiple of 8 elements, 16-byte aligned), whole tiles of k from k0 on
   __device__ __forceinline__ void start(const Operand& o, int64_t i0, int64_t k0) {
-    const T* base = static_cast<const T*>(o.base);
+    const T* b = static_cast<const T*>(o.base);
+    if (KIND == ROW) {
+      base = b + i0 * o.ld + k0;
+      base2 = base + o.half * o.ld;
+      const int last = (int)min((o.half ? o.half : o.size) - 1 - i0, (int64_t)ROWS);
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i)
-      src[i] = KIND == ROW ? base + index(o, i0, row(i)) * o.ld + k0 + 8 * piece()
-                           : base + (k0 + row(i)) * o.ld + min(i0 + 8 * piece(), o.size - 8);
+      for (int i = 0; i < PASSES; ++i) {
+        const int r = GATED_P && i >= PASSES / 2 ? row(i - PASSES / 2) : row(i);
+        off[i] = 2 * ((uint32_t)min(r, last) * (uint32_t)o.ld + 8 * piece());
+      }
+    } else {
+      base = b + k0 * o.ld + i0;
+      const int last = (int)min(o.size - 8 - i0, (int64_t)ROWS);
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) off[i] = 2 * ((uint32_t)row(i) * (uint32_t)o.ld + min(8 * piece(), last));
+    }
     step = KIND == ROW ? BK : BK * o.ld;
   }
   __device__ __forceinline__ void fetch(T* lds) {   // asynchronous: done when vmcnt says so
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      __builtin_amdgcn_global_load_lds((global_void*)src[i], (lds_void*)(lds + 8 * (i * LANES + wave * 64)), 16, 0, 0);
-      src[i] += step;
+      const T* b = GATED_P && i >= PASSES / 2 ? base2 : base;
+      __builtin_amdgcn_global_load_lds((global_void*)(reinterpret_cast<const char*>(b) + off[i]),
+                                       (lds_void*)(lds + 8 * (i * LANES + wave * 64)), 16, 0, 0);
     }
+    base += step;
+    base2 += step;
   }
   // any alignment, k from k0 to k1 (at most BK of them): zeros past k1 and past the operand's indices
   static __device__ __forceinline__ void copy(const Operand& o, int64_t i0, int64_t k0, int64_t k1, T* lds) {
@@ -235,8 +251,8 @@ __device__ __forceinline__ void activation(float g, int act, float& a, float& da
 template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI, bool AL>
 __global__ __launch_bounds__(WP * WQ * 64) void k_product(const Product a) {
   constexpr int LANES = WP * WQ * 64, TP = WP * FP * 32, TQ = WQ * FQ * 32;
-  typedef Tile<T, KP, TP, LANES> PT;
-  typedef Tile<T, KQ, TQ, LANES> QT;
+  typedef Tile<T, KP, TP, LANES, EPI == GATED> PT;
+  typedef Tile<T, KQ, TQ, LANES, false> QT;
   __shared__ __align__(16) T sp0[TP * BK], sq0[TQ * BK], sp1[TP * BK], sq1[TQ * BK];
   // XCD x (workgroups go to XCDs in turn) takes `per` consecutive tiles, in groups of eight rows of tiles: the tiles worked
   // on at a time then share their operands' rows in that XCD's L2
@@ -276,43 +292,46 @@ __global__ __launch_bounds__(WP * WQ * 64) void k_product(const Product a) {
   };
 
   const int64_t whole = AL ? (k1 - k0) / BK : 0;
-  for (int64_t k = k0 + whole * BK; k < k1; k += BK) {   // AL: what is left of k past the whole tiles
+  auto part = [&](int64_t k) {   // up to BK of k, of any alignment
     __syncthreads();
-    PT::copy(a.p, p0, k, k1, sp1);
-    QT::copy(a.q, q0, k, k1, sq1);
+    PT::copy(a.p, p0, k, min(k1, k + BK), sp1);
+    QT::copy(a.q, q0, k, min(k1, k + BK), sq1);
     __syncthreads();
     work(sp1, sq1);
-  }
+  };
   if constexpr (AL) {
+    if (k0 + whole * BK < k1) part(k0 + whole * BK);   // what is left of k past the whole tiles
+    PT pt;
+    QT qt;
+    pt.start(a.p, p0, k0);
+    qt.start(a.q, q0, k0);
     if (whole) {
-      PT pt;
-      QT qt;
-      pt.start(a.p, p0, k0);
-      qt.start(a.q, q0, k0);
       pt.fetch(sp0);
       qt.fetch(sq0);
-      // a tile's loads are waited for, then every wave is past its reads of the other buffer and its loads are here
-      auto ready = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-        __syncthreads();
-      };
-      for (int64_t t = 0;;) {
+    }
+    // a tile's loads are waited for, then every wave is past its reads of the other buffer and its loads are here
+    auto ready = [&]() {
+      __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+      __syncthreads();
+    };
+    for (int64_t t = 0; t < whole; t += 2) {
+      ready();
+      if (t + 1 < whole) {
+        pt.fetch(sp1);
+        qt.fetch(sq1);
+      }
+      work(sp0, sq0);
+      if (t + 1 < whole) {
         ready();
-        if (t + 1 < whole) {
-          pt.fetch(sp1);
-          qt.fetch(sq1);
-        }
-        work(sp0, sq0);
-        if (++t == whole) break;
-        ready();
-        if (t + 1 < whole) {
+        if (t + 2 < whole) {
           pt.fetch(sp0);
           qt.fetch(sq0);
         }
         work(sp1, sq1);
-        if (++t == whole) break;
       }
     }
+  } else {
+    for (int64_t k = k0; k < k1; k += BK) part(k);
   }
 
   const int64_t np = EPI == GATED ? a.p.half : a.p.size;
@@ -412,9 +431,11 @@ int launch_tiles(Product a, hipStream_t st) {
 
 // 256 x 256 tiles by eight waves where they give every CU one; 128 x 128 by four waves else
 constexpr int64_t CUS = 256;
+constexpr int64_t MAX_LD = (1 << 22);   // rows of memory up to which a tile's byte offsets fit 32 bits (256 rows)
 inline int64_t tiles_of(int64_t np, int64_t nq, int64_t t) { return ((np + t - 1) / t) * ((nq + t - 1) / t); }
 
 template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, bool al, hipStream_t st) {
+  al = al && a.p.ld <= MAX_LD && a.q.ld <= MAX_LD;
   if (!al) return launch_tiles<T, KP, KQ, 2, 2, 2, 2, EPI, false>(a, st);
   const int64_t np = a.p.half ? 2 * a.p.half : a.p.size;
   if (tiles_of(np, a.q.size, 256) * a.splits >= CUS / 2) return launch_tiles<T, KP, KQ, 4, 2, 2, 4, EPI, true>(a, st);
