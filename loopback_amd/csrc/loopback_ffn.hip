@@ -8,7 +8,7 @@
 //
 // Operands go through v_mfma_f32_32x32x16 (bf16 or fp16): lane l holds row (P) or column (Q) l mod 32 at k = 8 (l / 32) .. + 8;
 // of the 32 x 32 result it holds column l mod 32 and, in register r, row 4 (l / 32) + r mod 4 + 8 (r / 4): four consecutive p of
-// one q, which one exchange of lane halves makes eight (a 16-byte store). Tiles of 64 k sit in LDS twice, the next one filled
+// one q, which one exchange of lane halves makes eight (a 16-byte store). Tiles of 32 or 64 k sit in LDS twice, the next one filled
 // by direct global -> LDS loads while one is worked on. Such loads write 64 lanes' 16 bytes in order, so the tiles have no
 // padding; instead the 16-byte pieces of a row are permuted: ROW tiles (128-byte rows) by (row / 2) mod 8, so that 16 rows at
 // one k cover the 64 banks once, COL tiles (rows of the tile's width) by 4 (k mod 4), so that the four rows a transposing read
@@ -25,7 +25,6 @@
 
 namespace {
 
-constexpr int BK = 64;             // k per tile
 enum Kind { ROW, COL };
 enum Epi { STORE, PARTIAL, GATED, DGATED };
 
@@ -55,16 +54,18 @@ struct Operand {
   int64_t half;    // GATED: indices per half (tile indices past its middle are those of the second half); else 0
 };
 
-template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile {
-  static constexpr int PER = KIND == ROW ? 8 : ROWS / 8;   // 16-byte pieces per row of the tile
-  static constexpr int PASSES = ROWS * 8 / LANES, STEP = LANES / PER;
-  static_assert(ROWS * 8 % LANES == 0 && STEP % 16 == 0 && (KIND == ROW || ROWS >= 128), "tile shape");
+template <typename T, Kind KIND, int ROWS, int BK, int LANES, bool GATED_P> struct Tile {
+  static constexpr int PER = (KIND == ROW ? BK : ROWS) / 8;   // 16-byte pieces per row of the tile
+  static constexpr int PASSES = ROWS * BK / 8 / LANES, STEP = LANES / PER;
+  static_assert((BK == 64 || BK == 32) && ROWS * BK / 8 % LANES == 0 && STEP % (KIND == ROW ? 16 : 4) == 0 &&
+                (KIND == ROW || ROWS >= 128) && (!GATED_P || PASSES % 2 == 0), "tile shape");
 
+  static __device__ __forceinline__ int swizzle(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
   // this lane's piece of pass i: row i STEP + tid / PER, stored as piece tid % PER, which is piece `piece()` of memory's row
   static __device__ __forceinline__ int row(int i) { return i * STEP + (int)threadIdx.x / PER; }
   static __device__ __forceinline__ int piece() {
     const int r = (int)threadIdx.x / PER, c = (int)threadIdx.x % PER;
-    return KIND == ROW ? c ^ ((r >> 1) & 7) : c ^ (4 * (r & 3));
+    return KIND == ROW ? c ^ swizzle(r) : c ^ (4 * (r & 3));
   }
   // the operand's index of tile row r (ROW) from the tile's first index i0; past the end: the last one
   static __device__ __forceinline__ int64_t index(const Operand& o, int64_t i0, int r) {
@@ -138,7 +139,7 @@ template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile 
     const int lane = (int)threadIdx.x & 63, h = lane >> 5;
     if constexpr (KIND == ROW) {
       const int r = lane & 31;
-      return *reinterpret_cast<const uint4*>(lds + (r0 + r) * BK + 8 * ((2 * s + h) ^ ((r >> 1) & 7)));
+      return *reinterpret_cast<const uint4*>(lds + (r0 + r) * BK + 8 * ((2 * s + h) ^ swizzle(r)));
     } else {
       typedef __attribute__((address_space(3))) s16x4* lds4;
       const int j = lane & 15, kr = j >> 2;
@@ -195,7 +196,7 @@ struct Saved {
 // ---------------------------------------------------------------------------------------------------------------
 struct Product {
   Operand p, q;
-  int64_t k, run;          // k in all, and per split (a multiple of BK)
+  int64_t k, run;          // k in all, and per split
   void* out;               // [q][ldo]; PARTIAL: fp32 [split][q][ldo]
   int64_t ldo;
   void* saved;             // GATED: written (NULL: not wanted); DGATED: read
@@ -248,12 +249,13 @@ __device__ __forceinline__ void activation(float g, int act, float& a, float& da
   if (act && !(g2 < 1e4f)) da = g != g ? g : s;   // far out, where q' overflows: a is 0 or g
 }
 
-template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI, bool AL>
-__global__ __launch_bounds__(WP * WQ * 64) void k_product(const Product a) {
+template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, int BK, Epi EPI, bool AL>
+__global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP * FQ > 8 ? 1 : 2))) void k_product(const Product a) {
   constexpr int LANES = WP * WQ * 64, TP = WP * FP * 32, TQ = WQ * FQ * 32;
-  typedef Tile<T, KP, TP, LANES, EPI == GATED> PT;
-  typedef Tile<T, KQ, TQ, LANES, false> QT;
-  __shared__ __align__(16) T sp0[TP * BK], sq0[TQ * BK], sp1[TP * BK], sq1[TQ * BK];
+  typedef Tile<T, KP, TP, BK, LANES, EPI == GATED> PT;
+  typedef Tile<T, KQ, TQ, BK, LANES, false> QT;
+  // objects of their own: what is read is seen not to be what is being filled
+  __shared__ __align__(16) T sp0[TP * BK], sq0[TQ * BK], sp1[AL ? TP * BK : 8], sq1[AL ? TQ * BK : 8];
   // XCD x (workgroups go to XCDs in turn) takes `per` consecutive tiles, in groups of eight rows of tiles: the tiles worked
   // on at a time then share their operands' rows in that XCD's L2
   const int id = ((int)blockIdx.x & 7) * a.per + ((int)blockIdx.x >> 3);
@@ -265,8 +267,9 @@ __global__ __launch_bounds__(WP * WQ * 64) void k_product(const Product a) {
   const int64_t k0 = split * a.run, k1 = min(a.k, k0 + a.run);
   const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wp = wave % WP, wq = wave / WP;
-  // GATED: a wave's two P tiles are the gate's and the up projection's of the same columns
-  auto p_row = [&](int i) { return EPI == GATED ? i * (TP / 2) + 32 * wp : 32 * (wp * FP + i); };
+  // GATED: a wave's P tiles are the gate's and then the up projection's of the same columns
+  constexpr int FH = FP / 2;
+  auto p_row = [&](int i) { return EPI == GATED ? i / FH * (TP / 2) + 32 * (wp * FH + i % FH) : 32 * (wp * FP + i); };
 
   f32x16 acc[FP][FQ];
 #pragma unroll
@@ -276,62 +279,104 @@ __global__ __launch_bounds__(WP * WQ * 64) void k_product(const Product a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  auto work = [&](const T* sp, const T* sq) {
+  constexpr int STEPS = BK / 16, READS = (KP == COL ? 2 : 1) * FP + (KQ == COL ? 2 : 1) * FQ;
+  struct Frags { uint4 p[FP], q[FQ]; };
+  auto read = [&](const T* sp, const T* sq, int s, Frags& f) {
 #pragma unroll
-    for (int s = 0; s < BK / 16; ++s) {
-      uint4 fp[FP], fq[FQ];
+    for (int i = 0; i < FP; ++i) f.p[i] = PT::frag(sp, p_row(i), s);
 #pragma unroll
-      for (int i = 0; i < FP; ++i) fp[i] = PT::frag(sp, p_row(i), s);
+    for (int j = 0; j < FQ; ++j) f.q[j] = QT::frag(sq, 32 * (wq * FQ + j), s);
+  };
+  auto multiply = [&](const Frags& f) {
 #pragma unroll
-      for (int j = 0; j < FQ; ++j) fq[j] = QT::frag(sq, 32 * (wq * FQ + j), s);
+    for (int i = 0; i < FP; ++i)
 #pragma unroll
-      for (int i = 0; i < FP; ++i)
+      for (int j = 0; j < FQ; ++j) acc[i][j] = mfma(T{}, f.p[i], f.q[j], acc[i][j]);
+  };
+  // a step's matrix instructions with the next step's reads between them
+  auto interleave = [&]() {
 #pragma unroll
-        for (int j = 0; j < FQ; ++j) acc[i][j] = mfma(T{}, fp[i], fq[j], acc[i][j]);
+    for (int m = 0; m < FP * FQ; ++m) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, (READS + FP * FQ - 1) / (FP * FQ), 0);
     }
   };
 
-  const int64_t whole = AL ? (k1 - k0) / BK : 0;
-  auto part = [&](int64_t k) {   // up to BK of k, of any alignment
-    __syncthreads();
-    PT::copy(a.p, p0, k, min(k1, k + BK), sp1);
-    QT::copy(a.q, q0, k, min(k1, k + BK), sq1);
-    __syncthreads();
-    work(sp1, sq1);
+  auto copy = [&](int64_t k, T* sp, T* sq) {   // up to BK of k, of any alignment
+    PT::copy(a.p, p0, k, min(k1, k + BK), sp);
+    QT::copy(a.q, q0, k, min(k1, k + BK), sq);
   };
   if constexpr (AL) {
-    if (k0 + whole * BK < k1) part(k0 + whole * BK);   // what is left of k past the whole tiles
+    // Each step's operands are read while the step before it is multiplied. A tile's last step is multiplied after the
+    // barrier: every wave is past its reads of this tile, whose buffer is filled with the tile after the next one, and the
+    // next tile's loads have arrived, whose first step is read. What is left of k past the whole tiles is the first tile.
+    const int whole = (int)((k1 - k0) / BK), left = k0 + (int64_t)whole * BK < k1 ? 1 : 0, tiles = whole + left;
     PT pt;
     QT qt;
-    pt.start(a.p, p0, k0);
-    qt.start(a.q, q0, k0);
-    if (whole) {
-      pt.fetch(sp0);
-      qt.fetch(sq0);
-    }
-    // a tile's loads are waited for, then every wave is past its reads of the other buffer and its loads are here
-    auto ready = [&]() {
+    auto fetch = [&](T* sp, T* sq) {
+      pt.fetch(sp);
+      qt.fetch(sq);
+    };
+    Frags f[2];
+    auto steps = [&](const T* sp, const T* sq) {   // all but the last
+#pragma unroll
+      for (int s = 0; s + 1 < STEPS; ++s) {
+        read(sp, sq, s + 1, f[(s + 1) & 1]);
+        multiply(f[s & 1]);
+        interleave();
+      }
+    };
+    auto arrived = [&]() {
       __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
       __syncthreads();
     };
-    for (int64_t t = 0; t < whole; t += 2) {
-      ready();
-      if (t + 1 < whole) {
-        pt.fetch(sp1);
-        qt.fetch(sq1);
-      }
-      work(sp0, sq0);
-      if (t + 1 < whole) {
-        ready();
-        if (t + 2 < whole) {
-          pt.fetch(sp0);
-          qt.fetch(sq0);
-        }
-        work(sp1, sq1);
-      }
+    auto tile = [&](T* sp, T* sq, const T* np, const T* nq) {   // another after the next one
+      steps(sp, sq);
+      arrived();
+      read(np, nq, 0, f[0]);
+      fetch(sp, sq);
+      multiply(f[(STEPS - 1) & 1]);
+    };
+    if (left) copy(k0 + (int64_t)whole * BK, sp0, sq0);
+    pt.start(a.p, p0, k0);
+    qt.start(a.q, q0, k0);
+    if (!left && tiles) fetch(sp0, sq0);
+    arrived();
+    if (tiles > 1) fetch(sp1, sq1);
+    read(sp0, sq0, 0, f[0]);
+    int t = tiles;   // tiles to do
+    for (; t >= 4; t -= 2) {
+      tile(sp0, sq0, sp1, sq1);
+      tile(sp1, sq1, sp0, sq0);
+    }
+    const T *cp = sp0, *cq = sq0, *np = sp1, *nq = sq1;
+    if (t == 3) {
+      tile(sp0, sq0, sp1, sq1);
+      cp = sp1, cq = sq1, np = sp0, nq = sq0;
+    }
+    if (t >= 2) {
+      steps(cp, cq);
+      arrived();
+      read(np, nq, 0, f[0]);
+      multiply(f[(STEPS - 1) & 1]);
+      cp = np, cq = nq;
+    }
+    if (t) {
+      steps(cp, cq);
+      multiply(f[(STEPS - 1) & 1]);
     }
   } else {
-    for (int64_t k = k0; k < k1; k += BK) part(k);
+    for (int64_t k = k0; k < k1; k += BK) {
+      __syncthreads();
+      copy(k, sp0, sq0);
+      __syncthreads();
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        Frags f;
+        read(sp0, sq0, s, f);
+        multiply(f);
+      }
+    }
   }
 
   const int64_t np = EPI == GATED ? a.p.half : a.p.size;
@@ -340,15 +385,17 @@ __global__ __launch_bounds__(WP * WQ * 64) void k_product(const Product a) {
     const int64_t qt = q0 + 32 * (wq * FQ + j), q = qt + (lane & 31);
     const bool ok = q < a.q.size;
     if constexpr (EPI == GATED) {
-      const int64_t p = p0 + 32 * wp;
-      if (qt < a.q.size && p < np) {
+#pragma unroll
+      for (int i = 0; i < FH; ++i) {
+        const int64_t p = p0 + p_row(i);
+        if (qt >= a.q.size || p >= np) continue;   // wave-uniform
         f32x16 x, y, z;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           float av, da;
-          activation(acc[0][j][r], a.act, av, da);
-          z[r] = av * acc[1][j][r];
-          x[r] = acc[1][j][r] * da;
+          activation(acc[i][j][r], a.act, av, da);
+          z[r] = av * acc[FH + i][j][r];
+          x[r] = acc[FH + i][j][r] * da;
           y[r] = av;
         }
         store_tile<T, AL>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, z);
@@ -416,8 +463,9 @@ inline bool al2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) ==
 inline int launched() { return (int)hipGetLastError(); }
 constexpr int64_t MAX_SIZE = 0x7fffffff;   // of one dimension
 
-template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI, bool AL>
+template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, int BK, Epi EPI, bool AL>
 int launch_tiles(Product a, hipStream_t st) {
+  a.run = (a.run + BK - 1) / BK * BK;
   constexpr int TP = (EPI == GATED ? WP * FP * 16 : WP * FP * 32), TQ = WQ * FQ * 32;
   const int64_t np = EPI == GATED ? a.p.half : a.p.size;
   const int64_t tp = (np + TP - 1) / TP, tq = (a.q.size + TQ - 1) / TQ, tiles = tp * tq;
@@ -425,7 +473,7 @@ int launch_tiles(Product a, hipStream_t st) {
   a.tiles_p = (int)tp;
   a.tiles = (int)tiles;
   a.per = (int)((tiles * a.splits + 7) / 8);
-  hipLaunchKernelGGL((k_product<T, KP, KQ, WP, WQ, FP, FQ, EPI, AL>), dim3((unsigned)(8 * a.per)), dim3(WP * WQ * 64), 0, st, a);
+  hipLaunchKernelGGL((k_product<T, KP, KQ, WP, WQ, FP, FQ, BK, EPI, AL>), dim3((unsigned)(8 * a.per)), dim3(WP * WQ * 64), 0, st, a);
   return launched();
 }
 
@@ -436,10 +484,15 @@ inline int64_t tiles_of(int64_t np, int64_t nq, int64_t t) { return ((np + t - 1
 
 template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, bool al, hipStream_t st) {
   al = al && a.p.ld <= MAX_LD && a.q.ld <= MAX_LD;
-  if (!al) return launch_tiles<T, KP, KQ, 2, 2, 2, 2, EPI, false>(a, st);
+  if (!al) return launch_tiles<T, KP, KQ, 2, 2, 2, 2, 64, EPI, false>(a, st);
+#ifdef FFN_EXP
+  static const int cfg = getenv("FFN_CFG") ? atoi(getenv("FFN_CFG")) : 0;
+  if (cfg == 1) return launch_tiles<T, KP, KQ, 4, 2, 2, 4, 64, EPI, true>(a, st);
+  if (cfg == 2) return launch_tiles<T, KP, KQ, 2, 2, 2, 2, 64, EPI, true>(a, st);
+#endif
   const int64_t np = a.p.half ? 2 * a.p.half : a.p.size;
-  if (tiles_of(np, a.q.size, 256) * a.splits >= CUS / 2) return launch_tiles<T, KP, KQ, 4, 2, 2, 4, EPI, true>(a, st);
-  return launch_tiles<T, KP, KQ, 2, 2, 2, 2, EPI, true>(a, st);
+  if (tiles_of(np, a.q.size, 256) * a.splits >= CUS / 2) return launch_tiles<T, KP, KQ, 4, 2, 2, 4, 64, EPI, true>(a, st);
+  return launch_tiles<T, KP, KQ, 2, 2, 2, 2, 64, EPI, true>(a, st);
 }
 
 #define FFN_TYPE_SWITCH(DT, ...)                                 \
@@ -452,7 +505,7 @@ inline int sizes(int64_t a, int64_t b, int64_t c, int dtype) {
   return a > MAX_SIZE || b > MAX_SIZE || c > MAX_SIZE ? LDR_E_SHAPE : LDR_OK;
 }
 inline Product product(Operand p, Operand q, int64_t k, void* out, int64_t ldo) {
-  return Product{p, q, k, (k + BK - 1) / BK * BK, out, ldo, nullptr, 0, 0, 0, 1, 0, 0};
+  return Product{p, q, k, k, out, ldo, nullptr, 0, 0, 0, 1, 0, 0};
 }
 
 }  // namespace
@@ -539,7 +592,7 @@ int lbk_linear_dw(const void* dy, const void* x, float* scratch, void* dw, int64
   if (splits == 1) {
     FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, COL, STORE>(a, al, st)))
   }
-  a.run = ((t + splits - 1) / splits + BK - 1) / BK * BK;
+  a.run = ((t + splits - 1) / splits + 63) / 64 * 64;
   a.splits = (int)((t + a.run - 1) / a.run);
   a.out = scratch;
   FFN_TYPE_SWITCH(dtype, {
