@@ -249,6 +249,18 @@ __device__ __forceinline__ void activation(float g, int act, float& a, float& da
   if (act && !(g2 < 1e4f)) da = g != g ? g : s;   // far out, where q' overflows: a is 0 or g
 }
 
+// the order of a step: N matrix instructions, after the first of them the next step's READS (two each, so that the last
+// have arrived when the step ends), and LOADS tile loads spread over all
+template <int N, int READS, int LOADS, int M = 0> __device__ __forceinline__ void interleave() {
+  if constexpr (M < N) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    constexpr int r = READS - 2 * M > 2 ? 2 : READS - 2 * M, l = (M + 1) * LOADS / N - M * LOADS / N;
+    if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
+    if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x010, l, 0);
+    interleave<N, READS, LOADS, M + 1>();
+  }
+}
+
 template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, int BK, Epi EPI, bool AL>
 __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP * FQ > 8 ? 1 : 2))) void k_product(const Product a) {
   constexpr int LANES = WP * WQ * 64, TP = WP * FP * 32, TQ = WQ * FQ * 32;
@@ -293,15 +305,6 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
 #pragma unroll
       for (int j = 0; j < FQ; ++j) acc[i][j] = mfma(T{}, f.p[i], f.q[j], acc[i][j]);
   };
-  // a step's matrix instructions with the next step's reads between them
-  auto interleave = [&]() {
-#pragma unroll
-    for (int m = 0; m < FP * FQ; ++m) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, (READS + FP * FQ - 1) / (FP * FQ), 0);
-    }
-  };
-
   auto copy = [&](int64_t k, T* sp, T* sq) {   // up to BK of k, of any alignment
     PT::copy(a.p, p0, k, min(k1, k + BK), sp);
     QT::copy(a.q, q0, k, min(k1, k + BK), sq);
@@ -323,7 +326,7 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
       for (int s = 0; s + 1 < STEPS; ++s) {
         read(sp, sq, s + 1, f[(s + 1) & 1]);
         multiply(f[s & 1]);
-        interleave();
+        interleave<FP * FQ, READS, 0>();
       }
     };
     auto arrived = [&]() {
@@ -336,6 +339,7 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
       read(np, nq, 0, f[0]);
       fetch(sp, sq);
       multiply(f[(STEPS - 1) & 1]);
+      interleave<FP * FQ, READS, PT::PASSES + QT::PASSES>();
     };
     if (left) copy(k0 + (int64_t)whole * BK, sp0, sq0);
     pt.start(a.p, p0, k0);
