@@ -54,7 +54,14 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* h, const void* y, c
 
 /* ---- gated feed-forward block, bf16 and fp16 ---------------------------------------------------------------------
  * y = (a(x Wg^T) * (x Wu^T)) Wd^T for x [t, d], w = [Wg; Wu] [2 n, d], Wd [d_out, n]; activation 0: a(g) = g sigmoid(g)
- * (silu), 1: gelu in its tanh form. Sizes below 2^31, element alignment (2 bytes). */
+ * (silu), 1: gelu in its tanh form. Sizes below 2^31. Every matrix has its rows ld elements apart (up to 2^22). Operands are
+ * 16-byte aligned with ld a multiple of 8, all ld elements of a row readable -- lbk_pad_rows makes such a copy of one that
+ * is not -- or, for up to LBK_FEW_TOKENS tokens of lbk_linear_fwd, and of lbk_ffn_gate_up without `saved`, of any alignment.
+ * Results may have any. */
+#define LBK_FEW_TOKENS 64
+
+/* out [rows, ld] = x [rows, cols], contiguous, with zeros past the columns. */
+int lbk_pad_rows(const void* x, int64_t rows, int64_t cols, int64_t ld, void* out, int dtype, void* stream);
 
 /* Bytes of `saved`, what the backward needs of the two projections: (u a'(g), a(g)) per (token, column) in the kernels' own
  * order, 24 bits each. 16-byte aligned. */
@@ -62,21 +69,24 @@ int64_t lbk_ffn_saved_bytes(int64_t t, int64_t n);
 
 /* act [t, n] = round(a(x Wg^T) * (x Wu^T)): both projections, the activation and the product in one kernel. saved: NULL
  * where no backward follows. */
-int lbk_ffn_gate_up(const void* x, const void* w, void* act, void* saved, int64_t t, int64_t d, int64_t n, int activation,
-                    int dtype, void* stream);
+int lbk_ffn_gate_up(const void* x, int64_t ldx, const void* w, int64_t ldw, void* act, int64_t ld_act, void* saved, int64_t t,
+                    int64_t d, int64_t n, int activation, int dtype, void* stream);
 
 /* dgate_up [t, 2 n]: the gradients of the two projections for dy [t, d] (the block's output), the product dy Wd and the
  * activation's gradient in one kernel. w_down [d, n]. */
-int lbk_ffn_dgate_up(const void* dy, const void* w_down, const void* saved, void* dgate_up, int64_t t, int64_t n, int64_t d,
-                     int dtype, void* stream);
+int lbk_ffn_dgate_up(const void* dy, int64_t ld_dy, const void* w_down, int64_t ldw, const void* saved, void* dgate_up,
+                     int64_t ld_dgu, int64_t t, int64_t n, int64_t d, int dtype, void* stream);
 
-/* The block's plain products: y [t, n] = x [t, k] w [n, k]^T; dx [t, k] = dy [t, n] w [n, k]; dw [n, k] = dy^T x, whose
- * tokens are split where that fills the GPU (scratch: lbk_linear_dw_scratch floats, NULL where that is 0). */
-int lbk_linear_fwd(const void* x, const void* w, void* y, int64_t t, int64_t k, int64_t n, int dtype, void* stream);
-int lbk_linear_dx(const void* dy, const void* w, void* dx, int64_t t, int64_t n, int64_t k, int dtype, void* stream);
-int64_t lbk_linear_dw_scratch(int64_t t, int64_t n, int64_t k);
-int lbk_linear_dw(const void* dy, const void* x, float* scratch, void* dw, int64_t t, int64_t n, int64_t k, int dtype,
-                  void* stream);
+/* The block's plain products: y [t, n] = x [t, k] w [n, k]^T; dx [t, k] = dy [t, n] w [n, k]; dw [n, k] = dy^T x (contiguous).
+ * The summed dimension is split where that fills the GPU; scratch has lbk_linear_scratch(columns and rows of the result,
+ * summed dimension) floats (NULL where that is 0), 16-byte aligned. */
+int64_t lbk_linear_scratch(int64_t columns, int64_t rows, int64_t summed);
+int lbk_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t ldy, float* scratch, int64_t t,
+                   int64_t k, int64_t n, int dtype, void* stream);
+int lbk_linear_dx(const void* dy, int64_t ld_dy, const void* w, int64_t ldw, void* dx, int64_t ld_dx, float* scratch, int64_t t,
+                  int64_t n, int64_t k, int dtype, void* stream);
+int lbk_linear_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ldx, float* scratch, void* dw, int64_t t, int64_t n,
+                  int64_t k, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

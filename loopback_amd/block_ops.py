@@ -29,6 +29,8 @@ from .lm_ops import _again, _launchable, _stream, _watched, native
 
 ABI_VERSION = 1
 JOIN_MAX_WIDTH = 8192
+FEW_TOKENS = 64
+FFN_MAX_WIDTH = 2 ** 22 - 8   # elements between rows of the tiled products' operands
 MAX_ROWS = 2 ** 31 - 1
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -42,12 +44,13 @@ SIGNATURES = {
     "lbk_join_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _u32, _i32, _f32, _p, _p, _p, _p, _p, _p, _i64,
                             _i64, _i32, _p]),
     "lbk_ffn_saved_bytes": (_i64, [_i64, _i64]),
-    "lbk_ffn_gate_up": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _p]),
-    "lbk_ffn_dgate_up": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
-    "lbk_linear_fwd": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i32, _p]),
-    "lbk_linear_dx": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i32, _p]),
-    "lbk_linear_dw_scratch": (_i64, [_i64, _i64, _i64]),
-    "lbk_linear_dw": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "lbk_pad_rows": (_i32, [_p, _i64, _i64, _i64, _p, _i32, _p]),
+    "lbk_ffn_gate_up": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p]),
+    "lbk_ffn_dgate_up": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i32, _p]),
+    "lbk_linear_scratch": (_i64, [_i64, _i64, _i64]),
+    "lbk_linear_fwd": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
+    "lbk_linear_dx": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
+    "lbk_linear_dw": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _p]),
 }
 
 
@@ -340,24 +343,44 @@ def _ffn_torch(x, w_gate_up, w_down, activation):
     return F.linear(a * u, w_down)
 
 
+def _operand(t, code, st):
+    """(tensor, address, elements between rows) of contiguous rows as the tiled products take them: the tensor itself where its
+    rows are aligned, else a copy that is."""
+    cols = t.shape[-1]
+    if cols % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, t.data_ptr(), cols
+    rows, ld = t.numel() // cols, (cols + 7) // 8 * 8
+    out = torch.empty((rows, ld), device=t.device, dtype=t.dtype)
+    _run("lbk_pad_rows", t.data_ptr(), rows, cols, ld, out.data_ptr(), code, st)
+    return out, out.data_ptr(), ld
+
+
+def _scratch(columns, rows, summed, like):
+    n = LIB.lbk_linear_scratch(columns, rows, summed)
+    return torch.empty(n, device=like.device, dtype=torch.float32) if n else None
+
+
 def _ffn_forward(x, w_gate_up, w_down, activation, keep):
-    """y, and what the backward needs: the activations and the projections' saved values."""
-    t, d = x.numel() // x.shape[-1], x.shape[-1]
-    n, m, code, st = w_down.shape[1], w_down.shape[0], _CODES[x.dtype], _stream(x)
-    act = torch.empty((t, n), device=x.device, dtype=x.dtype)
+    """y, and what the backward needs: the activations (t, n rounded up to 8) and the projections' saved values."""
+    d, (m, n), code, st = x.shape[-1], w_down.shape, _CODES[x.dtype], _stream(x)
+    t = x.numel() // d
+    n8 = (n + 7) // 8 * 8
+    act = torch.empty((t, n8), device=x.device, dtype=x.dtype)
     saved = torch.empty(LIB.lbk_ffn_saved_bytes(t, n), device=x.device, dtype=torch.uint8) if keep else None
-    _run("lbk_ffn_gate_up", x.data_ptr(), w_gate_up.data_ptr(), act.data_ptr(), _ptr(saved), t, d, n, activation, code, st)
     y = torch.empty((*x.shape[:-1], m), device=x.device, dtype=x.dtype)
-    _run("lbk_linear_fwd", act.data_ptr(), w_down.data_ptr(), y.data_ptr(), t, n, m, code, st)
+    if t <= FEW_TOKENS and not keep:
+        (xp, ldx), (wp, ldw) = (x.data_ptr(), d), (w_gate_up.data_ptr(), d)
+    else:
+        x, xp, ldx = _operand(x, code, st)
+        w_gate_up, wp, ldw = _operand(w_gate_up, code, st)
+    _run("lbk_ffn_gate_up", xp, ldx, wp, ldw, act.data_ptr(), n8, _ptr(saved), t, d, n, activation, code, st)
+    if t <= FEW_TOKENS:
+        wp, ldw, scratch = w_down.data_ptr(), n, None
+    else:
+        w_down, wp, ldw = _operand(w_down, code, st)
+        scratch = _scratch(m, t, n, x)
+    _run("lbk_linear_fwd", act.data_ptr(), n8, wp, ldw, y.data_ptr(), m, _ptr(scratch), t, n, m, code, st)
     return y, act, saved
-
-
-def _linear_dw(dy, x, w, t, code, st):
-    dw = torch.empty_like(w)
-    size = LIB.lbk_linear_dw_scratch(t, *w.shape)
-    scratch = torch.empty(size, device=w.device, dtype=torch.float32) if size else None
-    _run("lbk_linear_dw", dy.data_ptr(), x.data_ptr(), _ptr(scratch), dw.data_ptr(), t, *w.shape, code, st)
-    return dw
 
 
 class _GatedFfn(torch.autograd.Function):
@@ -378,22 +401,32 @@ class _GatedFfn(torch.autograd.Function):
         if not _launchable(dy):
             fn = lambda x, g, d: _ffn_torch(x, g, d, ctx.activation)
             return *_again(fn, [x, w_gate_up, w_down], need[:3], dy), None
-        dy = dy.to(x.dtype).contiguous()
-        t, d = x.numel() // x.shape[-1], x.shape[-1]
-        (m, n), code, st = w_down.shape, _CODES[x.dtype], _stream(x)
+        d, (m, n), code, st = x.shape[-1], w_down.shape, _CODES[x.dtype], _stream(x)
+        t = x.numel() // d
+        dy, dyp, ld_dy = _operand(dy.to(x.dtype).contiguous(), code, st)
         dx = dw_gate_up = dw_down = None
         if need[0] or need[1]:
             if saved.data_ptr() % 16:
                 saved = saved.clone()   # a saved-tensor hook's
-            dgu = torch.empty((t, 2 * n), device=x.device, dtype=x.dtype)
-            _run("lbk_ffn_dgate_up", dy.data_ptr(), w_down.data_ptr(), saved.data_ptr(), dgu.data_ptr(), t, n, m, code, st)
+            ld = (2 * n + 7) // 8 * 8
+            dgu = torch.empty((t, ld), device=x.device, dtype=x.dtype)
+            wd, wp, ldw = _operand(w_down, code, st)
+            _run("lbk_ffn_dgate_up", dyp, ld_dy, wp, ldw, saved.data_ptr(), dgu.data_ptr(), ld, t, n, m, code, st)
             if need[0]:
                 dx = torch.empty_like(x)
-                _run("lbk_linear_dx", dgu.data_ptr(), w_gate_up.data_ptr(), dx.data_ptr(), t, 2 * n, d, code, st)
+                w, wp, ldw = _operand(w_gate_up, code, st)
+                s = _scratch(d, t, 2 * n, x)
+                _run("lbk_linear_dx", dgu.data_ptr(), ld, wp, ldw, dx.data_ptr(), d, _ptr(s), t, 2 * n, d, code, st)
             if need[1]:
-                dw_gate_up = _linear_dw(dgu, x, w_gate_up, t, code, st)
+                dw_gate_up = torch.empty_like(w_gate_up)
+                xs, xp, ldx = _operand(x, code, st)
+                s = _scratch(d, 2 * n, t, x)
+                _run("lbk_linear_dw", dgu.data_ptr(), ld, xp, ldx, _ptr(s), dw_gate_up.data_ptr(), t, 2 * n, d, code, st)
         if need[2]:
-            dw_down = _linear_dw(dy, act, w_down, t, code, st)
+            dw_down = torch.empty_like(w_down)
+            act, ap, ld_act = _operand(act, code, st)
+            s = _scratch(n, m, t, x)
+            _run("lbk_linear_dw", dyp, ld_dy, ap, ld_act, _ptr(s), dw_down.data_ptr(), t, m, n, code, st)
         return dx, dw_gate_up, dw_down, None
 
 
@@ -409,7 +442,7 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ac
                          f"{tuple(w_gate_up.shape)} and {tuple(w_down.shape)}")
     code = ACTIVATIONS[activation]
     if not (native(x, w_gate_up, w_down) and x.numel() > 0 and w_down.numel() > 0
-            and max(x.numel() // x.shape[-1], *w_gate_up.shape, *w_down.shape) <= MAX_ROWS):
+            and x.numel() // x.shape[-1] <= MAX_ROWS and max(*w_gate_up.shape, *w_down.shape) <= FFN_MAX_WIDTH):
         return _ffn_torch(x, w_gate_up, w_down, code)
     x, w_gate_up, w_down = _plain_rows(x, w_gate_up, w_down)   # recorded, where they copy
     if _records(x, w_gate_up, w_down):

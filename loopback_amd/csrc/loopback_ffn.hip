@@ -47,7 +47,7 @@ template <> struct CvtOf<_Float16> { typedef F16Cvt type; };
 // ---------------------------------------------------------------------------------------------------------------
 // one operand: where it lies, and its tile of ROWS indices (ROW) or columns (COL) x 64 k
 // ---------------------------------------------------------------------------------------------------------------
-struct Operand {
+struct Operand {   // 16-byte aligned, ld a multiple of 8; COL: every row's ld elements can be read
   const void* base;
   int64_t ld;      // elements between rows of memory
   int64_t size;    // indices
@@ -73,8 +73,7 @@ template <typename T, Kind KIND, int ROWS, int BK, int LANES, bool GATED_P> stru
     return min(i0 + r, o.size - 1);
   }
 
-  // aligned operands (rows of a multiple of 8 elements, 16-byte aligned), whole tiles of k from k0 on: a base that all lanes
-  // share and moves on by a tile, and each lane's byte offsets from it
+  // whole tiles of k from k0 on: a base that all lanes share and moves on by a tile, and each lane's byte offsets from it
   const T *base, *base2;   // GATED: of the first and the second half's indices
   uint32_t off[PASSES];
   int64_t step;
@@ -91,7 +90,7 @@ template <typename T, Kind KIND, int ROWS, int BK, int LANES, bool GATED_P> stru
       }
     } else {
       base = b + k0 * o.ld + i0;
-      const int last = (int)min(o.size - 8 - i0, (int64_t)ROWS);
+      const int last = (int)min((o.size - 1 - i0) & ~(int64_t)7, (int64_t)ROWS);
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) off[i] = 2 * ((uint32_t)row(i) * (uint32_t)o.ld + min(8 * piece(), last));
     }
@@ -108,7 +107,7 @@ template <typename T, Kind KIND, int ROWS, int BK, int LANES, bool GATED_P> stru
     base += step;
     base2 += step;
   }
-  // any alignment, k from k0 to k1 (at most BK of them): zeros past k1 and past the operand's indices
+  // k from k0 to k1, fewer than BK of them: zeros past k1 and past the operand's indices
   static __device__ __forceinline__ void copy(const Operand& o, int64_t i0, int64_t k0, int64_t k1, T* lds) {
     const T* base = static_cast<const T*>(o.base);
 #pragma unroll
@@ -124,7 +123,7 @@ template <typename T, Kind KIND, int ROWS, int BK, int LANES, bool GATED_P> stru
       }
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (left >= 8) {
-        v = UIO<T>::raw(p).u;
+        v = *reinterpret_cast<const uint4*>(p);
       } else if (left > 0) {
         struct { T e[8]; } e;
 #pragma unroll
@@ -197,8 +196,9 @@ struct Saved {
 struct Product {
   Operand p, q;
   int64_t k, run;          // k in all, and per split
-  void* out;               // [q][ldo]; PARTIAL: fp32 [split][q][ldo]
+  void* out;               // [q][ldo]; PARTIAL: fp32 [split][q][ldo], ldo a multiple of 4
   int64_t ldo;
+  bool out16;              // whole 16-byte vectors of the result are aligned
   void* saved;             // GATED: written (NULL: not wanted); DGATED: read
   int64_t saved_cols;      // its blocks of columns
   int tiles_p, tiles, splits, per;
@@ -207,8 +207,8 @@ struct Product {
 
 // 16 registers of a result tile (column q = this lane's, rows p0 + 4 h + r mod 4 + 8 (r / 4)) to out[p0 ..], rounded:
 // exchanged between the lane halves so that each lane has eight consecutive p, twice
-template <typename T, bool AL>
-__device__ __forceinline__ void store_tile(T* row, int64_t p0, int64_t np, bool ok, const f32x16& v) {
+template <typename T>
+__device__ __forceinline__ void store_tile(T* row, int64_t p0, int64_t np, bool ok, bool al, const f32x16& v) {
   typedef typename CvtOf<T>::type Cvt;
   const int h = ((int)threadIdx.x >> 5) & 1;
 #pragma unroll
@@ -223,16 +223,15 @@ __device__ __forceinline__ void store_tile(T* row, int64_t p0, int64_t np, bool 
       u[2 + e] = (unsigned)sw[1];
     }
     const int64_t p = p0 + 16 * g + 8 * h;
-    if (ok) {
-      if (AL ? p < np : p + 8 <= np) {
-        if (AL) *reinterpret_cast<uint4*>(row + p) = make_uint4(u[0], u[1], u[2], u[3]);
-        else *reinterpret_cast<u32x4_u16*>(row + p) = u32x4{u[0], u[1], u[2], u[3]};
-      } else if (!AL && p < np) {
-        struct { T e[8]; } e = __builtin_bit_cast(decltype(e), make_uint4(u[0], u[1], u[2], u[3]));
+    if (!ok) continue;
+    if (p + 8 <= np) {
+      if (al) *reinterpret_cast<uint4*>(row + p) = make_uint4(u[0], u[1], u[2], u[3]);
+      else *reinterpret_cast<u32x4_u16*>(row + p) = u32x4{u[0], u[1], u[2], u[3]};
+    } else if (p < np) {
+      struct { T e[8]; } e = __builtin_bit_cast(decltype(e), make_uint4(u[0], u[1], u[2], u[3]));
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (p + k < np) row[p + k] = e.e[k];
-      }
+      for (int k = 0; k < 8; ++k)
+        if (p + k < np) row[p + k] = e.e[k];
     }
   }
 }
@@ -261,13 +260,13 @@ template <int N, int READS, int LOADS, int M = 0> __device__ __forceinline__ voi
   }
 }
 
-template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, int BK, Epi EPI, bool AL>
+template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, int BK, Epi EPI>
 __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP * FQ > 8 ? 1 : 2))) void k_product(const Product a) {
   constexpr int LANES = WP * WQ * 64, TP = WP * FP * 32, TQ = WQ * FQ * 32;
   typedef Tile<T, KP, TP, BK, LANES, EPI == GATED> PT;
   typedef Tile<T, KQ, TQ, BK, LANES, false> QT;
   // objects of their own: what is read is seen not to be what is being filled
-  __shared__ __align__(16) T sp0[TP * BK], sq0[TQ * BK], sp1[AL ? TP * BK : 8], sq1[AL ? TQ * BK : 8];
+  __shared__ __align__(16) T sp0[TP * BK], sq0[TQ * BK], sp1[TP * BK], sq1[TQ * BK];
   // XCD x (workgroups go to XCDs in turn) takes `per` consecutive tiles, in groups of eight rows of tiles: the tiles worked
   // on at a time then share their operands' rows in that XCD's L2
   const int id = ((int)blockIdx.x & 7) * a.per + ((int)blockIdx.x >> 3);
@@ -305,11 +304,11 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
 #pragma unroll
       for (int j = 0; j < FQ; ++j) acc[i][j] = mfma(T{}, f.p[i], f.q[j], acc[i][j]);
   };
-  auto copy = [&](int64_t k, T* sp, T* sq) {   // up to BK of k, of any alignment
+  auto copy = [&](int64_t k, T* sp, T* sq) {   // fewer than BK of k
     PT::copy(a.p, p0, k, min(k1, k + BK), sp);
     QT::copy(a.q, q0, k, min(k1, k + BK), sq);
   };
-  if constexpr (AL) {
+  {
     // Each step's operands are read while the step before it is multiplied. A tile's last step is multiplied after the
     // barrier: every wave is past its reads of this tile, whose buffer is filled with the tile after the next one, and the
     // next tile's loads have arrived, whose first step is read. What is left of k past the whole tiles is the first tile.
@@ -369,18 +368,6 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
       steps(cp, cq);
       multiply(f[(STEPS - 1) & 1]);
     }
-  } else {
-    for (int64_t k = k0; k < k1; k += BK) {
-      __syncthreads();
-      copy(k, sp0, sq0);
-      __syncthreads();
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        Frags f;
-        read(sp0, sq0, s, f);
-        multiply(f);
-      }
-    }
   }
 
   const int64_t np = EPI == GATED ? a.p.half : a.p.size;
@@ -402,7 +389,7 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
           x[r] = acc[FH + i][j][r] * da;
           y[r] = av;
         }
-        store_tile<T, AL>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, z);
+        store_tile<T>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, a.out16, z);
         if (a.saved) {
           char* block = static_cast<char*>(a.saved) + ((qt >> 5) * a.saved_cols + (p >> 5)) * SAVED_BLOCK;
           Saved::put(block, x);
@@ -415,7 +402,7 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
         const int64_t p = p0 + p_row(i);
         if (qt >= a.q.size || p >= np) continue;   // wave-uniform
         if constexpr (EPI == STORE) {
-          store_tile<T, AL>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, acc[i][j]);
+          store_tile<T>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, a.out16, acc[i][j]);
         } else if constexpr (EPI == DGATED) {
           const char* block = static_cast<const char*>(a.saved) + ((qt >> 5) * a.saved_cols + (p >> 5)) * SAVED_BLOCK;
           float m[16];
@@ -424,19 +411,19 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
           Saved::get(block, m);
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[r] = acc[i][j][r] * m[r];
-          store_tile<T, AL>(row, p, np, ok, o);
+          store_tile<T>(row, p, np, ok, a.out16, o);
           Saved::get(block + SAVED_BLOCK / 2, m);
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[r] = acc[i][j][r] * m[r];
-          store_tile<T, AL>(row + np, p, np, ok, o);
+          store_tile<T>(row + np, p, np, ok, a.out16, o);
         } else {
           float* row = static_cast<float*>(a.out) + ((int64_t)split * a.q.size + q) * a.ldo;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int64_t pp = p + 8 * g + 4 * (lane >> 5);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (ok && pp + r < np) row[pp + r] = acc[i][j][4 * g + r];
+            if (ok && pp < np)   // ldo is np rounded up to a multiple of 4
+              *reinterpret_cast<float4*>(row + pp) =
+                  make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
           }
         }
       }
@@ -444,18 +431,157 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
   }
 }
 
-// out = round(sum of the splits' products, in order)
+// out [nq][ldo] = round(sum of the splits' products [nq][ldp], in order), four columns per lane
 template <typename T>
-__global__ __launch_bounds__(256) void k_split_sum(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ out) {
-  for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n; i += 4 * (int64_t)gridDim.x * 256) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int left = (int)min((int64_t)4, n - i);
-    for (int s = 0; s < splits; ++s)
+__global__ __launch_bounds__(256) void k_split_sum(const float* __restrict__ part, int splits, int64_t nq, int64_t np, int64_t ldp,
+                                                   T* __restrict__ out, int64_t ldo, bool al) {
+  const int64_t per = ldp / 4, all = nq * per, step = nq * ldp;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t q = i / per, p = 4 * (i - q * per);
+    const float* src = part + q * ldp + p;
+    float4 acc = *reinterpret_cast<const float4*>(src);
+    int s = 1;
+    for (; s + 4 <= splits; s += 4) {   // four splits' loads in flight
+      float4 e[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += k < left ? part[s * n + i + k] : 0.f;
+      for (int u = 0; u < 4; ++u) e[u] = *reinterpret_cast<const float4*>(src + (s + u) * step);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < left) st1(out + i + k, acc[k]);
+      for (int u = 0; u < 4; ++u) acc = make_float4(acc.x + e[u].x, acc.y + e[u].y, acc.z + e[u].z, acc.w + e[u].w);
+    }
+    for (; s < splits; ++s) {
+      const float4 e = *reinterpret_cast<const float4*>(src + s * step);
+      acc = make_float4(acc.x + e.x, acc.y + e.y, acc.z + e.z, acc.w + e.w);
+    }
+    T* o = out + q * ldo + p;
+    const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+    if (al && p + 4 <= np) {
+      typedef typename CvtOf<T>::type Cvt;
+      *reinterpret_cast<uint2*>(o) = make_uint2(Cvt::pack2(v[0], v[1]), Cvt::pack2(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (p + k < np) st1(o + k, v[k]);
+    }
+  }
+}
+
+// out [rows][ld] = x [rows][cols], zeros past the columns, for operands whose rows are not aligned; eight columns per lane
+template <typename T>
+__global__ __launch_bounds__(256) void k_pad_rows(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ld,
+                                                  T* __restrict__ out) {
+  const int64_t per = ld / 8, all = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per, c = 8 * (i - r * per);
+    const T* src = x + r * cols + c;
+    uint4 v;
+    if (c + 8 <= cols) {
+      v = UIO<T>::raw(src).u;
+    } else {
+      struct { T e[8]; } e;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e.e[k] = c + k < cols ? src[k] : (T)0;
+      v = __builtin_bit_cast(uint4, e);
+    }
+    *reinterpret_cast<uint4*>(out + r * ld + c) = v;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// few tokens (a serving step): y = x W^T, or the gated pair, for up to 16 MT tokens. The weights' stream bounds it, so they go
+// from memory to the matrix cores' registers (v_mfma_f32_16x16x32: lane l has row l mod 16): a workgroup takes 16 rows (of the
+// gate's and of the up projection's), its waves the columns in turns of 128, each lane 32 consecutive ones of its row (64
+// bytes), all rows' loads of a turn in flight together. The order of k is the same permutation for both operands. The waves'
+// sums meet in LDS, in order. Any alignment.
+// ---------------------------------------------------------------------------------------------------------------
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma16(bf16_t, uint4 a, uint4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(_Float16, uint4 a, uint4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <typename T, int MT, int PAIR, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
+                                                           T* __restrict__ y, int64_t ldy, int t, int64_t n, int64_t k, int act) {
+  __shared__ f32x4 s_acc[WAVES][PAIR][MT][64];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, r = lane & 15, quad = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, row = min(n0 + r, n - 1);
+  const T* wp[PAIR];
+  const T* xp[MT];
+#pragma unroll
+  for (int g = 0; g < PAIR; ++g) wp[g] = w + (g * n + row) * ldw + 32 * quad;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xp[m] = x + (int64_t)min(16 * m + r, t - 1) * ldx + 32 * quad;
+  f32x4 acc[PAIR][MT];
+#pragma unroll
+  for (int g = 0; g < PAIR; ++g)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[g][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t whole = k / 128;
+#pragma unroll MT > 2 ? 1 : 2
+  for (int64_t c = wave; c < whole; c += WAVES) {
+    uint4 wf[PAIR][4], xf[MT][4];
+#pragma unroll
+    for (int g = 0; g < PAIR; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_u16*>(wp[g] + 128 * c + 8 * j));
+        wf[g][j] = make_uint4(v.x, v.y, v.z, v.w);
+      }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) xf[m][j] = UIO<T>::raw(xp[m] + 128 * c + 8 * j).u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int g = 0; g < PAIR; ++g)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[g][m] = mfma16(T{}, wf[g][j], xf[m][j], acc[g][m]);
+  }
+  if (k % 128 && whole % WAVES == wave) {   // the last columns, zeros past them
+    auto piece = [&](const T* p, int64_t c) {
+      if (c + 8 <= k) return UIO<T>::raw(p + c - 32 * quad).u;
+      struct { T e[8]; } e;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e.e[i] = c + i < k ? p[c - 32 * quad + i] : (T)0;
+      return __builtin_bit_cast(uint4, e);
+    };
+    for (int j = 0; j < 4; ++j) {
+      const int64_t c = 128 * whole + 32 * quad + 8 * j;
+      uint4 wf[PAIR], xf[MT];
+#pragma unroll
+      for (int g = 0; g < PAIR; ++g) wf[g] = piece(wp[g], c);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) xf[m] = piece(xp[m], c);
+#pragma unroll
+      for (int g = 0; g < PAIR; ++g)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[g][m] = mfma16(T{}, wf[g], xf[m], acc[g][m]);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < PAIR; ++g)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) s_acc[wave][g][m][lane] = acc[g][m];
+  __syncthreads();
+  // element e of a 16 x 16 result: row e / 16 of the weights (register e / 16 mod 4 of lane 16 (e / 64) + token)
+  for (int i = (int)threadIdx.x; i < 256 * MT; i += 64 * WAVES) {
+    const int m = i >> 8, token = (i >> 4) & 15, rr = i & 15, from = 16 * (rr >> 2) + token;
+    float v[PAIR];
+#pragma unroll
+    for (int g = 0; g < PAIR; ++g) {
+      v[g] = 0.f;
+      for (int q = 0; q < WAVES; ++q) v[g] += s_acc[q][g][m][from][rr & 3];
+    }
+    float o = v[0];
+    if constexpr (PAIR == 2) {
+      float da;
+      activation(v[0], act, o, da);
+      o *= v[1];
+    }
+    if (16 * m + token < t && n0 + rr < n) st1(y + (int64_t)(16 * m + token) * ldy + n0 + rr, o);
   }
 }
 
@@ -465,148 +591,213 @@ __global__ __launch_bounds__(256) void k_split_sum(const float* __restrict__ par
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool al2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 inline int launched() { return (int)hipGetLastError(); }
+inline unsigned grid_of(int64_t n, int64_t cap) { return (unsigned)((n + 255) / 256 < cap ? (n + 255) / 256 : cap); }
 constexpr int64_t MAX_SIZE = 0x7fffffff;   // of one dimension
+constexpr int64_t MAX_LD = 1 << 22;        // rows of memory up to which a tile's byte offsets fit 32 bits (256 rows)
 
-template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, int BK, Epi EPI, bool AL>
-int launch_tiles(Product a, hipStream_t st) {
-  a.run = (a.run + BK - 1) / BK * BK;
-  constexpr int TP = (EPI == GATED ? WP * FP * 16 : WP * FP * 32), TQ = WQ * FQ * 32;
+template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI> int launch_tiles(Product a, hipStream_t st) {
+  constexpr int BK = 64, TP = (EPI == GATED ? WP * FP * 16 : WP * FP * 32), TQ = WQ * FQ * 32;
   const int64_t np = EPI == GATED ? a.p.half : a.p.size;
   const int64_t tp = (np + TP - 1) / TP, tq = (a.q.size + TQ - 1) / TQ, tiles = tp * tq;
   if (tiles * a.splits > 0xfffffff) return LDR_E_SHAPE;
   a.tiles_p = (int)tp;
   a.tiles = (int)tiles;
   a.per = (int)((tiles * a.splits + 7) / 8);
-  hipLaunchKernelGGL((k_product<T, KP, KQ, WP, WQ, FP, FQ, BK, EPI, AL>), dim3((unsigned)(8 * a.per)), dim3(WP * WQ * 64), 0, st, a);
+  hipLaunchKernelGGL((k_product<T, KP, KQ, WP, WQ, FP, FQ, BK, EPI>), dim3((unsigned)(8 * a.per)), dim3(WP * WQ * 64), 0, st, a);
   return launched();
 }
 
-// 256 x 256 tiles by eight waves where they give every CU one; 128 x 128 by four waves else
-constexpr int64_t CUS = 256;
-constexpr int64_t MAX_LD = (1 << 22);   // rows of memory up to which a tile's byte offsets fit 32 bits (256 rows)
-inline int64_t tiles_of(int64_t np, int64_t nq, int64_t t) { return ((np + t - 1) / t) * ((nq + t - 1) / t); }
+// Which tiles, and in how many splits of k, by the time they take: 256 x 256 ones of eight waves, one to a CU, 1.65 us per 64
+// k; 128 x 128 ones of four waves, two to a CU, 1.08 us (8192 x 2048 x 5632: 157-390 us against 173-470 for the six
+// products); 5 us around them; splits are written and read as fp32 (2 us for the launch that adds them).
+struct Tiling { bool big; int splits; };
+inline Tiling tiling_of(int64_t np, int64_t nq, int64_t k, bool may_split) {
+  constexpr int64_t CUS = 256;
+  Tiling best{false, 1};
+  double least = 1e30;
+  for (int big = 0; big < 2; ++big) {
+    const int64_t t = big ? 256 : 128, tiles = ((np + t - 1) / t) * ((nq + t - 1) / t), at_once = big ? CUS : 2 * CUS;
+    const int64_t ks = (k + 63) / 64, most = may_split ? (ks / 4 < 32 ? ks / 4 : 32) : 1;
+    for (int64_t s = 1; s <= (most < 1 ? 1 : most); ++s) {
+      const int64_t rounds = (tiles * s + at_once - 1) / at_once, each = (ks + s - 1) / s;
+      const double one = big ? 1.65 : tiles * s <= CUS ? 0.75 : 1.08;
+      const double us = rounds * (each * one + 5.0) + (s > 1 ? 2.0 + (double)s * np * nq * 8 / 4e6 : 0.0);
+      if (us < least) least = us, best = Tiling{big != 0, (int)s};
+    }
+  }
+  return best;
+}
+inline int64_t scratch_ld(int64_t np) { return (np + 3) / 4 * 4; }
 
-template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, bool al, hipStream_t st) {
-  al = al && a.p.ld <= MAX_LD && a.q.ld <= MAX_LD;
-  if (!al) return launch_tiles<T, KP, KQ, 2, 2, 2, 2, 64, EPI, false>(a, st);
-#ifdef FFN_EXP
-  static const int cfg = getenv("FFN_CFG") ? atoi(getenv("FFN_CFG")) : 0;
-  if (cfg == 1) return launch_tiles<T, KP, KQ, 4, 2, 2, 4, 64, EPI, true>(a, st);
-  if (cfg == 2) return launch_tiles<T, KP, KQ, 2, 2, 2, 2, 64, EPI, true>(a, st);
-#endif
-  const int64_t np = a.p.half ? 2 * a.p.half : a.p.size;
-  if (tiles_of(np, a.q.size, 256) * a.splits >= CUS / 2) return launch_tiles<T, KP, KQ, 4, 2, 2, 4, 64, EPI, true>(a, st);
-  return launch_tiles<T, KP, KQ, 2, 2, 2, 2, 64, EPI, true>(a, st);
+template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, bool big, hipStream_t st) {
+  return big ? launch_tiles<T, KP, KQ, 4, 2, 2, 4, EPI>(a, st) : launch_tiles<T, KP, KQ, 2, 2, 2, 2, EPI>(a, st);
+}
+template <typename T, Kind KP, Kind KQ> int plain_product(Product a, float* scratch, hipStream_t st) {
+  const int64_t np = a.p.size, nq = a.q.size;
+  const Tiling tl = tiling_of(np, nq, a.k, true);
+  const bool al = np % 8 == 0 && a.ldo % 8 == 0 && al16(a.out);
+  if (tl.splits == 1) {
+    a.out16 = al;
+    return launch_product<T, KP, KQ, STORE>(a, tl.big, st);
+  }
+  if (!scratch) return LDR_E_ARG;
+  void* const out = a.out;
+  const int64_t ldo = a.ldo, ldp = scratch_ld(np);
+  a.run = ((a.k + tl.splits - 1) / tl.splits + 63) / 64 * 64;
+  a.splits = (int)((a.k + a.run - 1) / a.run);
+  a.out = scratch;
+  a.ldo = ldp;
+  const int e = launch_product<T, KP, KQ, PARTIAL>(a, tl.big, st);
+  if (e) return e;
+  hipLaunchKernelGGL(k_split_sum<T>, dim3(grid_of(nq * ldp / 4, 4096)), dim3(256), 0, st, scratch, a.splits, nq, np, ldp,
+                     static_cast<T*>(out), ldo, al);
+  return launched();
+}
+
+template <typename T, int MT, int PAIR>
+int few(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t ldy, int64_t t, int64_t n, int64_t k, int act,
+        hipStream_t st) {
+  const int64_t blocks = (n + 15) / 16;
+  if (blocks > MAX_SIZE) return LDR_E_SHAPE;
+#define FEW(W) hipLaunchKernelGGL((k_few_tokens<T, MT, PAIR, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, static_cast<const T*>(x), \
+                                  ldx, static_cast<const T*>(w), ldw, static_cast<T*>(y), ldy, (int)t, n, k, act)
+  if (blocks >= 512) FEW(4);   // waves for every CU to have some eight
+  else FEW(8);
+#undef FEW
+  return launched();
+}
+template <typename T, int PAIR>
+int few_tokens(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t ldy, int64_t t, int64_t n, int64_t k, int act,
+               hipStream_t st) {
+  if (t <= 16) return few<T, 1, PAIR>(x, ldx, w, ldw, y, ldy, t, n, k, act, st);
+  if (t <= 32) return few<T, 2, PAIR>(x, ldx, w, ldw, y, ldy, t, n, k, act, st);
+  return few<T, 4, PAIR>(x, ldx, w, ldw, y, ldy, t, n, k, act, st);
 }
 
 #define FFN_TYPE_SWITCH(DT, ...)                                 \
   if ((DT) == LDR_BF16) { typedef bf16_t T; __VA_ARGS__; }       \
   else { typedef _Float16 T; __VA_ARGS__; }
 
-inline int sizes(int64_t a, int64_t b, int64_t c, int dtype) {
+// sizes of a product with t tokens: dtype, dimensions, and the rows' lengths
+inline int sizes(int64_t t, int64_t a, int64_t b, int dtype) {
   if (dtype != LDR_BF16 && dtype != LDR_F16) return LDR_E_DTYPE;
-  if (a < 0 || b < 1 || c < 1) return LDR_E_ARG;
-  return a > MAX_SIZE || b > MAX_SIZE || c > MAX_SIZE ? LDR_E_SHAPE : LDR_OK;
+  if (t < 0 || a < 1 || b < 1) return LDR_E_ARG;
+  return t > MAX_SIZE || a > MAX_SIZE || b > MAX_SIZE ? LDR_E_SHAPE : LDR_OK;
+}
+// an operand of the tiled kernels: rows of `cols` elements, ld apart
+inline int operand(const void* p, int64_t cols, int64_t ld) {
+  if (!p) return LDR_E_ARG;
+  if (ld < cols || ld > MAX_LD) return LDR_E_SHAPE;
+  return ld % 8 || !al16(p) ? LDR_E_ALIGN : LDR_OK;
 }
 inline Product product(Operand p, Operand q, int64_t k, void* out, int64_t ldo) {
-  return Product{p, q, k, k, out, ldo, nullptr, 0, 0, 0, 1, 0, 0};
+  Product a{};
+  a.p = p, a.q = q, a.k = a.run = k, a.out = out, a.ldo = ldo, a.splits = 1;
+  return a;
 }
 
 }  // namespace
 
 extern "C" {
 
+int lbk_pad_rows(const void* x, int64_t rows, int64_t cols, int64_t ld, void* out, int dtype, void* stream) {
+  const int e = sizes(rows, cols, ld, dtype);
+  if (e || rows == 0) return e;
+  if (!x || !out) return LDR_E_ARG;
+  if (ld < cols) return LDR_E_SHAPE;
+  if (ld % 8 || !al16(out) || !al2(x)) return LDR_E_ALIGN;
+  FFN_TYPE_SWITCH(dtype, hipLaunchKernelGGL(k_pad_rows<T>, dim3(grid_of(rows * (ld / 8), 8192)), dim3(256), 0,
+                                            static_cast<hipStream_t>(stream), static_cast<const T*>(x), rows, cols, ld,
+                                            static_cast<T*>(out)))
+  return launched();
+}
+
 int64_t lbk_ffn_saved_bytes(int64_t t, int64_t n) {
   return t < 1 || n < 1 ? 0 : ((t + 31) / 32) * ((n + 31) / 32) * SAVED_BLOCK;
 }
 
-int lbk_ffn_gate_up(const void* x, const void* w, void* act, void* saved, int64_t t, int64_t d, int64_t n, int activation,
-                    int dtype, void* stream) {
-  const int e = sizes(t, d, n, dtype);
+int lbk_ffn_gate_up(const void* x, int64_t ldx, const void* w, int64_t ldw, void* act, int64_t ld_act, void* saved, int64_t t,
+                    int64_t d, int64_t n, int activation, int dtype, void* stream) {
+  int e = sizes(t, d, n, dtype);
   if (e) return e;
-  if (activation != 0 && activation != 1) return LDR_E_ARG;
+  if ((activation != 0 && activation != 1) || ld_act < n) return LDR_E_ARG;
   if (t == 0) return LDR_OK;
   if (!x || !w || !act) return LDR_E_ARG;
   if (!al2(x) || !al2(w) || !al2(act) || !al16(saved)) return LDR_E_ALIGN;
-  const bool al = d % 8 == 0 && n % 8 == 0 && al16(x) && al16(w) && al16(act);
-  Product a = product({w, d, 2 * n, n}, {x, d, t, 0}, d, act, n);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (t <= LBK_FEW_TOKENS && !saved) {
+    if (ldx < d || ldw < d) return LDR_E_SHAPE;
+    FFN_TYPE_SWITCH(dtype, return (few_tokens<T, 2>(x, ldx, w, ldw, act, ld_act, t, n, d, activation, st)))
+  }
+  if ((e = operand(x, d, ldx)) || (e = operand(w, d, ldw))) return e;
+  Product a = product({w, ldw, 2 * n, n}, {x, ldx, t, 0}, d, act, ld_act);
+  a.out16 = ld_act % 8 == 0 && al16(act);
   a.saved = saved;
   a.saved_cols = (n + 31) / 32;
   a.act = activation;
-  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, GATED>(a, al, static_cast<hipStream_t>(stream))))
+  const bool big = tiling_of(2 * n, t, d, false).big;
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, GATED>(a, big, st)))
 }
 
-int lbk_ffn_dgate_up(const void* dy, const void* w_down, const void* saved, void* dgate_up, int64_t t, int64_t n, int64_t d,
-                     int dtype, void* stream) {
-  const int e = sizes(t, d, n, dtype);
+int lbk_ffn_dgate_up(const void* dy, int64_t ld_dy, const void* w_down, int64_t ldw, const void* saved, void* dgate_up, int64_t ld_dgu,
+                     int64_t t, int64_t n, int64_t d, int dtype, void* stream) {
+  int e = sizes(t, d, n, dtype);
   if (e) return e;
+  if (ld_dgu < 2 * n) return LDR_E_ARG;
   if (t == 0) return LDR_OK;
-  if (!dy || !w_down || !saved || !dgate_up) return LDR_E_ARG;
-  if (!al2(dy) || !al2(w_down) || !al2(dgate_up) || !al16(saved)) return LDR_E_ALIGN;
-  const bool al = d % 8 == 0 && n % 8 == 0 && al16(dy) && al16(w_down) && al16(dgate_up);
-  Product a = product({w_down, n, n, 0}, {dy, d, t, 0}, d, dgate_up, 2 * n);
+  if (!saved || !dgate_up) return LDR_E_ARG;
+  if (!al2(dgate_up) || !al16(saved)) return LDR_E_ALIGN;
+  if ((e = operand(dy, d, ld_dy)) || (e = operand(w_down, n, ldw))) return e;
+  Product a = product({w_down, ldw, n, 0}, {dy, ld_dy, t, 0}, d, dgate_up, ld_dgu);
+  a.out16 = n % 8 == 0 && ld_dgu % 8 == 0 && al16(dgate_up);
   a.saved = const_cast<void*>(saved);
   a.saved_cols = (n + 31) / 32;
-  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, DGATED>(a, al, static_cast<hipStream_t>(stream))))
+  const bool big = tiling_of(n, t, d, false).big;
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, DGATED>(a, big, static_cast<hipStream_t>(stream))))
 }
 
-int lbk_linear_fwd(const void* x, const void* w, void* y, int64_t t, int64_t k, int64_t n, int dtype, void* stream) {
-  const int e = sizes(t, k, n, dtype);
+int64_t lbk_linear_scratch(int64_t np, int64_t nq, int64_t k) {
+  if (np < 1 || nq < 1 || k < 1) return 0;
+  const Tiling tl = tiling_of(np, nq, k, true);
+  return tl.splits > 1 ? tl.splits * nq * scratch_ld(np) : 0;
+}
+
+int lbk_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t ldy, float* scratch, int64_t t, int64_t k,
+                   int64_t n, int dtype, void* stream) {
+  int e = sizes(t, k, n, dtype);
   if (e || t == 0) return e;
-  if (!x || !w || !y) return LDR_E_ARG;
-  if (!al2(x) || !al2(w) || !al2(y)) return LDR_E_ALIGN;
-  const bool al = k % 8 == 0 && n % 8 == 0 && al16(x) && al16(w) && al16(y);
-  const Product a = product({w, k, n, 0}, {x, k, t, 0}, k, y, n);
-  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, STORE>(a, al, static_cast<hipStream_t>(stream))))
-}
-
-int lbk_linear_dx(const void* dy, const void* w, void* dx, int64_t t, int64_t n, int64_t k, int dtype, void* stream) {
-  const int e = sizes(t, k, n, dtype);
-  if (e || t == 0) return e;
-  if (!dy || !w || !dx) return LDR_E_ARG;
-  if (!al2(dy) || !al2(w) || !al2(dx)) return LDR_E_ALIGN;
-  const bool al = k % 8 == 0 && n % 8 == 0 && al16(dy) && al16(w) && al16(dx);
-  const Product a = product({w, k, k, 0}, {dy, n, t, 0}, n, dx, k);
-  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, STORE>(a, al, static_cast<hipStream_t>(stream))))
-}
-
-static int64_t dw_splits(int64_t t, int64_t n, int64_t k) {
-  const int64_t tiles = tiles_of(n, k, 256), fill = CUS / tiles, most = t / 512;
-  const int64_t s = fill < most ? fill : most;
-  return s < 1 ? 1 : s;
-}
-
-int64_t lbk_linear_dw_scratch(int64_t t, int64_t n, int64_t k) {
-  if (t < 1 || n < 1 || k < 1) return 0;
-  const int64_t s = dw_splits(t, n, k);
-  return s > 1 ? s * n * k : 0;
-}
-
-int lbk_linear_dw(const void* dy, const void* x, float* scratch, void* dw, int64_t t, int64_t n, int64_t k, int dtype,
-                  void* stream) {
-  const int e = sizes(t, k, n, dtype);
-  if (e) return e;
-  if (!dw || (t > 0 && (!dy || !x))) return LDR_E_ARG;
-  if (!al2(dy) || !al2(x) || !al2(dw) || !al16(scratch)) return LDR_E_ALIGN;
+  if (!x || !w || !y || ldy < n) return LDR_E_ARG;
+  if (!al2(x) || !al2(w) || !al2(y) || !al16(scratch)) return LDR_E_ALIGN;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t splits = t < 1 ? 1 : dw_splits(t, n, k);
-  if (splits > 1 && !scratch) return LDR_E_ARG;
-  const bool al = k % 8 == 0 && n % 8 == 0 && al16(dy) && al16(x) && al16(dw);
-  Product a = product({x, k, k, 0}, {dy, n, n, 0}, t, dw, k);
-  if (splits == 1) {
-    FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, COL, STORE>(a, al, st)))
+  if (t <= LBK_FEW_TOKENS) {
+    if (ldx < k || ldw < k) return LDR_E_SHAPE;
+    FFN_TYPE_SWITCH(dtype, return (few_tokens<T, 1>(x, ldx, w, ldw, y, ldy, t, n, k, 0, st)))
   }
-  a.run = ((t + splits - 1) / splits + 63) / 64 * 64;
-  a.splits = (int)((t + a.run - 1) / a.run);
-  a.out = scratch;
-  FFN_TYPE_SWITCH(dtype, {
-    const int err = launch_product<T, COL, COL, PARTIAL>(a, al, st);
-    if (err) return err;
-    const int64_t blocks = (n * k / 4 + 255) / 256 + 1;
-    hipLaunchKernelGGL(k_split_sum<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, scratch, a.splits,
-                       n * k, static_cast<T*>(dw));
-  })
-  return launched();
+  if ((e = operand(x, k, ldx)) || (e = operand(w, k, ldw))) return e;
+  const Product a = product({w, ldw, n, 0}, {x, ldx, t, 0}, k, y, ldy);
+  FFN_TYPE_SWITCH(dtype, return (plain_product<T, ROW, ROW>(a, scratch, st)))
+}
+
+int lbk_linear_dx(const void* dy, int64_t ld_dy, const void* w, int64_t ldw, void* dx, int64_t ld_dx, float* scratch, int64_t t, int64_t n,
+                  int64_t k, int dtype, void* stream) {
+  int e = sizes(t, k, n, dtype);
+  if (e || t == 0) return e;
+  if (!dx || ld_dx < k) return LDR_E_ARG;
+  if (!al2(dx) || !al16(scratch)) return LDR_E_ALIGN;
+  if ((e = operand(dy, n, ld_dy)) || (e = operand(w, k, ldw))) return e;
+  const Product a = product({w, ldw, k, 0}, {dy, ld_dy, t, 0}, n, dx, ld_dx);
+  FFN_TYPE_SWITCH(dtype, return (plain_product<T, COL, ROW>(a, scratch, static_cast<hipStream_t>(stream))))
+}
+
+int lbk_linear_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ldx, float* scratch, void* dw, int64_t t, int64_t n, int64_t k,
+                  int dtype, void* stream) {
+  int e = sizes(t, k, n, dtype);
+  if (e) return e;
+  if (!dw || t < 1) return LDR_E_ARG;
+  if (!al2(dw) || !al16(scratch)) return LDR_E_ALIGN;
+  if ((e = operand(dy, n, ld_dy)) || (e = operand(x, k, ldx))) return e;
+  const Product a = product({x, ldx, k, 0}, {dy, ld_dy, n, 0}, t, dw, k);
+  FFN_TYPE_SWITCH(dtype, return (plain_product<T, COL, COL>(a, scratch, static_cast<hipStream_t>(stream))))
 }
 
 }  // extern "C"

@@ -36,7 +36,8 @@ FAMILIES = [("k_read_fwd", "read_fwd"), ("k_read_online", "read_fwd_online"), ("
             ("k_mean", "next_token_loss_fwd"), ("k_next_token_bwd", "next_token_loss_bwd"), ("k_rotary", "rotary"),
             ("k_attn_fwd", "attn_fwd"), ("k_attn_bwd", "attn_bwd"), ("k_wgrad", "wgrad"),
             # a block's feed-forward products, join and dropout
-            ("k_product", "ffn_product"), ("k_split_sum", "ffn_product"),
+            ("k_product", "ffn_product"), ("k_split_sum", "ffn_product"), ("k_few_tokens", "ffn_product"),
+            ("k_pad_rows", "ffn_product"),
             ("k_join_fwd", "join_fwd"), ("k_join_bwd", "join_bwd"), ("k_join_sum", "join_bwd"), ("k_dropout", "dropout")]
 COPY_BYTES = 1 << 30   # bench.py --copy-calibration copies 1 GiB
 

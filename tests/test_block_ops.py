@@ -24,6 +24,7 @@ def test_library():
     assert names == set(ops.SIGNATURES) and all(hasattr(ops.LIB, n) for n in names)
     define = lambda n: int(re.search(rf"#define {n} (\d+)", text).group(1))
     assert define("LBK_ABI_VERSION") == ops.ABI_VERSION and define("LBK_JOIN_MAX_WIDTH") == ops.JOIN_MAX_WIDTH
+    assert define("LBK_FEW_TOKENS") == ops.FEW_TOKENS
 
 
 def test_row_kernels_refuse():
@@ -49,20 +50,30 @@ def test_row_kernels_refuse():
 
 def test_products_refuse():
     L, p, null = ops.LIB, 4096, None
-    up = lambda x=p, w=p, act=p, saved=p, t=4, d=8, n=8, a=0, dt=1: L.lbk_ffn_gate_up(x, w, act, saved, t, d, n, a, dt, null)
+    up = lambda x=p, w=p, act=p, saved=p, t=100, d=8, n=8, a=0, dt=1, ldx=8, ldw=8, ld=8: L.lbk_ffn_gate_up(
+        x, ldx, w, ldw, act, ld, saved, t, d, n, a, dt, null)
     assert up(dt=0) == -4 and up(dt=3) == -4 and up(t=-1) == -1 and up(d=0) == -1 and up(n=0) == -1 and up(a=2) == -1
     assert up(x=null) == -1 and up(w=null) == -1 and up(act=null) == -1 and up(x=4097) == -3 and up(saved=4098) == -3
-    assert up(t=2 ** 31) == -2 and up(d=2 ** 31) == -2 and up(n=2 ** 31) == -2 and up(t=0, x=null) == 0
-    dn = lambda dy=p, w=p, saved=p, out=p, t=4, dt=2: L.lbk_ffn_dgate_up(dy, w, saved, out, t, 8, 8, dt, null)
+    assert up(t=2 ** 31) == -2 and up(d=2 ** 31) == -2 and up(n=2 ** 31, ld=2 ** 31) == -2 and up(t=0, x=null) == 0
+    assert up(x=4098) == -3 and up(ldx=12) == -3 and up(ldw=7) == -2 and up(ldw=2 ** 23) == -2 and up(ld=7) == -1
+    assert up(t=4, saved=null, ldx=7) == -2 and up(t=4, x=4097, saved=null) == -3
+    dn = lambda dy=p, w=p, saved=p, out=p, t=4, dt=2, lw=8, lo=16: L.lbk_ffn_dgate_up(dy, 8, w, lw, saved, out, lo, t, 8, 8, dt, null)
     assert dn(dt=0) == -4 and dn(dy=null) == -1 and dn(w=null) == -1 and dn(saved=null) == -1 and dn(out=null) == -1
-    assert dn(saved=4098) == -3 and dn(out=4097) == -3 and dn(t=0) == 0
+    assert dn(saved=4098) == -3 and dn(out=4097) == -3 and dn(t=0) == 0 and dn(lw=9) == -3 and dn(lo=15) == -1 and dn(w=4098) == -3
     for fn in (L.lbk_linear_fwd, L.lbk_linear_dx):
-        assert fn(p, p, p, 4, 8, 8, 0, null) == -4 and fn(null, p, p, 4, 8, 8, 1, null) == -1
-        assert fn(p, p, 4097, 4, 8, 8, 1, null) == -3 and fn(p, p, p, 4, 0, 8, 1, null) == -1 and fn(p, p, p, 0, 8, 8, 1, null) == 0
-    dw = lambda dy=p, s=p, out=p, t=4: L.lbk_linear_dw(dy, p, s, out, t, 8, 8, 1, null)
+        call = lambda x=p, w=p, y=p, t=100, k=8, ld=8, dt=1, s=null: fn(x, ld, w, 8, y, 8, s, t, k, 8, dt, null)
+        assert call(dt=0) == -4 and call(x=null) == -1 and call(w=null) == -1 and call(y=null) == -1 and call(y=4097) == -3
+        assert call(k=0) == -1 and call(t=0) == 0 and call(t=-1) == -1 and call(ld=12) == -3 and call(x=4098) == -3 and call(s=4100) == -3
+    assert L.lbk_linear_fwd(p, 7, p, 8, p, 8, null, 4, 8, 8, 1, null) == -2
+    dw = lambda dy=p, s=p, out=p, t=4: L.lbk_linear_dw(dy, 8, p, 8, s, out, t, 8, 8, 1, null)
     assert dw(dy=null) == -1 and dw(out=null) == -1 and dw(s=null, t=1 << 20) == -1 and dw(s=4100) == -3 and dw(t=-1) == -1
-    assert L.lbk_linear_dw_scratch(0, 8, 8) == 0 and L.lbk_linear_dw_scratch(100, 768, 768) == 0
-    assert L.lbk_linear_dw_scratch(1 << 20, 8, 8) > 0 and L.lbk_ffn_saved_bytes(33, 1) == 2 * 6144
+    assert dw(t=0) == -1
+    pad = lambda x=p, out=p, rows=4, cols=7, ld=8, dt=1: L.lbk_pad_rows(x, rows, cols, ld, out, dt, null)
+    assert pad(x=null) == -1 and pad(out=null) == -1 and pad(rows=0) == 0 and pad(ld=6) == -2 and pad(ld=9) == -3 and pad(dt=0) == -4
+    assert pad(out=4098) == -3 and pad(x=4097) == -3
+    assert L.lbk_linear_scratch(0, 8, 8) == 0 and L.lbk_linear_scratch(8192, 8192, 8192) == 0
+    assert L.lbk_linear_scratch(8, 9, 1 << 20) % (8 * 9) == 0 and L.lbk_linear_scratch(8, 9, 1 << 20) > 72
+    assert L.lbk_ffn_saved_bytes(33, 1) == 2 * 6144
 
 
 def test_ffn_form():
@@ -175,5 +186,5 @@ def test_every_kernel_has_a_family():
     for src in ("loopback_block.hip", "loopback_ffn.hip"):
         with open(os.path.join(ROOT, "loopback_amd", "csrc", src)) as f:
             names |= set(re.findall(r"__global__[^;{]*?\bvoid\s+(k_\w+)\s*\(", f.read(), flags=re.S))
-    assert {"k_dropout", "k_join_fwd", "k_join_bwd", "k_join_sum", "k_product", "k_split_sum"} <= names
+    assert {"k_dropout", "k_join_fwd", "k_join_bwd", "k_join_sum", "k_product", "k_split_sum", "k_few_tokens", "k_pad_rows"} <= names
     assert all(RS.family(f"void (anonymous namespace)::{n}<float, 1>(...)") != "torch / runtime" for n in names)
