@@ -58,7 +58,7 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* h, const void* y, c
  * 16-byte aligned with ld a multiple of 8, all ld elements of a row readable -- lbk_pad_rows makes such a copy of one that
  * is not -- or, for up to LBK_FEW_TOKENS tokens of lbk_linear_fwd, and of lbk_ffn_gate_up without `saved`, of any alignment.
  * Results may have any. */
-#define LBK_FEW_TOKENS 64
+#define LBK_FEW_TOKENS 32
 
 /* out [rows, ld] = x [rows, cols], contiguous, with zeros past the columns. */
 int lbk_pad_rows(const void* x, int64_t rows, int64_t cols, int64_t ld, void* out, int dtype, void* stream);

@@ -29,7 +29,7 @@ from .lm_ops import _again, _launchable, _stream, _watched, native
 
 ABI_VERSION = 1
 JOIN_MAX_WIDTH = 8192
-FEW_TOKENS = 64
+FEW_TOKENS = 32
 FFN_MAX_WIDTH = 2 ** 22 - 8   # elements between rows of the tiled products' operands
 MAX_ROWS = 2 ** 31 - 1
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}

@@ -489,9 +489,8 @@ __global__ __launch_bounds__(256) void k_pad_rows(const T* __restrict__ x, int64
 // ---------------------------------------------------------------------------------------------------------------
 // few tokens (a serving step): y = x W^T, or the gated pair, for up to 16 MT tokens. The weights' stream bounds it, so they go
 // from memory to the matrix cores' registers (v_mfma_f32_16x16x32: lane l has row l mod 16): a workgroup takes 16 rows (of the
-// gate's and of the up projection's), its waves the columns in turns of 128, each lane 32 consecutive ones of its row (64
-// bytes), all rows' loads of a turn in flight together. The order of k is the same permutation for both operands. The waves'
-// sums meet in LDS, in order. Any alignment.
+// gate's and of the up projection's), its waves the columns in turns of 128, each load instruction 64 consecutive bytes of 16
+// rows, all loads of a few turns in flight together. The waves' sums meet in LDS, in order. Any alignment.
 // ---------------------------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 mfma16(bf16_t, uint4 a, uint4 b, f32x4 c) {
@@ -501,7 +500,7 @@ __device__ __forceinline__ f32x4 mfma16(_Float16, uint4 a, uint4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <typename T, int MT, int PAIR, int WAVES>
+template <typename T, int MT, int PAIR, int WAVES, int U>
 __global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
                                                            T* __restrict__ y, int64_t ldy, int t, int64_t n, int64_t k, int act) {
   __shared__ f32x4 s_acc[WAVES][PAIR][MT][64];
@@ -510,46 +509,58 @@ __global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T* __restrict__
   const T* wp[PAIR];
   const T* xp[MT];
 #pragma unroll
-  for (int g = 0; g < PAIR; ++g) wp[g] = w + (g * n + row) * ldw + 32 * quad;
+  for (int g = 0; g < PAIR; ++g) wp[g] = w + (g * n + row) * ldw + 8 * quad;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xp[m] = x + (int64_t)min(16 * m + r, t - 1) * ldx + 32 * quad;
+  for (int m = 0; m < MT; ++m) xp[m] = x + (int64_t)min(16 * m + r, t - 1) * ldx + 8 * quad;
   f32x4 acc[PAIR][MT];
 #pragma unroll
   for (int g = 0; g < PAIR; ++g)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[g][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int64_t whole = k / 128;
-#pragma unroll MT > 2 ? 1 : 2
-  for (int64_t c = wave; c < whole; c += WAVES) {
-    uint4 wf[PAIR][4], xf[MT][4];
+  // a wave takes consecutive turns, the loads of U of them before the first is used (past its last one: that again, as zeros)
+  const int64_t each = (whole + WAVES - 1) / WAVES, end = min(whole, (wave + 1) * each);
+  for (int64_t c = wave * each; c < end; c += U) {
+    uint4 wf[U][PAIR][4], xf[U][MT][4];
 #pragma unroll
-    for (int g = 0; g < PAIR; ++g)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_u16*>(wp[g] + 128 * c + 8 * j));
-        wf[g][j] = make_uint4(v.x, v.y, v.z, v.w);
-      }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) xf[m][j] = UIO<T>::raw(xp[m] + 128 * c + 8 * j).u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = 128 * min(c + u, end - 1);
 #pragma unroll
       for (int g = 0; g < PAIR; ++g)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[g][m] = mfma16(T{}, wf[g][j], xf[m][j], acc[g][m]);
+        for (int j = 0; j < 4; ++j) wf[u][g][j] = UIO<T>::raw(wp[g] + at + 32 * j).u;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xf[u][m][j] = UIO<T>::raw(xp[m] + at + 32 * j).u;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool there = c + u < end;   // wave-uniform
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint4 xv = there ? xf[u][m][j] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int g = 0; g < PAIR; ++g) {
+            const uint4 wv = there ? wf[u][g][j] : make_uint4(0u, 0u, 0u, 0u);
+            acc[g][m] = mfma16(T{}, wv, xv, acc[g][m]);
+          }
+        }
+    }
   }
-  if (k % 128 && whole % WAVES == wave) {   // the last columns, zeros past them
+  if (k % 128 && wave == WAVES - 1) {   // the last columns, zeros past them
     auto piece = [&](const T* p, int64_t c) {
-      if (c + 8 <= k) return UIO<T>::raw(p + c - 32 * quad).u;
+      if (c + 8 <= k) return UIO<T>::raw(p + c - 8 * quad).u;
       struct { T e[8]; } e;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e.e[i] = c + i < k ? p[c - 32 * quad + i] : (T)0;
+      for (int i = 0; i < 8; ++i) e.e[i] = c + i < k ? p[c - 8 * quad + i] : (T)0;
       return __builtin_bit_cast(uint4, e);
     };
     for (int j = 0; j < 4; ++j) {
-      const int64_t c = 128 * whole + 32 * quad + 8 * j;
+      const int64_t c = 128 * whole + 32 * j + 8 * quad;
       uint4 wf[PAIR], xf[MT];
 #pragma unroll
       for (int g = 0; g < PAIR; ++g) wf[g] = piece(wp[g], c);
@@ -617,11 +628,12 @@ inline Tiling tiling_of(int64_t np, int64_t nq, int64_t k, bool may_split) {
   double least = 1e30;
   for (int big = 0; big < 2; ++big) {
     const int64_t t = big ? 256 : 128, tiles = ((np + t - 1) / t) * ((nq + t - 1) / t), at_once = big ? CUS : 2 * CUS;
+    // a round that does not fill the GPU is faster (less contention, a higher clock): 352 large tiles of 128 steps 335 us
+    auto step = [&](double f) { return big ? (f < 0.32 ? 0.9 : 0.55 + 1.1 * f) : (f < 0.4 ? 0.6 : 0.3 + 0.78 * f); };
     const int64_t ks = (k + 63) / 64, most = may_split ? (ks / 4 < 32 ? ks / 4 : 32) : 1;
     for (int64_t s = 1; s <= (most < 1 ? 1 : most); ++s) {
-      const int64_t rounds = (tiles * s + at_once - 1) / at_once, each = (ks + s - 1) / s;
-      const double one = big ? 1.65 : tiles * s <= CUS ? 0.75 : 1.08;
-      const double us = rounds * (each * one + 5.0) + (s > 1 ? 2.0 + (double)s * np * nq * 8 / 4e6 : 0.0);
+      const int64_t full = tiles * s / at_once, rest = tiles * s % at_once, each = (ks + s - 1) / s;
+      const double us = full * (each * step(1.0) + 5.0) + (rest ? each * step((double)rest / at_once) + 5.0 : 0.0) + (s > 1 ? 2.0 + (double)s * np * nq * 8 / 4e6 : 0.0);
       if (us < least) least = us, best = Tiling{big != 0, (int)s};
     }
   }
@@ -659,10 +671,20 @@ int few(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t
         hipStream_t st) {
   const int64_t blocks = (n + 15) / 16;
   if (blocks > MAX_SIZE) return LDR_E_SHAPE;
-#define FEW(W) hipLaunchKernelGGL((k_few_tokens<T, MT, PAIR, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, static_cast<const T*>(x), \
-                                  ldx, static_cast<const T*>(w), ldw, static_cast<T*>(y), ldy, (int)t, n, k, act)
-  if (blocks >= 512) FEW(4);   // waves for every CU to have some eight
-  else FEW(8);
+#define FEW(W, U) hipLaunchKernelGGL((k_few_tokens<T, MT, PAIR, W, U>), dim3((unsigned)blocks), dim3(64 * W), 0, st,                   \
+                                     static_cast<const T*>(x), ldx, static_cast<const T*>(w), ldw, static_cast<T*>(y), ldy, (int)t, n,  \
+                                     k, act)
+  // waves that share a workgroup's columns: more where there are few workgroups; as many turns' loads in flight as each has, up
+  // to what its registers hold
+  constexpr int MANY = PAIR > 1 ? 8 : 16, MOST = MT > 1 ? 2 : PAIR > 1 ? 4 : 3;
+  const int64_t turns = k / 128;
+  if (blocks >= 256) {
+    if (turns <= 4) FEW(4, 1);
+    else FEW(4, MOST);
+  } else {
+    if (turns <= MANY) FEW(MANY, 1);
+    else FEW(MANY, (MOST > 2 && PAIR > 1 ? 2 : MOST));
+  }
 #undef FEW
   return launched();
 }
@@ -670,8 +692,7 @@ template <typename T, int PAIR>
 int few_tokens(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t ldy, int64_t t, int64_t n, int64_t k, int act,
                hipStream_t st) {
   if (t <= 16) return few<T, 1, PAIR>(x, ldx, w, ldw, y, ldy, t, n, k, act, st);
-  if (t <= 32) return few<T, 2, PAIR>(x, ldx, w, ldw, y, ldy, t, n, k, act, st);
-  return few<T, 4, PAIR>(x, ldx, w, ldw, y, ldy, t, n, k, act, st);
+  return few<T, 2, PAIR>(x, ldx, w, ldw, y, ldy, t, n, k, act, st);
 }
 
 #define FFN_TYPE_SWITCH(DT, ...)                                 \
