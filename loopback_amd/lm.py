@@ -15,7 +15,12 @@ package's own kernels (lm_ops), the residual's add and its gradient inside the n
 head width 64 with its rotation; other attention is torch's SDPA restricted to its flash and
 memory-efficient kernels in 16-bit (never the math path's batched products in bf16).
 
+Options that the reference's model has not (all off by default): the MLP as one operator (`ffn="fused"`), a norm after each
+attention and MLP (`post_norm`), a learned gate per channel on their outputs (`gate`, its first value), a scale of what joins
+the residual stream (`residual_scale`) and dropout on the embedding and on what joins (`dropout`), all from block_ops.
+
     python -m loopback_amd.lm --steps 10 --warmup 3            # config 5: the Loopback LM step, tokens/s
+    python -m loopback_amd.lm --ffn fused --post-norm --gate 0.5 --dropout 0.1   # the same with these options
     python -m loopback_amd.lm --residual none                  # the same model as Plain Loop
     python -m loopback_amd.lm --prefill --batch 8 --seq 4096 [--graph]   # no-grad forward, tokens/s
 """
@@ -32,6 +37,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import block_ops
 from . import lm_ops as ops
 from .cell import LoopDeltaAttnRes
 
@@ -53,6 +59,11 @@ class LMConfig:
     tie_word_embeddings: bool = False
     residual: str | None = "delta_attnres"
     beta: float = 0.75
+    ffn: str = "composed"          # "fused": the MLP is block_ops.gated_ffn
+    post_norm: bool = False        # an RMSNorm on each attention's and MLP's output
+    gate: float | None = None      # a learned gate per channel on that output, from this value
+    residual_scale: float = 1.0
+    dropout: float = 0.0           # of the embedding and of what joins the residual stream, in training
 
     def __post_init__(self):
         if self.hidden_size % self.num_heads:
@@ -65,6 +76,10 @@ class LMConfig:
             raise ValueError("prelude, coda >= 0 and loop_blocks, loops >= 1")
         if not 0.0 <= float(self.beta) < 1.0:
             raise ValueError(f"beta must be in [0, 1), got {self.beta}")
+        if self.ffn not in ("composed", "fused"):
+            raise ValueError(f"ffn must be 'composed' or 'fused', got {self.ffn!r}")
+        if not 0.0 <= float(self.dropout) < 1.0:
+            raise ValueError(f"dropout must be in [0, 1), got {self.dropout}")
 
     @property
     def intermediate(self) -> int:
@@ -147,6 +162,11 @@ def linear(layer: nn.Module, x: torch.Tensor) -> torch.Tensor:
     return layer(x)
 
 
+def _plain_linear(layer: nn.Module) -> bool:
+    """Whether a layer is its weight: a linear layer without a bias that nothing watches or replaces."""
+    return type(layer) in (nn.Linear, Linear) and layer.bias is None and not _hooked(layer)
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: LMConfig):
         super().__init__()
@@ -179,15 +199,20 @@ class Attention(nn.Module):
 
 
 class SwiGLU(nn.Module):
+    fused = False
+
     def __init__(self, cfg: LMConfig):
         super().__init__()
         self.gate_up = nn.Linear(cfg.hidden_size, 2 * cfg.intermediate, bias=False)
         self.down = nn.Linear(cfg.intermediate, cfg.hidden_size, bias=False)
+        self.fused = cfg.ffn == "fused"
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if torch.jit.is_scripting():   # a scripted layer is torch operations
             g, u = self.gate_up(x).chunk(2, dim=-1)
             y = self.down(F.silu(g) * u)
+        elif self.fused and _plain_linear(self.gate_up) and _plain_linear(self.down):
+            y = block_ops.gated_ffn(x, self.gate_up.weight, self.down.weight)
         else:
             y = linear(self.down, ops.swiglu(linear(self.gate_up, x)))
         return y
@@ -211,18 +236,51 @@ def add_norm(norm: nn.Module, x: torch.Tensor, add: torch.Tensor | None = None):
     return h, norm(h)
 
 
+def join_norm(norm: nn.Module | None, x: torch.Tensor, y: torch.Tensor, post: nn.Module | None = None, **how):
+    """(h, norm(h)) of h = x + what is left of y after the norm `post` and how's gate, scale and dropout (block_ops.block_join);
+    norm None: (h, None). Norms whose call is hooked, or of other classes, are called."""
+    def plain(m):
+        return m is None or (type(m) in (nn.RMSNorm, RMSNorm) and m.eps is not None and m.weight is not None
+                             and m.weight.dim() == 1 and not _hooked(m))
+
+    if not plain(post):
+        y, post = post(y), None
+    called = None
+    if not plain(norm) or (post is not None and norm is not None and norm.eps != post.eps):
+        norm, called = None, norm
+    some = norm if norm is not None else post
+    h, n = block_ops.block_join(x, y, post_weight=None if post is None else post.weight,
+                                pre_weight=None if norm is None else norm.weight, eps=0.0 if some is None else some.eps, **how)
+    return h, n if called is None else called(h)
+
+
 class Block(nn.Module):
+    joined = False
+
     def __init__(self, cfg: LMConfig):
         super().__init__()
+        # what joins the residual stream: norms and gates of the attention's and the MLP's output
+        self.joined = cfg.post_norm or cfg.gate is not None or cfg.residual_scale != 1.0 or cfg.dropout > 0.0
+        self.residual_scale, self.dropout = float(cfg.residual_scale), float(cfg.dropout)
         self.attn_norm = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps)
         self.attn = Attention(cfg)
         self.mlp_norm = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps)
         self.mlp = SwiGLU(cfg)
+        self.attn_post = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps) if cfg.post_norm else None
+        self.mlp_post = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps) if cfg.post_norm else None
+        gate = None if cfg.gate is None else torch.full((cfg.hidden_size,), float(cfg.gate))
+        self.attn_gate = None if gate is None else nn.Parameter(gate)
+        self.mlp_gate = None if gate is None else nn.Parameter(gate.clone())
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, rng: torch.Tensor | None = None, site: int = 0) -> torch.Tensor:
+        """rng: the step's generator (block_ops), needed where the block drops; it uses the places site and site + 1."""
         x, n = add_norm(self.attn_norm, x)
-        x, n = add_norm(self.mlp_norm, x, self.attn(n))
-        return x + self.mlp(n)
+        if not self.joined:
+            x, n = add_norm(self.mlp_norm, x, self.attn(n))
+            return x + self.mlp(n)
+        how = {"scale": self.residual_scale, "dropout": self.dropout if self.training else 0.0, "rng": rng}
+        x, n = join_norm(self.mlp_norm, x, self.attn(n), self.attn_post, gate=self.attn_gate, site=site, **how)
+        return join_norm(None, x, self.mlp(n), self.mlp_post, gate=self.mlp_gate, site=site + 1, **how)[0]
 
 
 class LoopbackLM(nn.Module):
@@ -240,6 +298,8 @@ class LoopbackLM(nn.Module):
         self.head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False)
         self.read = (LoopDeltaAttnRes(cfg.hidden_size, cfg.loops, cfg.loop_blocks, beta=cfg.beta, eps=cfg.norm_eps)
                      if cfg.residual == "delta_attnres" else None)
+        if cfg.dropout > 0.0:   # dropout's generator: its seed, and the number of training forwards so far
+            self.register_buffer("rng", torch.zeros(2, dtype=torch.int64))
         self.reset_parameters()
 
     @torch.no_grad()
@@ -250,6 +310,12 @@ class LoopbackLM(nn.Module):
                 nn.init.normal_(m.weight, mean=0.0, std=std)
             elif isinstance(m, nn.RMSNorm):
                 nn.init.ones_(m.weight)
+            elif isinstance(m, Block) and self.cfg.gate is not None:
+                nn.init.constant_(m.attn_gate, self.cfg.gate)
+                nn.init.constant_(m.mlp_gate, self.cfg.gate)
+        if self.cfg.dropout > 0.0:
+            self.rng[0] = torch.randint(-2 ** 62, 2 ** 62, ())
+            self.rng[1] = 0
         if self.read is not None:
             self.read.reset_parameters()
         if self.cfg.tie_word_embeddings:
@@ -258,12 +324,26 @@ class LoopbackLM(nn.Module):
     def hidden(self, ids: torch.Tensor) -> torch.Tensor:
         cfg = self.cfg
         h = self.embed(ids)
+        at = {}      # where a block drops: the step's generator, and its place (two per block application, 0 the embedding's)
+        if cfg.dropout > 0.0 and self.training:
+            rng = self.rng.clone()   # the backward's own: the next forward's step does not change it
+            with torch.no_grad():
+                self.rng[1] += 1
+            h = block_ops.dropout(h, cfg.dropout, rng)
+            at = {"rng": rng, "site": 1}
+
+        def run(blk, x):
+            y = blk(x, **at)
+            if at:
+                at["site"] += 2
+            return y
+
         for blk in self.prelude:
-            h = blk(h)
+            h = run(blk, h)
         K = cfg.loop_blocks
         if self.read is None:                                   # Plain Loop
             for k in range(K * cfg.loops):
-                h = self.middle[k % K](h)
+                h = run(self.middle[k % K], h)
         else:                                                   # Loopback (modeling_looped_transformer.py:437-481)
             h0 = h
             stack = None
@@ -273,7 +353,7 @@ class LoopbackLM(nn.Module):
             for k in range(K * cfg.loops):
                 l, blk = divmod(k, K)
                 x = h
-                hs = self.middle[blk](x)
+                hs = run(self.middle[blk], x)
                 if stack is not None:
                     deltas.append(stack.write(k, hs, x))
                     h, coeffs, prior = self.read.combine(hs, h0, deltas, coeffs, prior, l, blk, keys=keys,
@@ -282,7 +362,7 @@ class LoopbackLM(nn.Module):
                     deltas.append(hs - x)
                     h, coeffs, prior = self.read.combine(hs, h0, deltas, coeffs, prior, l, blk, keys=keys)
         for blk in self.coda:
-            h = blk(h)
+            h = run(blk, h)
         return add_norm(self.norm, h)[1]
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
@@ -318,27 +398,34 @@ def bench(argv=None):
                     help="time the no-grad forward (logits) instead of the training step; with --graph replayed as "
                          "one HIP graph")
     ap.add_argument("--graph", action="store_true")
+    ap.add_argument("--ffn", default="composed", choices=["composed", "fused"], help="the MLP's operator")
+    ap.add_argument("--post-norm", action="store_true", help="a norm after each attention and MLP")
+    ap.add_argument("--gate", type=float, default=None, help="a learned gate per channel on their outputs, from this value")
+    ap.add_argument("--residual-scale", type=float, default=1.0)
+    ap.add_argument("--dropout", type=float, default=0.0, help="of the embedding and of what joins the residual stream")
     a = ap.parse_args(argv)
+    options = {"ffn": a.ffn, "post_norm": a.post_norm, "gate": a.gate, "residual_scale": a.residual_scale, "dropout": a.dropout}
     if not torch.cuda.is_available():
         print("lm: no GPU visible", file=sys.stderr)
         sys.exit(3)
     if a.prefill:
         dev = torch.device("cuda", 0)
-        cfg = LMConfig(residual=None if a.residual == "none" else "delta_attnres")
+        cfg = LMConfig(residual=None if a.residual == "none" else "delta_attnres", **options)
         torch.manual_seed(0)
         model = LoopbackLM(cfg).to(device=dev, dtype=torch.bfloat16)
         gen = torch.Generator(device=dev).manual_seed(1)
         ids = torch.randint(0, cfg.vocab_size, (a.batch, a.seq), device=dev, generator=gen)
         return _prefill(model, cfg, ids, a)
-    print(json.dumps(time_training(a.steps, a.warmup, a.batch, a.seq, a.residual)), flush=True)
+    print(json.dumps(time_training(a.steps, a.warmup, a.batch, a.seq, a.residual, **options)), flush=True)
 
 
 def time_training(steps: int = 10, warmup: int = 3, batch: int = 8, seq: int = 2048,
-                  residual: str = "delta_attnres") -> dict:
+                  residual: str = "delta_attnres", **options) -> dict:
     """Config 5's training step on cuda:0 -- the random-init LM in bf16, uniform random ids (batch, seq), AdamW --
-    timed over `steps` steps after `warmup`; residual "none" is the same model as Plain Loop. Returns the record."""
+    timed over `steps` steps after `warmup`; residual "none" is the same model as Plain Loop; options: LMConfig's. Returns
+    the record."""
     dev = torch.device("cuda", 0)
-    cfg = LMConfig(residual=None if residual == "none" else "delta_attnres")
+    cfg = LMConfig(residual=None if residual == "none" else "delta_attnres", **options)
     torch.manual_seed(0)
     model = LoopbackLM(cfg).to(device=dev, dtype=torch.bfloat16)
     gen = torch.Generator(device=dev).manual_seed(1)
