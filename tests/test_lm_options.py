@@ -90,7 +90,7 @@ def test_gradients_against_differences():
     g = torch.Generator().manual_seed(3)
     way = [torch.randn(p.shape, generator=g, dtype=torch.float64) for p in params]
     exact = sum((a * b).sum() for a, b in zip(grads, way))
-    eps, got = 1e-4, []
+    eps, got = 1e-5, []
     with torch.no_grad():
         for sign in (1, -1):
             for p, w in zip(params, way):
@@ -98,8 +98,9 @@ def test_gradients_against_differences():
             got.append(loss())
             for p, w in zip(params, way):
                 p -= sign * eps * w
-    # weights of 0.02 moved by 1e-4: the difference's next term is some (1e-4 / 0.02)^2 = 2.5e-5 of the slope times a third
-    # derivative's factors; the rotation rounds q and k to fp32, 6e-8 of them, so up to 6e-8 / 2e-4 = 3e-4 from that
+    # The difference is off by its next term, quadratic in the step: norms of outputs that weights of 0.02 make (0.02^2 times
+    # sums of 128, some 1e-2) bend over that size, so the step is far below it. The rotation rounds q and k to fp32, 6e-8 of
+    # them, which a step of 1e-5 turns into up to 6e-8 / 2e-5 = 3e-3.
     assert abs((got[0] - got[1]) / (2 * eps) - exact) <= 5e-3 * max(1.0, abs(exact))
 
 
