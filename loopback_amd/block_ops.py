@@ -24,6 +24,7 @@ import os
 import torch
 import torch.nn.functional as F
 
+from . import _host as H      # the launch path (csrc/host.cpp), bound below to the library
 from . import build as _build
 from .lm_ops import _again, _launchable, _stream, _watched, native
 
@@ -68,17 +69,14 @@ def _load() -> ctypes.CDLL:
 
 
 LIB = _load()
-_FN = {name: getattr(LIB, name) for name in SIGNATURES}
+_FN = {name: getattr(H, name, None) for name in SIGNATURES
+       if H.bind(name, ctypes.cast(getattr(LIB, name), ctypes.c_void_p).value)}
 
 
 def _run(name: str, *args) -> None:
     code = _FN[name](*args)
     if code:
         raise RuntimeError(f"{name}: refused or failed to launch (code {code})")
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _upcast(t: torch.Tensor) -> torch.Tensor:
@@ -173,11 +171,7 @@ def _autocast_only(x) -> bool:
 
 
 def _dropout_launch(x, rng, site, drop):
-    out = torch.empty_like(x)
-    d = x.shape[-1]
-    _run("lbk_dropout", x.data_ptr(), rng.data_ptr(), site, drop, out.data_ptr(), x.numel() // d, d, _CODES[x.dtype],
-         _stream(x))
-    return out
+    return H.dropout(x, rng, site, drop, _CODES[x.dtype], _stream(x))
 
 
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0) -> torch.Tensor:
@@ -220,16 +214,7 @@ def _join_torch(x, y, post, gate, pre, rng, site, drop, scale, eps):
 
 def _join_launch(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, keep):
     """h, n and, with `keep`, the rows' scales for a backward. Contiguous tensors."""
-    d = x.shape[-1]
-    rows = x.numel() // d
-    h = torch.empty_like(x)
-    n = None if pre is None else torch.empty_like(x)
-    r_post = torch.empty(rows, device=x.device, dtype=torch.float32) if keep and post is not None else None
-    r_pre = torch.empty(rows, device=x.device, dtype=torch.float32) if keep and pre is not None else None
-    _run("lbk_join_fwd", x.data_ptr(), y.data_ptr(), _ptr(post), _ptr(gate), gate_rows, _ptr(pre),
-         rng.data_ptr() if drop else None, site, drop, scale, eps, h.data_ptr(), _ptr(n), _ptr(r_post), _ptr(r_pre), rows, d,
-         _CODES[x.dtype], _stream(x))
-    return h, n, r_post, r_pre
+    return H.join_fwd(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, _CODES[x.dtype], _stream(x), keep)
 
 
 class _Join(torch.autograd.Function):
@@ -272,19 +257,10 @@ class _Join(torch.autograd.Function):
             out[2] = None if post is None else next(got)
             out[3] = None if gate is None else next(got)
             return tuple(out)
-        d = y.shape[-1]
-        rows = y.numel() // d
         dh, dn = _plain_rows(None if dh is None else dh.to(y.dtype), None if dn is None else dn.to(y.dtype))
-        new = lambda wanted, like: torch.empty_like(like) if wanted else None
-        dx, dy, dpost, dgate, dpre = new(nx, y), new(ny, y), new(npost, post), new(ngate, gate), new(npre, pre)
-        scratch = None
-        if npost or ngate or npre:
-            scratch = torch.empty(LIB.lbk_join_scratch(rows, d, gate_rows), device=y.device, dtype=torch.float32)
-        if nx or ny or scratch is not None:
-            _run("lbk_join_bwd", _ptr(dh), _ptr(dn), _ptr(h), y.data_ptr(), _ptr(post), _ptr(gate), gate_rows, _ptr(pre),
-                 _ptr(r_post), _ptr(r_pre), _ptr(rng), site, drop, scale, _ptr(dx), _ptr(dy), _ptr(dpost), _ptr(dgate),
-                 _ptr(dpre), _ptr(scratch), rows, d, _CODES[y.dtype], _stream(y))
-        out[0], out[1], out[2], out[3], out[5] = dx, dy, dpost, dgate, dpre
+        out[0], out[1], out[2], out[3], out[5] = H.join_bwd(
+            dh, dn, h, y, post, gate, gate_rows, pre, r_post, r_pre, rng, site, drop, scale, _CODES[y.dtype], _stream(y),
+            nx + 2 * ny + 4 * npost + 8 * ngate + 16 * npre)
         return tuple(out)
 
 
@@ -344,15 +320,15 @@ def _ffn_torch(x, w_gate_up, w_down, activation):
 
 
 def _operand(t, code, st):
-    """(tensor, address, elements between rows) of contiguous rows as the tiled products take them: the tensor itself where its
+    """(tensor, elements between rows) of contiguous rows as the tiled products take them: the tensor itself where its
     rows are aligned, else a copy that is."""
     cols = t.shape[-1]
     if cols % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t, t.data_ptr(), cols
+        return t, cols
     rows, ld = t.numel() // cols, (cols + 7) // 8 * 8
     out = torch.empty((rows, ld), device=t.device, dtype=t.dtype)
-    _run("lbk_pad_rows", t.data_ptr(), rows, cols, ld, out.data_ptr(), code, st)
-    return out, out.data_ptr(), ld
+    _run("lbk_pad_rows", t, rows, cols, ld, out, code, st)
+    return out, ld
 
 
 def _scratch(columns, rows, summed, like):
@@ -369,17 +345,17 @@ def _ffn_forward(x, w_gate_up, w_down, activation, keep):
     saved = torch.empty(LIB.lbk_ffn_saved_bytes(t, n), device=x.device, dtype=torch.uint8) if keep else None
     y = torch.empty((*x.shape[:-1], m), device=x.device, dtype=x.dtype)
     if t <= FEW_TOKENS and not keep:
-        (xp, ldx), (wp, ldw) = (x.data_ptr(), d), (w_gate_up.data_ptr(), d)
+        ldx = ldw = d
     else:
-        x, xp, ldx = _operand(x, code, st)
-        w_gate_up, wp, ldw = _operand(w_gate_up, code, st)
-    _run("lbk_ffn_gate_up", xp, ldx, wp, ldw, act.data_ptr(), n8, _ptr(saved), t, d, n, activation, code, st)
+        x, ldx = _operand(x, code, st)
+        w_gate_up, ldw = _operand(w_gate_up, code, st)
+    _run("lbk_ffn_gate_up", x, ldx, w_gate_up, ldw, act, n8, saved, t, d, n, activation, code, st)
     if t <= FEW_TOKENS:
-        wp, ldw, scratch = w_down.data_ptr(), n, None
+        ldw, scratch = n, None
     else:
-        w_down, wp, ldw = _operand(w_down, code, st)
+        w_down, ldw = _operand(w_down, code, st)
         scratch = _scratch(m, t, n, x)
-    _run("lbk_linear_fwd", act.data_ptr(), n8, wp, ldw, y.data_ptr(), m, _ptr(scratch), t, n, m, code, st)
+    _run("lbk_linear_fwd", act, n8, w_down, ldw, y, m, scratch, t, n, m, code, st)
     return y, act, saved
 
 
@@ -403,30 +379,27 @@ class _GatedFfn(torch.autograd.Function):
             return *_again(fn, [x, w_gate_up, w_down], need[:3], dy), None
         d, (m, n), code, st = x.shape[-1], w_down.shape, _CODES[x.dtype], _stream(x)
         t = x.numel() // d
-        dy, dyp, ld_dy = _operand(dy.to(x.dtype).contiguous(), code, st)
+        dy, ld_dy = _operand(dy.to(x.dtype).contiguous(), code, st)
         dx = dw_gate_up = dw_down = None
         if need[0] or need[1]:
             if saved.data_ptr() % 16:
                 saved = saved.clone()   # a saved-tensor hook's
             ld = (2 * n + 7) // 8 * 8
             dgu = torch.empty((t, ld), device=x.device, dtype=x.dtype)
-            wd, wp, ldw = _operand(w_down, code, st)
-            _run("lbk_ffn_dgate_up", dyp, ld_dy, wp, ldw, saved.data_ptr(), dgu.data_ptr(), ld, t, n, m, code, st)
+            wd, ldw = _operand(w_down, code, st)
+            _run("lbk_ffn_dgate_up", dy, ld_dy, wd, ldw, saved, dgu, ld, t, n, m, code, st)
             if need[0]:
                 dx = torch.empty_like(x)
-                w, wp, ldw = _operand(w_gate_up, code, st)
-                s = _scratch(d, t, 2 * n, x)
-                _run("lbk_linear_dx", dgu.data_ptr(), ld, wp, ldw, dx.data_ptr(), d, _ptr(s), t, 2 * n, d, code, st)
+                w, ldw = _operand(w_gate_up, code, st)
+                _run("lbk_linear_dx", dgu, ld, w, ldw, dx, d, _scratch(d, t, 2 * n, x), t, 2 * n, d, code, st)
             if need[1]:
                 dw_gate_up = torch.empty_like(w_gate_up)
-                xs, xp, ldx = _operand(x, code, st)
-                s = _scratch(d, 2 * n, t, x)
-                _run("lbk_linear_dw", dgu.data_ptr(), ld, xp, ldx, _ptr(s), dw_gate_up.data_ptr(), t, 2 * n, d, code, st)
+                xs, ldx = _operand(x, code, st)
+                _run("lbk_linear_dw", dgu, ld, xs, ldx, _scratch(d, 2 * n, t, x), dw_gate_up, t, 2 * n, d, code, st)
         if need[2]:
             dw_down = torch.empty_like(w_down)
-            act, ap, ld_act = _operand(act, code, st)
-            s = _scratch(n, m, t, x)
-            _run("lbk_linear_dw", dyp, ld_dy, ap, ld_act, _ptr(s), dw_down.data_ptr(), t, m, n, code, st)
+            act, ld_act = _operand(act, code, st)
+            _run("lbk_linear_dw", dy, ld_dy, act, ld_act, _scratch(n, m, t, x), dw_down, t, m, n, code, st)
         return dx, dw_gate_up, dw_down, None
 
 
