@@ -40,6 +40,10 @@ template <typename T> __device__ __forceinline__ typename IO<T>::Raw zero_unless
     return Sel16<T>::zero_unless(ok, r);
   }
 }
+// the same values, looked at anew: what is unpacked from them in a loop is not kept in twice the registers outside it
+template <typename T> __device__ __forceinline__ void anew(typename IO<T>::Raw& r) {
+  if constexpr (!std::is_same<T, float>::value) asm volatile("" : "+v"(r.u.x), "+v"(r.u.y), "+v"(r.u.z), "+v"(r.u.w));
+}
 template <typename T> struct Eight { T e[8]; };
 template <typename T, bool AL> __device__ __forceinline__ typename IO<T>::Raw load8(const T* p, int col, int d) {
   if constexpr (AL) {
@@ -123,6 +127,13 @@ __global__ __launch_bounds__(WG) void k_dropout(const T* __restrict__ x, const i
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int lanes_of(int lpr) { return lpr > WG ? lpr : WG; }
 
+// which of the workgroup's rows this lane has a share of; the same for a whole wave where rows are at least that wide, so that
+// the rows' addresses are scalar
+template <int LPR> __device__ __forceinline__ int group_of() {
+  const int g = (int)threadIdx.x / LPR;
+  return LPR >= 64 ? __builtin_amdgcn_readfirstlane(g) : g;
+}
+
 // sums over the lanes of a row; rows wider than a wave meet in LDS. The two slots take turns: a slot is written again only
 // after the barrier of the other one, which every wave reaches past its reads
 template <int LPR> struct RowSum {
@@ -154,23 +165,28 @@ template <typename T> struct JoinFwd {
   float scale, keep, eps;
 };
 
-template <typename T, int LPR, int VPT, bool AL>
+// PARTS: which parts the call has, known when the kernel is compiled (1 the norm before the next block, 2 the norm after this
+// one, 4 dropout), or ANY: looked up as it runs (rows that take the narrow loads)
+constexpr int ANY = -1;
+template <typename T, int LPR, int VPT, bool AL, int PARTS>
 __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) {
+  const bool has_pre = PARTS < 0 ? a.pre != nullptr : PARTS & 1, has_post = PARTS < 0 ? a.post != nullptr : PARTS & 2,
+             drops = PARTS < 0 ? a.drop != 0 : PARTS & 4;
   constexpr int LANES = lanes_of(LPR), R = LANES / LPR;
   __shared__ float s_red[2][LANES / 64];
   RowSum<LPR> row_sum{s_red};
-  const int d = a.d, lane = (int)threadIdx.x % LPR, grp = (int)threadIdx.x / LPR;
+  const int d = a.d, lane = (int)threadIdx.x % LPR, grp = group_of<LPR>();
   const float inv_d = 1.f / (float)d;
   typename IO<T>::Raw post[VPT], pre[VPT], gate[VPT];
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int col = 8 * (lane + LPR * v);
-    post[v] = a.post ? load8<T, AL>(a.post, col, d) : IO<T>::zero();
-    pre[v] = a.pre ? load8<T, AL>(a.pre, col, d) : IO<T>::zero();
+    post[v] = has_post ? load8<T, AL>(a.post, col, d) : IO<T>::zero();
+    pre[v] = has_pre ? load8<T, AL>(a.pre, col, d) : IO<T>::zero();
     gate[v] = IO<T>::zero();
   }
   Rng rng{0, 0, 0};
-  if (a.drop) rng = rng_of(a.rng);
+  if (drops) rng = rng_of(a.rng);
   int gate_row = -1;
   for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < a.rows; row0 += (int64_t)gridDim.x * R) {
     const int64_t mine = row0 + grp;
@@ -189,7 +205,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) 
       for (int v = 0; v < VPT; ++v) gate[v] = load8<T, AL>(a.gate + (int64_t)gate_row * d, 8 * (lane + LPR * v), d);
     }
     float r1 = 1.f;
-    if (a.post) {
+    if (has_post) {
       float ss = 0.f;
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
@@ -206,7 +222,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) 
     for (int v = 0; v < VPT; ++v) {
       float z[8], e[8];
       IO<T>::unpack(yr[v], z);
-      if (a.post) {
+      if (has_post) {
         IO<T>::unpack(post[v], e);
 #pragma unroll
         for (int k = 0; k < 8; ++k) z[k] *= r1 * e[k];
@@ -219,7 +235,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) 
       const int blk = lane + LPR * v;
 #pragma unroll
       for (int k = 0; k < 8; ++k) z[k] *= a.scale;
-      if (a.drop) drop8(z, (uint32_t)blk, (uint32_t)row, a.site, rng, a.drop, a.keep);
+      if (drops) drop8(z, (uint32_t)blk, (uint32_t)row, a.site, rng, a.drop, a.keep);
       IO<T>::unpack(xr[v], h[v]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -228,7 +244,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) 
       }
       if (ok) store8<T, AL>(a.h + ro, 8 * blk, d, h[v]);
     }
-    if (a.pre) {
+    if (has_pre) {
       const float r2 = rsqrtf(row_sum(ss) * inv_d + a.eps);
       if (a.r_pre && lane == 0 && ok) a.r_pre[row] = r2;
 #pragma unroll
@@ -258,27 +274,29 @@ template <typename T> struct JoinBwd {
 // belong to runs of gate_rows rows: a run that lies inside the workgroup's rows is finished here, a share of a longer one
 // goes to part_gate, first slot where the run began before this workgroup's rows, second where it ends after them.
 // gate_rows 1: each element's own.
-template <typename T, int LPR, int VPT, bool AL>
+template <typename T, int LPR, int VPT, bool AL, int PARTS>
 __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) {
+  const bool has_dn = PARTS < 0 ? a.dn != nullptr : PARTS & 1, has_post = PARTS < 0 ? a.post != nullptr : PARTS & 2,
+             drops = PARTS < 0 ? a.drop != 0 : PARTS & 4;
   constexpr int LANES = lanes_of(LPR), R = LANES / LPR, W = 8 * LPR * VPT;
   __shared__ float s_red[2][LANES / 64];
   __shared__ float s_sum[R > 1 ? R * W : 1];
   RowSum<LPR> row_sum{s_red};
-  const int d = a.d, lane = (int)threadIdx.x % LPR, grp = (int)threadIdx.x / LPR;
+  const int d = a.d, lane = (int)threadIdx.x % LPR, grp = group_of<LPR>();
   const float inv_d = 1.f / (float)d;
   typename IO<T>::Raw post[VPT], pre[VPT], gate[VPT];
   float d_post[VPT][8], d_pre[VPT][8], d_gate[VPT][8];
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int col = 8 * (lane + LPR * v);
-    post[v] = a.post ? load8<T, AL>(a.post, col, d) : IO<T>::zero();
-    pre[v] = a.pre ? load8<T, AL>(a.pre, col, d) : IO<T>::zero();
+    post[v] = has_post ? load8<T, AL>(a.post, col, d) : IO<T>::zero();
+    pre[v] = has_dn ? load8<T, AL>(a.pre, col, d) : IO<T>::zero();
     gate[v] = IO<T>::zero();
 #pragma unroll
     for (int k = 0; k < 8; ++k) d_post[v][k] = d_pre[v][k] = d_gate[v][k] = 0.f;
   }
   Rng rng{0, 0, 0};
-  if (a.drop) rng = rng_of(a.rng);
+  if (drops) rng = rng_of(a.rng);
   int gate_row = -1;
 
   // the row groups' column sums, added in order, to out (fp32) or out_t (rounded)
@@ -322,21 +340,34 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
         const int col = 8 * (lane + LPR * v);
-        if (a.dn) {
+        if (has_dn) {
           dnr[v] = load8<T, AL>(a.dn + ro, col, d);
           hr[v] = load8<T, AL>(a.h + ro, col, d);
         }
-        if (a.dh) dhr[v] = load8<T, AL>(a.dh + ro, col, d);
+        dhr[v] = a.dh ? load8<T, AL>(a.dh + ro, col, d) : IO<T>::zero();
         yr[v] = load8<T, AL>(a.y + ro, col, d);
+      }
+      if constexpr (R > 1) {   // a row that is not there adds nothing to the column sums
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+          if (has_dn) dnr[v] = zero_unless<T>(ok, dnr[v]);
+          dhr[v] = zero_unless<T>(ok, dhr[v]);
+        }
       }
       if (a.gate && row / a.gate_rows != gate_row) {
         gate_row = row / a.gate_rows;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) gate[v] = load8<T, AL>(a.gate + (int64_t)gate_row * d, 8 * (lane + LPR * v), d);
       }
-      const float q2 = a.dn ? a.r_pre[row] : 0.f, q1 = a.post ? a.r_post[row] : 1.f;
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        anew<T>(post[v]);
+        anew<T>(pre[v]);
+        anew<T>(gate[v]);
+      }
+      const float q2 = has_dn ? a.r_pre[row] : 0.f, q1 = has_post ? a.r_post[row] : 1.f;
       float g[VPT][8];   // the gradient of h
-      if (a.dn) {
+      if (has_dn) {
         float c = 0.f;   // sum dn pre h
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
@@ -346,7 +377,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
           IO<T>::unpack(pre[v], w);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            if (ok) d_pre[v][k] = __builtin_fmaf(g[v][k], e[k] * q2, d_pre[v][k]);
+            d_pre[v][k] = __builtin_fmaf(g[v][k], e[k] * q2, d_pre[v][k]);
             g[v][k] *= w[k];
             c = __builtin_fmaf(g[v][k], e[k], c);
           }
@@ -358,11 +389,9 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
           IO<T>::unpack(hr[v], e);
 #pragma unroll
           for (int k = 0; k < 8; ++k) g[v][k] = q2 * (g[v][k] - c * e[k]);
-          if (a.dh) {
-            IO<T>::unpack(dhr[v], e);
+          IO<T>::unpack(dhr[v], e);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) g[v][k] += e[k];
-          }
+          for (int k = 0; k < 8; ++k) g[v][k] += e[k];
         }
       } else {
 #pragma unroll
@@ -379,28 +408,28 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
         IO<T>::unpack(gate[v], gt);
 #pragma unroll
         for (int k = 0; k < 8; ++k) g[v][k] *= a.scale;
-        if (a.drop) drop8(g[v], (uint32_t)blk, (uint32_t)row, a.site, rng, a.drop, a.keep);
+        if (drops) drop8(g[v], (uint32_t)blk, (uint32_t)row, a.site, rng, a.drop, a.keep);
         if (a.gate) {
           float og[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            og[k] = g[v][k] * (a.post ? e[k] * q1 * w[k] : e[k]);
-            if (ok) d_gate[v][k] += og[k];
+            og[k] = g[v][k] * (has_post ? e[k] * q1 * w[k] : e[k]);
+            d_gate[v][k] += og[k];
             g[v][k] *= gt[k];
           }
           if (a.dgate && a.gate_rows == 1 && ok) store8<T, AL>(a.dgate + ro, 8 * blk, d, og);
         }
-        if (a.post) {
+        if (has_post) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            if (ok) d_post[v][k] = __builtin_fmaf(g[v][k], e[k] * q1, d_post[v][k]);
+            d_post[v][k] = __builtin_fmaf(g[v][k], e[k] * q1, d_post[v][k]);
             g[v][k] *= w[k];
             c = __builtin_fmaf(g[v][k], e[k], c);
           }
         }
       }
       if (a.dy) {
-        if (a.post) {
+        if (has_post) {
           c = row_sum(c) * q1 * q1 * inv_d;
 #pragma unroll
           for (int v = 0; v < VPT; ++v) {
@@ -493,7 +522,7 @@ inline int launched() { return (int)hipGetLastError(); }
 // lanes per row: the fewest that hold it in two vectors each up to a wave, in one beyond
 struct Shape { int lpr, vpt; };
 inline Shape shape_of(int64_t d) {
-  return d <= 32 ? Shape{4, 1} : d <= 128 ? Shape{16, 1} : d <= 512 ? Shape{64, 1} : d <= 1024 ? Shape{64, 2}
+  return d <= 32 ? Shape{4, 1} : d <= 128 ? Shape{16, 1} : d <= 512 ? Shape{64, 1} : d <= 1024 ? Shape{128, 1}
        : d <= 2048 ? Shape{256, 1} : d <= 4096 ? Shape{512, 1} : Shape{1024, 1};
 }
 
@@ -517,13 +546,23 @@ inline Plan plan_of(int64_t rows, int64_t d, int64_t gate_rows) {
   switch ((S).lpr) {                                                                      \
     case 4: { constexpr int LPR = 4, VPT = 1; __VA_ARGS__; } break;                       \
     case 16: { constexpr int LPR = 16, VPT = 1; __VA_ARGS__; } break;                     \
-    case 64:                                                                              \
-      if ((S).vpt == 1) { constexpr int LPR = 64, VPT = 1; __VA_ARGS__; }                 \
-      else { constexpr int LPR = 64, VPT = 2; __VA_ARGS__; }                              \
-      break;                                                                              \
+    case 64: { constexpr int LPR = 64, VPT = 1; __VA_ARGS__; } break;                     \
+    case 128: { constexpr int LPR = 128, VPT = 1; __VA_ARGS__; } break;                   \
     case 256: { constexpr int LPR = 256, VPT = 1; __VA_ARGS__; } break;                   \
     case 512: { constexpr int LPR = 512, VPT = 1; __VA_ARGS__; } break;                   \
     default: { constexpr int LPR = 1024, VPT = 1; __VA_ARGS__; } break;                   \
+  }
+
+#define LBK_PARTS_SWITCH(P, ...)                                 \
+  switch (P) {                                                   \
+    case 0: { constexpr int PARTS = 0; __VA_ARGS__; } break;     \
+    case 1: { constexpr int PARTS = 1; __VA_ARGS__; } break;     \
+    case 2: { constexpr int PARTS = 2; __VA_ARGS__; } break;     \
+    case 3: { constexpr int PARTS = 3; __VA_ARGS__; } break;     \
+    case 4: { constexpr int PARTS = 4; __VA_ARGS__; } break;     \
+    case 5: { constexpr int PARTS = 5; __VA_ARGS__; } break;     \
+    case 6: { constexpr int PARTS = 6; __VA_ARGS__; } break;     \
+    default: { constexpr int PARTS = 7; __VA_ARGS__; } break;    \
   }
 
 }  // namespace
@@ -586,8 +625,12 @@ int lbk_join_fwd(const void* x, const void* y, const void* post, const void* gat
                        static_cast<T*>(n), r_post, r_pre, (int)rows, (int)d, (int)gr, site, (uint32_t)drop, scale,
                        keep_scale(drop), eps};
     LBK_SHAPE_SWITCH(s, {
-      if (al) hipLaunchKernelGGL((k_join_fwd<T, LPR, VPT, true>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a);
-      else hipLaunchKernelGGL((k_join_fwd<T, LPR, VPT, false>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a);
+      if (al) {
+        LBK_PARTS_SWITCH((pre ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
+                         hipLaunchKernelGGL((k_join_fwd<T, LPR, VPT, true, PARTS>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a))
+      } else {
+        hipLaunchKernelGGL((k_join_fwd<T, LPR, VPT, false, ANY>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a);
+      }
     })
   })
   return launched();
@@ -629,8 +672,12 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* h, const void* y, c
                        scratch + 2 * parts * d, (int)rows, (int)d, (int)gr, (int)plan.per, site, (uint32_t)drop, scale,
                        keep_scale(drop)};
     LBK_SHAPE_SWITCH(s, {
-      if (al) hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, true>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a);
-      else hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, false>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a);
+      if (al) {
+        LBK_PARTS_SWITCH((dn ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
+                         hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, true, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
+      } else {
+        hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, false, ANY>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a);
+      }
     })
     const int err = launched();
     if (err) return err;
