@@ -337,26 +337,29 @@ def _scratch(columns, rows, summed, like):
 
 
 def _ffn_forward(x, w_gate_up, w_down, activation, keep):
-    """y, and what the backward needs: the activations (t, n rounded up to 8) and the projections' saved values."""
+    """y, and what the backward needs: the activations (t, n rounded up to 8), the projections' saved values, and the aligned
+    copies of x and the weights (None where they are aligned)."""
     d, (m, n), code, st = x.shape[-1], w_down.shape, _CODES[x.dtype], _stream(x)
     t = x.numel() // d
     n8 = (n + 7) // 8 * 8
     act = torch.empty((t, n8), device=x.device, dtype=x.dtype)
     saved = torch.empty(LIB.lbk_ffn_saved_bytes(t, n), device=x.device, dtype=torch.uint8) if keep else None
     y = torch.empty((*x.shape[:-1], m), device=x.device, dtype=x.dtype)
+    xs, wgu, wd = x, w_gate_up, w_down
     if t <= FEW_TOKENS and not keep:
         ldx = ldw = d
     else:
-        x, ldx = _operand(x, code, st)
-        w_gate_up, ldw = _operand(w_gate_up, code, st)
-    _run("lbk_ffn_gate_up", x, ldx, w_gate_up, ldw, act, n8, saved, t, d, n, activation, code, st)
+        xs, ldx = _operand(x, code, st)
+        wgu, ldw = _operand(w_gate_up, code, st)
+    _run("lbk_ffn_gate_up", xs, ldx, wgu, ldw, act, n8, saved, t, d, n, activation, code, st)
     if t <= FEW_TOKENS:
         ldw, scratch = n, None
     else:
-        w_down, ldw = _operand(w_down, code, st)
+        wd, ldw = _operand(w_down, code, st)
         scratch = _scratch(m, t, n, x)
-    _run("lbk_linear_fwd", act, n8, w_down, ldw, y, m, scratch, t, n, m, code, st)
-    return y, act, saved
+    _run("lbk_linear_fwd", act, n8, wd, ldw, y, m, scratch, t, n, m, code, st)
+    copies = [None if b is a else b for a, b in ((x, xs), (w_gate_up, wgu), (w_down, wd))] if keep else None
+    return y, act, saved, copies
 
 
 class _GatedFfn(torch.autograd.Function):
@@ -365,14 +368,14 @@ class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate_up, w_down, activation):
         need = ctx.needs_input_grad
-        y, act, saved = _ffn_forward(x, w_gate_up, w_down, activation, need[0] or need[1])
+        y, act, saved, copies = _ffn_forward(x, w_gate_up, w_down, activation, need[0] or need[1])
         ctx.activation = activation
-        ctx.save_for_backward(x, w_gate_up, w_down, act if need[2] else None, saved)
+        ctx.save_for_backward(x, w_gate_up, w_down, act if need[2] else None, saved, *(copies or (None, None, None)))
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, w_gate_up, w_down, act, saved = _plain_rows(*ctx.saved_tensors)
+        x, w_gate_up, w_down, act, saved, xs, wgu, wd = _plain_rows(*ctx.saved_tensors)
         need = ctx.needs_input_grad
         if not _launchable(dy):
             fn = lambda x, g, d: _ffn_torch(x, g, d, ctx.activation)
@@ -386,15 +389,15 @@ class _GatedFfn(torch.autograd.Function):
                 saved = saved.clone()   # a saved-tensor hook's
             ld = (2 * n + 7) // 8 * 8
             dgu = torch.empty((t, ld), device=x.device, dtype=x.dtype)
-            wd, ldw = _operand(w_down, code, st)
+            wd, ldw = _operand(w_down if wd is None else wd, code, st)
             _run("lbk_ffn_dgate_up", dy, ld_dy, wd, ldw, saved, dgu, ld, t, n, m, code, st)
             if need[0]:
                 dx = torch.empty_like(x)
-                w, ldw = _operand(w_gate_up, code, st)
+                w, ldw = _operand(w_gate_up if wgu is None else wgu, code, st)
                 _run("lbk_linear_dx", dgu, ld, w, ldw, dx, d, _scratch(d, t, 2 * n, x), t, 2 * n, d, code, st)
             if need[1]:
                 dw_gate_up = torch.empty_like(w_gate_up)
-                xs, ldx = _operand(x, code, st)
+                xs, ldx = _operand(x if xs is None else xs, code, st)
                 _run("lbk_linear_dw", dgu, ld, xs, ldx, _scratch(d, 2 * n, t, x), dw_gate_up, t, 2 * n, d, code, st)
         if need[2]:
             dw_down = torch.empty_like(w_down)

@@ -454,14 +454,15 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
   if (a.part_pre) flush(d_pre, a.part_pre + (int64_t)blockIdx.x * d, nullptr);
 }
 
-// The workgroups' shares summed in order and rounded: job 0 dpost, 1 dpre, 2 + b the gate run that crosses from workgroup b's
-// rows to b + 1's (by the first workgroup that has a share of it). 16 columns and 64 groups of shares per workgroup.
-constexpr int SUM_GROUPS = 64;
-template <typename T>
-__global__ __launch_bounds__(16 * SUM_GROUPS) void k_join_sum(const JoinBwd<T> a, T* __restrict__ d_post,
-                                                              T* __restrict__ d_pre, int parts) {
-  __shared__ float s[16 * SUM_GROUPS];
-  const int job = (int)blockIdx.y, d = a.d, c = (int)blockIdx.x * 16 + ((int)threadIdx.x & 15);
+// The workgroups' shares summed in order and rounded: job 0 dpost, 1 dpre, 2 + j the gate's run j where several workgroups have
+// a share of it. COLS columns and 1024 / COLS groups of shares per workgroup.
+constexpr int SUM_LANES = 1024;
+template <typename T, int COLS>
+__global__ __launch_bounds__(SUM_LANES) void k_join_sum(const JoinBwd<T> a, T* __restrict__ d_post, T* __restrict__ d_pre, int parts,
+                                                        int job0) {
+  constexpr int GROUPS = SUM_LANES / COLS;
+  __shared__ float s[SUM_LANES];
+  const int job = job0 + (int)blockIdx.y, d = a.d, c = (int)blockIdx.x * COLS + (int)threadIdx.x % COLS;
   const float *first, *rest;   // share 0, and share i > 0 at rest + i * step
   int64_t step = d;
   int count = parts;
@@ -475,36 +476,35 @@ __global__ __launch_bounds__(16 * SUM_GROUPS) void k_join_sum(const JoinBwd<T> a
     first = rest = a.part_pre;
     out = d_pre;
   } else {
-    const int64_t b = job - 2, cross = (b + 1) * a.per, run = cross / a.gate_rows, g0 = run * a.gate_rows;
-    if (g0 == cross || g0 < b * a.per) return;
-    const int64_t g1 = min((int64_t)a.rows, g0 + a.gate_rows);
+    const int64_t run = job - 2, g0 = run * a.gate_rows, g1 = min((int64_t)a.rows, g0 + a.gate_rows), b = g0 / a.per;
     count = (int)((g1 - 1) / a.per - b + 1);
+    if (count == 1) return;
     first = a.part_gate + (2 * b + 1) * d;
     rest = a.part_gate + 2 * b * d;
     step = 2 * (int64_t)d;
     out = a.dgate + run * d;
   }
-  const int grp = (int)threadIdx.x >> 4;
+  const int grp = (int)threadIdx.x / COLS;
   float acc = 0.f;
   if (c < d) {
     int i = grp;
-    if (i == 0 && count > 0) {
+    if (i == 0) {
       acc = first[c];
-      i = SUM_GROUPS;
+      i = GROUPS;
     }
-    for (; i + 3 * SUM_GROUPS < count; i += 4 * SUM_GROUPS) {   // four shares' loads in flight
+    for (; i + 3 * GROUPS < count; i += 4 * GROUPS) {   // four shares' loads in flight
       float e[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) e[u] = rest[(i + u * SUM_GROUPS) * step + c];
+      for (int u = 0; u < 4; ++u) e[u] = rest[(i + u * GROUPS) * step + c];
 #pragma unroll
       for (int u = 0; u < 4; ++u) acc += e[u];
     }
-    for (; i < count; i += SUM_GROUPS) acc += rest[i * step + c];
+    for (; i < count; i += GROUPS) acc += rest[i * step + c];
   }
   s[threadIdx.x] = acc;
   __syncthreads();
-  for (int w = SUM_GROUPS / 2; w > 0; w >>= 1) {
-    if (grp < w) s[threadIdx.x] += s[threadIdx.x + 16 * w];
+  for (int w = GROUPS / 2; w > 0; w >>= 1) {
+    if (grp < w) s[threadIdx.x] += s[threadIdx.x + COLS * w];
     __syncthreads();
   }
   if (grp == 0 && c < d) st1(out + c, s[threadIdx.x]);
@@ -527,14 +527,14 @@ inline Shape shape_of(int64_t d) {
 }
 
 // workgroups of the backward and the consecutive rows each takes: three workgroups per CU of 256 lanes where there are rows
-// for them. Gate runs of up to 64 rows are not cut.
+// for them. Gate runs no longer than that are not cut.
 struct Plan { int64_t per, parts; };
 inline Plan plan_of(int64_t rows, int64_t d, int64_t gate_rows) {
   const int lpr = shape_of(d).lpr, r = lpr > WG ? 1 : WG / lpr;
   const int64_t most = lpr > 512 ? 256 : lpr > WG ? 384 : 768;
   int64_t per = (rows + most - 1) / most;
   per = (per + r - 1) / r * r;
-  if (gate_rows > 1 && gate_rows <= 64) per = (per + gate_rows - 1) / gate_rows * gate_rows;
+  if (gate_rows > 1 && gate_rows <= per) per = per / gate_rows * gate_rows;
   return Plan{per, (rows + per - 1) / per};
 }
 
@@ -681,11 +681,17 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* h, const void* y, c
     })
     const int err = launched();
     if (err) return err;
-    // a gate's runs are cut between workgroups where `per` is not a multiple of them; one run over all rows is cut once
-    const int cuts = !dgate || gr == 1 || plan.per % gr == 0 || parts == 1 ? 0 : gr >= rows ? 1 : parts - 1;
-    if (dpost || dpre || cuts)
-      hipLaunchKernelGGL(k_join_sum<T>, dim3((unsigned)((d + 15) / 16), 2 + cuts), dim3(16 * SUM_GROUPS), 0, st, a,
-                         static_cast<T*>(dpost), static_cast<T*>(dpre), parts);
+    // a gate's runs that several workgroups have a share of: none where they are not cut. One over many workgroups is summed
+    // beside the weights' sums, in groups of shares; short ones with more columns to a workgroup
+    const int64_t runs = !dgate || gr == 1 || plan.per % gr == 0 ? 0 : (rows + gr - 1) / gr;
+    const bool beside = runs > 0 && (gr >= 32 * plan.per);
+    const unsigned jobs = beside ? 2 + (unsigned)runs : 2;
+    if (dpost || dpre || beside)
+      hipLaunchKernelGGL((k_join_sum<T, 16>), dim3((unsigned)((d + 15) / 16), jobs), dim3(SUM_LANES), 0, st, a,
+                         static_cast<T*>(dpost), static_cast<T*>(dpre), parts, 0);
+    if (runs && !beside)
+      hipLaunchKernelGGL((k_join_sum<T, 256>), dim3((unsigned)((d + 255) / 256), (unsigned)runs), dim3(SUM_LANES), 0, st, a,
+                         static_cast<T*>(dpost), static_cast<T*>(dpre), parts, 2);
   })
   return launched();
 }

@@ -176,9 +176,14 @@ struct Saved {
     p[64] = make_uint4(hi2(v[8], v[9]), hi2(v[10], v[11]), hi2(v[12], v[13]), hi2(v[14], v[15]));
     p[128] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  static __device__ __forceinline__ void get(const char* block, float (&v)[16]) {
+  struct Raw { uint4 v[6]; };   // both values of a block
+  static __device__ __forceinline__ void load(const char* block, Raw& r) {
     const uint4* p = reinterpret_cast<const uint4*>(block) + ((int)threadIdx.x & 63);
-    const uint4 a = p[0], b = p[64], c = p[128];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) r.v[i] = p[64 * i];
+  }
+  static __device__ __forceinline__ void get(const Raw& r, int which, float (&v)[16]) {
+    const uint4 a = r.v[3 * which], b = r.v[3 * which + 1], c = r.v[3 * which + 2];
     const unsigned hi[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, lo[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -236,16 +241,16 @@ __device__ __forceinline__ void store_tile(T* row, int64_t p0, int64_t np, bool 
   }
 }
 
-// a(g) and a'(g): silu, or gelu in its tanh form, g s(2 sqrt(2/pi) (g + 0.044715 g^3)) (the fast exponential's error, some
-// 2^-24 of its argument, is far below the results' rounding; where the argument is large the sigmoid is 0 or 1)
-__device__ __forceinline__ void activation(float g, int act, float& a, float& da) {
+// a(g) and a'(g): silu (ACT 0), or gelu in its tanh form (1), g s(2 sqrt(2/pi) (g + 0.044715 g^3)). The fast exponential and
+// reciprocal are off by some 2^-23 |q| and 2^-23, far below the results' rounding; where |q| is large the sigmoid is 0 or 1.
+template <int ACT> __device__ __forceinline__ void activation(float g, float& a, float& da) {
   const float g2 = g * g;
-  const float q = act ? g * __builtin_fmaf(0.07135481282553433f, g2, 1.5957691216057308f) : g;
-  const float dq = act ? __builtin_fmaf(0.21406443847660298f, g2, 1.5957691216057308f) : 1.f;
-  const float s = 1.f / (1.f + __expf(-q));
+  const float q = ACT ? g * __builtin_fmaf(0.07135481282553433f, g2, 1.5957691216057308f) : g;
+  const float dq = ACT ? __builtin_fmaf(0.21406443847660298f, g2, 1.5957691216057308f) : 1.f;
+  const float s = __builtin_amdgcn_rcpf(1.f + __expf(-q));
   a = g * s;
-  da = s + a * dq * (1.f - s);
-  if (act && !(g2 < 1e4f)) da = g != g ? g : s;   // far out, where q' overflows: a is 0 or g
+  da = __builtin_fmaf(a * dq, 1.f - s, s);
+  if (ACT && !(g2 < 1e4f)) da = g != g ? g : s;   // far out, where q' overflows: a is 0 or g
 }
 
 // the order of a step: N matrix instructions, after the first of them the next step's READS (two each, so that the last
@@ -371,6 +376,18 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
   }
 
   const int64_t np = EPI == GATED ? a.p.half : a.p.size;
+  // DGATED: the saved values of the next AHEAD blocks are in flight while one is worked on (what is stored could be what is
+  // loaded, for all the compiler knows: it would load each block after the stores of the one before)
+  constexpr int AHEAD = 2, BLOCKS = FP * FQ;
+  Saved::Raw raw[AHEAD];
+  auto load_saved = [&](int n) {   // block n = j FP + i; past the result: its last one
+    const int64_t qb = min(q0 + 32 * (wq * FQ + n / FP), a.q.size - 1) >> 5, pb = min(p0 + p_row(n % FP), np - 1) >> 5;
+    Saved::load(static_cast<const char*>(a.saved) + (qb * a.saved_cols + pb) * SAVED_BLOCK, raw[n % AHEAD]);
+  };
+  if constexpr (EPI == DGATED) {
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) load_saved(n);
+  }
 #pragma unroll
   for (int j = 0; j < FQ; ++j) {
     const int64_t qt = q0 + 32 * (wq * FQ + j), q = qt + (lane & 31);
@@ -381,14 +398,19 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
         const int64_t p = p0 + p_row(i);
         if (qt >= a.q.size || p >= np) continue;   // wave-uniform
         f32x16 x, y, z;
+        auto gated = [&](auto act) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float av, da;
-          activation(acc[i][j][r], a.act, av, da);
-          z[r] = av * acc[FH + i][j][r];
-          x[r] = acc[FH + i][j][r] * da;
-          y[r] = av;
-        }
+          for (int r = 0; r < 16; ++r) {
+            const float u = acc[FH + i][j][r];
+            float av, da;
+            activation<decltype(act)::value>(acc[i][j][r], av, da);
+            z[r] = av * u;
+            x[r] = u * da;
+            y[r] = av;
+          }
+        };
+        if (a.act) gated(std::integral_constant<int, 1>());   // uniform
+        else gated(std::integral_constant<int, 0>());
         store_tile<T>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, a.out16, z);
         if (a.saved) {
           char* block = static_cast<char*>(a.saved) + ((qt >> 5) * a.saved_cols + (p >> 5)) * SAVED_BLOCK;
@@ -400,22 +422,26 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
 #pragma unroll
       for (int i = 0; i < FP; ++i) {
         const int64_t p = p0 + p_row(i);
-        if (qt >= a.q.size || p >= np) continue;   // wave-uniform
-        if constexpr (EPI == STORE) {
-          store_tile<T>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, a.out16, acc[i][j]);
-        } else if constexpr (EPI == DGATED) {
-          const char* block = static_cast<const char*>(a.saved) + ((qt >> 5) * a.saved_cols + (p >> 5)) * SAVED_BLOCK;
+        if constexpr (EPI == DGATED) {
+          const int n = j * FP + i;
+          const Saved::Raw saved = raw[n % AHEAD];
+          if (n + AHEAD < BLOCKS) load_saved(n + AHEAD);
+          if (qt >= a.q.size || p >= np) continue;   // wave-uniform
           float m[16];
           f32x16 o;
           T* row = static_cast<T*>(a.out) + q * a.ldo;
-          Saved::get(block, m);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[r] = acc[i][j][r] * m[r];
-          store_tile<T>(row, p, np, ok, a.out16, o);
-          Saved::get(block + SAVED_BLOCK / 2, m);
+          for (int which = 0; which < 2; ++which) {
+            Saved::get(saved, which, m);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[r] = acc[i][j][r] * m[r];
-          store_tile<T>(row + np, p, np, ok, a.out16, o);
+            for (int r = 0; r < 16; ++r) o[r] = acc[i][j][r] * m[r];
+            store_tile<T>(row + which * np, p, np, ok, a.out16, o);
+          }
+          continue;
+        }
+        if (qt >= a.q.size || p >= np) continue;
+        if constexpr (EPI == STORE) {
+          store_tile<T>(static_cast<T*>(a.out) + q * a.ldo, p, np, ok, a.out16, acc[i][j]);
         } else {
           float* row = static_cast<float*>(a.out) + ((int64_t)split * a.q.size + q) * a.ldo;
 #pragma unroll
@@ -589,7 +615,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T* __restrict__
     float o = v[0];
     if constexpr (PAIR == 2) {
       float da;
-      activation(v[0], act, o, da);
+      if (act) activation<1>(v[0], o, da);
+      else activation<0>(v[0], o, da);
       o *= v[1];
     }
     if (16 * m + token < t && n0 + rr < n) st1(y + (int64_t)(16 * m + token) * ldy + n0 + rr, o);
