@@ -142,19 +142,9 @@ def _dropout_torch(x, rng, site, drop):
     return torch.where(keep, _upcast(x) * s, 0.0).to(x.dtype)
 
 
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, rng, site, drop):
-        ctx.site, ctx.drop = site, drop
-        ctx.save_for_backward(rng)
-        return _dropout_launch(x, rng, site, drop)
-
-    @staticmethod
-    def backward(ctx, dy):
-        rng, = ctx.saved_tensors
-        if _launchable(dy) and _dropout_native(dy, rng):
-            return _dropout_launch(dy.contiguous(), rng, ctx.site, ctx.drop), None, None, None
-        return _dropout_torch(dy, rng, ctx.site, ctx.drop), None, None, None
+def _dropout_backward(dy, rng, site, drop):
+    """The torch form of dropout's backward, for the node (csrc/host.cpp) where that has to be torch operations."""
+    return (_dropout_torch(dy, rng, site, drop),)
 
 
 def _dropout_native(x, rng) -> bool:
@@ -170,10 +160,6 @@ def _autocast_only(x) -> bool:
         return native(x, codes=_CODES)
 
 
-def _dropout_launch(x, rng, site, drop):
-    return H.dropout(x, rng, site, drop, _CODES[x.dtype], _stream(x))
-
-
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0) -> torch.Tensor:
     """x with each element dropped with probability p (to its 65536ths; 0 returns x) and the others multiplied by 1 / (1 - p);
     what is dropped is 0, also where x is not finite. The rows of the generator are those of x's last dimension."""
@@ -184,8 +170,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor | None, site: int = 0) 
         return x
     if not _dropout_native(x, rng):
         return _dropout_torch(x, rng, site, drop)
-    x = x.contiguous()
-    return _Dropout.apply(x, rng, site, drop) if _records(x) else _dropout_launch(x, rng, site, drop)
+    return H.dropout(x.contiguous(), rng, site, drop, _CODES[x.dtype], _stream(x), _records(x))
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -212,56 +197,52 @@ def _join_torch(x, y, post, gate, pre, rng, site, drop, scale, eps):
     return h.to(x.dtype), None if pre is None else _rms_torch(h, pre, eps).to(x.dtype)
 
 
-def _join_launch(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, keep):
-    """h, n and, with `keep`, the rows' scales for a backward. Contiguous tensors."""
-    return H.join_fwd(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, _CODES[x.dtype], _stream(x), keep)
+def _norm_grad(g, v, r):
+    """The gradient of v r, r = rsqrt(mean(v^2) + eps), from that of the product g."""
+    vh = v * r
+    return r * (g - vh * (g * vh).mean(-1, keepdim=True))
 
 
-class _Join(torch.autograd.Function):
-    """(h, n): the two take their gradients into one kernel. Saves h, y and the rows' scales."""
+def _sum_like(t, like):
+    """t summed over the dimensions that `like` is broadcast over."""
+    lead = t.dim() - like.dim()
+    dims = [*range(lead), *(i for i in range(lead, t.dim()) if like.shape[i - lead] == 1 and t.shape[i] != 1)]
+    return (t.sum(dims, keepdim=True) if dims else t).reshape(like.shape)
 
-    @staticmethod
-    def forward(ctx, x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps):
-        h, n, r_post, r_pre = _join_launch(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, True)
-        ctx.args = gate_rows, site, drop, scale, eps
-        ctx.save_for_backward(h if pre is not None else None, y, post, gate, pre, r_post, r_pre, rng if drop else None)
-        ctx.set_materialize_grads(False)
-        return h, n
 
-    @staticmethod
-    def backward(ctx, dh, dn):
-        gate_rows, site, drop, scale, eps = ctx.args
-        # a saved-tensor hook may give a tensor back with other strides than it was saved with
-        h, y, post, gate, pre, r_post, r_pre, rng = _plain_rows(*ctx.saved_tensors)
-        need = ctx.needs_input_grad
-        nx, ny, npost, ngate, npre = need[0], need[1], need[2], need[3], need[5] and dn is not None
-        out = [None] * 11
-        if dh is None and dn is None:
-            return tuple(out)
-        if not _launchable(dh, dn):
-            g = dh
-            if dn is not None:
-                gh, out[5] = _again(lambda h, w: _rms_torch(_upcast(h), w, eps).to(h.dtype), [h, pre], [True, npre], dn)
-                g = gh if dh is None else dh + gh
-            out[0] = g if nx else None
-            inputs = [t for t in (y, post, gate) if t is not None]
-            asked = [n for n, t in ((ny, y), (npost, post), (ngate, gate)) if t is not None]
+def _join_backward(dh, dn, h, y, post, gate, pre, rng, site, drop, need, scale, eps):
+    """The torch form of the join's backward, for the node (csrc/host.cpp): the gradients of x, y, post, gate and pre that need's
+    bits ask for, by their formulas (not by autograd: the node is locked while it runs, and the engine would wait for it). h is the
+    forward's (the norm's gradient is formed at it)."""
+    nx, ny, npost, ngate, npre = (bool(need & b) for b in (1, 2, 4, 8, 16))
+    dt, out = y.dtype, [None] * 5
+    g = None if dh is None else _upcast(dh)
+    if dn is not None:
+        hu, dnu = _upcast(h), _upcast(dn)
+        r2 = torch.rsqrt(hu.pow(2).mean(-1, keepdim=True) + eps)
+        gn = _norm_grad(dnu * _upcast(pre), hu, r2)
+        g = gn if g is None else g + gn
+        if npre:
+            out[4] = _sum_like(dnu * (hu * r2), pre).to(dt)
+    if nx:
+        out[0] = g.to(dt)
+    t, yu = g * scale, _upcast(y)
+    if drop:
+        t = _dropout_torch(t, rng, site, drop)
+    r1 = None if post is None else torch.rsqrt(yu.pow(2).mean(-1, keepdim=True) + eps)
+    yh = yu if post is None else yu * r1
+    if ngate:
+        out[3] = _sum_like(t * yh if post is None else t * yh * _upcast(post), gate).to(dt)
+    if gate is not None:
+        t = t * _upcast(gate)
+    if npost:
+        out[2] = _sum_like(t * yh, post).to(dt)
+    if ny:
+        out[1] = (t if post is None else _norm_grad(t * _upcast(post), yu, r1)).to(dt)
+    return tuple(out)
 
-            def branch(*ts):
-                it = iter(ts)
-                return _branch_torch(next(it), None if post is None else next(it), None if gate is None else next(it), rng,
-                                     site, drop, scale, eps).to(g.dtype)
 
-            got = iter(_again(branch, inputs, asked, g))
-            out[1] = next(got)
-            out[2] = None if post is None else next(got)
-            out[3] = None if gate is None else next(got)
-            return tuple(out)
-        dh, dn = _plain_rows(None if dh is None else dh.to(y.dtype), None if dn is None else dn.to(y.dtype))
-        out[0], out[1], out[2], out[3], out[5] = H.join_bwd(
-            dh, dn, h, y, post, gate, gate_rows, pre, r_post, r_pre, rng, site, drop, scale, _CODES[y.dtype], _stream(y),
-            nx + 2 * ny + 4 * npost + 8 * ngate + 16 * npre)
-        return tuple(out)
+H.torch_forms(_dropout_backward, _join_backward)
 
 
 def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
@@ -302,9 +283,8 @@ def block_join(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor | 
             and (not drop or (type(rng) is torch.Tensor and rng.is_contiguous()))):
         return _join_torch(x, y, post_weight, gate, pre_weight, rng, site, drop, scale, eps)
     x, y, post_weight, gate, pre_weight = _plain_rows(x, y, post_weight, gate, pre_weight)   # recorded, where they copy
-    if _records(*ts):
-        return _Join.apply(x, y, post_weight, gate, gate_rows, pre_weight, rng, site, drop, scale, eps)
-    return _join_launch(x, y, post_weight, gate, gate_rows, pre_weight, rng, site, drop, scale, eps, False)[:2]
+    return H.join(x, y, post_weight, gate, gate_rows, pre_weight, rng, site, drop, scale, eps, _CODES[x.dtype], _stream(x),
+                  _records(*ts))
 
 
 # ---------------------------------------------------------------------------------------------------------------

@@ -7,11 +7,13 @@
 // The entry points' addresses come from the library the Python binding loaded (bind), so both always call the same one.
 
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <cstring>
 #include <tuple>
@@ -245,14 +247,26 @@ PyObject* host_read_buffers(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// ---- block operators: the results' allocation and the launch in one call ------------------------------------------
-const at::Tensor* tensor_of(PyObject* o) {   // None: no tensor
-  if (o == Py_None) return nullptr;
+// ---- block operators: the results' allocation and the launch in one call, and their autograd nodes ------------------
+// The nodes are C++ ones: an ordinary backward then runs without Python (a Python node's costs the engine's thread some 40 us of
+// waiting for the interpreter and calling). One that has to see torch operations -- it is itself differentiated, a dispatch mode,
+// a transform or forward mode is on, its gradients are batched or of another kind -- calls the torch form in Python.
+using OptTensor = std::optional<at::Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+OptTensor opt_tensor(PyObject* o) {   // None: no tensor
+  if (o == Py_None) return std::nullopt;
   TORCH_CHECK_TYPE(THPVariable_Check(o), "a tensor or None");
-  return &THPVariable_Unpack(o);
+  return THPVariable_Unpack(o);
 }
-void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+const at::Tensor& tensor_of(PyObject* o) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o), "a tensor");
+  return THPVariable_Unpack(o);
+}
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* ptr(const OptTensor& t) { return t ? ptr(*t) : nullptr; }
+at::Tensor or_none(const OptTensor& t) { return t ? *t : at::Tensor(); }
 PyObject* wrapped(const at::Tensor& t) {
   if (t.defined()) return THPVariable_Wrap(t);
   Py_RETURN_NONE;
@@ -267,94 +281,233 @@ double float_of(PyObject* o) {
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
   return v;
 }
-template <typename F> void launch(const char* name, bool bound, F&& f) {
-  TORCH_CHECK(bound, name, ": entry point not bound");
-  int code;
-  Py_BEGIN_ALLOW_THREADS
-  code = f();
-  Py_END_ALLOW_THREADS
+void launched(const char* name, int code) {
   TORCH_CHECK(code == 0, name, ": refused or failed to launch (code ", code, ")");
 }
-template <size_t N> PyObject* tuple_of(const at::Tensor (&ts)[N]) {
-  PyObject* out = PyTuple_New(N);
+PyObject* tuple_of(const variable_list& ts) {
+  PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
   if (!out) throw python_error();
-  for (size_t i = 0; i < N; ++i) PyTuple_SET_ITEM(out, i, wrapped(ts[i]));
+  for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(out, i, wrapped(ts[i]));
+  return out;
+}
+struct NoGil {   // the interpreter is free while this lives
+  PyThreadState* state = PyEval_SaveThread();
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
+struct Gil {
+  PyGILState_STATE state = PyGILState_Ensure();
+  ~Gil() { PyGILState_Release(state); }
+};
+
+// the backwards' torch forms, Python functions of block_ops: dropout's and the join's
+PyObject* torch_forms[2] = {nullptr, nullptr};
+
+// torch_forms[which](*tensors, *numbers) with None for undefined tensors: its tuple of `results` tensors
+variable_list torch_form(int which, const variable_list& tensors, std::initializer_list<int64_t> ints,
+                         std::initializer_list<double> floats, size_t results) {
+  Gil gil;
+  TORCH_CHECK(torch_forms[which], "the block operators' torch forms are not bound");
+  struct Ref {
+    PyObject* o;
+    ~Ref() { Py_XDECREF(o); }
+  };
+  auto fail = []() {
+    python_error e;
+    e.persist();
+    throw e;
+  };
+  Ref args{PyTuple_New(static_cast<Py_ssize_t>(tensors.size() + ints.size() + floats.size()))};
+  if (!args.o) fail();
+  Py_ssize_t n = 0;
+  for (const at::Tensor& t : tensors) PyTuple_SET_ITEM(args.o, n++, wrapped(t));
+  for (int64_t v : ints) PyTuple_SET_ITEM(args.o, n++, PyLong_FromLongLong(v));
+  for (double v : floats) PyTuple_SET_ITEM(args.o, n++, PyFloat_FromDouble(v));
+  Ref got{PyObject_CallObject(torch_forms[which], args.o)};
+  if (!got.o) fail();
+  TORCH_CHECK(PyTuple_Check(got.o) && PyTuple_GET_SIZE(got.o) == static_cast<Py_ssize_t>(results), "a torch form's results");
+  variable_list out(results);
+  for (size_t i = 0; i < results; ++i) {
+    PyObject* o = PyTuple_GET_ITEM(got.o, static_cast<Py_ssize_t>(i));
+    if (o != Py_None) out[i] = tensor_of(o);
+  }
   return out;
 }
 
-// dropout(x, rng, site, drop, dtype, stream): contiguous x
+// whether a backward with these gradients runs on the kernels, for rows of `like`'s type and device
+bool on_kernels(const variable_list& grads, const at::Tensor& like) {
+  using c10::DispatchKey;
+  if (at::GradMode::is_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+      c10::impl::tls_is_dispatch_key_included(DispatchKey::FuncTorchDynamicLayerFrontMode))
+    return false;
+  constexpr c10::DispatchKeySet other({DispatchKey::Python, DispatchKey::Batched, DispatchKey::FuncTorchBatched,
+                                       DispatchKey::FuncTorchGradWrapper, DispatchKey::Functionalize, DispatchKey::ZeroTensor,
+                                       DispatchKey::Conjugate, DispatchKey::Negative});
+  for (const at::Tensor& g : grads)
+    if (g.defined() && (g.layout() != at::kStrided || g.device() != like.device() || g.scalar_type() != like.scalar_type() ||
+                        g.sizes() != like.sizes() || g.key_set().has_any(other) || g._fw_grad(0).defined()))
+      return false;
+  return true;
+}
+at::Tensor rows_of(const at::Tensor& t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
+
+at::Tensor dropout_run(const at::Tensor& x, const at::Tensor& rng, int64_t site, int64_t drop, int64_t dtype, int64_t stream) {
+  at::Tensor out = at::empty_like(x);
+  const int64_t d = x.size(-1);
+  TORCH_CHECK(BLOCK_FN(dropout), "lbk_dropout: entry point not bound");
+  launched("lbk_dropout", BLOCK_FN(dropout)(x.data_ptr(), static_cast<const int64_t*>(rng.data_ptr()), static_cast<uint32_t>(site),
+                                            static_cast<int>(drop), out.data_ptr(), x.numel() / d, d, static_cast<int>(dtype),
+                                            reinterpret_cast<void*>(stream)));
+  return out;
+}
+
+// Both nodes launch on the stream of their forward: the engine runs a node's backward on it.
+struct DropoutNode : torch::autograd::Function<DropoutNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& rng, int64_t site, int64_t drop,
+                            int64_t dtype, int64_t stream) {
+    ctx->save_for_backward({rng});
+    ctx->saved_data["numbers"] = std::vector<int64_t>{site, drop, dtype, stream};
+    ctx->set_materialize_grads(false);
+    return dropout_run(x, rng, site, drop, dtype, stream);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(6);
+    if (!grads[0].defined()) return out;
+    const at::Tensor rng = ctx->get_saved_variables()[0];
+    const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
+    if (on_kernels(grads, grads[0]) && grads[0].is_cuda() && rng.is_contiguous())
+      out[0] = dropout_run(rows_of(grads[0]), rng, n[0], n[1], n[2], n[3]);
+    else
+      out[0] = torch_form(0, {grads[0], rng}, {n[0], n[1]}, {}, 1)[0];
+    return out;
+  }
+};
+
+variable_list join_run(const at::Tensor& x, const at::Tensor& y, const OptTensor& post, const OptTensor& gate, int64_t gate_rows,
+                       const OptTensor& pre, const OptTensor& rng, int64_t site, int64_t drop, double scale, double eps,
+                       int64_t dtype, int64_t stream, bool keep) {   // h, n, r_post, r_pre
+  const int64_t d = x.size(-1), rows = x.numel() / d;
+  const auto f32 = at::TensorOptions().dtype(at::kFloat).device(x.device());
+  variable_list t{at::empty_like(x), pre ? at::empty_like(x) : at::Tensor(),
+                  keep && post ? at::empty({rows}, f32) : at::Tensor(), keep && pre ? at::empty({rows}, f32) : at::Tensor()};
+  TORCH_CHECK(BLOCK_FN(join_fwd), "lbk_join_fwd: entry point not bound");
+  launched("lbk_join_fwd",
+           BLOCK_FN(join_fwd)(x.data_ptr(), y.data_ptr(), ptr(post), ptr(gate), gate_rows, ptr(pre),
+                              drop ? static_cast<const int64_t*>(ptr(rng)) : nullptr, static_cast<uint32_t>(site),
+                              static_cast<int>(drop), static_cast<float>(scale), static_cast<float>(eps), t[0].data_ptr(), ptr(t[1]),
+                              static_cast<float*>(ptr(t[2])), static_cast<float*>(ptr(t[3])), rows, d, static_cast<int>(dtype),
+                              reinterpret_cast<void*>(stream)));
+  return t;
+}
+
+struct JoinNode : torch::autograd::Function<JoinNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& y, const OptTensor& post,
+                               const OptTensor& gate, const OptTensor& pre, const OptTensor& rng, int64_t gate_rows, int64_t site,
+                               int64_t drop, double scale, double eps, int64_t dtype, int64_t stream) {
+    variable_list t = join_run(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, true);
+    ctx->save_for_backward({pre ? t[0] : at::Tensor(), y, or_none(post), or_none(gate), or_none(pre), t[2], t[3], or_none(rng)});
+    ctx->saved_data["numbers"] = std::vector<int64_t>{gate_rows, site, drop, dtype, stream};
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    t.resize(pre ? 2 : 1);
+    return t;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(13);
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &y = saved[1], &post = saved[2], &gate = saved[3], &pre = saved[4], &rng = saved[7];
+    const at::Tensor dh = grads[0], dn = grads.size() > 1 ? grads[1] : at::Tensor();
+    if (!dh.defined() && !dn.defined()) return out;
+    const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
+    const double scale = ctx->saved_data["scale"].toDouble(), eps = ctx->saved_data["eps"].toDouble();
+    // the tensors among the inputs are the node's edges, in order
+    size_t edge = 0;
+    const bool nx = ctx->needs_input_grad(edge++), ny = ctx->needs_input_grad(edge++);
+    const bool npost = post.defined() && ctx->needs_input_grad(edge++), ngate = gate.defined() && ctx->needs_input_grad(edge++);
+    const bool npre = pre.defined() && ctx->needs_input_grad(edge++) && dn.defined();
+    if (!on_kernels({dh, dn}, y) || !y.is_cuda()) {
+      const int64_t need = nx + 2 * ny + 4 * npost + 8 * ngate + 16 * npre;
+      variable_list got = torch_form(1, {dh, dn, saved[0], y, post, gate, pre, rng}, {n[1], n[2], need}, {scale, eps}, 5);
+      std::copy(got.begin(), got.end(), out.begin());
+      return out;
+    }
+    // a saved-tensor hook may give a tensor back with other strides than it was saved with
+    variable_list s(saved.size());
+    for (size_t i = 0; i < s.size(); ++i) s[i] = rows_of(saved[i]);
+    const at::Tensor dhr = rows_of(dh), dnr = rows_of(dn);
+    const int64_t d = y.size(-1), rows = y.numel() / d;
+    if (nx) out[0] = at::empty_like(s[1]);
+    if (ny) out[1] = at::empty_like(s[1]);
+    if (npost) out[2] = at::empty_like(s[2]);
+    if (ngate) out[3] = at::empty_like(s[3]);
+    if (npre) out[4] = at::empty_like(s[4]);
+    at::Tensor scratch;
+    if (npost || ngate || npre) {
+      TORCH_CHECK(join_scratch, "lbk_join_scratch: entry point not bound");
+      scratch = at::empty({join_scratch(rows, d, n[0])}, at::TensorOptions().dtype(at::kFloat).device(y.device()));
+    }
+    TORCH_CHECK(BLOCK_FN(join_bwd), "lbk_join_bwd: entry point not bound");
+    launched("lbk_join_bwd",
+             BLOCK_FN(join_bwd)(ptr(dhr), ptr(dnr), ptr(s[0]), s[1].data_ptr(), ptr(s[2]), ptr(s[3]), n[0], ptr(s[4]),
+                                static_cast<const float*>(ptr(s[5])), static_cast<const float*>(ptr(s[6])),
+                                n[2] ? static_cast<const int64_t*>(ptr(s[7])) : nullptr, static_cast<uint32_t>(n[1]),
+                                static_cast<int>(n[2]), static_cast<float>(scale), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(out[3]),
+                                ptr(out[4]), static_cast<float*>(ptr(scratch)), rows, d, static_cast<int>(n[3]),
+                                reinterpret_cast<void*>(n[4])));
+    return out;
+  }
+};
+
+// dropout(x, rng, site, drop, dtype, stream, record): contiguous x
 PyObject* host_dropout(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 6, "dropout(x, rng, site, drop, dtype, stream)");
-  const at::Tensor &x = *tensor_of(args[0]), &rng = *tensor_of(args[1]);
+  TORCH_CHECK_TYPE(n == 7, "dropout(x, rng, site, drop, dtype, stream, record)");
+  const at::Tensor &x = tensor_of(args[0]), &rng = tensor_of(args[1]);
   const int64_t site = int_of(args[2]), drop = int_of(args[3]), dtype = int_of(args[4]), stream = int_of(args[5]);
-  at::Tensor out = at::empty_like(x);
-  const int64_t d = x.size(-1), rows = x.numel() / d;
-  launch("lbk_dropout", BLOCK_FN(dropout), [&] {
-    return BLOCK_FN(dropout)(x.data_ptr(), static_cast<const int64_t*>(rng.data_ptr()), static_cast<uint32_t>(site),
-                             static_cast<int>(drop), out.data_ptr(), rows, d, static_cast<int>(dtype),
-                             reinterpret_cast<void*>(stream));
-  });
+  const bool record = args[6] == Py_True;
+  at::Tensor out;
+  {
+    NoGil free;
+    out = record ? DropoutNode::apply(x, rng, site, drop, dtype, stream) : dropout_run(x, rng, site, drop, dtype, stream);
+  }
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
 
-// join_fwd(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, keep): (h, n, r_post, r_pre)
-PyObject* host_join_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+// join(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, record): (h, n or None), contiguous tensors
+PyObject* host_join(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 14, "join_fwd(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, keep)");
-  const at::Tensor &x = *tensor_of(args[0]), &y = *tensor_of(args[1]);
-  const at::Tensor *post = tensor_of(args[2]), *gate = tensor_of(args[3]), *pre = tensor_of(args[5]), *rng = tensor_of(args[6]);
+  TORCH_CHECK_TYPE(n == 14, "join(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, record)");
+  const at::Tensor &x = tensor_of(args[0]), &y = tensor_of(args[1]);
+  const OptTensor post = opt_tensor(args[2]), gate = opt_tensor(args[3]), pre = opt_tensor(args[5]);
   const int64_t gate_rows = int_of(args[4]), site = int_of(args[7]), drop = int_of(args[8]), dtype = int_of(args[11]),
                 stream = int_of(args[12]);
-  const float scale = static_cast<float>(float_of(args[9])), eps = static_cast<float>(float_of(args[10]));
-  const bool keep = args[13] == Py_True;
-  const int64_t d = x.size(-1), rows = x.numel() / d;
-  const auto f32 = at::TensorOptions().dtype(at::kFloat).device(x.device());
-  at::Tensor t[4] = {at::empty_like(x), pre ? at::empty_like(x) : at::Tensor(),
-                     keep && post ? at::empty({rows}, f32) : at::Tensor(), keep && pre ? at::empty({rows}, f32) : at::Tensor()};
-  launch("lbk_join_fwd", BLOCK_FN(join_fwd), [&] {
-    return BLOCK_FN(join_fwd)(x.data_ptr(), y.data_ptr(), ptr(post), ptr(gate), gate_rows, ptr(pre),
-                              drop ? static_cast<const int64_t*>(ptr(rng)) : nullptr, static_cast<uint32_t>(site),
-                              static_cast<int>(drop), scale, eps, t[0].data_ptr(), ptr(t[1]), static_cast<float*>(ptr(t[2])),
-                              static_cast<float*>(ptr(t[3])), rows, d, static_cast<int>(dtype), reinterpret_cast<void*>(stream));
-  });
+  const OptTensor rng = drop ? opt_tensor(args[6]) : std::nullopt;
+  const double scale = float_of(args[9]), eps = float_of(args[10]);
+  const bool record = args[13] == Py_True;
+  variable_list t;
+  {
+    NoGil free;
+    t = record ? JoinNode::apply(x, y, post, gate, pre, rng, gate_rows, site, drop, scale, eps, dtype, stream)
+               : join_run(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, false);
+    t.resize(2);
+  }
   return tuple_of(t);
   END_HANDLE_TH_ERRORS
 }
 
-// join_bwd(dh, dn, h, y, post, gate, gate_rows, pre, r_post, r_pre, rng, site, drop, scale, dtype, stream, need): (dx, dy, dpost,
-// dgate, dpre), those of need's bits 1, 2, 4, 8, 16
-PyObject* host_join_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 17, "join_bwd takes 17 arguments");
-  const at::Tensor *dh = tensor_of(args[0]), *dn = tensor_of(args[1]), *h = tensor_of(args[2]), *post = tensor_of(args[4]),
-                   *gate = tensor_of(args[5]), *pre = tensor_of(args[7]), *r_post = tensor_of(args[8]),
-                   *r_pre = tensor_of(args[9]), *rng = tensor_of(args[10]);
-  const at::Tensor& y = *tensor_of(args[3]);
-  const int64_t gate_rows = int_of(args[6]), site = int_of(args[11]), drop = int_of(args[12]), dtype = int_of(args[14]),
-                stream = int_of(args[15]), need = int_of(args[16]);
-  const float scale = static_cast<float>(float_of(args[13]));
-  const int64_t d = y.size(-1), rows = y.numel() / d;
-  at::Tensor t[5] = {need & 1 ? at::empty_like(y) : at::Tensor(), need & 2 ? at::empty_like(y) : at::Tensor(),
-                     need & 4 && post ? at::empty_like(*post) : at::Tensor(),
-                     need & 8 && gate ? at::empty_like(*gate) : at::Tensor(),
-                     need & 16 && pre && dn ? at::empty_like(*pre) : at::Tensor()};
-  at::Tensor scratch;
-  if (t[2].defined() || t[3].defined() || t[4].defined()) {
-    TORCH_CHECK(join_scratch, "lbk_join_scratch: entry point not bound");
-    scratch = at::empty({join_scratch(rows, d, gate_rows)}, at::TensorOptions().dtype(at::kFloat).device(y.device()));
+// torch_forms(dropout, join): the Python functions that the nodes call where a backward has to be torch operations
+PyObject* host_torch_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2 || !PyCallable_Check(args[0]) || !PyCallable_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "torch_forms(dropout, join)");
+    return nullptr;
   }
-  launch("lbk_join_bwd", BLOCK_FN(join_bwd), [&] {
-    return BLOCK_FN(join_bwd)(ptr(dh), ptr(dn), ptr(h), y.data_ptr(), ptr(post), ptr(gate), gate_rows, ptr(pre),
-                              static_cast<const float*>(ptr(r_post)), static_cast<const float*>(ptr(r_pre)),
-                              drop ? static_cast<const int64_t*>(ptr(rng)) : nullptr, static_cast<uint32_t>(site),
-                              static_cast<int>(drop), scale, ptr(t[0]), ptr(t[1]), ptr(t[2]), ptr(t[3]), ptr(t[4]),
-                              static_cast<float*>(ptr(scratch)), rows, d, static_cast<int>(dtype),
-                              reinterpret_cast<void*>(stream));
-  });
-  return tuple_of(t);
-  END_HANDLE_TH_ERRORS
+  for (int i = 0; i < 2; ++i) {
+    Py_INCREF(args[i]);
+    Py_XDECREF(torch_forms[i]);
+    torch_forms[i] = args[i];
+  }
+  Py_RETURN_NONE;
 }
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
@@ -366,8 +519,8 @@ PyMethodDef methods[] = {
     LBK_ENTRIES(X)
 #undef X
     {"dropout", FAST(&host_dropout), METH_FASTCALL, nullptr},
-    {"join_fwd", FAST(&host_join_fwd), METH_FASTCALL, nullptr},
-    {"join_bwd", FAST(&host_join_bwd), METH_FASTCALL, nullptr},
+    {"join", FAST(&host_join), METH_FASTCALL, nullptr},
+    {"torch_forms", FAST(&host_torch_forms), METH_FASTCALL, nullptr},
     {"bind", FAST(&host_bind), METH_FASTCALL, nullptr},
     {"alias", FAST(&host_alias), METH_FASTCALL, nullptr},
     {"read_buffers", FAST(&host_read_buffers), METH_FASTCALL, nullptr},

@@ -188,3 +188,28 @@ def test_every_kernel_has_a_family():
             names |= set(re.findall(r"__global__[^;{]*?\bvoid\s+(k_\w+)\s*\(", f.read(), flags=re.S))
     assert {"k_dropout", "k_join_fwd", "k_join_bwd", "k_join_sum", "k_product", "k_split_sum", "k_few_tokens", "k_pad_rows"} <= names
     assert all(RS.family(f"void (anonymous namespace)::{n}<float, 1>(...)") != "torch / runtime" for n in names)
+
+
+@pytest.mark.parametrize("gate", [None, (6,), (2, 1, 6), (2, 3, 6)])
+@pytest.mark.parametrize("post,pre,drop", [(True, True, 20000), (False, True, 0), (True, False, 20000), (False, False, 0)])
+def test_join_backward_form(gate, post, pre, drop):
+    """The backward that a node calls where it has to be torch operations: its gradients are autograd's of the forward's torch
+    form, also with one upstream gradient missing, in fp64, and those that are not asked for are not formed."""
+    rng = torch.tensor([3, 4])
+    x, y, p, g, w = (None if s is None else rnd(s, k).requires_grad_() for k, s in enumerate(
+        ((2, 3, 6), (2, 3, 6), (6,) if post else None, gate, (6,) if pre else None)))
+    h, n = ops._join_torch(x, y, p, g, w, rng, 1, drop, 0.6, 1e-3)
+    dh, dn = rnd((2, 3, 6), 8), rnd((2, 3, 6), 9) if pre else None
+    ins = [t for t in (x, y, p, g, w) if t is not None]
+    for a, b in ((dh, dn), (None, dn), (dh, None)):
+        outs = [(o, u) for o, u in ((h, a), (n, b)) if u is not None]
+        if not outs:
+            continue
+        ref = iter(torch.autograd.grad([o for o, _ in outs], ins, [u for _, u in outs], retain_graph=True, allow_unused=True))
+        ref = [None if t is None else next(ref) for t in (x, y, p, g, w)]
+        need = 3 + 4 * post + 8 * bool(gate) + 16 * (pre and b is not None)
+        got = ops._join_backward(a, b, h, y, p, g, w, rng, 1, drop, need, 0.6, 1e-3)
+        for k, (u, v) in enumerate(zip(got, ref)):
+            assert (u is not None) == bool(need >> k & 1) and (u is None or torch.allclose(u, v, atol=1e-12)), k
+    none = ops._join_backward(dh, dn, h, y, p, g, w, rng, 1, drop, 0, 0.6, 1e-3)
+    assert none == (None,) * 5
