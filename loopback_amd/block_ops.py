@@ -26,7 +26,7 @@ import torch.nn.functional as F
 
 from . import _host as H      # the launch path (csrc/host.cpp), bound below to the library
 from . import build as _build
-from .lm_ops import _again, _launchable, _stream, _watched, native
+from .lm_ops import _stream, _watched, native
 
 ABI_VERSION = 1
 JOIN_MAX_WIDTH = 8192
@@ -69,14 +69,8 @@ def _load() -> ctypes.CDLL:
 
 
 LIB = _load()
-_FN = {name: getattr(H, name, None) for name in SIGNATURES
-       if H.bind(name, ctypes.cast(getattr(LIB, name), ctypes.c_void_p).value)}
-
-
-def _run(name: str, *args) -> None:
-    code = _FN[name](*args)
-    if code:
-        raise RuntimeError(f"{name}: refused or failed to launch (code {code})")
+for _name in SIGNATURES:
+    H.bind(_name, ctypes.cast(getattr(LIB, _name), ctypes.c_void_p).value)
 
 
 def _upcast(t: torch.Tensor) -> torch.Tensor:
@@ -242,9 +236,6 @@ def _join_backward(dh, dn, h, y, post, gate, pre, rng, site, drop, need, scale, 
     return tuple(out)
 
 
-H.torch_forms(_dropout_backward, _join_backward)
-
-
 def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
     """The consecutive rows of x that share a row of the gate: (d,), or x's dimensions with the last leading ones 1."""
     lead, gl = x.shape[:-1], gate.shape[:-1]
@@ -299,91 +290,30 @@ def _ffn_torch(x, w_gate_up, w_down, activation):
     return F.linear(a * u, w_down)
 
 
-def _operand(t, code, st):
-    """(tensor, elements between rows) of contiguous rows as the tiled products take them: the tensor itself where its
-    rows are aligned, else a copy that is."""
-    cols = t.shape[-1]
-    if cols % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t, cols
-    rows, ld = t.numel() // cols, (cols + 7) // 8 * 8
-    out = torch.empty((rows, ld), device=t.device, dtype=t.dtype)
-    _run("lbk_pad_rows", t, rows, cols, ld, out, code, st)
-    return out, ld
-
-
-def _scratch(columns, rows, summed, like):
-    n = LIB.lbk_linear_scratch(columns, rows, summed)
-    return torch.empty(n, device=like.device, dtype=torch.float32) if n else None
-
-
-def _ffn_forward(x, w_gate_up, w_down, activation, keep):
-    """y, and what the backward needs: the activations (t, n rounded up to 8), the projections' saved values, and the aligned
-    copies of x and the weights (None where they are aligned)."""
-    d, (m, n), code, st = x.shape[-1], w_down.shape, _CODES[x.dtype], _stream(x)
-    t = x.numel() // d
-    n8 = (n + 7) // 8 * 8
-    act = torch.empty((t, n8), device=x.device, dtype=x.dtype)
-    saved = torch.empty(LIB.lbk_ffn_saved_bytes(t, n), device=x.device, dtype=torch.uint8) if keep else None
-    y = torch.empty((*x.shape[:-1], m), device=x.device, dtype=x.dtype)
-    xs, wgu, wd = x, w_gate_up, w_down
-    if t <= FEW_TOKENS and not keep:
-        ldx = ldw = d
+def _ffn_backward(dy, x, w_gate_up, w_down, activation, need):
+    """The torch form of the block's backward, for the node (csrc/host.cpp), by its formulas: the gradients of x, w_gate_up and
+    w_down that need's bits ask for."""
+    dt, n = x.dtype, w_down.shape[1]
+    x2, dy2 = x.reshape(-1, x.shape[-1]), dy.reshape(-1, dy.shape[-1])
+    g, u = (_upcast(t) for t in (x2 @ w_gate_up.t()).chunk(2, dim=-1))
+    if activation == 0:
+        q, dq = g, 1.0
     else:
-        xs, ldx = _operand(x, code, st)
-        wgu, ldw = _operand(w_gate_up, code, st)
-    _run("lbk_ffn_gate_up", xs, ldx, wgu, ldw, act, n8, saved, t, d, n, activation, code, st)
-    if t <= FEW_TOKENS:
-        ldw, scratch = n, None
-    else:
-        wd, ldw = _operand(w_down, code, st)
-        scratch = _scratch(m, t, n, x)
-    _run("lbk_linear_fwd", act, n8, wd, ldw, y, m, scratch, t, n, m, code, st)
-    copies = [None if b is a else b for a, b in ((x, xs), (w_gate_up, wgu), (w_down, wd))] if keep else None
-    return y, act, saved, copies
+        q, dq = 1.5957691216057308 * (g + 0.044715 * g.pow(3)), 1.5957691216057308 * (1 + 0.134145 * g.pow(2))
+    s = torch.sigmoid(q)
+    a = g * s
+    out = [None, None, None]
+    if need & 3:
+        dact = _upcast(dy2 @ w_down)
+        dgu = torch.cat((dact * u * (s + a * dq * (1 - s)), dact * a), -1).to(dt)
+        out[0] = (dgu @ w_gate_up).reshape(x.shape) if need & 1 else None
+        out[1] = dgu.t() @ x2 if need & 2 else None
+    if need & 4:
+        out[2] = dy2.t() @ (a * u).to(dt)
+    return tuple(out)
 
 
-class _GatedFfn(torch.autograd.Function):
-    """Saves x, the weights, the activations and (saved) u a'(g) and a(g) of the projections."""
-
-    @staticmethod
-    def forward(ctx, x, w_gate_up, w_down, activation):
-        need = ctx.needs_input_grad
-        y, act, saved, copies = _ffn_forward(x, w_gate_up, w_down, activation, need[0] or need[1])
-        ctx.activation = activation
-        ctx.save_for_backward(x, w_gate_up, w_down, act if need[2] else None, saved, *(copies or (None, None, None)))
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, w_gate_up, w_down, act, saved, xs, wgu, wd = _plain_rows(*ctx.saved_tensors)
-        need = ctx.needs_input_grad
-        if not _launchable(dy):
-            fn = lambda x, g, d: _ffn_torch(x, g, d, ctx.activation)
-            return *_again(fn, [x, w_gate_up, w_down], need[:3], dy), None
-        d, (m, n), code, st = x.shape[-1], w_down.shape, _CODES[x.dtype], _stream(x)
-        t = x.numel() // d
-        dy, ld_dy = _operand(dy.to(x.dtype).contiguous(), code, st)
-        dx = dw_gate_up = dw_down = None
-        if need[0] or need[1]:
-            if saved.data_ptr() % 16:
-                saved = saved.clone()   # a saved-tensor hook's
-            ld = (2 * n + 7) // 8 * 8
-            dgu = torch.empty((t, ld), device=x.device, dtype=x.dtype)
-            wd, ldw = _operand(w_down if wd is None else wd, code, st)
-            _run("lbk_ffn_dgate_up", dy, ld_dy, wd, ldw, saved, dgu, ld, t, n, m, code, st)
-            if need[0]:
-                dx = torch.empty_like(x)
-                w, ldw = _operand(w_gate_up if wgu is None else wgu, code, st)
-                _run("lbk_linear_dx", dgu, ld, w, ldw, dx, d, _scratch(d, t, 2 * n, x), t, 2 * n, d, code, st)
-            if need[1]:
-                dw_gate_up = torch.empty_like(w_gate_up)
-                xs, ldx = _operand(x if xs is None else xs, code, st)
-                _run("lbk_linear_dw", dgu, ld, xs, ldx, _scratch(d, 2 * n, t, x), dw_gate_up, t, 2 * n, d, code, st)
-        if need[2]:
-            dw_down = torch.empty_like(w_down)
-            act, ld_act = _operand(act, code, st)
-            _run("lbk_linear_dw", dy, ld_dy, act, ld_act, _scratch(n, m, t, x), dw_down, t, m, n, code, st)
-        return dx, dw_gate_up, dw_down, None
+H.torch_forms(_dropout_backward, _join_backward, _ffn_backward)
 
 
 def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
@@ -401,6 +331,4 @@ def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, ac
             and x.numel() // x.shape[-1] <= MAX_ROWS and max(*w_gate_up.shape, *w_down.shape) <= FFN_MAX_WIDTH):
         return _ffn_torch(x, w_gate_up, w_down, code)
     x, w_gate_up, w_down = _plain_rows(x, w_gate_up, w_down)   # recorded, where they copy
-    if _records(x, w_gate_up, w_down):
-        return _GatedFfn.apply(x, w_gate_up, w_down, code)
-    return _ffn_forward(x, w_gate_up, w_down, code, False)[0]
+    return H.gated_ffn(x, w_gate_up, w_down, code, _CODES[x.dtype], _stream(x), _records(x, w_gate_up, w_down))

@@ -160,8 +160,10 @@ enum Id {
   LBK_ENTRIES(X)
 #undef X
 };
-#define BLOCK_FN(name) Entry<decltype(&lbk_##name), ID_block_##name>::fn
+#define BLOCK_FN(name) (Entry<decltype(&lbk_##name), ID_block_##name>::fn)
 int64_t (*join_scratch)(int64_t, int64_t, int64_t) = nullptr;
+int64_t (*linear_scratch)(int64_t, int64_t, int64_t) = nullptr;
+int64_t (*ffn_saved_bytes)(int64_t, int64_t) = nullptr;
 
 struct Binding { const char* name; void (*bind)(void*); };
 const Binding bindings[] = {
@@ -172,6 +174,8 @@ const Binding bindings[] = {
     LBK_ENTRIES(X)
 #undef X
     {"lbk_join_scratch", [](void* p) { join_scratch = reinterpret_cast<decltype(join_scratch)>(p); }},
+    {"lbk_linear_scratch", [](void* p) { linear_scratch = reinterpret_cast<decltype(linear_scratch)>(p); }},
+    {"lbk_ffn_saved_bytes", [](void* p) { ffn_saved_bytes = reinterpret_cast<decltype(ffn_saved_bytes)>(p); }},
 };
 
 // bind(name, address) of an entry point; False for a name this module has no builtin for
@@ -299,8 +303,8 @@ struct Gil {
   ~Gil() { PyGILState_Release(state); }
 };
 
-// the backwards' torch forms, Python functions of block_ops: dropout's and the join's
-PyObject* torch_forms[2] = {nullptr, nullptr};
+// the backwards' torch forms, Python functions of block_ops: dropout's, the join's and the feed-forward block's
+PyObject* torch_forms[3] = {nullptr, nullptr, nullptr};
 
 // torch_forms[which](*tensors, *numbers) with None for undefined tensors: its tuple of `results` tensors
 variable_list torch_form(int which, const variable_list& tensors, std::initializer_list<int64_t> ints,
@@ -333,8 +337,8 @@ variable_list torch_form(int which, const variable_list& tensors, std::initializ
   return out;
 }
 
-// whether a backward with these gradients runs on the kernels, for rows of `like`'s type and device
-bool on_kernels(const variable_list& grads, const at::Tensor& like) {
+// whether a backward with these gradients runs on the kernels, for rows of `like`'s type and device, and its shape
+bool on_kernels(const variable_list& grads, const at::Tensor& like, bool same_shape = true) {
   using c10::DispatchKey;
   if (at::GradMode::is_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
       c10::impl::tls_is_dispatch_key_included(DispatchKey::FuncTorchDynamicLayerFrontMode))
@@ -344,7 +348,7 @@ bool on_kernels(const variable_list& grads, const at::Tensor& like) {
                                        DispatchKey::Conjugate, DispatchKey::Negative});
   for (const at::Tensor& g : grads)
     if (g.defined() && (g.layout() != at::kStrided || g.device() != like.device() || g.scalar_type() != like.scalar_type() ||
-                        g.sizes() != like.sizes() || g.key_set().has_any(other) || g._fw_grad(0).defined()))
+                        (same_shape && g.sizes() != like.sizes()) || g.key_set().has_any(other) || g._fw_grad(0).defined()))
       return false;
   return true;
 }
@@ -458,6 +462,130 @@ struct JoinNode : torch::autograd::Function<JoinNode> {
   }
 };
 
+// ---- gated feed-forward block: y = (a(x Wg^T) * (x Wu^T)) Wd^T ------------------------------------------------------
+struct Ffn {   // one call's sizes
+  int64_t t, d, n, m, act, dtype, stream;
+  int dt() const { return static_cast<int>(dtype); }
+  void* st() const { return reinterpret_cast<void*>(stream); }
+};
+struct Rows {
+  at::Tensor t;
+  int64_t ld;
+};
+// contiguous rows as the tiled products take them: the tensor itself where its rows are aligned, else a copy that is
+Rows operand(const at::Tensor& t, const Ffn& f) {
+  const int64_t cols = t.size(-1), ld = (cols + 7) / 8 * 8;
+  if (cols == ld && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return {t, cols};
+  const int64_t rows = t.numel() / cols;
+  at::Tensor out = at::empty({rows, ld}, t.options());
+  launched("lbk_pad_rows", BLOCK_FN(pad_rows)(t.data_ptr(), rows, cols, ld, out.data_ptr(), f.dt(), f.st()));
+  return {out, ld};
+}
+at::Tensor scratch_of(int64_t columns, int64_t rows, int64_t summed, const at::Tensor& like) {
+  const int64_t n = linear_scratch(columns, rows, summed);
+  return n ? at::empty({n}, at::TensorOptions().dtype(at::kFloat).device(like.device())) : at::Tensor();
+}
+
+// y, the activations (rows of n rounded up to 8), the projections' saved values, and the aligned copies of x and the weights
+// that were made (undefined where there was no need); `keep`: a backward follows that needs the saved values
+variable_list ffn_run(const at::Tensor& x, const at::Tensor& wgu, const at::Tensor& wd, const Ffn& f, bool keep) {
+  TORCH_CHECK(BLOCK_FN(ffn_gate_up) && BLOCK_FN(linear_fwd) && BLOCK_FN(pad_rows) && linear_scratch && ffn_saved_bytes,
+              "lbk_ffn_*: entry points not bound");
+  const int64_t n8 = (f.n + 7) / 8 * 8;
+  at::Tensor act = at::empty({f.t, n8}, x.options()), saved;
+  if (keep) saved = at::empty({ffn_saved_bytes(f.t, f.n)}, x.options().dtype(at::kByte));
+  auto shape = x.sizes().vec();
+  shape.back() = f.m;
+  at::Tensor y = at::empty(shape, x.options());
+  const bool few = f.t <= LBK_FEW_TOKENS;   // kernels that take any alignment
+  const Rows xs = few && !keep ? Rows{x, f.d} : operand(x, f), gu = few && !keep ? Rows{wgu, f.d} : operand(wgu, f);
+  launched("lbk_ffn_gate_up", BLOCK_FN(ffn_gate_up)(xs.t.data_ptr(), xs.ld, gu.t.data_ptr(), gu.ld, act.data_ptr(), n8, ptr(saved),
+                                                    f.t, f.d, f.n, static_cast<int>(f.act), f.dt(), f.st()));
+  const Rows down = few ? Rows{wd, f.n} : operand(wd, f);
+  const at::Tensor scratch = few ? at::Tensor() : scratch_of(f.m, f.t, f.n, x);
+  launched("lbk_linear_fwd", BLOCK_FN(linear_fwd)(act.data_ptr(), n8, down.t.data_ptr(), down.ld, y.data_ptr(), f.m,
+                                                  static_cast<float*>(ptr(scratch)), f.t, f.n, f.m, f.dt(), f.st()));
+  auto copy = [](const Rows& r, const at::Tensor& t) { return r.t.is_same(t) ? at::Tensor() : r.t; };
+  return {y, act, saved, copy(xs, x), copy(gu, wgu), copy(down, wd)};
+}
+
+struct FfnNode : torch::autograd::Function<FfnNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wgu, const at::Tensor& wd, int64_t act,
+                            int64_t dtype, int64_t stream) {
+    const Ffn f{x.numel() / x.size(-1), x.size(-1), wd.size(1), wd.size(0), act, dtype, stream};
+    const bool keep = x.requires_grad() || wgu.requires_grad();
+    variable_list t = ffn_run(x, wgu, wd, f, keep);
+    ctx->save_for_backward({x, wgu, wd, wd.requires_grad() ? t[1] : at::Tensor(), t[2], t[3], t[4], t[5]});
+    ctx->saved_data["numbers"] = std::vector<int64_t>{f.t, f.d, f.n, f.m, act, dtype, stream};
+    ctx->set_materialize_grads(false);
+    return t[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(6);
+    if (!grads[0].defined()) return out;
+    variable_list s = ctx->get_saved_variables();
+    const std::vector<int64_t> v = ctx->saved_data["numbers"].toIntVector();
+    const Ffn f{v[0], v[1], v[2], v[3], v[4], v[5], v[6]};
+    const bool nx = ctx->needs_input_grad(0), ngu = ctx->needs_input_grad(1), nd = ctx->needs_input_grad(2);
+    if (!on_kernels(grads, s[0], false) || !s[0].is_cuda()) {
+      const variable_list got = torch_form(2, {grads[0], s[0], s[1], s[2]}, {f.act, nx + 2 * ngu + 4 * nd}, {}, 3);
+      std::copy(got.begin(), got.end(), out.begin());
+      return out;
+    }
+    for (at::Tensor& t : s) t = rows_of(t);   // a saved-tensor hook may give one back with other strides
+    const Rows dy = operand(rows_of(grads[0]), f);
+    auto kept = [&](int copy, int of) { return s[copy].defined() ? operand(s[copy], f) : operand(s[of], f); };
+    if (nx || ngu) {
+      at::Tensor saved = s[4];
+      if (reinterpret_cast<uintptr_t>(saved.data_ptr()) % 16) saved = saved.clone();
+      const int64_t ld = (2 * f.n + 7) / 8 * 8;
+      const at::Tensor dgu = at::empty({f.t, ld}, s[0].options());
+      const Rows down = kept(7, 2);
+      launched("lbk_ffn_dgate_up", BLOCK_FN(ffn_dgate_up)(dy.t.data_ptr(), dy.ld, down.t.data_ptr(), down.ld, saved.data_ptr(),
+                                                          dgu.data_ptr(), ld, f.t, f.n, f.m, f.dt(), f.st()));
+      if (nx) {
+        out[0] = at::empty_like(s[0]);
+        const Rows gu = kept(6, 1);
+        const at::Tensor scratch = scratch_of(f.d, f.t, 2 * f.n, dgu);
+        launched("lbk_linear_dx", BLOCK_FN(linear_dx)(dgu.data_ptr(), ld, gu.t.data_ptr(), gu.ld, out[0].data_ptr(), f.d,
+                                                      static_cast<float*>(ptr(scratch)), f.t, 2 * f.n, f.d, f.dt(), f.st()));
+      }
+      if (ngu) {
+        out[1] = at::empty_like(s[1]);
+        const Rows xs = kept(5, 0);
+        const at::Tensor scratch = scratch_of(f.d, 2 * f.n, f.t, dgu);
+        launched("lbk_linear_dw", BLOCK_FN(linear_dw)(dgu.data_ptr(), ld, xs.t.data_ptr(), xs.ld, static_cast<float*>(ptr(scratch)),
+                                                      out[1].data_ptr(), f.t, 2 * f.n, f.d, f.dt(), f.st()));
+      }
+    }
+    if (nd) {
+      out[2] = at::empty_like(s[2]);
+      const Rows act = operand(s[3], f);
+      const at::Tensor scratch = scratch_of(f.n, f.m, f.t, act.t);
+      launched("lbk_linear_dw", BLOCK_FN(linear_dw)(dy.t.data_ptr(), dy.ld, act.t.data_ptr(), act.ld,
+                                                    static_cast<float*>(ptr(scratch)), out[2].data_ptr(), f.t, f.m, f.n, f.dt(), f.st()));
+    }
+    return out;
+  }
+};
+
+// gated_ffn(x, w_gate_up, w_down, activation, dtype, stream, record): contiguous tensors
+PyObject* host_gated_ffn(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 7, "gated_ffn(x, w_gate_up, w_down, activation, dtype, stream, record)");
+  const at::Tensor &x = tensor_of(args[0]), &wgu = tensor_of(args[1]), &wd = tensor_of(args[2]);
+  const int64_t act = int_of(args[3]), dtype = int_of(args[4]), stream = int_of(args[5]);
+  const bool record = args[6] == Py_True;
+  at::Tensor y;
+  {
+    NoGil free;
+    if (record) y = FfnNode::apply(x, wgu, wd, act, dtype, stream);
+    else y = ffn_run(x, wgu, wd, {x.numel() / x.size(-1), x.size(-1), wd.size(1), wd.size(0), act, dtype, stream}, false)[0];
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 // dropout(x, rng, site, drop, dtype, stream, record): contiguous x
 PyObject* host_dropout(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -496,13 +624,13 @@ PyObject* host_join(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// torch_forms(dropout, join): the Python functions that the nodes call where a backward has to be torch operations
+// torch_forms(dropout, join, ffn): the Python functions that the nodes call where a backward has to be torch operations
 PyObject* host_torch_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 2 || !PyCallable_Check(args[0]) || !PyCallable_Check(args[1])) {
-    PyErr_SetString(PyExc_TypeError, "torch_forms(dropout, join)");
+  if (n != 3 || !PyCallable_Check(args[0]) || !PyCallable_Check(args[1]) || !PyCallable_Check(args[2])) {
+    PyErr_SetString(PyExc_TypeError, "torch_forms(dropout, join, ffn)");
     return nullptr;
   }
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 3; ++i) {
     Py_INCREF(args[i]);
     Py_XDECREF(torch_forms[i]);
     torch_forms[i] = args[i];
@@ -520,6 +648,7 @@ PyMethodDef methods[] = {
 #undef X
     {"dropout", FAST(&host_dropout), METH_FASTCALL, nullptr},
     {"join", FAST(&host_join), METH_FASTCALL, nullptr},
+    {"gated_ffn", FAST(&host_gated_ffn), METH_FASTCALL, nullptr},
     {"torch_forms", FAST(&host_torch_forms), METH_FASTCALL, nullptr},
     {"bind", FAST(&host_bind), METH_FASTCALL, nullptr},
     {"alias", FAST(&host_alias), METH_FASTCALL, nullptr},

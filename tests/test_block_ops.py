@@ -213,3 +213,14 @@ def test_join_backward_form(gate, post, pre, drop):
             assert (u is not None) == bool(need >> k & 1) and (u is None or torch.allclose(u, v, atol=1e-12)), k
     none = ops._join_backward(dh, dn, h, y, p, g, w, rng, 1, drop, 0, 0.6, 1e-3)
     assert none == (None,) * 5
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_ffn_backward_form(act):
+    """The backward that a node calls where it has to be torch operations: autograd's gradients of the torch form, in fp64."""
+    x, g, d, dy = rnd((2, 3, 5), 1).requires_grad_(), rnd((8, 5), 2).requires_grad_(), rnd((6, 4), 3).requires_grad_(), rnd((2, 3, 6), 4)
+    code = ops.ACTIVATIONS[act]
+    ref = torch.autograd.grad(ops._ffn_torch(x, g, d, code), (x, g, d), dy)
+    for need in (7, 1, 2, 4, 0):
+        for k, (a, b) in enumerate(zip(ops._ffn_backward(dy, x, g, d, code, need), ref)):
+            assert (a is not None) == bool(need >> k & 1) and (a is None or torch.allclose(a, b, atol=1e-12))

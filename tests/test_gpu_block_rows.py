@@ -319,3 +319,64 @@ def test_two_streams():
     torch.cuda.synchronize()
     for a, b in zip(alone, got):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_hooks_batched_gradients_and_modes():
+    """Saved tensors that a hook gives back strided or unaligned; batched gradients and a dispatch mode take torch's operations."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from loopback_amd import block_ops as ops
+    args = [rnd(s, torch.float32, k) for k, s in enumerate(((3, 5, 40), (3, 5, 40), (40,), (3, 1, 40), (40,)))]
+    u, v, rng = rnd((3, 5, 40), torch.float32, 8), rnd((3, 5, 40), torch.float32, 9), rng_of(2)
+    leaf = lambda: [a.clone().requires_grad_() for a in args]
+    call = lambda x, y, post, gate, pre: ops.block_join(x, y, post_weight=post, gate=gate, scale=0.5, dropout=0.2, rng=rng,
+                                                        pre_weight=pre)
+    ins = leaf()
+    outs = call(*ins)
+    want = torch.autograd.grad(outs, ins, (u, v), retain_graph=True)
+    strided = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1) if t.dim() > 1 else t
+    for unpack in (strided, unaligned):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+            other = call(*ins)
+        for a, b in zip(torch.autograd.grad(other, ins, (u, v)), want):
+            assert (a - b).norm() <= 1e-6 * b.norm()
+    got = torch.autograd.grad(outs, ins, (torch.stack((u, 2 * u)), torch.stack((v, 2 * v))), is_grads_batched=True, retain_graph=True)
+    for a, b in zip(got, want):
+        assert (a[0] - b).norm() <= 1e-5 * b.norm() and (a[1] - 2 * b).norm() <= 1e-5 * b.norm()
+
+    class Count(TorchDispatchMode):
+        n = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            Count.n += 1
+            return func(*args, **(kwargs or {}))
+
+    with Count():
+        seen = torch.autograd.grad(outs, ins, (u, v), retain_graph=True)
+        h, _ = call(*args)
+    assert Count.n > 20 and (h - outs[0]).abs().max() <= 1e-6 * h.abs().max()
+    for a, b in zip(seen, want):
+        assert (a - b).norm() <= 1e-5 * b.norm()
+    x = rnd((6, 40), torch.float32, 10).requires_grad_()
+    y = ops.dropout(x, 0.5, rng)
+    g, = torch.autograd.grad(y, x, torch.ones(2, 6, 40, device=DEV), is_grads_batched=True)
+    assert torch.equal(g[0] != 0, ops.keep_mask((6, 40), 0.5, rng)) and torch.equal(g[0], g[1])
+
+
+def test_generator_changed_in_place():
+    """A generator that was changed before the backward of a call that took it is refused by autograd."""
+    from loopback_amd import block_ops as ops
+    x, rng = rnd((6, 40), torch.float32, 1).requires_grad_(), rng_of(3)
+    y = ops.dropout(x, 0.5, rng)
+    rng[1] += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_only_on_the_current_gpu(monkeypatch):
+    """Tensors of a GPU that is not the current one run the torch form."""
+    from loopback_amd import block_ops as ops
+    x = rnd((6, 40), torch.float32, 1)
+    want = ops.dropout(x, 0.5, rng_of(3)), ops.block_join(x, x)[0]
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: x.device.index + 1)
+    monkeypatch.setattr(ops, "H", None)   # a launch would fail
+    assert torch.equal(ops.dropout(x, 0.5, rng_of(3)), want[0]) and torch.equal(ops.block_join(x, x)[0], want[1])

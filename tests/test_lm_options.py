@@ -119,13 +119,11 @@ def test_training_step_on_the_kernels(dtype, options, monkeypatch):
         loss = m(ids)
         return loss.detach().double(), [g.double() for g in torch.autograd.grad(64.0 * loss, list(m.parameters()))]
 
-    nodes, real, H = [], block_ops._GatedFfn.apply, block_ops.H
+    nodes, H = [], block_ops.H
     counted = lambda name: lambda *a: nodes.append((name, a[-1])) or getattr(H, name)(*a)
-    native_path = type("Counted", (), {"join": staticmethod(counted("join")), "dropout": staticmethod(counted("dropout"))})
-    monkeypatch.setattr(block_ops, "H", native_path)
-    monkeypatch.setattr(block_ops._GatedFfn, "apply", lambda *a: nodes.append(("ffn", True)) or real(*a))
+    monkeypatch.setattr(block_ops, "H", type("Counted", (), {n: staticmethod(counted(n)) for n in ("join", "dropout", "gated_ffn")}))
     got = step(model)
-    assert set(nodes) == {(n, True) for n, on in (("ffn", "ffn" in options), ("join", len(options) > 1 or "ffn" not in options),
+    assert set(nodes) == {(n, True) for n, on in (("gated_ffn", "ffn" in options), ("join", len(options) > 1 or "ffn" not in options),
                                                   ("dropout", "dropout" in options)) if on}
     again = step(model)
     assert got[0] == again[0] and all(torch.equal(a, b) for a, b in zip(got[1], again[1]))
