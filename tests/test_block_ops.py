@@ -224,3 +224,28 @@ def test_ffn_backward_form(act):
     for need in (7, 1, 2, 4, 0):
         for k, (a, b) in enumerate(zip(ops._ffn_backward(dy, x, g, d, code, need), ref)):
             assert (a is not None) == bool(need >> k & 1) and (a is None or torch.allclose(a, b, atol=1e-12))
+
+
+def test_watched_calls_are_torch_operations():
+    """torch.compile in one graph, make_fx and fake tensors see torch operations, with the eager results."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    rng = torch.tensor([3, 4])
+    x, w, gu, d = rnd((2, 3, 8), 1, torch.float32), rnd((8,), 2, torch.float32), rnd((12, 8), 3, torch.float32), rnd((8, 6), 4, torch.float32)
+
+    def fn(x):
+        h, n = ops.block_join(x, ops.gated_ffn(x, gu, d), post_weight=w, gate=w, scale=0.5, dropout=0.3, rng=rng, site=2, pre_weight=w)
+        return h + ops.dropout(n, 0.2, rng, site=3)
+
+    ref = fn(x)
+    torch._dynamo.reset()
+    assert torch.allclose(torch.compile(fn, backend="eager", fullgraph=True)(x), ref, atol=1e-6)
+    assert torch.allclose(make_fx(fn)(rnd((2, 3, 8), 7, torch.float32))(x), ref, atol=1e-6)
+    with FakeTensorMode():
+        y = torch.empty(2, 3, 64, device="cuda", dtype=torch.bfloat16)
+        v, r = torch.empty(64, device="cuda", dtype=torch.bfloat16), torch.empty(2, device="cuda", dtype=torch.int64)
+        h, n = ops.block_join(y, y, post_weight=v, pre_weight=v, dropout=0.1, rng=r)
+        assert h.shape == n.shape == y.shape and ops.dropout(y, 0.1, r).device == y.device
+        assert ops.gated_ffn(y, torch.empty(96, 64, device="cuda", dtype=torch.bfloat16),
+                             torch.empty(32, 48, device="cuda", dtype=torch.bfloat16)).shape == (2, 3, 32)
+    assert torch.func.vmap(fn)(x[None]).shape == (1, 2, 3, 8)

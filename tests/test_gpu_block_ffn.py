@@ -75,7 +75,7 @@ def check(t, d, n, m, dtype, act="silu", place=lambda v: v, lead=None):
 
 
 @pytest.mark.parametrize("t,d,n,m", [(1, 1, 1, 1), (1, 8, 8, 8), (2, 64, 32, 64), (33, 65, 31, 63), (65, 128, 96, 40),
-                                     (128, 192, 128, 192), (129, 200, 264, 136), (257, 72, 520, 328), (300, 1001, 333, 77)])
+                                     (128, 192, 128, 192), (5, 1001, 333, 77), (31, 135, 1000, 129), (129, 200, 264, 136), (257, 72, 520, 328), (300, 1001, 333, 77)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_sizes(t, d, n, m, dtype, act):
@@ -200,3 +200,23 @@ def test_not_finite_rows_stay_alone():
         rest = [i for i in range(t) if i > 2]
         assert torch.equal(y[rest], y2[rest]) and torch.equal(dx[rest], dx2[rest]) and torch.equal(y[0], y2[0])
         assert y2[2].isnan().all() and not dx2[0].isfinite().all()
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last tokens' results and gradients are those of a call on them alone, to the
+    roundings of two orders of summation (a step of the result each)."""
+    from loopback_amd import block_ops as ops
+    t, d, n = 262200, 64, 4104
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, gu, wd, dy = (torch.randn(s, device=DEV, generator=g, dtype=torch.bfloat16) * k for s, k in
+                     (((t, d), 1.0), ((2 * n, d), 0.125), ((d, n), 0.02), ((t, d), 1.0)))
+    print(f"case ffn {t}x{d}x{n}", flush=True)
+
+    def run(a, b):
+        a = a.clone().requires_grad_()
+        y = ops.gated_ffn(a, gu, wd)
+        return y.detach(), torch.autograd.grad(y, a, b)[0]
+
+    got, ref = run(x, dy), run(x[-300:], dy[-300:])
+    for a, b in zip(got, ref):
+        assert (a[-300:] - b).float().norm() <= 2.0 ** -7 * b.float().norm()

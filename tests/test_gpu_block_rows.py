@@ -380,3 +380,48 @@ def test_only_on_the_current_gpu(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: x.device.index + 1)
     monkeypatch.setattr(ops, "H", None)   # a launch would fail
     assert torch.equal(ops.dropout(x, 0.5, rng_of(3)), want[0]) and torch.equal(ops.block_join(x, x)[0], want[1])
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last rows' results and gradients are those of a call on them alone; dropout's
+    mask there is the generator's."""
+    import numpy as np
+    from loopback_amd import block_ops as ops
+    rows, d = 262160, 8200
+    print(f"case rows {rows}x{d}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn((rows, d), device=DEV, generator=g, dtype=torch.bfloat16)
+    out, last = ops.dropout(x, 0.25, rng_of(3), site=5), rows - 1
+    u, m = np.uint64, np.uint64(0xFFFFFFFF)
+    seed, step = (int(v) for v in rng_of(3).cpu())
+    c = [np.arange(d // 8, dtype=u), np.full(d // 8, last, u), np.full(d // 8, 5, u), np.full(d // 8, step, u)]
+    k = [u(seed & 0xFFFFFFFF), u((seed >> 32) & 0xFFFFFFFF)]
+    for _ in range(10):
+        a, b = c[0] * u(0xD2511F53), c[2] * u(0xCD9E8D57)
+        c = [(b >> u(32)) ^ c[1] ^ k[0], b & m, (a >> u(32)) ^ c[3] ^ k[1], a & m]
+        k = [(k[0] + u(0x9E3779B9)) & m, (k[1] + u(0xBB67AE85)) & m]
+    keep = np.stack(c, -1).astype("<u4").view("<u2").reshape(d) >= 16384
+    keep = torch.from_numpy(keep).to(DEV)
+    assert torch.equal(out[last], torch.where(keep, x[last].float() * (65536 / 49152), 0.0).bfloat16())
+    x, w = x.view(-1)[:rows * 8192].view(rows, 8192), rnd((8192,), torch.bfloat16, 2)
+    del out
+
+    def run(v):
+        v = v.clone().requires_grad_()
+        h, n = ops.block_join(v, v, post_weight=w, pre_weight=w)
+        return h.detach(), n.detach(), torch.autograd.grad((h, n), v, (h.detach(), n.detach()))[0]
+
+    for a, b in zip(run(x), run(x[-50:])):
+        assert torch.equal(a[-50:], b)
+
+
+def test_anomaly_mode():
+    """The nodes under autograd's anomaly detection: a clean pass, and a NaN gradient that is found (in the first node it reaches)."""
+    from loopback_amd import block_ops as ops
+    x, w = rnd((4, 40), torch.float32, 1).requires_grad_(), rnd((40,), torch.float32, 2).requires_grad_()
+    with torch.autograd.set_detect_anomaly(True, check_nan=True):
+        h, n = ops.block_join(ops.dropout(x, 0.5, rng_of(1)), x, post_weight=w, pre_weight=w)
+        (h.sum() + n.sum()).backward()
+        h, n = ops.block_join(x, x, post_weight=w, pre_weight=w)
+        with pytest.raises(RuntimeError, match="returned nan values"):
+            (h.sum() * float("nan")).backward()
