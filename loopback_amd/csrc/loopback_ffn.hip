@@ -8,11 +8,17 @@
 //
 // Operands go through v_mfma_f32_32x32x16 (bf16 or fp16): lane l holds row (P) or column (Q) l mod 32 at k = 8 (l / 32) .. + 8;
 // of the 32 x 32 result it holds column l mod 32 and, in register r, row 4 (l / 32) + r mod 4 + 8 (r / 4): four consecutive p of
-// one q, which one exchange of lane halves makes eight (a 16-byte store). Tiles of 32 or 64 k sit in LDS twice, the next one filled
+// one q, which one exchange of lane halves makes eight (a 16-byte store). Tiles of 64 k sit in LDS twice, the next one filled
 // by direct global -> LDS loads while one is worked on. Such loads write 64 lanes' 16 bytes in order, so the tiles have no
 // padding; instead the 16-byte pieces of a row are permuted: ROW tiles (128-byte rows) by (row / 2) mod 8, so that 16 rows at
 // one k cover the 64 banks once, COL tiles (rows of the tile's width) by 4 (k mod 4), so that the four rows a transposing read
-// (ds_read_b64_tr_b16) takes together do.
+// (ds_read_b64_tr_b16) takes together do (SQ_LDS_BANK_CONFLICT: 0 for both kinds).
+//
+// The matrix cores bound it: 2 q p k operations, and a 256 x 256 tile reads 64 KiB for each 64 k it multiplies. 8192 x 2048 x 5632
+// in bf16: gate and up projection 319 us (1186 TFLOP/s; a library's product without the activation 349), down 145 us (121),
+// input gradient 278 us (273), weight gradients 347 and 160 us (343 and 176). Smaller tiles with more workgroups to a CU took
+// 5-11 % longer, 32 k per tile in three or four buffers 4-15 % (a barrier for half the work), four waves of 128 x 128 12-17 %,
+// a raised wave priority around the products 0-14 %; reloading one tile throughout, without memory traffic, only 3-5 % less.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -24,6 +30,8 @@
 #include "device_io.h"
 
 namespace {
+
+constexpr int BK = 64;   // k per tile
 
 enum Kind { ROW, COL };
 enum Epi { STORE, PARTIAL, GATED, DGATED };
@@ -54,13 +62,13 @@ struct Operand {   // 16-byte aligned, ld a multiple of 8; COL: every row's ld e
   int64_t half;    // GATED: indices per half (tile indices past its middle are those of the second half); else 0
 };
 
-template <typename T, Kind KIND, int ROWS, int BK, int LANES, bool GATED_P> struct Tile {
+template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile {
   static constexpr int PER = (KIND == ROW ? BK : ROWS) / 8;   // 16-byte pieces per row of the tile
   static constexpr int PASSES = ROWS * BK / 8 / LANES, STEP = LANES / PER;
-  static_assert((BK == 64 || BK == 32) && ROWS * BK / 8 % LANES == 0 && STEP % (KIND == ROW ? 16 : 4) == 0 &&
+  static_assert(ROWS * BK / 8 % LANES == 0 && STEP % (KIND == ROW ? 16 : 4) == 0 &&
                 (KIND == ROW || ROWS >= 128) && (!GATED_P || PASSES % 2 == 0), "tile shape");
 
-  static __device__ __forceinline__ int swizzle(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
+  static __device__ __forceinline__ int swizzle(int r) { return (r >> 1) & 7; }
   // this lane's piece of pass i: row i STEP + tid / PER, stored as piece tid % PER, which is piece `piece()` of memory's row
   static __device__ __forceinline__ int row(int i) { return i * STEP + (int)threadIdx.x / PER; }
   static __device__ __forceinline__ int piece() {
@@ -157,7 +165,8 @@ template <typename T, Kind KIND, int ROWS, int BK, int LANES, bool GATED_P> stru
 // activation's gradient is multiplied by. Kept as the upper 24 bits of their fp32 values: 16 would double the input and
 // gate/up weight gradients' squared error (three roundings of 2^-9 instead of two). In blocks of 32 tokens x 32 columns in the
 // matrix cores' own order, so both kernels move them as whole vectors: 64 lanes x 16 values, upper 16 bits as two planes of
-// eight values a lane, then the next eight bits: 3072 bytes for each of the two.
+// eight values a lane, then the next eight bits: 3072 bytes for each of the two. Stores and loads past the caches: gate and up
+// projection of 8192 x 2048 x 5632 382 -> 342 us, the gradient that reads them 266 -> 238.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int64_t SAVED_BLOCK = 6144;
 struct Saved {
@@ -272,11 +281,13 @@ template <int N, int READS, int LOADS, int M = 0> __device__ __forceinline__ voi
   }
 }
 
-template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, int BK, Epi EPI>
-__global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP * FQ > 8 ? 1 : 2))) void k_product(const Product a) {
+// WP x WQ waves of FP x FQ results of 32 x 32. Two waves to a SIMD: eight of 256 x 256 (128 KiB of LDS, one workgroup to a CU), or
+// two workgroups of four of 128 x 128; which one: tiling_of.
+template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI>
+__global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(2))) void k_product(const Product a) {
   constexpr int LANES = WP * WQ * 64, TP = WP * FP * 32, TQ = WQ * FQ * 32;
-  typedef Tile<T, KP, TP, BK, LANES, EPI == GATED> PT;
-  typedef Tile<T, KQ, TQ, BK, LANES, false> QT;
+  typedef Tile<T, KP, TP, LANES, EPI == GATED> PT;
+  typedef Tile<T, KQ, TQ, LANES, false> QT;
   // objects of their own: what is read is seen not to be what is being filled
   __shared__ __align__(16) T sp0[TP * BK], sq0[TQ * BK], sp1[TP * BK], sq1[TQ * BK];
   // XCD x (workgroups go to XCDs in turn) takes `per` consecutive tiles, in groups of eight rows of tiles: the tiles worked
@@ -464,7 +475,8 @@ __global__ __launch_bounds__(WP * WQ * 64) __attribute__((amdgpu_waves_per_eu(FP
   }
 }
 
-// out [nq][ldo] = round(sum of the splits' products [nq][ldp], in order), four columns per lane
+// out [nq][ldo] = round(sum of the splits' products [nq][ldp], in order: the same bits every time), four columns per lane. Its
+// reads bound it, mostly out of the caches: 9.7 us for the weight gradients of 16384 x 768 x 2048.
 template <typename T>
 __global__ __launch_bounds__(256) void k_split_sum(const float* __restrict__ part, int splits, int64_t nq, int64_t np, int64_t ldp,
                                                    T* __restrict__ out, int64_t ldo, bool al) {
@@ -498,7 +510,8 @@ __global__ __launch_bounds__(256) void k_split_sum(const float* __restrict__ par
   }
 }
 
-// out [rows][ld] = x [rows][cols], zeros past the columns, for operands whose rows are not aligned; eight columns per lane
+// out [rows][ld] = x [rows][cols], zeros past the columns, for operands whose rows are not aligned; eight columns per lane. 4 to 6 us for each
+// operand of 1001 x 1001 x 2731; the products on unaligned rows, element by element, took 708 us a pass there and take 217 so.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pad_rows(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ld,
                                                   T* __restrict__ out) {
@@ -523,7 +536,8 @@ __global__ __launch_bounds__(256) void k_pad_rows(const T* __restrict__ x, int64
 // few tokens (a serving step): y = x W^T, or the gated pair, for up to 16 MT tokens. The weights' stream bounds it, so they go
 // from memory to the matrix cores' registers (v_mfma_f32_16x16x32: lane l has row l mod 16): a workgroup takes 16 rows (of the
 // gate's and of the up projection's), its waves the columns in turns of 128, each load instruction 64 consecutive bytes of 16
-// rows, all loads of a few turns in flight together. The waves' sums meet in LDS, in order. Any alignment.
+// rows, all loads of a few turns in flight together. The waves' sums meet in LDS, in order. Any alignment. One token at 2048 x
+// 5632 in bf16: 13 us for gate and up projection (3.6 TB/s of weights) and 9 us for the down projection (2.6); 32 tokens 19 and 23.
 // ---------------------------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 mfma16(bf16_t, uint4 a, uint4 b, f32x4 c) {
@@ -641,14 +655,14 @@ constexpr int64_t MAX_SIZE = 0x7fffffff;   // of one dimension
 constexpr int64_t MAX_LD = 1 << 22;        // rows of memory up to which a tile's byte offsets fit 32 bits (256 rows)
 
 template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI> int launch_tiles(Product a, hipStream_t st) {
-  constexpr int BK = 64, TP = (EPI == GATED ? WP * FP * 16 : WP * FP * 32), TQ = WQ * FQ * 32;
+  constexpr int TP = (EPI == GATED ? WP * FP * 16 : WP * FP * 32), TQ = WQ * FQ * 32;
   const int64_t np = EPI == GATED ? a.p.half : a.p.size;
   const int64_t tp = (np + TP - 1) / TP, tq = (a.q.size + TQ - 1) / TQ, tiles = tp * tq;
   if (tiles * a.splits > 0xfffffff) return LDR_E_SHAPE;
   a.tiles_p = (int)tp;
   a.tiles = (int)tiles;
   a.per = (int)((tiles * a.splits + 7) / 8);
-  hipLaunchKernelGGL((k_product<T, KP, KQ, WP, WQ, FP, FQ, BK, EPI>), dim3((unsigned)(8 * a.per)), dim3(WP * WQ * 64), 0, st, a);
+  hipLaunchKernelGGL((k_product<T, KP, KQ, WP, WQ, FP, FQ, EPI>), dim3((unsigned)(8 * a.per)), dim3(WP * WQ * 64), 0, st, a);
   return launched();
 }
 
@@ -709,7 +723,7 @@ int few(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t
                                      static_cast<const T*>(x), ldx, static_cast<const T*>(w), ldw, static_cast<T*>(y), ldy, (int)t, n,  \
                                      k, act)
   // waves that share a workgroup's columns: more where there are few workgroups; as many turns' loads in flight as each has, up
-  // to what its registers hold
+  // to what its registers hold (one token at 2048 x 5632: 13 and 9 us; with one turn's 21 and 14)
   constexpr int MANY = PAIR > 1 ? 8 : 16, MOST = MT > 1 ? 2 : PAIR > 1 ? 4 : 3;
   const int64_t turns = k / 128;
   if (blocks >= 256) {
