@@ -20,6 +20,7 @@ import argparse
 import csv
 import json
 import os
+import re
 import sys
 
 FAMILIES = [("k_read_fwd", "read_fwd"), ("k_read_online", "read_fwd_online"), ("k_bwd1", "read_bwd1"), ("k_dv_assemble", "dv_assemble"),
@@ -141,7 +142,8 @@ def stats_table(path, top):
     lines = [f"rocprofv3 --stats over the whole run ({total / 1e6:.1f} ms of kernel time in all; names shortened):",
              "", "| kernel | calls | total ms | average us | % |", "|---|---|---|---|---|"]
     for r in st[:top]:
-        name = r["Name"].replace("(anonymous namespace)::", "").replace("void ", "").split("(")[0][:80]
+        name = r["Name"].replace("(anonymous namespace)::", "").replace("void ", "")
+        name = re.sub(r"\(\w+\)(?=\d)", "", name).split("(")[0][:80]   # an enumerator among the template's arguments: (Kind)1
         lines.append(f"| `{name}` | {r['Calls']} | {float(r['TotalDurationNs']) / 1e6:.2f} | "
                      f"{float(r['AverageNs']) / 1e3:.1f} | {r['Percentage']} |")
     fams = {}
