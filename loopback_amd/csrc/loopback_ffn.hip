@@ -11,12 +11,12 @@
 // one q, which one exchange of lane halves makes eight (a 16-byte store). Tiles of 64 k sit in LDS twice, the next one filled
 // by direct global -> LDS loads while one is worked on. Such loads write 64 lanes' 16 bytes in order, so the tiles have no
 // padding; instead the 16-byte pieces of a row are permuted: ROW tiles (128-byte rows) by (row / 2) mod 8, so that 16 rows at
-// one k cover the 64 banks once, COL tiles (rows of the tile's width) by 4 (k mod 4), so that the four rows a transposing read
+// one k cover the 64 banks once, COL tiles (rows of the tile's width) by 4 (k mod 4), or 4 (k / 2 mod 2), so that the four rows a transposing read
 // (ds_read_b64_tr_b16) takes together do (SQ_LDS_BANK_CONFLICT: 0 for both kinds).
 //
 // The matrix cores bound it: 2 q p k operations, and a 256 x 256 tile reads 64 KiB for each 64 k it multiplies. 8192 x 2048 x 5632
-// in bf16: gate and up projection 319 us (1186 TFLOP/s; a library's product without the activation 349), down 145 us (121),
-// input gradient 278 us (273), weight gradients 347 and 160 us (343 and 176). Smaller tiles with more workgroups to a CU took
+// in bf16: gate and up projection 314 us (1202 TFLOP/s; a library's product without the activation 352), down 151 us (125),
+// input gradient 289 us (273), weight gradients 317 and 157 us (339 and 171). Smaller tiles with more workgroups to a CU took
 // 5-11 % longer, 32 k per tile in three or four buffers 4-15 % (a barrier for half the work), four waves of 128 x 128 12-17 %,
 // a raised wave priority around the products 0-14 %; reloading one tile throughout, without memory traffic, only 3-5 % less.
 
@@ -64,16 +64,18 @@ struct Operand {   // 16-byte aligned, ld a multiple of 8; COL: every row's ld e
 
 template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile {
   static constexpr int PER = (KIND == ROW ? BK : ROWS) / 8;   // 16-byte pieces per row of the tile
-  static constexpr int PASSES = ROWS * BK / 8 / LANES, STEP = LANES / PER;
-  static_assert(ROWS * BK / 8 % LANES == 0 && STEP % (KIND == ROW ? 16 : 4) == 0 &&
-                (KIND == ROW || ROWS >= 128) && (!GATED_P || PASSES % 2 == 0), "tile shape");
+  static constexpr int PASSES = ROWS * BK / 8 / LANES;
+  static_assert(ROWS * BK / 8 % LANES == 0 && (KIND == ROW ? LANES / PER % 16 == 0 : ROWS % 64 == 0 && ROWS >= 128) &&
+                (!GATED_P || PASSES % 2 == 0), "tile shape");
 
   static __device__ __forceinline__ int swizzle(int r) { return (r >> 1) & 7; }
-  // this lane's piece of pass i: row i STEP + tid / PER, stored as piece tid % PER, which is piece `piece()` of memory's row
-  static __device__ __forceinline__ int row(int i) { return i * STEP + (int)threadIdx.x / PER; }
-  static __device__ __forceinline__ int piece() {
-    const int r = (int)threadIdx.x / PER, c = (int)threadIdx.x % PER;
-    return KIND == ROW ? c ^ swizzle(r) : c ^ (4 * (r & 3));
+  // COL: the block of 32 columns that row r has in the place of block 0 (rows of 192 columns begin 32 banks apart by themselves)
+  static __device__ __forceinline__ int block(int r) { return ROWS % 128 ? (r >> 1) & 1 : r & 3; }
+  // this lane's piece of pass i: the tile's row it is in, and which piece of memory's row is stored there
+  static __device__ __forceinline__ int row(int i) { return (int)((i * LANES + threadIdx.x) / PER); }
+  static __device__ __forceinline__ int piece(int i) {
+    const int r = row(i), c = (int)((i * LANES + threadIdx.x) % PER);
+    return KIND == ROW ? c ^ swizzle(r) : c ^ (4 * block(r));
   }
   // the operand's index of tile row r (ROW) from the tile's first index i0; past the end: the last one
   static __device__ __forceinline__ int64_t index(const Operand& o, int64_t i0, int r) {
@@ -94,13 +96,13 @@ template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile 
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
         const int r = GATED_P && i >= PASSES / 2 ? row(i - PASSES / 2) : row(i);
-        off[i] = 2 * ((uint32_t)min(r, last) * (uint32_t)o.ld + 8 * piece());
+        off[i] = 2 * ((uint32_t)min(r, last) * (uint32_t)o.ld + 8 * piece(i));
       }
     } else {
       base = b + k0 * o.ld + i0;
       const int last = (int)min((o.size - 1 - i0) & ~(int64_t)7, (int64_t)ROWS);
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) off[i] = 2 * ((uint32_t)row(i) * (uint32_t)o.ld + min(8 * piece(), last));
+      for (int i = 0; i < PASSES; ++i) off[i] = 2 * ((uint32_t)row(i) * (uint32_t)o.ld + min(8 * piece(i), last));
     }
     step = KIND == ROW ? BK : BK * o.ld;
   }
@@ -123,11 +125,11 @@ template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile 
       const T* p;
       int64_t left;   // elements of this piece that exist
       if (KIND == ROW) {
-        p = base + index(o, i0, row(i)) * o.ld + k0 + 8 * piece();
-        left = k1 - k0 - 8 * piece();
+        p = base + index(o, i0, row(i)) * o.ld + k0 + 8 * piece(i);
+        left = k1 - k0 - 8 * piece(i);
       } else {
-        p = base + (k0 + row(i)) * o.ld + i0 + 8 * piece();
-        left = k0 + row(i) < k1 ? o.size - i0 - 8 * piece() : 0;
+        p = base + (k0 + row(i)) * o.ld + i0 + 8 * piece(i);
+        left = k0 + row(i) < k1 ? o.size - i0 - 8 * piece(i) : 0;
       }
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (left >= 8) {
@@ -150,7 +152,7 @@ template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile 
     } else {
       typedef __attribute__((address_space(3))) s16x4* lds4;
       const int j = lane & 15, kr = j >> 2;
-      const int col = 32 * ((r0 >> 5) ^ kr) + (lane & 16) + 4 * (j & 3);
+      const int col = 32 * ((r0 >> 5) ^ block(kr)) + (lane & 16) + 4 * (j & 3);
       const T* p = lds + (16 * s + 8 * h + kr) * ROWS + col;
       const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(const_cast<T*>(p)));
       const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(const_cast<T*>(p + 4 * ROWS)));
@@ -666,31 +668,43 @@ template <typename T, Kind KP, Kind KQ, int WP, int WQ, int FP, int FQ, Epi EPI>
   return launched();
 }
 
-// Which tiles, and in how many splits of k, by the time they take: 256 x 256 ones of eight waves, one to a CU, 1.65 us per 64
-// k; 128 x 128 ones of four waves, two to a CU, 1.08 us (8192 x 2048 x 5632: 157-390 us against 173-470 for the six
-// products); 5 us around them; splits are written and read as fp32 (2 us for the launch that adds them).
-struct Tiling { bool big; int splits; };
-inline Tiling tiling_of(int64_t np, int64_t nq, int64_t k, bool may_split) {
+// Which tiles, and in how many splits of k, by the time they take: 128 x 128 ones of four waves, two to a CU; 256 x 256 ones of
+// eight waves, one to a CU; 192 (of P) x 256 likewise, which divide some sizes better (768: 256 tiles instead of 192 at 16384
+// tokens, 50.0 -> 47.2 and 94.8 -> 90.0 us; 8192 x 2048 x 5632: 348 -> 321 and 167 -> 160 for the weight gradients, but 152 -> 200
+// for the down product). A round of tiles takes a step per 64 k, the shorter the fewer of them the GPU holds (less contention, a
+// higher clock), and what surrounds the steps; splits are written and read as fp32. The constants are a fit to 59 products
+// of sides from 250 to 16384, in bf16; over 48 others the choice is 0.9 % behind the fastest of the three in the mean, 16 % at
+// most.
+enum Shape { SMALL, BIG, WIDE };
+struct Tiling { Shape shape; int splits; };
+inline Tiling tiling_of(int64_t np, int64_t nq, int64_t k, bool plain) {   // plain: may be split, and of any shape
   constexpr int64_t CUS = 256;
-  Tiling best{false, 1};
+  constexpr struct { double least, fixed, filled, around; } US[] = {{0.5, 0.43, 0.66, 4.3}, {1.0, 0.48, 1.1, 8.6}, {1.0, 0.46, 0.74, 6.7}};
+  Tiling best{SMALL, 1};
   double least = 1e30;
-  for (int big = 0; big < 2; ++big) {
-    const int64_t t = big ? 256 : 128, tiles = ((np + t - 1) / t) * ((nq + t - 1) / t), at_once = big ? CUS : 2 * CUS;
-    // a round that does not fill the GPU is faster (less contention, a higher clock): 352 large tiles of 128 steps 335 us
-    auto step = [&](double f) { return big ? (f < 0.32 ? 0.9 : 0.55 + 1.1 * f) : (f < 0.4 ? 0.6 : 0.3 + 0.78 * f); };
-    const int64_t ks = (k + 63) / 64, most = may_split ? (ks / 4 < 32 ? ks / 4 : 32) : 1;
+  for (int shape = SMALL; shape <= (plain ? WIDE : BIG); ++shape) {
+    const int64_t tp = shape == SMALL ? 128 : shape == BIG ? 256 : 192, tq = shape == SMALL ? 128 : 256;
+    const int64_t tiles = ((np + tp - 1) / tp) * ((nq + tq - 1) / tq), at_once = shape == SMALL ? 2 * CUS : CUS;
+    auto round = [&](double part, int64_t steps) {   // of so many steps, that holds `part` of what the GPU does
+      const double step = US[shape].fixed + US[shape].filled * part;
+      return steps * (step < US[shape].least ? US[shape].least : step) + US[shape].around;
+    };
+    const int64_t ks = (k + 63) / 64, most = plain ? (ks / 4 < 32 ? ks / 4 : 32) : 1;
     for (int64_t s = 1; s <= (most < 1 ? 1 : most); ++s) {
       const int64_t full = tiles * s / at_once, rest = tiles * s % at_once, each = (ks + s - 1) / s;
-      const double us = full * (each * step(1.0) + 5.0) + (rest ? each * step((double)rest / at_once) + 5.0 : 0.0) + (s > 1 ? 2.0 + (double)s * np * nq * 8 / 4e6 : 0.0);
-      if (us < least) least = us, best = Tiling{big != 0, (int)s};
+      const double us = full * round(1.0, each) + (rest ? round((double)rest / at_once, each) : 0.0) +
+                        (s > 1 ? 1.4 + (double)s * np * nq * 8 / 4e6 : 0.0);
+      if (us < least) least = us, best = Tiling{(Shape)shape, (int)s};
     }
   }
   return best;
 }
 inline int64_t scratch_ld(int64_t np) { return (np + 3) / 4 * 4; }
 
-template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, bool big, hipStream_t st) {
-  return big ? launch_tiles<T, KP, KQ, 4, 2, 2, 4, EPI>(a, st) : launch_tiles<T, KP, KQ, 2, 2, 2, 2, EPI>(a, st);
+template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, Shape shape, hipStream_t st) {
+  if constexpr (EPI == STORE || EPI == PARTIAL)
+    if (shape == WIDE) return launch_tiles<T, KP, KQ, 2, 4, 3, 2, EPI>(a, st);
+  return shape == SMALL ? launch_tiles<T, KP, KQ, 2, 2, 2, 2, EPI>(a, st) : launch_tiles<T, KP, KQ, 4, 2, 2, 4, EPI>(a, st);
 }
 template <typename T, Kind KP, Kind KQ> int plain_product(Product a, float* scratch, hipStream_t st) {
   const int64_t np = a.p.size, nq = a.q.size;
@@ -698,7 +712,7 @@ template <typename T, Kind KP, Kind KQ> int plain_product(Product a, float* scra
   const bool al = np % 8 == 0 && a.ldo % 8 == 0 && al16(a.out);
   if (tl.splits == 1) {
     a.out16 = al;
-    return launch_product<T, KP, KQ, STORE>(a, tl.big, st);
+    return launch_product<T, KP, KQ, STORE>(a, tl.shape, st);
   }
   if (!scratch) return LDR_E_ARG;
   void* const out = a.out;
@@ -707,7 +721,7 @@ template <typename T, Kind KP, Kind KQ> int plain_product(Product a, float* scra
   a.splits = (int)((a.k + a.run - 1) / a.run);
   a.out = scratch;
   a.ldo = ldp;
-  const int e = launch_product<T, KP, KQ, PARTIAL>(a, tl.big, st);
+  const int e = launch_product<T, KP, KQ, PARTIAL>(a, tl.shape, st);
   if (e) return e;
   hipLaunchKernelGGL(k_split_sum<T>, dim3(grid_of(nq * ldp / 4, 4096)), dim3(256), 0, st, scratch, a.splits, nq, np, ldp,
                      static_cast<T*>(out), ldo, al);
@@ -804,8 +818,8 @@ int lbk_ffn_gate_up(const void* x, int64_t ldx, const void* w, int64_t ldw, void
   a.saved = saved;
   a.saved_cols = (n + 31) / 32;
   a.act = activation;
-  const bool big = tiling_of(2 * n, t, d, false).big;
-  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, GATED>(a, big, st)))
+  const Shape shape = tiling_of(2 * n, t, d, false).shape;
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, GATED>(a, shape, st)))
 }
 
 int lbk_ffn_dgate_up(const void* dy, int64_t ld_dy, const void* w_down, int64_t ldw, const void* saved, void* dgate_up, int64_t ld_dgu,
@@ -823,8 +837,8 @@ int lbk_ffn_dgate_up(const void* dy, int64_t ld_dy, const void* w_down, int64_t 
   a.saved_cols = (n + 31) / 32;
   // a short sum beside ten bytes moved per element: two workgroups to a CU, one's loads and stores beside the other's products
   // (16384 x 768 x 2048: 100 us against 110 with the large tiles; 8192 x 2048 x 5632: 230 against 224)
-  const bool big = d > 1024 && tiling_of(n, t, d, false).big;
-  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, DGATED>(a, big, static_cast<hipStream_t>(stream))))
+  const Shape shape = d > 1024 ? tiling_of(n, t, d, false).shape : SMALL;
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, DGATED>(a, shape, static_cast<hipStream_t>(stream))))
 }
 
 int64_t lbk_linear_scratch(int64_t np, int64_t nq, int64_t k) {

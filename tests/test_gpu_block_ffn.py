@@ -89,6 +89,47 @@ def test_large(t, d, n, dtype):
     check(t, d, n, d, dtype)
 
 
+@pytest.mark.parametrize("columns,rows,k", [(2504, 4001, 300), (760, 16001, 264), (528, 3040, 6061), (200, 300, 72), (1496, 4104, 1000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_products(columns, rows, k, dtype):
+    """Each product of the block by itself, its result of `columns` x `rows`, every tile shape among the sizes, whole and in splits;
+    one rounding of the fp32 sum (k products, errors of 2^-24 of the partial sums' size each), and nothing past the result."""
+    from loopback_amd import block_ops as ops
+    lib, code, st = ops.LIB, 1 if dtype is torch.bfloat16 else 2, torch.cuda.current_stream().cuda_stream
+    print(f"case products {columns} {rows} {k} {dtype}", flush=True)
+
+    def operand(r, c, seed):   # rows of c elements, in rows of a multiple of 8
+        out = torch.zeros((r, (c + 7) // 8 * 8), dtype=dtype, device=DEV)
+        out[:, :c] = rnd((r, c), dtype, seed)
+        return out, out.shape[1], out[:, :c].double()
+
+    def scratch():
+        return torch.empty(max(4, lib.lbk_linear_scratch(columns, rows, k)), device=DEV)
+
+    def test(name, call, ref, terms):
+        outs = []
+        for _ in range(2):
+            out = torch.full((rows + 1, columns), 7.0, dtype=dtype, device=DEV)
+            s = scratch()
+            assert call(out.data_ptr(), s.data_ptr()) == 0
+            torch.cuda.synchronize()
+            assert (out[-1] == 7).all(), name
+            outs.append(out[:-1])
+        assert torch.equal(outs[0], outs[1]), name   # a fixed order
+        tiny = 2.0 ** -25 if dtype is torch.float16 else 0.0
+        off = (outs[0].double() - ref).abs()
+        assert not (off > HALF[dtype] * ref.abs() + 1e-5 * terms + tiny).any(), (name, off.max().item())
+
+    (p, lp, pv), (q, lq, qv) = operand(columns, k, 1), operand(rows, k, 2)          # k along both operands' rows
+    (pt, lpt, ptv), (qt, lqt, qtv) = operand(k, columns, 3), operand(k, rows, 4)    # the columns, the rows along them
+    test("forward", lambda o, s: lib.lbk_linear_fwd(q.data_ptr(), lq, p.data_ptr(), lp, o, columns, s, rows, k, columns, code, st),
+         qv @ pv.t().contiguous(), qv.abs() @ pv.abs().t().contiguous())
+    test("input gradient", lambda o, s: lib.lbk_linear_dx(q.data_ptr(), lq, pt.data_ptr(), lpt, o, columns, s, rows, k, columns, code, st),
+         qv @ ptv, qv.abs() @ ptv.abs())
+    test("weight gradient", lambda o, s: lib.lbk_linear_dw(qt.data_ptr(), lqt, pt.data_ptr(), lpt, s, o, k, rows, columns, code, st),
+         qtv.t().contiguous() @ ptv, qtv.abs().t().contiguous() @ ptv.abs())
+
+
 @pytest.mark.parametrize("t", [1, 2, 3, 7, 8, 16, 17, 31, 32, 48, 64, 65, 100])
 def test_few_tokens(t):
     check(t, 768, 2048, 768, torch.bfloat16)
