@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define LBK_ABI_VERSION 1
+#define LBK_ABI_VERSION 2   /* 2: lbk_join_bwd takes x in h's place */
 int lbk_abi_version(void);
 
 /* ---- dropout ----------------------------------------------------------------------------------------------------
@@ -46,8 +46,8 @@ int64_t lbk_join_scratch(int64_t rows, int64_t d, int64_t gate_rows);
 
 /* The gradients for dh and dn (either may be NULL, not both; dn needs pre): dx = dh + the norm's share, dy through the
  * dropout, scale, gate and norm, and the sums dpost, dgate (gate's shape), dpre, rounded once. Each result may be NULL
- * (not wanted). h is the forward's result, y its input. */
-int lbk_join_bwd(const void* dh, const void* dn, const void* h, const void* y, const void* post, const void* gate,
+ * (not wanted). x and y are the forward's inputs: the norm's gradient is formed at x + z before its rounding. */
+int lbk_join_bwd(const void* dh, const void* dn, const void* x, const void* y, const void* post, const void* gate,
                  int64_t gate_rows, const void* pre, const float* r_post, const float* r_pre, const int64_t* rng,
                  uint32_t site, int drop, float scale, void* dx, void* dy, void* dpost, void* dgate, void* dpre,
                  float* scratch, int64_t rows, int64_t d, int dtype, void* stream);

@@ -28,7 +28,7 @@ from . import _host as H      # the launch path (csrc/host.cpp), bound below to 
 from . import build as _build
 from .lm_ops import _stream, _watched, native
 
-ABI_VERSION = 1
+ABI_VERSION = 2
 JOIN_MAX_WIDTH = 8192
 FEW_TOKENS = 32
 FFN_MAX_WIDTH = 2 ** 22 - 8   # elements between rows of the tiled products' operands
@@ -204,15 +204,15 @@ def _sum_like(t, like):
     return (t.sum(dims, keepdim=True) if dims else t).reshape(like.shape)
 
 
-def _join_backward(dh, dn, h, y, post, gate, pre, rng, site, drop, need, scale, eps):
+def _join_backward(dh, dn, x, y, post, gate, pre, rng, site, drop, need, scale, eps):
     """The torch form of the join's backward, for the node (csrc/host.cpp): the gradients of x, y, post, gate and pre that need's
-    bits ask for, by their formulas (not by autograd: the node is locked while it runs, and the engine would wait for it). h is the
-    forward's (the norm's gradient is formed at it)."""
+    bits ask for, by their formulas (not by autograd: the node is locked while it runs, and the engine would wait for it). The
+    norm's gradient is formed at the sum before its rounding."""
     nx, ny, npost, ngate, npre = (bool(need & b) for b in (1, 2, 4, 8, 16))
     dt, out = y.dtype, [None] * 5
     g = None if dh is None else _upcast(dh)
     if dn is not None:
-        hu, dnu = _upcast(h), _upcast(dn)
+        hu, dnu = _upcast(x) + _branch_torch(y, post, gate, rng, site, drop, scale, eps), _upcast(dn)
         r2 = torch.rsqrt(hu.pow(2).mean(-1, keepdim=True) + eps)
         gn = _norm_grad(dnu * _upcast(pre), hu, r2)
         g = gn if g is None else g + gn

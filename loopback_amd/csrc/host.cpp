@@ -408,7 +408,7 @@ struct JoinNode : torch::autograd::Function<JoinNode> {
                                const OptTensor& gate, const OptTensor& pre, const OptTensor& rng, int64_t gate_rows, int64_t site,
                                int64_t drop, double scale, double eps, int64_t dtype, int64_t stream) {
     variable_list t = join_run(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, true);
-    ctx->save_for_backward({pre ? t[0] : at::Tensor(), y, or_none(post), or_none(gate), or_none(pre), t[2], t[3], or_none(rng)});
+    ctx->save_for_backward({pre ? x : at::Tensor(), y, or_none(post), or_none(gate), or_none(pre), t[2], t[3], or_none(rng)});
     ctx->saved_data["numbers"] = std::vector<int64_t>{gate_rows, site, drop, dtype, stream};
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["eps"] = eps;

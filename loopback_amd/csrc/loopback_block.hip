@@ -88,10 +88,8 @@ __device__ __forceinline__ uint4 philox(uint32_t block, uint32_t row, uint32_t s
   }
   return make_uint4(c0, c1, c2, c3);
 }
-// v = kept ? v * s : 0, eight columns from one block of the generator
-__device__ __forceinline__ void drop8(float (&v)[8], uint32_t block, uint32_t row, uint32_t site, const Rng& r, uint32_t drop,
-                                      float s) {
-  const uint4 w = philox(block, row, site, r);
+// v = kept ? v * s : 0, eight columns from one block w of the generator
+__device__ __forceinline__ void drop8(float (&v)[8], const uint4& w, uint32_t drop, float s) {
   const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
@@ -115,7 +113,7 @@ __global__ __launch_bounds__(WG) void k_dropout(const T* __restrict__ x, const i
     const int64_t o = row * d + 8 * b;
     float v[8];
     IO<T>::unpack(load8<T, AL>(x + o, 0, left), v);
-    drop8(v, (uint32_t)b, (uint32_t)row, site, r, drop, s);
+    drop8(v, philox((uint32_t)b, (uint32_t)row, site, r), drop, s);
     store8<T, AL>(out + o, 0, left, v);
   }
 }
@@ -236,7 +234,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) 
       const int blk = lane + LPR * v;
 #pragma unroll
       for (int k = 0; k < 8; ++k) z[k] *= a.scale;
-      if (drops) drop8(z, (uint32_t)blk, (uint32_t)row, a.site, rng, a.drop, a.keep);
+      if (drops) drop8(z, philox((uint32_t)blk, (uint32_t)row, a.site, rng), a.drop, a.keep);
       IO<T>::unpack(xr[v], h[v]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -261,7 +259,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) 
 }
 
 template <typename T> struct JoinBwd {
-  const T *dh, *dn, *h, *y, *post, *gate, *pre;
+  const T *dh, *dn, *x, *y, *post, *gate, *pre;
   const float *r_post, *r_pre;
   const int64_t* rng;
   T *dx, *dy, *dgate;
@@ -271,12 +269,15 @@ template <typename T> struct JoinBwd {
   float scale, keep;
 };
 
+// The next norm's gradient is formed at the sum before it was rounded, from x, y and the mask: at the rounded one, which would be read
+// in x's place, dpre has up to 7.5 times the error of its own rounding (few rows), so 1.0.
 // A workgroup takes `per` consecutive rows and keeps the column sums of the three weight gradients in registers. The gate's
 // belong to runs of gate_rows rows: a run that lies inside the workgroup's rows is finished here, a share of a longer one
 // goes to part_gate, first slot where the run began before this workgroup's rows, second where it ends after them.
 // gate_rows 1: each element's own. Its vector arithmetic bounds it (the generator, unpacking, two row sums), beside the stream of six
-// rows: 16384 x 768 in bf16 with all parts 44 us (3.4 TB/s; two vectors a lane on half the lanes took 72, held to fewer registers
-// 121 to 210 with spills; loading the next row ahead changed nothing, 43.4 against 43.7), 6825 x 2048 in fp16 without dropout 41 us (4.1 TB/s).
+// rows: 16384 x 768 in bf16 with all parts 42 us (3.6 TB/s; two vectors a lane on half the lanes took 72, held to fewer registers
+// 121 to 210 with spills; loading the next row ahead changed nothing, 43.4 against 43.7), 6825 x 2048 in fp16 without dropout 36
+// us (4.7 TB/s).
 template <typename T, int LPR, int VPT, bool AL, int PARTS>
 __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) {
   const bool has_dn = PARTS < 0 ? a.dn != nullptr : PARTS & 1, has_post = PARTS < 0 ? a.post != nullptr : PARTS & 2,
@@ -339,13 +340,13 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
       const bool ok = row0 + grp < s1;
       const int row = (int)(ok ? row0 + grp : s1 - 1);
       const int64_t ro = (int64_t)row * d;
-      typename IO<T>::Raw hr[VPT], yr[VPT], dhr[VPT], dnr[VPT];
+      typename IO<T>::Raw xr[VPT], yr[VPT], dhr[VPT], dnr[VPT];
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
         const int col = 8 * (lane + LPR * v);
         if (has_dn) {
           dnr[v] = load8<T, AL>(a.dn + ro, col, d);
-          hr[v] = load8<T, AL>(a.h + ro, col, d);
+          xr[v] = load8<T, AL>(a.x + ro, col, d);
         }
         dhr[v] = a.dh ? load8<T, AL>(a.dh + ro, col, d) : IO<T>::zero();
         yr[v] = load8<T, AL>(a.y + ro, col, d);
@@ -369,29 +370,47 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
         anew<T>(gate[v]);
       }
       const float q2 = has_dn ? a.r_pre[row] : 0.f, q1 = has_post ? a.r_post[row] : 1.f;
+      uint4 words[VPT];
+#pragma unroll
+      for (int v = 0; v < VPT; ++v)
+        words[v] = drops ? philox((uint32_t)(lane + LPR * v), (uint32_t)row, a.site, rng) : make_uint4(0u, 0u, 0u, 0u);
       float g[VPT][8];   // the gradient of h
       if (has_dn) {
-        float c = 0.f;   // sum dn pre h
+        float h[VPT][8], c = 0.f;   // h before its rounding; sum dn pre h
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-          float e[8], w[8];
+          float e[8], z[8];
+          IO<T>::unpack(yr[v], z);
+          if (has_post) {
+            IO<T>::unpack(post[v], e);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] *= q1 * e[k];
+          }
+          if (a.gate) {
+            IO<T>::unpack(gate[v], e);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] *= e[k];
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) z[k] *= a.scale;
+          if (drops) drop8(z, words[v], a.drop, a.keep);
+          IO<T>::unpack(xr[v], h[v]);
           IO<T>::unpack(dnr[v], g[v]);
-          IO<T>::unpack(hr[v], e);
-          IO<T>::unpack(pre[v], w);
+          IO<T>::unpack(pre[v], e);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            d_pre[v][k] = __builtin_fmaf(g[v][k], e[k] * q2, d_pre[v][k]);
-            g[v][k] *= w[k];
-            c = __builtin_fmaf(g[v][k], e[k], c);
+            h[v][k] += z[k];
+            d_pre[v][k] = __builtin_fmaf(g[v][k], h[v][k] * q2, d_pre[v][k]);
+            g[v][k] *= e[k];
+            c = __builtin_fmaf(g[v][k], h[v][k], c);
           }
         }
         c = row_sum(c) * q2 * q2 * inv_d;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
           float e[8];
-          IO<T>::unpack(hr[v], e);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) g[v][k] = q2 * (g[v][k] - c * e[k]);
+          for (int k = 0; k < 8; ++k) g[v][k] = q2 * (g[v][k] - c * h[v][k]);
           IO<T>::unpack(dhr[v], e);
 #pragma unroll
           for (int k = 0; k < 8; ++k) g[v][k] += e[k];
@@ -411,7 +430,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
         IO<T>::unpack(gate[v], gt);
 #pragma unroll
         for (int k = 0; k < 8; ++k) g[v][k] *= a.scale;
-        if (drops) drop8(g[v], (uint32_t)blk, (uint32_t)row, a.site, rng, a.drop, a.keep);
+        if (drops) drop8(g[v], words[v], a.drop, a.keep);
         if (a.gate) {
           float og[8];
 #pragma unroll
@@ -645,19 +664,19 @@ int64_t lbk_join_scratch(int64_t rows, int64_t d, int64_t gate_rows) {
   return plan_of(rows, d, gate_rows).parts * 4 * d;
 }
 
-int lbk_join_bwd(const void* dh, const void* dn, const void* h, const void* y, const void* post, const void* gate,
+int lbk_join_bwd(const void* dh, const void* dn, const void* x, const void* y, const void* post, const void* gate,
                  int64_t gate_rows, const void* pre, const float* r_post, const float* r_pre, const int64_t* rng,
                  uint32_t site, int drop, float scale, void* dx, void* dy, void* dpost, void* dgate, void* dpre,
                  float* scratch, int64_t rows, int64_t d, int dtype, void* stream) {
   if (rows == 0) drop = 0;
   const int e = join_shape(rows, d, gate_rows, gate, drop, rng, dtype);
   if (e || rows == 0) return e;
-  if ((!dh && !dn) || !y || (dn && (!h || !pre || !r_pre)) || (post && !r_post)) return LDR_E_ARG;
+  if ((!dh && !dn) || !y || (dn && (!x || !pre || !r_pre)) || (post && !r_post)) return LDR_E_ARG;
   if ((dpost && !post) || (dgate && !gate) || (dpre && !dn)) return LDR_E_ARG;
   if (!dx && !dy && !dpost && !dgate && !dpre) return LDR_OK;
   if ((dpost || dgate || dpre) && !scratch) return LDR_E_ARG;
   bool al = d % 8 == 0;
-  for (const void* p : {dh, dn, h, y, post, gate, pre, (const void*)dx, (const void*)dy, (const void*)dgate,
+  for (const void* p : {dh, dn, x, y, post, gate, pre, (const void*)dx, (const void*)dy, (const void*)dgate,
                         (const void*)scratch}) {
     if (!al_of(p, dtype)) return LDR_E_ALIGN;
     al = al && al16(p);
@@ -669,7 +688,7 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* h, const void* y, c
   const int parts = (int)plan.parts;
   hipStream_t st = static_cast<hipStream_t>(stream);
   LBK_TYPE_SWITCH(dtype, {
-    const JoinBwd<T> a{static_cast<const T*>(dh), static_cast<const T*>(dn), static_cast<const T*>(h),
+    const JoinBwd<T> a{static_cast<const T*>(dh), static_cast<const T*>(dn), static_cast<const T*>(x),
                        static_cast<const T*>(y), static_cast<const T*>(post), static_cast<const T*>(gate),
                        static_cast<const T*>(pre), r_post, r_pre, rng, static_cast<T*>(dx), static_cast<T*>(dy),
                        static_cast<T*>(dgate), dpost ? scratch : nullptr, dpre ? scratch + parts * d : nullptr,
@@ -679,6 +698,9 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* h, const void* y, c
       if (al) {
         LBK_PARTS_SWITCH((dn ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
                          hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, true, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
+      } else if constexpr (LPR == 1024) {   // 128 registers a lane: looked up, 108 spill (16384 x 5001: 999 us, 473 so)
+        LBK_PARTS_SWITCH((dn ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
+                         hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, false, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
       } else {
         hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, false, ANY>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a);
       }

@@ -208,10 +208,10 @@ def test_join_backward_form(gate, post, pre, drop):
         ref = iter(torch.autograd.grad([o for o, _ in outs], ins, [u for _, u in outs], retain_graph=True, allow_unused=True))
         ref = [None if t is None else next(ref) for t in (x, y, p, g, w)]
         need = 3 + 4 * post + 8 * bool(gate) + 16 * (pre and b is not None)
-        got = ops._join_backward(a, b, h, y, p, g, w, rng, 1, drop, need, 0.6, 1e-3)
+        got = ops._join_backward(a, b, x, y, p, g, w, rng, 1, drop, need, 0.6, 1e-3)
         for k, (u, v) in enumerate(zip(got, ref)):
             assert (u is not None) == bool(need >> k & 1) and (u is None or torch.allclose(u, v, atol=1e-12)), k
-    none = ops._join_backward(dh, dn, h, y, p, g, w, rng, 1, drop, 0, 0.6, 1e-3)
+    none = ops._join_backward(dh, dn, x, y, p, g, w, rng, 1, drop, 0, 0.6, 1e-3)
     assert none == (None,) * 5
 
 
@@ -249,3 +249,17 @@ def test_watched_calls_are_torch_operations():
         assert ops.gated_ffn(y, torch.empty(96, 64, device="cuda", dtype=torch.bfloat16),
                              torch.empty(32, 48, device="cuda", dtype=torch.bfloat16)).shape == (2, 3, 32)
     assert torch.func.vmap(fn)(x[None]).shape == (1, 2, 3, 8)
+
+
+@pytest.mark.parametrize("dtype,half", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+def test_join_backward_is_at_the_unrounded_sum(dtype, half):
+    """The torch form's gradients in 16 bits, of one row, where no sum hides a rounding: one rounding of the exact ones each (and
+    fp32 round-off, 1e-5 of their size), the weight's of the norm after the rounded sum among them."""
+    g = torch.Generator().manual_seed(5)
+    x, y, post, pre, dh, dn = (torch.randn(s, generator=g).to(dtype) for s in ((1, 64), (1, 64), (64,), (64,), (1, 64), (1, 64)))
+    got = ops._join_backward(dh, dn, x, y, post, None, pre, None, 0, 0, 31 - 8, 0.7, 1e-6)
+    leaves = [t.double().requires_grad_() for t in (x, y, post, pre)]
+    h, n = ops._join_torch(leaves[0], leaves[1], leaves[2], None, leaves[3], None, 0, 0, 0.7, 1e-6)
+    ref = torch.autograd.grad((h, n), leaves, (dh.double(), dn.double()))
+    for a, b in zip((got[0], got[1], got[2], got[4]), ref):
+        assert ((a.double() - b).abs() <= half * b.abs() + 1e-5 * b.pow(2).mean().sqrt()).all()

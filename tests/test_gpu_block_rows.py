@@ -3,7 +3,7 @@ rounded once, so each element lies within half a step of the result's type (2^-8
 of an fp32 one) plus fp32 round-off (1e-5 of the result's RMS; a dropped element is exactly 0). A norm's gradient is a difference r (t - v mean(t v)),
 which cancels where a row has one or few elements: its fp32 round-off is that of its two terms, each of at most 16 roundings
 (products, the row scale, a sum over up to 1024 lanes by pairs), 16 * 2^-24 = 2^-20 of r (|t| + |v| mean |t v|). The backward's formulas are
-evaluated at the h that the forward returned, which is what it saves. Sizes: one element, the edges of a vector, of the lanes
+evaluated at the sum before its rounding. Sizes: one element, the edges of a vector, of the lanes
 that share a row and of each row shape, odd widths, unaligned rows; gates whose runs of rows end inside and at a workgroup's."""
 import pytest
 import torch
@@ -41,10 +41,10 @@ def unaligned(t):
     return out
 
 
-def join64(x, y, post, gate, pre, mask, scale, eps, h_saved, dh, dn):
-    """(h, n) and the gradients of x, y, post, gate, pre in fp64 by their formulas, the backward's at h_saved."""
+def join64(x, y, post, gate, pre, mask, scale, eps, dh, dn):
+    """(h, n) and the gradients of x, y, post, gate, pre in fp64 by their formulas."""
     f = lambda t: None if t is None else t.detach().double()
-    x, y, post, gate, pre, hs, dh, dn = map(f, (x, y, post, gate, pre, h_saved, dh, dn))
+    x, y, post, gate, pre, dh, dn = map(f, (x, y, post, gate, pre, dh, dn))
     d = x.shape[-1]
     r1 = (y.pow(2).mean(-1, keepdim=True) + eps).rsqrt() if post is not None else 1.0
     yh, w = y * r1, 1.0 if post is None else post
@@ -58,7 +58,7 @@ def join64(x, y, post, gate, pre, mask, scale, eps, h_saved, dh, dn):
         out["n"] = h * r2 * pre
     g = torch.zeros_like(x) if dh is None else dh
     if dn is not None:
-        hh = hs * r2
+        hh = h * r2
         t = dn * pre
         g = g + r2 * (t - hh * (t * hh).mean(-1, keepdim=True))
         slack["dx"] = terms(t, hh, r2)
@@ -100,7 +100,7 @@ def check_join(shape, dtype, post, gate, pre, p, scale=0.7, eps=1e-6, place=lamb
     if p:
         drop = round(65536 * p)
         mask = ops.keep_mask(shape, p, rng, 9).double() * (65536 / max(1, 65536 - drop))   # p = 1 keeps nothing
-    ref, slack = join64(x, y, pw, gw, nw, mask, scale, eps, h, dh, dn)
+    ref, slack = join64(x, y, pw, gw, nw, mask, scale, eps, dh, dn)
     got = {"h": h, "n": n, "dx": x.grad, "dy": y.grad, "dpost": pw is not None and pw.grad, "dgate": gw is not None and gw.grad,
            "dpre": nw is not None and nw.grad}
     for k, r in ref.items():
