@@ -512,7 +512,7 @@ __global__ __launch_bounds__(256) void k_split_sum(const float* __restrict__ par
   }
 }
 
-// out [rows][ld] = x [rows][cols], zeros past the columns, for operands whose rows are not aligned; eight columns per lane. 4 to 6 us for each
+// out [rows][ld] = x [rows][cols], zeros past the columns, for operands whose rows are not aligned; eight columns per lane. 3 to 6 us for each
 // operand of 1001 x 1001 x 2731; the products on unaligned rows, element by element, took 708 us a pass there and take 217 so.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pad_rows(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ld,
