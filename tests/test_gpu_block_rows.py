@@ -425,3 +425,26 @@ def test_anomaly_mode():
         h, n = ops.block_join(x, x, post_weight=w, pre_weight=w)
         with pytest.raises(RuntimeError, match="returned nan values"):
             (h.sum() * float("nan")).backward()
+
+
+def test_inputs_changed_before_the_backward():
+    """x and y are what the backward reads: changed in place, it refuses; h and n are not, and may be."""
+    from loopback_amd import block_ops as ops
+    x0, y0, w = (rnd(s, torch.bfloat16, k).requires_grad_() for k, s in enumerate(((40, 136), (40, 136), (136,))))
+    dh, dn = rnd((40, 136), torch.bfloat16, 5), rnd((40, 136), torch.bfloat16, 6)
+
+    def run(change):
+        x, y = x0 * 1, y0 * 1
+        h, n = ops.block_join(x, y, post_weight=w, pre_weight=w, dropout=0.1, rng=rng_of(2))
+        f = (h * dh).sum() + (n * dn).sum()   # keeps dh and dn, not h and n
+        with torch.no_grad():
+            for t in change(x, y, h, n):
+                t.add_(1.0)
+        return torch.autograd.grad(f, (x0, y0, w))
+
+    want = run(lambda x, y, h, n: ())
+    for a, b in zip(run(lambda x, y, h, n: (h, n)), want):
+        assert torch.equal(a, b)
+    for change in (lambda x, y, h, n: (x,), lambda x, y, h, n: (y,)):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            run(change)
