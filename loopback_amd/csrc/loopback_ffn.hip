@@ -165,10 +165,10 @@ template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile 
 // ---------------------------------------------------------------------------------------------------------------
 // what the backward needs of the gate and up projections: (u a'(g), a(g)) of each (token, inner column), which the
 // activation's gradient is multiplied by. Kept as the upper 24 bits of their fp32 values: 16 would double the input and
-// gate/up weight gradients' squared error (three roundings of 2^-9 instead of two). In blocks of 32 tokens x 32 columns in the
+// gate/up weight gradients' squared error (three roundings instead of two). In blocks of 32 tokens x 32 columns in the
 // matrix cores' own order, so both kernels move them as whole vectors: 64 lanes x 16 values, upper 16 bits as two planes of
-// eight values a lane, then the next eight bits: 3072 bytes for each of the two. Stores and loads past the caches: gate and up
-// projection of 8192 x 2048 x 5632 382 -> 342 us, the gradient that reads them 266 -> 238.
+// eight values a lane, then the next eight bits: half a block's bytes for each of the two. Stores and loads past the
+// caches: gate and up projection of 8192 x 2048 x 5632 382 -> 342 us, the gradient that reads them 266 -> 238.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int64_t SAVED_BLOCK = 6144;
 struct Saved {
