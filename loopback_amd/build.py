@@ -75,7 +75,8 @@ def _start(src, lib: str, verbose: bool, defines) -> tuple:
 
 
 def _start_host(verbose: bool) -> tuple:
-    """The host extension: plain C++, linked to the libtorch of the running interpreter."""
+    """The host extension: plain C++ (the HIP runtime's header for a stream's handle), linked to the libtorch of the running
+    interpreter."""
     import sysconfig
 
     import torch
@@ -83,9 +84,9 @@ def _start_host(verbose: bool) -> tuple:
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = HOST_LIB + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
-           *[f"-I{i}" for i in include_paths()], f"-I{sysconfig.get_paths()['include']}", "-o", tmp, HOST_SRC,
-           f"-L{lib}", "-lc10", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__", f"-I{INCLUDE}",
+           f"-I{ROCM}/include", *[f"-I{i}" for i in include_paths()], f"-I{sysconfig.get_paths()['include']}", "-o", tmp, HOST_SRC,
+           f"-L{lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{lib}"]
     if verbose:
         print(" ".join(cmd), flush=True)
     return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True), tmp, HOST_LIB

@@ -13,7 +13,9 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPStream.h>
 
 #include <cstring>
 #include <tuple>
@@ -352,6 +354,11 @@ bool on_kernels(const variable_list& grads, const at::Tensor& like, bool same_sh
       return false;
   return true;
 }
+// A backward launches where its results are allocated and its gradients copied: on the current stream of their GPU. The engine
+// makes that the forward's stream; a node that is called by itself runs on its caller's.
+int64_t stream_of(const at::Tensor& t) {
+  return static_cast<int64_t>(reinterpret_cast<intptr_t>(c10::hip::getCurrentHIPStream(t.device().index()).stream()));
+}
 at::Tensor rows_of(const at::Tensor& t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
 
 at::Tensor dropout_run(const at::Tensor& x, const at::Tensor& rng, int64_t site, int64_t drop, int64_t dtype, int64_t stream) {
@@ -364,12 +371,11 @@ at::Tensor dropout_run(const at::Tensor& x, const at::Tensor& rng, int64_t site,
   return out;
 }
 
-// Both nodes launch on the stream of their forward: the engine runs a node's backward on it.
 struct DropoutNode : torch::autograd::Function<DropoutNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& rng, int64_t site, int64_t drop,
                             int64_t dtype, int64_t stream) {
     ctx->save_for_backward({rng});
-    ctx->saved_data["numbers"] = std::vector<int64_t>{site, drop, dtype, stream};
+    ctx->saved_data["numbers"] = std::vector<int64_t>{site, drop, dtype};
     ctx->set_materialize_grads(false);
     return dropout_run(x, rng, site, drop, dtype, stream);
   }
@@ -378,10 +384,12 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
     if (!grads[0].defined()) return out;
     const at::Tensor rng = ctx->get_saved_variables()[0];
     const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
-    if (on_kernels(grads, grads[0]) && grads[0].is_cuda() && rng.is_contiguous())
-      out[0] = dropout_run(rows_of(grads[0]), rng, n[0], n[1], n[2], n[3]);
-    else
+    if (!on_kernels(grads, grads[0]) || !grads[0].is_cuda() || !rng.is_contiguous()) {
       out[0] = torch_form(0, {grads[0], rng}, {n[0], n[1]}, {}, 1)[0];
+      return out;
+    }
+    const c10::DeviceGuard on(grads[0].device());
+    out[0] = dropout_run(rows_of(grads[0]), rng, n[0], n[1], n[2], stream_of(grads[0]));
     return out;
   }
 };
@@ -409,7 +417,7 @@ struct JoinNode : torch::autograd::Function<JoinNode> {
                                int64_t drop, double scale, double eps, int64_t dtype, int64_t stream) {
     variable_list t = join_run(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, true);
     ctx->save_for_backward({pre ? x : at::Tensor(), y, or_none(post), or_none(gate), or_none(pre), t[2], t[3], or_none(rng)});
-    ctx->saved_data["numbers"] = std::vector<int64_t>{gate_rows, site, drop, dtype, stream};
+    ctx->saved_data["numbers"] = std::vector<int64_t>{gate_rows, site, drop, dtype};
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["eps"] = eps;
     ctx->set_materialize_grads(false);
@@ -435,6 +443,7 @@ struct JoinNode : torch::autograd::Function<JoinNode> {
       std::copy(got.begin(), got.end(), out.begin());
       return out;
     }
+    const c10::DeviceGuard on(y.device());
     // a saved-tensor hook may give a tensor back with other strides than it was saved with
     variable_list s(saved.size());
     for (size_t i = 0; i < s.size(); ++i) s[i] = rows_of(saved[i]);
@@ -457,7 +466,7 @@ struct JoinNode : torch::autograd::Function<JoinNode> {
                                 n[2] ? static_cast<const int64_t*>(ptr(s[7])) : nullptr, static_cast<uint32_t>(n[1]),
                                 static_cast<int>(n[2]), static_cast<float>(scale), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(out[3]),
                                 ptr(out[4]), static_cast<float*>(ptr(scratch)), rows, d, static_cast<int>(n[3]),
-                                reinterpret_cast<void*>(n[4])));
+                                reinterpret_cast<void*>(stream_of(y))));
     return out;
   }
 };
@@ -516,7 +525,7 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     const bool keep = x.requires_grad() || wgu.requires_grad();
     variable_list t = ffn_run(x, wgu, wd, f, keep);
     ctx->save_for_backward({x, wgu, wd, wd.requires_grad() ? t[1] : at::Tensor(), t[2], t[3], t[4], t[5]});
-    ctx->saved_data["numbers"] = std::vector<int64_t>{f.t, f.d, f.n, f.m, act, dtype, stream};
+    ctx->saved_data["numbers"] = std::vector<int64_t>{f.t, f.d, f.n, f.m, act, dtype};
     ctx->set_materialize_grads(false);
     return t[0];
   }
@@ -525,13 +534,15 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     if (!grads[0].defined()) return out;
     variable_list s = ctx->get_saved_variables();
     const std::vector<int64_t> v = ctx->saved_data["numbers"].toIntVector();
-    const Ffn f{v[0], v[1], v[2], v[3], v[4], v[5], v[6]};
+    Ffn f{v[0], v[1], v[2], v[3], v[4], v[5], 0};
     const bool nx = ctx->needs_input_grad(0), ngu = ctx->needs_input_grad(1), nd = ctx->needs_input_grad(2);
     if (!on_kernels(grads, s[0], false) || !s[0].is_cuda()) {
       const variable_list got = torch_form(2, {grads[0], s[0], s[1], s[2]}, {f.act, nx + 2 * ngu + 4 * nd}, {}, 3);
       std::copy(got.begin(), got.end(), out.begin());
       return out;
     }
+    const c10::DeviceGuard on(s[0].device());
+    f.stream = stream_of(s[0]);
     for (at::Tensor& t : s) t = rows_of(t);   // a saved-tensor hook may give one back with other strides
     const Rows dy = operand(rows_of(grads[0]), f);
     auto kept = [&](int copy, int of) { return s[copy].defined() ? operand(s[copy], f) : operand(s[of], f); };
