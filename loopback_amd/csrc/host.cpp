@@ -359,6 +359,15 @@ bool on_kernels(const variable_list& grads, const at::Tensor& like, bool same_sh
 int64_t stream_of(const at::Tensor& t) {
   return static_cast<int64_t>(reinterpret_cast<intptr_t>(c10::hip::getCurrentHIPStream(t.device().index()).stream()));
 }
+// The kernels index a saved tensor by the forward's sizes; a saved-tensor hook may give back any other.
+void as_saved(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, int64_t rows, int64_t cols) {
+  if (!t.defined()) return;
+  TORCH_CHECK(t.layout() == at::kStrided && t.device() == like.device() && t.scalar_type() == type && t.dim() > 0 &&
+                  t.numel() == rows * cols && t.size(-1) == cols,
+              "a block operator's saved tensor came back from a hook with another shape, type or device: ", t.toString(), " ", t.sizes(),
+              " on ", t.device());
+}
+int64_t code_of(at::ScalarType t) { return t == at::kFloat ? LDR_F32 : t == at::kBFloat16 ? LDR_BF16 : t == at::kHalf ? LDR_F16 : -1; }
 at::Tensor rows_of(const at::Tensor& t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
 
 at::Tensor dropout_run(const at::Tensor& x, const at::Tensor& rng, int64_t site, int64_t drop, int64_t dtype, int64_t stream) {
@@ -375,7 +384,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& rng, int64_t site, int64_t drop,
                             int64_t dtype, int64_t stream) {
     ctx->save_for_backward({rng});
-    ctx->saved_data["numbers"] = std::vector<int64_t>{site, drop, dtype};
+    ctx->saved_data["numbers"] = std::vector<int64_t>{site, drop};
     ctx->set_materialize_grads(false);
     return dropout_run(x, rng, site, drop, dtype, stream);
   }
@@ -384,12 +393,15 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
     if (!grads[0].defined()) return out;
     const at::Tensor rng = ctx->get_saved_variables()[0];
     const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
-    if (!on_kernels(grads, grads[0]) || !grads[0].is_cuda() || !rng.is_contiguous()) {
-      out[0] = torch_form(0, {grads[0], rng}, {n[0], n[1]}, {}, 1)[0];
+    const at::Tensor& g = grads[0];   // its own rows: nothing of the forward's sizes is indexed
+    as_saved(rng, g, at::kLong, 1, 2);
+    const int64_t code = code_of(g.scalar_type());
+    if (!on_kernels(grads, g) || !g.is_cuda() || !rng.is_contiguous() || code < 0 || g.dim() == 0 || g.numel() == 0) {
+      out[0] = torch_form(0, {g, rng}, {n[0], n[1]}, {}, 1)[0];
       return out;
     }
-    const c10::DeviceGuard on(grads[0].device());
-    out[0] = dropout_run(rows_of(grads[0]), rng, n[0], n[1], n[2], stream_of(grads[0]));
+    const c10::DeviceGuard on(g.device());
+    out[0] = dropout_run(rows_of(g), rng, n[0], n[1], code, stream_of(g));
     return out;
   }
 };
@@ -417,7 +429,7 @@ struct JoinNode : torch::autograd::Function<JoinNode> {
                                int64_t drop, double scale, double eps, int64_t dtype, int64_t stream) {
     variable_list t = join_run(x, y, post, gate, gate_rows, pre, rng, site, drop, scale, eps, dtype, stream, true);
     ctx->save_for_backward({pre ? x : at::Tensor(), y, or_none(post), or_none(gate), or_none(pre), t[2], t[3], or_none(rng)});
-    ctx->saved_data["numbers"] = std::vector<int64_t>{gate_rows, site, drop, dtype};
+    ctx->saved_data["numbers"] = std::vector<int64_t>{gate_rows, site, drop, dtype, x.numel() / x.size(-1), x.size(-1)};
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["eps"] = eps;
     ctx->set_materialize_grads(false);
@@ -432,6 +444,17 @@ struct JoinNode : torch::autograd::Function<JoinNode> {
     if (!dh.defined() && !dn.defined()) return out;
     const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
     const double scale = ctx->saved_data["scale"].toDouble(), eps = ctx->saved_data["eps"].toDouble();
+    const int64_t rows = n[4], d = n[5];
+    const at::ScalarType type = y.scalar_type();
+    TORCH_CHECK(code_of(type) == n[3], "the block join's y came back from a hook with another type: ", type);
+    as_saved(saved[0], y, type, rows, d);
+    as_saved(y, y, type, rows, d);
+    as_saved(post, y, type, 1, d);
+    as_saved(gate, y, type, (rows + n[0] - 1) / n[0], d);
+    as_saved(pre, y, type, 1, d);
+    as_saved(saved[5], y, at::kFloat, 1, rows);
+    as_saved(saved[6], y, at::kFloat, 1, rows);
+    as_saved(rng, y, at::kLong, 1, 2);
     // the tensors among the inputs are the node's edges, in order
     size_t edge = 0;
     const bool nx = ctx->needs_input_grad(edge++), ny = ctx->needs_input_grad(edge++);
@@ -444,11 +467,10 @@ struct JoinNode : torch::autograd::Function<JoinNode> {
       return out;
     }
     const c10::DeviceGuard on(y.device());
-    // a saved-tensor hook may give a tensor back with other strides than it was saved with
+    // the strides need not be those it was saved with
     variable_list s(saved.size());
     for (size_t i = 0; i < s.size(); ++i) s[i] = rows_of(saved[i]);
     const at::Tensor dhr = rows_of(dh), dnr = rows_of(dn);
-    const int64_t d = y.size(-1), rows = y.numel() / d;
     if (nx) out[0] = at::empty_like(s[1]);
     if (ny) out[1] = at::empty_like(s[1]);
     if (npost) out[2] = at::empty_like(s[2]);
@@ -535,6 +557,17 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     variable_list s = ctx->get_saved_variables();
     const std::vector<int64_t> v = ctx->saved_data["numbers"].toIntVector();
     Ffn f{v[0], v[1], v[2], v[3], v[4], v[5], 0};
+    const at::ScalarType type = s[0].scalar_type();
+    TORCH_CHECK(code_of(type) == f.dtype, "the feed-forward block's x came back from a hook with another type: ", type);
+    const int64_t d8 = (f.d + 7) / 8 * 8, n8 = (f.n + 7) / 8 * 8;
+    as_saved(s[0], s[0], type, f.t, f.d);
+    as_saved(s[1], s[0], type, 2 * f.n, f.d);
+    as_saved(s[2], s[0], type, f.m, f.n);
+    as_saved(s[3], s[0], type, f.t, n8);
+    as_saved(s[4], s[0], at::kByte, 1, ffn_saved_bytes(f.t, f.n));
+    as_saved(s[5], s[0], type, f.t, d8);
+    as_saved(s[6], s[0], type, 2 * f.n, d8);
+    as_saved(s[7], s[0], type, f.m, n8);
     const bool nx = ctx->needs_input_grad(0), ngu = ctx->needs_input_grad(1), nd = ctx->needs_input_grad(2);
     if (!on_kernels(grads, s[0], false) || !s[0].is_cuda()) {
       const variable_list got = torch_form(2, {grads[0], s[0], s[1], s[2]}, {f.act, nx + 2 * ngu + 4 * nd}, {}, 3);
@@ -543,7 +576,9 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     }
     const c10::DeviceGuard on(s[0].device());
     f.stream = stream_of(s[0]);
-    for (at::Tensor& t : s) t = rows_of(t);   // a saved-tensor hook may give one back with other strides
+    TORCH_CHECK(grads[0].dim() > 0 && grads[0].size(-1) == f.m && grads[0].numel() == f.t * f.m,
+                "the feed-forward block's gradient has the wrong shape: ", grads[0].sizes());
+    for (at::Tensor& t : s) t = rows_of(t);   // the strides need not be those it was saved with
     const Rows dy = operand(rows_of(grads[0]), f);
     auto kept = [&](int copy, int of) { return s[copy].defined() ? operand(s[copy], f) : operand(s[of], f); };
     if (nx || ngu) {

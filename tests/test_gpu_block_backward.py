@@ -52,3 +52,57 @@ def test_on_the_callers_stream():
                 graph.replay()
                 torch.cuda.synchronize()
                 assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want)), (name, k)
+
+
+def test_a_gradient_of_another_shape_or_type():
+    """What a program hands to a node itself is checked before a kernel indexes by it: dropout takes the gradient's own type and rows,
+    the feed-forward block's has to be its output's."""
+    from loopback_amd import block_ops as ops
+    x, rng = rnd((6, 40), torch.bfloat16, 1).requires_grad_(), rng_of(3)
+    node = ops.dropout(x, 0.5, rng).grad_fn
+    *_, (_, *block) = nodes()
+    scale = torch.tensor(2.0, device=DEV)
+    with torch.no_grad():
+        for g in (rnd((6, 40), torch.float32, 2), rnd((6, 40), torch.float16, 3), rnd((3, 24), torch.bfloat16, 4),
+                  rnd((6, 40), torch.float64, 5), rnd((0, 40), torch.bfloat16, 6), rnd((6, 0), torch.bfloat16, 7), rnd((), torch.float32, 8)):
+            got, _ = node(g)   # and of rng
+            keep = ops.keep_mask(g.shape, 0.5, rng)
+            assert got.dtype is g.dtype and torch.equal(got, torch.where(keep, g * scale.to(g.dtype), 0.0)), g.shape
+        node, (dy,) = block
+        assert "Ffn" in node.name()
+        node(dy)
+        for bad in (dy[:2], dy[..., :64], dy.view(-1)):
+            with pytest.raises(RuntimeError, match="wrong shape"):
+                node(bad)
+
+
+@pytest.mark.parametrize("change", [lambda t: t.flatten()[:1].clone(), lambda t: t.repeat(*t.shape[:-1], 2) if t.dim() else t,
+                                    lambda t: t.to(torch.int16), lambda t: t.cpu()])
+def test_saved_tensors_that_a_hook_changed(change):
+    """Each saved tensor in turn comes back from a saved-tensor hook with another shape, type or device: the backward is refused."""
+    from loopback_amd import block_ops as ops
+    x, y, w, g = (rnd(s, torch.bfloat16, k).requires_grad_() for k, s in enumerate(((6, 40), (6, 40), (40,), (6, 40))))
+    up, down = rnd((2 * 20, 40), torch.bfloat16, 8, 0.1).requires_grad_(), rnd((40, 20), torch.bfloat16, 9, 0.1).requires_grad_()
+    odd, odd_up = rnd((6, 39), torch.bfloat16, 5).requires_grad_(), rnd((2 * 20, 39), torch.bfloat16, 6, 0.1).requires_grad_()
+    odd_down = rnd((40, 19), torch.bfloat16, 7, 0.1).requires_grad_()
+    calls = {"dropout": lambda: ops.dropout(x, 0.5, rng_of(1)),
+             "join": lambda: sum(ops.block_join(x, y, post_weight=w, gate=g, dropout=0.5, rng=rng_of(2), pre_weight=w)),
+             "ffn": lambda: ops.gated_ffn(x, up, down), "odd": lambda: ops.gated_ffn(odd, odd_up[:38], odd_down)}
+    for name, call in calls.items():
+        counted = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: counted.append(t) or t, lambda t: t):
+            out = call()
+        out.float().sum().backward()
+        for k in range(len(counted)):
+            print(f"case changed {name} {k}", flush=True)
+            seen = []
+
+            def unpack(t, k=k):
+                seen.append(t)
+                return change(t) if len(seen) - 1 == k else t
+
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+                out = call()
+            with pytest.raises((RuntimeError, IndexError)):
+                out.backward(torch.ones_like(out))
+                torch.cuda.synchronize()
