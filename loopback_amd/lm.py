@@ -321,14 +321,28 @@ class LoopbackLM(nn.Module):
         if self.cfg.tie_word_embeddings:
             self.head.weight = self.embed.weight
 
-    def hidden(self, ids: torch.Tensor) -> torch.Tensor:
+    def next_rng(self) -> torch.Tensor | None:
+        """The generator of a training forward, a copy that later ones do not change, and the model's own moved on by a step; None
+        where the model drops nothing. For forward and hidden where one forward's computation may run again (activation
+        checkpointing), which has to draw the same masks."""
+        if not (self.cfg.dropout > 0.0 and self.training):
+            return None
+        # A forward that a backward computes again would take the next step's masks: the gradients of another function.
+        if not torch.compiler.is_compiling() and torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("a forward with dropout that runs inside a backward pass (activation checkpointing) needs the "
+                               "generator of the one it repeats: rng = model.next_rng() before it, model(ids, rng) in it")
+        rng = self.rng.clone()
+        with torch.no_grad():
+            self.rng[1] += 1
+        return rng
+
+    def hidden(self, ids: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
+        """rng: the step's dropout generator (next_rng); None takes the model's next one."""
         cfg = self.cfg
         h = self.embed(ids)
         at = {}      # where a block drops: the step's generator, and its place (two per block application, 0 the embedding's)
         if cfg.dropout > 0.0 and self.training:
-            rng = self.rng.clone()   # the backward's own: the next forward's step does not change it
-            with torch.no_grad():
-                self.rng[1] += 1
+            rng = self.next_rng() if rng is None else rng
             h = block_ops.dropout(h, cfg.dropout, rng)
             at = {"rng": rng, "site": 1}
 
@@ -365,8 +379,8 @@ class LoopbackLM(nn.Module):
             h = run(blk, h)
         return add_norm(self.norm, h)[1]
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
-        return ops.next_token_loss(self.head(self.hidden(ids)), ids)
+    def forward(self, ids: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
+        return ops.next_token_loss(self.head(self.hidden(ids, rng)), ids)
 
     def num_params(self) -> int:
         seen = {id(p): p.numel() for p in self.parameters()}
