@@ -297,15 +297,16 @@ def _ffn_backward(dy, x, w_gate_up, w_down, activation, need):
     x2, dy2 = x.reshape(-1, x.shape[-1]), dy.reshape(-1, dy.shape[-1])
     g, u = (_upcast(t) for t in (x2 @ w_gate_up.t()).chunk(2, dim=-1))
     if activation == 0:
-        q, dq = g, 1.0
+        c, q, dq = g, g, 1.0
     else:
-        q, dq = 1.5957691216057308 * (g + 0.044715 * g.pow(3)), 1.5957691216057308 * (1 + 0.134145 * g.pow(2))
+        c = g.clamp(-100.0, 100.0)   # past these s is 0 or 1 and its derivative 0, and dq would overflow
+        q, dq = 1.5957691216057308 * (c + 0.044715 * c.pow(3)), 1.5957691216057308 * (1 + 0.134145 * c.pow(2))
     s = torch.sigmoid(q)
     a = g * s
     out = [None, None, None]
     if need & 3:
         dact = _upcast(dy2 @ w_down)
-        dgu = torch.cat((dact * u * (s + a * dq * (1 - s)), dact * a), -1).to(dt)
+        dgu = torch.cat((dact * u * (s + c * s * dq * (1 - s)), dact * a), -1).to(dt)
         out[0] = (dgu @ w_gate_up).reshape(x.shape) if need & 1 else None
         out[1] = dgu.t() @ x2 if need & 2 else None
     if need & 4:
