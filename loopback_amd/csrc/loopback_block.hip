@@ -351,13 +351,9 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
         dhr[v] = a.dh ? load8<T, AL>(a.dh + ro, col, d) : IO<T>::zero();
         yr[v] = load8<T, AL>(a.y + ro, col, d);
       }
-      if constexpr (R > 1) {   // a row that is not there adds nothing to the column sums
-#pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-          if (has_dn) dnr[v] = zero_unless<T>(ok, dnr[v]);
-          dhr[v] = zero_unless<T>(ok, dhr[v]);
-        }
-      }
+      // a row that is not there (its lanes work on the last one again) adds nothing to the column sums: not zeros either, which
+      // would be NaN beside an infinite factor
+      const bool there = R == 1 || ok;
       if (a.gate && row / a.gate_rows != gate_row) {
         gate_row = row / a.gate_rows;
 #pragma unroll
@@ -400,7 +396,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             h[v][k] += z[k];
-            d_pre[v][k] = __builtin_fmaf(g[v][k], h[v][k] * q2, d_pre[v][k]);
+            if (there) d_pre[v][k] = __builtin_fmaf(g[v][k], h[v][k] * q2, d_pre[v][k]);
             g[v][k] *= e[k];
             c = __builtin_fmaf(g[v][k], h[v][k], c);
           }
@@ -436,7 +432,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             og[k] = g[v][k] * (has_post ? e[k] * q1 * w[k] : e[k]);
-            d_gate[v][k] += og[k];
+            if (there) d_gate[v][k] += og[k];
             g[v][k] *= gt[k];
           }
           if (a.dgate && a.gate_rows == 1 && ok) store8<T, AL>(a.dgate + ro, 8 * blk, d, og);
@@ -444,7 +440,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
         if (has_post) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            d_post[v][k] = __builtin_fmaf(g[v][k], e[k] * q1, d_post[v][k]);
+            if (there) d_post[v][k] = __builtin_fmaf(g[v][k], e[k] * q1, d_post[v][k]);
             g[v][k] *= w[k];
             c = __builtin_fmaf(g[v][k], e[k], c);
           }

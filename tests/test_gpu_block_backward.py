@@ -106,3 +106,21 @@ def test_saved_tensors_that_a_hook_changed(change):
             with pytest.raises((RuntimeError, IndexError)):
                 out.backward(torch.ones_like(out))
                 torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [8, 40, 200, 768, 1001])
+def test_infinite_in_the_last_row(d, dtype):
+    """An infinity in the last of a few rows, which the lanes of rows past the end look at too, gives the gate the gradient of the
+    formula: infinite in its column, finite in the others."""
+    from loopback_amd import block_ops as ops
+    print(f"case infinite {d} {dtype}", flush=True)
+    for shape, gshape in (((3, d), (d,)), ((2, 3, d), (2, 1, d)), ((1, d), (d,))):
+        x, y, dh = (rnd(shape, dtype, k) for k in (1, 2, 3))
+        gate = rnd((d,), dtype, 4).expand(gshape).contiguous().requires_grad_()
+        y.view(-1, d)[-1, 5] = float("inf")
+        dh.view(-1, d)[-1, 5] = 2.0
+        h, _ = ops.block_join(x, y, gate=gate)
+        got, = torch.autograd.grad(h, gate, dh)
+        want = (dh.double() * y.double()).flatten(0, -2).sum(0) if len(gshape) == 1 else (dh.double() * y.double()).sum(1, keepdim=True)
+        assert want.isinf().sum() == 1 and torch.equal(got.isinf(), want.isinf()) and not got.isnan().any(), (shape, got, want)
