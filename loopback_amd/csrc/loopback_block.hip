@@ -119,7 +119,7 @@ __global__ __launch_bounds__(WG) void k_dropout(const T* __restrict__ x, const i
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// block join. LPR lanes share a row, VPT vectors of eight columns each; the workgroup's lanes / LPR rows go side by side.
+// block join. LPR lanes share a row, eight columns each; the workgroup's lanes / LPR rows go side by side.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int lanes_of(int lpr) { return lpr > WG ? lpr : WG; }
 
@@ -163,27 +163,22 @@ template <typename T> struct JoinFwd {
 
 // Reads x and y, writes h and n and two statistics a row: the rows' stream bounds it. 16384 x 768 in bf16 with all parts 21 us (4.8
 // TB/s), 6825 x 2048 in fp16 23 us (4.9 TB/s). LPR lanes to a row of LPR x 8 columns at most, so that a lane holds its
-// eight in registers; rows are given to workgroups by plan_of.
+// eight in registers.
 // PARTS: which parts the call has, known when the kernel is compiled (1 the norm before the next block, 2 the norm after this
 // one, 4 dropout), or ANY: looked up as it runs (rows that take the narrow loads)
 constexpr int ANY = -1;
-template <typename T, int LPR, int VPT, bool AL, int PARTS>
+template <typename T, int LPR, bool AL, int PARTS>
 __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) {
   const bool has_pre = PARTS < 0 ? a.pre != nullptr : PARTS & 1, has_post = PARTS < 0 ? a.post != nullptr : PARTS & 2,
              drops = PARTS < 0 ? a.drop != 0 : PARTS & 4;
   constexpr int LANES = lanes_of(LPR), R = LANES / LPR;
   __shared__ float s_red[2][LANES / 64];
   RowSum<LPR> row_sum{s_red};
-  const int d = a.d, lane = (int)threadIdx.x % LPR, grp = group_of<LPR>();
+  const int d = a.d, lane = (int)threadIdx.x % LPR, col = 8 * lane, grp = group_of<LPR>();
   const float inv_d = 1.f / (float)d;
-  typename IO<T>::Raw post[VPT], pre[VPT], gate[VPT];
-#pragma unroll
-  for (int v = 0; v < VPT; ++v) {
-    const int col = 8 * (lane + LPR * v);
-    post[v] = has_post ? load8<T, AL>(a.post, col, d) : IO<T>::zero();
-    pre[v] = has_pre ? load8<T, AL>(a.pre, col, d) : IO<T>::zero();
-    gate[v] = IO<T>::zero();
-  }
+  const typename IO<T>::Raw post = has_post ? load8<T, AL>(a.post, col, d) : IO<T>::zero(),
+                            pre = has_pre ? load8<T, AL>(a.pre, col, d) : IO<T>::zero();
+  typename IO<T>::Raw gate = IO<T>::zero();
   Rng rng{0, 0, 0};
   if (drops) rng = rng_of(a.rng);
   int gate_row = -1;
@@ -192,68 +187,49 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_fwd(const JoinFwd<T> a) 
     const bool ok = mine < a.rows;
     const int row = (int)(ok ? mine : a.rows - 1);
     const int64_t ro = (int64_t)row * d;
-    typename IO<T>::Raw xr[VPT], yr[VPT];
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      xr[v] = load8<T, AL>(a.x + ro, 8 * (lane + LPR * v), d);
-      yr[v] = load8<T, AL>(a.y + ro, 8 * (lane + LPR * v), d);
-    }
+    const typename IO<T>::Raw xr = load8<T, AL>(a.x + ro, col, d), yr = load8<T, AL>(a.y + ro, col, d);
     if (a.gate && row / a.gate_rows != gate_row) {
       gate_row = row / a.gate_rows;
-#pragma unroll
-      for (int v = 0; v < VPT; ++v) gate[v] = load8<T, AL>(a.gate + (int64_t)gate_row * d, 8 * (lane + LPR * v), d);
+      gate = load8<T, AL>(a.gate + (int64_t)gate_row * d, col, d);
     }
     float r1 = 1.f;
     if (has_post) {
-      float ss = 0.f;
+      float e[8], ss = 0.f;
+      IO<T>::unpack(yr, e);
 #pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        float e[8];
-        IO<T>::unpack(yr[v], e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ss = __builtin_fmaf(e[k], e[k], ss);
-      }
+      for (int k = 0; k < 8; ++k) ss = __builtin_fmaf(e[k], e[k], ss);
       r1 = rsqrtf(row_sum(ss) * inv_d + a.eps);
       if (a.r_post && lane == 0 && ok) a.r_post[row] = r1;
     }
-    float h[VPT][8], ss = 0.f;
+    float h[8], z[8], e[8], ss = 0.f;
+    IO<T>::unpack(yr, z);
+    if (has_post) {
+      IO<T>::unpack(post, e);
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      float z[8], e[8];
-      IO<T>::unpack(yr[v], z);
-      if (has_post) {
-        IO<T>::unpack(post[v], e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) z[k] *= r1 * e[k];
-      }
-      if (a.gate) {
-        IO<T>::unpack(gate[v], e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) z[k] *= e[k];
-      }
-      const int blk = lane + LPR * v;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) z[k] *= a.scale;
-      if (drops) drop8(z, philox((uint32_t)blk, (uint32_t)row, a.site, rng), a.drop, a.keep);
-      IO<T>::unpack(xr[v], h[v]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        h[v][k] += z[k];
-        ss = __builtin_fmaf(h[v][k], h[v][k], ss);
-      }
-      if (ok) store8<T, AL>(a.h + ro, 8 * blk, d, h[v]);
+      for (int k = 0; k < 8; ++k) z[k] *= r1 * e[k];
     }
+    if (a.gate) {
+      IO<T>::unpack(gate, e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z[k] *= e[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] *= a.scale;
+    if (drops) drop8(z, philox((uint32_t)lane, (uint32_t)row, a.site, rng), a.drop, a.keep);
+    IO<T>::unpack(xr, h);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      h[k] += z[k];
+      ss = __builtin_fmaf(h[k], h[k], ss);
+    }
+    if (ok) store8<T, AL>(a.h + ro, col, d, h);
     if (has_pre) {
       const float r2 = rsqrtf(row_sum(ss) * inv_d + a.eps);
       if (a.r_pre && lane == 0 && ok) a.r_pre[row] = r2;
+      IO<T>::unpack(pre, e);
 #pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        float e[8];
-        IO<T>::unpack(pre[v], e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] *= h[v][k] * r2;
-        if (ok) store8<T, AL>(a.n + ro, 8 * (lane + LPR * v), d, e);
-      }
+      for (int k = 0; k < 8; ++k) e[k] *= h[k] * r2;
+      if (ok) store8<T, AL>(a.n + ro, col, d, e);
     }
   }
 }
@@ -278,44 +254,33 @@ template <typename T> struct JoinBwd {
 // rows: 16384 x 768 in bf16 with all parts 42 us (3.6 TB/s; two vectors a lane on half the lanes took 72, held to fewer registers
 // 121 to 210 with spills; loading the next row ahead changed nothing, 43.4 against 43.7), 6825 x 2048 in fp16 without dropout 36
 // us (4.7 TB/s).
-template <typename T, int LPR, int VPT, bool AL, int PARTS>
+template <typename T, int LPR, bool AL, int PARTS>
 __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) {
   const bool has_dn = PARTS < 0 ? a.dn != nullptr : PARTS & 1, has_post = PARTS < 0 ? a.post != nullptr : PARTS & 2,
              drops = PARTS < 0 ? a.drop != 0 : PARTS & 4;
-  constexpr int LANES = lanes_of(LPR), R = LANES / LPR, W = 8 * LPR * VPT;
+  constexpr int LANES = lanes_of(LPR), R = LANES / LPR, W = 8 * LPR;
   __shared__ float s_red[2][LANES / 64];
   __shared__ float s_sum[R > 1 ? R * W : 1];
   RowSum<LPR> row_sum{s_red};
-  const int d = a.d, lane = (int)threadIdx.x % LPR, grp = group_of<LPR>();
+  const int d = a.d, lane = (int)threadIdx.x % LPR, col = 8 * lane, grp = group_of<LPR>();
   const float inv_d = 1.f / (float)d;
-  typename IO<T>::Raw post[VPT], pre[VPT], gate[VPT];
-  float d_post[VPT][8], d_pre[VPT][8], d_gate[VPT][8];
+  typename IO<T>::Raw post = has_post ? load8<T, AL>(a.post, col, d) : IO<T>::zero(),
+                      pre = has_dn ? load8<T, AL>(a.pre, col, d) : IO<T>::zero(), gate = IO<T>::zero();
+  float d_post[8], d_pre[8], d_gate[8];
 #pragma unroll
-  for (int v = 0; v < VPT; ++v) {
-    const int col = 8 * (lane + LPR * v);
-    post[v] = has_post ? load8<T, AL>(a.post, col, d) : IO<T>::zero();
-    pre[v] = has_dn ? load8<T, AL>(a.pre, col, d) : IO<T>::zero();
-    gate[v] = IO<T>::zero();
-#pragma unroll
-    for (int k = 0; k < 8; ++k) d_post[v][k] = d_pre[v][k] = d_gate[v][k] = 0.f;
-  }
+  for (int k = 0; k < 8; ++k) d_post[k] = d_pre[k] = d_gate[k] = 0.f;
   Rng rng{0, 0, 0};
   if (drops) rng = rng_of(a.rng);
   int gate_row = -1;
 
   // the row groups' column sums, added in order, to out (fp32) or out_t (rounded)
-  auto flush = [&](float (&acc)[VPT][8], float* out, T* out_t) {
+  auto flush = [&](float (&acc)[8], float* out, T* out_t) {
     if constexpr (R == 1) {
-#pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        const int col = 8 * (lane + LPR * v);
-        if (out) store8<float, AL>(out, col, d, acc[v]);
-        else store8<T, AL>(out_t, col, d, acc[v]);
-      }
+      if (out) store8<float, AL>(out, col, d, acc);
+      else store8<T, AL>(out_t, col, d, acc);
     } else {
       __syncthreads();
-#pragma unroll
-      for (int v = 0; v < VPT; ++v) IO<float>::store(s_sum + grp * W + 8 * (lane + LPR * v), acc[v]);
+      IO<float>::store(s_sum + grp * W + col, acc);
       __syncthreads();
       for (int c = (int)threadIdx.x; c < d; c += LANES) {
         float t = s_sum[c];
@@ -325,9 +290,7 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
       }
     }
 #pragma unroll
-    for (int v = 0; v < VPT; ++v)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) acc[v][k] = 0.f;
+    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
   };
 
   const bool runs = a.dgate && a.gate_rows > 1;   // gate sums over runs of rows
@@ -340,126 +303,95 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
       const bool ok = row0 + grp < s1;
       const int row = (int)(ok ? row0 + grp : s1 - 1);
       const int64_t ro = (int64_t)row * d;
-      typename IO<T>::Raw xr[VPT], yr[VPT], dhr[VPT], dnr[VPT];
-#pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        const int col = 8 * (lane + LPR * v);
-        if (has_dn) {
-          dnr[v] = load8<T, AL>(a.dn + ro, col, d);
-          xr[v] = load8<T, AL>(a.x + ro, col, d);
-        }
-        dhr[v] = a.dh ? load8<T, AL>(a.dh + ro, col, d) : IO<T>::zero();
-        yr[v] = load8<T, AL>(a.y + ro, col, d);
+      typename IO<T>::Raw xr, yr, dhr, dnr;
+      if (has_dn) {
+        dnr = load8<T, AL>(a.dn + ro, col, d);
+        xr = load8<T, AL>(a.x + ro, col, d);
       }
+      dhr = a.dh ? load8<T, AL>(a.dh + ro, col, d) : IO<T>::zero();
+      yr = load8<T, AL>(a.y + ro, col, d);
       // a row that is not there (its lanes work on the last one again) adds nothing to the column sums: not zeros either, which
       // would be NaN beside an infinite factor
       const bool there = R == 1 || ok;
       if (a.gate && row / a.gate_rows != gate_row) {
         gate_row = row / a.gate_rows;
-#pragma unroll
-        for (int v = 0; v < VPT; ++v) gate[v] = load8<T, AL>(a.gate + (int64_t)gate_row * d, 8 * (lane + LPR * v), d);
+        gate = load8<T, AL>(a.gate + (int64_t)gate_row * d, col, d);
       }
-#pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        anew<T>(post[v]);
-        anew<T>(pre[v]);
-        anew<T>(gate[v]);
-      }
+      anew<T>(post);
+      anew<T>(pre);
+      anew<T>(gate);
       const float q2 = has_dn ? a.r_pre[row] : 0.f, q1 = has_post ? a.r_post[row] : 1.f;
-      uint4 words[VPT];
-#pragma unroll
-      for (int v = 0; v < VPT; ++v)
-        words[v] = drops ? philox((uint32_t)(lane + LPR * v), (uint32_t)row, a.site, rng) : make_uint4(0u, 0u, 0u, 0u);
-      float g[VPT][8];   // the gradient of h
+      const uint4 words = drops ? philox((uint32_t)lane, (uint32_t)row, a.site, rng) : make_uint4(0u, 0u, 0u, 0u);
+      float g[8];   // the gradient of h
       if (has_dn) {
-        float h[VPT][8], c = 0.f;   // h before its rounding; sum dn pre h
+        float h[8], e[8], z[8], c = 0.f;   // h before its rounding; sum dn pre h
+        IO<T>::unpack(yr, z);
+        if (has_post) {
+          IO<T>::unpack(post, e);
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-          float e[8], z[8];
-          IO<T>::unpack(yr[v], z);
-          if (has_post) {
-            IO<T>::unpack(post[v], e);
+          for (int k = 0; k < 8; ++k) z[k] *= q1 * e[k];
+        }
+        if (a.gate) {
+          IO<T>::unpack(gate, e);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) z[k] *= q1 * e[k];
-          }
-          if (a.gate) {
-            IO<T>::unpack(gate[v], e);
+          for (int k = 0; k < 8; ++k) z[k] *= e[k];
+        }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) z[k] *= e[k];
-          }
+        for (int k = 0; k < 8; ++k) z[k] *= a.scale;
+        if (drops) drop8(z, words, a.drop, a.keep);
+        IO<T>::unpack(xr, h);
+        IO<T>::unpack(dnr, g);
+        IO<T>::unpack(pre, e);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) z[k] *= a.scale;
-          if (drops) drop8(z, words[v], a.drop, a.keep);
-          IO<T>::unpack(xr[v], h[v]);
-          IO<T>::unpack(dnr[v], g[v]);
-          IO<T>::unpack(pre[v], e);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            h[v][k] += z[k];
-            if (there) d_pre[v][k] = __builtin_fmaf(g[v][k], h[v][k] * q2, d_pre[v][k]);
-            g[v][k] *= e[k];
-            c = __builtin_fmaf(g[v][k], h[v][k], c);
-          }
+        for (int k = 0; k < 8; ++k) {
+          h[k] += z[k];
+          if (there) d_pre[k] = __builtin_fmaf(g[k], h[k] * q2, d_pre[k]);
+          g[k] *= e[k];
+          c = __builtin_fmaf(g[k], h[k], c);
         }
         c = row_sum(c) * q2 * q2 * inv_d;
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-          float e[8];
+        for (int k = 0; k < 8; ++k) g[k] = q2 * (g[k] - c * h[k]);
+        IO<T>::unpack(dhr, e);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) g[v][k] = q2 * (g[v][k] - c * h[v][k]);
-          IO<T>::unpack(dhr[v], e);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) g[v][k] += e[k];
-        }
+        for (int k = 0; k < 8; ++k) g[k] += e[k];
       } else {
-#pragma unroll
-        for (int v = 0; v < VPT; ++v) IO<T>::unpack(dhr[v], g[v]);
+        IO<T>::unpack(dhr, g);
       }
       float c = 0.f;       // sum of the normed row's gradient times y
+      if (a.dx && ok) store8<T, AL>(a.dx + ro, col, d, g);
+      float e[8], w[8], gt[8];
+      IO<T>::unpack(yr, e);
+      IO<T>::unpack(post, w);
+      IO<T>::unpack(gate, gt);
 #pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        const int blk = lane + LPR * v;
-        if (a.dx && ok) store8<T, AL>(a.dx + ro, 8 * blk, d, g[v]);
-        float e[8], w[8], gt[8];
-        IO<T>::unpack(yr[v], e);
-        IO<T>::unpack(post[v], w);
-        IO<T>::unpack(gate[v], gt);
+      for (int k = 0; k < 8; ++k) g[k] *= a.scale;
+      if (drops) drop8(g, words, a.drop, a.keep);
+      if (a.gate) {
+        float og[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g[v][k] *= a.scale;
-        if (drops) drop8(g[v], words[v], a.drop, a.keep);
-        if (a.gate) {
-          float og[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            og[k] = g[v][k] * (has_post ? e[k] * q1 * w[k] : e[k]);
-            if (there) d_gate[v][k] += og[k];
-            g[v][k] *= gt[k];
-          }
-          if (a.dgate && a.gate_rows == 1 && ok) store8<T, AL>(a.dgate + ro, 8 * blk, d, og);
+        for (int k = 0; k < 8; ++k) {
+          og[k] = g[k] * (has_post ? e[k] * q1 * w[k] : e[k]);
+          if (there) d_gate[k] += og[k];
+          g[k] *= gt[k];
         }
-        if (has_post) {
+        if (a.dgate && a.gate_rows == 1 && ok) store8<T, AL>(a.dgate + ro, col, d, og);
+      }
+      if (has_post) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (there) d_post[v][k] = __builtin_fmaf(g[v][k], e[k] * q1, d_post[v][k]);
-            g[v][k] *= w[k];
-            c = __builtin_fmaf(g[v][k], e[k], c);
-          }
+        for (int k = 0; k < 8; ++k) {
+          if (there) d_post[k] = __builtin_fmaf(g[k], e[k] * q1, d_post[k]);
+          g[k] *= w[k];
+          c = __builtin_fmaf(g[k], e[k], c);
         }
       }
       if (a.dy) {
         if (has_post) {
           c = row_sum(c) * q1 * q1 * inv_d;
 #pragma unroll
-          for (int v = 0; v < VPT; ++v) {
-            float e[8];
-            IO<T>::unpack(yr[v], e);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) g[v][k] = q1 * (g[v][k] - c * e[k]);
-          }
+          for (int k = 0; k < 8; ++k) g[k] = q1 * (g[k] - c * e[k]);
         }
-#pragma unroll
-        for (int v = 0; v < VPT; ++v)
-          if (ok) store8<T, AL>(a.dy + ro, 8 * (lane + LPR * v), d, g[v]);
+        if (ok) store8<T, AL>(a.dy + ro, col, d, g);
       }
     }
     if (runs) {
@@ -538,18 +470,16 @@ inline bool dtype_ok(int dt) { return dt == LDR_F32 || dt == LDR_BF16 || dt == L
 inline unsigned grid_of(int64_t blocks, int64_t cap) { return (unsigned)(blocks < cap ? blocks : cap); }
 inline int launched() { return (int)hipGetLastError(); }
 
-// lanes per row: the fewest that hold it in two vectors each up to a wave, in one beyond
-struct Shape { int lpr, vpt; };
-inline Shape shape_of(int64_t d) {
-  return d <= 32 ? Shape{4, 1} : d <= 128 ? Shape{16, 1} : d <= 512 ? Shape{64, 1} : d <= 1024 ? Shape{128, 1}
-       : d <= 2048 ? Shape{256, 1} : d <= 4096 ? Shape{512, 1} : Shape{1024, 1};
+// lanes per row, eight columns each: 4, 16 or 64 of a wave, or 2 to 16 waves
+inline int lanes_per_row(int64_t d) {
+  return d <= 32 ? 4 : d <= 128 ? 16 : d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024;
 }
 
 // workgroups of the backward and the consecutive rows each takes: three workgroups per CU of 256 lanes where there are rows
 // for them. Gate runs no longer than that are not cut.
 struct Plan { int64_t per, parts; };
 inline Plan plan_of(int64_t rows, int64_t d, int64_t gate_rows) {
-  const int lpr = shape_of(d).lpr, r = lpr > WG ? 1 : WG / lpr;
+  const int lpr = lanes_per_row(d), r = lpr > WG ? 1 : WG / lpr;
   const int64_t most = lpr > 512 ? 256 : lpr > WG ? 384 : 768;
   int64_t per = (rows + most - 1) / most;
   per = (per + r - 1) / r * r;
@@ -561,15 +491,15 @@ inline Plan plan_of(int64_t rows, int64_t d, int64_t gate_rows) {
   if ((DT) == LDR_BF16) { typedef bf16_t T; __VA_ARGS__; }       \
   else if ((DT) == LDR_F16) { typedef _Float16 T; __VA_ARGS__; } \
   else { typedef float T; __VA_ARGS__; }
-#define LBK_SHAPE_SWITCH(S, ...)                                                          \
-  switch ((S).lpr) {                                                                      \
-    case 4: { constexpr int LPR = 4, VPT = 1; __VA_ARGS__; } break;                       \
-    case 16: { constexpr int LPR = 16, VPT = 1; __VA_ARGS__; } break;                     \
-    case 64: { constexpr int LPR = 64, VPT = 1; __VA_ARGS__; } break;                     \
-    case 128: { constexpr int LPR = 128, VPT = 1; __VA_ARGS__; } break;                   \
-    case 256: { constexpr int LPR = 256, VPT = 1; __VA_ARGS__; } break;                   \
-    case 512: { constexpr int LPR = 512, VPT = 1; __VA_ARGS__; } break;                   \
-    default: { constexpr int LPR = 1024, VPT = 1; __VA_ARGS__; } break;                   \
+#define LBK_LANES_SWITCH(N, ...)                                      \
+  switch (N) {                                                        \
+    case 4: { constexpr int LPR = 4; __VA_ARGS__; } break;            \
+    case 16: { constexpr int LPR = 16; __VA_ARGS__; } break;          \
+    case 64: { constexpr int LPR = 64; __VA_ARGS__; } break;          \
+    case 128: { constexpr int LPR = 128; __VA_ARGS__; } break;        \
+    case 256: { constexpr int LPR = 256; __VA_ARGS__; } break;        \
+    case 512: { constexpr int LPR = 512; __VA_ARGS__; } break;        \
+    default: { constexpr int LPR = 1024; __VA_ARGS__; } break;        \
   }
 
 #define LBK_PARTS_SWITCH(P, ...)                                 \
@@ -633,9 +563,8 @@ int lbk_join_fwd(const void* x, const void* y, const void* post, const void* gat
     if (!al_of(p, dtype)) return LDR_E_ALIGN;
     al = al && al16(p);
   }
-  const Shape s = shape_of(d);
-  const int r = s.lpr > WG ? 1 : WG / s.lpr;
-  const unsigned grid = grid_of((rows + r - 1) / r, s.lpr > WG ? 1024 : 2048);
+  const int lpr = lanes_per_row(d), r = lpr > WG ? 1 : WG / lpr;
+  const unsigned grid = grid_of((rows + r - 1) / r, lpr > WG ? 1024 : 2048);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t gr = !gate || gate_rows > rows ? rows : gate_rows;
   LBK_TYPE_SWITCH(dtype, {
@@ -643,12 +572,12 @@ int lbk_join_fwd(const void* x, const void* y, const void* post, const void* gat
                        static_cast<const T*>(gate), static_cast<const T*>(pre), rng, static_cast<T*>(h),
                        static_cast<T*>(n), r_post, r_pre, (int)rows, (int)d, (int)gr, site, (uint32_t)drop, scale,
                        keep_scale(drop), eps};
-    LBK_SHAPE_SWITCH(s, {
+    LBK_LANES_SWITCH(lpr, {
       if (al) {
         LBK_PARTS_SWITCH((pre ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
-                         hipLaunchKernelGGL((k_join_fwd<T, LPR, VPT, true, PARTS>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a))
+                         hipLaunchKernelGGL((k_join_fwd<T, LPR, true, PARTS>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a))
       } else {
-        hipLaunchKernelGGL((k_join_fwd<T, LPR, VPT, false, ANY>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a);
+        hipLaunchKernelGGL((k_join_fwd<T, LPR, false, ANY>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a);
       }
     })
   })
@@ -680,7 +609,6 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* x, const void* y, c
   if (!al_of(scratch, LDR_F32) || !al_of(dpost, dtype) || !al_of(dpre, dtype)) return LDR_E_ALIGN;
   const int64_t gr = !gate || gate_rows > rows ? rows : gate_rows;
   const Plan plan = plan_of(rows, d, gate ? gate_rows : rows);
-  const Shape s = shape_of(d);
   const int parts = (int)plan.parts;
   hipStream_t st = static_cast<hipStream_t>(stream);
   LBK_TYPE_SWITCH(dtype, {
@@ -690,15 +618,15 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* x, const void* y, c
                        static_cast<T*>(dgate), dpost ? scratch : nullptr, dpre ? scratch + parts * d : nullptr,
                        scratch + 2 * parts * d, (int)rows, (int)d, (int)gr, (int)plan.per, site, (uint32_t)drop, scale,
                        keep_scale(drop)};
-    LBK_SHAPE_SWITCH(s, {
+    LBK_LANES_SWITCH(lanes_per_row(d), {
       if (al) {
         LBK_PARTS_SWITCH((dn ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
-                         hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, true, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
+                         hipLaunchKernelGGL((k_join_bwd<T, LPR, true, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
       } else if constexpr (LPR == 1024) {   // 128 registers a lane: looked up, 108 spill (16384 x 5001: 999 us, 473 so)
         LBK_PARTS_SWITCH((dn ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
-                         hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, false, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
+                         hipLaunchKernelGGL((k_join_bwd<T, LPR, false, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
       } else {
-        hipLaunchKernelGGL((k_join_bwd<T, LPR, VPT, false, ANY>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a);
+        hipLaunchKernelGGL((k_join_bwd<T, LPR, false, ANY>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a);
       }
     })
     const int err = launched();
