@@ -39,6 +39,7 @@ template <typename T> __device__ __forceinline__ typename IO<T>::Raw zero_unless
 // the same values, looked at anew: what is unpacked from them in a loop is not kept in twice the registers outside it
 template <typename T> __device__ __forceinline__ void anew(typename IO<T>::Raw& r) {
   if constexpr (!std::is_same<T, float>::value) asm volatile("" : "+v"(r.u.x), "+v"(r.u.y), "+v"(r.u.z), "+v"(r.u.w));
+  else asm volatile("" : "+v"(r.a.x), "+v"(r.a.y), "+v"(r.a.z), "+v"(r.a.w), "+v"(r.b.x), "+v"(r.b.y), "+v"(r.b.z), "+v"(r.b.w));
 }
 template <typename T> struct Eight { T e[8]; };
 template <typename T, bool AL> __device__ __forceinline__ typename IO<T>::Raw load8(const T* p, int col, int d) {
@@ -254,6 +255,8 @@ template <typename T> struct JoinBwd {
 // rows: 16384 x 768 in bf16 with all parts 42 us (3.6 TB/s; two vectors a lane on half the lanes took 72, held to fewer registers
 // 121 to 210 with spills; loading the next row ahead changed nothing, 43.4 against 43.7), 6825 x 2048 in fp16 without dropout 36
 // us (4.7 TB/s).
+// Rows wider than 4096 take 16 waves of 128 registers: with both norms some are spilled (12 to 108 bytes a lane). 512 lanes of two
+// vectors spill nothing and are slower: 16384 x 5001 in bf16 394 -> 470 us, 8192 x 8192 226 -> 255.
 template <typename T, int LPR, bool AL, int PARTS>
 __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) {
   const bool has_dn = PARTS < 0 ? a.dn != nullptr : PARTS & 1, has_post = PARTS < 0 ? a.post != nullptr : PARTS & 2,
@@ -350,6 +353,11 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_join_bwd(const JoinBwd<T> a) 
           c = __builtin_fmaf(g[k], h[k], c);
         }
         c = row_sum(c) * q2 * q2 * inv_d;
+        if constexpr (LPR > 512) {   // 128 registers a lane: fewer unpacked values kept (bf16 8192 x 8192 251 -> 197 us)
+          anew<T>(yr);
+          anew<T>(post);
+          anew<T>(gate);
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) g[k] = q2 * (g[k] - c * h[k]);
         IO<T>::unpack(dhr, e);
@@ -622,7 +630,7 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* x, const void* y, c
       if (al) {
         LBK_PARTS_SWITCH((dn ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
                          hipLaunchKernelGGL((k_join_bwd<T, LPR, true, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
-      } else if constexpr (LPR == 1024) {   // 128 registers a lane: looked up, 108 spill (16384 x 5001: 999 us, 473 so)
+      } else if constexpr (LPR == 1024) {   // 128 registers a lane: looked up, 108 spill (16384 x 5001 with all parts: 999 us, 390 so)
         LBK_PARTS_SWITCH((dn ? 1 : 0) + (post ? 2 : 0) + (drop ? 4 : 0),
                          hipLaunchKernelGGL((k_join_bwd<T, LPR, false, PARTS>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
       } else {
