@@ -211,7 +211,7 @@ class SwiGLU(nn.Module):
         if torch.jit.is_scripting():   # a scripted layer is torch operations
             g, u = self.gate_up(x).chunk(2, dim=-1)
             y = self.down(F.silu(g) * u)
-        elif self.fused and _plain_linear(self.gate_up) and _plain_linear(self.down):
+        elif self.fused and isinstance(x, torch.Tensor) and _plain_linear(self.gate_up) and _plain_linear(self.down):
             y = block_ops.gated_ffn(x, self.gate_up.weight, self.down.weight)
         else:
             y = linear(self.down, ops.swiglu(linear(self.gate_up, x)))
@@ -238,11 +238,17 @@ def add_norm(norm: nn.Module, x: torch.Tensor, add: torch.Tensor | None = None):
 
 def join_norm(norm: nn.Module | None, x: torch.Tensor, y: torch.Tensor, post: nn.Module | None = None, **how):
     """(h, norm(h)) of h = x + what is left of y after the norm `post` and how's gate, scale and dropout (block_ops.block_join);
-    norm None: (h, None). Norms whose call is hooked, or of other classes, are called."""
+    norm None: (h, None). Norms whose call is hooked, or of other classes, are called. A torch.fx trace sees the modules and torch
+    operations."""
     def plain(m):
         return m is None or (type(m) in (nn.RMSNorm, RMSNorm) and m.eps is not None and m.weight is not None
                              and m.weight.dim() == 1 and not _hooked(m))
 
+    if not isinstance(x, torch.Tensor) and not how["dropout"]:
+        y = y if post is None else post(y)
+        y = y if how["gate"] is None else y * how["gate"]
+        h = x + y * how["scale"]
+        return h, None if norm is None else norm(h)
     if not plain(post):
         y, post = post(y), None
     called = None

@@ -1,0 +1,46 @@
+"""The language model's options from block_ops under torch.fx: layers built from them are traced as the default ones are."""
+import pytest
+import torch
+
+from loopback_amd import lm
+
+
+class AttentionLeaf(torch.fx.Tracer):
+    def is_leaf_module(self, m, name):
+        return isinstance(m, lm.Attention) or super().is_leaf_module(m, name)
+
+
+def cfg(**options):
+    return lm.LMConfig(hidden_size=128, num_heads=2, hidden_ratio=2, **options)
+
+
+def test_fused_feed_forward():
+    """A fused SwiGLU's trace has its linear layers as leaves and torch's operations between, with the eager results; it can be
+    scripted, and its layers quantized."""
+    torch.manual_seed(0)
+    mlp, x = lm.SwiGLU(cfg(ffn="fused")), torch.randn(2, 8, 128)
+    traced = torch.fx.symbolic_trace(mlp)
+    assert [n.target for n in traced.graph.nodes if n.op == "call_module"] == ["gate_up", "down"]
+    assert torch.allclose(traced(x), mlp(x), atol=1e-6) and torch.allclose(torch.jit.script(mlp)(x), mlp(x), atol=1e-6)
+    composed = lm.SwiGLU(cfg())
+    composed.load_state_dict(mlp.state_dict())
+    quantized = [torch.ao.quantization.quantize_dynamic(m, {torch.nn.Linear}, dtype=torch.qint8)(x) for m in (mlp, composed)]
+    assert torch.equal(*quantized) and not torch.equal(quantized[0], mlp(x))
+
+
+@pytest.mark.parametrize("options", [{"post_norm": True}, {"gate": 0.5}, {"residual_scale": 0.7}, {"ffn": "fused", "post_norm": True,
+                                     "gate": 0.5, "residual_scale": 0.7, "dropout": 0.2}])
+def test_block(options):
+    """A block's trace calls its norms, attention and linear layers, with the eager results (in fp32, to round-off); dropout is an
+    evaluation's, nothing."""
+    torch.manual_seed(0)
+    block, x = lm.Block(cfg(**options)).eval(), torch.randn(2, 8, 128)
+    with torch.no_grad():
+        for p in block.parameters():
+            p += 0.1 * torch.randn(p.shape)
+    tracer = AttentionLeaf()
+    graph = tracer.trace(block)
+    post = [["attn_post"], ["mlp_post"]] if "post_norm" in options else [[], []]
+    assert [n.target for n in graph.nodes if n.op == "call_module"] == \
+        ["attn_norm", "attn", *post[0], "mlp_norm", "mlp.gate_up", "mlp.down", *post[1]]
+    assert torch.allclose(torch.fx.GraphModule(tracer.root, graph)(x), block(x), atol=1e-5)
