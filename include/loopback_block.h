@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define LBK_ABI_VERSION 2   /* 2: lbk_join_bwd takes x in h's place */
+#define LBK_ABI_VERSION 3   /* 2: lbk_join_bwd takes x in h's place; 3: lbk_product_tiling */
 int lbk_abi_version(void);
 
 /* ---- dropout ----------------------------------------------------------------------------------------------------
@@ -81,6 +81,11 @@ int lbk_ffn_dgate_up(const void* dy, int64_t ld_dy, const void* w_down, int64_t 
  * The summed dimension is split where that fills the GPU; scratch has lbk_linear_scratch(columns and rows of the result,
  * summed dimension) floats (NULL where that is 0), 16-byte aligned. */
 int64_t lbk_linear_scratch(int64_t columns, int64_t rows, int64_t summed);
+
+/* Which tiles the product of a result of `columns` x `rows` takes on the tiled kernels: 0 is 128 x 128, 1 is 256 x 256 and
+ * 2 is 192 x 256 (columns x rows), and into *splits in how many the summed dimension is split. product: 0 the plain ones, 1 the
+ * gate and up projection (columns 2 n, rows t, summed d), 2 the gradients of the two (columns n, rows t, summed d). */
+int lbk_product_tiling(int product, int64_t columns, int64_t rows, int64_t summed, int* splits);
 int lbk_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t ldy, float* scratch, int64_t t,
                    int64_t k, int64_t n, int dtype, void* stream);
 int lbk_linear_dx(const void* dy, int64_t ld_dy, const void* w, int64_t ldw, void* dx, int64_t ld_dx, float* scratch, int64_t t,

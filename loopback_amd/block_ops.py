@@ -28,7 +28,7 @@ from . import _host as H      # the launch path (csrc/host.cpp), bound below to 
 from . import build as _build
 from .lm_ops import _stream, _watched, native
 
-ABI_VERSION = 2
+ABI_VERSION = 3
 JOIN_MAX_WIDTH = 8192
 FEW_TOKENS = 32
 FFN_MAX_WIDTH = 2 ** 22 - 8   # elements between rows of the tiled products' operands
@@ -49,6 +49,7 @@ SIGNATURES = {
     "lbk_ffn_gate_up": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p]),
     "lbk_ffn_dgate_up": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i32, _p]),
     "lbk_linear_scratch": (_i64, [_i64, _i64, _i64]),
+    "lbk_product_tiling": (_i32, [_i32, _i64, _i64, _i64, ctypes.POINTER(_i32)]),
     "lbk_linear_fwd": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
     "lbk_linear_dx": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
     "lbk_linear_dw": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i32, _p]),

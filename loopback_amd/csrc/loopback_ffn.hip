@@ -699,6 +699,11 @@ inline Tiling tiling_of(int64_t np, int64_t nq, int64_t k, bool plain) {   // pl
   }
   return best;
 }
+// the gated products' shapes: gate and up projection of t tokens, d -> 2 n, and their gradients, n columns summed over d
+inline Shape gated_shape(int64_t t, int64_t d, int64_t n) { return tiling_of(2 * n, t, d, false).shape; }
+// a short sum beside ten bytes moved per element: two workgroups to a CU, one's loads and stores beside the other's products
+// (16384 x 768 x 2048: 100 us against 110 with the large tiles; 8192 x 2048 x 5632: 230 against 224)
+inline Shape dgated_shape(int64_t t, int64_t d, int64_t n) { return d > 1024 ? tiling_of(n, t, d, false).shape : SMALL; }
 inline int64_t scratch_ld(int64_t np) { return (np + 3) / 4 * 4; }
 
 template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, Shape shape, hipStream_t st) {
@@ -818,8 +823,7 @@ int lbk_ffn_gate_up(const void* x, int64_t ldx, const void* w, int64_t ldw, void
   a.saved = saved;
   a.saved_cols = (n + 31) / 32;
   a.act = activation;
-  const Shape shape = tiling_of(2 * n, t, d, false).shape;
-  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, GATED>(a, shape, st)))
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, ROW, ROW, GATED>(a, gated_shape(t, d, n), st)))
 }
 
 int lbk_ffn_dgate_up(const void* dy, int64_t ld_dy, const void* w_down, int64_t ldw, const void* saved, void* dgate_up, int64_t ld_dgu,
@@ -835,16 +839,24 @@ int lbk_ffn_dgate_up(const void* dy, int64_t ld_dy, const void* w_down, int64_t 
   a.out16 = n % 8 == 0 && ld_dgu % 8 == 0 && al16(dgate_up);
   a.saved = const_cast<void*>(saved);
   a.saved_cols = (n + 31) / 32;
-  // a short sum beside ten bytes moved per element: two workgroups to a CU, one's loads and stores beside the other's products
-  // (16384 x 768 x 2048: 100 us against 110 with the large tiles; 8192 x 2048 x 5632: 230 against 224)
-  const Shape shape = d > 1024 ? tiling_of(n, t, d, false).shape : SMALL;
-  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, DGATED>(a, shape, static_cast<hipStream_t>(stream))))
+  FFN_TYPE_SWITCH(dtype, return (launch_product<T, COL, ROW, DGATED>(a, dgated_shape(t, d, n), static_cast<hipStream_t>(stream))))
 }
 
 int64_t lbk_linear_scratch(int64_t np, int64_t nq, int64_t k) {
   if (np < 1 || nq < 1 || k < 1) return 0;
   const Tiling tl = tiling_of(np, nq, k, true);
   return tl.splits > 1 ? tl.splits * nq * scratch_ld(np) : 0;
+}
+
+int lbk_product_tiling(int product, int64_t columns, int64_t rows, int64_t summed, int* splits) {
+  if (product < 0 || product > 2 || !splits) return LDR_E_ARG;
+  if (columns < 1 || rows < 1 || summed < 1 || (product == 1 && columns % 2)) return LDR_E_SHAPE;
+  *splits = 1;
+  if (product == 1) return gated_shape(rows, summed, columns / 2);
+  if (product == 2) return dgated_shape(rows, summed, columns);
+  const Tiling tl = tiling_of(columns, rows, summed, true);
+  *splits = tl.splits;
+  return tl.shape;
 }
 
 int lbk_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, void* y, int64_t ldy, float* scratch, int64_t t, int64_t k,
