@@ -124,3 +124,29 @@ def test_infinite_in_the_last_row(d, dtype):
         got, = torch.autograd.grad(h, gate, dh)
         want = (dh.double() * y.double()).flatten(0, -2).sum(0) if len(gshape) == 1 else (dh.double() * y.double()).sum(1, keepdim=True)
         assert want.isinf().sum() == 1 and torch.equal(got.isinf(), want.isinf()) and not got.isnan().any(), (shape, got, want)
+
+
+def test_offloaded_and_checkpointed():
+    """Saved tensors kept on the host, and a pass computed again by checkpointing (both kinds), give the plain pass's bits."""
+    from torch.utils.checkpoint import checkpoint
+    from loopback_amd import block_ops as ops
+    for d, n in ((136, 72), (65, 31)):   # aligned rows, and copies that are
+        x, y, w = (rnd(s, torch.bfloat16, k).requires_grad_() for k, s in enumerate(((70, d), (70, d), (d,))))
+        up, down = rnd((2 * n, d), torch.bfloat16, 8, 0.1).requires_grad_(), rnd((d, n), torch.bfloat16, 9, 0.1).requires_grad_()
+        dh, rng, leaves = rnd((70, d), torch.bfloat16, 6), rng_of(4), (x, y, w, up, down)
+
+        def run(x, y, w, up, down):
+            h, m = ops.block_join(x, y, post_weight=w, gate=w, dropout=0.2, rng=rng, site=1, pre_weight=w)
+            return h + ops.dropout(ops.gated_ffn(m, up, down), 0.3, rng, site=2)
+
+        want = torch.autograd.grad(run(*leaves), leaves, dh)
+        with torch.autograd.graph.save_on_cpu():
+            out = run(*leaves)
+        got = [torch.autograd.grad(out, leaves, dh)]
+        got += [torch.autograd.grad(checkpoint(run, *leaves, use_reentrant=False), leaves, dh)]
+        for p in leaves:
+            p.grad = None
+        checkpoint(run, *leaves, use_reentrant=True).backward(dh)
+        got += [[p.grad for p in leaves]]
+        for g in got:
+            assert all(torch.equal(a, b) for a, b in zip(g, want)), d
