@@ -1,8 +1,7 @@
-// host.cpp -- the module's launch path as a CPython extension: every ldr_* entry point, and those of the block operators
-// (lbk_*), as a builtin that takes tensors, None, numbers and address tables as they are, and the allocations around a read, a
-// block join and dropout. A launch through ctypes costs 4-5 us
-// of argument conversion (up to 30 arguments, each tensor's address fetched in Python before), and a small pass is a few
-// dozen of them: these cost about 1 us.
+// host.cpp -- the module's launch path as a CPython extension: every ldr_* entry point as a builtin that takes tensors, None,
+// numbers and address tables as they are, the allocations around a read, and the block operators (lbk_*) with the allocations
+// and autograd nodes around them. A launch through ctypes costs 4-5 us of argument conversion (up to 30 arguments, each
+// tensor's address fetched in Python before), and a small pass is a few dozen of them: these cost about 1 us.
 //
 // The entry points' addresses come from the library the Python binding loaded (bind), so both always call the same one.
 
@@ -91,19 +90,6 @@ template <> struct Arg<int> {
     const long x = PyLong_AsLong(o);
     if (x == -1 && PyErr_Occurred()) return false;
     v = static_cast<int>(x);
-    return true;
-  }
-};
-template <> struct Arg<uint32_t> {
-  uint32_t v = 0;
-  bool set(PyObject* o) {
-    const unsigned long long x = PyLong_AsUnsignedLongLong(o);
-    if (x == static_cast<unsigned long long>(-1) && PyErr_Occurred()) return false;
-    if (x > 0xffffffffull) {
-      PyErr_SetString(PyExc_OverflowError, "a 32-bit unsigned argument");
-      return false;
-    }
-    v = static_cast<uint32_t>(x);
     return true;
   }
 };
@@ -688,9 +674,6 @@ PyObject* host_torch_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {
 #define X(name) {#name, FAST((&Entry<decltype(&ldr_##name), ID_##name>::call)), METH_FASTCALL, nullptr},
     LDR_ENTRIES(X)
-#undef X
-#define X(name) {"lbk_" #name, FAST((&Entry<decltype(&lbk_##name), ID_block_##name>::call)), METH_FASTCALL, nullptr},
-    LBK_ENTRIES(X)
 #undef X
     {"dropout", FAST(&host_dropout), METH_FASTCALL, nullptr},
     {"join", FAST(&host_join), METH_FASTCALL, nullptr},
