@@ -699,11 +699,15 @@ inline Tiling tiling_of(int64_t np, int64_t nq, int64_t k, bool plain) {   // pl
   }
   return best;
 }
-// the gated products' shapes: gate and up projection of t tokens, d -> 2 n, and their gradients, n columns summed over d
+// the gated products' shapes: gate and up projection of t tokens, d -> 2 n, and their gradients, n columns summed over d. The first
+// by the plain products' model: of 27 sizes, d from 512 to 8192, it chose the slower one once (2048 x 2048 x 5632: 104 us, 100)
 inline Shape gated_shape(int64_t t, int64_t d, int64_t n) { return tiling_of(2 * n, t, d, false).shape; }
-// a short sum beside ten bytes moved per element: two workgroups to a CU, one's loads and stores beside the other's products
-// (16384 x 768 x 2048: 100 us against 110 with the large tiles; 8192 x 2048 x 5632: 230 against 224)
-inline Shape dgated_shape(int64_t t, int64_t d, int64_t n) { return d > 1024 ? tiling_of(n, t, d, false).shape : SMALL; }
+// a short sum beside ten bytes moved per element: two workgroups to a CU, one's loads and stores beside the other's products.
+// us with the small and the large tiles: 16384 x 512 x 1408 65 and 79, 16384 x 768 x 2048 103 and 114, 16384 x 1024 x 2816 154
+// and 169, 16384 x 1280 x 3456 215 and 237, 16384 x 1536 x 4096 288 and 310, 8192 x 2048 x 5632 234 and 240; 8192 x 2560 x 6912 369
+// and 362, 4096 x 2816 x 7680 207 and 198, 8192 x 4096 x 11008 881 and 837, 8192 x 6144 x 5632 626 and 537. Past 2048 the time
+// model of the plain products chooses, which is not fitted to this kernel (2048 x 4096 x 11008: 229, where the small ones take 213)
+inline Shape dgated_shape(int64_t t, int64_t d, int64_t n) { return d > 2048 ? tiling_of(n, t, d, false).shape : SMALL; }
 inline int64_t scratch_ld(int64_t np) { return (np + 3) / 4 * 4; }
 
 template <typename T, Kind KP, Kind KQ, Epi EPI> int launch_product(const Product& a, Shape shape, hipStream_t st) {

@@ -14,7 +14,7 @@ SHAPES = {0: "128 x 128", 1: "256 x 256", 2: "192 x 256"}
 PLAIN = {(129, 300, 71): (0, False), (56, 125, 523): (0, True), (8087, 1405, 331): (1, False), (247, 6397, 16391): (1, True),
          (408, 7293, 8203): (1, True), (920, 8317, 73): (2, False), (151, 8317, 4109): (2, True)}
 # tokens, inner, width: the tiles of the gate and up projection and of the two's gradients
-GATED = {(300, 152, 200): (0, 0), (6013, 665, 201): (1, 0), (8317, 919, 1033): (0, 1)}
+GATED = {(300, 152, 200): (0, 0), (6013, 665, 201): (1, 0), (8317, 919, 2057): (0, 1)}
 
 
 def tiling(product, columns, rows, summed):
