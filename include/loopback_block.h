@@ -64,7 +64,7 @@ int lbk_join_bwd(const void* dh, const void* dn, const void* x, const void* y, c
 int lbk_pad_rows(const void* x, int64_t rows, int64_t cols, int64_t ld, void* out, int dtype, void* stream);
 
 /* Bytes of `saved`, what the backward needs of the two projections: (u a'(g), a(g)) per (token, column) in the kernels' own
- * order, 24 bits each. 16-byte aligned. */
+ * order, 24 bits each (six bytes per token and column, of blocks of 32 x 32). 16-byte aligned. */
 int64_t lbk_ffn_saved_bytes(int64_t t, int64_t n);
 
 /* act [t, n] = round(a(x Wg^T) * (x Wu^T)): both projections, the activation and the product in one kernel. saved: NULL

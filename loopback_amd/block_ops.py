@@ -7,9 +7,10 @@
   * `dropout(x, p, rng, site)`: dropout whose mask comes from a counter-based generator and is never stored.
 
 The row kernels take plain fp32, bf16 and fp16 tensors of the current GPU where nothing has to see torch operations (lm_ops.native
-says what does); everything else -- the CPU, other types, tracers, transforms -- runs the torch form of the same operator:
-the same formulas and the same masks. A backward that is itself differentiated, or watched, runs the torch form too. Tensors
-of any strides are taken (the kernels work on contiguous rows; others are copied).
+says what does); everything else -- the CPU, other types, mixed types, autocast (but for dropout), tracers, transforms -- runs
+the torch form of the same operator: the same formulas and the same masks. A backward that is itself differentiated, or
+watched, runs the torch form too. Tensors of any strides are taken (the kernels work on contiguous rows; others are copied). Saved tensors that a hook gives
+back with another shape, type or device are refused.
 
 Dropout's generator: `rng` is an int64 tensor (seed, step) on the inputs' device, read when a kernel runs: a captured graph
 draws a new mask when the program has changed it, and a backward reads it again, so the program changes a copy, not the
@@ -321,7 +322,8 @@ H.torch_forms(_dropout_backward, _join_backward, _ffn_backward)
 def gated_ffn(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """(a(x Wg^T) * (x Wu^T)) Wd^T of x (..., d), w_gate_up (2 n, d) = [Wg; Wu] and w_down (m, n); a is "silu" or "gelu" (its
     tanh form). On the kernels the projections, the activation and their product are one fp32 value rounded once, and the
-    backward's gradients of the two projections are formed from 24 bits of them."""
+    backward's gradients of the two projections are formed from 24 bits of them. A recorded call keeps 8 bytes per token and
+    inner column for its backward (the activations and those bits)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, got {activation!r}")
     if w_gate_up.dim() != 2 or w_down.dim() != 2 or x.dim() < 1 or w_gate_up.shape[1] != x.shape[-1] \

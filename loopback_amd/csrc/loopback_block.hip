@@ -162,8 +162,9 @@ template <typename T> struct JoinFwd {
   float scale, keep, eps;
 };
 
-// Reads x and y, writes h and n and two statistics a row: the rows' stream bounds it. 16384 x 768 in bf16 with all parts 21 us (4.8
-// TB/s), 6825 x 2048 in fp16 23 us (4.9 TB/s). LPR lanes to a row of LPR x 8 columns at most, so that a lane holds its
+// Reads x and y, writes h and n and two statistics a row: the rows' stream bounds it, beside the vector units (0.7 of the time with
+// the generator, 0.46 without). 16384 x 768 in bf16 with all parts 19 to 21 us (4.8 to 5.2 TB/s), 6825 x 2048 in fp16 18 to 23 us (4.9
+// to 5.8 TB/s). LPR lanes to a row of LPR x 8 columns at most, so that a lane holds its
 // eight in registers.
 // PARTS: which parts the call has, known when the kernel is compiled (1 the norm before the next block, 2 the norm after this
 // one, 4 dropout), or ANY: looked up as it runs (rows that take the narrow loads)
@@ -251,10 +252,10 @@ template <typename T> struct JoinBwd {
 // A workgroup takes `per` consecutive rows and keeps the column sums of the three weight gradients in registers. The gate's
 // belong to runs of gate_rows rows: a run that lies inside the workgroup's rows is finished here, a share of a longer one
 // goes to part_gate, first slot where the run began before this workgroup's rows, second where it ends after them.
-// gate_rows 1: each element's own. Its vector arithmetic bounds it (the generator, unpacking, two row sums), beside the stream of six
-// rows: 16384 x 768 in bf16 with all parts 42 us (3.6 TB/s; two vectors a lane on half the lanes took 72, held to fewer registers
-// 121 to 210 with spills; loading the next row ahead changed nothing, 43.4 against 43.7), 6825 x 2048 in fp16 without dropout 36
-// us (4.7 TB/s).
+// gate_rows 1: each element's own. Nothing is saturated: counters at 16384 x 768 in bf16 with all parts have the vector units issue
+// for 0.64 of the time, the rows move at 4.4 TB/s and the waves wait for 0.45 of their cycles, at 2.9 waves to a SIMD (148 registers);
+// without dropout at 6825 x 2048 in fp16 0.43, 5.6 TB/s and 0.59. 36 to 42 us and 33 to 36 us by machine (two vectors a lane on half
+// the lanes took 72, held to fewer registers 121 to 210 with spills; loading the next row ahead changed nothing, 43.4 against 43.7).
 // Rows wider than 4096 take 16 waves of 128 registers: with both norms some are spilled (12 to 108 bytes a lane). 512 lanes of two
 // vectors spill nothing and are slower: 16384 x 5001 in bf16 394 -> 470 us, 8192 x 8192 226 -> 255.
 template <typename T, int LPR, bool AL, int PARTS>

@@ -17,7 +17,7 @@
 // The matrix cores bound it: 2 q p k operations, and a 256 x 256 tile reads 64 KiB for each 64 k it multiplies. 8192 x 2048 x 5632
 // in bf16: gate and up projection 314 us (1202 TFLOP/s; a library's product without the activation 352), down 151 us (125),
 // input gradient 289 us (273), weight gradients 317 and 157 us (339 and 171). Smaller tiles with more workgroups to a CU took
-// 5-11 % longer, 32 k per tile in three or four buffers 4-15 % (a barrier for half the work), four waves of 128 x 128 12-17 %,
+// 5-11 % longer (the projections' gradient apart: dgated_shape), 32 k per tile in three or four buffers 4-15 % (a barrier for half the work), four waves of 128 x 128 12-17 %,
 // a raised wave priority around the products 0-14 %; reloading one tile throughout, without memory traffic, only 3-5 % less.
 
 #include <hip/hip_runtime.h>
@@ -164,7 +164,8 @@ template <typename T, Kind KIND, int ROWS, int LANES, bool GATED_P> struct Tile 
 
 // ---------------------------------------------------------------------------------------------------------------
 // what the backward needs of the gate and up projections: (u a'(g), a(g)) of each (token, inner column), which the
-// activation's gradient is multiplied by. Kept as the upper 24 bits of their fp32 values: 16 would double the input and
+// activation's gradient is multiplied by. Kept as the upper 24 bits of their fp32 values, the rest cut off (less than 2^-15 of the
+// value): 16 would double the input and
 // gate/up weight gradients' squared error (three roundings instead of two). In blocks of 32 tokens x 32 columns in the
 // matrix cores' own order, so both kernels move them as whole vectors: 64 lanes x 16 values, upper 16 bits as two planes of
 // eight values a lane, then the next eight bits: half a block's bytes for each of the two. Stores and loads past the
@@ -539,7 +540,10 @@ __global__ __launch_bounds__(256) void k_pad_rows(const T* __restrict__ x, int64
 // from memory to the matrix cores' registers (v_mfma_f32_16x16x32: lane l has row l mod 16): a workgroup takes 16 rows (of the
 // gate's and of the up projection's), its waves the columns in turns of 128, each load instruction 64 consecutive bytes of 16
 // rows, all loads of a few turns in flight together. The waves' sums meet in LDS, in order. Any alignment. One token at 2048 x
-// 5632 in bf16: 13 us for gate and up projection (3.6 TB/s of weights) and 9 us for the down projection (2.6); 32 tokens 19 and 23.
+// 5632 in bf16: 11 to 13 us for gate and up projection (3.6 TB/s of weights) and 8 to 9 us for the down projection (2.6).
+// LBK_FEW_TOKENS is one limit for both products. us here and on the tiles, bf16: gate and up projection 32 x 768 x 2048 5.1 and 7.9,
+// 32 x 2048 x 5632 18 and 22, 32 x 4096 x 11008 46 and 45; down 32 x 768 x 2048 7.5 and 8.6, but 8 x 2048 x 5632 10.1 and 11.1,
+// 16 x 2048 x 5632 11.9 and 11.5, 32 x 2048 x 5632 21 and 13, 1 x 4096 x 11008 22 and 21, 32 x 4096 x 11008 32 and 22.
 // ---------------------------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 mfma16(bf16_t, uint4 a, uint4 b, f32x4 c) {
