@@ -244,10 +244,10 @@ def join_norm(norm: nn.Module | None, x: torch.Tensor, y: torch.Tensor, post: nn
         return m is None or (type(m) in (nn.RMSNorm, RMSNorm) and m.eps is not None and m.weight is not None
                              and m.weight.dim() == 1 and not _hooked(m))
 
-    if not isinstance(x, torch.Tensor) and not how["dropout"]:
+    if not isinstance(x, torch.Tensor) and not how.get("dropout"):
         y = y if post is None else post(y)
-        y = y if how["gate"] is None else y * how["gate"]
-        h = x + y * how["scale"]
+        y = y if how.get("gate") is None else y * how["gate"]
+        h = x + y * how.get("scale", 1.0)
         return h, None if norm is None else norm(h)
     if not plain(post):
         y, post = post(y), None

@@ -44,3 +44,19 @@ def test_block(options):
     assert [n.target for n in graph.nodes if n.op == "call_module"] == \
         ["attn_norm", "attn", *post[0], "mlp_norm", "mlp.gate_up", "mlp.down", *post[1]]
     assert torch.allclose(torch.fx.GraphModule(tracer.root, graph)(x), block(x), atol=1e-5)
+
+
+def test_join_alone():
+    """The join of two values without a gate, a scale or a norm before it, traced by itself."""
+    class Join(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm = torch.nn.RMSNorm(16, eps=1e-6)
+
+        def forward(self, x, y):
+            return lm.join_norm(self.norm, x, y)
+
+    torch.manual_seed(0)
+    join, x, y = Join(), torch.randn(3, 16), torch.randn(3, 16)
+    for a, b in zip(torch.fx.symbolic_trace(join)(x, y), join(x, y)):
+        assert torch.allclose(a, b, atol=1e-6)
