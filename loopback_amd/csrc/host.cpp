@@ -1,6 +1,6 @@
 // host.cpp -- the module's launch path as a CPython extension: every ldr_* entry point as a builtin that takes tensors, None,
-// numbers and address tables as they are, the allocations around a read, and the block operators (lbk_*) with the allocations
-// and autograd nodes around them. A launch through ctypes costs 4-5 us of argument conversion (up to 30 arguments, each
+// numbers and address tables as they are, the allocations around a read, and the block operators (lbk_*) and the model's (lmo_*)
+// with the allocations and autograd nodes around them. A launch through ctypes costs 4-5 us of argument conversion (up to 30 arguments, each
 // tensor's address fetched in Python before), and a small pass is a few dozen of them: these cost about 1 us.
 //
 // The entry points' addresses come from the library the Python binding loaded (bind), so both always call the same one.
@@ -21,6 +21,7 @@
 #include <utility>
 
 #include "loopback_block.h"
+#include "loopback_model.h"
 #include "loopback_read.h"
 
 namespace {
@@ -140,6 +141,8 @@ template <typename... A, int ID> struct Entry<int (*)(A...), ID> {
 #define LBK_ENTRIES(X)                                                                                            \
   X(dropout) X(join_fwd) X(join_bwd) X(pad_rows) X(ffn_gate_up) X(ffn_dgate_up) X(linear_fwd) X(linear_dx) X(linear_dw)
 
+#define LMO_ENTRIES(X) X(layer_norm_fwd) X(layer_norm_bwd) X(distill_fwd) X(distill_bwd)
+
 enum Id {
 #define X(name) ID_##name,
   LDR_ENTRIES(X)
@@ -147,11 +150,16 @@ enum Id {
 #define X(name) ID_block_##name,
   LBK_ENTRIES(X)
 #undef X
+#define X(name) ID_model_##name,
+  LMO_ENTRIES(X)
+#undef X
 };
 #define BLOCK_FN(name) (Entry<decltype(&lbk_##name), ID_block_##name>::fn)
+#define MODEL_FN(name) (Entry<decltype(&lmo_##name), ID_model_##name>::fn)
 int64_t (*join_scratch)(int64_t, int64_t, int64_t) = nullptr;
 int64_t (*linear_scratch)(int64_t, int64_t, int64_t) = nullptr;
 int64_t (*ffn_saved_bytes)(int64_t, int64_t) = nullptr;
+int64_t (*layer_norm_scratch)(int64_t, int64_t) = nullptr;
 
 struct Binding { const char* name; void (*bind)(void*); };
 const Binding bindings[] = {
@@ -161,6 +169,10 @@ const Binding bindings[] = {
 #define X(name) {"lbk_" #name, &Entry<decltype(&lbk_##name), ID_block_##name>::bind},
     LBK_ENTRIES(X)
 #undef X
+#define X(name) {"lmo_" #name, &Entry<decltype(&lmo_##name), ID_model_##name>::bind},
+    LMO_ENTRIES(X)
+#undef X
+    {"lmo_layer_norm_scratch", [](void* p) { layer_norm_scratch = reinterpret_cast<decltype(layer_norm_scratch)>(p); }},
     {"lbk_join_scratch", [](void* p) { join_scratch = reinterpret_cast<decltype(join_scratch)>(p); }},
     {"lbk_linear_scratch", [](void* p) { linear_scratch = reinterpret_cast<decltype(linear_scratch)>(p); }},
     {"lbk_ffn_saved_bytes", [](void* p) { ffn_saved_bytes = reinterpret_cast<decltype(ffn_saved_bytes)>(p); }},
@@ -291,14 +303,16 @@ struct Gil {
   ~Gil() { PyGILState_Release(state); }
 };
 
-// the backwards' torch forms, Python functions of block_ops: dropout's, the join's and the feed-forward block's
-PyObject* torch_forms[3] = {nullptr, nullptr, nullptr};
+// the backwards' torch forms, Python functions: of block_ops dropout's, the join's and the feed-forward block's, of model_ops
+// layer norm's and the distillation loss's
+constexpr int FORMS = 5, BLOCK_FORMS = 3;
+PyObject* torch_forms[FORMS] = {};
 
 // torch_forms[which](*tensors, *numbers) with None for undefined tensors: its tuple of `results` tensors
 variable_list torch_form(int which, const variable_list& tensors, std::initializer_list<int64_t> ints,
                          std::initializer_list<double> floats, size_t results) {
   Gil gil;
-  TORCH_CHECK(torch_forms[which], "the block operators' torch forms are not bound");
+  TORCH_CHECK(torch_forms[which], "the operators' torch forms are not bound");
   struct Ref {
     PyObject* o;
     ~Ref() { Py_XDECREF(o); }
@@ -350,7 +364,7 @@ void as_saved(const at::Tensor& t, const at::Tensor& like, at::ScalarType type, 
   if (!t.defined()) return;
   TORCH_CHECK(t.layout() == at::kStrided && t.device() == like.device() && t.scalar_type() == type && t.dim() > 0 &&
                   t.numel() == rows * cols && t.size(-1) == cols,
-              "a block operator's saved tensor came back from a hook with another shape, type or device: ", t.toString(), " ", t.sizes(),
+              "an operator's saved tensor came back from a hook with another shape, type or device: ", t.toString(), " ", t.sizes(),
               " on ", t.device());
 }
 int64_t code_of(at::ScalarType t) { return t == at::kFloat ? LDR_F32 : t == at::kBFloat16 ? LDR_BF16 : t == at::kHalf ? LDR_F16 : -1; }
@@ -656,18 +670,220 @@ PyObject* host_join(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the model's operators: layer norm, the distillation loss --------------------------------------------------------
+// h (the rounded sum; undefined without add), y, and the rows' mean and rstd where a backward follows
+variable_list layer_norm_run(const at::Tensor& x, const OptTensor& add, const OptTensor& w, const OptTensor& b, double eps,
+                             int64_t dtype, int64_t stream, bool keep) {
+  const int64_t d = x.size(-1), rows = x.numel() / d;
+  variable_list t{add ? at::empty_like(x) : at::Tensor(), at::empty_like(x),
+                  keep ? at::empty({rows, 2}, at::TensorOptions().dtype(at::kFloat).device(x.device())) : at::Tensor()};
+  TORCH_CHECK(MODEL_FN(layer_norm_fwd), "lmo_layer_norm_fwd: entry point not bound");
+  launched("lmo_layer_norm_fwd",
+           MODEL_FN(layer_norm_fwd)(x.data_ptr(), ptr(add), ptr(w), ptr(b), ptr(t[0]), t[1].data_ptr(), static_cast<float*>(ptr(t[2])),
+                                    rows, d, static_cast<float>(eps), static_cast<int>(dtype), reinterpret_cast<void*>(stream)));
+  return t;
+}
+
+// (h, y) of rows x + add, or (x, y): the gradient that comes back along the first joins the norm's in one pass
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& add, const OptTensor& w, const OptTensor& b,
+                               double eps, int64_t dtype, int64_t stream) {
+    variable_list t = layer_norm_run(x, add, w, b, eps, dtype, stream, true);
+    if (!add) t[0] = x;
+    ctx->save_for_backward({t[0], or_none(w), t[2]});
+    ctx->saved_data["numbers"] = std::vector<int64_t>{x.numel() / x.size(-1), x.size(-1), dtype, add.has_value(), b.has_value()};
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    if (add && !x.requires_grad() && !add->requires_grad()) ctx->mark_non_differentiable({t[0]});
+    t.resize(2);
+    return t;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(7);
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &h = saved[0], &w = saved[1], &stats = saved[2], &dh = grads[0], &dy = grads[1];
+    if (!dh.defined() && !dy.defined()) return out;
+    const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
+    const double eps = ctx->saved_data["eps"].toDouble();
+    const int64_t rows = n[0], d = n[1];
+    const bool added = n[3];
+    size_t edge = 0;   // the tensors among the inputs are the node's edges, in order
+    const bool nx = ctx->needs_input_grad(edge++), nadd = added && ctx->needs_input_grad(edge++);
+    const bool nw = w.defined() && ctx->needs_input_grad(edge++), nb = n[4] && ctx->needs_input_grad(edge++);
+    auto give = [&](const at::Tensor& dx) {
+      if (nx) out[0] = dx;
+      if (nadd) out[1] = dx;
+    };
+    if (!dy.defined()) {   // only the residual stream goes on
+      give(dh);
+      return out;
+    }
+    const at::ScalarType type = h.scalar_type();
+    TORCH_CHECK(code_of(type) == n[2], "the layer norm's rows came back from a hook with another type: ", type);
+    as_saved(h, dy, type, rows, d);
+    as_saved(w, h, type, 1, d);
+    as_saved(stats, h, at::kFloat, rows, 2);
+    if (!on_kernels({dh, dy}, h) || !h.is_cuda()) {
+      const variable_list got = torch_form(3, {dh, dy, h, w}, {(nx || nadd) + 2 * nw + 4 * nb}, {eps}, 3);
+      give(got[0]);
+      out[2] = got[1];
+      out[3] = got[2];
+      return out;
+    }
+    const c10::DeviceGuard on(h.device());
+    const at::Tensor hr = rows_of(h), wr = rows_of(w), sr = rows_of(stats), dhr = rows_of(dh), dyr = rows_of(dy);
+    at::Tensor dx, scratch;
+    if (nx || nadd) dx = at::empty_like(hr);
+    if (nw) out[2] = at::empty({d}, hr.options());
+    if (nb) out[3] = at::empty({d}, hr.options());
+    if (nw || nb) {
+      TORCH_CHECK(layer_norm_scratch, "lmo_layer_norm_scratch: entry point not bound");
+      scratch = at::empty({layer_norm_scratch(rows, d)}, at::TensorOptions().dtype(at::kFloat).device(h.device()));
+    }
+    TORCH_CHECK(MODEL_FN(layer_norm_bwd), "lmo_layer_norm_bwd: entry point not bound");
+    launched("lmo_layer_norm_bwd",
+             MODEL_FN(layer_norm_bwd)(dyr.data_ptr(), hr.data_ptr(), ptr(wr), static_cast<const float*>(sr.data_ptr()), ptr(dhr), ptr(dx),
+                                      ptr(out[2]), ptr(out[3]), static_cast<float*>(ptr(scratch)), rows, d, static_cast<int>(n[2]),
+                                      reinterpret_cast<void*>(stream_of(h))));
+    give(dx);
+    return out;
+  }
+};
+
+// layer_norm(x, add, w, b, eps, dtype, stream, record): (h or x, y), contiguous tensors
+PyObject* host_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 8, "layer_norm(x, add, w, b, eps, dtype, stream, record)");
+  const at::Tensor& x = tensor_of(args[0]);
+  const OptTensor add = opt_tensor(args[1]), w = opt_tensor(args[2]), b = opt_tensor(args[3]);
+  const double eps = float_of(args[4]);
+  const int64_t dtype = int_of(args[5]), stream = int_of(args[6]);
+  const bool record = args[7] == Py_True;
+  variable_list t;
+  {
+    NoGil free;
+    t = record ? LayerNormNode::apply(x, add, w, b, eps, dtype, stream) : layer_norm_run(x, add, w, b, eps, dtype, stream, false);
+    t.resize(2);
+    if (!t[0].defined()) t[0] = x;
+  }
+  return tuple_of(t);
+  END_HANDLE_TH_ERRORS
+}
+
+struct DistillCall {   // one call's operands and sizes
+  at::Tensor logits, top, ids, lse, labels;   // lse, labels: may be undefined
+  double tau, hard;
+  int64_t dtype, stream;
+  int64_t vocab() const { return logits.size(-1); }
+  int64_t rows() const { return logits.numel() / vocab(); }
+  int64_t k() const { return top.size(-1); }
+  int wide() const { return ids.scalar_type() == at::kLong; }
+  int top_dtype() const { return static_cast<int>(code_of(top.scalar_type())); }
+  void* st() const { return reinterpret_cast<void*>(stream); }
+};
+
+variable_list distill_run(const DistillCall& c) {   // loss, the rows' saved values, the gradient's factors
+  const auto f32 = at::TensorOptions().dtype(at::kFloat).device(c.logits.device());
+  variable_list t{at::empty({}, f32), at::empty({c.rows(), LMO_DISTILL_SAVED}, f32), at::empty({2}, f32)};
+  TORCH_CHECK(MODEL_FN(distill_fwd), "lmo_distill_fwd: entry point not bound");
+  launched("lmo_distill_fwd",
+           MODEL_FN(distill_fwd)(c.logits.data_ptr(), c.top.data_ptr(), c.top_dtype(), c.ids.data_ptr(), c.wide(),
+                                 static_cast<const float*>(ptr(c.lse)), static_cast<const int64_t*>(ptr(c.labels)),
+                                 static_cast<float>(c.tau), static_cast<float>(c.hard), static_cast<float*>(t[1].data_ptr()),
+                                 static_cast<float*>(t[2].data_ptr()), static_cast<float*>(t[0].data_ptr()), c.rows(), c.vocab(), c.k(),
+                                 static_cast<int>(c.dtype), c.st()));
+  return t;
+}
+
+struct DistillNode : torch::autograd::Function<DistillNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& top, const at::Tensor& ids,
+                            const OptTensor& lse, const OptTensor& labels, double tau, double hard, int64_t dtype, int64_t stream) {
+    const DistillCall c{logits, top, ids, or_none(lse), or_none(labels), tau, hard, dtype, stream};
+    variable_list t = distill_run(c);
+    ctx->save_for_backward({logits, top, ids, c.lse, c.labels, t[1], t[2]});
+    ctx->saved_data["numbers"] = std::vector<int64_t>{c.rows(), c.vocab(), c.k(), dtype};
+    ctx->saved_data["tau"] = tau;
+    ctx->saved_data["hard"] = hard;
+    ctx->set_materialize_grads(false);
+    return t[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(9);
+    const at::Tensor& g = grads[0];
+    if (!g.defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
+    const double tau = ctx->saved_data["tau"].toDouble(), hard = ctx->saved_data["hard"].toDouble();
+    const at::Tensor& logits = s[0];
+    TORCH_CHECK(code_of(logits.scalar_type()) == n[3], "the loss's logits came back from a hook with another type: ", logits.scalar_type());
+    TORCH_CHECK(code_of(s[1].scalar_type()) >= 0 && (s[2].scalar_type() == at::kLong || s[2].scalar_type() == at::kInt),
+                "the loss's teacher came back from a hook with another type");
+    as_saved(logits, g, logits.scalar_type(), n[0], n[1]);
+    as_saved(s[1], logits, s[1].scalar_type(), n[0], n[2]);
+    as_saved(s[2], logits, s[2].scalar_type(), n[0], n[2]);
+    if (s[3].defined()) as_saved(s[3].reshape({-1}), logits, at::kFloat, 1, n[0]);
+    if (s[4].defined()) as_saved(s[4].reshape({-1}), logits, at::kLong, 1, n[0]);
+    as_saved(s[5], logits, at::kFloat, n[0], LMO_DISTILL_SAVED);
+    as_saved(s[6], logits, at::kFloat, 1, 2);
+    if (!on_kernels(grads, s[6], false) || !logits.is_cuda() || g.numel() != 1) {
+      out[0] = torch_form(4, {g, logits, s[1], s[2], s[3], s[4]}, {}, {tau, hard}, 1)[0];
+      return out;
+    }
+    const c10::DeviceGuard on(logits.device());
+    const DistillCall c{rows_of(logits), rows_of(s[1]), rows_of(s[2]), rows_of(s[3]), rows_of(s[4]), tau, hard, n[3], stream_of(logits)};
+    const at::Tensor saved = rows_of(s[5]), coef = rows_of(s[6]);
+    out[0] = at::empty_like(c.logits);
+    TORCH_CHECK(MODEL_FN(distill_bwd), "lmo_distill_bwd: entry point not bound");
+    launched("lmo_distill_bwd",
+             MODEL_FN(distill_bwd)(c.logits.data_ptr(), c.top.data_ptr(), c.top_dtype(), c.ids.data_ptr(), c.wide(),
+                                   static_cast<const int64_t*>(ptr(c.labels)), static_cast<float>(tau),
+                                   static_cast<const float*>(saved.data_ptr()), static_cast<const float*>(coef.data_ptr()),
+                                   static_cast<const float*>(g.data_ptr()), out[0].data_ptr(), c.rows(), c.vocab(), c.k(),
+                                   c.lse.defined(), static_cast<int>(c.dtype), c.st()));
+    return out;
+  }
+};
+
+// distill(logits, top, ids, lse, labels, tau, hard, dtype, stream, record): the loss, contiguous tensors
+PyObject* host_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 10, "distill(logits, top, ids, lse, labels, tau, hard, dtype, stream, record)");
+  const at::Tensor &logits = tensor_of(args[0]), &top = tensor_of(args[1]), &ids = tensor_of(args[2]);
+  const OptTensor lse = opt_tensor(args[3]), labels = opt_tensor(args[4]);
+  const double tau = float_of(args[5]), hard = float_of(args[6]);
+  const int64_t dtype = int_of(args[7]), stream = int_of(args[8]);
+  const bool record = args[9] == Py_True;
+  at::Tensor loss;
+  {
+    NoGil free;
+    loss = record ? DistillNode::apply(logits, top, ids, lse, labels, tau, hard, dtype, stream)
+                  : distill_run({logits, top, ids, or_none(lse), or_none(labels), tau, hard, dtype, stream})[0];
+  }
+  return THPVariable_Wrap(loss);
+  END_HANDLE_TH_ERRORS
+}
+
 // torch_forms(dropout, join, ffn): the Python functions that the nodes call where a backward has to be torch operations
-PyObject* host_torch_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 3 || !PyCallable_Check(args[0]) || !PyCallable_Check(args[1]) || !PyCallable_Check(args[2])) {
-    PyErr_SetString(PyExc_TypeError, "torch_forms(dropout, join, ffn)");
+PyObject* set_forms(PyObject* const* args, Py_ssize_t n, int first, int count, const char* what) {
+  bool ok = n == count;
+  for (int i = 0; ok && i < count; ++i) ok = PyCallable_Check(args[i]);
+  if (!ok) {
+    PyErr_SetString(PyExc_TypeError, what);
     return nullptr;
   }
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < count; ++i) {
     Py_INCREF(args[i]);
-    Py_XDECREF(torch_forms[i]);
-    torch_forms[i] = args[i];
+    Py_XDECREF(torch_forms[first + i]);
+    torch_forms[first + i] = args[i];
   }
   Py_RETURN_NONE;
+}
+PyObject* host_torch_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return set_forms(args, n, 0, BLOCK_FORMS, "torch_forms(dropout, join, ffn)");
+}
+// model_forms(layer_norm, distill): the same of the model's operators
+PyObject* host_model_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return set_forms(args, n, BLOCK_FORMS, FORMS - BLOCK_FORMS, "model_forms(layer_norm, distill)");
 }
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
@@ -679,6 +895,9 @@ PyMethodDef methods[] = {
     {"join", FAST(&host_join), METH_FASTCALL, nullptr},
     {"gated_ffn", FAST(&host_gated_ffn), METH_FASTCALL, nullptr},
     {"torch_forms", FAST(&host_torch_forms), METH_FASTCALL, nullptr},
+    {"layer_norm", FAST(&host_layer_norm), METH_FASTCALL, nullptr},
+    {"distill", FAST(&host_distill), METH_FASTCALL, nullptr},
+    {"model_forms", FAST(&host_model_forms), METH_FASTCALL, nullptr},
     {"bind", FAST(&host_bind), METH_FASTCALL, nullptr},
     {"alias", FAST(&host_alias), METH_FASTCALL, nullptr},
     {"read_buffers", FAST(&host_read_buffers), METH_FASTCALL, nullptr},

@@ -1,0 +1,728 @@
+// loopback_model.hip -- MI355X (gfx950, CDNA4) kernels of layer norm and of the distillation loss from a teacher's highest
+// logits, forward and backward. All are bound by the HBM stream of their rows: fp32 statistics, one rounding per result.
+// Every sum has a fixed order: results are deterministic.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "loopback_model.h"
+#include "loopback_read.h"
+#include "row_io.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------
+// layer norm. LPR lanes to a row, VPT times eight columns each, the whole row in registers: the mean, then the squares of
+// the differences from it (not the mean of squares, which would cancel where the mean is large), then the result.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T> struct NormFwd {
+  const T *x, *add, *w, *b;
+  T *h, *y;
+  float* stats;
+  int rows, d;
+  float eps;
+};
+
+template <typename T, int LPR, int VPT, bool AL>
+__global__ __launch_bounds__(lanes_of(LPR)) void k_layer_norm_fwd(const NormFwd<T> a) {
+  constexpr int LANES = lanes_of(LPR), R = LANES / LPR;
+  __shared__ float s_red[2][LANES / 64];
+  RowSum<LPR> row_sum{s_red};
+  const int d = a.d, lane = (int)threadIdx.x % LPR, grp = group_of<LPR>();
+  const float inv_d = 1.f / (float)d;
+  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < a.rows; row0 += (int64_t)gridDim.x * R) {
+    const bool ok = row0 + grp < a.rows;
+    const int64_t row = ok ? row0 + grp : a.rows - 1, ro = row * d;
+    typename IO<T>::Raw xr[VPT], ar[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      xr[v] = load8<T, AL>(a.x + ro, 8 * (lane + LPR * v), d);
+      if (a.add) ar[v] = load8<T, AL>(a.add + ro, 8 * (lane + LPR * v), d);
+    }
+    float h[VPT][8], m = 0.f, ss = 0.f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      IO<T>::unpack(xr[v], h[v]);
+      if (a.add) {
+        float e[8];
+        IO<T>::unpack(ar[v], e);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[v][k] = IO<T>::round(h[v][k] + e[k]);
+        if (ok) store8<T, AL>(a.h + ro, 8 * (lane + LPR * v), d, h[v]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m += h[v][k];   // zeros past the row's end
+    }
+    m = row_sum(m) * inv_d;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        h[v][k] -= m;
+        const bool in = 8 * (lane + LPR * v) + (AL ? 0 : k) < d;
+        ss = in ? __builtin_fmaf(h[v][k], h[v][k], ss) : ss;
+      }
+    const float r = rsqrtf(row_sum(ss) * inv_d + a.eps);
+    if (a.stats && lane == 0 && ok) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(m, r);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int col = 8 * (lane + LPR * v);
+      float e[8];
+      if (a.w) {
+        IO<T>::unpack(load8<T, AL>(a.w, col, d), e);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[v][k] *= r * e[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[v][k] *= r;
+      }
+      if (a.b) {
+        IO<T>::unpack(load8<T, AL>(a.b, col, d), e);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[v][k] += e[k];
+      }
+      if (ok) store8<T, AL>(a.y + ro, col, d, h[v]);
+    }
+  }
+}
+
+template <typename T> struct NormBwd {
+  const T *dy, *h, *w;
+  const float* stats;
+  const T* dres;
+  T* dx;
+  float *part_w, *part_b;   // [workgroups][d]; NULL: not wanted
+  int rows, d, per;
+};
+
+// A workgroup takes `per` consecutive rows and keeps the columns' sums of dy hat and dy in registers; its row groups' sums
+// meet in LDS, one partial row a workgroup.
+template <typename T, int LPR, int VPT, bool AL>
+__global__ __launch_bounds__(lanes_of(LPR)) void k_layer_norm_bwd(const NormBwd<T> a) {
+  constexpr int LANES = lanes_of(LPR), R = LANES / LPR, W = 8 * LPR;
+  __shared__ float s_red[2][LANES / 64];
+  __shared__ float s_sum[R > 1 ? R * W : 1];
+  RowSum<LPR> row_sum{s_red};
+  const int d = a.d, lane = (int)threadIdx.x % LPR, grp = group_of<LPR>();
+  const float inv_d = 1.f / (float)d;
+  typename IO<T>::Raw wr[VPT];
+  float dw[VPT][8], db[VPT][8];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    wr[v] = a.w ? load8<T, AL>(a.w, 8 * (lane + LPR * v), d) : IO<T>::zero();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) dw[v][k] = db[v][k] = 0.f;
+  }
+  const int64_t r0 = (int64_t)blockIdx.x * a.per, r1 = min((int64_t)a.rows, r0 + a.per);
+  for (int64_t row0 = r0; row0 < r1; row0 += R) {
+    const bool ok = row0 + grp < r1, there = R == 1 || ok;   // a row that is not there adds nothing to the sums
+    const int64_t row = ok ? row0 + grp : r1 - 1, ro = row * d;
+    typename IO<T>::Raw yr[VPT], hr[VPT], rr[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int col = 8 * (lane + LPR * v);
+      yr[v] = load8<T, AL>(a.dy + ro, col, d);
+      hr[v] = load8<T, AL>(a.h + ro, col, d);
+      if (a.dres) rr[v] = load8<T, AL>(a.dres + ro, col, d);
+      anew<T>(wr[v]);
+    }
+    const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * row);
+    float t[VPT][8], hat[VPT][8], c1 = 0.f, c2 = 0.f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float w[8];
+      IO<T>::unpack(yr[v], t[v]);
+      IO<T>::unpack(hr[v], hat[v]);
+      if (a.w) IO<T>::unpack(wr[v], w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float g = t[v][k], x = (hat[v][k] - st.x) * st.y;
+        hat[v][k] = x;
+        if (there) {
+          dw[v][k] = __builtin_fmaf(g, x, dw[v][k]);
+          db[v][k] += g;
+        }
+        const float u = a.w ? g * w[k] : g;   // zeros past the row's end
+        t[v][k] = u;
+        c1 += u;
+        c2 = __builtin_fmaf(u, x, c2);
+      }
+    }
+    if (!a.dx) continue;
+    c1 = row_sum(c1) * inv_d;
+    c2 = row_sum(c2) * inv_d;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float e[8];
+      if (a.dres) IO<T>::unpack(rr[v], e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        t[v][k] = st.y * (t[v][k] - c1 - hat[v][k] * c2);
+        if (a.dres) t[v][k] += e[k];
+      }
+      if (ok) store8<T, AL>(a.dx + ro, 8 * (lane + LPR * v), d, t[v]);
+    }
+  }
+  auto flush = [&](float (&acc)[VPT][8], float* out) {
+    if constexpr (R == 1) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) store8<float, AL>(out, 8 * (lane + LPR * v), d, acc[v]);
+    } else {
+      static_assert(VPT == 1, "several rows to a workgroup only where a lane has one vector");
+      __syncthreads();
+      IO<float>::store(s_sum + grp * W + 8 * lane, acc[0]);
+      __syncthreads();
+      for (int c = (int)threadIdx.x; c < d; c += LANES) {
+        float s = s_sum[c];
+        for (int g = 1; g < R; ++g) s += s_sum[g * W + c];
+        out[c] = s;
+      }
+    }
+  };
+  if (a.part_w) flush(dw, a.part_w + (int64_t)blockIdx.x * d);
+  if (a.part_b) flush(db, a.part_b + (int64_t)blockIdx.x * d);
+}
+
+// dw (blockIdx.y 0) and db (1): the workgroups' partial rows summed in order by 64 groups for 16 columns, then the groups
+constexpr int SUM_LANES = 1024, SUM_COLS = 16;
+template <typename T>
+__global__ __launch_bounds__(SUM_LANES) void k_layer_norm_sum(const float* __restrict__ part_w, const float* __restrict__ part_b,
+                                                              T* __restrict__ dw, T* __restrict__ db, int parts, int d) {
+  constexpr int GROUPS = SUM_LANES / SUM_COLS;
+  __shared__ float s[SUM_LANES];
+  const float* part = blockIdx.y ? part_b : part_w;
+  T* out = blockIdx.y ? db : dw;
+  if (!out) return;
+  const int tid = (int)threadIdx.x, c = (int)blockIdx.x * SUM_COLS + tid % SUM_COLS, grp = tid / SUM_COLS;
+  float acc = 0.f;
+  if (c < d) {
+    int i = grp;
+    for (; i + 3 * GROUPS < parts; i += 4 * GROUPS) {   // four partial rows' loads in flight
+      float e[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) e[u] = part[(int64_t)(i + u * GROUPS) * d + c];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) acc += e[u];
+    }
+    for (; i < parts; i += GROUPS) acc += part[(int64_t)i * d + c];
+  }
+  s[tid] = acc;
+  __syncthreads();
+  for (int w = GROUPS / 2; w > 0; w >>= 1) {
+    if (grp < w) s[tid] += s[tid + SUM_COLS * w];
+    __syncthreads();
+  }
+  if (grp == 0 && c < d) st1(out + c, s[tid]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// distillation. One workgroup per row of logits. The forward streams it once: a running maximum m and the sums of
+// exp((x - m) / tau) and, with labels at a temperature, of exp(x - m); with a teacher_lse the named classes, marked in a
+// bitmap in LDS (a byte for the eight logits of a vector), are summed apart from the others, so that the others' share
+// q_rest never comes from a difference. The backward streams the row again and writes the gradient as if no class were
+// named, then, past a barrier, the row's k named elements once more with theirs.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr float LOG2E = 1.4426950408889634f;
+
+// what the forward keeps of a row
+struct DistillRow {
+  float kl, ce;           // the row's terms
+  float counts, labelled; // 1 or 0
+  float m, l, l1;         // the maximum, and the logs of the sums of exp((x - m) / tau) and exp(x - m)
+  float mr, lr;           // the same of the classes that are not named
+  float all, rest;        // P + rest, and rest
+  float teacher;          // p_i = exp(top_i / tau - teacher)
+};
+static_assert(sizeof(DistillRow) == LMO_DISTILL_SAVED * sizeof(float), "saved row");
+
+struct Sums {   // running maximum, sum of exp((x - m) / tau) and, HARD, of exp(x - m)
+  float m = -INFINITY, s = 0.f, s1 = 0.f;
+};
+template <bool HARD> __device__ __forceinline__ void grow(Sums& a, float mx, float c, float c1) {   // the maximum, to mx at least
+  if (mx > a.m) {
+    a.s *= __builtin_amdgcn_exp2f((a.m - mx) * c);
+    if (HARD) a.s1 *= __builtin_amdgcn_exp2f((a.m - mx) * c1);
+    a.m = mx;
+  }
+}
+template <bool HARD> __device__ __forceinline__ void take(Sums& a, float x, float c, float c1) {
+  if (x != x) {
+    a.s = a.s1 = x;
+    if (a.m == -INFINITY) a.m = 0.f;
+    return;
+  }
+  grow<HARD>(a, x, c, c1);
+  if (a.m == -INFINITY) return;
+  a.s += __builtin_amdgcn_exp2f((x - a.m) * c);
+  if (HARD) a.s1 += __builtin_amdgcn_exp2f((x - a.m) * c1);
+}
+// two sets of sums as one
+template <bool HARD> __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c, float c1) {
+  Sums r;
+  r.m = fmaxf(a.m, b.m);
+  const float fa = a.m == r.m ? 1.f : exp2f((a.m - r.m) * c), fb = b.m == r.m ? 1.f : exp2f((b.m - r.m) * c);
+  r.s = a.s * fa + b.s * fb;
+  if (HARD) {
+    const float ga = a.m == r.m ? 1.f : exp2f((a.m - r.m) * c1), gb = b.m == r.m ? 1.f : exp2f((b.m - r.m) * c1);
+    r.s1 = a.s1 * ga + b.s1 * gb;
+  }
+  return r;
+}
+template <typename Op, int WAVES> __device__ __forceinline__ float wg_reduce(float v, float* red, Op op) {   // to every lane
+  v = lanes_reduce(v, 64, op);
+  __syncthreads();   // red may still be read from the reduction before
+  if (((int)threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int k = 1; k < WAVES; ++k) v = op(v, red[k]);
+  return v;
+}
+// the lanes' sums as the workgroup's (fmaxf skips a NaN maximum; sums carry it)
+template <bool HARD, int WAVES> __device__ __forceinline__ Sums wg_joined(Sums a, float* red, float c, float c1) {
+  Sums r;
+  r.m = wg_reduce<MaxOp, WAVES>(a.m, red, MaxOp());
+  r.s = wg_reduce<AddOp, WAVES>(a.m == r.m ? a.s : a.s * exp2f((a.m - r.m) * c), red, AddOp());
+  if (HARD) r.s1 = wg_reduce<AddOp, WAVES>(a.m == r.m ? a.s1 : a.s1 * exp2f((a.m - r.m) * c1), red, AddOp());
+  return r;
+}
+
+__device__ __forceinline__ float ld_as(const void* p, int64_t i, int dtype) {
+  return dtype == LDR_F32 ? static_cast<const float*>(p)[i]
+         : dtype == LDR_BF16 ? ld1(static_cast<const bf16_t*>(p) + i) : ld1(static_cast<const _Float16*>(p) + i);
+}
+// a named class as an int: -1 names nothing, vocab stands for any past the last
+__device__ __forceinline__ int id_of(const void* ids, int wide, int64_t i, int vocab) {
+  const int64_t v = wide ? static_cast<const int64_t*>(ids)[i] : (int64_t) static_cast<const int32_t*>(ids)[i];
+  return v < 0 ? -1 : v >= vocab ? vocab : (int)v;
+}
+
+struct Distill {
+  const void *logits, *top, *ids;
+  const float* teacher_lse;
+  const int64_t* labels;
+  DistillRow* saved;
+  const float *coef, *dloss;
+  void* dlogits;
+  int vocab, k, top_dtype, wide;
+  float tau;
+};
+
+template <typename T, int LANES, bool TAIL, bool HARD>
+__global__ __launch_bounds__(LANES) void k_distill_fwd(const Distill a) {
+  constexpr int WAVES = LANES / 64, U = 4;
+  extern __shared__ unsigned s_map[];   // TAIL: the named classes' bits, 32 to a word
+  __shared__ float red[WAVES];
+  const int64_t row = blockIdx.x;
+  const int vocab = a.vocab, k = a.k, tid = (int)threadIdx.x, nv = vocab >> 3;
+  const T* x = static_cast<const T*>(a.logits) + row * vocab;
+  const float c = LOG2E / a.tau, c1 = LOG2E;
+  const int64_t label = a.labels ? a.labels[row] : -100;
+  // the teacher: which classes count, its maximum and sum
+  float zm = -INFINITY, named = 0.f, bad = 0.f;
+  for (int i = tid; i < k; i += LANES) {
+    const int id = id_of(a.ids, a.wide, row * k + i, vocab);
+    if (id < 0) continue;
+    named = 1.f;
+    if (id >= vocab) bad = 1.f;
+    zm = fmaxf(zm, ld_as(a.top, row * k + i, a.top_dtype) * c);
+  }
+  const bool counts = wg_reduce<MaxOp, WAVES>(named, red, MaxOp()) > 0.f;
+  const bool labelled = label != -100;
+  DistillRow out{};
+  if (!counts && !labelled) {   // workgroup-uniform
+    if (tid == 0) a.saved[row] = out;
+    return;
+  }
+  bad = wg_reduce<MaxOp, WAVES>(bad, red, MaxOp());
+  if (TAIL) {
+    const int words = (vocab + 31) >> 5;
+    for (int i = tid; i < words; i += LANES) s_map[i] = 0u;
+    __syncthreads();
+    for (int i = tid; i < k; i += LANES) {
+      const int id = id_of(a.ids, a.wide, row * k + i, vocab);
+      if (id >= 0 && id < vocab) atomicOr(s_map + (id >> 5), 1u << (id & 31));   // bits: no order to depend on
+    }
+    __syncthreads();
+  }
+  float others = 1.f;   // whether a class is left that is not named
+  if (TAIL && k >= vocab) {
+    float n = 0.f;
+    for (int i = tid; i < (vocab + 31) >> 5; i += LANES) n += (float)__popc(s_map[i]);
+    others = wg_reduce<AddOp, WAVES>(n, red, AddOp()) < (float)vocab ? 1.f : 0.f;
+  }
+  Sums s, sn;   // of the classes (TAIL: those not named), and of the named ones
+  auto vec = [&](const typename IO<T>::Raw& r, int v) {
+    float e[8];
+    IO<T>::unpack(r, e);
+    if (TAIL) {
+      const unsigned bits = reinterpret_cast<const unsigned char*>(s_map)[v];
+      if (bits) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (bits >> j & 1u) {
+            take<HARD>(sn, e[j], c, c1);
+            e[j] = -INFINITY;
+          }
+      }
+    }
+    float mx = e[0];
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      mx = fmaxf(mx, e[j]);
+      nan |= e[j] != e[j];
+    }
+    grow<HARD>(s, mx, c, c1);
+    const float m = s.m == -INFINITY ? 0.f : s.m;
+    float t = 0.f, t1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      t += __builtin_amdgcn_exp2f((e[j] - m) * c);
+      if (HARD) t1 += __builtin_amdgcn_exp2f((e[j] - m) * c1);
+    }
+    s.s = nan ? NAN : s.s + t;
+    if (HARD) s.s1 = nan ? NAN : s.s1 + t1;
+    s.m = nan ? m : s.m;   // a NaN stays in the sum, whose maximum has to be a number
+  };
+  int v = tid;
+  for (; v + (U - 1) * LANES < nv; v += U * LANES) {   // U loads in flight
+    typename IO<T>::Raw r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = UIO<T>::raw_nt(x + 8 * (int64_t)(v + u * LANES));
+#pragma unroll
+    for (int u = 0; u < U; ++u) vec(r[u], v + u * LANES);
+  }
+  for (; v < nv; v += LANES) vec(UIO<T>::raw_nt(x + 8 * (int64_t)v), v);
+  if (tid < (vocab & 7)) {
+    const int i = 8 * nv + tid;
+    if (TAIL && (s_map[i >> 5] >> (i & 31) & 1u)) take<HARD>(sn, ld1(x + i), c, c1);
+    else take<HARD>(s, ld1(x + i), c, c1);
+  }
+  s = wg_joined<HARD, WAVES>(s, red, c, c1);
+  if (TAIL) {
+    out.mr = s.m;
+    out.lr = logf(s.s);
+    s = joined<HARD>(s, wg_joined<HARD, WAVES>(sn, red, c, c1), c, c1);
+  }
+  out.m = s.m;
+  out.l = logf(s.s);   // kept apart from the maximum: their sum would lose it beside large logits
+  out.l1 = HARD ? logf(s.s1) : out.l;
+  if (counts) {
+    // p_i = exp(z_i - teacher) of z = top / tau
+    float teacher;
+    if (TAIL) {
+      teacher = a.teacher_lse[row];
+    } else {
+      zm = wg_reduce<MaxOp, WAVES>(zm, red, MaxOp());
+      float zs = 0.f;
+      for (int i = tid; i < k; i += LANES)
+        if (id_of(a.ids, a.wide, row * k + i, vocab) >= 0) zs += exp2f(ld_as(a.top, row * k + i, a.top_dtype) * c - zm);
+      zs = wg_reduce<AddOp, WAVES>(zs, red, AddOp());
+      teacher = (zm + log2f(zs)) * (1.f / LOG2E);
+    }
+    const float inv_tau = 1.f / a.tau;
+    float kl = 0.f, P = 0.f;
+    for (int i = tid; i < k; i += LANES) {
+      const int id = id_of(a.ids, a.wide, row * k + i, vocab);
+      if (id < 0 || id >= vocab) continue;
+      const float lp = ld_as(a.top, row * k + i, a.top_dtype) * inv_tau - teacher, p = expf(lp);
+      P += p;
+      if (!(p <= 0.f)) kl += p * (lp - ((ld1(x + id) - s.m) * inv_tau - out.l));
+    }
+    kl = wg_reduce<AddOp, WAVES>(kl, red, AddOp());
+    P = wg_reduce<AddOp, WAVES>(P, red, AddOp());
+    if (TAIL) {
+      out.rest = P != P ? P : others * fmaxf(0.f, 1.f - P);
+      if (out.rest > 0.f) kl += out.rest * (logf(out.rest) - ((out.mr - out.m) * inv_tau + out.lr - out.l));
+    }
+    out.kl = bad > 0.f ? NAN : kl;
+    out.all = P + out.rest;
+    out.counts = 1.f;
+    out.teacher = teacher;
+  }
+  if (labelled) {
+    out.ce = label >= 0 && label < vocab ? out.l1 + (out.m - ld1(x + label)) : NAN;
+    out.labelled = 1.f;
+  }
+  if (tid == 0) a.saved[row] = out;
+}
+
+// the loss, and what the rows' gradients are multiplied by, by one workgroup: lane sums in order, then a fixed tree
+constexpr int MEAN_LANES = 1024;
+__global__ __launch_bounds__(MEAN_LANES) void k_distill_mean(const DistillRow* __restrict__ saved, int64_t rows, float tau,
+                                                             float hard, float* __restrict__ coef, float* __restrict__ loss) {
+  __shared__ float4 s[MEAN_LANES];
+  const int tid = (int)threadIdx.x;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [](float4& p, const float4& q) {
+    p.x += q.x;
+    p.y += q.y;
+    p.z += q.z;
+    p.w += q.w;
+  };
+  int64_t i = tid;
+  for (; i + 3 * MEAN_LANES < rows; i += 4 * MEAN_LANES) {   // four rows' loads in flight
+    float4 e[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) e[u] = *reinterpret_cast<const float4*>(saved + i + u * MEAN_LANES);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add(a, e[u]);
+  }
+  for (; i < rows; i += MEAN_LANES) add(a, *reinterpret_cast<const float4*>(saved + i));
+  s[tid] = a;
+  __syncthreads();
+  for (int w = MEAN_LANES / 2; w > 0; w >>= 1) {
+    if (tid < w) add(s[tid], s[tid + w]);
+    __syncthreads();
+  }
+  if (tid == 0) {
+    const float n = fmaxf(s[0].z, 1.f), m = fmaxf(s[0].w, 1.f);   // counts are exact below 2^24 rows a lane's sum
+    const float soft = (1.f - hard) * tau;
+    coef[0] = soft / n;
+    coef[1] = hard / m;
+    *loss = soft * tau * (s[0].x / n) + hard * (s[0].y / m);
+  }
+}
+
+template <typename T, int LANES, bool TAIL, bool HARD>
+__global__ __launch_bounds__(LANES) void k_distill_bwd(const Distill a) {
+  constexpr int U = 4;
+  extern __shared__ unsigned s_dyn[];   // k ids, k probabilities
+  int* s_id = reinterpret_cast<int*>(s_dyn);
+  float* s_p = reinterpret_cast<float*>(s_dyn) + a.k;
+  const int64_t row = blockIdx.x;
+  const int vocab = a.vocab, k = a.k, tid = (int)threadIdx.x, nv = vocab >> 3;
+  const T* x = static_cast<const T*>(a.logits) + row * vocab;
+  T* o = static_cast<T*>(a.dlogits) + row * vocab;
+  const DistillRow r = a.saved[row];
+  const float g = *a.dloss, zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (r.counts == 0.f && r.labelled == 0.f) {   // workgroup-uniform
+    for (int v = tid; v < nv; v += LANES) UIO<T>::store(o + 8 * (int64_t)v, zero);
+    if (tid < (vocab & 7)) st1(o + 8 * nv + tid, 0.f);
+    return;
+  }
+  const float inv_tau = 1.f / a.tau, c = LOG2E / a.tau;
+  const float ga = r.counts != 0.f ? g * a.coef[0] : 0.f, gb = HARD && r.labelled != 0.f ? g * a.coef[1] : 0.f;
+  const float qa = ga * r.all, ra = TAIL ? ga * r.rest : 0.f;   // factors of softmax(x / tau), and of the others' own softmax
+  const int64_t label = HARD && r.labelled != 0.f ? a.labels[row] : -1;
+  const float l2 = r.l * LOG2E, l12 = r.l1 * LOG2E, lr2 = r.lr * LOG2E;
+  if (r.counts != 0.f)
+    for (int i = tid; i < k; i += LANES) {
+      const int id = id_of(a.ids, a.wide, row * k + i, vocab);
+      s_id[i] = id;
+      s_p[i] = id < 0 ? 0.f : expf(ld_as(a.top, row * k + i, a.top_dtype) * inv_tau - r.teacher);
+    }
+  // the gradient at class i of logit e; `named`: less p, its teacher's probability, instead of the others' share
+  auto grad = [&](float e, int64_t i, bool named, float p) {
+    float t = qa * __builtin_amdgcn_exp2f((e - r.m) * c - l2);
+    if (HARD) t += gb * (__builtin_amdgcn_exp2f((e - r.m) * LOG2E - l12) - (i == label ? 1.f : 0.f));
+    if (named) t -= ga * p;
+    else if (TAIL) t -= r.rest > 0.f ? ra * __builtin_amdgcn_exp2f((e - r.mr) * c - lr2) : 0.f;
+    return t;
+  };
+  auto vec = [&](const typename IO<T>::Raw& raw, int v) {
+    float e[8];
+    IO<T>::unpack(raw, e);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = grad(e[j], 8 * (int64_t)v + j, false, 0.f);
+    UIO<T>::store(o + 8 * (int64_t)v, e);
+  };
+  int v = tid;
+  for (; v + (U - 1) * LANES < nv; v += U * LANES) {   // U loads in flight
+    typename IO<T>::Raw raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = UIO<T>::raw_nt(x + 8 * (int64_t)(v + u * LANES));
+#pragma unroll
+    for (int u = 0; u < U; ++u) vec(raw[u], v + u * LANES);
+  }
+  for (; v < nv; v += LANES) vec(UIO<T>::raw_nt(x + 8 * (int64_t)v), v);
+  if (tid < (vocab & 7)) {
+    const int64_t i = 8 * (int64_t)nv + tid;
+    st1(o + i, grad(ld1(x + i), i, false, 0.f));
+  }
+  if (r.counts == 0.f) return;
+  __syncthreads();   // orders the row's stores before those below, and the named classes in LDS
+  for (int i = tid; i < k; i += LANES) {
+    const int id = s_id[i];
+    if (id < 0 || id >= vocab) continue;
+    float p = 0.f;
+    for (int j = 0; j < k; ++j) p += s_id[j] == id ? s_p[j] : 0.f;   // a class named twice: both write the same value
+    st1(o + id, grad(ld1(x + id), id, true, p));
+  }
+}
+
+inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool al_of(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == LDR_F32 ? 3u : 1u)) == 0; }
+inline bool dtype_ok(int dt) { return dt == LDR_F32 || dt == LDR_BF16 || dt == LDR_F16; }
+inline unsigned grid_of(int64_t blocks, int64_t cap) { return (unsigned)(blocks < cap ? blocks : cap); }
+inline int launched() { return (int)hipGetLastError(); }
+
+#define LMO_TYPE_SWITCH(DT, ...)                                 \
+  if ((DT) == LDR_BF16) { typedef bf16_t T; __VA_ARGS__; }       \
+  else if ((DT) == LDR_F16) { typedef _Float16 T; __VA_ARGS__; } \
+  else { typedef float T; __VA_ARGS__; }
+#define LMO_BOOL_SWITCH(V, NAME, ...)                            \
+  if (V) { constexpr bool NAME = true; __VA_ARGS__; }            \
+  else { constexpr bool NAME = false; __VA_ARGS__; }
+#define LMO_LANES_SWITCH(N, V, ...)                                                   \
+  switch (N) {                                                                        \
+    case 4: { constexpr int LPR = 4, VPT = 1; __VA_ARGS__; } break;                   \
+    case 16: { constexpr int LPR = 16, VPT = 1; __VA_ARGS__; } break;                 \
+    case 64: { constexpr int LPR = 64, VPT = 1; __VA_ARGS__; } break;                 \
+    case 128: { constexpr int LPR = 128, VPT = 1; __VA_ARGS__; } break;               \
+    case 256: { constexpr int LPR = 256, VPT = 1; __VA_ARGS__; } break;               \
+    case 512: { constexpr int LPR = 512, VPT = 1; __VA_ARGS__; } break;               \
+    default:                                                                          \
+      if ((V) == 1) { constexpr int LPR = 1024, VPT = 1; __VA_ARGS__; }               \
+      else { constexpr int LPR = 1024, VPT = 2; __VA_ARGS__; }                        \
+      break;                                                                          \
+  }
+
+// lanes per row, eight columns each (twice eight past 8192): 4, 16 or 64 of a wave, or 2 to 16 waves
+inline int lanes_per_row(int64_t d) {
+  return d <= 32 ? 4 : d <= 128 ? 16 : d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024;
+}
+struct Plan { int64_t per, parts; };   // the backward's consecutive rows of a workgroup, and its workgroups
+inline Plan plan_of(int64_t rows, int64_t d) {
+  const int lpr = lanes_per_row(d), r = lpr > WG ? 1 : WG / lpr;
+  const int64_t most = lpr > 512 ? 256 : lpr > WG ? 384 : 768;
+  int64_t per = (rows + most - 1) / most;
+  per = (per + r - 1) / r * r;
+  return Plan{per, (rows + per - 1) / per};
+}
+int norm_shape(int64_t rows, int64_t d, int dtype) {
+  if (!dtype_ok(dtype)) return LDR_E_DTYPE;
+  if (d < 1 || d > LMO_NORM_MAX_WIDTH) return LDR_E_SHAPE;
+  if (rows < 0 || rows > 0x7fffffff) return LDR_E_ARG;
+  return LDR_OK;
+}
+
+// workgroups of 1024 lanes where there are too few rows for the CUs, of 256 otherwise
+inline bool wide_workgroups(int64_t rows) { return rows <= 512; }
+
+int distill_args(const Distill& a, int64_t rows, int64_t vocab, int64_t k, int dtype, bool tail) {
+  if (!dtype_ok(dtype) || !dtype_ok(a.top_dtype)) return LDR_E_DTYPE;
+  if (vocab < 1 || vocab > 0x7fffffff - 8 || k < 1 || k > LMO_DISTILL_MAX_TOP || (tail && vocab > LMO_DISTILL_MAX_TAIL))
+    return LDR_E_SHAPE;
+  if (rows < 0 || rows > 0x7fffffff || !(a.tau > 0.f) || !(a.tau < INFINITY)) return LDR_E_ARG;
+  if (rows > 0 && (!a.logits || !a.top || !a.ids || !a.saved)) return LDR_E_ARG;
+  if (!al_of(a.logits, dtype) || !al_of(a.dlogits, dtype) || !al_of(a.top, a.top_dtype) || !al16(a.saved) ||
+      (reinterpret_cast<uintptr_t>(a.ids) & (a.wide ? 7u : 3u)) || (reinterpret_cast<uintptr_t>(a.labels) & 7u) ||
+      !al_of(a.teacher_lse, LDR_F32))
+    return LDR_E_ALIGN;
+  return LDR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lmo_abi_version(void) { return LMO_ABI_VERSION; }
+
+int lmo_layer_norm_fwd(const void* x, const void* add, const void* w, const void* b, void* h_out, void* y, float* stats,
+                       int64_t rows, int64_t d, float eps, int dtype, void* stream) {
+  const int e = norm_shape(rows, d, dtype);
+  if (e || rows == 0) return e;
+  if (!x || !y || (add && !h_out)) return LDR_E_ARG;
+  bool al = d % 8 == 0;
+  for (const void* p : {x, add, w, b, (const void*)(add ? h_out : nullptr), (const void*)y}) {
+    if (!al_of(p, dtype)) return LDR_E_ALIGN;
+    al = al && al16(p);
+  }
+  if (reinterpret_cast<uintptr_t>(stats) & 7u) return LDR_E_ALIGN;
+  const int lpr = lanes_per_row(d), r = lpr > WG ? 1 : WG / lpr;
+  const unsigned grid = grid_of((rows + r - 1) / r, lpr > WG ? 1024 : 2048);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  LMO_TYPE_SWITCH(dtype, {
+    const NormFwd<T> a{static_cast<const T*>(x), static_cast<const T*>(add), static_cast<const T*>(w), static_cast<const T*>(b),
+                       static_cast<T*>(h_out), static_cast<T*>(y), stats, (int)rows, (int)d, eps};
+    LMO_LANES_SWITCH(lpr, d <= 8192 ? 1 : 2,
+        LMO_BOOL_SWITCH(al, AL, hipLaunchKernelGGL((k_layer_norm_fwd<T, LPR, VPT, AL>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a)))
+  })
+  return launched();
+}
+
+int64_t lmo_layer_norm_scratch(int64_t rows, int64_t d) {
+  return rows < 1 || d < 1 ? 0 : 2 * d * plan_of(rows, d).parts;
+}
+
+int lmo_layer_norm_bwd(const void* dy, const void* h, const void* w, const float* stats, const void* dres, void* dx,
+                       void* dw, void* db, float* scratch, int64_t rows, int64_t d, int dtype, void* stream) {
+  const int e = norm_shape(rows, d, dtype);
+  if (e || rows == 0) return e;
+  if (!dy || !h || !stats || ((dw || db) && !scratch)) return LDR_E_ARG;
+  if (!dx && !dw && !db) return LDR_OK;
+  bool al = d % 8 == 0;
+  for (const void* p : {dy, h, w, dres, (const void*)dx, (const void*)scratch}) {
+    if (!al_of(p, dtype)) return LDR_E_ALIGN;
+    al = al && al16(p);
+  }
+  if (!al_of(scratch, LDR_F32) || !al_of(dw, dtype) || !al_of(db, dtype) || (reinterpret_cast<uintptr_t>(stats) & 7u))
+    return LDR_E_ALIGN;
+  const Plan plan = plan_of(rows, d);
+  const int parts = (int)plan.parts;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  LMO_TYPE_SWITCH(dtype, {
+    const NormBwd<T> a{static_cast<const T*>(dy), static_cast<const T*>(h), static_cast<const T*>(w), stats,
+                       static_cast<const T*>(dres), static_cast<T*>(dx), dw ? scratch : nullptr,
+                       db ? scratch + parts * d : nullptr, (int)rows, (int)d, (int)plan.per};
+    LMO_LANES_SWITCH(lanes_per_row(d), d <= 8192 ? 1 : 2,
+        LMO_BOOL_SWITCH(al, AL, hipLaunchKernelGGL((k_layer_norm_bwd<T, LPR, VPT, AL>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a)))
+    const int err = launched();
+    if (err) return err;
+    if (dw || db)
+      hipLaunchKernelGGL(k_layer_norm_sum<T>, dim3((unsigned)((d + SUM_COLS - 1) / SUM_COLS), 2), dim3(SUM_LANES), 0, st, a.part_w,
+                         a.part_b, static_cast<T*>(dw), static_cast<T*>(db), parts, (int)d);
+  })
+  return launched();
+}
+
+int lmo_distill_fwd(const void* logits, const void* top, int top_dtype, const void* ids, int wide_ids,
+                    const float* teacher_lse, const int64_t* labels, float tau, float hard, float* saved, float* coef,
+                    float* loss, int64_t rows, int64_t vocab, int64_t k, int dtype, void* stream) {
+  const Distill a{logits, top, ids, teacher_lse, labels, reinterpret_cast<DistillRow*>(saved), nullptr, nullptr, nullptr,
+                  (int)vocab, (int)k, top_dtype, wide_ids, tau};
+  const int e = distill_args(a, rows, vocab, k, dtype, teacher_lse != nullptr);
+  if (e) return e;
+  if (!coef || !loss || !(hard >= 0.f && hard <= 1.f)) return LDR_E_ARG;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (rows > 0) {
+    const size_t map = teacher_lse ? ((size_t)vocab + 31) / 32 * 4 : 0;
+    // at temperature 1 the two sums are one
+    LMO_TYPE_SWITCH(dtype, LMO_BOOL_SWITCH(teacher_lse != nullptr, TAIL, LMO_BOOL_SWITCH(labels != nullptr && tau != 1.f, HARD, {
+      if (wide_workgroups(rows))
+        hipLaunchKernelGGL((k_distill_fwd<T, 1024, TAIL, HARD>), dim3((unsigned)rows), dim3(1024), map, st, a);
+      else
+        hipLaunchKernelGGL((k_distill_fwd<T, 256, TAIL, HARD>), dim3((unsigned)rows), dim3(256), map, st, a);
+    })))
+    const int err = launched();
+    if (err) return err;
+  }
+  hipLaunchKernelGGL(k_distill_mean, dim3(1), dim3(MEAN_LANES), 0, st, reinterpret_cast<const DistillRow*>(saved), rows, tau, hard,
+                     coef, loss);
+  return launched();
+}
+
+int lmo_distill_bwd(const void* logits, const void* top, int top_dtype, const void* ids, int wide_ids,
+                    const int64_t* labels, float tau, const float* saved, const float* coef, const float* dloss,
+                    void* dlogits, int64_t rows, int64_t vocab, int64_t k, int tail, int dtype, void* stream) {
+  const Distill a{logits, top, ids, nullptr, labels, reinterpret_cast<DistillRow*>(const_cast<float*>(saved)), coef, dloss,
+                  dlogits, (int)vocab, (int)k, top_dtype, wide_ids, tau};
+  const int e = distill_args(a, rows, vocab, k, dtype, tail != 0);
+  if (e || rows == 0) return e;
+  if (!coef || !dloss || !dlogits) return LDR_E_ARG;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const size_t lds = 8 * (size_t)k;
+  LMO_TYPE_SWITCH(dtype, LMO_BOOL_SWITCH(tail != 0, TAIL, LMO_BOOL_SWITCH(labels != nullptr, HARD, {
+    if (wide_workgroups(rows))
+      hipLaunchKernelGGL((k_distill_bwd<T, 1024, TAIL, HARD>), dim3((unsigned)rows), dim3(1024), lds, st, a);
+    else
+      hipLaunchKernelGGL((k_distill_bwd<T, 256, TAIL, HARD>), dim3((unsigned)rows), dim3(256), lds, st, a);
+  })))
+  return launched();
+}
+
+}  // extern "C"
