@@ -1,7 +1,7 @@
 /*
  * loopback_model.h -- C ABI of libloopback_model.so: MI355X (gfx950) kernels of a language model's training step that stand
- * beside those of loopback_lm.h: layer norm with the residual's add, and the distillation loss from a teacher's highest
- * logits, each forward and backward in passes over their rows.
+ * beside those of loopback_lm.h: layer norm with the residual's add and the distillation loss from a teacher's highest
+ * logits, each forward and backward in passes over their rows, and differential attention on the matrix cores.
  *
  * Conventions: device pointers; dtype is LDR_F32, LDR_BF16 or LDR_F16 (loopback_read.h); every statistic and sum is fp32,
  * results are rounded once from fp32; stream is a hipStream_t; nothing synchronizes with the host or allocates. The return
@@ -64,6 +64,40 @@ int lmo_distill_fwd(const void* logits, const void* top, int top_dtype, const vo
 int lmo_distill_bwd(const void* logits, const void* top, int top_dtype, const void* ids, int wide_ids,
                     const int64_t* labels, float tau, const float* saved, const float* coef, const float* dloss,
                     void* dlogits, int64_t rows, int64_t vocab, int64_t k, int tail, int dtype, void* stream);
+
+/* ---- differential attention -----------------------------------------------------------------------------------------
+ * y[b, i, h] = (P1 - lam P2) v, Pm = softmax over the keys j that the query sees of scale q[b, i, 2 h + m - 1] k[b, j, 2 h' + m - 1],
+ * h' = h hk / H: groups of H / hk heads share a pair of keys and its values. q [b, tq, 2 H, dh], k [b, tk, 2 hk, dh], v [b, tk,
+ * hk, dv], bf16 or fp16, by strides in elements, multiples of 8, the last dimension's 1 and bases 16-byte aligned; dh a multiple
+ * of 8 up to 128, dv up to 256. Query i sees the keys j < lengths[b] (NULL: tk) and, causal, j <= starts[b] + i (NULL: tk - tq);
+ * one that sees none has zeros and no gradient. Keys and values at and past lengths[b] are not read into anything; lengths are
+ * taken as within 0 .. tk. lam by strides too (0 where it is shared), fp32 where lam32, else the rows' type. */
+typedef struct { const void* p; int64_t b, t, h; } lmo_strides;
+typedef struct { int64_t b, tq, tk, h, hk, dh, dv; int causal; float scale; } lmo_diff_shape;
+
+/* Floats of lmo_diff_attn_fwd's scratch; record: with second and lse. */
+int64_t lmo_diff_attn_scratch(const lmo_diff_shape* shape, int record);
+
+/* out [b, tq, H, dv] contiguous. For a backward, both or neither: second [b, tq, H, dv], P2 v, and lse [2, b, H, tq], the base-2
+ * logarithms of the sums of exp(scores) (infinite for a query that sees no key). */
+int lmo_diff_attn_fwd(const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
+                      const int32_t* lengths, const int32_t* starts, void* out, void* second, float* lse, float* scratch,
+                      const lmo_diff_shape* shape, int dtype, void* stream);
+
+/* What dlam has: one value, one per head [H], or one per query and head [b, tq, H]; of lam's type. */
+#define LMO_LAM_LAYER 0
+#define LMO_LAM_HEAD 1
+#define LMO_LAM_TOKEN 2
+
+/* Floats of lmo_diff_attn_bwd's scratch. */
+int64_t lmo_diff_attn_bwd_scratch(const lmo_diff_shape* shape, int lam_kind);
+
+/* The gradients, contiguous, of the forward's shapes: dq, and, where wanted (dk and dv both or neither), dk, dv and dlam. dy is
+ * contiguous. Rows of dk and dv that no query sees are zeros. */
+int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
+                      const int32_t* lengths, const int32_t* starts, const void* out, const void* second, const float* lse,
+                      const void* dy, void* dq, void* dk, void* dv, void* dlam, int lam_kind, float* scratch,
+                      const lmo_diff_shape* shape, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,5 +1,5 @@
 """Build libloopback_read.so (the read's kernels and C ABI), libloopback_lm.so (the language model's), libloopback_block.so (a
-block's feed-forward, join and dropout) and libloopback_model.so (layer norm, the distillation loss)
+block's feed-forward, join and dropout) and libloopback_model.so (layer norm, differential attention, the distillation loss)
 in-tree with hipcc for gfx950 (MI355X), and _host.so, the Python module's launch path, with g++ against torch's headers.
 
     python -m loopback_amd.build                          # compile, print the commands
@@ -29,7 +29,7 @@ LM_SRC = os.path.join(HERE, "csrc", "loopback_lm.hip")
 LM_LIB = os.path.join(HERE, "libloopback_lm.so")
 BLOCK_SRC = [os.path.join(HERE, "csrc", f) for f in ("loopback_block.hip", "loopback_ffn.hip")]
 BLOCK_LIB = os.path.join(HERE, "libloopback_block.so")
-MODEL_SRC = [os.path.join(HERE, "csrc", f) for f in ("loopback_model.hip",)]
+MODEL_SRC = [os.path.join(HERE, "csrc", f) for f in ("loopback_model.hip", "loopback_diff_attn.hip")]
 MODEL_LIB = os.path.join(HERE, "libloopback_model.so")
 HOST_SRC = os.path.join(HERE, "csrc", "host.cpp")
 HOST_LIB = os.path.join(HERE, "_host.so")

@@ -141,7 +141,7 @@ template <typename... A, int ID> struct Entry<int (*)(A...), ID> {
 #define LBK_ENTRIES(X)                                                                                            \
   X(dropout) X(join_fwd) X(join_bwd) X(pad_rows) X(ffn_gate_up) X(ffn_dgate_up) X(linear_fwd) X(linear_dx) X(linear_dw)
 
-#define LMO_ENTRIES(X) X(layer_norm_fwd) X(layer_norm_bwd) X(distill_fwd) X(distill_bwd)
+#define LMO_ENTRIES(X) X(layer_norm_fwd) X(layer_norm_bwd) X(distill_fwd) X(distill_bwd) X(diff_attn_fwd) X(diff_attn_bwd)
 
 enum Id {
 #define X(name) ID_##name,
@@ -160,6 +160,8 @@ int64_t (*join_scratch)(int64_t, int64_t, int64_t) = nullptr;
 int64_t (*linear_scratch)(int64_t, int64_t, int64_t) = nullptr;
 int64_t (*ffn_saved_bytes)(int64_t, int64_t) = nullptr;
 int64_t (*layer_norm_scratch)(int64_t, int64_t) = nullptr;
+int64_t (*diff_attn_scratch)(const lmo_diff_shape*, int) = nullptr;
+int64_t (*diff_attn_bwd_scratch)(const lmo_diff_shape*, int) = nullptr;
 
 struct Binding { const char* name; void (*bind)(void*); };
 const Binding bindings[] = {
@@ -173,6 +175,8 @@ const Binding bindings[] = {
     LMO_ENTRIES(X)
 #undef X
     {"lmo_layer_norm_scratch", [](void* p) { layer_norm_scratch = reinterpret_cast<decltype(layer_norm_scratch)>(p); }},
+    {"lmo_diff_attn_scratch", [](void* p) { diff_attn_scratch = reinterpret_cast<decltype(diff_attn_scratch)>(p); }},
+    {"lmo_diff_attn_bwd_scratch", [](void* p) { diff_attn_bwd_scratch = reinterpret_cast<decltype(diff_attn_bwd_scratch)>(p); }},
     {"lbk_join_scratch", [](void* p) { join_scratch = reinterpret_cast<decltype(join_scratch)>(p); }},
     {"lbk_linear_scratch", [](void* p) { linear_scratch = reinterpret_cast<decltype(linear_scratch)>(p); }},
     {"lbk_ffn_saved_bytes", [](void* p) { ffn_saved_bytes = reinterpret_cast<decltype(ffn_saved_bytes)>(p); }},
@@ -304,8 +308,8 @@ struct Gil {
 };
 
 // the backwards' torch forms, Python functions: of block_ops dropout's, the join's and the feed-forward block's, of model_ops
-// layer norm's and the distillation loss's
-constexpr int FORMS = 5, BLOCK_FORMS = 3;
+// layer norm's, the distillation loss's and differential attention's
+constexpr int FORMS = 6, BLOCK_FORMS = 3;
 PyObject* torch_forms[FORMS] = {};
 
 // torch_forms[which](*tensors, *numbers) with None for undefined tensors: its tuple of `results` tensors
@@ -670,7 +674,7 @@ PyObject* host_join(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// ---- the model's operators: layer norm, the distillation loss --------------------------------------------------------
+// ---- the model's operators: layer norm, the distillation loss, differential attention --------------------------------------------------------
 // h (the rounded sum; undefined without add), y, and the rows' mean and rstd where a backward follows
 variable_list layer_norm_run(const at::Tensor& x, const OptTensor& add, const OptTensor& w, const OptTensor& b, double eps,
                              int64_t dtype, int64_t stream, bool keep) {
@@ -864,6 +868,151 @@ PyObject* host_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // torch_forms(dropout, join, ffn): the Python functions that the nodes call where a backward has to be torch operations
+// q [b, tq, 2 h, dh], k [b, tk, 2 hk, dh], v [b, tk, hk, dv] as the kernels take them: themselves, or contiguous copies
+at::Tensor attn_rows(const at::Tensor& t) {
+  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(1) <= (1 << 23) && t.stride(2) <= (1 << 23);
+  for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
+  if (ok) return t;
+  at::Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+lmo_strides strides_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+lmo_strides lam_strides(const at::Tensor& t) {   // one value, one per head, or one per query and head
+  return t.dim() == 3 ? lmo_strides{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}
+                      : lmo_strides{t.data_ptr(), 0, 0, t.dim() == 1 ? t.stride(0) : 0};
+}
+int lam_kind(const at::Tensor& t) { return t.dim() == 3 ? LMO_LAM_TOKEN : t.dim() == 1 ? LMO_LAM_HEAD : LMO_LAM_LAYER; }
+
+struct DiffCall {
+  at::Tensor q, k, v, lam, lengths, starts;   // the last two may be undefined
+  bool causal;
+  double scale;
+  int64_t dtype, stream;
+  lmo_diff_shape shape() const {
+    return {q.size(0), q.size(1), k.size(1), q.size(2) / 2, v.size(2), q.size(3), v.size(3), causal, static_cast<float>(scale)};
+  }
+  int lam32() const { return lam.scalar_type() == at::kFloat; }
+  const int32_t* len() const { return static_cast<const int32_t*>(ptr(lengths)); }
+  const int32_t* start() const { return static_cast<const int32_t*>(ptr(starts)); }
+  void* st() const { return reinterpret_cast<void*>(stream); }
+};
+
+variable_list diff_attn_run(const DiffCall& c, bool keep) {   // y, P2 v and the logarithms (undefined unless kept)
+  const lmo_diff_shape s = c.shape();
+  const auto f32 = at::TensorOptions().dtype(at::kFloat).device(c.q.device());
+  variable_list t{at::empty({s.b, s.tq, s.h, s.dv}, c.q.options()), at::Tensor(), at::Tensor()};
+  if (keep) {
+    t[1] = at::empty_like(t[0]);
+    t[2] = at::empty({2, s.b, s.h, s.tq}, f32);
+  }
+  TORCH_CHECK(MODEL_FN(diff_attn_fwd) && diff_attn_scratch, "lmo_diff_attn_fwd: entry point not bound");
+  const int64_t n = diff_attn_scratch(&s, keep);
+  const at::Tensor scratch = n ? at::empty({n}, f32) : at::Tensor();
+  const at::Tensor q = attn_rows(c.q), k = attn_rows(c.k), v = attn_rows(c.v);
+  const lmo_strides qs = strides_of(q), ks = strides_of(k), vs = strides_of(v), ls = lam_strides(c.lam);
+  launched("lmo_diff_attn_fwd",
+           MODEL_FN(diff_attn_fwd)(&qs, &ks, &vs, &ls, c.lam32(), c.len(), c.start(), t[0].data_ptr(), ptr(t[1]),
+                                   static_cast<float*>(ptr(t[2])), static_cast<float*>(ptr(scratch)), &s, static_cast<int>(c.dtype), c.st()));
+  return t;
+}
+
+struct DiffAttnNode : torch::autograd::Function<DiffAttnNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& lam,
+                            const OptTensor& lengths, const OptTensor& starts, bool causal, double scale, int64_t dtype, int64_t stream) {
+    const DiffCall c{q, k, v, lam, or_none(lengths), or_none(starts), causal, scale, dtype, stream};
+    const variable_list t = diff_attn_run(c, true);
+    ctx->save_for_backward({q, k, v, lam, c.lengths, c.starts, t[0], t[1], t[2]});
+    const lmo_diff_shape s = c.shape();
+    ctx->saved_data["numbers"] = std::vector<int64_t>{s.b, s.tq, s.tk, s.h, s.hk, s.dh, s.dv, dtype, causal, lam.dim(), lam.scalar_type() == at::kFloat};
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return t[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(10);
+    const at::Tensor& dy = grads[0];
+    if (!dy.defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const std::vector<int64_t> n = ctx->saved_data["numbers"].toIntVector();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const int64_t b = n[0], tq = n[1], tk = n[2], h = n[3], hk = n[4], dh = n[5], dv = n[6];
+    const at::ScalarType type = s[0].scalar_type();
+    TORCH_CHECK(code_of(type) == n[7], "the attention's queries came back from a hook with another type: ", type);
+    auto sized = [&](const at::Tensor& t, at::ScalarType ty, at::IntArrayRef sizes) {
+      if (!t.defined()) return;
+      TORCH_CHECK(t.layout() == at::kStrided && t.device() == dy.device() && t.scalar_type() == ty && t.sizes() == sizes,
+                  "an operator's saved tensor came back from a hook with another shape, type or device: ", t.toString(), " ", t.sizes(),
+                  " on ", t.device());
+    };
+    sized(s[0], type, {b, tq, 2 * h, dh});
+    sized(s[1], type, {b, tk, 2 * hk, dh});
+    sized(s[2], type, {b, tk, hk, dv});
+    const at::ScalarType lam_type = n[10] ? at::kFloat : type;
+    if (n[9] == 0) sized(s[3], lam_type, {});
+    else if (n[9] == 1) sized(s[3], lam_type, {h});
+    else sized(s[3], lam_type, {b, tq, h});
+    sized(s[4], at::kInt, {b});
+    sized(s[5], at::kInt, {b});
+    sized(s[6], type, {b, tq, h, dv});
+    sized(s[7], type, {b, tq, h, dv});
+    sized(s[8], at::kFloat, {2, b, h, tq});
+    const bool nq = ctx->needs_input_grad(0), nk = ctx->needs_input_grad(1), nv = ctx->needs_input_grad(2), nl = ctx->needs_input_grad(3);
+    if (!on_kernels(grads, s[6]) || !s[0].is_cuda()) {
+      const variable_list got =
+          torch_form(5, {dy, s[0], s[1], s[2], s[3], s[4], s[5]}, {n[8], nq + 2 * nk + 4 * nv + 8 * nl}, {scale}, 4);
+      std::copy(got.begin(), got.end(), out.begin());
+      return out;
+    }
+    const c10::DeviceGuard on(dy.device());
+    auto aligned = [](const at::Tensor& t) {
+      const at::Tensor r = rows_of(t);
+      return reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 ? r.clone() : r;
+    };
+    const DiffCall c{attn_rows(s[0]), attn_rows(s[1]), attn_rows(s[2]), s[3], rows_of(s[4]), rows_of(s[5]), n[8] != 0, scale, n[7], stream_of(dy)};
+    const at::Tensor y = aligned(s[6]), second = aligned(s[7]), lse = rows_of(s[8]), g = aligned(dy);
+    const lmo_diff_shape sh = c.shape();
+    const int kind = lam_kind(c.lam);
+    TORCH_CHECK(MODEL_FN(diff_attn_bwd) && diff_attn_bwd_scratch, "lmo_diff_attn_bwd: entry point not bound");
+    const at::Tensor scratch = at::empty({diff_attn_bwd_scratch(&sh, kind)}, at::TensorOptions().dtype(at::kFloat).device(dy.device()));
+    const at::Tensor dq = at::empty({b, tq, 2 * h, dh}, g.options());
+    at::Tensor dk, dval, dlam;
+    if (nk || nv) {
+      dk = at::empty({b, tk, 2 * hk, dh}, g.options());
+      dval = at::empty({b, tk, hk, dv}, g.options());
+    }
+    if (nl) dlam = at::empty(c.lam.sizes(), c.lam.options());
+    const lmo_strides qs = strides_of(c.q), ks = strides_of(c.k), vs = strides_of(c.v), ls = lam_strides(c.lam);
+    launched("lmo_diff_attn_bwd",
+             MODEL_FN(diff_attn_bwd)(&qs, &ks, &vs, &ls, c.lam32(), c.len(), c.start(), y.data_ptr(), second.data_ptr(),
+                                     static_cast<const float*>(lse.data_ptr()), g.data_ptr(), dq.data_ptr(), ptr(dk), ptr(dval), ptr(dlam), kind,
+                                     static_cast<float*>(scratch.data_ptr()), &sh, static_cast<int>(c.dtype), c.st()));
+    if (nq) out[0] = dq;
+    if (nk) out[1] = dk;
+    if (nv) out[2] = dval;
+    if (nl) out[3] = dlam;
+    return out;
+  }
+};
+
+// diff_attn(q, k, v, lam, lengths, starts, causal, scale, dtype, stream, record): y
+PyObject* host_diff_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 11, "diff_attn(q, k, v, lam, lengths, starts, causal, scale, dtype, stream, record)");
+  const at::Tensor &q = tensor_of(args[0]), &k = tensor_of(args[1]), &v = tensor_of(args[2]), &lam = tensor_of(args[3]);
+  const OptTensor lengths = opt_tensor(args[4]), starts = opt_tensor(args[5]);
+  const bool causal = args[6] == Py_True, record = args[10] == Py_True;
+  const double scale = float_of(args[7]);
+  const int64_t dtype = int_of(args[8]), stream = int_of(args[9]);
+  at::Tensor y;
+  {
+    NoGil free;
+    y = record ? DiffAttnNode::apply(q, k, v, lam, lengths, starts, causal, scale, dtype, stream)
+               : diff_attn_run({q, k, v, lam, or_none(lengths), or_none(starts), causal, scale, dtype, stream}, false)[0];
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_forms(PyObject* const* args, Py_ssize_t n, int first, int count, const char* what) {
   bool ok = n == count;
   for (int i = 0; ok && i < count; ++i) ok = PyCallable_Check(args[i]);
@@ -881,9 +1030,9 @@ PyObject* set_forms(PyObject* const* args, Py_ssize_t n, int first, int count, c
 PyObject* host_torch_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return set_forms(args, n, 0, BLOCK_FORMS, "torch_forms(dropout, join, ffn)");
 }
-// model_forms(layer_norm, distill): the same of the model's operators
+// model_forms(layer_norm, distill, diff_attn): the same of the model's operators
 PyObject* host_model_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return set_forms(args, n, BLOCK_FORMS, FORMS - BLOCK_FORMS, "model_forms(layer_norm, distill)");
+  return set_forms(args, n, BLOCK_FORMS, FORMS - BLOCK_FORMS, "model_forms(layer_norm, distill, diff_attn)");
 }
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
@@ -897,6 +1046,7 @@ PyMethodDef methods[] = {
     {"torch_forms", FAST(&host_torch_forms), METH_FASTCALL, nullptr},
     {"layer_norm", FAST(&host_layer_norm), METH_FASTCALL, nullptr},
     {"distill", FAST(&host_distill), METH_FASTCALL, nullptr},
+    {"diff_attn", FAST(&host_diff_attn), METH_FASTCALL, nullptr},
     {"model_forms", FAST(&host_model_forms), METH_FASTCALL, nullptr},
     {"bind", FAST(&host_bind), METH_FASTCALL, nullptr},
     {"alias", FAST(&host_alias), METH_FASTCALL, nullptr},

@@ -1,0 +1,1143 @@
+// loopback_diff_attn.hip -- MI355X (gfx950, CDNA4) kernels of differential attention, bf16 and fp16, forward and backward:
+//
+//   y = (P1 - lam P2) v,   Pi = softmax(c qi ki^T) over the keys that a query sees
+//
+// Both maps of a head go through one pass over its keys, each with its own running maximum and sum (fp32 scores, statistics
+// and accumulators; the probabilities and score gradients enter the matrix cores in 16 bits). The difference is taken of the
+// two fp32 results. Backward, with D1 = dy . (P1 v), D2 = dy . (P2 v) and dA = dy v^T, which both maps share:
+//
+//   dS1 = P1 (dA - D1),  dS2 = -lam P2 (dA - D2),  dqi = c dSi ki,  dki = c dSi^T qi,  dv = (P1 - lam P2)^T dy,
+//   dlam = -sum over the keys of P2 dA (from the fp32 values: D2 has the rounding of the saved P2 v)
+//
+// Operands go through v_mfma_f32_32x32x16 (dk and dv: 16x16x32): lane l holds row (A) or column (B) l mod 32 at k = 8 (l / 32) .. + 8; of the
+// 32 x 32 result it holds column l mod 32 and, in register r, row 4 (l / 32) + r mod 4 + 8 (r / 4). Scores are formed so that
+// the next product sums over their rows: a result is then the next one's B operand as it lies in the registers, its k order
+// that of Cols32. What a wave keeps in registers are its 32 queries (forward, dq) or keys (dk, dv); the others come through
+// LDS in tiles of 64 rows, two buffers, filled by direct loads. A tile's rows are unpadded and its 16-byte pieces permuted
+// (swizzle), so that neither the reads of rows nor the transposing reads of columns meet in a bank.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "loopback_model.h"
+#include "loopback_read.h"
+#include "device_io.h"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
+
+constexpr int WG = 256, QB = 128, TILE = 64;      // lanes, rows kept per workgroup (32 a wave), rows per LDS tile
+constexpr float LAZY = 8.f;                        // the maximum moves when it grows by 2^8 or more
+constexpr float NONE = -1e30f;                     // the maximum of no scores: finite, so that differences from it are
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T> struct Mat;
+template <> struct Mat<bf16_t> {
+  typedef Bf16Cvt Cvt;
+  static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mat<_Float16> {
+  typedef F16Cvt Cvt;
+  static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+// registers 8 s .. 8 s + 7 of a result as the B operand of the next product's 16-row step s
+template <typename T> __device__ __forceinline__ uint4 operand(const f32x16& x, int s) {
+  typedef typename Mat<T>::Cvt C;
+  return make_uint4(C::pack2(x[8 * s], x[8 * s + 1]), C::pack2(x[8 * s + 2], x[8 * s + 3]), C::pack2(x[8 * s + 4], x[8 * s + 5]),
+                    C::pack2(x[8 * s + 6], x[8 * s + 7]));
+}
+template <typename T> __device__ __forceinline__ uint2 packed4(const f32x4& x) {
+  typedef typename Mat<T>::Cvt C;
+  return make_uint2(C::pack2(x[0], x[1]), C::pack2(x[2], x[3]));
+}
+__device__ __forceinline__ float other_half(float x, bool sum) {   // x joined with the other lane half's
+  const unsigned u = __float_as_uint(x);
+  const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float a = __uint_as_float((unsigned)sw[0]), b = __uint_as_float((unsigned)sw[1]);
+  return sum ? a + b : fmaxf(a, b);
+}
+// keeps the compiler from loading operands ahead across it: they would not fit the registers
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+// the row of a result's register r in lane half h
+__device__ __forceinline__ int row_of(int r, int h) { return 4 * h + (r & 3) + 8 * (r >> 2); }
+
+// ---------------------------------------------------------------------------------------------------------------
+// rows in LDS, of W elements (64, 128 or 256) in pieces of 16 bytes, piece p of row r in place p ^ swizzle(r). What reads them
+// together then meets in no bank (64 of 4 bytes): 16 rows at one piece; four rows, aligned, at four pieces; eight at two.
+// Each lane's offsets are formed once; what is added to them in the loops is known at compile time.
+// ---------------------------------------------------------------------------------------------------------------
+template <int W> __device__ __forceinline__ int swizzle(int r) {
+  return (W == 64 ? (r >> 1 & 1) << 2 : (r & 1) << 3 | (r >> 1 & 1) << 2) | (r >> 2 & 1) << 1 | (r >> 3 & 1);
+}
+typedef __attribute__((address_space(3))) s16x4* lds4;
+__device__ __forceinline__ uint4 four_and_four(const void* p, const void* q) {   // a column's elements of two times four rows
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(const_cast<void*>(p)));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(const_cast<void*>(q)));
+  const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
+  return make_uint4(ua.x, ua.y, ub.x, ub.y);
+}
+// operands of v_mfma_f32_32x32x16
+template <typename T, int W> struct Rows32 {   // A: rows r0 + l mod 32, columns 16 ks + 8 (l / 32) .. + 8
+  int o[8];
+  __device__ __forceinline__ Rows32() {
+    const int lane = (int)threadIdx.x & 63, r = lane & 31;
+#pragma unroll
+    for (int v = 0; v < 8; ++v) o[v] = r * W + 8 * ((2 * v) ^ ((lane >> 5) ^ swizzle<W>(r)));
+  }
+  __device__ __forceinline__ uint4 at(const T* tile, int r0, int ks) const {   // r0 a multiple of 32
+    return *reinterpret_cast<const uint4*>(tile + o[W == 64 ? ks & 3 : ks & 7] + r0 * W + 128 * (ks >> 3));
+  }
+};
+template <typename T, int W> struct Cols32 {   // A: columns c0 + l mod 32, rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}, h = l / 32
+  int o[4], p[4];
+  __device__ __forceinline__ Cols32() {
+    const int lane = (int)threadIdx.x & 63, j = lane & 15, r = 4 * (lane >> 5) + (j >> 2);
+    const int piece = (lane >> 4 & 1) * 2 + ((j & 3) >> 1), half = 4 * (j & 1);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      o[v] = r * W + 8 * ((4 * v) ^ (piece ^ swizzle<W>(r))) + half;
+      p[v] = (r + 8) * W + 8 * ((4 * v) ^ (piece ^ swizzle<W>(r + 8))) + half;
+    }
+  }
+  __device__ __forceinline__ uint4 at(const T* tile, int r0, int c0) const {   // r0 a multiple of 16, c0 of 32
+    const int v = (c0 >> 5) & (W == 64 ? 1 : 3), more = r0 * W + 128 * (c0 >> 7);
+    return four_and_four(tile + o[v] + more, tile + p[v] + more);
+  }
+};
+// operands of v_mfma_f32_16x16x32
+template <typename T, int W> struct Rows16 {   // A: rows r0 + l mod 16, columns 32 ks + 8 (l / 16) .. + 8
+  int o[4];
+  __device__ __forceinline__ Rows16() {
+    const int lane = (int)threadIdx.x & 63, r = lane & 15;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) o[v] = r * W + 8 * ((4 * v) ^ ((lane >> 4) ^ swizzle<W>(r)));
+  }
+  __device__ __forceinline__ uint4 at(const T* tile, int r0, int ks) const {   // r0 a multiple of 16
+    return *reinterpret_cast<const uint4*>(tile + o[W == 64 ? ks & 1 : ks & 3] + r0 * W + 128 * (ks >> 2));
+  }
+};
+template <typename T, int W> struct Cols16 {   // A: columns c0 + l mod 16, rows r0 + {4 g + 0..3, 16 + 4 g + 0..3}, g = l / 16
+  int o[8];
+  __device__ __forceinline__ Cols16() {
+    const int lane = (int)threadIdx.x & 63, j = lane & 15, r = 4 * (lane >> 4) + (j >> 2);
+#pragma unroll
+    for (int v = 0; v < 8; ++v) o[v] = r * W + 8 * ((2 * v) ^ (((j & 3) >> 1) ^ swizzle<W>(r))) + 4 * (j & 1);
+  }
+  __device__ __forceinline__ uint4 at(const T* tile, int r0, int c0) const {   // r0 a multiple of 32, c0 of 16
+    const T* p = tile + o[(c0 >> 4) & (W == 64 ? 3 : 7)] + r0 * W + 128 * (c0 >> 7);
+    return four_and_four(p, p + 16 * W);
+  }
+};
+
+// Fills N rows of LDS from memory by LANES lanes (whole waves). MAPS rows of memory of W / MAPS elements (`width` of them
+// exist, the columns past them repeat the first piece: what they meet is zero) lie side by side in a row of LDS. Rows past
+// row `last` repeat it.
+template <typename T, int W, int MAPS, int N, int LANES> struct Fill {
+  static constexpr int P = W / 8, PASSES = N * P / LANES, PM = P / MAPS, ROWS = LANES / P, VAR = ROWS >= 16 ? 1 : 16 / ROWS;
+  static_assert(N * P % LANES == 0 && N % 16 == 0, "whole passes, whole turns of the swizzle");
+  const T* base;      // row 0
+  int64_t stride;     // elements between rows
+  uint32_t off[VAR];  // bytes, of a pass's rows from its first
+  // the piece that is stored in this lane's place, in elements from the row's start
+  static __device__ __forceinline__ uint32_t col(int lane, int v, int64_t map_stride, int width) {
+    const int p = (lane % P) ^ swizzle<W>(lane / P + ROWS * v), m = p / PM, c = 8 * (p % PM);
+    return (uint32_t)(m * (int)map_stride) + (uint32_t)(c < width ? c : 0);
+  }
+  __device__ __forceinline__ Fill(const T* base_, int64_t stride_, int64_t map_stride, int width) : base(base_), stride(stride_) {
+    const int lane = (int)threadIdx.x % LANES;
+#pragma unroll
+    for (int v = 0; v < VAR; ++v) off[v] = 2u * ((uint32_t)(lane / P) * (uint32_t)stride + col(lane, v, map_stride, width));
+  }
+  __device__ __forceinline__ void fetch(int row0, int last, T* lds) const {   // asynchronous: done when vmcnt says so
+    const int wave = LANES == 64 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x % LANES) >> 6);
+    const bool whole = row0 + N - 1 <= last;
+    int r = (int)(threadIdx.x % LANES) / P;
+    if (!whole) asm volatile("" : "+v"(r));   // formed here, where it is rarely needed
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const char* b = reinterpret_cast<const char*>(base + (int64_t)(row0 + ROWS * i) * stride);
+      lds_void* to = (lds_void*)(lds + 8 * (i * LANES + wave * 64));
+      if (whole) {
+        __builtin_amdgcn_global_load_lds((global_void*)(b + off[i % VAR]), to, 16, 0, 0);
+      } else {
+        const int64_t back = max(row0 + ROWS * i + r - last, 0) * (2 * stride);
+        __builtin_amdgcn_global_load_lds((global_void*)(b + off[i % VAR] - back), to, 16, 0, 0);
+      }
+    }
+  }
+};
+__device__ __forceinline__ void filled() {   // this wave's loads are in LDS; then every wave's
+  __builtin_amdgcn_s_waitcnt(0x0f70);        // vmcnt(0)
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+struct Strided { const void* p; int64_t b, t, h; };   // elements between batches, tokens and heads; columns lie side by side
+struct Diff {
+  Strided q, k, v, lam;
+  const int *lengths, *starts;   // NULL: tk, and tk - tq
+  void *out, *second;            // y and P2 v [b, tq, h, dv]; second NULL: no backward follows
+  float* lse;                    // [2][b h][tq]: base-2 logarithms of the sums of exponentials
+  int b, tq, tk, h, hk, dh, dv;
+  int causal, lam32;             // lam32: lam is fp32, else the rows' type
+  float c, scale;                // scale log2(e), and scale
+  // backward
+  const void* dy;
+  void *dq, *dk, *dval;
+  float *delta, *dlam;           // [2][b h][tq], and dlam's parts
+  int dlam_rows;                 // dlam per query, else per workgroup
+  // a split of the keys
+  int splits, chunk;
+  float* part;
+};
+
+template <typename T> __device__ __forceinline__ float lam_at(const Diff& a, int b, int t, int h) {
+  const int64_t o = b * a.lam.b + t * a.lam.t + h * a.lam.h;
+  return a.lam32 ? static_cast<const float*>(a.lam.p)[o] : ld1(static_cast<const T*>(a.lam.p) + o);
+}
+__device__ __forceinline__ int length_of(const Diff& a, int b) { return a.lengths ? min(max(a.lengths[b], 0), a.tk) : a.tk; }
+__device__ __forceinline__ int start_of(const Diff& a, int b) {   // far positions all mean every key or none
+  const int far = (1 << 30) - 1;
+  return a.starts ? min(max(a.starts[b], -far), far) : a.tk - a.tq;
+}
+// the keys that query i sees: those before this one
+__device__ __forceinline__ int seen_by(const Diff& a, int i, int start, int len) {
+  return a.causal ? min(max(start + i + 1, 0), len) : len;   // start and i below 2^30
+}
+
+// Which block of which head a workgroup takes: `items` (batches times heads of keys) go to the eight XCDs in turn where they
+// divide by eight, so that a head's keys are read from one L2; the blocks with the most work first.
+struct Work { int item, g, block; };
+__device__ __forceinline__ bool work_of(int items, int groups, int blocks, Work& w) {
+  const int id = (int)blockIdx.x;
+  int unit;
+  if (items % 8 == 0) {
+    const int i = id >> 3, per = items >> 3;
+    w.item = (id & 7) + 8 * (i % per);
+    unit = i / per;
+  } else {
+    w.item = id % items;
+    unit = id / items;
+  }
+  w.g = unit % groups;
+  w.block = unit / groups;
+  return w.block < blocks;
+}
+
+__device__ __forceinline__ uint4 only(bool ok, const uint4& a) {   // a, or zeros
+  return make_uint4(ok ? a.x : 0u, ok ? a.y : 0u, ok ? a.z : 0u, ok ? a.w : 0u);
+}
+// a wave's 32 rows as B operands: row r, columns 16 ks + 8 (l / 32) .. + 8, zeros past `width`
+template <typename T, int W> struct Kept {
+  uint4 f[W / 16];
+  __device__ __forceinline__ void load(const T* row, int width) {
+    const int h = ((int)threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int ks = 0; ks < W / 16; ++ks) {
+      const int c = 16 * ks + 8 * h;
+      f[ks] = only(c < width, *reinterpret_cast<const uint4*>(row + min(c, width - 8)));
+    }
+  }
+};
+
+// One map's running softmax of a query (a lane pair's column)
+struct Soft { float m = NONE, l = 0.f; };
+// a tile's scores of one map, as probabilities relative to the running maximum, packed: p[4 i' ...]; o, and l, are rescaled
+template <typename T, int NB, int DB>
+__device__ __forceinline__ void soft_step(f32x16 (&s)[NB], Soft& st, f32x16 (&o)[DB], uint4 (&p)[2 * NB], float c) {
+  float mx = s[0][0];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
+  mx = other_half(mx, false) * c;
+  if (__any(mx > st.m + LAZY)) {
+    const float mn = fmaxf(st.m, mx), a = st.m == mn ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
+    st.m = mn;
+    st.l *= a;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= a;
+  }
+  float ls[4] = {0.f, 0.f, 0.f, 0.f};   // four sums: no chain of dependent adds
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], c, -st.m));
+      ls[r & 3] += s[i][r];
+    }
+    p[2 * i] = operand<T>(s[i], 0);
+    p[2 * i + 1] = operand<T>(s[i], 1);
+  }
+  st.l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+}
+
+template <int DH, int DV> constexpr int waves_fwd() { return DH + DV <= 192 ? 2 : 1; }
+
+// ---------------------------------------------------------------------------------------------------------------
+// forward: 128 queries of a head per workgroup
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int DH, int DV>
+__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_fwd(const Diff a) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int KT = TILE * 2 * DH, VT = TILE * DV, DB = DV / 32;
+  T* s_k = reinterpret_cast<T*>(lds);
+  T* s_v = s_k + 2 * KT;
+  const int lane = (int)threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int groups = a.h / a.hk, blocks = (a.tq + QB - 1) / QB;
+  Work wk;
+  if (!work_of(a.b * a.hk, groups, blocks, wk)) return;
+  const int q0 = (blocks - 1 - wk.block) * QB, b = wk.item / a.hk, hk = wk.item - b * a.hk, head = hk * groups + wk.g;
+  const int len = length_of(a, b), start = start_of(a, b);
+  const int w0 = q0 + 32 * wave, query = w0 + (lane & 31), qrow = min(query, a.tq - 1);
+  const T* qp = static_cast<const T*>(a.q.p) + b * a.q.b + qrow * a.q.t + 2 * head * a.q.h;
+  Kept<T, DH> q[2];
+  q[0].load(qp, a.dh);
+  q[1].load(qp + a.q.h, a.dh);
+  const int seen = seen_by(a, qrow, start, len);
+  const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len);             // of the workgroup's queries
+  const int wmost = w0 < a.tq ? seen_by(a, min(w0 + 32, a.tq) - 1, start, len) : 0, wleast = seen_by(a, min(w0, a.tq - 1), start, len);
+  const Rows32<T, 2 * DH> krows;
+  const Cols32<T, DV> vcols;
+  f32x16 o1[DB], o2[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o1[d] = o2[d] = zero16();
+  Soft sm1, sm2;
+  const int ntiles = (most + TILE - 1) / TILE;
+  const Fill<T, 2 * DH, 2, TILE, WG> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
+  const Fill<T, DV, 1, TILE, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
+  if (ntiles > 0) {
+    kf.fetch(0, len - 1, s_k);
+    vf.fetch(0, len - 1, s_v);
+    filled();
+  }
+  auto tile = [&](int j, auto buffer) {
+    constexpr int cur = decltype(buffer)::value;   // known: the buffers' offsets go into the reads' own
+    const int k0 = j * TILE;
+    if (j + 1 < ntiles) {   // the other buffer's readers are past the barrier below
+      kf.fetch(k0 + TILE, len - 1, s_k + (cur ^ 1) * KT);
+      vf.fetch(k0 + TILE, len - 1, s_v + (cur ^ 1) * VT);
+    }
+    if (k0 < wmost) {
+      const T* kt = s_k + cur * KT;
+      const T* vt = s_v + cur * VT;
+      uint4 p1[4], p2[4];
+      auto scores = [&](int map, f32x16 (&s)[2]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[i] = zero16();
+#pragma unroll
+          for (int ks = 0; ks < DH / 16; ++ks) s[i] = Mat<T>::mfma(krows.at(kt, 32 * i, map * (DH / 16) + ks), q[map].f[ks], s[i]);
+        }
+        if (k0 + TILE > wleast) {   // wave-uniform: keys that some query of the wave does not see
+          const int left = seen - k0 - 4 * half;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * i + row_of(r, 0) >= left) s[i][r] = -INFINITY;
+        }
+      };
+      f32x16 s[2];
+      scores(0, s);
+      in_order();
+      soft_step<T>(s, sm1, o1, p1, a.c);
+      in_order();
+      scores(1, s);
+      in_order();
+      soft_step<T>(s, sm2, o2, p2, a.c);
+      in_order();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          if (d % 2 == 0) in_order();
+          const uint4 v = vcols.at(vt, 16 * i, 32 * d);
+          o1[d] = Mat<T>::mfma(v, p1[i], o1[d]);
+          o2[d] = Mat<T>::mfma(v, p2[i], o2[d]);
+        }
+    }
+    if (j + 1 < ntiles) filled();
+  };
+  for (int j = 0; j < ntiles; j += 2) {
+    tile(j, std::integral_constant<int, 0>());
+    if (j + 1 < ntiles) tile(j + 1, std::integral_constant<int, 1>());
+  }
+  const float l1 = other_half(sm1.l, true), l2 = other_half(sm2.l, true);
+  if (query >= a.tq) return;
+  // a query that sees no key: zeros, and an infinite logarithm, which makes every probability 0
+  const float lam = lam_at<T>(a, b, query, head), i1 = l1 > 0.f || l1 != l1 ? 1.f / l1 : 0.f, i2 = l2 > 0.f || l2 != l2 ? 1.f / l2 : 0.f;
+  const int64_t orow = (((int64_t)b * a.tq + query) * a.h + head) * a.dv;
+  T* op = static_cast<T*>(a.out) + orow;
+  T* sp = static_cast<T*>(a.second) + orow;
+  typedef typename Mat<T>::Cvt C;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * d + 8 * g + 4 * half;
+      if (col < a.dv) {
+        float y[4], z[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          z[k] = o2[d][4 * g + k] * i2;
+          y[k] = o1[d][4 * g + k] * i1 - lam * z[k];
+        }
+        *reinterpret_cast<uint2*>(op + col) = make_uint2(C::pack2(y[0], y[1]), C::pack2(y[2], y[3]));
+        if (a.second) *reinterpret_cast<uint2*>(sp + col) = make_uint2(C::pack2(z[0], z[1]), C::pack2(z[2], z[3]));
+      }
+    }
+  if (a.lse && half == 0) {
+    const int64_t n = ((int64_t)b * a.h + head) * a.tq + query;
+    a.lse[n] = i1 != 0.f ? sm1.m + __builtin_amdgcn_logf(l1) : INFINITY;
+    a.lse[n + (int64_t)a.b * a.h * a.tq] = i2 != 0.f ? sm2.m + __builtin_amdgcn_logf(l2) : INFINITY;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// few queries: the (query, head of the group) pairs of a head of keys are the 32 rows of one block (tq times the group at
+// most 32). A workgroup takes a chunk of its keys; its waves take tiles of 32 of them in turn, each through LDS of its own,
+// two tiles in flight; their results meet in LDS, and those of the chunks in k_diff_join.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int FEW = 32;
+template <int DH, int DV> constexpr int few_waves() { return 2 * DH + DV <= 256 ? 4 : 2; }
+template <int DH, int DV> constexpr int few_lds() { return few_waves<DH, DV>() * 2 * FEW * (2 * DH + DV) * 2; }
+template <int DV> constexpr int few_row() { return 2 * DV + 4; }   // floats of a row's partial result: o1, o2, m1, l1, m2, l2
+
+// a row's partial results as one: their common maximum, the sums and the values. at(i): the i-th partial row
+template <int DV, typename At>
+__device__ __forceinline__ void join_row(At at, int n, int col, float& y1, float& y2) {
+  float m1 = NONE, m2 = NONE;
+  for (int i = 0; i < n; ++i) {
+    const float* p = at(i) + 2 * DV;
+    m1 = fmaxf(m1, p[0]);
+    m2 = fmaxf(m2, p[2]);
+  }
+  float l1 = 0.f, l2 = 0.f;
+  y1 = y2 = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const float* p = at(i);
+    const float f1 = __builtin_amdgcn_exp2f(p[2 * DV] - m1), f2 = __builtin_amdgcn_exp2f(p[2 * DV + 2] - m2);
+    l1 = __builtin_fmaf(p[2 * DV + 1], f1, l1);
+    l2 = __builtin_fmaf(p[2 * DV + 3], f2, l2);
+    y1 = __builtin_fmaf(p[col], f1, y1);
+    y2 = __builtin_fmaf(p[DV + col], f2, y2);
+  }
+  y1 = l1 > 0.f || l1 != l1 ? y1 / l1 : 0.f;
+  y2 = l2 > 0.f || l2 != l2 ? y2 / l2 : 0.f;
+}
+
+template <typename T, int DH, int DV>
+__global__ __launch_bounds__((64 * few_waves<DH, DV>())) __attribute__((amdgpu_waves_per_eu(1))) void k_diff_few(const Diff a) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int WAVES = few_waves<DH, DV>(), KT = FEW * 2 * DH, VT = FEW * DV, DB = DV / 32, ROW = few_row<DV>();
+  const int lane = (int)threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int groups = a.h / a.hk, rows = a.tq * groups;
+  const int item = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - item * a.splits, b = item / a.hk, hk = item - b * a.hk;
+  const int len = length_of(a, b), start = start_of(a, b);
+  T* s_k = reinterpret_cast<T*>(lds) + wave * 2 * (KT + VT);
+  T* s_v = s_k + 2 * KT;
+  const int row = min(lane & 31, rows - 1), query = row / groups, head = hk * groups + row - query * groups;
+  const T* qp = static_cast<const T*>(a.q.p) + b * a.q.b + query * a.q.t + 2 * head * a.q.h;
+  Kept<T, DH> q[2];
+  q[0].load(qp, a.dh);
+  q[1].load(qp + a.q.h, a.dh);
+  const int seen = seen_by(a, query, start, len);
+  const int c0 = split * a.chunk, c1 = min(c0 + a.chunk, seen_by(a, a.tq - 1, start, len)), least = seen_by(a, 0, start, len);
+  const Rows32<T, 2 * DH> krows;
+  const Cols32<T, DV> vcols;
+  f32x16 o1[DB], o2[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o1[d] = o2[d] = zero16();
+  Soft sm1, sm2;
+  const Fill<T, 2 * DH, 2, FEW, 64> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
+  const Fill<T, DV, 1, FEW, 64> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
+  constexpr int LOADS = decltype(kf)::PASSES + decltype(vf)::PASSES;   // of a tile
+  static_assert(LOADS < 64, "what vmcnt counts");
+  const int first = c0 + FEW * wave, step = FEW * WAVES;
+  if (first < c1) {
+    kf.fetch(first, len - 1, s_k);
+    vf.fetch(first, len - 1, s_v);
+  }
+  int cur = 0;
+  for (int k0 = first; k0 < c1; k0 += step, cur ^= 1) {
+    if (k0 + step < c1) {
+      kf.fetch(k0 + step, len - 1, s_k + (cur ^ 1) * KT);
+      vf.fetch(k0 + step, len - 1, s_v + (cur ^ 1) * VT);
+      __builtin_amdgcn_s_waitcnt(0x0f70 | (LOADS & 15) | (LOADS >> 4 << 14));   // vmcnt: all but the next tile's loads
+    } else {
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+    }
+    wave_lds_sync();
+    const T* kt = s_k + cur * KT;
+    const T* vt = s_v + cur * VT;
+    uint4 p1[2], p2[2];
+    auto scores = [&](int map, f32x16 (&s)[1]) {
+      s[0] = zero16();
+#pragma unroll
+      for (int ks = 0; ks < DH / 16; ++ks) s[0] = Mat<T>::mfma(krows.at(kt, 0, map * (DH / 16) + ks), q[map].f[ks], s[0]);
+      if (k0 + FEW > least) {
+        const int left = seen - k0 - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (row_of(r, 0) >= left) s[0][r] = -INFINITY;
+      }
+    };
+    f32x16 s[1];
+    scores(0, s);
+    soft_step<T>(s, sm1, o1, p1, a.c);
+    scores(1, s);
+    soft_step<T>(s, sm2, o2, p2, a.c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const uint4 v = vcols.at(vt, 16 * i, 32 * d);
+        o1[d] = Mat<T>::mfma(v, p1[i], o1[d]);
+        o2[d] = Mat<T>::mfma(v, p2[i], o2[d]);
+      }
+    wave_lds_sync();   // the tile's reads are done before the one after the next is loaded over it
+  }
+  const float l1 = other_half(sm1.l, true), l2 = other_half(sm2.l, true);
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(lds);   // [wave][32 rows][ROW]
+  static_assert(few_waves<DH, DV>() * FEW * few_row<DV>() * 4 <= 160 * 1024 && few_lds<DH, DV>() <= 160 * 1024,
+                "the tiles, and the waves' results, in LDS");
+  if ((lane & 31) < rows) {
+    float* p = part + (wave * FEW + (lane & 31)) * ROW;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = 32 * d + 8 * g + 4 * half;
+        *reinterpret_cast<float4*>(p + col) = make_float4(o1[d][4 * g], o1[d][4 * g + 1], o1[d][4 * g + 2], o1[d][4 * g + 3]);
+        *reinterpret_cast<float4*>(p + DV + col) = make_float4(o2[d][4 * g], o2[d][4 * g + 1], o2[d][4 * g + 2], o2[d][4 * g + 3]);
+      }
+    if (half == 0) *reinterpret_cast<float4*>(p + 2 * DV) = make_float4(sm1.m, l1, sm2.m, l2);
+  }
+  __syncthreads();
+  for (int i = (int)threadIdx.x; i < rows * DV; i += 64 * WAVES) {
+    const int r = i / DV, col = i - r * DV, qi = r / groups, hd = hk * groups + r - qi * groups;
+    if (a.splits == 1) {
+      float y1, y2;
+      join_row<DV>([&](int w) { return part + (w * FEW + r) * ROW; }, WAVES, col, y1, y2);
+      if (col < a.dv)
+        st1(static_cast<T*>(a.out) + (((int64_t)b * a.tq + qi) * a.h + hd) * a.dv + col, y1 - lam_at<T>(a, b, qi, hd) * y2);
+    } else {   // the waves' sums relative to their common maximum
+      float m1 = NONE, m2 = NONE, s1 = 0.f, s2 = 0.f, y1 = 0.f, y2 = 0.f;
+      for (int w = 0; w < WAVES; ++w) {
+        const float* p = part + (w * FEW + r) * ROW + 2 * DV;
+        m1 = fmaxf(m1, p[0]);
+        m2 = fmaxf(m2, p[2]);
+      }
+      for (int w = 0; w < WAVES; ++w) {
+        const float* p = part + (w * FEW + r) * ROW;
+        const float f1 = __builtin_amdgcn_exp2f(p[2 * DV] - m1), f2 = __builtin_amdgcn_exp2f(p[2 * DV + 2] - m2);
+        s1 = __builtin_fmaf(p[2 * DV + 1], f1, s1);
+        s2 = __builtin_fmaf(p[2 * DV + 3], f2, s2);
+        y1 = __builtin_fmaf(p[col], f1, y1);
+        y2 = __builtin_fmaf(p[DV + col], f2, y2);
+      }
+      float* out = a.part + ((int64_t)((item * rows) + r) * a.splits + split) * ROW;
+      out[col] = y1;
+      out[DV + col] = y2;
+      if (col == 0) *reinterpret_cast<float4*>(out + 2 * DV) = make_float4(m1, s1, m2, s2);
+    }
+  }
+}
+
+// the chunks' partial rows: one workgroup of DV lanes per row
+template <typename T, int DV> __global__ __launch_bounds__(DV) void k_diff_join(const Diff a) {
+  constexpr int ROW = few_row<DV>();
+  const int groups = a.h / a.hk, rows = a.tq * groups, item = (int)blockIdx.x / rows, r = (int)blockIdx.x - item * rows;
+  const int b = item / a.hk, hk = item - b * a.hk, query = r / groups, head = hk * groups + r - query * groups, col = (int)threadIdx.x;
+  const float* p = a.part + (int64_t)blockIdx.x * a.splits * ROW;
+  float y1, y2;
+  join_row<DV>([&](int i) { return p + (int64_t)i * ROW; }, a.splits, col, y1, y2);
+  if (col < a.dv)
+    st1(static_cast<T*>(a.out) + (((int64_t)b * a.tq + query) * a.h + head) * a.dv + col, y1 - lam_at<T>(a, b, query, head) * y2);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// backward: dq, the deltas and dlam's parts. 128 queries of a head per workgroup, as the forward
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int DH, int DV>
+__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_bwd_q(const Diff a) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ float s_dlam[4];
+  constexpr int KT = TILE * 2 * DH, VT = TILE * DV, QB_ = DH / 32;
+  T* s_k = reinterpret_cast<T*>(lds);
+  T* s_v = s_k + 2 * KT;
+  const int lane = (int)threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int groups = a.h / a.hk, blocks = (a.tq + QB - 1) / QB;
+  Work wk;
+  if (!work_of(a.b * a.hk, groups, blocks, wk)) return;
+  const int qblock = blocks - 1 - wk.block, q0 = qblock * QB, b = wk.item / a.hk, hk = wk.item - b * a.hk, head = hk * groups + wk.g;
+  const int len = length_of(a, b), start = start_of(a, b);
+  const int w0 = q0 + 32 * wave, query = w0 + (lane & 31), qrow = min(query, a.tq - 1);
+  const T* qp = static_cast<const T*>(a.q.p) + b * a.q.b + qrow * a.q.t + 2 * head * a.q.h;
+  const int64_t orow = (((int64_t)b * a.tq + qrow) * a.h + head) * a.dv;
+  Kept<T, DH> q[2];
+  Kept<T, DV> g;
+  q[0].load(qp, a.dh);
+  q[1].load(qp + a.q.h, a.dh);
+  g.load(static_cast<const T*>(a.dy) + orow, a.dv);
+  const float lam = lam_at<T>(a, b, qrow, head);
+  float d1 = 0.f, d2 = 0.f;   // dy . y, dy . (P2 v)
+#pragma unroll
+  for (int ks = 0; ks < DV / 16; ++ks) {
+    const int col = 16 * ks + 8 * half;
+    if (col < a.dv) {
+      float u[8], y[8], z[8];
+      IO<T>::unpack(typename IO<T>::Raw{g.f[ks]}, u);
+      IO<T>::load(static_cast<const T*>(a.out) + orow + col, y);
+      IO<T>::load(static_cast<const T*>(a.second) + orow + col, z);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        d1 = __builtin_fmaf(u[k], y[k], d1);
+        d2 = __builtin_fmaf(u[k], z[k], d2);
+      }
+    }
+  }
+  d2 = other_half(d2, true);
+  d1 = __builtin_fmaf(lam, d2, other_half(d1, true));
+  const int64_t n = ((int64_t)b * a.h + head) * a.tq + qrow, all = (int64_t)a.b * a.h * a.tq;
+  const float ls1 = a.lse[n], ls2 = a.lse[n + all];
+  if (query < a.tq && half == 0) {
+    a.delta[n] = d1;
+    a.delta[n + all] = d2;
+  }
+  const int seen = seen_by(a, qrow, start, len);
+  const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len);
+  const int wmost = w0 < a.tq ? seen_by(a, min(w0 + 32, a.tq) - 1, start, len) : 0, wleast = seen_by(a, min(w0, a.tq - 1), start, len);
+  const Rows32<T, 2 * DH> krows;
+  const Rows32<T, DV> vrows;
+  const Cols32<T, 2 * DH> kcols;
+  f32x16 dq[2][QB_];
+#pragma unroll
+  for (int d = 0; d < QB_; ++d) dq[0][d] = dq[1][d] = zero16();
+  float dlam = 0.f;
+  const int ntiles = (most + TILE - 1) / TILE;
+  const Fill<T, 2 * DH, 2, TILE, WG> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
+  const Fill<T, DV, 1, TILE, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
+  if (ntiles > 0) {
+    kf.fetch(0, len - 1, s_k);
+    vf.fetch(0, len - 1, s_v);
+    filled();
+  }
+  auto tile = [&](int j, auto buffer) {
+    constexpr int cur = decltype(buffer)::value;   // known: the buffers' offsets go into the reads' own
+    const int k0 = j * TILE;
+    if (j + 1 < ntiles) {
+      kf.fetch(k0 + TILE, len - 1, s_k + (cur ^ 1) * KT);
+      vf.fetch(k0 + TILE, len - 1, s_v + (cur ^ 1) * VT);
+    }
+    if (k0 < wmost) {
+      const T* kt = s_k + cur * KT;
+      const T* vt = s_v + cur * VT;
+      const bool edge = k0 + TILE > wleast;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x16 da = zero16();
+#pragma unroll
+        for (int ks = 0; ks < DV / 16; ++ks) da = Mat<T>::mfma(vrows.at(vt, 32 * i, ks), g.f[ks], da);
+        in_order();
+#pragma unroll
+        for (int map = 0; map < 2; ++map) {
+          f32x16 s = zero16();
+#pragma unroll
+          for (int ks = 0; ks < DH / 16; ++ks) s = Mat<T>::mfma(krows.at(kt, 32 * i, map * (DH / 16) + ks), q[map].f[ks], s);
+          if (edge) {
+            const int left = seen - k0 - 4 * half;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * i + row_of(r, 0) >= left) s[r] = -INFINITY;
+          }
+          const float ls = map ? ls2 : ls1, d = map ? d2 : d1;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -ls));
+            if (map) dlam = __builtin_fmaf(p, da[r], dlam);
+            s[r] = p * (da[r] - d);
+          }
+          in_order();
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const uint4 ds = operand<T>(s, st);
+#pragma unroll
+            for (int e = 0; e < QB_; ++e)
+              dq[map][e] = Mat<T>::mfma(kcols.at(kt, 32 * i + 16 * st, map * DH + 32 * e), ds, dq[map][e]);
+          }
+          in_order();
+        }
+      }
+    }
+    if (j + 1 < ntiles) filled();
+  };
+  for (int j = 0; j < ntiles; j += 2) {
+    tile(j, std::integral_constant<int, 0>());
+    if (j + 1 < ntiles) tile(j + 1, std::integral_constant<int, 1>());
+  }
+  typedef typename Mat<T>::Cvt C;
+  if (query < a.tq) {
+    T* row = static_cast<T*>(a.dq) + (((int64_t)b * a.tq + query) * 2 * a.h + 2 * head) * a.dh;
+#pragma unroll
+    for (int map = 0; map < 2; ++map) {
+      const float f = map ? -lam * a.scale : a.scale;
+#pragma unroll
+      for (int e = 0; e < QB_; ++e)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int col = 32 * e + 8 * k + 4 * half;
+          const f32x16& v = dq[map][e];
+          if (col < a.dh)
+            *reinterpret_cast<uint2*>(row + map * a.dh + col) =
+                make_uint2(C::pack2(v[4 * k] * f, v[4 * k + 1] * f), C::pack2(v[4 * k + 2] * f, v[4 * k + 3] * f));
+        }
+    }
+  }
+  if (!a.dlam) return;
+  dlam = query < a.tq ? -other_half(dlam, true) : 0.f;
+  if (a.dlam_rows) {
+    if (query < a.tq && half == 0) a.dlam[((int64_t)b * a.tq + query) * a.h + head] = dlam;
+    return;
+  }
+  dlam = lanes_reduce(dlam, 32, AddOp());
+  if (lane == 0) s_dlam[wave] = dlam;
+  __syncthreads();
+  if (threadIdx.x == 0) a.dlam[(int64_t)head * (a.b * blocks) + b * blocks + qblock] = (s_dlam[0] + s_dlam[1]) + (s_dlam[2] + s_dlam[3]);
+}
+
+// dlam: `n` parts of each of `outs` results in a row, summed in order by 256 lanes, then a tree; or (n 1) only converted
+template <typename T> __global__ __launch_bounds__(WG) void k_diff_dlam(const float* __restrict__ part, int64_t n, int64_t outs, T* __restrict__ out) {
+  __shared__ float s[WG];
+  const int tid = (int)threadIdx.x;
+  if (n == 1) {
+    for (int64_t i = (int64_t)blockIdx.x * WG + tid; i < outs; i += (int64_t)gridDim.x * WG) st1(out + i, part[i]);
+    return;
+  }
+  float acc = 0.f;
+  for (int64_t i = tid; i < n; i += WG) acc += part[blockIdx.x * n + i];
+  s[tid] = acc;
+  __syncthreads();
+  for (int w = WG / 2; w > 0; w >>= 1) {
+    if (tid < w) s[tid] += s[tid + w];
+    __syncthreads();
+  }
+  if (tid == 0) st1(out + blockIdx.x, s[0]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// backward: dk and dv. 128 keys of a head of keys per workgroup, 32 a wave, over the queries of its group's heads one after
+// another. Here the scores' rows are queries, whose four or five numbers come from LDS for every row a lane has: by
+// v_mfma_f32_16x16x32 a lane has 4 of 16 rows, not 16 of 32, and half as much is read for them, and held.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int W> struct Kept16 {   // a wave's 32 rows as B operands: row 16 n + l mod 16, columns 32 ks + 8 (l / 16) .. + 8
+  uint4 f[2][W / 32];
+  __device__ __forceinline__ void load(int n, const T* row, int width, bool there) {   // zeros past `width`, and for no row
+    const int g = ((int)threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int ks = 0; ks < W / 32; ++ks) {
+      const int c = 32 * ks + 8 * g;
+      f[n][ks] = only(c < width && there, *reinterpret_cast<const uint4*>(row + min(c, width - 8)));
+    }
+  }
+};
+
+template <typename T, int DH, int DV, bool TOKEN>   // TOKEN: lam differs between queries
+__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_bwd_kv(const Diff a) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int QT = TILE * 2 * DH, GT = TILE * DV, KB = DH / 16, VB = DV / 16, NUMBERS = TOKEN ? 5 : 4;
+  T* s_q = reinterpret_cast<T*>(lds);
+  T* s_g = s_q + 2 * QT;
+  float* s_row = reinterpret_cast<float*>(s_g + 2 * GT);   // [2 buffers][lse1, lse2, D1, D2, lam][64]
+  const int tid = (int)threadIdx.x, lane = tid & 63, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = a.h / a.hk, blocks = (a.tk + QB - 1) / QB;
+  Work wk;
+  if (!work_of(a.b * a.hk, 1, blocks, wk)) return;
+  const int kb = wk.block * QB, b = wk.item / a.hk, hk = wk.item - b * a.hk;
+  const int len = length_of(a, b), start = start_of(a, b);
+  const int w0 = kb + 32 * wave;
+  Kept16<T, DH> k[2];
+  Kept16<T, DV> v;
+  int from[2];   // the first query that sees the lane's keys
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int key = w0 + 16 * n + (lane & 15), krow = min(key, a.tk - 1);
+    const bool there = key < len;   // what is past the length is not read into anything: a NaN would reach a product of zeros
+    const T* kp = static_cast<const T*>(a.k.p) + b * a.k.b + krow * a.k.t + 2 * hk * a.k.h;
+    k[0].load(n, kp, a.dh, there);
+    k[1].load(n, kp + a.k.h, a.dh, there);
+    v.load(n, static_cast<const T*>(a.v.p) + b * a.v.b + krow * a.v.t + hk * a.v.h, a.dv, there);
+    from[n] = !there ? 0x7fffffff : a.causal ? max(key - start, 0) : 0;
+  }
+  const Rows16<T, 2 * DH> qrows;
+  const Rows16<T, DV> grows;
+  const Cols16<T, 2 * DH> qcols;
+  const Cols16<T, DV> gcols;
+  f32x4 dk[2][KB][2], dv[VB][2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+#pragma unroll
+    for (int d = 0; d < KB; ++d) dk[0][d][n] = dk[1][d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < VB; ++d) dv[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // the first query that sees the workgroup's first key
+  const int first_q = a.causal ? max(kb - start, 0) : 0, first = first_q / TILE;
+  const int ntiles = kb < len && first_q < a.tq ? (a.tq + TILE - 1) / TILE - first : 0, total = ntiles * groups;
+  const int64_t all = (int64_t)a.b * a.h * a.tq;
+  const T* qbase = static_cast<const T*>(a.q.p) + b * a.q.b + 2 * hk * groups * a.q.h;
+  const T* gbase = static_cast<const T*>(a.dy) + ((int64_t)b * a.tq * a.h + hk * groups) * a.dv;
+  Fill<T, 2 * DH, 2, TILE, WG> qf(qbase, a.q.t, a.q.h, a.dh);
+  Fill<T, DV, 1, TILE, WG> gf(gbase, (int64_t)a.h * a.dv, 0, a.dv);
+  auto fetch = [&](int row0, int head, int buf) {   // a tile of one of the group's heads
+    qf.base = qbase + 2 * head * a.q.h;
+    gf.base = gbase + head * a.dv;
+    qf.fetch(row0, a.tq - 1, s_q + buf * QT);
+    gf.fetch(row0, a.tq - 1, s_g + buf * GT);
+    const int t = min(row0 + lane, a.tq - 1);
+    const int64_t n = ((int64_t)b * a.h + hk * groups + head) * a.tq + t;
+    float* o = s_row + buf * 5 * TILE;
+    o[tid] = wave == 0 ? a.lse[n] : wave == 1 ? a.lse[n + all] : wave == 2 ? a.delta[n] : a.delta[n + all];
+    if (TOKEN && wave == 0) o[4 * TILE + lane] = lam_at<T>(a, b, t, hk * groups + head);
+  };
+  if (total > 0) {
+    fetch(first * TILE, 0, 0);
+    filled();
+  }
+  int at = first, head = 0;
+  auto tile = [&](int it, auto buffer) {
+    constexpr int cur = decltype(buffer)::value;
+    const int q0 = at * TILE;
+    const float lam = TOKEN ? 0.f : lam_at<T>(a, b, 0, hk * groups + head);
+    if (++at == first + ntiles) {
+      at = first;
+      ++head;
+    }
+    if (it + 1 < total) fetch(at * TILE, head, cur ^ 1);
+    // the keys that the tile's last and first queries see: whether any of this wave's is among them, and whether all are
+    if (w0 < seen_by(a, min(q0 + TILE, a.tq) - 1, start, len)) {
+      const T* qt = s_q + cur * QT;
+      const T* gt = s_g + cur * GT;
+      const float* sr = s_row + cur * 5 * TILE + 4 * grp;
+      const bool edge = w0 + 32 > seen_by(a, q0, start, len) || q0 + TILE > a.tq;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint2 pd[2][2], p1[2][2], p2[2][2];   // [16 queries][16 keys]: P1 - lam P2, dS1, dS2
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r0 = 32 * i + 16 * u;
+          f32x4 da[2], s1[2], s2[2];
+          in_order();
+#pragma unroll
+          for (int n = 0; n < 2; ++n) da[n] = s1[n] = s2[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < DV / 32; ++ks) {
+            if (ks % 2 == 0) in_order();
+            const uint4 x = grows.at(gt, r0, ks);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) da[n] = Mat<T>::mfma16(x, v.f[n][ks], da[n]);
+          }
+#pragma unroll
+          for (int ks = 0; ks < DH / 32; ++ks) {
+            const uint4 x = qrows.at(qt, r0, ks), y = qrows.at(qt, r0, DH / 32 + ks);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              s1[n] = Mat<T>::mfma16(x, k[0].f[n][ks], s1[n]);
+              s2[n] = Mat<T>::mfma16(y, k[1].f[n][ks], s2[n]);
+            }
+          }
+          in_order();
+          if (edge) {
+            const int here = q0 + 4 * grp, left = a.tq - here;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (r0 + r >= left || here + r0 + r < from[n]) s1[n][r] = s2[n][r] = -INFINITY;
+          }
+          f32x4 x[NUMBERS];
+#pragma unroll
+          for (int e = 0; e < NUMBERS; ++e) x[e] = *reinterpret_cast<const f32x4*>(sr + e * TILE + r0);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float q1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[n][r], a.c, -x[0][r]));
+              const float q2 = (TOKEN ? x[NUMBERS - 1][r] : lam) * __builtin_amdgcn_exp2f(__builtin_fmaf(s2[n][r], a.c, -x[1][r]));
+              s1[n][r] = q1 * (da[n][r] - x[2][r]);
+              s2[n][r] = q2 * (x[3][r] - da[n][r]);
+              da[n][r] = q1 - q2;
+            }
+            pd[u][n] = packed4<T>(da[n]);
+            p1[u][n] = packed4<T>(s1[n]);
+            p2[u][n] = packed4<T>(s2[n]);
+          }
+        }
+        in_order();
+        auto both = [](const uint2 (&p)[2][2], int n) { return make_uint4(p[0][n].x, p[0][n].y, p[1][n].x, p[1][n].y); };
+#pragma unroll
+        for (int d = 0; d < VB; ++d) {
+          if (d % 2 == 0) in_order();
+          const uint4 x = gcols.at(gt, 32 * i, 16 * d);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) dv[d][n] = Mat<T>::mfma16(x, both(pd, n), dv[d][n]);
+        }
+#pragma unroll
+        for (int d = 0; d < KB; ++d) {
+          in_order();
+          const uint4 x = qcols.at(qt, 32 * i, 16 * d), y = qcols.at(qt, 32 * i, DH + 16 * d);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            dk[0][d][n] = Mat<T>::mfma16(x, both(p1, n), dk[0][d][n]);
+            dk[1][d][n] = Mat<T>::mfma16(y, both(p2, n), dk[1][d][n]);
+          }
+        }
+      }
+    }
+    if (it + 1 < total) filled();
+  };
+  for (int it = 0; it < total; it += 2) {
+    tile(it, std::integral_constant<int, 0>());
+    if (it + 1 < total) tile(it + 1, std::integral_constant<int, 1>());
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int key = w0 + 16 * n + (lane & 15);
+    if (key >= a.tk) continue;
+    T* krow = static_cast<T*>(a.dk) + (((int64_t)b * a.tk + key) * 2 * a.hk + 2 * hk) * a.dh;
+    T* vrow = static_cast<T*>(a.dval) + (((int64_t)b * a.tk + key) * a.hk + hk) * a.dv;
+#pragma unroll
+    for (int d = 0; d < KB; ++d) {
+      const int col = 16 * d + 4 * grp;
+      if (col < a.dh) {
+        *reinterpret_cast<uint2*>(krow + col) = packed4<T>(dk[0][d][n] * a.scale);
+        *reinterpret_cast<uint2*>(krow + a.dh + col) = packed4<T>(dk[1][d][n] * a.scale);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < VB; ++d) {
+      const int col = 16 * d + 4 * grp;
+      if (col < a.dv) *reinterpret_cast<uint2*>(vrow + col) = packed4<T>(dv[d][n]);
+    }
+  }
+}
+
+inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline int launched() { return (int)hipGetLastError(); }
+
+#define DIFF_SWITCH(DT, DHS, DVS, ...)                                                                                        \
+  if ((DT) == LDR_BF16) { typedef bf16_t T; DIFF_SIZES(DHS, DVS, __VA_ARGS__) }                                                \
+  else { typedef _Float16 T; DIFF_SIZES(DHS, DVS, __VA_ARGS__) }
+#define DIFF_SIZES(DHS, DVS, ...)                                                                                             \
+  if ((DHS) <= 64 && (DVS) <= 64) { constexpr int DH = 64, DV = 64; __VA_ARGS__; }                                             \
+  else if ((DHS) <= 64 && (DVS) <= 128) { constexpr int DH = 64, DV = 128; __VA_ARGS__; }                                      \
+  else if ((DVS) <= 128) { constexpr int DH = 128, DV = 128; __VA_ARGS__; }                                                    \
+  else { constexpr int DH = 128, DV = 256; __VA_ARGS__; }
+
+constexpr int64_t MOST = 0x7fffff;
+int diff_args(const lmo_diff_shape* s, const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, int dtype) {
+  if (dtype != LDR_BF16 && dtype != LDR_F16) return LDR_E_DTYPE;
+  if (!s || !q || !k || !v) return LDR_E_ARG;
+  if (s->b < 0 || s->tq < 0 || s->tk < 1 || s->hk < 1 || s->h < s->hk || s->h % s->hk || s->b * s->h > MOST || s->tq >= (1 << 30) ||
+      s->tk >= (1 << 30))
+    return LDR_E_ARG;
+  if (s->dh < 8 || s->dh > 128 || s->dh % 8 || s->dv < 8 || s->dv > 256 || s->dv % 8) return LDR_E_SHAPE;
+  if (!(s->scale > 0.f) || !(s->scale < INFINITY)) return LDR_E_ARG;
+  for (const lmo_strides* t : {q, k, v}) {
+    if (!t->p && s->b * s->tq > 0) return LDR_E_ARG;
+    if (!al16(t->p) || t->b % 8 || t->t % 8 || t->h % 8) return LDR_E_ALIGN;
+    if (t->b < 0 || t->t < 0 || t->h < 0 || t->t > (1 << 23) || t->h > (1 << 23)) return LDR_E_SHAPE;   // 64 rows within 32 bits
+  }
+  return LDR_OK;
+}
+Diff diff_of(const lmo_diff_shape* s, const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
+             const int32_t* lengths, const int32_t* starts) {
+  Diff a{};
+  a.q = {q->p, q->b, q->t, q->h};
+  a.k = {k->p, k->b, k->t, k->h};
+  a.v = {v->p, v->b, v->t, v->h};
+  a.lam = {lam->p, lam->b, lam->t, lam->h};
+  a.lengths = lengths;
+  a.starts = starts;
+  a.b = (int)s->b;
+  a.tq = (int)s->tq;
+  a.tk = (int)s->tk;
+  a.h = (int)s->h;
+  a.hk = (int)s->hk;
+  a.dh = (int)s->dh;
+  a.dv = (int)s->dv;
+  a.causal = s->causal;
+  a.lam32 = lam32;
+  a.scale = s->scale;
+  a.c = s->scale * LOG2E;
+  return a;
+}
+inline int64_t blocks_of(int64_t t) { return (t + QB - 1) / QB; }
+// the dynamic LDS that a kernel is allowed has to be raised past 64 KiB, once per kernel and device
+template <typename K, K KERNEL> int allow_lds(int bytes) {
+  static std::atomic<uint64_t> done{0};   // a bit per device
+  int dev = 0;
+  if (bytes <= 65536) return 0;
+  int e = (int)hipGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e || (done.load(std::memory_order_relaxed) & bit)) return e;
+  e = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (!e && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+#define ALLOW_LDS(BYTES, ...) allow_lds<decltype(&__VA_ARGS__), &__VA_ARGS__>(BYTES)
+
+// chunks of the keys for the kernel of few queries: enough workgroups for the CUs, chunks of 256 keys at least
+struct Chunks { int64_t splits, chunk; };
+inline Chunks chunks_of(const lmo_diff_shape* s) {
+  const int64_t items = s->b * s->hk, want = (512 + items - 1) / (items > 0 ? items : 1), most = (s->tk + 255) / 256;
+  int64_t n = want < most ? want : most;
+  n = n < 1 ? 1 : n;
+  const int64_t chunk = ((s->tk + n - 1) / n + 127) / 128 * 128;
+  return {(s->tk + chunk - 1) / chunk, chunk};
+}
+inline bool few(const lmo_diff_shape* s) { return s->tq * (s->h / s->hk) <= FEW; }
+inline int padded_dv(const lmo_diff_shape* s) { return s->dv <= 64 && s->dh <= 64 ? 64 : s->dv <= 128 ? 128 : 256; }
+
+}  // namespace
+
+extern "C" {
+
+int64_t lmo_diff_attn_scratch(const lmo_diff_shape* s, int record) {
+  if (!s || record || s->hk < 1 || s->b < 1 || s->tq < 1 || !few(s)) return 0;
+  const Chunks n = chunks_of(s);
+  return n.splits == 1 ? 0 : s->b * s->h * s->tq * n.splits * (2 * padded_dv(s) + 4);
+}
+
+int lmo_diff_attn_fwd(const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
+                      const int32_t* lengths, const int32_t* starts, void* out, void* second, float* lse, float* scratch,
+                      const lmo_diff_shape* s, int dtype, void* stream) {
+  int e = diff_args(s, q, k, v, dtype);
+  if (e) return e;
+  if (s->b * s->tq == 0) return LDR_OK;
+  if (!lam || !lam->p || !out || !second != !lse) return LDR_E_ARG;
+  if (!al16(out) || !al16(second) || !al16(scratch)) return LDR_E_ALIGN;
+  Diff a = diff_of(s, q, k, v, lam, lam32, lengths, starts);
+  a.out = out;
+  a.second = second;
+  a.lse = lse;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (!lse && few(s)) {
+    const Chunks n = chunks_of(s);
+    if (n.splits > 1 && !scratch) return LDR_E_ARG;
+    a.splits = (int)n.splits;
+    a.chunk = (int)n.chunk;
+    a.part = scratch;
+    const int64_t grid = s->b * s->hk * n.splits;
+    if (grid > 0x7fffffff) return LDR_E_SHAPE;
+    DIFF_SWITCH(dtype, s->dh, s->dv, {
+      constexpr int stage = few_lds<DH, DV>(), joined = few_waves<DH, DV>() * FEW * few_row<DV>() * 4, bytes = stage > joined ? stage : joined;
+      if ((e = ALLOW_LDS(bytes, k_diff_few<T, DH, DV>))) return e;
+      hipLaunchKernelGGL((k_diff_few<T, DH, DV>), dim3((unsigned)grid), dim3(64 * few_waves<DH, DV>()), bytes, st, a);
+      if ((e = launched())) return e;
+      if (n.splits > 1) hipLaunchKernelGGL((k_diff_join<T, DV>), dim3((unsigned)(s->b * s->h * s->tq)), dim3(DV), 0, st, a);
+    })
+    return launched();
+  }
+  const int64_t grid = s->b * s->h * blocks_of(s->tq);
+  if (grid > 0x7fffffff) return LDR_E_SHAPE;
+  DIFF_SWITCH(dtype, s->dh, s->dv, {
+    constexpr int bytes = 2 * TILE * (2 * DH + DV) * 2;
+    if ((e = ALLOW_LDS(bytes, k_diff_fwd<T, DH, DV>))) return e;
+    hipLaunchKernelGGL((k_diff_fwd<T, DH, DV>), dim3((unsigned)grid), dim3(WG), bytes, st, a);
+  })
+  return launched();
+}
+
+int64_t lmo_diff_attn_bwd_scratch(const lmo_diff_shape* s, int lam_kind) {
+  if (!s || s->b < 1 || s->tq < 1) return 0;
+  return 2 * s->b * s->h * s->tq + (lam_kind == LMO_LAM_TOKEN ? s->b * s->tq * s->h : s->h * s->b * blocks_of(s->tq));
+}
+
+int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
+                      const int32_t* lengths, const int32_t* starts, const void* out, const void* second, const float* lse,
+                      const void* dy, void* dq, void* dk, void* dv, void* dlam, int lam_kind, float* scratch,
+                      const lmo_diff_shape* s, int dtype, void* stream) {
+  int e = diff_args(s, q, k, v, dtype);
+  if (e) return e;
+  if (lam_kind < LMO_LAM_LAYER || lam_kind > LMO_LAM_TOKEN) return LDR_E_ARG;
+  if (s->b * s->tq == 0) return LDR_OK;
+  if (!lam || !lam->p || !out || !second || !lse || !dy || !dq || !scratch || !dk != !dv) return LDR_E_ARG;
+  for (const void* p : {out, second, dy, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)scratch})
+    if (!al16(p)) return LDR_E_ALIGN;
+  Diff a = diff_of(s, q, k, v, lam, lam32, lengths, starts);
+  a.out = const_cast<void*>(out);
+  a.second = const_cast<void*>(second);
+  a.lse = const_cast<float*>(lse);
+  a.dy = dy;
+  a.dq = dq;
+  a.dk = dk;
+  a.dval = dv;
+  a.delta = scratch;
+  a.dlam = dlam ? scratch + 2 * s->b * s->h * s->tq : nullptr;
+  a.dlam_rows = lam_kind == LMO_LAM_TOKEN;
+  const int64_t qblocks = blocks_of(s->tq), grid_q = s->b * s->h * qblocks, grid_k = s->b * s->hk * blocks_of(s->tk);
+  if (grid_q > 0x7fffffff || grid_k > 0x7fffffff) return LDR_E_SHAPE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  DIFF_SWITCH(dtype, s->dh, s->dv, {
+    constexpr int bytes = 2 * TILE * (2 * DH + DV) * 2, rows = 2 * 5 * TILE * 4;
+    if ((e = ALLOW_LDS(bytes, k_diff_bwd_q<T, DH, DV>))) return e;
+    hipLaunchKernelGGL((k_diff_bwd_q<T, DH, DV>), dim3((unsigned)grid_q), dim3(WG), bytes, st, a);
+    if ((e = launched())) return e;
+    if (dlam) {
+      const int64_t all = s->b * s->tq * s->h, outs = lam_kind == LMO_LAM_TOKEN ? all : lam_kind == LMO_LAM_HEAD ? s->h : 1;
+      const int64_t n = lam_kind == LMO_LAM_TOKEN ? 1 : lam_kind == LMO_LAM_HEAD ? s->b * qblocks : s->h * s->b * qblocks;
+      const int64_t grid = lam_kind == LMO_LAM_TOKEN || n == 1 ? (outs + WG - 1) / WG : outs;
+      const unsigned g = (unsigned)(grid < 4096 || n != 1 ? grid : 4096);
+      if (lam32) hipLaunchKernelGGL(k_diff_dlam<float>, dim3(g), dim3(WG), 0, st, a.dlam, n, outs, static_cast<float*>(dlam));
+      else hipLaunchKernelGGL(k_diff_dlam<T>, dim3(g), dim3(WG), 0, st, a.dlam, n, outs, static_cast<T*>(dlam));
+      if ((e = launched())) return e;
+    }
+    if (dk && lam->t) {
+      if ((e = ALLOW_LDS(bytes + rows, k_diff_bwd_kv<T, DH, DV, true>))) return e;
+      hipLaunchKernelGGL((k_diff_bwd_kv<T, DH, DV, true>), dim3((unsigned)grid_k), dim3(WG), bytes + rows, st, a);
+    } else if (dk) {
+      if ((e = ALLOW_LDS(bytes + rows, k_diff_bwd_kv<T, DH, DV, false>))) return e;
+      hipLaunchKernelGGL((k_diff_bwd_kv<T, DH, DV, false>), dim3((unsigned)grid_k), dim3(WG), bytes + rows, st, a);
+    }
+  })
+  return launched();
+}
+
+}  // extern "C"

@@ -3,6 +3,8 @@
 
   * `layer_norm(x, weight, bias)` and `add_layer_norm(x, add, weight, bias)`, the latter with the residual's add before the
     norm and, in its backward, the gradient that comes back along the residual stream;
+  * `diff_attention(q, k, v, lam)`: differential attention, (softmax(q1 k1^T) - lam softmax(q2 k2^T)) v, for whole sequences, chunks
+    of new tokens and single ones (bf16 and fp16);
   * `distill_loss(logits, top_logits, top_ids, ...)`: the divergence of a model's logits from a teacher's highest ones, with
     the labels' cross entropy mixed in where they are given.
 
@@ -36,6 +38,10 @@ SIGNATURES = {
     "lmo_layer_norm_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _f32, _i32, _p]),
     "lmo_layer_norm_scratch": (_i64, [_i64, _i64]),
     "lmo_layer_norm_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
+    "lmo_diff_attn_scratch": (_i64, [_p, _i32]),
+    "lmo_diff_attn_fwd": (_i32, [_p, _p, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _p, _i32, _p]),
+    "lmo_diff_attn_bwd_scratch": (_i64, [_p, _i32]),
+    "lmo_diff_attn_bwd": (_i32, [_p, _p, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _p, _p, _i32, _p]),
     "lmo_distill_fwd": (_i32, [_p, _p, _i32, _p, _i32, _p, _p, _f32, _f32, _p, _p, _p, _i64, _i64, _i64, _i32, _p]),
     "lmo_distill_bwd": (_i32, [_p, _p, _i32, _p, _i32, _p, _f32, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _p]),
 }
@@ -137,6 +143,140 @@ def add_layer_norm(x: torch.Tensor, add: torch.Tensor | None, weight: torch.Tens
         return h, _norm_torch(h, weight, bias, eps)
     x, add, weight, bias = _plain_rows(x, add, weight, bias)
     return H.layer_norm(x, add, weight, bias, eps, _CODES[x.dtype], _stream(x), _records(x, add, weight, bias))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# differential attention
+# ---------------------------------------------------------------------------------------------------------------
+ATTN_MAX_DH, ATTN_MAX_DV, ATTN_MAX_TOKENS, ATTN_MAX_HEADS = 128, 256, 2 ** 30 - 1, 0x7fffff
+
+
+def _seen(b, tq, tk, causal, lengths, starts, device):
+    """(b, tq, tk): which keys each query sees."""
+    j = torch.arange(tk, device=device)
+    i = torch.arange(tq, device=device).view(-1, 1)
+    seen = torch.ones((b, tq, tk), dtype=torch.bool, device=device)
+    if causal:
+        start = tk - tq if starts is None else starts.view(-1, 1, 1)
+        seen = seen & (j <= start + i)
+    return seen if lengths is None else seen & (j < lengths.view(-1, 1, 1))
+
+
+def _maps(q, k, causal, scale, lengths, starts):
+    """Both softmax maps (b, hk, group, 2, tq, tk) of the unrounded q and k."""
+    (b, tq, h2, dh), tk, hk = q.shape, k.shape[1], k.shape[2] // 2
+    q = q.reshape(b, tq, hk, h2 // (2 * hk), 2, dh).permute(0, 2, 3, 4, 1, 5)
+    k = k.reshape(b, tk, hk, 1, 2, dh).permute(0, 2, 3, 4, 5, 1)
+    s = q.matmul(k.expand(b, hk, q.shape[2], 2, dh, tk).contiguous()) * scale
+    s = torch.where(_seen(b, tq, tk, causal, lengths, starts, q.device).view(b, 1, 1, 1, tq, tk), s, -torch.inf)
+    if tk:
+        s = s - s.detach().amax(-1, keepdim=True).clamp_min(-1e30)   # finite where no key is seen
+    e = torch.exp(s)
+    total = e.sum(-1, keepdim=True)
+    return e / torch.where(total == 0, 1.0, total)
+
+
+def _held(t, lengths):
+    """t (b, tk, ...) with zeros past the lengths: what is there is not read into anything."""
+    if lengths is None:
+        return t
+    there = torch.arange(t.shape[1], device=t.device) < lengths.view(-1, 1)
+    return torch.where(there.view(*there.shape, *(1 for _ in t.shape[2:])), t, 0.0)
+
+
+def _lam_of(lam, b, tq, hk, group):
+    """lam as (b, hk, group, tq, 1)."""
+    return lam.expand(b, tq, hk * group).reshape(b, tq, hk, group).permute(0, 2, 3, 1).unsqueeze(-1)
+
+
+def _diff_torch(q, k, v, lam, causal, scale, lengths, starts):
+    dt, (b, tq), hk, group = q.dtype, q.shape[:2], v.shape[2], q.shape[2] // (2 * v.shape[2])
+    k, v = _held(_upcast(k), lengths), _held(_upcast(v), lengths)
+    p = _maps(_upcast(q), k, causal, scale, lengths, starts)
+    a = p[:, :, :, 0] - _lam_of(_upcast(lam), b, tq, hk, group) * p[:, :, :, 1]
+    y = a.matmul(v.permute(0, 2, 1, 3).unsqueeze(2).expand(b, hk, group, v.shape[1], v.shape[3]).contiguous())
+    return y.permute(0, 3, 1, 2, 4).reshape(b, tq, hk * group, v.shape[3]).to(dt)
+
+
+def _diff_backward(dy, q, k, v, lam, lengths, starts, causal, need, scale):
+    """The torch form of differential attention's backward, for the node (csrc/host.cpp), by its formulas: the gradients of q, k, v
+    and lam that need's bits ask for."""
+    dt, (b, tq, h2, dh), (tk, hk, dv) = q.dtype, q.shape, v.shape[1:]
+    group = h2 // (2 * hk)
+    qu, ku, vu = _upcast(q), _held(_upcast(k), lengths), _held(_upcast(v), lengths)
+    p = _maps(qu, ku, causal, scale, lengths, starts)
+    l1 = _lam_of(_upcast(lam), b, tq, hk, group)
+    g = _upcast(dy).reshape(b, tq, hk, group, dv).permute(0, 2, 3, 1, 4)                   # (b, hk, group, tq, dv)
+    da = g.matmul(vu.permute(0, 2, 3, 1).unsqueeze(2).expand(b, hk, group, dv, tk).contiguous())
+    p1, p2 = p[:, :, :, 0], p[:, :, :, 1]
+    d1, d2 = (p1 * da).sum(-1, keepdim=True), (p2 * da).sum(-1, keepdim=True)
+    ds = torch.stack((p1 * (da - d1), -l1 * p2 * (da - d2)), 3) * scale                    # (b, hk, group, 2, tq, tk)
+    out = [None] * 4
+    if need & 1:
+        kk = ku.reshape(b, tk, hk, 1, 2, dh).permute(0, 2, 3, 4, 1, 5).expand(b, hk, group, 2, tk, dh).contiguous()
+        out[0] = ds.matmul(kk).permute(0, 4, 1, 2, 3, 5).reshape(q.shape).to(dt)
+    if need & 2:
+        qq = qu.reshape(b, tq, hk, group, 2, dh).permute(0, 2, 3, 4, 1, 5).contiguous()
+        dk = ds.transpose(-1, -2).contiguous().matmul(qq).sum(2)                           # (b, hk, 2, tk, dh)
+        out[1] = dk.permute(0, 3, 1, 2, 4).reshape(k.shape).to(dt)
+    if need & 4:
+        dval = (p1 - l1 * p2).transpose(-1, -2).contiguous().matmul(g.contiguous()).sum(2)
+        out[2] = dval.permute(0, 2, 1, 3).reshape(v.shape).to(dt)
+    if need & 8:
+        dl = -d2.squeeze(-1).permute(0, 3, 1, 2).reshape(b, tq, hk * group)
+        out[3] = (dl if lam.dim() == 3 else dl.sum((0, 1)) if lam.dim() == 1 else dl.sum()).to(lam.dtype)
+    return tuple(out)
+
+
+def attention_native(q, k, v, lam) -> bool:
+    """Whether the kernels take the call: bf16 or fp16, widths that are multiples of 8 up to 128 and 256, lam of their type or fp32."""
+    return (native(q, k, v) and (type(lam) is torch.Tensor or type(lam) is torch.nn.Parameter) and lam.dtype in (q.dtype, torch.float32)
+            and q.numel() > 0 and k.numel() > 0 and q.shape[3] % 8 == 0 and q.shape[3] <= ATTN_MAX_DH and v.shape[3] % 8 == 0
+            and 0 < v.shape[3] <= ATTN_MAX_DV and max(q.shape[1], k.shape[1]) <= ATTN_MAX_TOKENS and q.shape[0] * q.shape[2] <= ATTN_MAX_HEADS)
+
+
+def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, *, causal: bool = True,
+                   scale: float | None = None, lengths: torch.Tensor | None = None,
+                   starts: torch.Tensor | None = None) -> torch.Tensor:
+    """Differential attention of H heads, each of two maps: y = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v.
+
+    q (b, tq, 2 H, dh), rows 2 h and 2 h + 1 head h's two queries; k (b, tk, 2 G, dh) and v (b, tk, G, dv), G dividing H: H / G heads
+    in a row share a pair of keys and its values. lam is one value (), one per head (H,) or one per query and head (b, tq, H), of
+    q's type or fp32. Returns (b, tq, H, dv). scale: dh^-0.5 unless given, above 0.
+
+    A query i of batch row n sees the keys j < lengths[n] (all tk without it) and, where causal, j <= starts[n] + i: starts is the
+    position of the first query among the keys, tk - tq without it (the queries are the last tokens). A query that sees no key has
+    zeros and no gradient. What k and v hold at and past lengths is not read into anything, and its gradient is zero. lengths and
+    starts are int32 or int64 (b,), read when a kernel runs. Differentiable in q, k, v and lam."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or not (q.is_floating_point() and k.is_floating_point() and v.is_floating_point()):
+        raise ValueError(f"diff_attention takes floating point q (b, tq, 2 H, dh), k (b, tk, 2 G, dh), v (b, tk, G, dv), got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    b, tq, h2, dh = q.shape
+    tk, g = v.shape[1], v.shape[2]
+    if k.shape != (b, tk, 2 * g, dh) or v.shape[0] != b or g < 1 or h2 % (2 * g) or h2 == 0 or dh == 0 or v.shape[3] == 0:
+        raise ValueError(f"diff_attention takes q (b, tq, 2 H, dh), k (b, tk, 2 G, dh), v (b, tk, G, dv), G dividing H, got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    h = h2 // 2
+    if not isinstance(lam, torch.Tensor) or not lam.is_floating_point() or tuple(lam.shape) not in ((), (h,), (b, tq, h)):
+        raise ValueError(f"lam is a floating point tensor (), ({h},) or ({b}, {tq}, {h}), got "
+                         f"{tuple(lam.shape) if isinstance(lam, torch.Tensor) else lam!r}")
+    for t in (k, v, lam):
+        if t.device != q.device:
+            raise ValueError(f"q is on {q.device}, k, v or lam on {t.device}")
+    scale = dh ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale is above 0, got {scale}")
+    for name, t in (("lengths", lengths), ("starts", starts)):
+        if t is not None and (t.dtype not in (torch.int32, torch.int64) or t.shape != (b,) or t.device != q.device):
+            raise ValueError(f"{name} is an int32 or int64 tensor ({b},) on {q.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    causal = bool(causal)
+    plain = all(t is None or type(t) is torch.Tensor for t in (lengths, starts))
+    if not (plain and attention_native(q, k, v, lam)):
+        return _diff_torch(q, k, v, lam, causal, scale, lengths, starts)
+    lengths, starts = (t if t is None or t.dtype is torch.int32 else t.clamp(-ATTN_MAX_TOKENS, ATTN_MAX_TOKENS).int()
+                       for t in (lengths, starts))
+    lengths, starts = _plain_rows(lengths, starts)
+    return H.diff_attn(q, k, v, lam, lengths, starts, causal, scale, _CODES[q.dtype], _stream(q), _records(q, k, v, lam))
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -275,4 +415,4 @@ def distill_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.
                      _records(logits))
 
 
-H.model_forms(_norm_backward, _distill_backward)
+H.model_forms(_norm_backward, _distill_backward, _diff_backward)

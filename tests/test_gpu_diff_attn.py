@@ -1,0 +1,326 @@
+"""Differential attention (model_ops.diff_attention) on the kernels against its formulas in fp64 on the same inputs.
+
+h is half a step of the type (2^-8 of a bf16 value, 2^-11 of an fp16 one), u = 2^-24. Bounds, element by element:
+  * a score is a sum of dh products in fp32, so it is within (dh + 8) u of the sum of their absolute values S; the probabilities, and
+    the sums over at most n keys that divide them, are within e = 2 (dh + 8) u max S + (n / 64 + 64) u of themselves (a wave's lane
+    adds the keys of a 64-key tile in four sums, then tile after tile);
+  * forward: each probability enters the product rounded to the type, so P v is within (h + 2 e) sum p |v|, y within that for both
+    maps, and is rounded once more;
+  * backward: D1 and D2 come from the rounded y and P2 v, so they are within dy . (their bounds); a score gradient is within
+    p (bound of D) + e |p (dA - D)| and is rounded to the type before the products that sum it, as the combined map is; dlam sums
+    p dA in fp32. A result is rounded once;
+  * what is rounded below a type's smallest normal number may lose all of it: 2^-25 in fp16 (half of its smallest subnormal), 2^-126
+    in bf16 and fp32 (flushed), times a few for the products that it enters (FLOOR)."""
+import math
+
+import pytest
+import torch
+
+from gpu_helpers import DEV
+from loopback_amd import model_ops as M
+
+pytestmark = pytest.mark.gpu
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TYPES = [torch.bfloat16, torch.float16]
+U = 2.0 ** -24
+FLOOR = {torch.bfloat16: 2.0 ** -124, torch.float16: 2.0 ** -25}
+
+
+def rnd(shape, dtype, seed, std=1.0, mean=0.0):
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std + mean
+    return x.to(dtype).to(DEV)
+
+
+def close(got, ref, slack, what):
+    half = HALF.get(got.dtype, U)
+    tiny = 2.0 ** -25 if got.dtype is torch.float16 else 0.0
+    bad = (got.double() - ref).abs() > half * (ref.abs() + slack) + slack + tiny
+    worst = ((got.double() - ref).abs() / (half * (ref.abs() + slack) + slack + tiny + 1e-300)).max().item()
+    assert got.shape == ref.shape and got.isfinite().all() and not bad.any(), (what, int(bad.sum()), worst)
+
+
+def reference(q, k, v, lam, dy, causal=True, scale=None, lengths=None, starts=None):
+    """{name: (value, slack)}."""
+    half, floor = HALF[q.dtype], FLOOR[q.dtype]
+    f = lambda t: t.double()  # noqa: E731
+    (b, tq, h2, dh), (tk, hk, dv) = q.shape, v.shape[1:]
+    h = h2 // 2
+    scale = dh ** -0.5 if scale is None else scale
+    dev = q.device
+    out = {n: (torch.zeros(s, dtype=torch.float64, device=dev), torch.zeros(s, dtype=torch.float64, device=dev))
+           for n, s in (("y", (b, tq, h, dv)), ("dq", q.shape), ("dk", k.shape), ("dv", v.shape), ("dlam", (b, tq, h)))}
+    lam_all = f(lam).expand(b, tq, h)
+    i, j = torch.arange(tq, device=dev).view(-1, 1), torch.arange(tk, device=dev)
+    for n in range(b):
+        length = tk if lengths is None else min(max(int(lengths[n]), 0), tk)
+        start = tk - tq if starts is None else int(starts[n])
+        seen = (j < length) & ((j <= start + i) if causal else torch.ones_like(i, dtype=torch.bool))
+        for x in range(h):
+            g = x // (h // hk)
+            vv, vals = torch.where((j < length).view(-1, 1), f(v[n, :, g]), 0.0), []
+            for m in range(2):
+                kk = torch.where((j < length).view(-1, 1), f(k[n, :, 2 * g + m]), 0.0)
+                qq = f(q[n, :, 2 * x + m])
+                s = (qq @ kk.T * scale).masked_fill(~seen, -math.inf)
+                p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+                size = torch.where(seen, qq.abs() @ kk.abs().T * scale, 0.0).amax(-1, keepdim=True)
+                e = 2 * (dh + 8) * U * size + (tk / 64 + 64) * U
+                vals.append((p, e, kk, qq))
+            (p1, e1, k1, q1), (p2, e2, k2, q2) = vals
+            lm = lam_all[n, :, x].unsqueeze(-1)
+            pv1, pv2 = (half + 2 * e1) * (p1 @ vv.abs()), (half + 2 * e2) * (p2 @ vv.abs())
+            z = p2 @ vv
+            y = p1 @ vv - lm * z
+            by = pv1 + lm.abs() * pv2 + 4 * U * (p1 @ vv.abs() + (lm * z).abs())
+            by = by + floor * (1 + lm.abs()) * (seen.double() @ vv.abs())
+            out["y"][0][n, :, x], out["y"][1][n, :, x] = y, by
+            if dy is None:
+                continue
+            g_ = f(dy[n, :, x])
+            da = g_ @ vv.T
+            eda = (dv + 8) * U * (g_.abs() @ vv.abs().T)
+            d1, d2 = (p1 * da).sum(-1, keepdim=True), (p2 * da).sum(-1, keepdim=True)
+            b2 = (g_.abs() * (half * (z.abs() + pv2) + pv2 + (dv + 8) * U * z.abs())).sum(-1, keepdim=True)
+            b1 = (g_.abs() * (half * (y.abs() + by) + by + (dv + 8) * U * (y.abs() + (lm * z).abs()))).sum(-1, keepdim=True) + lm.abs() * b2
+            for m, (p, e, kk, qq, d, bd, w) in enumerate(((p1, e1, k1, q1, d1, b1, torch.ones_like(lm)), (p2, e2, k2, q2, d2, b2, -lm))):
+                ds = p * (da - d) * w
+                bs = w.abs() * p * (bd + eda + 4 * U * (da.abs() + d.abs())) + (half + e + 8 * U) * ds.abs()
+                bs = bs + half * w.abs() * p * (bd + eda) + floor * seen * (1 + da.abs() + d.abs()) * (1 + w.abs())
+                out["dq"][0][n, :, 2 * x + m], out["dq"][1][n, :, 2 * x + m] = ds @ kk * scale, (bs + tk * U * ds.abs()) @ kk.abs() * scale
+                out["dk"][0][n, :, 2 * g + m] += ds.T @ qq * scale
+                out["dk"][1][n, :, 2 * g + m] += (bs + tq * U * ds.abs()).T @ qq.abs() * scale
+            a = p1 - lm * p2
+            out["dv"][0][n, :, g] += a.T @ g_
+            out["dv"][1][n, :, g] += (half * a.abs() + (e1 + 4 * U) * p1 * (1 + half) + (e2 + 4 * U) * p2 * lm.abs() * (1 + half)
+                                      + tq * U * (p1 + lm.abs() * p2) + floor * seen * (1 + lm.abs())).T @ g_.abs()
+            out["dlam"][0][n, :, x] = -d2.squeeze(-1)
+            out["dlam"][1][n, :, x] = (p2 * ((e2 + 2 * U + tk * U) * da.abs() + eda)).sum(-1)
+    if lam.dim() < 3:
+        dims = (0, 1) if lam.dim() == 1 else (0, 1, 2)
+        val, s = out["dlam"]
+        out["dlam"] = (val.sum(dims), s.sum(dims) + (b * tq * h) * U * val.abs().sum(dims))
+    return out
+
+
+def operands(b, tq, tk, h, hk, dh, dv, dtype, lam="head", seed=1, std=1.0):
+    shape = {"layer": (), "head": (h,), "token": (b, tq, h)}[lam]
+    return [rnd((b, tq, 2 * h, dh), dtype, seed, std), rnd((b, tk, 2 * hk, dh), dtype, seed + 1, std), rnd((b, tk, hk, dv), dtype, seed + 2),
+            rnd(shape, dtype, seed + 3, 0.3, 0.5)]
+
+
+def ints(*v, dtype=torch.int32):
+    return torch.tensor(v, dtype=dtype, device=DEV)
+
+
+def check(ts, train=True, **how):
+    dy = rnd((*ts[0].shape[:2], ts[0].shape[2] // 2, ts[2].shape[3]), ts[0].dtype, 77) if train else None
+    ref = reference(*ts, dy, **how)
+    plain = M.diff_attention(*ts, **how)
+    close(plain, *ref["y"], "y")
+    if not train:
+        return
+    leaves = [t.detach().requires_grad_() for t in ts]
+    y = M.diff_attention(*leaves, **how)
+    close(y.detach(), *ref["y"], "recorded y")
+    for name, g in zip(("dq", "dk", "dv", "dlam"), torch.autograd.grad(y, leaves, dy)):
+        close(g, *ref[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dh,dv", [(64, 128), (64, 64), (40, 80), (8, 8), (32, 64), (128, 256), (96, 192), (128, 128), (64, 192)])
+@pytest.mark.parametrize("t", [1, 2, 31, 65, 200])
+def test_widths_and_lengths(t, dh, dv, dtype):
+    check(operands(2, t, t, 2, 1, dh, dv, dtype))
+
+
+@pytest.mark.parametrize("lam", ["layer", "head", "token"])
+@pytest.mark.parametrize("b,h,hk", [(1, 1, 1), (3, 4, 4), (2, 6, 2), (4, 8, 2)])
+def test_heads_and_lambda(b, h, hk, lam):
+    check(operands(b, 130, 130, h, hk, 64, 128, torch.bfloat16, lam))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lambda_in_fp32_negative_and_zero(dtype):
+    ts = operands(2, 70, 70, 4, 2, 64, 128, dtype)
+    for lam in (torch.tensor([0.7, -0.4, 0.0, 1.5], device=DEV), torch.tensor(-0.3, device=DEV), torch.randn(2, 70, 4, device=DEV)):
+        check([*ts[:3], lam])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("tq,tk", [(1, 1), (1, 700), (3, 64), (5, 333), (40, 41), (100, 300), (129, 1000), (70, 30)])
+def test_chunks(tq, tk, causal):
+    """Queries that are the last tokens; more queries than keys: the first ones see none."""
+    check(operands(2, tq, tk, 4, 2, 64, 128, torch.bfloat16), causal=causal)
+
+
+@pytest.mark.parametrize("train", [True, False])
+@pytest.mark.parametrize("wide", [torch.int32, torch.int64])
+def test_ragged(train, wide):
+    """Lengths and positions of each sequence: none, one, inside and at a tile's end, past the tensor; queries before the first key."""
+    b, tk = 8, 300
+    lengths = ints(0, 1, 63, 64, 65, 300, 1000, -4, dtype=wide)
+    for tq in (1, 5, 150):
+        ts = operands(b, tq, tk, 4, 2, 64, 128, torch.bfloat16, "token")
+        check(ts, train, lengths=lengths)
+        check(ts, train, lengths=lengths, starts=lengths.clamp(0, tk) - tq)
+        check(ts, train, lengths=lengths, starts=ints(-1000, 0, 5, -3, 64, 299, 2 ** 31 - 1, -2 ** 31, dtype=wide))
+        check(ts, train, lengths=lengths, causal=False)
+
+
+def test_what_is_past_the_lengths():
+    """NaN and infinities in an unwritten cache reach nothing, and their gradient is zero."""
+    lengths = ints(0, 1, 70, 128, 199)
+    for tq in (1, 200):
+        ts = operands(5, tq, 200, 4, 2, 64, 128, torch.bfloat16)
+        how = {"lengths": lengths, "starts": lengths - tq if tq == 1 else ints(0, 0, 0, 0, 0)}
+        ref = M.diff_attention(*ts, **how)
+        for n, length in enumerate(lengths.tolist()):
+            ts[1][n, length:], ts[2][n, length:] = math.nan, math.inf
+        assert torch.equal(M.diff_attention(*ts, **how), ref) and not ref[0].any()
+        leaves = [t.detach().requires_grad_() for t in ts]
+        grads = torch.autograd.grad(M.diff_attention(*leaves, **how), leaves, torch.ones_like(ref))
+        assert all(g.isfinite().all() for g in grads)
+        for n, length in enumerate(lengths.tolist()):
+            assert not grads[1][n, length:].any() and not grads[2][n, length:].any()
+        assert not grads[0][0].any()
+
+
+@pytest.mark.parametrize("b,tq,tk,h,hk", [(1, 1, 20000, 2, 1), (2, 8, 5000, 8, 2), (32, 1, 1500, 4, 4), (1, 32, 4097, 1, 1), (300, 1, 40, 2, 2)])
+def test_few_queries_over_long_caches(b, tq, tk, h, hk):
+    ts = operands(b, tq, tk, h, hk, 64, 128, torch.bfloat16)
+    check(ts, False)
+    g = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, tk + 1, (b,), generator=g, dtype=torch.int32).to(DEV)
+    check(ts, False, lengths=lengths, starts=lengths - tq)
+
+
+def test_far_scores():
+    """Scores of hundreds, rising and falling along the keys: the running maximum moves at every tile, or never."""
+    for sign in (1.0, -1.0):
+        q, k, v, lam = operands(1, 200, 200, 2, 1, 64, 128, torch.bfloat16)
+        ramp = torch.linspace(0, 30, 200, device=DEV).view(1, -1, 1, 1)
+        k = (k * 0.1 + sign * ramp * 0.25).to(k.dtype)
+        q = (q * 0.1 + 3.0).to(q.dtype)
+        check([q, k, v, lam])
+
+
+def test_scale_strides_alignment():
+    dt = torch.bfloat16
+    q, k, v, lam = operands(2, 90, 90, 4, 2, 64, 128, dt)
+    ref = M.diff_attention(q, k, v, lam, scale=0.3)
+    check([q, k, v, lam], scale=0.3)
+    fused = torch.cat((q.flatten(2), k.flatten(2), v.flatten(2)), -1)      # one projection's output, split
+    parts = fused.split([512, 256, 256], -1)
+    views = [parts[0].view(2, 90, 8, 64), parts[1].view(2, 90, 4, 64), parts[2].view(2, 90, 2, 128)]
+    assert torch.equal(M.diff_attention(*views, lam, scale=0.3), ref)
+    odd = [torch.empty(t.numel() + 1, dtype=dt, device=DEV)[1:].view(t.shape).copy_(t) for t in (q, k, v)]
+    assert torch.equal(M.diff_attention(*odd, lam, scale=0.3), ref)
+    turned = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]      # heads before tokens
+    assert torch.equal(M.diff_attention(*turned, lam, scale=0.3), ref)
+    last = [t.transpose(2, 3).contiguous().transpose(2, 3) for t in (q, k, v)]        # columns apart
+    assert torch.equal(M.diff_attention(*last, lam, scale=0.3), ref)
+    shared = M.diff_attention(q, k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1), lam.unsqueeze(0).expand(2, 90, 4), scale=0.3)
+    assert torch.equal(shared[0], ref[0])
+    leaves = [t.detach().requires_grad_() for t in (*odd, lam)]
+    a = torch.autograd.grad(M.diff_attention(*leaves, scale=0.3).transpose(1, 2), leaves, torch.ones(2, 4, 90, 128, device=DEV, dtype=dt))
+    leaves = [t.detach().requires_grad_() for t in (*last, lam)]
+    b = torch.autograd.grad(M.diff_attention(*leaves, scale=0.3), leaves, torch.ones((), device=DEV, dtype=dt).expand(2, 90, 4, 128))
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+def test_gradients_that_are_asked_for():
+    ts = operands(2, 77, 77, 4, 2, 64, 128, torch.bfloat16)
+    dy = rnd((2, 77, 4, 128), torch.bfloat16, 9)
+    leaves = [t.clone().requires_grad_() for t in ts]
+    full = torch.autograd.grad(M.diff_attention(*leaves), leaves, dy)
+    for need in range(1, 16):
+        leaves = [t.clone().requires_grad_(bool(need >> i & 1)) for i, t in enumerate(ts)]
+        got = torch.autograd.grad(M.diff_attention(*leaves), [t for t in leaves if t.requires_grad], dy)
+        for a, b in zip(got, [g for i, g in enumerate(full) if need >> i & 1]):
+            assert torch.equal(a, b)
+
+
+def test_against_differences():
+    """The kernels' gradient along a direction against differences of the plain forward in fp64."""
+    ts = operands(1, 40, 40, 2, 1, 64, 128, torch.float16)
+    dy = rnd((1, 40, 2, 128), torch.float16, 9)
+    leaves = [t.clone().requires_grad_() for t in ts]
+    got = torch.autograd.grad(M.diff_attention(*leaves), leaves, dy)
+    f = [t.double().cpu() for t in ts]
+    eps = 1e-5
+    for i, g in enumerate(got):
+        d = torch.randn(f[i].shape, generator=torch.Generator().manual_seed(i), dtype=torch.float64)
+        side = [M.diff_attention(*[t + s * eps * d if n == i else t for n, t in enumerate(f)]) for s in (1, -1)]
+        want = ((side[0] - side[1]) / (2 * eps) * dy.double().cpu()).sum()
+        # the bounds above, each element's, along the direction
+        ref = reference(*ts, dy)[("dq", "dk", "dv", "dlam")[i]]
+        slack = ((HALF[torch.float16] * ref[0].abs() + 2 * ref[1]).cpu() * d.abs()).sum() + 1e-6 * want.abs()
+        assert abs((g.double().cpu() * d).sum() - want) <= slack
+
+
+def test_streams_graphs_and_the_same_bits():
+    ts = operands(3, 150, 150, 4, 2, 64, 128, torch.bfloat16, "token")
+    lengths = ints(150, 20, 0)
+    dy = rnd((3, 150, 4, 128), torch.bfloat16, 9)
+
+    def step(n):
+        leaves = [t.detach().requires_grad_() for t in ts]
+        y = M.diff_attention(*leaves, lengths=n)
+        few = M.diff_attention(ts[0][:, -1:].detach(), *(t.detach() for t in ts[1:3]), torch.ones((), device=DEV), lengths=n)
+        return (y.detach(), few, *torch.autograd.grad(y, leaves, dy))
+
+    want = step(lengths)
+    for a, b in zip(step(lengths), want):
+        assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(lengths)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(lengths)
+    for n in ((150, 20, 0), (3, 150, 64), (0, 0, 1)):
+        lengths.copy_(ints(*n))
+        ts[0].add_(0.125)
+        want = [t.clone() for t in step(lengths)]
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_watched_and_differentiated_backwards():
+    ts = operands(1, 9, 9, 2, 1, 16, 32, torch.bfloat16)
+    leaves = [t.requires_grad_() for t in ts]
+    y = M.diff_attention(*leaves)
+    dy = rnd(y.shape, y.dtype, 9)
+    plain = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    graphed = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    for a, b in zip(plain, graphed):
+        assert (a.double() - b.double()).norm() <= 0.02 * b.double().norm()
+    again = torch.autograd.grad(sum((g.float() ** 2).sum() for g in graphed), leaves)
+    assert all(g.isfinite().all() and g.any() for g in again)
+    rows = torch.autograd.grad(y, leaves[0], torch.stack((dy, 2 * dy)), is_grads_batched=True, retain_graph=True)[0]
+    assert (rows[0].double() - plain[0].double()).norm() <= 0.02 * plain[0].double().norm()
+    for bad in (lambda t: t.reshape(-1)[:8], lambda t: t.cpu(), lambda t: t.double()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, bad):
+            o = M.diff_attention(*leaves)
+        with pytest.raises(RuntimeError, match="hook"):
+            o.sum().backward()
+    with torch.autograd.graph.save_on_cpu():
+        o = M.diff_attention(*leaves)
+    for a, b in zip(torch.autograd.grad(o, leaves, dy), plain):
+        assert torch.equal(a, b)
+
+
+def test_empty():
+    for b, tq, tk in ((0, 4, 4), (2, 0, 4), (2, 4, 0)):
+        ts = [t.requires_grad_() for t in operands(b, tq, tk, 2, 1, 64, 128, torch.bfloat16)]
+        y = M.diff_attention(*ts)
+        assert y.shape == (b, tq, 2, 128) and not y.any()
+        y.sum().backward()
+        assert all(t.grad is not None and not t.grad.any() for t in ts)

@@ -179,3 +179,115 @@ def test_distill_refusals():
                 lambda: M.distill_loss(x[:, :0], top, ids), lambda: M.distill_loss(x, top.to("meta"), ids)):
         with pytest.raises(ValueError):
             bad()
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# differential attention
+# ---------------------------------------------------------------------------------------------------------------
+def attn(b=2, tq=5, tk=5, h=4, g=2, dh=4, dv=6, lam=(4,)):
+    return rnd(b, tq, 2 * h, dh), rnd(b, tk, 2 * g, dh, seed=2), rnd(b, tk, g, dv, seed=3), rnd(*lam, seed=4)
+
+
+def test_attention_is_the_difference_of_two():
+    """Against torch's attention over each map, its heads of keys repeated."""
+    q, k, v, lam = attn()
+    maps = [F.scaled_dot_product_attention(q[:, :, m::2].transpose(1, 2), k[:, :, m::2].transpose(1, 2).repeat_interleave(2, 1),
+                                           v.transpose(1, 2).repeat_interleave(2, 1), is_causal=True) for m in (0, 1)]
+    want = (maps[0] - lam.view(1, 4, 1, 1) * maps[1]).transpose(1, 2)
+    assert torch.allclose(M.diff_attention(q, k, v, lam), want, atol=1e-12)
+    assert torch.allclose(M.diff_attention(q, k, v, lam.expand(2, 5, 4)), want, atol=1e-12)
+    one = M.diff_attention(q, k, v, torch.tensor(0.25, dtype=torch.float64), causal=False, scale=0.7)
+    maps = [F.scaled_dot_product_attention(q[:, :, m::2].transpose(1, 2), k[:, :, m::2].transpose(1, 2).repeat_interleave(2, 1),
+                                           v.transpose(1, 2).repeat_interleave(2, 1), scale=0.7) for m in (0, 1)]
+    assert torch.allclose(one, (maps[0] - 0.25 * maps[1]).transpose(1, 2), atol=1e-12)
+
+
+def test_attention_masks():
+    """A token at a time over a growing cache gives what the whole sequence gives; rows that see nothing are zeros; what is past
+    the lengths is not read into anything."""
+    q, k, v, lam = attn()
+    whole = M.diff_attention(q, k, v, lam)
+    for i in range(5):
+        n = torch.tensor([i + 1, i + 1])
+        cache = k.clone(), v.clone()
+        for c in cache:
+            c[:, i + 1:] = math.nan
+        assert torch.allclose(M.diff_attention(q[:, i:i + 1], *cache, lam, lengths=n, starts=n.int() - 1), whole[:, i:i + 1], atol=1e-12)
+    assert torch.allclose(M.diff_attention(q[:, 3:], k, v, lam), whole[:, 3:], atol=1e-12)
+    more = M.diff_attention(q, k[:, :2], v[:, :2], lam)          # more queries than keys: the first three see none
+    assert not more[:, :3].any() and more[:, 3:].ne(0).all()
+    none = M.diff_attention(q, k, v, lam, lengths=torch.tensor([0, 5]))
+    assert not none[0].any() and torch.equal(none[1], whole[1])
+    for tq, tk in ((0, 3), (3, 0)):
+        ts = [t.requires_grad_() for t in attn(tq=tq, tk=tk)]
+        y = M.diff_attention(*ts)
+        assert y.shape == (2, tq, 4, 6) and not y.any()
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("lam", [(), (4,), (2, 3, 4)])
+def test_attention_gradients(lam):
+    ts = [t.requires_grad_() for t in attn(tq=3, lam=lam)]
+    how = {"lengths": torch.tensor([5, 2]), "starts": torch.tensor([2, -2])}
+    f = lambda *a: M.diff_attention(*a, **how)  # noqa: E731
+    assert torch.autograd.gradcheck(f, ts)
+    if lam == (4,):
+        assert torch.autograd.gradgradcheck(f, ts)
+    dy = rnd(2, 3, 4, 6, seed=9)
+    want = torch.autograd.grad(f(*ts), ts, dy)
+    got = M._diff_backward(dy, *(t.detach() for t in ts), how["lengths"], how["starts"], 1, 15, 0.5)
+    for a, b in zip(got, want):
+        assert a.shape == b.shape and torch.allclose(a, b, atol=1e-12)
+
+
+def test_attention_refusals():
+    q, k, v, lam = attn()
+    n = torch.tensor([1, 2])
+    for bad in (lambda: M.diff_attention(q[0], k, v, lam), lambda: M.diff_attention(q.long(), k, v, lam), lambda: M.diff_attention(q, k[:1], v, lam),
+                lambda: M.diff_attention(q, k[:, :4], v, lam), lambda: M.diff_attention(q, k[..., :3], v, lam),
+                lambda: M.diff_attention(q[:, :, :7], k, v, lam), lambda: M.diff_attention(q[:, :, :6], k, v, lam[:3]),
+                lambda: M.diff_attention(q, k[:, :, :3], v, lam), lambda: M.diff_attention(q, k, v, lam[:3]),
+                lambda: M.diff_attention(q, k, v, 0.5), lambda: M.diff_attention(q, k, v, lam.long()),
+                lambda: M.diff_attention(q, k, v, lam.view(1, 4)), lambda: M.diff_attention(q, k, v, lam, scale=0.0),
+                lambda: M.diff_attention(q, k, v, lam, scale=-1.0), lambda: M.diff_attention(q, k, v, lam, scale=math.inf),
+                lambda: M.diff_attention(q, k, v, lam, lengths=n.float()), lambda: M.diff_attention(q, k, v, lam, lengths=n[:1]),
+                lambda: M.diff_attention(q, k, v, lam, starts=n.view(1, 2)), lambda: M.diff_attention(q, k, v, lam, starts=n.to("meta")),
+                lambda: M.diff_attention(q, k.to("meta"), v, lam)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+class Strides(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("b", ctypes.c_int64), ("t", ctypes.c_int64), ("h", ctypes.c_int64)]
+
+
+class Shape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("b", "tq", "tk", "h", "hk", "dh", "dv")] + [("causal", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+def test_attention_argument_checks_before_launch():
+    L, p, ref = M.LIB, 4096, ctypes.byref
+
+    def fwd(dtype=1, q=(p, 512, 512, 64), lam=p, out=p, second=None, lse=None, scratch=p, **s):
+        sizes = {"b": 1, "tq": 8, "tk": 8, "h": 2, "hk": 1, "dh": 64, "dv": 128, "causal": 1, "scale": 0.125, **s}
+        k, v, lm = Strides(p, 1024, 128, 64), Strides(p, 1024, 128, 128), Strides(lam, 0, 0, 0)
+        return L.lmo_diff_attn_fwd(ref(Strides(*q)), ref(k), ref(v), ref(lm), 1, None, None, out, second, lse, scratch, ref(Shape(**sizes)),
+                                   dtype, None)
+
+    assert fwd(b=0) == 0 and fwd(tq=0) == 0
+    assert fwd(dtype=0) == -4 and fwd(dtype=3) == -4
+    for s in ({"dh": 0}, {"dh": 12}, {"dh": 136}, {"dv": 264}, {"dv": 4}):
+        assert fwd(**s) == -2, s
+    for s in ({"tk": 0}, {"hk": 0}, {"h": 3, "hk": 2}, {"h": 1, "hk": 2}, {"scale": 0.0}, {"scale": math.inf}, {"scale": math.nan}, {"tq": 2 ** 30},
+              {"tk": 2 ** 30}, {"b": 2 ** 23}, {"b": -1}, {"lam": None}, {"out": None}, {"second": p}, {"lse": p}, {"q": (None, 512, 512, 64)}):
+        assert fwd(**s) == -1, s
+    for q in ((p + 8, 512, 512, 64), (p, 512, 516, 64), (p, 4, 512, 64), (p, 512, 512, 60)):
+        assert fwd(q=q) == -3
+    assert fwd(q=(p, 512, 2 ** 24, 64)) == -2 and fwd(q=(p, -512, 512, 64)) == -2
+    assert fwd(out=p + 2) == -3
+    few = Shape(1, 1, 100000, 2, 1, 64, 128, 1, 0.125)
+    assert L.lmo_diff_attn_scratch(ref(few), 0) > 0 and L.lmo_diff_attn_scratch(ref(few), 1) == 0
+    assert fwd(tq=1, tk=100000, scratch=None) == -1
+    s = Strides(p, 1024, 128, 64)
+    assert L.lmo_diff_attn_bwd(ref(s), ref(s), ref(s), ref(s), 1, None, None, p, p, p, p, p, p, None, None, 0, p, ref(few), 1, None) == -1
+    assert L.lmo_diff_attn_bwd(ref(s), ref(s), ref(s), ref(s), 1, None, None, p, p, p, p, p, p, p, p, 7, p, ref(few), 1, None) == -1
