@@ -53,8 +53,14 @@ template <> struct Mat<bf16_t> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
+struct F16Pair : F16Cvt {   // both at once; a multiplication that goes into the conversion rounds once instead of twice
+  static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+  }
+};
 template <> struct Mat<_Float16> {
-  typedef F16Cvt Cvt;
+  typedef F16Pair Cvt;
   static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -92,70 +98,94 @@ __device__ __forceinline__ int row_of(int r, int h) { return 4 * h + (r & 3) + 8
 // ---------------------------------------------------------------------------------------------------------------
 // rows in LDS, of W elements (64, 128 or 256) in pieces of 16 bytes, piece p of row r in place p ^ swizzle(r). What reads them
 // together then meets in no bank (64 of 4 bytes): 16 rows at one piece; four rows, aligned, at four pieces; eight at two.
-// Each lane's offsets are formed once; what is added to them in the loops is known at compile time.
+// Addresses are bytes from the start of LDS (a kernel has one block of it): a few offsets of a lane, formed once, and what is
+// known at compile time, which goes into the instruction. (Arrays of their own cost an address register for each of them and
+// each offset: 100 spilled registers in the kernel of dk and dv.)
 // ---------------------------------------------------------------------------------------------------------------
 template <int W> __device__ __forceinline__ int swizzle(int r) {
   return (W == 64 ? (r >> 1 & 1) << 2 : (r & 1) << 3 | (r >> 1 & 1) << 2) | (r >> 2 & 1) << 1 | (r >> 3 & 1);
 }
-typedef __attribute__((address_space(3))) s16x4* lds4;
-__device__ __forceinline__ uint4 four_and_four(const void* p, const void* q) {   // a column's elements of two times four rows
-  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(const_cast<void*>(p)));
-  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(const_cast<void*>(q)));
+__device__ __forceinline__ int kept(int x) {   // held as it is, not formed again from what it was formed from
+  asm volatile("" : "+v"(x));
+  return x;
+}
+template <typename V> __device__ __forceinline__ V lds_at(int at) { return *reinterpret_cast<__attribute__((address_space(3))) const V*>(at); }
+__device__ __forceinline__ uint4 sixteen(int at) { return __builtin_bit_cast(uint4, lds_at<u32x4>(at)); }
+__device__ __forceinline__ uint4 four_and_four(int p, int q) {   // a column's elements of two times four rows
+  typedef __attribute__((address_space(3))) s16x4* lds4;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4>(p));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds4>(q));
   const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
   return make_uint4(ua.x, ua.y, ub.x, ub.y);
 }
 // operands of v_mfma_f32_32x32x16
-template <typename T, int W> struct Rows32 {   // A: rows r0 + l mod 32, columns 16 ks + 8 (l / 32) .. + 8
-  int o[8];
+template <int W> struct Rows32 {   // A: rows r0 + l mod 32, columns 16 ks + 8 (l / 32) .. + 8
+  int o[W == 64 ? 4 : 8];
   __device__ __forceinline__ Rows32() {
     const int lane = (int)threadIdx.x & 63, r = lane & 31;
 #pragma unroll
-    for (int v = 0; v < 8; ++v) o[v] = r * W + 8 * ((2 * v) ^ ((lane >> 5) ^ swizzle<W>(r)));
+    for (int v = 0; v < (W == 64 ? 4 : 8); ++v) o[v] = kept(2 * (r * W + 8 * ((2 * v) ^ ((lane >> 5) ^ swizzle<W>(r)))));
   }
-  __device__ __forceinline__ uint4 at(const T* tile, int r0, int ks) const {   // r0 a multiple of 32
-    return *reinterpret_cast<const uint4*>(tile + o[W == 64 ? ks & 3 : ks & 7] + r0 * W + 128 * (ks >> 3));
+  __device__ __forceinline__ uint4 at(int tile, int r0, int ks) const {   // r0 a multiple of 32
+    return sixteen(o[W == 64 ? ks & 3 : ks & 7] + tile + 2 * (r0 * W + 128 * (ks >> 3)));
   }
 };
-template <typename T, int W> struct Cols32 {   // A: columns c0 + l mod 32, rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}, h = l / 32
-  int o[4], p[4];
+template <int W> struct Cols32 {   // A: columns c0 + l mod 32, rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}, h = l / 32
+  static constexpr int V = W == 64 ? 2 : 4;
+  int o[V], p[V];
   __device__ __forceinline__ Cols32() {
     const int lane = (int)threadIdx.x & 63, j = lane & 15, r = 4 * (lane >> 5) + (j >> 2);
     const int piece = (lane >> 4 & 1) * 2 + ((j & 3) >> 1), half = 4 * (j & 1);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      o[v] = r * W + 8 * ((4 * v) ^ (piece ^ swizzle<W>(r))) + half;
-      p[v] = (r + 8) * W + 8 * ((4 * v) ^ (piece ^ swizzle<W>(r + 8))) + half;
+    for (int v = 0; v < V; ++v) {
+      o[v] = kept(2 * (r * W + 8 * ((4 * v) ^ (piece ^ swizzle<W>(r))) + half));
+      p[v] = kept(2 * ((r + 8) * W + 8 * ((4 * v) ^ (piece ^ swizzle<W>(r + 8))) + half));
     }
   }
-  __device__ __forceinline__ uint4 at(const T* tile, int r0, int c0) const {   // r0 a multiple of 16, c0 of 32
-    const int v = (c0 >> 5) & (W == 64 ? 1 : 3), more = r0 * W + 128 * (c0 >> 7);
-    return four_and_four(tile + o[v] + more, tile + p[v] + more);
+  __device__ __forceinline__ uint4 at(int tile, int r0, int c0) const {   // r0 a multiple of 16, c0 of 32
+    const int v = (c0 >> 5) & (V - 1), more = tile + 2 * (r0 * W + 128 * (c0 >> 7));
+    return four_and_four(o[v] + more, p[v] + more);
   }
 };
 // operands of v_mfma_f32_16x16x32
-template <typename T, int W> struct Rows16 {   // A: rows r0 + l mod 16, columns 32 ks + 8 (l / 16) .. + 8
-  int o[4];
+template <int W> struct Rows16 {   // A: rows r0 + l mod 16, columns 32 ks + 8 (l / 16) .. + 8
+  int o[W == 64 ? 2 : 4];
   __device__ __forceinline__ Rows16() {
     const int lane = (int)threadIdx.x & 63, r = lane & 15;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) o[v] = r * W + 8 * ((4 * v) ^ ((lane >> 4) ^ swizzle<W>(r)));
+    for (int v = 0; v < (W == 64 ? 2 : 4); ++v) o[v] = kept(2 * (r * W + 8 * ((4 * v) ^ ((lane >> 4) ^ swizzle<W>(r)))));
   }
-  __device__ __forceinline__ uint4 at(const T* tile, int r0, int ks) const {   // r0 a multiple of 16
-    return *reinterpret_cast<const uint4*>(tile + o[W == 64 ? ks & 1 : ks & 3] + r0 * W + 128 * (ks >> 2));
+  __device__ __forceinline__ uint4 at(int tile, int r0, int ks) const {   // r0 a multiple of 16
+    return sixteen(o[W == 64 ? ks & 1 : ks & 3] + tile + 2 * (r0 * W + 128 * (ks >> 2)));
   }
 };
-template <typename T, int W> struct Cols16 {   // A: columns c0 + l mod 16, rows r0 + {4 g + 0..3, 16 + 4 g + 0..3}, g = l / 16
-  int o[8];
+template <int W> struct Cols16 {   // A: columns c0 + l mod 16, rows r0 + {4 g + 0..3, 16 + 4 g + 0..3}, g = l / 16
+  int o[W == 64 ? 4 : 8];
   __device__ __forceinline__ Cols16() {
     const int lane = (int)threadIdx.x & 63, j = lane & 15, r = 4 * (lane >> 4) + (j >> 2);
 #pragma unroll
-    for (int v = 0; v < 8; ++v) o[v] = r * W + 8 * ((2 * v) ^ (((j & 3) >> 1) ^ swizzle<W>(r))) + 4 * (j & 1);
+    for (int v = 0; v < (W == 64 ? 4 : 8); ++v) o[v] = kept(2 * (r * W + 8 * ((2 * v) ^ (((j & 3) >> 1) ^ swizzle<W>(r))) + 4 * (j & 1)));
   }
-  __device__ __forceinline__ uint4 at(const T* tile, int r0, int c0) const {   // r0 a multiple of 32, c0 of 16
-    const T* p = tile + o[(c0 >> 4) & (W == 64 ? 3 : 7)] + r0 * W + 128 * (c0 >> 7);
-    return four_and_four(p, p + 16 * W);
+  __device__ __forceinline__ uint4 at(int tile, int r0, int c0) const {   // r0 a multiple of 32, c0 of 16
+    const int p = o[(c0 >> 4) & (W == 64 ? 3 : 7)] + tile + 2 * (r0 * W + 128 * (c0 >> 7));
+    return four_and_four(p, p + 32 * W);
   }
 };
+
+// the offsets for rows of W elements: the given ones, where they are
+template <template <int> class R, int W, typename O> __device__ __forceinline__ auto of_width(const O& given) {
+  if constexpr (std::is_same<O, R<W>>::value) return given;
+  else return R<W>();
+}
+
+// 16 bytes (or 4) of memory for each lane, at base + off, to LDS at `to` and what follows it in the lanes' order. In assembly:
+// the compiler would wait for it before any read of LDS, of the other buffer too. The data is there past filled().
+__device__ __forceinline__ void load_lds16(const void* base, uint32_t off, int to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds4(const void* base, uint32_t off, int to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
 
 // Fills N rows of LDS from memory by LANES lanes (whole waves). MAPS rows of memory of W / MAPS elements (`width` of them
 // exist, the columns past them repeat the first piece: what they meet is zero) lie side by side in a row of LDS. Rows past
@@ -174,23 +204,19 @@ template <typename T, int W, int MAPS, int N, int LANES> struct Fill {
   __device__ __forceinline__ Fill(const T* base_, int64_t stride_, int64_t map_stride, int width) : base(base_), stride(stride_) {
     const int lane = (int)threadIdx.x % LANES;
 #pragma unroll
-    for (int v = 0; v < VAR; ++v) off[v] = 2u * ((uint32_t)(lane / P) * (uint32_t)stride + col(lane, v, map_stride, width));
+    for (int v = 0; v < VAR; ++v) off[v] = (uint32_t)kept(2u * ((uint32_t)(lane / P) * (uint32_t)stride + col(lane, v, map_stride, width)));
   }
-  __device__ __forceinline__ void fetch(int row0, int last, T* lds) const {   // asynchronous: done when vmcnt says so
-    const int wave = LANES == 64 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x % LANES) >> 6);
-    const bool whole = row0 + N - 1 <= last;
-    int r = (int)(threadIdx.x % LANES) / P;
-    if (!whole) asm volatile("" : "+v"(r));   // formed here, where it is rarely needed
+  __device__ __forceinline__ void fetch(int row0, int last, int to) const {   // asynchronous: done when vmcnt says so
+    to += LANES == 64 ? 0 : 1024 * __builtin_amdgcn_readfirstlane((int)(threadIdx.x % LANES) >> 6);
+    const char* b = reinterpret_cast<const char*>(base + (int64_t)row0 * stride);
+    if (row0 + N - 1 <= last) {
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const char* b = reinterpret_cast<const char*>(base + (int64_t)(row0 + ROWS * i) * stride);
-      lds_void* to = (lds_void*)(lds + 8 * (i * LANES + wave * 64));
-      if (whole) {
-        __builtin_amdgcn_global_load_lds((global_void*)(b + off[i % VAR]), to, 16, 0, 0);
-      } else {
-        const int64_t back = max(row0 + ROWS * i + r - last, 0) * (2 * stride);
-        __builtin_amdgcn_global_load_lds((global_void*)(b + off[i % VAR] - back), to, 16, 0, 0);
-      }
+      for (int i = 0; i < PASSES; ++i) load_lds16(b + 2 * i * ROWS * stride, off[i % VAR], to + 16 * i * LANES);
+    } else {
+      const int r = kept((int)(threadIdx.x % LANES) / P);   // formed here, where it is rarely needed, and not kept
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+        load_lds16(b, off[i % VAR] + 2u * (uint32_t)(min(r + ROWS * i, last - row0) - r) * (uint32_t)stride, to + 16 * i * LANES);
     }
   }
 };
@@ -212,8 +238,8 @@ struct Diff {
   // backward
   const void* dy;
   void *dq, *dk, *dval;
-  float *delta, *dlam;           // [2][b h][tq], and dlam's parts
-  int dlam_rows;                 // dlam per query, else per workgroup
+  float *delta, *dlam;           // D1, D2 and, where lam has queries, lam [b h][tq]; dlam's parts
+  int lam_rows;                  // lam has queries; dlam is per query, else per workgroup
   // a split of the keys
   int splits, chunk;
   float* part;
@@ -309,10 +335,9 @@ template <int DH, int DV> constexpr int waves_fwd() { return DH + DV <= 192 ? 2 
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int DH, int DV>
 __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_fwd(const Diff a) {
-  extern __shared__ __align__(16) char lds[];
   constexpr int KT = TILE * 2 * DH, VT = TILE * DV, DB = DV / 32;
-  T* s_k = reinterpret_cast<T*>(lds);
-  T* s_v = s_k + 2 * KT;
+  extern __shared__ __align__(16) char lds_block[];   // two tiles of keys, two of values
+  constexpr int K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT;
   const int lane = (int)threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int groups = a.h / a.hk, blocks = (a.tq + QB - 1) / QB;
@@ -328,8 +353,8 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
   const int seen = seen_by(a, qrow, start, len);
   const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len);             // of the workgroup's queries
   const int wmost = w0 < a.tq ? seen_by(a, min(w0 + 32, a.tq) - 1, start, len) : 0, wleast = seen_by(a, min(w0, a.tq - 1), start, len);
-  const Rows32<T, 2 * DH> krows;
-  const Cols32<T, DV> vcols;
+  const Rows32<2 * DH> krows;
+  const Cols32<DV> vcols;
   f32x16 o1[DB], o2[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) o1[d] = o2[d] = zero16();
@@ -338,20 +363,20 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
   const Fill<T, 2 * DH, 2, TILE, WG> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
   const Fill<T, DV, 1, TILE, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
   if (ntiles > 0) {
-    kf.fetch(0, len - 1, s_k);
-    vf.fetch(0, len - 1, s_v);
-    filled();
+    kf.fetch(0, len - 1, K0);
+    vf.fetch(0, len - 1, V0);
   }
+  filled();   // in every case: a wait for what was loaded above, left to the loop, would wait there for the tiles too
   auto tile = [&](int j, auto buffer) {
     constexpr int cur = decltype(buffer)::value;   // known: the buffers' offsets go into the reads' own
     const int k0 = j * TILE;
     if (j + 1 < ntiles) {   // the other buffer's readers are past the barrier below
-      kf.fetch(k0 + TILE, len - 1, s_k + (cur ^ 1) * KT);
-      vf.fetch(k0 + TILE, len - 1, s_v + (cur ^ 1) * VT);
+      kf.fetch(k0 + TILE, len - 1, cur ? K0 : K1);
+      vf.fetch(k0 + TILE, len - 1, cur ? V0 : V1);
     }
     if (k0 < wmost) {
-      const T* kt = s_k + cur * KT;
-      const T* vt = s_v + cur * VT;
+      constexpr int kt = cur ? K1 : K0;
+      constexpr int vt = cur ? V1 : V0;
       uint4 p1[4], p2[4];
       auto scores = [&](int map, f32x16 (&s)[2]) {
 #pragma unroll
@@ -460,15 +485,14 @@ __device__ __forceinline__ void join_row(At at, int n, int col, float& y1, float
 
 template <typename T, int DH, int DV>
 __global__ __launch_bounds__((64 * few_waves<DH, DV>())) __attribute__((amdgpu_waves_per_eu(1))) void k_diff_few(const Diff a) {
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(16) char lds_block[];
   constexpr int WAVES = few_waves<DH, DV>(), KT = FEW * 2 * DH, VT = FEW * DV, DB = DV / 32, ROW = few_row<DV>();
   const int lane = (int)threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int groups = a.h / a.hk, rows = a.tq * groups;
   const int item = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - item * a.splits, b = item / a.hk, hk = item - b * a.hk;
   const int len = length_of(a, b), start = start_of(a, b);
-  T* s_k = reinterpret_cast<T*>(lds) + wave * 2 * (KT + VT);
-  T* s_v = s_k + 2 * KT;
+  const int s_k = wave * 4 * (KT + VT), s_v = s_k + 4 * KT;   // the wave's two tiles of keys, and of values
   const int row = min(lane & 31, rows - 1), query = row / groups, head = hk * groups + row - query * groups;
   const T* qp = static_cast<const T*>(a.q.p) + b * a.q.b + query * a.q.t + 2 * head * a.q.h;
   Kept<T, DH> q[2];
@@ -476,8 +500,8 @@ __global__ __launch_bounds__((64 * few_waves<DH, DV>())) __attribute__((amdgpu_w
   q[1].load(qp + a.q.h, a.dh);
   const int seen = seen_by(a, query, start, len);
   const int c0 = split * a.chunk, c1 = min(c0 + a.chunk, seen_by(a, a.tq - 1, start, len)), least = seen_by(a, 0, start, len);
-  const Rows32<T, 2 * DH> krows;
-  const Cols32<T, DV> vcols;
+  const Rows32<2 * DH> krows;
+  const Cols32<DV> vcols;
   f32x16 o1[DB], o2[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) o1[d] = o2[d] = zero16();
@@ -494,15 +518,14 @@ __global__ __launch_bounds__((64 * few_waves<DH, DV>())) __attribute__((amdgpu_w
   int cur = 0;
   for (int k0 = first; k0 < c1; k0 += step, cur ^= 1) {
     if (k0 + step < c1) {
-      kf.fetch(k0 + step, len - 1, s_k + (cur ^ 1) * KT);
-      vf.fetch(k0 + step, len - 1, s_v + (cur ^ 1) * VT);
+      kf.fetch(k0 + step, len - 1, s_k + (cur ^ 1) * 2 * KT);
+      vf.fetch(k0 + step, len - 1, s_v + (cur ^ 1) * 2 * VT);
       __builtin_amdgcn_s_waitcnt(0x0f70 | (LOADS & 15) | (LOADS >> 4 << 14));   // vmcnt: all but the next tile's loads
     } else {
       __builtin_amdgcn_s_waitcnt(0x0f70);
     }
     wave_lds_sync();
-    const T* kt = s_k + cur * KT;
-    const T* vt = s_v + cur * VT;
+    const int kt = s_k + cur * 2 * KT, vt = s_v + cur * 2 * VT;
     uint4 p1[2], p2[2];
     auto scores = [&](int map, f32x16 (&s)[1]) {
       s[0] = zero16();
@@ -532,7 +555,7 @@ __global__ __launch_bounds__((64 * few_waves<DH, DV>())) __attribute__((amdgpu_w
   }
   const float l1 = other_half(sm1.l, true), l2 = other_half(sm2.l, true);
   __syncthreads();
-  float* part = reinterpret_cast<float*>(lds);   // [wave][32 rows][ROW]
+  float* part = reinterpret_cast<float*>(lds_block);   // [wave][32 rows][ROW]
   static_assert(few_waves<DH, DV>() * FEW * few_row<DV>() * 4 <= 160 * 1024 && few_lds<DH, DV>() <= 160 * 1024,
                 "the tiles, and the waves' results, in LDS");
   if ((lane & 31) < rows) {
@@ -595,11 +618,9 @@ template <typename T, int DV> __global__ __launch_bounds__(DV) void k_diff_join(
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int DH, int DV>
 __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_bwd_q(const Diff a) {
-  extern __shared__ __align__(16) char lds[];
-  __shared__ float s_dlam[4];
   constexpr int KT = TILE * 2 * DH, VT = TILE * DV, QB_ = DH / 32;
-  T* s_k = reinterpret_cast<T*>(lds);
-  T* s_v = s_k + 2 * KT;
+  extern __shared__ __align__(16) char lds_block[];   // two tiles of keys, two of values; four floats
+  constexpr int K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT;
   const int lane = (int)threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int groups = a.h / a.hk, blocks = (a.tq + QB - 1) / QB;
@@ -639,13 +660,14 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
   if (query < a.tq && half == 0) {
     a.delta[n] = d1;
     a.delta[n + all] = d2;
+    if (a.lam_rows) a.delta[n + 2 * all] = lam;   // as fp32, for the kernel below
   }
   const int seen = seen_by(a, qrow, start, len);
   const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len);
   const int wmost = w0 < a.tq ? seen_by(a, min(w0 + 32, a.tq) - 1, start, len) : 0, wleast = seen_by(a, min(w0, a.tq - 1), start, len);
-  const Rows32<T, 2 * DH> krows;
-  const Rows32<T, DV> vrows;
-  const Cols32<T, 2 * DH> kcols;
+  const Rows32<2 * DH> krows;
+  const auto vrows = of_width<Rows32, DV>(krows);
+  const Cols32<2 * DH> kcols;
   f32x16 dq[2][QB_];
 #pragma unroll
   for (int d = 0; d < QB_; ++d) dq[0][d] = dq[1][d] = zero16();
@@ -654,20 +676,20 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
   const Fill<T, 2 * DH, 2, TILE, WG> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
   const Fill<T, DV, 1, TILE, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
   if (ntiles > 0) {
-    kf.fetch(0, len - 1, s_k);
-    vf.fetch(0, len - 1, s_v);
-    filled();
+    kf.fetch(0, len - 1, K0);
+    vf.fetch(0, len - 1, V0);
   }
+  filled();   // in every case: a wait for what was loaded above, left to the loop, would wait there for the tiles too
   auto tile = [&](int j, auto buffer) {
     constexpr int cur = decltype(buffer)::value;   // known: the buffers' offsets go into the reads' own
     const int k0 = j * TILE;
     if (j + 1 < ntiles) {
-      kf.fetch(k0 + TILE, len - 1, s_k + (cur ^ 1) * KT);
-      vf.fetch(k0 + TILE, len - 1, s_v + (cur ^ 1) * VT);
+      kf.fetch(k0 + TILE, len - 1, cur ? K0 : K1);
+      vf.fetch(k0 + TILE, len - 1, cur ? V0 : V1);
     }
     if (k0 < wmost) {
-      const T* kt = s_k + cur * KT;
-      const T* vt = s_v + cur * VT;
+      constexpr int kt = cur ? K1 : K0;
+      constexpr int vt = cur ? V1 : V0;
       const bool edge = k0 + TILE > wleast;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -731,11 +753,13 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
   }
   if (!a.dlam) return;
   dlam = query < a.tq ? -other_half(dlam, true) : 0.f;
-  if (a.dlam_rows) {
+  if (a.lam_rows) {
     if (query < a.tq && half == 0) a.dlam[((int64_t)b * a.tq + query) * a.h + head] = dlam;
     return;
   }
   dlam = lanes_reduce(dlam, 32, AddOp());
+  float* s_dlam = reinterpret_cast<float*>(lds_block);
+  __syncthreads();   // the last tile has been read
   if (lane == 0) s_dlam[wave] = dlam;
   __syncthreads();
   if (threadIdx.x == 0) a.dlam[(int64_t)head * (a.b * blocks) + b * blocks + qblock] = (s_dlam[0] + s_dlam[1]) + (s_dlam[2] + s_dlam[3]);
@@ -765,6 +789,7 @@ template <typename T> __global__ __launch_bounds__(WG) void k_diff_dlam(const fl
 // another. Here the scores' rows are queries, whose four or five numbers come from LDS for every row a lane has: by
 // v_mfma_f32_16x16x32 a lane has 4 of 16 rows, not 16 of 32, and half as much is read for them, and held.
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int KVT = 32;   // queries of a tile
 template <typename T, int W> struct Kept16 {   // a wave's 32 rows as B operands: row 16 n + l mod 16, columns 32 ks + 8 (l / 16) .. + 8
   uint4 f[2][W / 32];
   __device__ __forceinline__ void load(int n, const T* row, int width, bool there) {   // zeros past `width`, and for no row
@@ -779,11 +804,10 @@ template <typename T, int W> struct Kept16 {   // a wave's 32 rows as B operands
 
 template <typename T, int DH, int DV, bool TOKEN>   // TOKEN: lam differs between queries
 __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_bwd_kv(const Diff a) {
-  extern __shared__ __align__(16) char lds[];
-  constexpr int QT = TILE * 2 * DH, GT = TILE * DV, KB = DH / 16, VB = DV / 16, NUMBERS = TOKEN ? 5 : 4;
-  T* s_q = reinterpret_cast<T*>(lds);
-  T* s_g = s_q + 2 * QT;
-  float* s_row = reinterpret_cast<float*>(s_g + 2 * GT);   // [2 buffers][lse1, lse2, D1, D2, lam][64]
+  extern __shared__ __align__(16) char lds_block[];
+  constexpr int QT = KVT * 2 * DH, GT = KVT * DV, KB = DH / 16, VB = DV / 16, NUMBERS = TOKEN ? 5 : 4;
+  // two tiles of queries and of dy, this workgroup's values, and twice lse1, lse2, D1, D2, lam of the tile's queries
+  constexpr int Q0 = 0, Q1 = 2 * QT, G0 = 4 * QT, G1 = 4 * QT + 2 * GT, VALUES = 4 * (QT + GT), R0 = VALUES + 2 * QB * DV, R1 = R0 + 4 * NUMBERS * KVT;
   const int tid = (int)threadIdx.x, lane = tid & 63, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = a.h / a.hk, blocks = (a.tk + QB - 1) / QB;
@@ -793,7 +817,6 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
   const int len = length_of(a, b), start = start_of(a, b);
   const int w0 = kb + 32 * wave;
   Kept16<T, DH> k[2];
-  Kept16<T, DV> v;
   int from[2];   // the first query that sees the lane's keys
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -802,13 +825,12 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
     const T* kp = static_cast<const T*>(a.k.p) + b * a.k.b + krow * a.k.t + 2 * hk * a.k.h;
     k[0].load(n, kp, a.dh, there);
     k[1].load(n, kp + a.k.h, a.dh, there);
-    v.load(n, static_cast<const T*>(a.v.p) + b * a.v.b + krow * a.v.t + hk * a.v.h, a.dv, there);
     from[n] = !there ? 0x7fffffff : a.causal ? max(key - start, 0) : 0;
   }
-  const Rows16<T, 2 * DH> qrows;
-  const Rows16<T, DV> grows;
-  const Cols16<T, 2 * DH> qcols;
-  const Cols16<T, DV> gcols;
+  const Rows16<2 * DH> qrows;
+  const Cols16<2 * DH> qcols;
+  const auto grows = of_width<Rows16, DV>(qrows);
+  const auto gcols = of_width<Cols16, DV>(qcols);
   f32x4 dk[2][KB][2], dv[VB][2];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -818,115 +840,139 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
     for (int d = 0; d < VB; ++d) dv[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   // the first query that sees the workgroup's first key
-  const int first_q = a.causal ? max(kb - start, 0) : 0, first = first_q / TILE;
-  const int ntiles = kb < len && first_q < a.tq ? (a.tq + TILE - 1) / TILE - first : 0, total = ntiles * groups;
+  const int first_q = a.causal ? max(kb - start, 0) : 0, first = first_q / KVT;
+  const int ntiles = kb < len && first_q < a.tq ? (a.tq + KVT - 1) / KVT - first : 0, total = ntiles * groups;
   const int64_t all = (int64_t)a.b * a.h * a.tq;
   const T* qbase = static_cast<const T*>(a.q.p) + b * a.q.b + 2 * hk * groups * a.q.h;
   const T* gbase = static_cast<const T*>(a.dy) + ((int64_t)b * a.tq * a.h + hk * groups) * a.dv;
-  Fill<T, 2 * DH, 2, TILE, WG> qf(qbase, a.q.t, a.q.h, a.dh);
-  Fill<T, DV, 1, TILE, WG> gf(gbase, (int64_t)a.h * a.dv, 0, a.dv);
-  auto fetch = [&](int row0, int head, int buf) {   // a tile of one of the group's heads
+  Fill<T, 2 * DH, 2, KVT, WG> qf(qbase, a.q.t, a.q.h, a.dh);
+  Fill<T, DV, 1, KVT, WG> gf(gbase, (int64_t)a.h * a.dv, 0, a.dv);
+  auto fetch = [&](int row0, int head, int s_q, int s_g, int s_row) {   // a tile of one of the group's heads
     qf.base = qbase + 2 * head * a.q.h;
     gf.base = gbase + head * a.dv;
-    qf.fetch(row0, a.tq - 1, s_q + buf * QT);
-    gf.fetch(row0, a.tq - 1, s_g + buf * GT);
-    const int t = min(row0 + lane, a.tq - 1);
-    const int64_t n = ((int64_t)b * a.h + hk * groups + head) * a.tq + t;
-    float* o = s_row + buf * 5 * TILE;
-    o[tid] = wave == 0 ? a.lse[n] : wave == 1 ? a.lse[n + all] : wave == 2 ? a.delta[n] : a.delta[n + all];
-    if (TOKEN && wave == 0) o[4 * TILE + lane] = lam_at<T>(a, b, t, hk * groups + head);
+    qf.fetch(row0, a.tq - 1, s_q);
+    gf.fetch(row0, a.tq - 1, s_g);
+    // a wave loads 32 of two of the numbers
+    const int64_t n = ((int64_t)b * a.h + hk * groups + head) * a.tq + row0;
+    const uint32_t row = 4u * (uint32_t)min(lane & 31, a.tq - 1 - row0);
+    if (wave < 2) {
+      const float* of = (wave ? a.delta : a.lse) + n;
+      load_lds4(of, row + (lane & 32 ? (uint32_t)(4 * all) : 0u), s_row + wave * 8 * KVT);
+    }
+    if (TOKEN && wave == 2 && lane < 32) load_lds4(a.delta + n + 2 * all, row, s_row + 16 * KVT);
   };
+  Rows16<DV> vrows;   // of the wave's keys
+#pragma unroll
+  for (int e = 0; e < (DV == 64 ? 2 : 4); ++e) vrows.o[e] = kept(vrows.o[e] + wave * 64 * DV);
+  const int numbers = kept(16 * grp);
   if (total > 0) {
-    fetch(first * TILE, 0, 0);
-    filled();
+    const Fill<T, DV, 1, QB, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
+    vf.fetch(kb, len - 1, VALUES);
+    fetch(first * KVT, 0, Q0, G0, R0);
+  }
+  filled();
+  if (a.dv < DV) {   // the values' columns past the last repeat some, as dy's do: zeros in their place
+    for (int i = tid; i < QB * (DV / 8); i += WG) {
+      const int r = i / (DV / 8), p = i % (DV / 8);
+      if (8 * p >= a.dv) *reinterpret_cast<uint4*>(lds_block + VALUES + 2 * (r * DV + 8 * (p ^ swizzle<DV>(r)))) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __syncthreads();
   }
   int at = first, head = 0;
   auto tile = [&](int it, auto buffer) {
     constexpr int cur = decltype(buffer)::value;
-    const int q0 = at * TILE;
+    const int q0 = at * KVT;
     const float lam = TOKEN ? 0.f : lam_at<T>(a, b, 0, hk * groups + head);
     if (++at == first + ntiles) {
       at = first;
       ++head;
     }
-    if (it + 1 < total) fetch(at * TILE, head, cur ^ 1);
+    if (it + 1 < total) fetch(at * KVT, head, cur ? Q0 : Q1, cur ? G0 : G1, cur ? R0 : R1);
     // the keys that the tile's last and first queries see: whether any of this wave's is among them, and whether all are
-    if (w0 < seen_by(a, min(q0 + TILE, a.tq) - 1, start, len)) {
-      const T* qt = s_q + cur * QT;
-      const T* gt = s_g + cur * GT;
-      const float* sr = s_row + cur * 5 * TILE + 4 * grp;
-      const bool edge = w0 + 32 > seen_by(a, q0, start, len) || q0 + TILE > a.tq;
+    if (w0 < seen_by(a, min(q0 + KVT, a.tq) - 1, start, len)) {
+      constexpr int qt = cur ? Q1 : Q0, gt = cur ? G1 : G0, rt = cur ? R1 : R0;
+      const bool edge = w0 + 32 > seen_by(a, q0, start, len) || q0 + KVT > a.tq;
+      uint2 pd[2][2], p1[2][2], p2[2][2];   // [16 queries][16 keys]: P1 - lam P2, dS1, dS2
+      f32x4 da[2][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint2 pd[2][2], p1[2][2], p2[2][2];   // [16 queries][16 keys]: P1 - lam P2, dS1, dS2
+      for (int u = 0; u < 2; ++u) da[u][0] = da[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r0 = 32 * i + 16 * u;
-          f32x4 da[2], s1[2], s2[2];
-          in_order();
+      for (int ks = 0; ks < DV / 32; ++ks) {
+        uint4 x[2], y[2];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) da[n] = s1[n] = s2[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int ks = 0; ks < DV / 32; ++ks) {
-            if (ks % 2 == 0) in_order();
-            const uint4 x = grows.at(gt, r0, ks);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) da[n] = Mat<T>::mfma16(x, v.f[n][ks], da[n]);
-          }
-#pragma unroll
-          for (int ks = 0; ks < DH / 32; ++ks) {
-            const uint4 x = qrows.at(qt, r0, ks), y = qrows.at(qt, r0, DH / 32 + ks);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              s1[n] = Mat<T>::mfma16(x, k[0].f[n][ks], s1[n]);
-              s2[n] = Mat<T>::mfma16(y, k[1].f[n][ks], s2[n]);
-            }
-          }
-          in_order();
-          if (edge) {
-            const int here = q0 + 4 * grp, left = a.tq - here;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (r0 + r >= left || here + r0 + r < from[n]) s1[n][r] = s2[n][r] = -INFINITY;
-          }
-          f32x4 x[NUMBERS];
-#pragma unroll
-          for (int e = 0; e < NUMBERS; ++e) x[e] = *reinterpret_cast<const f32x4*>(sr + e * TILE + r0);
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float q1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[n][r], a.c, -x[0][r]));
-              const float q2 = (TOKEN ? x[NUMBERS - 1][r] : lam) * __builtin_amdgcn_exp2f(__builtin_fmaf(s2[n][r], a.c, -x[1][r]));
-              s1[n][r] = q1 * (da[n][r] - x[2][r]);
-              s2[n][r] = q2 * (x[3][r] - da[n][r]);
-              da[n][r] = q1 - q2;
-            }
-            pd[u][n] = packed4<T>(da[n]);
-            p1[u][n] = packed4<T>(s1[n]);
-            p2[u][n] = packed4<T>(s2[n]);
-          }
-        }
-        in_order();
-        auto both = [](const uint2 (&p)[2][2], int n) { return make_uint4(p[0][n].x, p[0][n].y, p[1][n].x, p[1][n].y); };
-#pragma unroll
-        for (int d = 0; d < VB; ++d) {
-          if (d % 2 == 0) in_order();
-          const uint4 x = gcols.at(gt, 32 * i, 16 * d);
-#pragma unroll
-          for (int n = 0; n < 2; ++n) dv[d][n] = Mat<T>::mfma16(x, both(pd, n), dv[d][n]);
+        for (int e = 0; e < 2; ++e) {
+          x[e] = grows.at(gt, 16 * e, ks);
+          y[e] = vrows.at(VALUES, 16 * e, ks);
         }
 #pragma unroll
-        for (int d = 0; d < KB; ++d) {
-          in_order();
-          const uint4 x = qcols.at(qt, 32 * i, 16 * d), y = qcols.at(qt, 32 * i, DH + 16 * d);
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) da[u][n] = Mat<T>::mfma16(x[u], y[n], da[u][n]);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r0 = 16 * u;
+        f32x4 s1[2], s2[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) s1[n] = s2[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < DH / 32; ++ks) {
+          const uint4 x = qrows.at(qt, r0, ks), y = qrows.at(qt, r0, DH / 32 + ks);
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            dk[0][d][n] = Mat<T>::mfma16(x, both(p1, n), dk[0][d][n]);
-            dk[1][d][n] = Mat<T>::mfma16(y, both(p2, n), dk[1][d][n]);
+            s1[n] = Mat<T>::mfma16(x, k[0].f[n][ks], s1[n]);
+            s2[n] = Mat<T>::mfma16(y, k[1].f[n][ks], s2[n]);
           }
+        }
+        if (edge) {
+          const int here = q0 + 4 * grp, left = a.tq - here;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r0 + r >= left || here + r0 + r < from[n]) s1[n][r] = s2[n][r] = -INFINITY;
+        }
+        auto number = [&](int e) { return lds_at<f32x4>(numbers + rt + 4 * (e * KVT + r0)); };
+        const f32x4 ls1 = number(0), ls2 = number(1);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s1[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[n][r], a.c, -ls1[r]));
+            s2[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s2[n][r], a.c, -ls2[r]));
+          }
+        f32x4 lm;
+        if (TOKEN) lm = number(NUMBERS - 1);
+        const f32x4 d1 = number(2), d2 = number(3);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float q1 = s1[n][r], q2 = s2[n][r] * (TOKEN ? lm[r] : lam), x = da[u][n][r];
+            da[u][n][r] = q1 - q2;
+            s1[n][r] = q1 * (x - d1[r]);
+            s2[n][r] = q2 * (d2[r] - x);
+          }
+          pd[u][n] = packed4<T>(da[u][n]);
+          p1[u][n] = packed4<T>(s1[n]);
+          p2[u][n] = packed4<T>(s2[n]);
+        }
+      }
+      in_order();
+      auto both = [](const uint2 (&p)[2][2], int n) { return make_uint4(p[0][n].x, p[0][n].y, p[1][n].x, p[1][n].y); };
+#pragma unroll
+      for (int d = 0; d < VB; ++d) {
+        const uint4 x = gcols.at(gt, 0, 16 * d);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) dv[d][n] = Mat<T>::mfma16(x, both(pd, n), dv[d][n]);
+      }
+#pragma unroll
+      for (int d = 0; d < KB; ++d) {
+        const uint4 x = qcols.at(qt, 0, 16 * d), y = qcols.at(qt, 0, DH + 16 * d);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          dk[0][d][n] = Mat<T>::mfma16(x, both(p1, n), dk[0][d][n]);
+          dk[1][d][n] = Mat<T>::mfma16(y, both(p2, n), dk[1][d][n]);
         }
       }
     }
@@ -1087,7 +1133,7 @@ int lmo_diff_attn_fwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
 
 int64_t lmo_diff_attn_bwd_scratch(const lmo_diff_shape* s, int lam_kind) {
   if (!s || s->b < 1 || s->tq < 1) return 0;
-  return 2 * s->b * s->h * s->tq + (lam_kind == LMO_LAM_TOKEN ? s->b * s->tq * s->h : s->h * s->b * blocks_of(s->tq));
+  return (lam_kind == LMO_LAM_TOKEN ? 3 : 2) * s->b * s->h * s->tq + (lam_kind == LMO_LAM_TOKEN ? s->b * s->tq * s->h : s->h * s->b * blocks_of(s->tq));
 }
 
 int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
@@ -1110,13 +1156,13 @@ int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
   a.dk = dk;
   a.dval = dv;
   a.delta = scratch;
-  a.dlam = dlam ? scratch + 2 * s->b * s->h * s->tq : nullptr;
-  a.dlam_rows = lam_kind == LMO_LAM_TOKEN;
+  a.dlam = dlam ? scratch + (lam_kind == LMO_LAM_TOKEN ? 3 : 2) * s->b * s->h * s->tq : nullptr;
+  a.lam_rows = lam_kind == LMO_LAM_TOKEN;
   const int64_t qblocks = blocks_of(s->tq), grid_q = s->b * s->h * qblocks, grid_k = s->b * s->hk * blocks_of(s->tk);
   if (grid_q > 0x7fffffff || grid_k > 0x7fffffff) return LDR_E_SHAPE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   DIFF_SWITCH(dtype, s->dh, s->dv, {
-    constexpr int bytes = 2 * TILE * (2 * DH + DV) * 2, rows = 2 * 5 * TILE * 4;
+    constexpr int bytes = 2 * TILE * (2 * DH + DV) * 2;
     if ((e = ALLOW_LDS(bytes, k_diff_bwd_q<T, DH, DV>))) return e;
     hipLaunchKernelGGL((k_diff_bwd_q<T, DH, DV>), dim3((unsigned)grid_q), dim3(WG), bytes, st, a);
     if ((e = launched())) return e;
@@ -1129,12 +1175,13 @@ int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
       else hipLaunchKernelGGL(k_diff_dlam<T>, dim3(g), dim3(WG), 0, st, a.dlam, n, outs, static_cast<T*>(dlam));
       if ((e = launched())) return e;
     }
-    if (dk && lam->t) {
-      if ((e = ALLOW_LDS(bytes + rows, k_diff_bwd_kv<T, DH, DV, true>))) return e;
-      hipLaunchKernelGGL((k_diff_bwd_kv<T, DH, DV, true>), dim3((unsigned)grid_k), dim3(WG), bytes + rows, st, a);
+    constexpr int kv_bytes = 2 * (2 * KVT * (2 * DH + DV) + QB * DV) + 2 * 5 * KVT * 4;
+    if (dk && lam_kind == LMO_LAM_TOKEN) {
+      if ((e = ALLOW_LDS(kv_bytes, k_diff_bwd_kv<T, DH, DV, true>))) return e;
+      hipLaunchKernelGGL((k_diff_bwd_kv<T, DH, DV, true>), dim3((unsigned)grid_k), dim3(WG), kv_bytes, st, a);
     } else if (dk) {
-      if ((e = ALLOW_LDS(bytes + rows, k_diff_bwd_kv<T, DH, DV, false>))) return e;
-      hipLaunchKernelGGL((k_diff_bwd_kv<T, DH, DV, false>), dim3((unsigned)grid_k), dim3(WG), bytes + rows, st, a);
+      if ((e = ALLOW_LDS(kv_bytes, k_diff_bwd_kv<T, DH, DV, false>))) return e;
+      hipLaunchKernelGGL((k_diff_bwd_kv<T, DH, DV, false>), dim3((unsigned)grid_k), dim3(WG), kv_bytes, st, a);
     }
   })
   return launched();
