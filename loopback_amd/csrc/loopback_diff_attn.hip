@@ -103,7 +103,7 @@ __device__ __forceinline__ int row_of(int r, int h) { return 4 * h + (r & 3) + 8
 // each offset: 100 spilled registers in the kernel of dk and dv.)
 // ---------------------------------------------------------------------------------------------------------------
 template <int W> __device__ __forceinline__ int swizzle(int r) {
-  return (W == 64 ? (r >> 1 & 1) << 2 : (r & 1) << 3 | (r >> 1 & 1) << 2) | (r >> 2 & 1) << 1 | (r >> 3 & 1);
+  return (W == 64 ? (r >> 1 & 1) << 2 : (r & 1) << 3 | (r >> 1 & 1) << 2) | ((r >> 2 ^ r >> 3) & 1) << 1 | (r >> 3 & 1);
 }
 __device__ __forceinline__ int kept(int x) {   // held as it is, not formed again from what it was formed from
   asm volatile("" : "+v"(x));
@@ -121,10 +121,11 @@ __device__ __forceinline__ uint4 four_and_four(int p, int q) {   // a column's e
 // operands of v_mfma_f32_32x32x16
 template <int W> struct Rows32 {   // A: rows r0 + l mod 32, columns 16 ks + 8 (l / 32) .. + 8
   int o[W == 64 ? 4 : 8];
-  __device__ __forceinline__ Rows32() {
+  __device__ __forceinline__ explicit Rows32(int ks0 = 0) {   // ks counted from ks0, 0 or half the row's
     const int lane = (int)threadIdx.x & 63, r = lane & 31;
 #pragma unroll
-    for (int v = 0; v < (W == 64 ? 4 : 8); ++v) o[v] = kept(2 * (r * W + 8 * ((2 * v) ^ ((lane >> 5) ^ swizzle<W>(r)))));
+    for (int v = 0; v < (W == 64 ? 4 : 8); ++v)
+      o[v] = kept(2 * (r * W + 8 * ((2 * (v + ks0) & 15) ^ ((lane >> 5) ^ swizzle<W>(r))) + 128 * (ks0 >> 3)));
   }
   __device__ __forceinline__ uint4 at(int tile, int r0, int ks) const {   // r0 a multiple of 32
     return sixteen(o[W == 64 ? ks & 3 : ks & 7] + tile + 2 * (r0 * W + 128 * (ks >> 3)));
@@ -132,19 +133,18 @@ template <int W> struct Rows32 {   // A: rows r0 + l mod 32, columns 16 ks + 8 (
 };
 template <int W> struct Cols32 {   // A: columns c0 + l mod 32, rows r0 + {4 h + 0..3, 8 + 4 h + 0..3}, h = l / 32
   static constexpr int V = W == 64 ? 2 : 4;
-  int o[V], p[V];
+  int o[V];   // of the first four rows; for the others the swizzle turns the two lowest bits of the piece
   __device__ __forceinline__ Cols32() {
     const int lane = (int)threadIdx.x & 63, j = lane & 15, r = 4 * (lane >> 5) + (j >> 2);
     const int piece = (lane >> 4 & 1) * 2 + ((j & 3) >> 1), half = 4 * (j & 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       o[v] = kept(2 * (r * W + 8 * ((4 * v) ^ (piece ^ swizzle<W>(r))) + half));
-      p[v] = kept(2 * ((r + 8) * W + 8 * ((4 * v) ^ (piece ^ swizzle<W>(r + 8))) + half));
     }
   }
   __device__ __forceinline__ uint4 at(int tile, int r0, int c0) const {   // r0 a multiple of 16, c0 of 32
     const int v = (c0 >> 5) & (V - 1), more = tile + 2 * (r0 * W + 128 * (c0 >> 7));
-    return four_and_four(o[v] + more, p[v] + more);
+    return four_and_four(o[v] + more, (o[v] ^ 48) + more + 16 * W);
   }
 };
 // operands of v_mfma_f32_16x16x32
@@ -160,14 +160,14 @@ template <int W> struct Rows16 {   // A: rows r0 + l mod 16, columns 32 ks + 8 (
   }
 };
 template <int W> struct Cols16 {   // A: columns c0 + l mod 16, rows r0 + {4 g + 0..3, 16 + 4 g + 0..3}, g = l / 16
-  int o[W == 64 ? 4 : 8];
+  int o[W == 64 ? 2 : 4];   // of every other 16 columns: the others are 32 bytes from them, forward or back
   __device__ __forceinline__ Cols16() {
     const int lane = (int)threadIdx.x & 63, j = lane & 15, r = 4 * (lane >> 4) + (j >> 2);
 #pragma unroll
-    for (int v = 0; v < (W == 64 ? 4 : 8); ++v) o[v] = kept(2 * (r * W + 8 * ((2 * v) ^ (((j & 3) >> 1) ^ swizzle<W>(r))) + 4 * (j & 1)));
+    for (int v = 0; v < (W == 64 ? 2 : 4); ++v) o[v] = kept(2 * (r * W + 8 * ((4 * v) ^ (((j & 3) >> 1) ^ swizzle<W>(r))) + 4 * (j & 1)));
   }
   __device__ __forceinline__ uint4 at(int tile, int r0, int c0) const {   // r0 a multiple of 32, c0 of 16
-    const int p = o[(c0 >> 4) & (W == 64 ? 3 : 7)] + tile + 2 * (r0 * W + 128 * (c0 >> 7));
+    const int v = (c0 >> 4) & (W == 64 ? 3 : 7), p = (v & 1 ? o[v >> 1] ^ 32 : o[v >> 1]) + tile + 2 * (r0 * W + 128 * (c0 >> 7));
     return four_and_four(p, p + 32 * W);
   }
 };
@@ -238,9 +238,9 @@ struct Diff {
   // backward
   const void* dy;
   void *dq, *dk, *dval;
-  float *delta, *dlam;           // D1, D2 and, where lam has queries, lam [b h][tq]; dlam's parts
+  float *delta, *dlam;           // four or, where lam has queries, five numbers [b h][tq] for k_diff_bwd_kv; dlam's parts
   int lam_rows;                  // lam has queries; dlam is per query, else per workgroup
-  // a split of the keys
+  // keys in chunks (few queries), or tiles of queries in parts (dk and dv)
   int splits, chunk;
   float* part;
 };
@@ -295,7 +295,10 @@ template <typename T, int W> struct Kept {
 };
 
 // One map's running softmax of a query (a lane pair's column)
-struct Soft { float m = NONE, l = 0.f; };
+struct Soft {
+  float m = NONE, l[4] = {0.f, 0.f, 0.f, 0.f};   // four sums: no chain of dependent adds
+  __device__ __forceinline__ float sum() const { return other_half((l[0] + l[1]) + (l[2] + l[3]), true); }
+};
 // a tile's scores of one map, as probabilities relative to the running maximum, packed: p[4 i' ...]; o, and l, are rescaled
 template <typename T, int NB, int DB>
 __device__ __forceinline__ void soft_step(f32x16 (&s)[NB], Soft& st, f32x16 (&o)[DB], uint4 (&p)[2 * NB], float c) {
@@ -308,110 +311,107 @@ __device__ __forceinline__ void soft_step(f32x16 (&s)[NB], Soft& st, f32x16 (&o)
   if (__any(mx > st.m + LAZY)) {
     const float mn = fmaxf(st.m, mx), a = st.m == mn ? 1.f : __builtin_amdgcn_exp2f(st.m - mn);
     st.m = mn;
-    st.l *= a;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) st.l[k] *= a;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] *= a;
   }
-  float ls[4] = {0.f, 0.f, 0.f, 0.f};   // four sums: no chain of dependent adds
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], c, -st.m));
-      ls[r & 3] += s[i][r];
+      st.l[r & 3] += s[i][r];
     }
     p[2 * i] = operand<T>(s[i], 0);
     p[2 * i + 1] = operand<T>(s[i], 1);
   }
-  st.l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 }
 
-template <int DH, int DV> constexpr int waves_fwd() { return DH + DV <= 192 ? 2 : 1; }
+template <int DH, int DV> constexpr int waves_bwd() { return DH + DV <= 192 ? 2 : 1; }   // waves to a SIMD, by their registers
 
 // ---------------------------------------------------------------------------------------------------------------
-// forward: 128 queries of a head per workgroup
+// forward: 64 queries of a head per workgroup, two waves for each 32 of them, one for each map. (Both maps in one wave read
+// the values once for both, but hold 256 registers, so two waves to a SIMD, in which the vector units, a wave's softmax, wait
+// for its products and the other way round; so it is three here.) The vector units bound it: per 32 x 32 scores of a map 16
+// exponentials of 16 cycles and some five operations of 4 for each, 580 cycles, against 384 of matrix cores.
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int FW = 4, FQ = 16 * FW, FT = 32, FL = 64 * FW;   // waves and queries of a workgroup, keys of a tile, lanes
+template <int DH, int DV> constexpr int waves_fwd() { return DV <= 128 ? 3 : 2; }
+template <int DH, int DV> constexpr int fwd_lds() {   // two tiles; at the end a map's results
+  const int tiles = 2 * FT * (2 * DH + DV) * 2, results = FQ * DV * 4;
+  return tiles > results ? tiles : results;
+}
 template <typename T, int DH, int DV>
-__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_fwd(const Diff a) {
-  constexpr int KT = TILE * 2 * DH, VT = TILE * DV, DB = DV / 32;
+__global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_fwd(const Diff a) {
   extern __shared__ __align__(16) char lds_block[];   // two tiles of keys, two of values
-  constexpr int K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT;
+  constexpr int KT = FT * 2 * DH, VT = FT * DV, DB = DV / 32, K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT;
   const int lane = (int)threadIdx.x & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int groups = a.h / a.hk, blocks = (a.tq + QB - 1) / QB;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), map = wave & 1;
+  const int groups = a.h / a.hk, blocks = (a.tq + FQ - 1) / FQ;
   Work wk;
   if (!work_of(a.b * a.hk, groups, blocks, wk)) return;
-  const int q0 = (blocks - 1 - wk.block) * QB, b = wk.item / a.hk, hk = wk.item - b * a.hk, head = hk * groups + wk.g;
+  const int q0 = (blocks - 1 - wk.block) * FQ, b = wk.item / a.hk, hk = wk.item - b * a.hk, head = hk * groups + wk.g;
   const int len = length_of(a, b), start = start_of(a, b);
-  const int w0 = q0 + 32 * wave, query = w0 + (lane & 31), qrow = min(query, a.tq - 1);
-  const T* qp = static_cast<const T*>(a.q.p) + b * a.q.b + qrow * a.q.t + 2 * head * a.q.h;
-  Kept<T, DH> q[2];
-  q[0].load(qp, a.dh);
-  q[1].load(qp + a.q.h, a.dh);
+  const int w0 = q0 + 32 * (wave >> 1), query = w0 + (lane & 31), qrow = min(query, a.tq - 1);
+  Kept<T, DH> q;
+  q.load(static_cast<const T*>(a.q.p) + b * a.q.b + qrow * a.q.t + (2 * head + map) * a.q.h, a.dh);
   const int seen = seen_by(a, qrow, start, len);
-  const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len);             // of the workgroup's queries
+  const int most = seen_by(a, min(q0 + FQ, a.tq) - 1, start, len);             // of the workgroup's queries
   const int wmost = w0 < a.tq ? seen_by(a, min(w0 + 32, a.tq) - 1, start, len) : 0, wleast = seen_by(a, min(w0, a.tq - 1), start, len);
-  const Rows32<2 * DH> krows;
+  const Rows32<2 * DH> krows(map * (DH / 16));
   const Cols32<DV> vcols;
-  f32x16 o1[DB], o2[DB];
+  f32x16 o[DB];
 #pragma unroll
-  for (int d = 0; d < DB; ++d) o1[d] = o2[d] = zero16();
-  Soft sm1, sm2;
-  const int ntiles = (most + TILE - 1) / TILE;
-  const Fill<T, 2 * DH, 2, TILE, WG> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
-  const Fill<T, DV, 1, TILE, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
+  for (int d = 0; d < DB; ++d) o[d] = zero16();
+  Soft sm;
+  const int ntiles = (most + FT - 1) / FT;
+  const Fill<T, 2 * DH, 2, FT, FL> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
+  const Fill<T, DV, 1, FT, FL> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
   if (ntiles > 0) {
     kf.fetch(0, len - 1, K0);
     vf.fetch(0, len - 1, V0);
   }
   filled();   // in every case: a wait for what was loaded above, left to the loop, would wait there for the tiles too
   auto tile = [&](int j, auto buffer) {
-    constexpr int cur = decltype(buffer)::value;   // known: the buffers' offsets go into the reads' own
-    const int k0 = j * TILE;
+    constexpr int cur = decltype(buffer)::value, kt = cur ? K1 : K0, vt = cur ? V1 : V0;   // known: they go into the reads' offsets
+    const int k0 = j * FT;
     if (j + 1 < ntiles) {   // the other buffer's readers are past the barrier below
-      kf.fetch(k0 + TILE, len - 1, cur ? K0 : K1);
-      vf.fetch(k0 + TILE, len - 1, cur ? V0 : V1);
+      kf.fetch(k0 + FT, len - 1, cur ? K0 : K1);
+      vf.fetch(k0 + FT, len - 1, cur ? V0 : V1);
     }
-    if (k0 < wmost) {
-      constexpr int kt = cur ? K1 : K0;
-      constexpr int vt = cur ? V1 : V0;
-      uint4 p1[4], p2[4];
-      auto scores = [&](int map, f32x16 (&s)[2]) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          s[i] = zero16();
+    for (int n = 0; n < FT / 32; ++n) {
+      const int k1 = k0 + 32 * n;
+      if (k1 >= wmost) break;
+      f32x16 s[1];
+      s[0] = zero16();
+      uint4 x[DH / 16], v[DB];   // operands, read before they are needed
 #pragma unroll
-          for (int ks = 0; ks < DH / 16; ++ks) s[i] = Mat<T>::mfma(krows.at(kt, 32 * i, map * (DH / 16) + ks), q[map].f[ks], s[i]);
-        }
-        if (k0 + TILE > wleast) {   // wave-uniform: keys that some query of the wave does not see
-          const int left = seen - k0 - 4 * half;
+      for (int ks = 0; ks < DH / 16; ++ks) x[ks] = krows.at(kt, 32 * n, ks);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (32 * i + row_of(r, 0) >= left) s[i][r] = -INFINITY;
-        }
-      };
-      f32x16 s[2];
-      scores(0, s);
-      in_order();
-      soft_step<T>(s, sm1, o1, p1, a.c);
-      in_order();
-      scores(1, s);
-      in_order();
-      soft_step<T>(s, sm2, o2, p2, a.c);
+      for (int d = 0; d < DB; ++d) v[d] = vcols.at(vt, 32 * n, 32 * d);
       in_order();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int ks = 0; ks < DH / 16; ++ks) s[0] = Mat<T>::mfma(x[ks], q.f[ks], s[0]);
+      if (k1 + 32 > wleast) {   // wave-uniform: keys that some query of the wave does not see
+        const int left = seen - k1 - 4 * half;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          if (d % 2 == 0) in_order();
-          const uint4 v = vcols.at(vt, 16 * i, 32 * d);
-          o1[d] = Mat<T>::mfma(v, p1[i], o1[d]);
-          o2[d] = Mat<T>::mfma(v, p2[i], o2[d]);
-        }
+        for (int r = 0; r < 16; ++r)
+          if (row_of(r, 0) >= left) s[0][r] = -INFINITY;
+      }
+      uint4 p[2];
+      soft_step<T>(s, sm, o, p, a.c);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        o[d] = Mat<T>::mfma(v[d], p[0], o[d]);
+        v[d] = vcols.at(vt, 32 * n + 16, 32 * d);
+      }
+      in_order();
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] = Mat<T>::mfma(v[d], p[1], o[d]);
     }
     if (j + 1 < ntiles) filled();
   };
@@ -419,35 +419,38 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
     tile(j, std::integral_constant<int, 0>());
     if (j + 1 < ntiles) tile(j + 1, std::integral_constant<int, 1>());
   }
-  const float l1 = other_half(sm1.l, true), l2 = other_half(sm2.l, true);
-  if (query >= a.tq) return;
   // a query that sees no key: zeros, and an infinite logarithm, which makes every probability 0
-  const float lam = lam_at<T>(a, b, query, head), i1 = l1 > 0.f || l1 != l1 ? 1.f / l1 : 0.f, i2 = l2 > 0.f || l2 != l2 ? 1.f / l2 : 0.f;
+  const float l = sm.sum(), inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  if (a.lse && half == 0 && query < a.tq)
+    a.lse[(((int64_t)map * a.b + b) * a.h + head) * a.tq + query] = inv != 0.f ? sm.m + __builtin_amdgcn_logf(l) : INFINITY;
   const int64_t orow = (((int64_t)b * a.tq + query) * a.h + head) * a.dv;
   T* op = static_cast<T*>(a.out) + orow;
   T* sp = static_cast<T*>(a.second) + orow;
-  typedef typename Mat<T>::Cvt C;
+  float* mine = reinterpret_cast<float*>(lds_block) + (wave >> 1) * 32 * DV + 4 * lane;   // [register / 4][lane][4]
+  __syncthreads();   // the last tile has been read
+  if (map) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 z = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]} * inv;
+        *reinterpret_cast<f32x4*>(mine + (4 * d + g) * 256) = z;
+        const int col = 32 * d + 8 * g + 4 * half;
+        if (a.second && col < a.dv && query < a.tq) *reinterpret_cast<uint2*>(sp + col) = packed4<T>(z);
+      }
+  }
+  __syncthreads();
+  if (map || query >= a.tq) return;
+  const float lam = lam_at<T>(a, b, query, head);
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int col = 32 * d + 8 * g + 4 * half;
-      if (col < a.dv) {
-        float y[4], z[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          z[k] = o2[d][4 * g + k] * i2;
-          y[k] = o1[d][4 * g + k] * i1 - lam * z[k];
-        }
-        *reinterpret_cast<uint2*>(op + col) = make_uint2(C::pack2(y[0], y[1]), C::pack2(y[2], y[3]));
-        if (a.second) *reinterpret_cast<uint2*>(sp + col) = make_uint2(C::pack2(z[0], z[1]), C::pack2(z[2], z[3]));
-      }
+      const f32x4 z = *reinterpret_cast<const f32x4*>(mine + (4 * d + g) * 256);
+      const f32x4 y = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]} * inv - lam * z;
+      if (col < a.dv) *reinterpret_cast<uint2*>(op + col) = packed4<T>(y);
     }
-  if (a.lse && half == 0) {
-    const int64_t n = ((int64_t)b * a.h + head) * a.tq + query;
-    a.lse[n] = i1 != 0.f ? sm1.m + __builtin_amdgcn_logf(l1) : INFINITY;
-    a.lse[n + (int64_t)a.b * a.h * a.tq] = i2 != 0.f ? sm2.m + __builtin_amdgcn_logf(l2) : INFINITY;
-  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -553,7 +556,7 @@ __global__ __launch_bounds__((64 * few_waves<DH, DV>())) __attribute__((amdgpu_w
       }
     wave_lds_sync();   // the tile's reads are done before the one after the next is loaded over it
   }
-  const float l1 = other_half(sm1.l, true), l2 = other_half(sm2.l, true);
+  const float l1 = sm1.sum(), l2 = sm2.sum();
   __syncthreads();
   float* part = reinterpret_cast<float*>(lds_block);   // [wave][32 rows][ROW]
   static_assert(few_waves<DH, DV>() * FEW * few_row<DV>() * 4 <= 160 * 1024 && few_lds<DH, DV>() <= 160 * 1024,
@@ -617,7 +620,7 @@ template <typename T, int DV> __global__ __launch_bounds__(DV) void k_diff_join(
 // backward: dq, the deltas and dlam's parts. 128 queries of a head per workgroup, as the forward
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int DH, int DV>
-__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_bwd_q(const Diff a) {
+__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<DH, DV>())))) void k_diff_bwd_q(const Diff a) {
   constexpr int KT = TILE * 2 * DH, VT = TILE * DV, QB_ = DH / 32;
   extern __shared__ __align__(16) char lds_block[];   // two tiles of keys, two of values; four floats
   constexpr int K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT;
@@ -657,10 +660,13 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
   d1 = __builtin_fmaf(lam, d2, other_half(d1, true));
   const int64_t n = ((int64_t)b * a.h + head) * a.tq + qrow, all = (int64_t)a.b * a.h * a.tq;
   const float ls1 = a.lse[n], ls2 = a.lse[n + all];
-  if (query < a.tq && half == 0) {
-    a.delta[n] = d1;
-    a.delta[n + all] = d2;
-    if (a.lam_rows) a.delta[n + 2 * all] = lam;   // as fp32, for the kernel below
+  if (query < a.tq && half == 0) {   // what the kernel of dk and dv reads: see there
+    const float sign = lam < 0.f ? -1.f : 1.f;
+    a.delta[n] = ls1;
+    a.delta[n + all] = ls2 - __builtin_amdgcn_logf(fabsf(lam));
+    a.delta[n + 2 * all] = -d1;
+    a.delta[n + 3 * all] = sign * (d2 - d1);
+    if (a.lam_rows) a.delta[n + 4 * all] = -sign;
   }
   const int seen = seen_by(a, qrow, start, len);
   const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len);
@@ -696,7 +702,6 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
         f32x16 da = zero16();
 #pragma unroll
         for (int ks = 0; ks < DV / 16; ++ks) da = Mat<T>::mfma(vrows.at(vt, 32 * i, ks), g.f[ks], da);
-        in_order();
 #pragma unroll
         for (int map = 0; map < 2; ++map) {
           f32x16 s = zero16();
@@ -715,7 +720,6 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
             if (map) dlam = __builtin_fmaf(p, da[r], dlam);
             s[r] = p * (da[r] - d);
           }
-          in_order();
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
             const uint4 ds = operand<T>(s, st);
@@ -723,7 +727,6 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
             for (int e = 0; e < QB_; ++e)
               dq[map][e] = Mat<T>::mfma(kcols.at(kt, 32 * i + 16 * st, map * DH + 32 * e), ds, dq[map][e]);
           }
-          in_order();
         }
       }
     }
@@ -786,8 +789,13 @@ template <typename T> __global__ __launch_bounds__(WG) void k_diff_dlam(const fl
 
 // ---------------------------------------------------------------------------------------------------------------
 // backward: dk and dv. 128 keys of a head of keys per workgroup, 32 a wave, over the queries of its group's heads one after
-// another. Here the scores' rows are queries, whose four or five numbers come from LDS for every row a lane has: by
-// v_mfma_f32_16x16x32 a lane has 4 of 16 rows, not 16 of 32, and half as much is read for them, and held.
+// another, or a part of them: the first keys of a causal sequence have the most queries, and a group's heads add to them; parts of
+// at most `limit` tiles, their fp32 results summed by k_diff_kv_sum, leave no CU behind the others.
+// Here the scores' rows are queries, whose four or five numbers come from LDS for every row a lane has: by
+// v_mfma_f32_16x16x32 a lane has 4 of 16 rows, not 16 of 32, and half as much is read for them, and held. With s = -1 where lam < 0,
+// else 1, and P2' = |lam| P2 = exp2(c s2 - (lse2 - log2 |lam|)), the numbers are lse1, lse2 - log2 |lam|, -D1 (where the product
+// for dA begins), s (D2 - D1) and -s, so that
+//   P = P1 - s P2',   dS1 = P1 (dA - D1),   dS2 = P2' (s (D2 - D1) - s (dA - D1))
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int KVT = 32;   // queries of a tile
 template <typename T, int W> struct Kept16 {   // a wave's 32 rows as B operands: row 16 n + l mod 16, columns 32 ks + 8 (l / 16) .. + 8
@@ -802,8 +810,16 @@ template <typename T, int W> struct Kept16 {   // a wave's 32 rows as B operands
   }
 };
 
+// the tiles of queries that a block of keys has in one head, from which on, and its parts
+struct KvTiles { int first, n, parts; };
+__device__ __forceinline__ KvTiles kv_tiles(const Diff& a, int b, int kb) {
+  const int first_q = a.causal ? max(kb - start_of(a, b), 0) : 0, first = first_q / KVT;
+  const int n = kb < length_of(a, b) && first_q < a.tq ? (a.tq + KVT - 1) / KVT - first : 0;
+  return {first, n, min(a.splits, max(1, (n * (a.h / a.hk) + a.chunk - 1) / a.chunk))};
+}
+
 template <typename T, int DH, int DV, bool TOKEN>   // TOKEN: lam differs between queries
-__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_bwd_kv(const Diff a) {
+__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<DH, DV>())))) void k_diff_bwd_kv(const Diff a) {
   extern __shared__ __align__(16) char lds_block[];
   constexpr int QT = KVT * 2 * DH, GT = KVT * DV, KB = DH / 16, VB = DV / 16, NUMBERS = TOKEN ? 5 : 4;
   // two tiles of queries and of dy, this workgroup's values, and twice lse1, lse2, D1, D2, lam of the tile's queries
@@ -812,8 +828,10 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = a.h / a.hk, blocks = (a.tk + QB - 1) / QB;
   Work wk;
-  if (!work_of(a.b * a.hk, 1, blocks, wk)) return;
+  if (!work_of(a.b * a.hk, a.splits, blocks, wk)) return;
   const int kb = wk.block * QB, b = wk.item / a.hk, hk = wk.item - b * a.hk;
+  const KvTiles kv = kv_tiles(a, b, kb);
+  if (wk.g >= kv.parts) return;
   const int len = length_of(a, b), start = start_of(a, b);
   const int w0 = kb + 32 * wave;
   Kept16<T, DH> k[2];
@@ -839,9 +857,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
 #pragma unroll
     for (int d = 0; d < VB; ++d) dv[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // the first query that sees the workgroup's first key
-  const int first_q = a.causal ? max(kb - start, 0) : 0, first = first_q / KVT;
-  const int ntiles = kb < len && first_q < a.tq ? (a.tq + KVT - 1) / KVT - first : 0, total = ntiles * groups;
+  const int per = (kv.n * groups + kv.parts - 1) / kv.parts, it0 = wk.g * per, it1 = min(it0 + per, kv.n * groups);
   const int64_t all = (int64_t)a.b * a.h * a.tq;
   const T* qbase = static_cast<const T*>(a.q.p) + b * a.q.b + 2 * hk * groups * a.q.h;
   const T* gbase = static_cast<const T*>(a.dy) + ((int64_t)b * a.tq * a.h + hk * groups) * a.dv;
@@ -853,22 +869,23 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
     qf.fetch(row0, a.tq - 1, s_q);
     gf.fetch(row0, a.tq - 1, s_g);
     // a wave loads 32 of two of the numbers
-    const int64_t n = ((int64_t)b * a.h + hk * groups + head) * a.tq + row0;
+    const float* of = a.delta + ((int64_t)b * a.h + hk * groups + head) * a.tq + row0;
     const uint32_t row = 4u * (uint32_t)min(lane & 31, a.tq - 1 - row0);
-    if (wave < 2) {
-      const float* of = (wave ? a.delta : a.lse) + n;
-      load_lds4(of, row + (lane & 32 ? (uint32_t)(4 * all) : 0u), s_row + wave * 8 * KVT);
-    }
-    if (TOKEN && wave == 2 && lane < 32) load_lds4(a.delta + n + 2 * all, row, s_row + 16 * KVT);
+    if (wave < 2) load_lds4(of + 2 * wave * all, row + (lane & 32 ? (uint32_t)(4 * all) : 0u), s_row + wave * 8 * KVT);
+    if (TOKEN && wave == 2 && lane < 32) load_lds4(of + 4 * all, row, s_row + 16 * KVT);
   };
-  Rows16<DV> vrows;   // of the wave's keys
-#pragma unroll
-  for (int e = 0; e < (DV == 64 ? 2 : 4); ++e) vrows.o[e] = kept(vrows.o[e] + wave * 64 * DV);
+  const int mine = kept(wave * 64 * DV);   // the offset of the wave's values
   const int numbers = kept(16 * grp);
-  if (total > 0) {
+  int head = kv.n ? it0 / kv.n : 0, at = kv.first + it0 - head * kv.n;
+  auto minus_of = [&](int head) {   // -s of a head, waited for here and not where it is used
+    const float lam = TOKEN || head >= groups ? 0.f : lam_at<T>(a, b, 0, hk * groups + head);
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(lam < 0.f ? 1.f : -1.f)));
+  };
+  float next_minus = minus_of(head);
+  if (it0 < it1) {
     const Fill<T, DV, 1, QB, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
     vf.fetch(kb, len - 1, VALUES);
-    fetch(first * KVT, 0, Q0, G0, R0);
+    fetch(at * KVT, head, Q0, G0, R0);
   }
   filled();
   if (a.dv < DV) {   // the values' columns past the last repeat some, as dy's do: zeros in their place
@@ -878,16 +895,16 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
     }
     __syncthreads();
   }
-  int at = first, head = 0;
   auto tile = [&](int it, auto buffer) {
     constexpr int cur = decltype(buffer)::value;
     const int q0 = at * KVT;
-    const float lam = TOKEN ? 0.f : lam_at<T>(a, b, 0, hk * groups + head);
-    if (++at == first + ntiles) {
-      at = first;
+    const float minus = next_minus;
+    if (++at == kv.first + kv.n) {
+      at = kv.first;
       ++head;
+      next_minus = minus_of(head);
     }
-    if (it + 1 < total) fetch(at * KVT, head, cur ? Q0 : Q1, cur ? G0 : G1, cur ? R0 : R1);
+    if (it + 1 < it1) fetch(at * KVT, head, cur ? Q0 : Q1, cur ? G0 : G1, cur ? R0 : R1);
     // the keys that the tile's last and first queries see: whether any of this wave's is among them, and whether all are
     if (w0 < seen_by(a, min(q0 + KVT, a.tq) - 1, start, len)) {
       constexpr int qt = cur ? Q1 : Q0, gt = cur ? G1 : G0, rt = cur ? R1 : R0;
@@ -895,14 +912,14 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
       uint2 pd[2][2], p1[2][2], p2[2][2];   // [16 queries][16 keys]: P1 - lam P2, dS1, dS2
       f32x4 da[2][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) da[u][0] = da[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < 2; ++u) da[u][0] = da[u][1] = lds_at<f32x4>(numbers + rt + 4 * (2 * KVT + 16 * u));
 #pragma unroll
       for (int ks = 0; ks < DV / 32; ++ks) {
         uint4 x[2], y[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           x[e] = grows.at(gt, 16 * e, ks);
-          y[e] = vrows.at(VALUES, 16 * e, ks);
+          y[e] = grows.at(mine + VALUES, 16 * e, ks);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -941,17 +958,17 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
             s1[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[n][r], a.c, -ls1[r]));
             s2[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s2[n][r], a.c, -ls2[r]));
           }
-        f32x4 lm;
-        if (TOKEN) lm = number(NUMBERS - 1);
-        const f32x4 d1 = number(2), d2 = number(3);
+        f32x4 sg;
+        if (TOKEN) sg = number(NUMBERS - 1);
+        const f32x4 d = number(3);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float q1 = s1[n][r], q2 = s2[n][r] * (TOKEN ? lm[r] : lam), x = da[u][n][r];
-            da[u][n][r] = q1 - q2;
-            s1[n][r] = q1 * (x - d1[r]);
-            s2[n][r] = q2 * (d2[r] - x);
+            const float q1 = s1[n][r], q2 = s2[n][r], x = da[u][n][r], m = TOKEN ? sg[r] : minus;
+            da[u][n][r] = __builtin_fmaf(m, q2, q1);
+            s1[n][r] = q1 * x;
+            s2[n][r] = q2 * __builtin_fmaf(m, x, d[r]);
           }
           pd[u][n] = packed4<T>(da[u][n]);
           p1[u][n] = packed4<T>(s1[n]);
@@ -976,16 +993,33 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
         }
       }
     }
-    if (it + 1 < total) filled();
+    if (it + 1 < it1) filled();
   };
-  for (int it = 0; it < total; it += 2) {
+  for (int it = it0; it < it1; it += 2) {
     tile(it, std::integral_constant<int, 0>());
-    if (it + 1 < total) tile(it + 1, std::integral_constant<int, 1>());
+    if (it + 1 < it1) tile(it + 1, std::integral_constant<int, 1>());
   }
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const int key = w0 + 16 * n + (lane & 15);
     if (key >= a.tk) continue;
+    if (kv.parts > 1) {   // [dk1 | dk2 | dv] of a key, not scaled
+      float* row = a.part + ((((int64_t)wk.item * blocks + wk.block) * a.splits + wk.g) * QB + (key - kb)) * (2 * a.dh + a.dv);
+#pragma unroll
+      for (int d = 0; d < KB; ++d) {
+        const int col = 16 * d + 4 * grp;
+        if (col < a.dh) {
+          *reinterpret_cast<f32x4*>(row + col) = dk[0][d][n];
+          *reinterpret_cast<f32x4*>(row + a.dh + col) = dk[1][d][n];
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < VB; ++d) {
+        const int col = 16 * d + 4 * grp;
+        if (col < a.dv) *reinterpret_cast<f32x4*>(row + 2 * a.dh + col) = dv[d][n];
+      }
+      continue;
+    }
     T* krow = static_cast<T*>(a.dk) + (((int64_t)b * a.tk + key) * 2 * a.hk + 2 * hk) * a.dh;
     T* vrow = static_cast<T*>(a.dval) + (((int64_t)b * a.tk + key) * a.hk + hk) * a.dv;
 #pragma unroll
@@ -1001,6 +1035,26 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
       const int col = 16 * d + 4 * grp;
       if (col < a.dv) *reinterpret_cast<uint2*>(vrow + col) = packed4<T>(dv[d][n]);
     }
+  }
+}
+
+// the parts of a block of keys, in order, scaled and rounded: SUM_ROWS keys of a block per workgroup, four columns a lane
+constexpr int SUM_ROWS = 8;
+template <typename T> __global__ __launch_bounds__(WG) void k_diff_kv_sum(const Diff a) {
+  const int blocks = (a.tk + QB - 1) / QB, item = (int)blockIdx.x / blocks, kb = ((int)blockIdx.x - item * blocks) * QB;
+  const int b = item / a.hk, hk = item - b * a.hk, parts = kv_tiles(a, b, kb).parts, row = 2 * a.dh + a.dv, per = row / 4;
+  if (parts == 1) return;
+  const float* p = a.part + (int64_t)blockIdx.x * a.splits * QB * row;
+  const int k0 = (int)blockIdx.y * SUM_ROWS, k1 = min(min(k0 + SUM_ROWS, QB), a.tk - kb);
+  for (int i = k0 * per + (int)threadIdx.x; i < k1 * per; i += WG) {
+    const int key = i / per, col = 4 * (i - key * per);
+    const float* x = p + (int64_t)key * row + col;
+    f32x4 t = *reinterpret_cast<const f32x4*>(x);
+    for (int s = 1; s < parts; ++s) t += *reinterpret_cast<const f32x4*>(x + (int64_t)s * QB * row);
+    if (col < 2 * a.dh)
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.dk) + (((int64_t)b * a.tk + kb + key) * 2 * a.hk + 2 * hk) * a.dh + col) = packed4<T>(t * a.scale);
+    else
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.dval) + (((int64_t)b * a.tk + kb + key) * a.hk + hk) * a.dv + col - 2 * a.dh) = packed4<T>(t);
   }
 }
 
@@ -1023,6 +1077,7 @@ int diff_args(const lmo_diff_shape* s, const lmo_strides* q, const lmo_strides* 
   if (s->b < 0 || s->tq < 0 || s->tk < 1 || s->hk < 1 || s->h < s->hk || s->h % s->hk || s->b * s->h > MOST || s->tq >= (1 << 30) ||
       s->tk >= (1 << 30))
     return LDR_E_ARG;
+  if (s->b * s->h * s->tq >= (1 << 29)) return LDR_E_SHAPE;   // a number of each within 32 bits of bytes
   if (s->dh < 8 || s->dh > 128 || s->dh % 8 || s->dv < 8 || s->dv > 256 || s->dv % 8) return LDR_E_SHAPE;
   if (!(s->scale > 0.f) || !(s->scale < INFINITY)) return LDR_E_ARG;
   for (const lmo_strides* t : {q, k, v}) {
@@ -1078,6 +1133,23 @@ inline Chunks chunks_of(const lmo_diff_shape* s) {
   const int64_t chunk = ((s->tk + n - 1) / n + 127) / 128 * 128;
   return {(s->tk + chunk - 1) / chunk, chunk};
 }
+// parts of the tiles of queries for dk and dv: those of a causal sequence (positions and lengths are the kernel's to know), so that
+// the longest takes little more than its share of what the CUs hold at once
+struct Parts { int64_t splits, limit; };
+inline Parts kv_parts(const lmo_diff_shape* s) {
+  const int64_t blocks = blocks_of(s->tk), tiles = (s->tq + KVT - 1) / KVT, groups = s->h / s->hk, slots = s->dh <= 64 && s->dv <= 128 ? 512 : 256;
+  int64_t all = 0, most = 0;
+  for (int64_t i = 0; i < blocks; ++i) {
+    const int64_t from = s->causal ? i * QB - (s->tk - s->tq) : 0, n = from < s->tq ? (tiles - (from > 0 ? from / KVT : 0)) * groups : 0;
+    all += n;
+    most = n > most ? n : most;
+  }
+  const int64_t share = (all * s->b * s->hk + slots - 1) / slots;
+  int64_t limit = share + (share + 2) / 3;
+  limit = limit < 16 ? 16 : limit;
+  const int64_t splits = (most + limit - 1) / limit;
+  return {splits < 1 ? 1 : splits > 16 ? 16 : splits, limit};
+}
 inline bool few(const lmo_diff_shape* s) { return s->tq * (s->h / s->hk) <= FEW; }
 inline int padded_dv(const lmo_diff_shape* s) { return s->dv <= 64 && s->dh <= 64 ? 64 : s->dv <= 128 ? 128 : 256; }
 
@@ -1121,19 +1193,22 @@ int lmo_diff_attn_fwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
     })
     return launched();
   }
-  const int64_t grid = s->b * s->h * blocks_of(s->tq);
+  const int64_t grid = s->b * s->h * ((s->tq + FQ - 1) / FQ);
   if (grid > 0x7fffffff) return LDR_E_SHAPE;
   DIFF_SWITCH(dtype, s->dh, s->dv, {
-    constexpr int bytes = 2 * TILE * (2 * DH + DV) * 2;
+    constexpr int bytes = fwd_lds<DH, DV>();
     if ((e = ALLOW_LDS(bytes, k_diff_fwd<T, DH, DV>))) return e;
-    hipLaunchKernelGGL((k_diff_fwd<T, DH, DV>), dim3((unsigned)grid), dim3(WG), bytes, st, a);
+    hipLaunchKernelGGL((k_diff_fwd<T, DH, DV>), dim3((unsigned)grid), dim3(FL), bytes, st, a);
   })
   return launched();
 }
 
 int64_t lmo_diff_attn_bwd_scratch(const lmo_diff_shape* s, int lam_kind) {
-  if (!s || s->b < 1 || s->tq < 1) return 0;
-  return (lam_kind == LMO_LAM_TOKEN ? 3 : 2) * s->b * s->h * s->tq + (lam_kind == LMO_LAM_TOKEN ? s->b * s->tq * s->h : s->h * s->b * blocks_of(s->tq));
+  if (!s || s->b < 1 || s->tq < 1 || s->tk < 1 || s->hk < 1 || s->h < s->hk) return 0;
+  const int64_t numbers = lam_kind == LMO_LAM_TOKEN ? 5 : 4, parts = lam_kind == LMO_LAM_TOKEN ? s->b * s->tq * s->h : s->h * s->b * blocks_of(s->tq);
+  const Parts kv = kv_parts(s);
+  return (numbers * s->b * s->h * s->tq + parts + 3) / 4 * 4 +
+         (kv.splits > 1 ? s->b * s->hk * blocks_of(s->tk) * kv.splits * QB * (2 * s->dh + s->dv) : 0);
 }
 
 int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
@@ -1156,9 +1231,14 @@ int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
   a.dk = dk;
   a.dval = dv;
   a.delta = scratch;
-  a.dlam = dlam ? scratch + (lam_kind == LMO_LAM_TOKEN ? 3 : 2) * s->b * s->h * s->tq : nullptr;
+  const Parts kv = kv_parts(s);
+  const int64_t numbers = (lam_kind == LMO_LAM_TOKEN ? 5 : 4) * s->b * s->h * s->tq;
+  a.dlam = dlam ? scratch + numbers : nullptr;
+  a.splits = (int)kv.splits;
+  a.chunk = (int)kv.limit;
+  a.part = scratch + (numbers + (lam_kind == LMO_LAM_TOKEN ? s->b * s->tq * s->h : s->h * s->b * blocks_of(s->tq)) + 3) / 4 * 4;
   a.lam_rows = lam_kind == LMO_LAM_TOKEN;
-  const int64_t qblocks = blocks_of(s->tq), grid_q = s->b * s->h * qblocks, grid_k = s->b * s->hk * blocks_of(s->tk);
+  const int64_t qblocks = blocks_of(s->tq), grid_q = s->b * s->h * qblocks, grid_k = s->b * s->hk * blocks_of(s->tk) * kv.splits;
   if (grid_q > 0x7fffffff || grid_k > 0x7fffffff) return LDR_E_SHAPE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   DIFF_SWITCH(dtype, s->dh, s->dv, {
@@ -1182,6 +1262,10 @@ int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
     } else if (dk) {
       if ((e = ALLOW_LDS(kv_bytes, k_diff_bwd_kv<T, DH, DV, false>))) return e;
       hipLaunchKernelGGL((k_diff_bwd_kv<T, DH, DV, false>), dim3((unsigned)grid_k), dim3(WG), kv_bytes, st, a);
+    }
+    if (dk && kv.splits > 1) {
+      if ((e = launched())) return e;
+      hipLaunchKernelGGL(k_diff_kv_sum<T>, dim3((unsigned)(grid_k / kv.splits), QB / SUM_ROWS), dim3(WG), 0, st, a);
     }
   })
   return launched();

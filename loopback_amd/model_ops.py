@@ -148,7 +148,7 @@ def add_layer_norm(x: torch.Tensor, add: torch.Tensor | None, weight: torch.Tens
 # ---------------------------------------------------------------------------------------------------------------
 # differential attention
 # ---------------------------------------------------------------------------------------------------------------
-ATTN_MAX_DH, ATTN_MAX_DV, ATTN_MAX_TOKENS, ATTN_MAX_HEADS = 128, 256, 2 ** 30 - 1, 0x7fffff
+ATTN_MAX_DH, ATTN_MAX_DV, ATTN_MAX_TOKENS, ATTN_MAX_HEADS, ATTN_MAX_ROWS = 128, 256, 2 ** 30 - 1, 0x7fffff, 2 ** 29
 
 
 def _seen(b, tq, tk, causal, lengths, starts, device):
@@ -232,7 +232,8 @@ def attention_native(q, k, v, lam) -> bool:
     """Whether the kernels take the call: bf16 or fp16, widths that are multiples of 8 up to 128 and 256, lam of their type or fp32."""
     return (native(q, k, v) and (type(lam) is torch.Tensor or type(lam) is torch.nn.Parameter) and lam.dtype in (q.dtype, torch.float32)
             and q.numel() > 0 and k.numel() > 0 and q.shape[3] % 8 == 0 and q.shape[3] <= ATTN_MAX_DH and v.shape[3] % 8 == 0
-            and 0 < v.shape[3] <= ATTN_MAX_DV and max(q.shape[1], k.shape[1]) <= ATTN_MAX_TOKENS and q.shape[0] * q.shape[2] <= ATTN_MAX_HEADS)
+            and 0 < v.shape[3] <= ATTN_MAX_DV and max(q.shape[1], k.shape[1]) <= ATTN_MAX_TOKENS and q.shape[0] * q.shape[2] <= ATTN_MAX_HEADS
+            and q.shape[0] * q.shape[1] * q.shape[2] // 2 < ATTN_MAX_ROWS)
 
 
 def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, *, causal: bool = True,
