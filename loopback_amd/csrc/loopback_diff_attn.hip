@@ -339,7 +339,7 @@ template <int DH, int DV> constexpr int waves_bwd() { return DH + DV <= 192 ? 2 
 // exponentials of 16 cycles and some five operations of 4 for each, 580 cycles, against 384 of matrix cores.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int FW = 4, FQ = 16 * FW, FT = 32, FL = 64 * FW;   // waves and queries of a workgroup, keys of a tile, lanes
-template <int DH, int DV> constexpr int waves_fwd() { return DV <= 128 ? 3 : 2; }
+template <int DH, int DV> constexpr int waves_fwd() { return DH <= 64 && DV <= 128 ? 3 : 2; }
 template <int DH, int DV> constexpr int fwd_lds() {   // two tiles; at the end a map's results
   const int tiles = 2 * FT * (2 * DH + DV) * 2, results = FQ * DV * 4;
   return tiles > results ? tiles : results;
@@ -389,10 +389,13 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
       f32x16 s[1];
       s[0] = zero16();
       uint4 x[DH / 16], v[DB];   // operands, read before they are needed
+      constexpr bool AHEAD = DB <= 4;   // wider: the registers do not hold them
 #pragma unroll
       for (int ks = 0; ks < DH / 16; ++ks) x[ks] = krows.at(kt, 32 * n, ks);
+      if (AHEAD) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d) v[d] = vcols.at(vt, 32 * n, 32 * d);
+        for (int d = 0; d < DB; ++d) v[d] = vcols.at(vt, 32 * n, 32 * d);
+      }
       in_order();
 #pragma unroll
       for (int ks = 0; ks < DH / 16; ++ks) s[0] = Mat<T>::mfma(x[ks], q.f[ks], s[0]);
@@ -406,12 +409,12 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
       soft_step<T>(s, sm, o, p, a.c);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        o[d] = Mat<T>::mfma(v[d], p[0], o[d]);
-        v[d] = vcols.at(vt, 32 * n + 16, 32 * d);
+        o[d] = Mat<T>::mfma(AHEAD ? v[d] : vcols.at(vt, 32 * n, 32 * d), p[0], o[d]);
+        if (AHEAD) v[d] = vcols.at(vt, 32 * n + 16, 32 * d);
       }
-      in_order();
+      if (AHEAD) in_order();
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] = Mat<T>::mfma(v[d], p[1], o[d]);
+      for (int d = 0; d < DB; ++d) o[d] = Mat<T>::mfma(AHEAD ? v[d] : vcols.at(vt, 32 * n + 16, 32 * d), p[1], o[d]);
     }
     if (j + 1 < ntiles) filled();
   };
@@ -455,165 +458,172 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
 
 // ---------------------------------------------------------------------------------------------------------------
 // few queries: the (query, head of the group) pairs of a head of keys are the 32 rows of one block (tq times the group at
-// most 32). A workgroup takes a chunk of its keys; its waves take tiles of 32 of them in turn, each through LDS of its own,
-// two tiles in flight; their results meet in LDS, and those of the chunks in k_diff_join.
+// most 32). A workgroup takes a chunk of its keys, in tiles of 64: two waves for each map, each with 32 keys of a tile. The
+// keys' and values' stream bounds it, so the probabilities enter the products as two 16-bit parts: their rounding is not added to
+// the result's. The waves' results meet in LDS, and those of the chunks in k_diff_join.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int FEW = 32;
-template <int DH, int DV> constexpr int few_waves() { return 2 * DH + DV <= 256 ? 4 : 2; }
-template <int DH, int DV> constexpr int few_lds() { return few_waves<DH, DV>() * 2 * FEW * (2 * DH + DV) * 2; }
+constexpr int FEW = 32, NT = 64;   // rows, keys of a tile
 template <int DV> constexpr int few_row() { return 2 * DV + 4; }   // floats of a row's partial result: o1, o2, m1, l1, m2, l2
-
-// a row's partial results as one: their common maximum, the sums and the values. at(i): the i-th partial row
-template <int DV, typename At>
-__device__ __forceinline__ void join_row(At at, int n, int col, float& y1, float& y2) {
-  float m1 = NONE, m2 = NONE;
-  for (int i = 0; i < n; ++i) {
-    const float* p = at(i) + 2 * DV;
-    m1 = fmaxf(m1, p[0]);
-    m2 = fmaxf(m2, p[2]);
-  }
-  float l1 = 0.f, l2 = 0.f;
-  y1 = y2 = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const float* p = at(i);
-    const float f1 = __builtin_amdgcn_exp2f(p[2 * DV] - m1), f2 = __builtin_amdgcn_exp2f(p[2 * DV + 2] - m2);
-    l1 = __builtin_fmaf(p[2 * DV + 1], f1, l1);
-    l2 = __builtin_fmaf(p[2 * DV + 3], f2, l2);
-    y1 = __builtin_fmaf(p[col], f1, y1);
-    y2 = __builtin_fmaf(p[DV + col], f2, y2);
-  }
-  y1 = l1 > 0.f || l1 != l1 ? y1 / l1 : 0.f;
-  y2 = l2 > 0.f || l2 != l2 ? y2 / l2 : 0.f;
+template <int DH, int DV> constexpr int few_lds() {   // two tiles; at the end the four waves' results
+  const int tiles = 2 * NT * (2 * DH + DV) * 2, results = 4 * FEW * (DV + 2) * 4;
+  return tiles > results ? tiles : results;
 }
 
 template <typename T, int DH, int DV>
-__global__ __launch_bounds__((64 * few_waves<DH, DV>())) __attribute__((amdgpu_waves_per_eu(1))) void k_diff_few(const Diff a) {
+__global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu(2))) void k_diff_few(const Diff a) {
   extern __shared__ __align__(16) char lds_block[];
-  constexpr int WAVES = few_waves<DH, DV>(), KT = FEW * 2 * DH, VT = FEW * DV, DB = DV / 32, ROW = few_row<DV>();
+  constexpr int KT = NT * 2 * DH, VT = NT * DV, DB = DV / 32, K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT, ROW = few_row<DV>();
+  typedef typename Mat<T>::Cvt C;
   const int lane = (int)threadIdx.x & 63, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), map = wave & 1, part = wave >> 1;
   const int groups = a.h / a.hk, rows = a.tq * groups;
   const int item = (int)blockIdx.x / a.splits, split = (int)blockIdx.x - item * a.splits, b = item / a.hk, hk = item - b * a.hk;
   const int len = length_of(a, b), start = start_of(a, b);
-  const int s_k = wave * 4 * (KT + VT), s_v = s_k + 4 * KT;   // the wave's two tiles of keys, and of values
   const int row = min(lane & 31, rows - 1), query = row / groups, head = hk * groups + row - query * groups;
-  const T* qp = static_cast<const T*>(a.q.p) + b * a.q.b + query * a.q.t + 2 * head * a.q.h;
-  Kept<T, DH> q[2];
-  q[0].load(qp, a.dh);
-  q[1].load(qp + a.q.h, a.dh);
+  Kept<T, DH> q;
+  q.load(static_cast<const T*>(a.q.p) + b * a.q.b + query * a.q.t + (2 * head + map) * a.q.h, a.dh);
   const int seen = seen_by(a, query, start, len);
   const int c0 = split * a.chunk, c1 = min(c0 + a.chunk, seen_by(a, a.tq - 1, start, len)), least = seen_by(a, 0, start, len);
-  const Rows32<2 * DH> krows;
+  const Rows32<2 * DH> krows(map * (DH / 16));
   const Cols32<DV> vcols;
-  f32x16 o1[DB], o2[DB];
+  f32x16 o[DB];
 #pragma unroll
-  for (int d = 0; d < DB; ++d) o1[d] = o2[d] = zero16();
-  Soft sm1, sm2;
-  const Fill<T, 2 * DH, 2, FEW, 64> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
-  const Fill<T, DV, 1, FEW, 64> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
-  constexpr int LOADS = decltype(kf)::PASSES + decltype(vf)::PASSES;   // of a tile
-  static_assert(LOADS < 64, "what vmcnt counts");
-  const int first = c0 + FEW * wave, step = FEW * WAVES;
-  if (first < c1) {
-    kf.fetch(first, len - 1, s_k);
-    vf.fetch(first, len - 1, s_v);
+  for (int d = 0; d < DB; ++d) o[d] = zero16();
+  Soft sm;
+  const Fill<T, 2 * DH, 2, NT, WG> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
+  const Fill<T, DV, 1, NT, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
+  if (c0 < c1) {
+    kf.fetch(c0, len - 1, K0);
+    vf.fetch(c0, len - 1, V0);
   }
-  int cur = 0;
-  for (int k0 = first; k0 < c1; k0 += step, cur ^= 1) {
-    if (k0 + step < c1) {
-      kf.fetch(k0 + step, len - 1, s_k + (cur ^ 1) * 2 * KT);
-      vf.fetch(k0 + step, len - 1, s_v + (cur ^ 1) * 2 * VT);
-      __builtin_amdgcn_s_waitcnt(0x0f70 | (LOADS & 15) | (LOADS >> 4 << 14));   // vmcnt: all but the next tile's loads
-    } else {
-      __builtin_amdgcn_s_waitcnt(0x0f70);
+  filled();
+  auto tile = [&](int k0, auto buffer) {
+    constexpr int cur = decltype(buffer)::value;
+    if (k0 + NT < c1) {
+      kf.fetch(k0 + NT, len - 1, cur ? K0 : K1);
+      vf.fetch(k0 + NT, len - 1, cur ? V0 : V1);
     }
-    wave_lds_sync();
-    const int kt = s_k + cur * 2 * KT, vt = s_v + cur * 2 * VT;
-    uint4 p1[2], p2[2];
-    auto scores = [&](int map, f32x16 (&s)[1]) {
+    const int k1 = k0 + 32 * part, kt = (cur ? K1 : K0) + 64 * part * 2 * DH, vt = (cur ? V1 : V0) + 64 * part * DV;
+    if (k1 < c1) {
+      f32x16 s[1];
       s[0] = zero16();
 #pragma unroll
-      for (int ks = 0; ks < DH / 16; ++ks) s[0] = Mat<T>::mfma(krows.at(kt, 0, map * (DH / 16) + ks), q[map].f[ks], s[0]);
-      if (k0 + FEW > least) {
-        const int left = seen - k0 - 4 * half;
+      for (int ks = 0; ks < DH / 16; ++ks) s[0] = Mat<T>::mfma(krows.at(kt, 0, ks), q.f[ks], s[0]);
+      if (k1 + 32 > min(least, c1)) {   // past the chunk too: those keys are the next one's
+        const int left = min(seen, c1) - k1 - 4 * half;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (row_of(r, 0) >= left) s[0][r] = -INFINITY;
       }
-    };
-    f32x16 s[1];
-    scores(0, s);
-    soft_step<T>(s, sm1, o1, p1, a.c);
-    scores(1, s);
-    soft_step<T>(s, sm2, o2, p2, a.c);
+      uint4 p[2], rest[2];
+      soft_step<T>(s, sm, o, p, a.c);   // s: the probabilities before their rounding
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w[4] = {p[i].x, p[i].y, p[i].z, p[i].w};
+        uint32_t x[4];
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const uint4 v = vcols.at(vt, 16 * i, 32 * d);
-        o1[d] = Mat<T>::mfma(v, p1[i], o1[d]);
-        o2[d] = Mat<T>::mfma(v, p2[i], o2[d]);
+        for (int k = 0; k < 4; ++k) {
+          float u, v;
+          C::unpack2(w[k], u, v);
+          x[k] = C::pack2(s[0][8 * i + 2 * k] - u, s[0][8 * i + 2 * k + 1] - v);
+        }
+        rest[i] = make_uint4(x[0], x[1], x[2], x[3]);
       }
-    wave_lds_sync();   // the tile's reads are done before the one after the next is loaded over it
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const uint4 v = vcols.at(vt, 16 * i, 32 * d);
+          o[d] = Mat<T>::mfma(v, p[i], o[d]);
+          o[d] = Mat<T>::mfma(v, rest[i], o[d]);
+        }
+    }
+    if (k0 + NT < c1) filled();
+  };
+  for (int k0 = c0; k0 < c1; k0 += 2 * NT) {
+    tile(k0, std::integral_constant<int, 0>());
+    if (k0 + NT < c1) tile(k0 + NT, std::integral_constant<int, 1>());
   }
-  const float l1 = sm1.sum(), l2 = sm2.sum();
-  __syncthreads();
-  float* part = reinterpret_cast<float*>(lds_block);   // [wave][32 rows][ROW]
-  static_assert(few_waves<DH, DV>() * FEW * few_row<DV>() * 4 <= 160 * 1024 && few_lds<DH, DV>() <= 160 * 1024,
-                "the tiles, and the waves' results, in LDS");
+  const float l = sm.sum();
+  __syncthreads();   // the last tile has been read
+  float* mine = reinterpret_cast<float*>(lds_block);   // [wave][32 rows][DV + 2]: o, m, l
   if ((lane & 31) < rows) {
-    float* p = part + (wave * FEW + (lane & 31)) * ROW;
+    float* p = mine + (wave * FEW + (lane & 31)) * (DV + 2);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = 32 * d + 8 * g + 4 * half;
-        *reinterpret_cast<float4*>(p + col) = make_float4(o1[d][4 * g], o1[d][4 * g + 1], o1[d][4 * g + 2], o1[d][4 * g + 3]);
-        *reinterpret_cast<float4*>(p + DV + col) = make_float4(o2[d][4 * g], o2[d][4 * g + 1], o2[d][4 * g + 2], o2[d][4 * g + 3]);
-      }
-    if (half == 0) *reinterpret_cast<float4*>(p + 2 * DV) = make_float4(sm1.m, l1, sm2.m, l2);
+      for (int r = 0; r < 16; ++r) p[32 * d + row_of(r, half)] = o[d][r];
+    if (half == 0) {
+      p[DV] = sm.m;
+      p[DV + 1] = l;
+    }
   }
   __syncthreads();
-  for (int i = (int)threadIdx.x; i < rows * DV; i += 64 * WAVES) {
+  for (int i = (int)threadIdx.x; i < rows * DV; i += WG) {
     const int r = i / DV, col = i - r * DV, qi = r / groups, hd = hk * groups + r - qi * groups;
+    float y[2], m[2], sum[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {   // the map's two waves
+      const float *p0 = mine + (e * FEW + r) * (DV + 2), *p1 = p0 + 2 * FEW * (DV + 2);
+      m[e] = fmaxf(p0[DV], p1[DV]);
+      const float f0 = __builtin_amdgcn_exp2f(p0[DV] - m[e]), f1 = __builtin_amdgcn_exp2f(p1[DV] - m[e]);
+      sum[e] = p0[DV + 1] * f0 + p1[DV + 1] * f1;
+      y[e] = p0[col] * f0 + p1[col] * f1;
+    }
     if (a.splits == 1) {
-      float y1, y2;
-      join_row<DV>([&](int w) { return part + (w * FEW + r) * ROW; }, WAVES, col, y1, y2);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) y[e] = sum[e] > 0.f || sum[e] != sum[e] ? y[e] / sum[e] : 0.f;
       if (col < a.dv)
-        st1(static_cast<T*>(a.out) + (((int64_t)b * a.tq + qi) * a.h + hd) * a.dv + col, y1 - lam_at<T>(a, b, qi, hd) * y2);
-    } else {   // the waves' sums relative to their common maximum
-      float m1 = NONE, m2 = NONE, s1 = 0.f, s2 = 0.f, y1 = 0.f, y2 = 0.f;
-      for (int w = 0; w < WAVES; ++w) {
-        const float* p = part + (w * FEW + r) * ROW + 2 * DV;
-        m1 = fmaxf(m1, p[0]);
-        m2 = fmaxf(m2, p[2]);
-      }
-      for (int w = 0; w < WAVES; ++w) {
-        const float* p = part + (w * FEW + r) * ROW;
-        const float f1 = __builtin_amdgcn_exp2f(p[2 * DV] - m1), f2 = __builtin_amdgcn_exp2f(p[2 * DV + 2] - m2);
-        s1 = __builtin_fmaf(p[2 * DV + 1], f1, s1);
-        s2 = __builtin_fmaf(p[2 * DV + 3], f2, s2);
-        y1 = __builtin_fmaf(p[col], f1, y1);
-        y2 = __builtin_fmaf(p[DV + col], f2, y2);
-      }
-      float* out = a.part + ((int64_t)((item * rows) + r) * a.splits + split) * ROW;
-      out[col] = y1;
-      out[DV + col] = y2;
-      if (col == 0) *reinterpret_cast<float4*>(out + 2 * DV) = make_float4(m1, s1, m2, s2);
+        st1(static_cast<T*>(a.out) + (((int64_t)b * a.tq + qi) * a.h + hd) * a.dv + col, y[0] - lam_at<T>(a, b, qi, hd) * y[1]);
+    } else {
+      float* out = a.part + ((int64_t)(item * rows + r) * a.splits + split) * ROW;
+      out[col] = y[0];
+      out[DV + col] = y[1];
+      if (col == 0) *reinterpret_cast<float4*>(out + 2 * DV) = make_float4(m[0], sum[0], m[1], sum[1]);
     }
   }
 }
 
-// the chunks' partial rows: one workgroup of DV lanes per row
-template <typename T, int DV> __global__ __launch_bounds__(DV) void k_diff_join(const Diff a) {
-  constexpr int ROW = few_row<DV>();
+// the chunks' partial rows as one: their common maxima, then their sums and values relative to them. A workgroup per row, a lane
+// per column of one map
+constexpr int MOST_CHUNKS = 256;
+template <typename T, int DV> __global__ __launch_bounds__(2 * DV) void k_diff_join(const Diff a) {
+  constexpr int ROW = few_row<DV>(), LANES = 2 * DV;
+  __shared__ float s_f[2][MOST_CHUNKS], s_y[DV];
   const int groups = a.h / a.hk, rows = a.tq * groups, item = (int)blockIdx.x / rows, r = (int)blockIdx.x - item * rows;
-  const int b = item / a.hk, hk = item - b * a.hk, query = r / groups, head = hk * groups + r - query * groups, col = (int)threadIdx.x;
-  const float* p = a.part + (int64_t)blockIdx.x * a.splits * ROW;
-  float y1, y2;
-  join_row<DV>([&](int i) { return p + (int64_t)i * ROW; }, a.splits, col, y1, y2);
-  if (col < a.dv)
-    st1(static_cast<T*>(a.out) + (((int64_t)b * a.tq + query) * a.h + head) * a.dv + col, y1 - lam_at<T>(a, b, query, head) * y2);
+  const int b = item / a.hk, hk = item - b * a.hk, query = r / groups, head = hk * groups + r - query * groups;
+  const int tid = (int)threadIdx.x, map = tid / DV, col = tid - map * DV, n = a.splits;
+  const float* p = a.part + (int64_t)blockIdx.x * n * ROW;
+  for (int i = tid; i < 2 * n; i += LANES) s_f[i & 1][i >> 1] = p[(int64_t)(i >> 1) * ROW + 2 * DV + 2 * (i & 1)];
+  __syncthreads();
+  float m = NONE;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, s_f[map][i]);
+  float sum = 0.f, y = 0.f;
+  int i = 0;
+  for (; i + 4 <= n; i += 4) {   // four chunks' loads in flight
+    float x[4], l[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      x[u] = p[(int64_t)(i + u) * ROW + map * DV + col];
+      l[u] = p[(int64_t)(i + u) * ROW + 2 * DV + 2 * map + 1];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float f = __builtin_amdgcn_exp2f(s_f[map][i + u] - m);
+      y = __builtin_fmaf(x[u], f, y);
+      sum = __builtin_fmaf(l[u], f, sum);
+    }
+  }
+  for (; i < n; ++i) {
+    const float f = __builtin_amdgcn_exp2f(s_f[map][i] - m);
+    y = __builtin_fmaf(p[(int64_t)i * ROW + map * DV + col], f, y);
+    sum = __builtin_fmaf(p[(int64_t)i * ROW + 2 * DV + 2 * map + 1], f, sum);
+  }
+  y = sum > 0.f || sum != sum ? y / sum : 0.f;
+  if (map) s_y[col] = y;
+  __syncthreads();
+  if (!map && col < a.dv)
+    st1(static_cast<T*>(a.out) + (((int64_t)b * a.tq + query) * a.h + head) * a.dv + col, y - lam_at<T>(a, b, query, head) * s_y[col]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -1124,13 +1134,13 @@ template <typename K, K KERNEL> int allow_lds(int bytes) {
 }
 #define ALLOW_LDS(BYTES, ...) allow_lds<decltype(&__VA_ARGS__), &__VA_ARGS__>(BYTES)
 
-// chunks of the keys for the kernel of few queries: enough workgroups for the CUs, chunks of 256 keys at least
+// chunks of the keys for the kernel of few queries: workgroups for the CUs twice over, chunks of 256 keys at least
 struct Chunks { int64_t splits, chunk; };
 inline Chunks chunks_of(const lmo_diff_shape* s) {
   const int64_t items = s->b * s->hk, want = (512 + items - 1) / (items > 0 ? items : 1), most = (s->tk + 255) / 256;
   int64_t n = want < most ? want : most;
-  n = n < 1 ? 1 : n;
-  const int64_t chunk = ((s->tk + n - 1) / n + 127) / 128 * 128;
+  n = n < 1 ? 1 : n > MOST_CHUNKS ? MOST_CHUNKS : n;
+  const int64_t chunk = ((s->tk + n - 1) / n + NT - 1) / NT * NT;
   return {(s->tk + chunk - 1) / chunk, chunk};
 }
 // parts of the tiles of queries for dk and dv: those of a causal sequence (positions and lengths are the kernel's to know), so that
@@ -1185,11 +1195,11 @@ int lmo_diff_attn_fwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
     const int64_t grid = s->b * s->hk * n.splits;
     if (grid > 0x7fffffff) return LDR_E_SHAPE;
     DIFF_SWITCH(dtype, s->dh, s->dv, {
-      constexpr int stage = few_lds<DH, DV>(), joined = few_waves<DH, DV>() * FEW * few_row<DV>() * 4, bytes = stage > joined ? stage : joined;
+      constexpr int bytes = few_lds<DH, DV>();
       if ((e = ALLOW_LDS(bytes, k_diff_few<T, DH, DV>))) return e;
-      hipLaunchKernelGGL((k_diff_few<T, DH, DV>), dim3((unsigned)grid), dim3(64 * few_waves<DH, DV>()), bytes, st, a);
+      hipLaunchKernelGGL((k_diff_few<T, DH, DV>), dim3((unsigned)grid), dim3(WG), bytes, st, a);
       if ((e = launched())) return e;
-      if (n.splits > 1) hipLaunchKernelGGL((k_diff_join<T, DV>), dim3((unsigned)(s->b * s->h * s->tq)), dim3(DV), 0, st, a);
+      if (n.splits > 1) hipLaunchKernelGGL((k_diff_join<T, DV>), dim3((unsigned)(s->b * s->h * s->tq)), dim3(2 * DV), 0, st, a);
     })
     return launched();
   }
