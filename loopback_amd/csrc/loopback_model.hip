@@ -226,16 +226,18 @@ __global__ __launch_bounds__(SUM_LANES) void k_layer_norm_sum(const float* __res
 // ---------------------------------------------------------------------------------------------------------------
 constexpr float LOG2E = 1.4426950408889634f;
 
-// what the forward keeps of a row
-struct DistillRow {
-  float kl, ce;           // the row's terms
+// what the forward keeps of a row: its terms (all rows' first, side by side for their mean), and what its gradient needs
+struct DistillTerms {
+  float kl, ce;
   float counts, labelled; // 1 or 0
+};
+struct alignas(16) DistillRow {
   float m, l, l1;         // the maximum, and the logs of the sums of exp((x - m) / tau) and exp(x - m)
   float mr, lr;           // the same of the classes that are not named
   float all, rest;        // P + rest, and rest
   float teacher;          // p_i = exp(top_i / tau - teacher)
 };
-static_assert(sizeof(DistillRow) == LMO_DISTILL_SAVED * sizeof(float), "saved row");
+static_assert(sizeof(DistillTerms) + sizeof(DistillRow) == LMO_DISTILL_SAVED * sizeof(float), "saved row");
 
 struct Sums {   // running maximum, sum of exp((x - m) / tau) and, HARD, of exp(x - m)
   float m = -INFINITY, s = 0.f, s1 = 0.f;
@@ -303,40 +305,75 @@ struct Distill {
   const void *logits, *top, *ids;
   const float* teacher_lse;
   const int64_t* labels;
+  DistillTerms* terms;
   DistillRow* saved;
   const float *coef, *dloss;
   void* dlogits;
   int vocab, k, top_dtype, wide;
   float tau;
+  int64_t row0;   // of this launch's first row
+  int parts;      // the backward's workgroups of a row
 };
 
-template <typename T, int LANES, bool TAIL, bool HARD>
+// U vectors of eight that a lane takes at a time, NT: past the caches
+template <typename T, int LANES, int U, bool NT> struct Vectors {
+  typename IO<T>::Raw r[U];
+  __device__ __forceinline__ void load(const T* x, int v0, int nv) {   // past the end: the last one again
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const T* p = x + 8 * (int64_t)min(v0 + (int)threadIdx.x + u * LANES, nv - 1);
+      r[u] = NT ? UIO<T>::raw_nt(p) : UIO<T>::raw(p);
+    }
+  }
+};
+template <typename T, bool NT> __device__ __forceinline__ void store_stream(T* p, const float (&o)[8]) {
+  if constexpr (!NT) {
+    UIO<T>::store(p, o);
+  } else if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4)
+      __builtin_nontemporal_store(u32x4{__float_as_uint(o[i]), __float_as_uint(o[i + 1]), __float_as_uint(o[i + 2]), __float_as_uint(o[i + 3])},
+                                  reinterpret_cast<u32x4_u32*>(p + i));
+  } else {
+    typedef typename std::conditional<std::is_same<T, bf16_t>::value, Bf16Cvt, F16Cvt>::type Cvt;
+    __builtin_nontemporal_store(u32x4{Cvt::pack2(o[0], o[1]), Cvt::pack2(o[2], o[3]), Cvt::pack2(o[4], o[5]), Cvt::pack2(o[6], o[7])},
+                                reinterpret_cast<u32x4_u16*>(p));
+  }
+}
+
+// POW: 0 no second sum (no labels, or temperature 1, where it is the first); 2 and 4 temperatures whose exp((x - m) / tau), squared
+// once or twice, is the second sum's exponential; 1 any other
+template <typename T, int LANES, bool TAIL, int POW, bool NT>
 __global__ __launch_bounds__(LANES) void k_distill_fwd(const Distill a) {
-  constexpr int WAVES = LANES / 64, U = 4;
+  constexpr int WAVES = LANES / 64, U = sizeof(T) == 4 ? 1 : 2, STEP = U * LANES;
+  constexpr bool HARD = POW != 0;
   extern __shared__ unsigned s_map[];   // TAIL: the named classes' bits, 32 to a word
   __shared__ float red[WAVES];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.row0 + blockIdx.x;
   const int vocab = a.vocab, k = a.k, tid = (int)threadIdx.x, nv = vocab >> 3;
   const T* x = static_cast<const T*>(a.logits) + row * vocab;
   const float c = LOG2E / a.tau, c1 = LOG2E;
   const int64_t label = a.labels ? a.labels[row] : -100;
   // the teacher: which classes count, its maximum and sum
-  float zm = -INFINITY, named = 0.f, bad = 0.f;
+  float zm = -INFINITY, named = 0.f;   // named: 1 with a class that counts, 2 with one past the last
   for (int i = tid; i < k; i += LANES) {
     const int id = id_of(a.ids, a.wide, row * k + i, vocab);
     if (id < 0) continue;
-    named = 1.f;
-    if (id >= vocab) bad = 1.f;
+    named = fmaxf(named, id >= vocab ? 2.f : 1.f);
     zm = fmaxf(zm, ld_as(a.top, row * k + i, a.top_dtype) * c);
   }
-  const bool counts = wg_reduce<MaxOp, WAVES>(named, red, MaxOp()) > 0.f;
+  named = wg_reduce<MaxOp, WAVES>(named, red, MaxOp());
+  const bool counts = named > 0.f;
   const bool labelled = label != -100;
   DistillRow out{};
+  DistillTerms terms{};
   if (!counts && !labelled) {   // workgroup-uniform
-    if (tid == 0) a.saved[row] = out;
+    if (tid == 0) {
+      a.terms[row] = terms;
+      a.saved[row] = out;
+    }
     return;
   }
-  bad = wg_reduce<MaxOp, WAVES>(bad, red, MaxOp());
   if (TAIL) {
     const int words = (vocab + 31) >> 5;
     for (int i = tid; i < words; i += LANES) s_map[i] = 0u;
@@ -354,48 +391,56 @@ __global__ __launch_bounds__(LANES) void k_distill_fwd(const Distill a) {
     others = wg_reduce<AddOp, WAVES>(n, red, AddOp()) < (float)vocab ? 1.f : 0.f;
   }
   Sums s, sn;   // of the classes (TAIL: those not named), and of the named ones
-  auto vec = [&](const typename IO<T>::Raw& r, int v) {
-    float e[8];
-    IO<T>::unpack(r, e);
-    if (TAIL) {
-      const unsigned bits = reinterpret_cast<const unsigned char*>(s_map)[v];
-      if (bits) {
+  auto use = [&](const Vectors<T, LANES, U, NT>& from, int v0) {
+    float e[U][8], mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (bits >> j & 1u) {
-            take<HARD>(sn, e[j], c, c1);
-            e[j] = -INFINITY;
-          }
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + tid + u * LANES;
+      IO<T>::unpack(from.r[u], e[u]);
+      if (v >= nv) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[u][j] = -INFINITY;
+      } else if (TAIL) {
+        const unsigned bits = reinterpret_cast<const unsigned char*>(s_map)[v];
+        if (bits) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (bits >> j & 1u) {
+              take<HARD>(sn, e[u][j], c, c1);
+              e[u][j] = -INFINITY;
+            }
+        }
       }
-    }
-    float mx = e[0];
-    bool nan = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      mx = fmaxf(mx, e[j]);
-      nan |= e[j] != e[j];
+      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, e[u][j]);   // passes a NaN over, which the sums keep
     }
     grow<HARD>(s, mx, c, c1);
     const float m = s.m == -INFINITY ? 0.f : s.m;
-    float t = 0.f, t1 = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      t += __builtin_amdgcn_exp2f((e[j] - m) * c);
-      if (HARD) t1 += __builtin_amdgcn_exp2f((e[j] - m) * c1);
+    for (int u = 0; u < U; ++u) {
+      float t = 0.f, t1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = e[u][j] - m, x1 = __builtin_amdgcn_exp2f(d * c), x2 = x1 * x1;
+        t += x1;
+        if (POW == 1) t1 += __builtin_amdgcn_exp2f(d * c1);
+        else if (POW == 2) t1 = __builtin_fmaf(x1, x1, t1);
+        else if (POW == 4) t1 = __builtin_fmaf(x2, x2, t1);
+      }
+      s.s += t;
+      if (HARD) s.s1 += t1;
     }
-    s.s = nan ? NAN : s.s + t;
-    if (HARD) s.s1 = nan ? NAN : s.s1 + t1;
-    s.m = nan ? m : s.m;   // a NaN stays in the sum, whose maximum has to be a number
   };
-  int v = tid;
-  for (; v + (U - 1) * LANES < nv; v += U * LANES) {   // U loads in flight
-    typename IO<T>::Raw r[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) r[u] = UIO<T>::raw_nt(x + 8 * (int64_t)(v + u * LANES));
-#pragma unroll
-    for (int u = 0; u < U; ++u) vec(r[u], v + u * LANES);
+  if (nv > 0) {   // the next vectors' loads are in flight while these are summed
+    Vectors<T, LANES, U, NT> r0, r1;
+    r0.load(x, 0, nv);
+    for (int v0 = 0; v0 < nv; v0 += 2 * STEP) {   // the same for every lane
+      if (v0 + STEP < nv) r1.load(x, v0 + STEP, nv);
+      use(r0, v0);
+      if (v0 + 2 * STEP < nv) r0.load(x, v0 + 2 * STEP, nv);
+      if (v0 + STEP < nv) use(r1, v0 + STEP);
+    }
   }
-  for (; v < nv; v += LANES) vec(UIO<T>::raw_nt(x + 8 * (int64_t)v), v);
   if (tid < (vocab & 7)) {
     const int i = 8 * nv + tid;
     if (TAIL && (s_map[i >> 5] >> (i & 31) & 1u)) take<HARD>(sn, ld1(x + i), c, c1);
@@ -438,21 +483,24 @@ __global__ __launch_bounds__(LANES) void k_distill_fwd(const Distill a) {
       out.rest = P != P ? P : others * fmaxf(0.f, 1.f - P);
       if (out.rest > 0.f) kl += out.rest * (logf(out.rest) - ((out.mr - out.m) * inv_tau + out.lr - out.l));
     }
-    out.kl = bad > 0.f ? NAN : kl;
+    terms.kl = named > 1.f ? NAN : kl;
     out.all = P + out.rest;
-    out.counts = 1.f;
+    terms.counts = 1.f;
     out.teacher = teacher;
   }
   if (labelled) {
-    out.ce = label >= 0 && label < vocab ? out.l1 + (out.m - ld1(x + label)) : NAN;
-    out.labelled = 1.f;
+    terms.ce = label >= 0 && label < vocab ? out.l1 + (out.m - ld1(x + label)) : NAN;
+    terms.labelled = 1.f;
   }
-  if (tid == 0) a.saved[row] = out;
+  if (tid == 0) {
+    a.terms[row] = terms;
+    a.saved[row] = out;
+  }
 }
 
 // the loss, and what the rows' gradients are multiplied by, by one workgroup: lane sums in order, then a fixed tree
 constexpr int MEAN_LANES = 1024;
-__global__ __launch_bounds__(MEAN_LANES) void k_distill_mean(const DistillRow* __restrict__ saved, int64_t rows, float tau,
+__global__ __launch_bounds__(MEAN_LANES) void k_distill_mean(const DistillTerms* __restrict__ terms, int64_t rows, float tau,
                                                              float hard, float* __restrict__ coef, float* __restrict__ loss) {
   __shared__ float4 s[MEAN_LANES];
   const int tid = (int)threadIdx.x;
@@ -464,14 +512,15 @@ __global__ __launch_bounds__(MEAN_LANES) void k_distill_mean(const DistillRow* _
     p.w += q.w;
   };
   int64_t i = tid;
-  for (; i + 3 * MEAN_LANES < rows; i += 4 * MEAN_LANES) {   // four rows' loads in flight
-    float4 e[4];
+  const float4* row = reinterpret_cast<const float4*>(terms);
+  for (; i + 7 * MEAN_LANES < rows; i += 8 * MEAN_LANES) {   // eight rows' loads in flight
+    float4 e[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) e[u] = *reinterpret_cast<const float4*>(saved + i + u * MEAN_LANES);
+    for (int u = 0; u < 8; ++u) e[u] = row[i + u * MEAN_LANES];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) add(a, e[u]);
+    for (int u = 0; u < 8; ++u) add(a, e[u]);
   }
-  for (; i < rows; i += MEAN_LANES) add(a, *reinterpret_cast<const float4*>(saved + i));
+  for (; i < rows; i += MEAN_LANES) add(a, row[i]);
   s[tid] = a;
   __syncthreads();
   for (int w = MEAN_LANES / 2; w > 0; w >>= 1) {
@@ -487,70 +536,82 @@ __global__ __launch_bounds__(MEAN_LANES) void k_distill_mean(const DistillRow* _
   }
 }
 
-template <typename T, int LANES, bool TAIL, bool HARD>
-__global__ __launch_bounds__(LANES) void k_distill_bwd(const Distill a) {
-  constexpr int U = 4;
+// A class that is neither named nor the label gets F softmax(x / tau) + gb softmax(x). TAIL: its share of the teacher's rest
+// goes with the softmax of the classes that are not named, of which softmax(x / tau) is the 2^-D'th part (D >= 0), so one exponential
+// carries both. HARD: the labels' softmax is another one; at temperature 1 it is the same and in F too.
+// A workgroup takes U vectors a lane of one row, a.parts workgroups in turn a row: what all of them have in flight lies close together.
+template <typename T> constexpr int BWD_AT_ONCE = sizeof(T) == 4 ? 2 : 4;
+template <typename T, bool TAIL, bool HARD, bool NT> __global__ __launch_bounds__(WG) void k_distill_bwd(const Distill a) {
+  constexpr int U = BWD_AT_ONCE<T>, STEP = U * WG;
   extern __shared__ unsigned s_dyn[];   // k ids, k probabilities
   int* s_id = reinterpret_cast<int*>(s_dyn);
   float* s_p = reinterpret_cast<float*>(s_dyn) + a.k;
-  const int64_t row = blockIdx.x;
-  const int vocab = a.vocab, k = a.k, tid = (int)threadIdx.x, nv = vocab >> 3;
+  const int64_t row = a.row0 + blockIdx.x / a.parts;
+  const int vocab = a.vocab, tid = (int)threadIdx.x, nv = vocab >> 3, part = (int)blockIdx.x % a.parts;
+  const int v0 = part * STEP, c0 = 8 * v0, c1 = part == a.parts - 1 ? vocab : c0 + 8 * STEP;   // vectors from v0, classes c0 to c1
   const T* x = static_cast<const T*>(a.logits) + row * vocab;
   T* o = static_cast<T*>(a.dlogits) + row * vocab;
+  Vectors<T, WG, U, NT> raw;
+  if (nv > 0) raw.load(x, v0, nv);
+  const DistillTerms n = a.terms[row];
   const DistillRow r = a.saved[row];
   const float g = *a.dloss, zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (r.counts == 0.f && r.labelled == 0.f) {   // workgroup-uniform
-    for (int v = tid; v < nv; v += LANES) UIO<T>::store(o + 8 * (int64_t)v, zero);
-    if (tid < (vocab & 7)) st1(o + 8 * nv + tid, 0.f);
+  const bool labelled = a.labels && n.labelled != 0.f;
+  if (n.counts == 0.f && !labelled) {   // workgroup-uniform
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + tid + u * WG < nv) store_stream<T, NT>(o + 8 * (int64_t)(v0 + tid + u * WG), zero);
+    if (c1 == vocab && tid < (vocab & 7)) st1(o + 8 * (int64_t)nv + tid, 0.f);
     return;
   }
+  const int k = n.counts != 0.f ? a.k : 0;
   const float inv_tau = 1.f / a.tau, c = LOG2E / a.tau;
-  const float ga = r.counts != 0.f ? g * a.coef[0] : 0.f, gb = HARD && r.labelled != 0.f ? g * a.coef[1] : 0.f;
-  const float qa = ga * r.all, ra = TAIL ? ga * r.rest : 0.f;   // factors of softmax(x / tau), and of the others' own softmax
-  const int64_t label = HARD && r.labelled != 0.f ? a.labels[row] : -1;
-  const float l2 = r.l * LOG2E, l12 = r.l1 * LOG2E, lr2 = r.lr * LOG2E;
-  if (r.counts != 0.f)
-    for (int i = tid; i < k; i += LANES) {
-      const int id = id_of(a.ids, a.wide, row * k + i, vocab);
-      s_id[i] = id;
-      s_p[i] = id < 0 ? 0.f : expf(ld_as(a.top, row * k + i, a.top_dtype) * inv_tau - r.teacher);
-    }
-  // the gradient at class i of logit e; `named`: less p, its teacher's probability, instead of the others' share
-  auto grad = [&](float e, int64_t i, bool named, float p) {
-    float t = qa * __builtin_amdgcn_exp2f((e - r.m) * c - l2);
-    if (HARD) t += gb * (__builtin_amdgcn_exp2f((e - r.m) * LOG2E - l12) - (i == label ? 1.f : 0.f));
-    if (named) t -= ga * p;
-    else if (TAIL) t -= r.rest > 0.f ? ra * __builtin_amdgcn_exp2f((e - r.mr) * c - lr2) : 0.f;
+  const float ga = k ? g * a.coef[0] : 0.f, gb = labelled ? g * a.coef[1] : 0.f;
+  const float qa = ga * r.all, l2 = r.l * LOG2E, l12 = r.l1 * LOG2E, lr2 = r.lr * LOG2E;
+  const bool rest = TAIL && r.rest > 0.f;
+  const float share = rest ? __builtin_amdgcn_exp2f((r.mr - r.m) * c + (lr2 - l2)) : 1.f;   // 2^-D
+  const float base = rest ? r.mr : r.m, lb = rest ? lr2 : l2, minus = rest ? ga * r.rest : 0.f;
+  const float unnamed = qa * share - minus, F = HARD ? unnamed : (qa + gb) * share - minus;
+  const int64_t label = labelled ? a.labels[row] : -1;
+  for (int i = tid; i < k; i += WG) {
+    const int id = id_of(a.ids, a.wide, row * k + i, vocab);
+    const bool here = id >= c0 && id < c1;
+    s_id[i] = here ? id : -1;
+    s_p[i] = here ? expf(ld_as(a.top, row * k + i, a.top_dtype) * inv_tau - r.teacher) : 0.f;
+  }
+  auto grad = [&](float e) {
+    float t = F * __builtin_amdgcn_exp2f((e - base) * c - lb);
+    if (HARD) t = __builtin_fmaf(gb, __builtin_amdgcn_exp2f((e - r.m) * LOG2E - l12), t);
     return t;
   };
-  auto vec = [&](const typename IO<T>::Raw& raw, int v) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int v = v0 + tid + u * WG;
     float e[8];
-    IO<T>::unpack(raw, e);
+    IO<T>::unpack(raw.r[u], e);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = grad(e[j], 8 * (int64_t)v + j, false, 0.f);
-    UIO<T>::store(o + 8 * (int64_t)v, e);
-  };
-  int v = tid;
-  for (; v + (U - 1) * LANES < nv; v += U * LANES) {   // U loads in flight
-    typename IO<T>::Raw raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = UIO<T>::raw_nt(x + 8 * (int64_t)(v + u * LANES));
-#pragma unroll
-    for (int u = 0; u < U; ++u) vec(raw[u], v + u * LANES);
+    for (int j = 0; j < 8; ++j) e[j] = grad(e[j]);
+    if (v < nv) store_stream<T, NT>(o + 8 * (int64_t)v, e);
   }
-  for (; v < nv; v += LANES) vec(UIO<T>::raw_nt(x + 8 * (int64_t)v), v);
-  if (tid < (vocab & 7)) {
+  if (c1 == vocab && tid < (vocab & 7)) {
     const int64_t i = 8 * (int64_t)nv + tid;
-    st1(o + i, grad(ld1(x + i), i, false, 0.f));
+    st1(o + i, grad(ld1(x + i)));
   }
-  if (r.counts == 0.f) return;
   __syncthreads();   // orders the row's stores before those below, and the named classes in LDS
-  for (int i = tid; i < k; i += LANES) {
-    const int id = s_id[i];
-    if (id < 0 || id >= vocab) continue;
+  for (int i = tid; i <= k; i += WG) {   // the named classes, and the label
+    const int64_t id = i < k ? s_id[i] : label;
+    if (id < c0 || id >= c1) continue;
     float p = 0.f;
-    for (int j = 0; j < k; ++j) p += s_id[j] == id ? s_p[j] : 0.f;   // a class named twice: both write the same value
-    st1(o + id, grad(ld1(x + id), id, true, p));
+    bool named = false;
+    for (int j = 0; j < k; ++j)   // a class named twice, or the label named: all write the same value
+      if (s_id[j] == id) {
+        p += s_p[j];
+        named = true;
+      }
+    const float e = ld1(x + id);
+    float t = named ? qa * __builtin_amdgcn_exp2f((e - r.m) * c - l2) - ga * p : unnamed * __builtin_amdgcn_exp2f((e - base) * c - lb);
+    if (labelled) t += gb * (__builtin_amdgcn_exp2f((e - r.m) * LOG2E - l12) - (id == label ? 1.f : 0.f));
+    st1(o + id, t);
   }
 }
 
@@ -567,6 +628,13 @@ inline int launched() { return (int)hipGetLastError(); }
 #define LMO_BOOL_SWITCH(V, NAME, ...)                            \
   if (V) { constexpr bool NAME = true; __VA_ARGS__; }            \
   else { constexpr bool NAME = false; __VA_ARGS__; }
+#define LMO_POW_SWITCH(P, ...)                         \
+  switch (P) {                                         \
+    case 0: { constexpr int POW = 0; __VA_ARGS__; } break; \
+    case 2: { constexpr int POW = 2; __VA_ARGS__; } break; \
+    case 4: { constexpr int POW = 4; __VA_ARGS__; } break; \
+    default: { constexpr int POW = 1; __VA_ARGS__; } break; \
+  }
 #define LMO_LANES_SWITCH(N, V, ...)                                                   \
   switch (N) {                                                                        \
     case 4: { constexpr int LPR = 4, VPT = 1; __VA_ARGS__; } break;                   \
@@ -600,6 +668,12 @@ int norm_shape(int64_t rows, int64_t d, int dtype) {
   return LDR_OK;
 }
 
+// rows go to the launches so many workgroups at a time
+constexpr int64_t MOST_GROUPS = 1 << 22;
+// logits that the 256 MB of the last cache do not hold beside their gradient go past the caches
+inline bool past_caches(int64_t rows, int64_t vocab, int dtype) {
+  return rows * vocab > (int64_t)(dtype == LDR_F32 ? 32 : 64) << 20;
+}
 // workgroups of 1024 lanes where there are too few rows for the CUs, of 256 otherwise
 inline bool wide_workgroups(int64_t rows) { return rows <= 512; }
 
@@ -683,25 +757,29 @@ int lmo_layer_norm_bwd(const void* dy, const void* h, const void* w, const float
 int lmo_distill_fwd(const void* logits, const void* top, int top_dtype, const void* ids, int wide_ids,
                     const float* teacher_lse, const int64_t* labels, float tau, float hard, float* saved, float* coef,
                     float* loss, int64_t rows, int64_t vocab, int64_t k, int dtype, void* stream) {
-  const Distill a{logits, top, ids, teacher_lse, labels, reinterpret_cast<DistillRow*>(saved), nullptr, nullptr, nullptr,
-                  (int)vocab, (int)k, top_dtype, wide_ids, tau};
+  Distill a{logits, top, ids, teacher_lse, labels, reinterpret_cast<DistillTerms*>(saved),
+            reinterpret_cast<DistillRow*>(saved + 4 * rows), nullptr, nullptr, nullptr,
+                  (int)vocab, (int)k, top_dtype, wide_ids, tau, 0, 1};
   const int e = distill_args(a, rows, vocab, k, dtype, teacher_lse != nullptr);
   if (e) return e;
   if (!coef || !loss || !(hard >= 0.f && hard <= 1.f)) return LDR_E_ARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (rows > 0) {
-    const size_t map = teacher_lse ? ((size_t)vocab + 31) / 32 * 4 : 0;
-    // at temperature 1 the two sums are one
-    LMO_TYPE_SWITCH(dtype, LMO_BOOL_SWITCH(teacher_lse != nullptr, TAIL, LMO_BOOL_SWITCH(labels != nullptr && tau != 1.f, HARD, {
+  const size_t map = teacher_lse ? ((size_t)vocab + 31) / 32 * 4 : 0;
+  const int pow = !labels || tau == 1.f ? 0 : tau == 2.f ? 2 : tau == 4.f ? 4 : 1;
+  for (; a.row0 < rows; a.row0 += MOST_GROUPS) {
+    const unsigned grid = (unsigned)(rows - a.row0 < MOST_GROUPS ? rows - a.row0 : MOST_GROUPS);
+    LMO_TYPE_SWITCH(dtype, LMO_BOOL_SWITCH(teacher_lse != nullptr, TAIL, LMO_POW_SWITCH(pow, {
       if (wide_workgroups(rows))
-        hipLaunchKernelGGL((k_distill_fwd<T, 1024, TAIL, HARD>), dim3((unsigned)rows), dim3(1024), map, st, a);
+        hipLaunchKernelGGL((k_distill_fwd<T, 1024, TAIL, POW, false>), dim3(grid), dim3(1024), map, st, a);
+      else if (past_caches(rows, vocab, dtype))
+        hipLaunchKernelGGL((k_distill_fwd<T, WG, TAIL, POW, true>), dim3(grid), dim3(WG), map, st, a);
       else
-        hipLaunchKernelGGL((k_distill_fwd<T, 256, TAIL, HARD>), dim3((unsigned)rows), dim3(256), map, st, a);
+        hipLaunchKernelGGL((k_distill_fwd<T, WG, TAIL, POW, false>), dim3(grid), dim3(WG), map, st, a);
     })))
     const int err = launched();
     if (err) return err;
   }
-  hipLaunchKernelGGL(k_distill_mean, dim3(1), dim3(MEAN_LANES), 0, st, reinterpret_cast<const DistillRow*>(saved), rows, tau, hard,
+  hipLaunchKernelGGL(k_distill_mean, dim3(1), dim3(MEAN_LANES), 0, st, a.terms, rows, tau, hard,
                      coef, loss);
   return launched();
 }
@@ -709,20 +787,25 @@ int lmo_distill_fwd(const void* logits, const void* top, int top_dtype, const vo
 int lmo_distill_bwd(const void* logits, const void* top, int top_dtype, const void* ids, int wide_ids,
                     const int64_t* labels, float tau, const float* saved, const float* coef, const float* dloss,
                     void* dlogits, int64_t rows, int64_t vocab, int64_t k, int tail, int dtype, void* stream) {
-  const Distill a{logits, top, ids, nullptr, labels, reinterpret_cast<DistillRow*>(const_cast<float*>(saved)), coef, dloss,
-                  dlogits, (int)vocab, (int)k, top_dtype, wide_ids, tau};
+  Distill a{logits, top, ids, nullptr, labels, reinterpret_cast<DistillTerms*>(const_cast<float*>(saved)),
+            reinterpret_cast<DistillRow*>(const_cast<float*>(saved) + 4 * rows), coef, dloss,
+                  dlogits, (int)vocab, (int)k, top_dtype, wide_ids, tau, 0, 1};
   const int e = distill_args(a, rows, vocab, k, dtype, tail != 0);
   if (e || rows == 0) return e;
   if (!coef || !dloss || !dlogits) return LDR_E_ARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const size_t lds = 8 * (size_t)k;
-  LMO_TYPE_SWITCH(dtype, LMO_BOOL_SWITCH(tail != 0, TAIL, LMO_BOOL_SWITCH(labels != nullptr, HARD, {
-    if (wide_workgroups(rows))
-      hipLaunchKernelGGL((k_distill_bwd<T, 1024, TAIL, HARD>), dim3((unsigned)rows), dim3(1024), lds, st, a);
-    else
-      hipLaunchKernelGGL((k_distill_bwd<T, 256, TAIL, HARD>), dim3((unsigned)rows), dim3(256), lds, st, a);
-  })))
-  return launched();
+  const int64_t step = 8 * WG * (dtype == LDR_F32 ? BWD_AT_ONCE<float> : BWD_AT_ONCE<bf16_t>);
+  a.parts = (int)((vocab + step - 1) / step);
+  for (const int64_t most = MOST_GROUPS / a.parts > 0 ? MOST_GROUPS / a.parts : 1; a.row0 < rows; a.row0 += most) {
+    const unsigned grid = (unsigned)(rows - a.row0 < most ? rows - a.row0 : most) * (unsigned)a.parts;
+    LMO_TYPE_SWITCH(dtype, LMO_BOOL_SWITCH(tail != 0, TAIL, LMO_BOOL_SWITCH(labels != nullptr && tau != 1.f, HARD,
+        LMO_BOOL_SWITCH(past_caches(rows, vocab, dtype), NT,
+            hipLaunchKernelGGL((k_distill_bwd<T, TAIL, HARD, NT>), dim3(grid), dim3(WG), lds, st, a)))))
+    const int err = launched();
+    if (err) return err;
+  }
+  return LDR_OK;
 }
 
 }  // extern "C"
