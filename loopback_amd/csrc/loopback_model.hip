@@ -101,7 +101,7 @@ template <typename T> struct NormBwd {
 // meet in LDS, one partial row a workgroup.
 template <typename T, int LPR, int VPT, bool AL>
 __global__ __launch_bounds__(lanes_of(LPR)) void k_layer_norm_bwd(const NormBwd<T> a) {
-  constexpr int LANES = lanes_of(LPR), R = LANES / LPR, W = 8 * LPR;
+  constexpr int LANES = lanes_of(LPR), R = LANES / LPR, W = 8 * LPR * VPT;
   __shared__ float s_red[2][LANES / 64];
   __shared__ float s_sum[R > 1 ? R * W : 1];
   RowSum<LPR> row_sum{s_red};
@@ -170,9 +170,9 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_layer_norm_bwd(const NormBwd<
 #pragma unroll
       for (int v = 0; v < VPT; ++v) store8<float, AL>(out, 8 * (lane + LPR * v), d, acc[v]);
     } else {
-      static_assert(VPT == 1, "several rows to a workgroup only where a lane has one vector");
       __syncthreads();
-      IO<float>::store(s_sum + grp * W + 8 * lane, acc[0]);
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) IO<float>::store(s_sum + grp * W + 8 * (lane + LPR * v), acc[v]);
       __syncthreads();
       for (int c = (int)threadIdx.x; c < d; c += LANES) {
         float s = s_sum[c];
@@ -185,9 +185,10 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_layer_norm_bwd(const NormBwd<
   if (a.part_b) flush(db, a.part_b + (int64_t)blockIdx.x * d);
 }
 
-// dw (blockIdx.y 0) and db (1): the workgroups' partial rows summed in order by 64 groups for 16 columns, then the groups
-constexpr int SUM_LANES = 1024, SUM_COLS = 16;
-template <typename T>
+// dw (blockIdx.y 0) and db (1): the workgroups' partial rows summed in order by a workgroup's groups of COLS lanes, then the groups.
+// Wide rows take whole lines of 256 bytes; of narrow ones the workgroups would be too few
+constexpr int SUM_LANES = 1024;
+template <typename T, int SUM_COLS>
 __global__ __launch_bounds__(SUM_LANES) void k_layer_norm_sum(const float* __restrict__ part_w, const float* __restrict__ part_b,
                                                               T* __restrict__ dw, T* __restrict__ db, int parts, int d) {
   constexpr int GROUPS = SUM_LANES / SUM_COLS;
@@ -618,6 +619,7 @@ template <typename T, bool TAIL, bool HARD, bool NT> __global__ __launch_bounds_
 inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool al_of(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == LDR_F32 ? 3u : 1u)) == 0; }
 inline bool dtype_ok(int dt) { return dt == LDR_F32 || dt == LDR_BF16 || dt == LDR_F16; }
+constexpr int64_t MOST_GROUPS = 1 << 22;   // of a launch: its lanes are counted in 32 bits
 inline unsigned grid_of(int64_t blocks, int64_t cap) { return (unsigned)(blocks < cap ? blocks : cap); }
 inline int launched() { return (int)hipGetLastError(); }
 
@@ -635,28 +637,33 @@ inline int launched() { return (int)hipGetLastError(); }
     case 4: { constexpr int POW = 4; __VA_ARGS__; } break; \
     default: { constexpr int POW = 1; __VA_ARGS__; } break; \
   }
-#define LMO_LANES_SWITCH(N, V, ...)                                                   \
-  switch (N) {                                                                        \
-    case 4: { constexpr int LPR = 4, VPT = 1; __VA_ARGS__; } break;                   \
-    case 16: { constexpr int LPR = 16, VPT = 1; __VA_ARGS__; } break;                 \
-    case 64: { constexpr int LPR = 64, VPT = 1; __VA_ARGS__; } break;                 \
-    case 128: { constexpr int LPR = 128, VPT = 1; __VA_ARGS__; } break;               \
-    case 256: { constexpr int LPR = 256, VPT = 1; __VA_ARGS__; } break;               \
-    case 512: { constexpr int LPR = 512, VPT = 1; __VA_ARGS__; } break;               \
-    default:                                                                          \
-      if ((V) == 1) { constexpr int LPR = 1024, VPT = 1; __VA_ARGS__; }               \
-      else { constexpr int LPR = 1024, VPT = 2; __VA_ARGS__; }                        \
-      break;                                                                          \
-  }
+#define LMO_CASE(L, V, ...) case 8 * L + V: { constexpr int LPR = L, VPT = V; __VA_ARGS__; } break;
+#define LMO_LANES_SWITCH(S, ...)                                                                                           \
+  switch (8 * (S).lpr + (S).vpt) {                                                                                         \
+    LMO_CASE(4, 1, __VA_ARGS__) LMO_CASE(16, 1, __VA_ARGS__) LMO_CASE(64, 1, __VA_ARGS__) LMO_CASE(128, 2, __VA_ARGS__)    \
+    LMO_CASE(256, 2, __VA_ARGS__) LMO_CASE(512, 4, __VA_ARGS__)
 
-// lanes per row, eight columns each (twice eight past 8192): 4, 16 or 64 of a wave, or 2 to 16 waves
-inline int lanes_per_row(int64_t d) {
-  return d <= 32 ? 4 : d <= 128 ? 16 : d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024;
+// Lanes to a row, and vectors of eight columns to a lane. Few lanes with several loads each in flight beat many lanes with one, whose
+// rows are a load and two barriers long (30000 x 2048 bf16 backward: 128 lanes 71 us, 256 100; 4096 x 16384: 512 lanes 97 us, 1024 250),
+// until the backward's column sums leave too few waves. Rows of up to 1024 columns are one wave's in the backward (no barriers: 21.5 us
+// for 16384 x 768, 26 with two); the forward, which has no sums to keep, is faster with two (18.4 and 19.5).
+struct Lanes { int lpr, vpt; };
+inline Lanes lanes_of_row(int64_t rows, int64_t d, bool backward) {
+  if (d <= 32) return {4, 1};
+  if (d <= 128) return {16, 1};
+  if (d <= 512) return {64, 1};
+  if (d <= 1024) return backward ? Lanes{64, 2} : Lanes{128, 1};
+  if (d <= 2048) return backward || rows > 256 ? Lanes{128, 2} : Lanes{256, 1};   // 1 x 2048: 3.0 and 2.2 us
+  if (d <= 4096) return {256, 2};
+  if (d <= 8192) return backward ? Lanes{256, 4} : Lanes{512, 2};
+  return {512, 4};
 }
-struct Plan { int64_t per, parts; };   // the backward's consecutive rows of a workgroup, and its workgroups
+// The backward's consecutive rows of a workgroup, and its workgroups: as many as run at once (3 to a CU, 2 of the wider rows, whose
+// partial sums cost more too, 1 of the widest).
+struct Plan { int64_t per, parts; };
 inline Plan plan_of(int64_t rows, int64_t d) {
-  const int lpr = lanes_per_row(d), r = lpr > WG ? 1 : WG / lpr;
-  const int64_t most = lpr > 512 ? 256 : lpr > WG ? 384 : 768;
+  const int lpr = lanes_of_row(rows, d, true).lpr, r = lpr > WG ? 1 : WG / lpr;
+  const int64_t most = d <= 1024 ? 768 : d <= 8192 ? 512 : 256;
   int64_t per = (rows + most - 1) / most;
   per = (per + r - 1) / r * r;
   return Plan{per, (rows + per - 1) / per};
@@ -668,8 +675,6 @@ int norm_shape(int64_t rows, int64_t d, int dtype) {
   return LDR_OK;
 }
 
-// rows go to the launches so many workgroups at a time
-constexpr int64_t MOST_GROUPS = 1 << 22;
 // logits that the 256 MB of the last cache do not hold beside their gradient go past the caches
 inline bool past_caches(int64_t rows, int64_t vocab, int dtype) {
   return rows * vocab > (int64_t)(dtype == LDR_F32 ? 32 : 64) << 20;
@@ -707,14 +712,20 @@ int lmo_layer_norm_fwd(const void* x, const void* add, const void* w, const void
     al = al && al16(p);
   }
   if (reinterpret_cast<uintptr_t>(stats) & 7u) return LDR_E_ALIGN;
-  const int lpr = lanes_per_row(d), r = lpr > WG ? 1 : WG / lpr;
-  const unsigned grid = grid_of((rows + r - 1) / r, lpr > WG ? 1024 : 2048);
+  const Lanes lanes = lanes_of_row(rows, d, false);
+  const int lpr = lanes.lpr, r = lpr > WG ? 1 : WG / lpr;
+  const unsigned grid = grid_of((rows + r - 1) / r, MOST_GROUPS / 4);
   hipStream_t st = static_cast<hipStream_t>(stream);
   LMO_TYPE_SWITCH(dtype, {
     const NormFwd<T> a{static_cast<const T*>(x), static_cast<const T*>(add), static_cast<const T*>(w), static_cast<const T*>(b),
                        static_cast<T*>(h_out), static_cast<T*>(y), stats, (int)rows, (int)d, eps};
-    LMO_LANES_SWITCH(lpr, d <= 8192 ? 1 : 2,
-        LMO_BOOL_SWITCH(al, AL, hipLaunchKernelGGL((k_layer_norm_fwd<T, LPR, VPT, AL>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a)))
+    LMO_BOOL_SWITCH(al, AL, {
+      LMO_LANES_SWITCH(lanes, hipLaunchKernelGGL((k_layer_norm_fwd<T, LPR, VPT, AL>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a))
+      LMO_CASE(128, 1, hipLaunchKernelGGL((k_layer_norm_fwd<T, LPR, VPT, AL>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a))
+      LMO_CASE(256, 1, hipLaunchKernelGGL((k_layer_norm_fwd<T, LPR, VPT, AL>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a))
+      LMO_CASE(512, 2, hipLaunchKernelGGL((k_layer_norm_fwd<T, LPR, VPT, AL>), dim3(grid), dim3(lanes_of(LPR)), 0, st, a))
+      }
+    })
   })
   return launched();
 }
@@ -743,13 +754,20 @@ int lmo_layer_norm_bwd(const void* dy, const void* h, const void* w, const float
     const NormBwd<T> a{static_cast<const T*>(dy), static_cast<const T*>(h), static_cast<const T*>(w), stats,
                        static_cast<const T*>(dres), static_cast<T*>(dx), dw ? scratch : nullptr,
                        db ? scratch + parts * d : nullptr, (int)rows, (int)d, (int)plan.per};
-    LMO_LANES_SWITCH(lanes_per_row(d), d <= 8192 ? 1 : 2,
-        LMO_BOOL_SWITCH(al, AL, hipLaunchKernelGGL((k_layer_norm_bwd<T, LPR, VPT, AL>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a)))
+    LMO_BOOL_SWITCH(al, AL, {
+      LMO_LANES_SWITCH(lanes_of_row(rows, d, true), hipLaunchKernelGGL((k_layer_norm_bwd<T, LPR, VPT, AL>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
+      LMO_CASE(64, 2, hipLaunchKernelGGL((k_layer_norm_bwd<T, LPR, VPT, AL>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
+      LMO_CASE(256, 4, hipLaunchKernelGGL((k_layer_norm_bwd<T, LPR, VPT, AL>), dim3(parts), dim3(lanes_of(LPR)), 0, st, a))
+      }
+    })
     const int err = launched();
     if (err) return err;
     if (dw || db)
-      hipLaunchKernelGGL(k_layer_norm_sum<T>, dim3((unsigned)((d + SUM_COLS - 1) / SUM_COLS), 2), dim3(SUM_LANES), 0, st, a.part_w,
-                         a.part_b, static_cast<T*>(dw), static_cast<T*>(db), parts, (int)d);
+      LMO_BOOL_SWITCH(d > 2048, WIDE, {
+        constexpr int COLS = WIDE ? 64 : 16;
+        hipLaunchKernelGGL((k_layer_norm_sum<T, COLS>), dim3((unsigned)((d + COLS - 1) / COLS), 2), dim3(SUM_LANES), 0, st, a.part_w,
+                           a.part_b, static_cast<T*>(dw), static_cast<T*>(db), parts, (int)d);
+      })
   })
   return launched();
 }
