@@ -17,10 +17,13 @@ memory-efficient kernels in 16-bit (never the math path's batched products in bf
 
 Options that the reference's model has not (all off by default): the MLP as one operator (`ffn="fused"`), a norm after each
 attention and MLP (`post_norm`), a learned gate per channel on their outputs (`gate`, its first value), a scale of what joins
-the residual stream (`residual_scale`) and dropout on the embedding and on what joins (`dropout`), all from block_ops.
+the residual stream (`residual_scale`) and dropout on the embedding and on what joins (`dropout`), all from block_ops; layer norms
+(`norm="layer"`), differential attention (`attention="differential"`: the heads in pairs, one's map less lambda of the other's) and a
+training step towards a teacher's highest logits (`LoopbackLM.distill`), from model_ops.
 
     python -m loopback_amd.lm --steps 10 --warmup 3            # config 5: the Loopback LM step, tokens/s
     python -m loopback_amd.lm --ffn fused --post-norm --gate 0.5 --dropout 0.1   # the same with these options
+    python -m loopback_amd.lm --norm layer --attention differential --teacher-top 64 --temperature 2 --hard-weight 0.5
     python -m loopback_amd.lm --residual none                  # the same model as Plain Loop
     python -m loopback_amd.lm --prefill --batch 8 --seq 4096 [--graph]   # no-grad forward, tokens/s
 """
@@ -37,7 +40,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import block_ops
+from . import block_ops, model_ops
 from . import lm_ops as ops
 from .cell import LoopDeltaAttnRes
 
@@ -64,6 +67,9 @@ class LMConfig:
     gate: float | None = None      # a learned gate per channel on that output, from this value
     residual_scale: float = 1.0
     dropout: float = 0.0           # of the embedding and of what joins the residual stream, in training
+    norm: str = "rms"              # "layer": layer norms, with a bias
+    attention: str = "softmax"     # "differential": heads in pairs (model_ops.diff_attention)
+    attention_lambda: float = 0.5  # the learned lambda of a pair, its first value
 
     def __post_init__(self):
         if self.hidden_size % self.num_heads:
@@ -80,6 +86,12 @@ class LMConfig:
             raise ValueError(f"ffn must be 'composed' or 'fused', got {self.ffn!r}")
         if not 0.0 <= float(self.dropout) < 1.0:
             raise ValueError(f"dropout must be in [0, 1), got {self.dropout}")
+        if self.norm not in ("rms", "layer"):
+            raise ValueError(f"norm must be 'rms' or 'layer', got {self.norm!r}")
+        if self.attention not in ("softmax", "differential"):
+            raise ValueError(f"attention must be 'softmax' or 'differential', got {self.attention!r}")
+        if self.attention == "differential" and self.num_heads % 2:
+            raise ValueError(f"differential attention takes its heads in pairs, got num_heads {self.num_heads}")
 
     @property
     def intermediate(self) -> int:
@@ -198,6 +210,27 @@ class Attention(nn.Module):
         return a.transpose(1, 2).reshape(B, T, self.h * self.dh)
 
 
+class DiffAttention(Attention):
+    """Differential attention: heads 2 j and 2 j + 1 are the two maps of pair j, whose values are both heads' together; a learned
+    lambda per pair, and an RMSNorm of each pair's output, which the difference of two maps leaves small."""
+
+    def __init__(self, cfg: LMConfig):
+        super().__init__(cfg)
+        self.lam = nn.Parameter(torch.full((self.h // 2,), float(cfg.attention_lambda)))
+        self.head_norm = nn.RMSNorm(2 * self.dh, eps=cfg.norm_eps)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return linear(self.o, self.attend(linear(self.qkv, x)))
+
+    def attend(self, qkv: torch.Tensor) -> torch.Tensor:
+        B, T, _ = qkv.shape
+        heads = qkv.view(B, T, 3, self.h, self.dh)
+        q, k = self.rotary(heads[:, :, :2]).unbind(2)
+        v = heads[:, :, 2].view(B, T, self.h // 2, 2 * self.dh)
+        y = model_ops.diff_attention(q, k, v, self.lam)
+        return add_norm(self.head_norm, y)[1].reshape(B, T, self.h * self.dh)
+
+
 class SwiGLU(nn.Module):
     fused = False
 
@@ -232,8 +265,15 @@ def add_norm(norm: nn.Module, x: torch.Tensor, add: torch.Tensor | None = None):
     that comes back along the first output joins the norm's in one, unless the norm's call is hooked."""
     if type(norm) in (nn.RMSNorm, RMSNorm) and ops.norm_native(x, norm.weight, add, norm.eps) and not _hooked(norm):
         return ops.add_rms_norm(x, add, norm.weight, norm.eps)
+    if (type(norm) is nn.LayerNorm and len(norm.normalized_shape) == 1 and not _hooked(norm)
+            and model_ops.norm_native(x, add, norm.weight, norm.bias)):
+        return model_ops.add_layer_norm(x, add, norm.weight, norm.bias, norm.eps)
     h = x if add is None else x + add
     return h, norm(h)
+
+
+def make_norm(cfg: LMConfig) -> nn.Module:
+    return (nn.LayerNorm if cfg.norm == "layer" else nn.RMSNorm)(cfg.hidden_size, eps=cfg.norm_eps)
 
 
 def join_norm(norm: nn.Module | None, x: torch.Tensor, y: torch.Tensor, post: nn.Module | None = None, **how):
@@ -249,15 +289,18 @@ def join_norm(norm: nn.Module | None, x: torch.Tensor, y: torch.Tensor, post: nn
         y = y if how.get("gate") is None else y * how["gate"]
         h = x + y * how.get("scale", 1.0)
         return h, None if norm is None else norm(h)
+    def call(m, t):
+        return add_norm(m, t)[1] if type(m) is nn.LayerNorm else m(t)
+
     if not plain(post):
-        y, post = post(y), None
+        y, post = call(post, y), None
     called = None
     if not plain(norm) or (post is not None and norm is not None and norm.eps != post.eps):
         norm, called = None, norm
     some = norm if norm is not None else post
     h, n = block_ops.block_join(x, y, post_weight=None if post is None else post.weight,
                                 pre_weight=None if norm is None else norm.weight, eps=0.0 if some is None else some.eps, **how)
-    return h, n if called is None else called(h)
+    return h, n if called is None else call(called, h)
 
 
 class Block(nn.Module):
@@ -268,12 +311,12 @@ class Block(nn.Module):
         # what joins the residual stream: norms and gates of the attention's and the MLP's output
         self.joined = cfg.post_norm or cfg.gate is not None or cfg.residual_scale != 1.0 or cfg.dropout > 0.0
         self.residual_scale, self.dropout = float(cfg.residual_scale), float(cfg.dropout)
-        self.attn_norm = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps)
-        self.attn = Attention(cfg)
-        self.mlp_norm = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps)
+        self.attn_norm = make_norm(cfg)
+        self.attn = (DiffAttention if cfg.attention == "differential" else Attention)(cfg)
+        self.mlp_norm = make_norm(cfg)
         self.mlp = SwiGLU(cfg)
-        self.attn_post = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps) if cfg.post_norm else None
-        self.mlp_post = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps) if cfg.post_norm else None
+        self.attn_post = make_norm(cfg) if cfg.post_norm else None
+        self.mlp_post = make_norm(cfg) if cfg.post_norm else None
         gate = None if cfg.gate is None else torch.full((cfg.hidden_size,), float(cfg.gate))
         self.attn_gate = None if gate is None else nn.Parameter(gate)
         self.mlp_gate = None if gate is None else nn.Parameter(gate.clone())
@@ -300,7 +343,7 @@ class LoopbackLM(nn.Module):
         self.prelude = nn.ModuleList(Block(cfg) for _ in range(cfg.prelude))
         self.middle = nn.ModuleList(Block(cfg) for _ in range(cfg.loop_blocks))   # shared over the R iterations
         self.coda = nn.ModuleList(Block(cfg) for _ in range(cfg.coda))
-        self.norm = nn.RMSNorm(cfg.hidden_size, eps=cfg.norm_eps)
+        self.norm = make_norm(cfg)
         self.head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False)
         self.read = (LoopDeltaAttnRes(cfg.hidden_size, cfg.loops, cfg.loop_blocks, beta=cfg.beta, eps=cfg.norm_eps)
                      if cfg.residual == "delta_attnres" else None)
@@ -314,8 +357,12 @@ class LoopbackLM(nn.Module):
         for m in self.modules():
             if isinstance(m, (nn.Linear, nn.Embedding)):
                 nn.init.normal_(m.weight, mean=0.0, std=std)
-            elif isinstance(m, nn.RMSNorm):
+            elif isinstance(m, (nn.RMSNorm, nn.LayerNorm)):
                 nn.init.ones_(m.weight)
+                if isinstance(m, nn.LayerNorm):
+                    nn.init.zeros_(m.bias)
+            elif isinstance(m, DiffAttention):
+                nn.init.constant_(m.lam, self.cfg.attention_lambda)
             elif isinstance(m, Block) and self.cfg.gate is not None:
                 nn.init.constant_(m.attn_gate, self.cfg.gate)
                 nn.init.constant_(m.mlp_gate, self.cfg.gate)
@@ -388,14 +435,39 @@ class LoopbackLM(nn.Module):
     def forward(self, ids: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
         return ops.next_token_loss(self.head(self.hidden(ids, rng)), ids)
 
+    def distill(self, ids: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.Tensor, rng: torch.Tensor | None = None, *,
+                temperature: float = 1.0, teacher_lse: torch.Tensor | None = None, hard_weight: float = 0.0) -> torch.Tensor:
+        """The distillation loss (model_ops.distill_loss) towards a teacher's highest logits (B, T, k) of the classes top_ids at each
+        position of ids (teacher_top), mixed with the next tokens' cross entropy by hard_weight."""
+        logits = self.head(self.hidden(ids, rng))
+        labels = None
+        if hard_weight:
+            labels = torch.cat((ids[:, 1:], torch.full_like(ids[:, :1], -100)), 1).long()
+        return model_ops.distill_loss(logits, top_logits, top_ids, temperature=temperature, teacher_lse=teacher_lse, labels=labels,
+                                      hard_weight=hard_weight)
+
     def num_params(self) -> int:
         seen = {id(p): p.numel() for p in self.parameters()}
         return sum(seen.values())
 
 
-def train_step(model: LoopbackLM, opt: torch.optim.Optimizer, ids: torch.Tensor) -> torch.Tensor:
-    """One training step: loss, backward, optimizer step, gradients released. Returns the loss (not synchronized)."""
-    loss = model(ids)
+@torch.no_grad()
+def teacher_top(model: LoopbackLM, ids: torch.Tensor, k: int, temperature: float = 1.0):
+    """What a teacher says of ids (B, T): its k highest logits, their classes (B, T, k), and the log of its sum of
+    exp(logit / temperature) over the vocabulary (B, T) in fp32, for LoopbackLM.distill. In evaluation, without dropout."""
+    was = model.training
+    model.eval()
+    logits = model.head(model.hidden(ids))
+    model.train(was)
+    top = torch.topk(logits, k, dim=-1)
+    lse = torch.stack([torch.logsumexp(row.float() / temperature, -1) for row in logits])   # a sequence at a time: fp32 rows are large
+    return top.values, top.indices, lse
+
+
+def train_step(model: LoopbackLM, opt: torch.optim.Optimizer, ids: torch.Tensor, teacher: tuple | None = None, **how) -> torch.Tensor:
+    """One training step: loss, backward, optimizer step, gradients released. Returns the loss (not synchronized). teacher: the
+    teacher's highest logits and their classes, and how's options, for LoopbackLM.distill."""
+    loss = model(ids) if teacher is None else model.distill(ids, *teacher, **how)
     loss.backward()
     opt.step()
     opt.zero_grad(set_to_none=True)
@@ -423,8 +495,15 @@ def bench(argv=None):
     ap.add_argument("--gate", type=float, default=None, help="a learned gate per channel on their outputs, from this value")
     ap.add_argument("--residual-scale", type=float, default=1.0)
     ap.add_argument("--dropout", type=float, default=0.0, help="of the embedding and of what joins the residual stream")
+    ap.add_argument("--norm", default="rms", choices=["rms", "layer"])
+    ap.add_argument("--attention", default="softmax", choices=["softmax", "differential"])
+    ap.add_argument("--teacher-top", type=int, default=0, metavar="K",
+                    help="train towards the K highest logits of another random model, found before the steps")
+    ap.add_argument("--temperature", type=float, default=1.0, help="of the distillation")
+    ap.add_argument("--hard-weight", type=float, default=0.0, help="the labels' weight in the distillation")
     a = ap.parse_args(argv)
-    options = {"ffn": a.ffn, "post_norm": a.post_norm, "gate": a.gate, "residual_scale": a.residual_scale, "dropout": a.dropout}
+    options = {"ffn": a.ffn, "post_norm": a.post_norm, "gate": a.gate, "residual_scale": a.residual_scale, "dropout": a.dropout,
+               "norm": a.norm, "attention": a.attention}
     if not torch.cuda.is_available():
         print("lm: no GPU visible", file=sys.stderr)
         sys.exit(3)
@@ -436,14 +515,17 @@ def bench(argv=None):
         gen = torch.Generator(device=dev).manual_seed(1)
         ids = torch.randint(0, cfg.vocab_size, (a.batch, a.seq), device=dev, generator=gen)
         return _prefill(model, cfg, ids, a)
-    print(json.dumps(time_training(a.steps, a.warmup, a.batch, a.seq, a.residual, **options)), flush=True)
+    print(json.dumps(time_training(a.steps, a.warmup, a.batch, a.seq, a.residual, a.teacher_top, a.temperature, a.hard_weight,
+                                   **options)), flush=True)
 
 
 def time_training(steps: int = 10, warmup: int = 3, batch: int = 8, seq: int = 2048,
-                  residual: str = "delta_attnres", **options) -> dict:
+                  residual: str = "delta_attnres", teacher_k: int = 0, temperature: float = 1.0, hard_weight: float = 0.0,
+                  **options) -> dict:
     """Config 5's training step on cuda:0 -- the random-init LM in bf16, uniform random ids (batch, seq), AdamW --
-    timed over `steps` steps after `warmup`; residual "none" is the same model as Plain Loop; options: LMConfig's. Returns
-    the record."""
+    timed over `steps` steps after `warmup`; residual "none" is the same model as Plain Loop; teacher_k: the steps
+    distill that many of another random model's highest logits, which it gives before them; options: LMConfig's. Returns the
+    record."""
     dev = torch.device("cuda", 0)
     cfg = LMConfig(residual=None if residual == "none" else "delta_attnres", **options)
     torch.manual_seed(0)
@@ -451,14 +533,19 @@ def time_training(steps: int = 10, warmup: int = 3, batch: int = 8, seq: int = 2
     gen = torch.Generator(device=dev).manual_seed(1)
     ids = torch.randint(0, cfg.vocab_size, (batch, seq), device=dev, generator=gen)
     opt = make_optimizer(model)
+    teacher, how = None, {}
+    if teacher_k:
+        other = LoopbackLM(cfg).to(device=dev, dtype=torch.bfloat16)
+        teacher, how = teacher_top(other, ids, teacher_k, temperature)[:2], {"temperature": temperature, "hard_weight": hard_weight}
+        del other
     for _ in range(warmup):
-        train_step(model, opt, ids)
+        train_step(model, opt, ids, teacher, **how)
     torch.cuda.synchronize()
     gc.collect()
     gc.freeze()
     t0 = time.perf_counter()
     for _ in range(steps):
-        loss = train_step(model, opt, ids)
+        loss = train_step(model, opt, ids, teacher, **how)
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0
     gc.unfreeze()
@@ -468,6 +555,8 @@ def time_training(steps: int = 10, warmup: int = 3, batch: int = 8, seq: int = 2
            "params": model.num_params(), "dtype": "bf16", "data": "uniform random token ids",
            "optimizer": "AdamW (foreach)",
            "config": {"topology": cfg.topology(), **asdict(cfg), "batch": batch, "seq": seq}}
+    if teacher_k:
+        rec["distill"] = {"teacher_top": teacher_k, **how}
     del model, opt, ids
     torch.cuda.empty_cache()
     return rec

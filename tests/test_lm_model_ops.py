@@ -1,0 +1,261 @@
+"""The language model with layer norms, differential attention and a distillation step (model_ops together, as a training step
+calls them): on the CPU in torch operations, on the GPU on the kernels."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from loopback_amd import block_ops, lm, model_ops
+
+SMALL = dict(hidden_size=128, num_heads=2, vocab_size=97, prelude=1, loop_blocks=2, loops=2, coda=1, hidden_ratio=2)
+ALL = dict(norm="layer", attention="differential")
+MORE = dict(ALL, post_norm=True, gate=0.5, residual_scale=0.7)
+HOW = dict(temperature=2.0, hard_weight=0.25)
+
+
+def make(device="cpu", dtype=torch.float32, seed=0, residual=None, **options):
+    torch.manual_seed(seed)
+    return lm.LoopbackLM(lm.LMConfig(**(SMALL | options), residual=residual)).to(device, dtype)
+
+
+def ids_of(b, t, device="cpu"):
+    return torch.randint(0, 97, (b, t), generator=torch.Generator().manual_seed(5)).to(device)
+
+
+def teacher_of(ids, dtype, k=5):
+    g = torch.Generator().manual_seed(9)
+    top = torch.randn(*ids.shape, k, generator=g).sort(-1, descending=True).values
+    classes = torch.rand(*ids.shape, 97, generator=g).argsort(-1)[..., :k]
+    classes[0, 0] = -1   # a position that says nothing
+    return top.to(ids.device, dtype), classes.to(ids.device)
+
+
+def layer_norm(x, m):
+    c = x - x.mean(-1, keepdim=True)
+    return c * torch.rsqrt((c * c).mean(-1, keepdim=True) + m.eps) * m.weight + m.bias
+
+
+def diff_attention(att, x):
+    """The pair's two maps written out."""
+    B, T, D = x.shape
+    q, k, v = (x @ att.qkv.weight.T).view(B, T, 3, att.h, att.dh).unbind(2)
+    q, k = att.rotary(q), att.rotary(k)
+    out = []
+    for j in range(att.h // 2):
+        maps = []
+        for e in (2 * j, 2 * j + 1):
+            s = q[:, :, e] @ k[:, :, e].transpose(1, 2) * att.dh ** -0.5
+            maps.append(s.masked_fill(torch.ones(T, T).triu(1).bool(), -torch.inf).softmax(-1))
+        y = (maps[0] - att.lam[j] * maps[1]) @ v[:, :, 2 * j:2 * j + 2].reshape(B, T, 2 * att.dh)
+        out.append(y * torch.rsqrt((y * y).mean(-1, keepdim=True) + att.head_norm.eps) * att.head_norm.weight)
+    return torch.cat(out, -1) @ att.o.weight.T
+
+
+def test_configuration():
+    """The options add their own parameters alone, initialised also on the meta device; what cannot be is refused."""
+    plain, more = make(), make(**ALL)
+    assert not any(isinstance(m, (torch.nn.LayerNorm, lm.DiffAttention)) for m in plain.modules())
+    blocks = ("prelude.0", "middle.0", "middle.1", "coda.0")
+    assert set(more.state_dict()) - set(plain.state_dict()) == {"norm.bias"} | {
+        f"{b}.{p}" for b in blocks for p in ("attn_norm.bias", "mlp_norm.bias", "attn.lam", "attn.head_norm.weight")}
+    with torch.device("meta"):
+        empty = lm.LoopbackLM(lm.LMConfig(**SMALL, **ALL, attention_lambda=0.3))
+    empty = empty.to_empty(device="cpu")
+    empty.reset_parameters()
+    assert (empty.coda[0].attn.lam == 0.3).all() and (empty.norm.bias == 0).all() and (empty.norm.weight == 1).all()
+    for bad in ({"norm": "batch"}, {"attention": "linear"}, {"attention": "differential", "num_heads": 1}):
+        with pytest.raises(ValueError):
+            lm.LMConfig(**(SMALL | bad))
+
+
+@pytest.mark.parametrize("options", [ALL, MORE])
+def test_block_formula(options):
+    """A block is its formula in fp64, and hooked norms are called."""
+    torch.manual_seed(1)
+    blk = lm.Block(lm.LMConfig(**(SMALL | {"num_heads": 4} | options))).double()
+    with torch.no_grad():
+        for p in blk.parameters():
+            p += 0.1 * torch.randn(p.shape)
+    x = torch.randn(2, 6, 128, dtype=torch.float64)
+    a = diff_attention(blk.attn, layer_norm(x, blk.attn_norm))
+    h = x + (a if "gate" not in options else 0.7 * blk.attn_gate * layer_norm(a, blk.attn_post))
+    m = blk.mlp(layer_norm(h, blk.mlp_norm))
+    ref = h + (m if "gate" not in options else 0.7 * blk.mlp_gate * layer_norm(m, blk.mlp_post))
+    # the rotation rounds q and k to fp32; everything else is fp64
+    assert torch.allclose(blk(x), ref, atol=1e-5, rtol=1e-5)
+    seen = []
+    for n in (blk.attn_norm, blk.mlp_norm, blk.attn.head_norm):
+        n.register_forward_hook(lambda m, i, o: seen.append(m))
+    assert torch.allclose(blk(x), ref, atol=1e-5, rtol=1e-5) and len(seen) == 3
+
+
+def test_block_trace():
+    """torch.fx sees a block's norms, attention and linear layers."""
+    class Leaf(torch.fx.Tracer):
+        def is_leaf_module(self, m, name):
+            return isinstance(m, lm.Attention) or super().is_leaf_module(m, name)
+
+    torch.manual_seed(0)
+    x = torch.randn(2, 8, 128)
+    for options in (ALL, MORE):
+        block = lm.Block(lm.LMConfig(**SMALL, **options)).eval()
+        tracer = Leaf()
+        graph = tracer.trace(block)
+        post = [["attn_post"], ["mlp_post"]] if "post_norm" in options else [[], []]
+        assert [n.target for n in graph.nodes if n.op == "call_module"] == \
+            ["attn_norm", "attn", *post[0], "mlp_norm", "mlp.gate_up", "mlp.down", *post[1]]
+        assert torch.allclose(torch.fx.GraphModule(tracer.root, graph)(x), block(x), atol=1e-5)
+
+
+def test_distill_formula():
+    """The loss of a step from a stored teacher, and with the teacher's remaining probability, written out."""
+    model, ids = make(dtype=torch.float64, **ALL), ids_of(2, 7)
+    top, classes = teacher_of(ids, torch.float64)
+    got = model.distill(ids, top, classes, **HOW).double()
+    logits = model.head(model.hidden(ids))
+    p = (top / 2).softmax(-1)
+    kl = (p * (p.log() - (logits / 2).log_softmax(-1).gather(-1, classes.clamp_min(0)))).sum(-1).flatten()[1:].mean()
+    ce = F.cross_entropy(logits[:, :-1].reshape(-1, 97), ids[:, 1:].reshape(-1))
+    assert abs(got - (0.75 * 4 * kl + 0.25 * ce)) <= 1e-5 * abs(got)
+    other = make(dtype=torch.float64, seed=3, **ALL).train()
+    top, classes, lse = lm.teacher_top(other, ids, 5, temperature=2.0)
+    x = other.head(other.hidden(ids)).detach()
+    assert other.training and torch.equal(top, x.topk(5, -1).values) and torch.equal(x.gather(-1, classes), top)
+    assert torch.allclose(lse.double(), (x / 2).logsumexp(-1), atol=1e-5)
+    got = model.distill(ids, top, classes, temperature=2.0, teacher_lse=lse)
+    full, q = (x / 2).softmax(-1), (logits / 2).softmax(-1)
+    named = torch.zeros_like(full, dtype=torch.bool).scatter(-1, classes, True)
+    event = lambda t: torch.cat((t.gather(-1, classes), t.masked_fill(named, 0).sum(-1, keepdim=True)), -1)
+    ref = 4 * (event(full) * (event(full).log() - event(q).log())).sum(-1).mean()
+    assert abs(got - ref) <= 1e-4 * abs(ref) + 1e-6   # fp32 lse: 1e-7 of 4, over divergences of 1e-3
+
+
+def test_gradients_against_differences():
+    """The gradient of a distillation step along a random direction is the loss's central difference, in fp64."""
+    model, ids = make(dtype=torch.float64, **MORE), ids_of(2, 7)
+    teacher = teacher_of(ids, torch.float64)
+    params = list(model.parameters())
+    with torch.no_grad():
+        for p in params:   # weights of 0.02 would leave norms that bend within a step
+            p += 0.1 * torch.randn(p.shape, generator=torch.Generator().manual_seed(11), dtype=torch.float64)
+    grads = torch.autograd.grad(model.distill(ids, *teacher, **HOW), params)
+    g = torch.Generator().manual_seed(3)
+    way = [torch.randn(p.shape, generator=g, dtype=torch.float64) for p in params]
+    exact = sum((a * b).sum() for a, b in zip(grads, way))
+    eps, got = 1e-4, []
+    with torch.no_grad():
+        for sign in (1, -1):
+            for p, w in zip(params, way):
+                p += sign * eps * w
+            got.append(model.distill(ids, *teacher, **HOW).double())
+            for p, w in zip(params, way):
+                p -= sign * eps * w
+    # The rotation rounds q and k to fp32, 6e-8 of them: 6e-8 / 1e-4 is 6e-4 of the difference. The next term is eps^2 times a
+    # constant: steps of 1e-3, 3e-4 and 1e-4 are off by 1.87, 0.182 and 0.0214, which is 1.9e6 eps^2, and the gradient is 6.645 at
+    # the limit; at 1e-4 that is 3.2e-3 of it.
+    assert abs((got[0] - got[1]) / (2 * eps) - exact) <= 1e-2 * max(1.0, abs(exact))
+
+
+def test_training_steps():
+    """train_step with a teacher runs and moves every parameter."""
+    model, ids = make(**MORE), ids_of(2, 9)
+    before = [p.detach().clone() for p in model.parameters()]
+    loss = lm.train_step(model, lm.make_optimizer(model), ids, teacher_of(ids, torch.float32), **HOW)
+    assert loss.dim() == 0 and torch.isfinite(loss) and all(not torch.equal(a, b) for a, b in zip(before, model.parameters()))
+
+
+def counted(monkeypatch):
+    """The names of model_ops' calls of the native nodes."""
+    nodes, H = [], model_ops.H
+    names = ("layer_norm", "diff_attn", "distill")
+    call = lambda n: lambda *a: nodes.append(n) or getattr(H, n)(*a)
+    monkeypatch.setattr(model_ops, "H", type("Counted", (), {n: staticmethod(call(n)) for n in names}))
+    return nodes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("options", [ALL, MORE])
+def test_training_step_on_the_kernels(dtype, options, monkeypatch):
+    """Loss and gradients of a distillation step on the kernels are no further from the same model in fp64 than on torch's
+    operations, to a fifth; a second pass gives the same bits."""
+    print(f"case lm model ops {options} {dtype}", flush=True)
+    model, ids = make("cuda", dtype, **options), ids_of(3, 65, "cuda")
+    teacher = teacher_of(ids, dtype)
+    state = {k: v.clone() for k, v in model.state_dict().items()}
+
+    def step(m, i, t):
+        m.load_state_dict({k: v.to(m.embed.weight.device, m.embed.weight.dtype) for k, v in state.items()})
+        loss = m.distill(i, *t, **HOW)
+        return loss.detach().double().cpu(), [g.double().cpu() for g in torch.autograd.grad(64.0 * loss, list(m.parameters()))]
+
+    nodes = counted(monkeypatch)
+    got = step(model, ids, teacher)
+    norms = 13 if options is ALL else 25   # 6 block applications of 2, or 4, and the last
+    assert nodes.count("layer_norm") == norms and nodes.count("diff_attn") == 6 and nodes.count("distill") == 1
+    again = step(model, ids, teacher)
+    assert got[0] == again[0] and all(torch.equal(a, b) for a, b in zip(got[1], again[1]))
+    monkeypatch.undo()
+    for where in (model_ops, block_ops, lm.ops):
+        monkeypatch.setattr(where, "native", lambda *a, **k: False)
+    ref = step(model, ids, teacher)
+    exact = step(make("cpu", torch.float64, **options), ids.cpu(), (teacher[0].cpu().double(), teacher[1].cpu()))
+    # Lambda's gradient is a sum that cancels: weights of 0.02 make both maps nearly alike, so y is about (1 - lambda) (second map) v,
+    # and the norm behind it takes a factor of y out again. Its terms are those of sum(gain dgain) / (1 - lambda), without the
+    # cancellation, and what they round to is in proportion to their size, |dgain| summed / 0.5, not to what is left of them.
+    names = [n for n, _ in model.named_parameters()]
+    gains = {n: g.abs().sum() / 0.5 for n, g in zip(names, exact[1]) if n.endswith("head_norm.weight")}
+    size = [q.norm() + gains.get(n.replace("attn.lam", "attn.head_norm.weight"), 0.0) * n.endswith("attn.lam") for n, q in zip(names, exact[1])]
+    far = lambda a: torch.stack([(p - q).norm() / (s + 1e-9) for p, q, s in zip(a[1], exact[1], size)])
+    # gradients pass through the model's other 16-bit operations alike: the largest distance of any parameter's
+    assert far(got).max() <= 1.2 * far(ref).max() + 1e-3, (far(got), far(ref))
+    assert abs(got[0] - exact[0]) <= 1.2 * abs(ref[0] - exact[0]) + 2e-3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("residual", ["delta_attnres", None])
+def test_captured_training_pass(residual):
+    """A distillation step as one captured graph: each replay gives what the eager pass gives from the same inputs, new ones copied
+    in and eager work between the replays."""
+    model = make("cuda", torch.bfloat16, residual=residual, **MORE)
+    ids, params = ids_of(2, 64, "cuda"), list(model.parameters())
+    top, classes = teacher_of(ids, torch.bfloat16)
+
+    def step():
+        loss = model.distill(ids, top, classes, **HOW)
+        return [loss.detach(), *torch.autograd.grad(loss, params)]
+
+    inputs = []
+    for k in range(3):
+        inputs.append((ids.roll(k, 1).clone(), top.roll(k, 0).clone()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    eager = []
+    for i, t in inputs:
+        ids.copy_(i), top.copy_(t)
+        eager.append([x.clone() for x in step()])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k, (i, t) in enumerate(inputs):
+        ids.copy_(i), top.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, eager[k]):
+            assert torch.equal(a, b), k
+        assert torch.isfinite(torch.randn(1000, device="cuda").sum())
+
+
+@pytest.mark.gpu
+def test_checkpointed_step():
+    """Activation checkpointing repeats the forward with the same result and gradients."""
+    from torch.utils.checkpoint import checkpoint
+    model, ids = make("cuda", torch.bfloat16, **ALL), ids_of(2, 33, "cuda")
+    teacher, params = teacher_of(ids, torch.bfloat16), list(model.parameters())
+    loss = model.distill(ids, *teacher, **HOW)
+    grads = torch.autograd.grad(loss, params)
+    again = checkpoint(lambda: model.distill(ids, *teacher, **HOW), use_reentrant=False)
+    assert again == loss and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, params), grads))
