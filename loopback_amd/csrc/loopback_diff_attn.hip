@@ -262,8 +262,7 @@ __device__ __forceinline__ int seen_by(const Diff& a, int i, int start, int len)
 // Which block of which head a workgroup takes: `items` (batches times heads of keys) go to the eight XCDs in turn where they
 // divide by eight, so that a head's keys are read from one L2; the blocks with the most work first.
 struct Work { int item, g, block; };
-__device__ __forceinline__ bool work_of(int items, int groups, int blocks, Work& w) {
-  const int id = (int)blockIdx.x;
+__device__ __forceinline__ bool work_of(int id, int items, int groups, int blocks, Work& w) {
   int unit;
   if (items % 8 == 0) {
     const int i = id >> 3, per = items >> 3;
@@ -344,15 +343,17 @@ template <int DH, int DV> constexpr int fwd_lds() {   // two tiles; at the end a
   const int tiles = 2 * FT * (2 * DH + DV) * 2, results = FQ * DV * 4;
   return tiles > results ? tiles : results;
 }
-template <typename T, int DH, int DV>
+template <int DV> constexpr int partial_row() { return 2 * DV + 4; }   // floats of a row's partial result: o1, o2, m1, l1, m2, l2
+template <typename T, int DH, int DV, bool SPLIT>
 __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<DH, DV>())))) void k_diff_fwd(const Diff a) {
   extern __shared__ __align__(16) char lds_block[];   // two tiles of keys, two of values
   constexpr int KT = FT * 2 * DH, VT = FT * DV, DB = DV / 32, K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT;
   const int lane = (int)threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), map = wave & 1;
   const int groups = a.h / a.hk, blocks = (a.tq + FQ - 1) / FQ;
+  const int all = a.b * a.h * blocks, split = SPLIT ? (int)blockIdx.x / all : 0;
   Work wk;
-  if (!work_of(a.b * a.hk, groups, blocks, wk)) return;
+  if (!work_of((int)blockIdx.x - split * all, a.b * a.hk, groups, blocks, wk)) return;
   const int q0 = (blocks - 1 - wk.block) * FQ, b = wk.item / a.hk, hk = wk.item - b * a.hk, head = hk * groups + wk.g;
   const int len = length_of(a, b), start = start_of(a, b);
   const int w0 = q0 + 32 * (wave >> 1), query = w0 + (lane & 31), qrow = min(query, a.tq - 1);
@@ -367,12 +368,13 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = zero16();
   Soft sm;
-  const int ntiles = (most + FT - 1) / FT;
+  const int first = SPLIT ? split * a.chunk / FT : 0, last = (most + FT - 1) / FT;   // a chunk has whole tiles
+  const int ntiles = SPLIT ? min(last, first + a.chunk / FT) : last;
   const Fill<T, 2 * DH, 2, FT, FL> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
   const Fill<T, DV, 1, FT, FL> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
-  if (ntiles > 0) {
-    kf.fetch(0, len - 1, K0);
-    vf.fetch(0, len - 1, V0);
+  if (ntiles > first) {
+    kf.fetch(first * FT, len - 1, K0);
+    vf.fetch(first * FT, len - 1, V0);
   }
   filled();   // in every case: a wait for what was loaded above, left to the loop, would wait there for the tiles too
   auto tile = [&](int j, auto buffer) {
@@ -418,9 +420,23 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
     }
     if (j + 1 < ntiles) filled();
   };
-  for (int j = 0; j < ntiles; j += 2) {
+  for (int j = first; j < ntiles; j += 2) {
     tile(j, std::integral_constant<int, 0>());
     if (j + 1 < ntiles) tile(j + 1, std::integral_constant<int, 1>());
+  }
+  if constexpr (SPLIT) {
+    const float l = sm.sum();
+    if (query >= a.tq) return;
+    float* p = a.part + (((int64_t)wk.item * a.tq * groups + query * groups + wk.g) * a.splits + split) * partial_row<DV>();
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = 32 * d + 8 * g + 4 * half;
+        if (col < a.dv) *reinterpret_cast<f32x4*>(p + map * DV + col) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+      }
+    if (half == 0) *reinterpret_cast<float2*>(p + 2 * DV + 2 * map) = make_float2(sm.m, l);
+    return;
   }
   // a query that sees no key: zeros, and an infinite logarithm, which makes every probability 0
   const float l = sm.sum(), inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -463,7 +479,6 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
 // the result's. The waves' results meet in LDS, and those of the chunks in k_diff_join.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int FEW = 32, NT = 64;   // rows, keys of a tile
-template <int DV> constexpr int few_row() { return 2 * DV + 4; }   // floats of a row's partial result: o1, o2, m1, l1, m2, l2
 template <int DH, int DV> constexpr int few_lds() {   // two tiles; at the end the four waves' results
   const int tiles = 2 * NT * (2 * DH + DV) * 2, results = 4 * FEW * (DV + 2) * 4;
   return tiles > results ? tiles : results;
@@ -472,7 +487,7 @@ template <int DH, int DV> constexpr int few_lds() {   // two tiles; at the end t
 template <typename T, int DH, int DV>
 __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu(2))) void k_diff_few(const Diff a) {
   extern __shared__ __align__(16) char lds_block[];
-  constexpr int KT = NT * 2 * DH, VT = NT * DV, DB = DV / 32, K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT, ROW = few_row<DV>();
+  constexpr int KT = NT * 2 * DH, VT = NT * DV, DB = DV / 32, K0 = 0, K1 = 2 * KT, V0 = 4 * KT, V1 = 4 * KT + 2 * VT, ROW = partial_row<DV>();
   typedef typename Mat<T>::Cvt C;
   const int lane = (int)threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), map = wave & 1, part = wave >> 1;
@@ -584,46 +599,87 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu(2))) void k_
   }
 }
 
-// the chunks' partial rows as one: their common maxima, then their sums and values relative to them. A workgroup per row, a lane
-// per column of one map
-constexpr int MOST_CHUNKS = 256;
-template <typename T, int DV> __global__ __launch_bounds__(2 * DV) void k_diff_join(const Diff a) {
-  constexpr int ROW = few_row<DV>(), LANES = 2 * DV;
-  __shared__ float s_f[2][MOST_CHUNKS], s_y[DV];
-  const int groups = a.h / a.hk, rows = a.tq * groups, item = (int)blockIdx.x / rows, r = (int)blockIdx.x - item * rows;
+// The chunks' partial rows [batch and head of keys][query][head of its group] as one, relative to the running maxima: DV / 4 lanes to
+// a row, four columns of both maps each, four chunks' loads in flight. SHARED, few rows: the workgroup's groups of lanes take the
+// chunks of one row in turn, and meet in LDS.
+constexpr int MOST_CHUNKS = 256, SHARED_ROWS = 4096;
+struct Joined {
+  float m[2] = {NONE, NONE}, l[2] = {0.f, 0.f};
+  f32x4 o[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  // N chunks' maxima and sums (m1, l1, m2, l2) and values
+  template <int N> __device__ __forceinline__ void add(const float4 (&e)[N], const f32x4 (&x)[2][N]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float most = m[k];
+#pragma unroll
+      for (int u = 0; u < N; ++u) most = fmaxf(most, k ? e[u].z : e[u].x);
+      const float f = __builtin_amdgcn_exp2f(m[k] - most);
+      m[k] = most;
+      l[k] *= f;
+      o[k] *= f;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const float w = __builtin_amdgcn_exp2f((k ? e[u].z : e[u].x) - most);
+        l[k] = __builtin_fmaf(k ? e[u].w : e[u].y, w, l[k]);
+        o[k] += x[k][u] * w;
+      }
+    }
+  }
+};
+template <typename T, int DV, bool SHARED> __global__ __launch_bounds__(WG) void k_diff_join(const Diff a) {
+  constexpr int ROW = partial_row<DV>(), L = DV / 4, G = WG / L, U = 4;
+  __shared__ __align__(16) float s_part[SHARED ? G * ROW : 4];
+  const int tid = (int)threadIdx.x, lane = tid % L, grp = tid / L, groups = a.h / a.hk, rows = a.tq * groups, n = a.splits;
+  const int64_t at = SHARED ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * G + grp;
+  if (at >= (int64_t)a.b * a.hk * rows) return;   // SHARED: the grid is the rows
+  const int item = (int)(at / rows), r = (int)(at - (int64_t)item * rows);
   const int b = item / a.hk, hk = item - b * a.hk, query = r / groups, head = hk * groups + r - query * groups;
-  const int tid = (int)threadIdx.x, map = tid / DV, col = tid - map * DV, n = a.splits;
-  const float* p = a.part + (int64_t)blockIdx.x * n * ROW;
-  for (int i = tid; i < 2 * n; i += LANES) s_f[i & 1][i >> 1] = p[(int64_t)(i >> 1) * ROW + 2 * DV + 2 * (i & 1)];
-  __syncthreads();
-  float m = NONE;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, s_f[map][i]);
-  float sum = 0.f, y = 0.f;
-  int i = 0;
-  for (; i + 4 <= n; i += 4) {   // four chunks' loads in flight
-    float x[4], l[4];
+  const float* p = a.part + at * n * ROW;
+  const float lam = lam_at<T>(a, b, query, head);
+  Joined s;
+  auto take = [&](auto many, int i, int step) {
+    constexpr int N = decltype(many)::value;
+    float4 e[N];
+    f32x4 x[2][N];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      x[u] = p[(int64_t)(i + u) * ROW + map * DV + col];
-      l[u] = p[(int64_t)(i + u) * ROW + 2 * DV + 2 * map + 1];
+    for (int u = 0; u < N; ++u) {
+      const float* c = p + (int64_t)(i + u * step) * ROW;
+      e[u] = *reinterpret_cast<const float4*>(c + 2 * DV);
+      x[0][u] = *reinterpret_cast<const f32x4*>(c + 4 * lane);
+      x[1][u] = *reinterpret_cast<const f32x4*>(c + DV + 4 * lane);
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float f = __builtin_amdgcn_exp2f(s_f[map][i + u] - m);
-      y = __builtin_fmaf(x[u], f, y);
-      sum = __builtin_fmaf(l[u], f, sum);
+    s.template add<N>(e, x);
+  };
+  constexpr int step = SHARED ? G : 1;
+  int i = SHARED ? grp : 0;
+  for (; i + (U - 1) * step < n; i += U * step) take(std::integral_constant<int, U>(), i, step);
+  for (; i < n; i += step) take(std::integral_constant<int, 1>(), i, step);
+  if constexpr (SHARED) {
+    float* mine = s_part + grp * ROW;
+    *reinterpret_cast<f32x4*>(mine + 4 * lane) = s.o[0];
+    *reinterpret_cast<f32x4*>(mine + DV + 4 * lane) = s.o[1];
+    if (lane == 0) *reinterpret_cast<float4*>(mine + 2 * DV) = make_float4(s.m[0], s.l[0], s.m[1], s.l[1]);
+    __syncthreads();
+    if (grp) return;
+    for (int g = 1; g < G; ++g) {
+      const float* c = s_part + g * ROW;
+      const float4 e[1] = {*reinterpret_cast<const float4*>(c + 2 * DV)};
+      const f32x4 x[2][1] = {{*reinterpret_cast<const f32x4*>(c + 4 * lane)}, {*reinterpret_cast<const f32x4*>(c + DV + 4 * lane)}};
+      s.add<1>(e, x);
     }
   }
-  for (; i < n; ++i) {
-    const float f = __builtin_amdgcn_exp2f(s_f[map][i] - m);
-    y = __builtin_fmaf(p[(int64_t)i * ROW + map * DV + col], f, y);
-    sum = __builtin_fmaf(p[(int64_t)i * ROW + 2 * DV + 2 * map + 1], f, sum);
+  bool sees[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    sees[k] = s.l[k] > 0.f || s.l[k] != s.l[k];
+    s.o[k] *= sees[k] ? 1.f / s.l[k] : 0.f;
+    if (a.lse && lane == 0)
+      a.lse[(((int64_t)k * a.b + b) * a.h + head) * a.tq + query] = sees[k] ? s.m[k] + __builtin_amdgcn_logf(s.l[k]) : INFINITY;
   }
-  y = sum > 0.f || sum != sum ? y / sum : 0.f;
-  if (map) s_y[col] = y;
-  __syncthreads();
-  if (!map && col < a.dv)
-    st1(static_cast<T*>(a.out) + (((int64_t)b * a.tq + query) * a.h + head) * a.dv + col, y - lam_at<T>(a, b, query, head) * s_y[col]);
+  if (4 * lane >= a.dv) return;
+  const int64_t o = (((int64_t)b * a.tq + query) * a.h + head) * a.dv + 4 * lane;
+  if (a.second) *reinterpret_cast<uint2*>(static_cast<T*>(a.second) + o) = packed4<T>(s.o[1]);
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + o) = packed4<T>(s.o[0] - lam * s.o[1]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -638,7 +694,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int groups = a.h / a.hk, blocks = (a.tq + QB - 1) / QB;
   Work wk;
-  if (!work_of(a.b * a.hk, groups, blocks, wk)) return;
+  if (!work_of((int)blockIdx.x, a.b * a.hk, groups, blocks, wk)) return;
   const int qblock = blocks - 1 - wk.block, q0 = qblock * QB, b = wk.item / a.hk, hk = wk.item - b * a.hk, head = hk * groups + wk.g;
   const int len = length_of(a, b), start = start_of(a, b);
   const int w0 = q0 + 32 * wave, query = w0 + (lane & 31), qrow = min(query, a.tq - 1);
@@ -838,7 +894,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = a.h / a.hk, blocks = (a.tk + QB - 1) / QB;
   Work wk;
-  if (!work_of(a.b * a.hk, a.splits, blocks, wk)) return;
+  if (!work_of((int)blockIdx.x, a.b * a.hk, a.splits, blocks, wk)) return;
   const int kb = wk.block * QB, b = wk.item / a.hk, hk = wk.item - b * a.hk;
   const KvTiles kv = kv_tiles(a, b, kb);
   if (wk.g >= kv.parts) return;
@@ -1134,14 +1190,18 @@ template <typename K, K KERNEL> int allow_lds(int bytes) {
 }
 #define ALLOW_LDS(BYTES, ...) allow_lds<decltype(&__VA_ARGS__), &__VA_ARGS__>(BYTES)
 
-// chunks of the keys for the kernel of few queries: workgroups for the CUs twice over, chunks of 256 keys at least
+inline bool few(const lmo_diff_shape* s) { return s->tq * (s->h / s->hk) <= FEW; }
+// Chunks of the keys: enough workgroups for the CUs twice over, chunks of 256 keys at least. Blocks of 64 queries (not `few`: the rows
+// of the kernel of few queries) are split where that makes three chunks at least: 3 x 333 new tokens over 1001 keys, 6 heads, 26.5 us
+// whole and 15.7 + 5.0 for the join in three; 3 x 683 tokens, 4 heads of 128|256, 33.2 whole and 23.2 + 9.7 in two.
 struct Chunks { int64_t splits, chunk; };
-inline Chunks chunks_of(const lmo_diff_shape* s) {
-  const int64_t items = s->b * s->hk, want = (512 + items - 1) / (items > 0 ? items : 1), most = (s->tk + 255) / 256;
+inline Chunks chunks_of(const lmo_diff_shape* s, bool few) {
+  const int64_t items = few ? s->b * s->hk : s->b * s->h * ((s->tq + FQ - 1) / FQ), most = s->tk / 256;
+  const int64_t want = few ? (512 + items - 1) / (items > 0 ? items : 1) : items > 0 ? 512 / items : 1;
   int64_t n = want < most ? want : most;
-  n = n < 1 ? 1 : n > MOST_CHUNKS ? MOST_CHUNKS : n;
+  n = n < (few ? 1 : 3) ? 1 : n > MOST_CHUNKS ? MOST_CHUNKS : n;
   const int64_t chunk = ((s->tk + n - 1) / n + NT - 1) / NT * NT;
-  return {(s->tk + chunk - 1) / chunk, chunk};
+  return {s->tk < 1 ? 1 : (s->tk + chunk - 1) / chunk, chunk};
 }
 // parts of the tiles of queries for dk and dv: those of a causal sequence (positions and lengths are the kernel's to know), so that
 // the longest takes little more than its share of what the CUs hold at once
@@ -1160,7 +1220,6 @@ inline Parts kv_parts(const lmo_diff_shape* s) {
   const int64_t splits = (most + limit - 1) / limit;
   return {splits < 1 ? 1 : splits > 16 ? 16 : splits, limit};
 }
-inline bool few(const lmo_diff_shape* s) { return s->tq * (s->h / s->hk) <= FEW; }
 inline int padded_dv(const lmo_diff_shape* s) { return s->dv <= 64 && s->dh <= 64 ? 64 : s->dv <= 128 ? 128 : 256; }
 
 }  // namespace
@@ -1168,8 +1227,8 @@ inline int padded_dv(const lmo_diff_shape* s) { return s->dv <= 64 && s->dh <= 6
 extern "C" {
 
 int64_t lmo_diff_attn_scratch(const lmo_diff_shape* s, int record) {
-  if (!s || record || s->hk < 1 || s->b < 1 || s->tq < 1 || !few(s)) return 0;
-  const Chunks n = chunks_of(s);
+  if (!s || s->hk < 1 || s->b < 1 || s->tq < 1) return 0;
+  const Chunks n = chunks_of(s, !record && few(s));
   return n.splits == 1 ? 0 : s->b * s->h * s->tq * n.splits * (2 * padded_dv(s) + 4);
 }
 
@@ -1186,29 +1245,35 @@ int lmo_diff_attn_fwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
   a.second = second;
   a.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (!lse && few(s)) {
-    const Chunks n = chunks_of(s);
-    if (n.splits > 1 && !scratch) return LDR_E_ARG;
-    a.splits = (int)n.splits;
-    a.chunk = (int)n.chunk;
-    a.part = scratch;
-    const int64_t grid = s->b * s->hk * n.splits;
-    if (grid > 0x7fffffff) return LDR_E_SHAPE;
-    DIFF_SWITCH(dtype, s->dh, s->dv, {
+  const bool fewer = !lse && few(s);
+  const Chunks n = chunks_of(s, fewer);
+  if (n.splits > 1 && !scratch) return LDR_E_ARG;
+  a.splits = (int)n.splits;
+  a.chunk = (int)n.chunk;
+  a.part = scratch;
+  const int64_t grid = (fewer ? s->b * s->hk : s->b * s->h * ((s->tq + FQ - 1) / FQ)) * n.splits;
+  if (grid > 0x7fffffff) return LDR_E_SHAPE;
+  DIFF_SWITCH(dtype, s->dh, s->dv, {
+    if (fewer) {
       constexpr int bytes = few_lds<DH, DV>();
       if ((e = ALLOW_LDS(bytes, k_diff_few<T, DH, DV>))) return e;
       hipLaunchKernelGGL((k_diff_few<T, DH, DV>), dim3((unsigned)grid), dim3(WG), bytes, st, a);
-      if ((e = launched())) return e;
-      if (n.splits > 1) hipLaunchKernelGGL((k_diff_join<T, DV>), dim3((unsigned)(s->b * s->h * s->tq)), dim3(2 * DV), 0, st, a);
-    })
-    return launched();
-  }
-  const int64_t grid = s->b * s->h * ((s->tq + FQ - 1) / FQ);
-  if (grid > 0x7fffffff) return LDR_E_SHAPE;
-  DIFF_SWITCH(dtype, s->dh, s->dv, {
-    constexpr int bytes = fwd_lds<DH, DV>();
-    if ((e = ALLOW_LDS(bytes, k_diff_fwd<T, DH, DV>))) return e;
-    hipLaunchKernelGGL((k_diff_fwd<T, DH, DV>), dim3((unsigned)grid), dim3(FL), bytes, st, a);
+    } else if (n.splits > 1) {
+      constexpr int bytes = fwd_lds<DH, DV>();
+      if ((e = ALLOW_LDS(bytes, k_diff_fwd<T, DH, DV, true>))) return e;
+      hipLaunchKernelGGL((k_diff_fwd<T, DH, DV, true>), dim3((unsigned)grid), dim3(FL), bytes, st, a);
+    } else {
+      constexpr int bytes = fwd_lds<DH, DV>();
+      if ((e = ALLOW_LDS(bytes, k_diff_fwd<T, DH, DV, false>))) return e;
+      hipLaunchKernelGGL((k_diff_fwd<T, DH, DV, false>), dim3((unsigned)grid), dim3(FL), bytes, st, a);
+    }
+    if ((e = launched())) return e;
+    const int64_t rows = s->b * s->h * s->tq;
+    if (n.splits > 1 && rows <= SHARED_ROWS) {
+      hipLaunchKernelGGL((k_diff_join<T, DV, true>), dim3((unsigned)rows), dim3(WG), 0, st, a);
+    } else if (n.splits > 1) {
+      hipLaunchKernelGGL((k_diff_join<T, DV, false>), dim3((unsigned)((rows * (DV / 4) + WG - 1) / WG)), dim3(WG), 0, st, a);
+    }
   })
   return launched();
 }

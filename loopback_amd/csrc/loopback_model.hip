@@ -762,12 +762,13 @@ int lmo_layer_norm_bwd(const void* dy, const void* h, const void* w, const float
     })
     const int err = launched();
     if (err) return err;
-    if (dw || db)
+    if (dw || db) {
       LMO_BOOL_SWITCH(d > 2048, WIDE, {
         constexpr int COLS = WIDE ? 64 : 16;
         hipLaunchKernelGGL((k_layer_norm_sum<T, COLS>), dim3((unsigned)((d + COLS - 1) / COLS), 2), dim3(SUM_LANES), 0, st, a.part_w,
                            a.part_b, static_cast<T*>(dw), static_cast<T*>(db), parts, (int)d);
       })
+    }
   })
   return launched();
 }

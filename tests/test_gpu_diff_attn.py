@@ -194,6 +194,20 @@ def test_few_queries_over_long_caches(b, tq, tk, h, hk):
     check(ts, False, lengths=lengths, starts=lengths - tq)
 
 
+@pytest.mark.parametrize("train", [True, False])
+@pytest.mark.parametrize("b,tq,tk,h,hk,dh,dv,dtype", [
+    (1, 333, 2049, 4, 2, 64, 128, torch.bfloat16), (2, 65, 5000, 2, 1, 40, 80, torch.float16), (1, 1, 3000, 2, 2, 64, 64, torch.bfloat16),
+    (1, 700, 1100, 6, 3, 128, 256, torch.bfloat16), (3, 2000, 800, 1, 1, 32, 32, torch.float16)])
+def test_few_blocks_over_long_keys(b, tq, tk, h, hk, dh, dv, dtype, train):
+    """Blocks of queries too few for the CUs, whose keys go in chunks: sequences that end before a chunk, and within one."""
+    ts = operands(b, tq, tk, h, hk, dh, dv, dtype, "token")
+    check(ts, train)
+    check(ts, train, causal=False)
+    lengths = ints(*(min(tk, 255 + 300 * i) for i in range(b)))
+    check(ts, train, lengths=lengths, starts=lengths - tq // 2)
+    check(ts, train, lengths=ints(*(0 if i == 0 else tk for i in range(b))), starts=ints(*(-3 if i == 0 else 600 for i in range(b))))
+
+
 def test_far_scores():
     """Scores of hundreds, rising and falling along the keys: the running maximum moves at every tile, or never."""
     for sign in (1.0, -1.0):
