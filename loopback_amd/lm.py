@@ -457,8 +457,10 @@ def teacher_top(model: LoopbackLM, ids: torch.Tensor, k: int, temperature: float
     exp(logit / temperature) over the vocabulary (B, T) in fp32, for LoopbackLM.distill. In evaluation, without dropout."""
     was = model.training
     model.eval()
-    logits = model.head(model.hidden(ids))
-    model.train(was)
+    try:
+        logits = model.head(model.hidden(ids))
+    finally:
+        model.train(was)
     top = torch.topk(logits, k, dim=-1)
     lse = torch.stack([torch.logsumexp(row.float() / temperature, -1) for row in logits])   # a sequence at a time: fp32 rows are large
     return top.values, top.indices, lse

@@ -208,6 +208,23 @@ def test_few_blocks_over_long_keys(b, tq, tk, h, hk, dh, dv, dtype, train):
     check(ts, train, lengths=ints(*(0 if i == 0 else tk for i in range(b))), starts=ints(*(-3 if i == 0 else 600 for i in range(b))))
 
 
+def test_a_cache_past_32_bits():
+    """Keys and values as parts of wide rows, 5 GB from the first to the last: the result and the gradients of compact copies."""
+    tk, wide = 20000, 2 ** 17
+    big = torch.empty(tk * wide, dtype=torch.bfloat16, device=DEV).view(1, tk, wide)
+    q, k, v, lam = operands(1, 3, tk, 2, 1, 64, 128, torch.bfloat16)
+    far = [big[:, :, 64:192].view(1, tk, 2, 64), big[:, :, wide - 128:].view(1, tk, 1, 128)]
+    far[0].copy_(k), far[1].copy_(v)
+    assert (tk - 1) * wide * 2 > 2 ** 32 and torch.equal(M.diff_attention(q, *far, lam), M.diff_attention(q, k, v, lam))
+    leaves = [t.detach().requires_grad_() for t in (q, *far, lam)]
+    near = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    a, b = M.diff_attention(*leaves), M.diff_attention(*near)
+    dy = rnd(a.shape, torch.bfloat16, 7)
+    assert torch.equal(a, b)
+    for x, y in zip(torch.autograd.grad(a, leaves, dy), torch.autograd.grad(b, near, dy)):
+        assert torch.equal(x, y)
+
+
 def test_far_scores():
     """Scores of hundreds, rising and falling along the keys: the running maximum moves at every tile, or never."""
     for sign in (1.0, -1.0):

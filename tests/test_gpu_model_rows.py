@@ -274,6 +274,62 @@ def test_distill(rows, vocab, k, tau, hard, dtype):
     check_distill(x, top.to(dtype), ids.to(torch.int32), lse=lse_of(top.to(dtype), ids, tau), **args)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tau", [0.5, 3.0, 4.0, 7.5])
+@pytest.mark.parametrize("rows,vocab,k", [(5, 2049, 64), (700, 9001, 12)])
+def test_distill_temperatures(rows, vocab, k, tau, dtype):
+    """The labels' softmax beside one at other temperatures."""
+    ids, top, labels = teacher_of(rows, vocab, k, 5)
+    x = rnd((rows, vocab), dtype, 6, 3.0)
+    args = {"labels": labels, "tau": tau, "hard": 0.3, "scale": 1024.0 if dtype is torch.float16 else 1.0}
+    check_distill(x, top, ids, **args)
+    check_distill(x, top, ids, lse=lse_of(top, ids, tau), **args)
+
+
+@pytest.mark.parametrize("tau,hard", [(1.0, 0.0), (1.0, 0.3), (2.0, 0.3), (4.0, 0.3), (3.0, 0.3)])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distill_past_the_caches(dtype, tail, tau, hard):
+    """Logits of more than the caches hold, and the same rows in two calls of half as many: a row's gradient is the same value, less
+    by the number of rows, a power of two."""
+    rows, vocab, k = 4096, 16397, 7
+    x = torch.empty(rows, vocab, dtype=dtype, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(2)).requires_grad_()
+    ids, top, labels = teacher_of(rows, vocab, k, 3, pad=False)
+    top, labels = top.to(dtype), labels.clamp_min(0) if hard else None
+    lse = lse_of(top, ids, tau) if tail else None
+    def run(at):
+        part = [None if t is None else t[at] for t in (lse, labels)]
+        loss = M.distill_loss(x[at], top[at], ids[at], temperature=tau, teacher_lse=part[0], labels=part[1], hard_weight=hard)
+        return loss, torch.autograd.grad(loss, x)[0][at]
+    whole, grad = run(slice(None))
+    halves = [slice(0, rows // 2), slice(rows // 2, rows)]
+    # a mean of 4096 fp32 terms within 16 roundings of their sum
+    assert abs(whole - sum(run(at)[0] for at in halves) / 2) <= 64 * U * abs(whole)
+    for at in halves:
+        assert torch.equal(2 * grad[at], run(at)[1])
+
+
+def test_rows_past_32_bits():
+    """More than 2^31 elements: the last rows are what they are alone."""
+    x = torch.empty(140000, 16384, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(4))
+    last = x[-9:].clone()
+    leaf, alone = x.requires_grad_(), last.clone().requires_grad_()
+    y, z = M.layer_norm(leaf), M.layer_norm(alone)
+    assert x.numel() > 2 ** 31 and torch.equal(y[-9:], z)
+    g = torch.autograd.grad(y, leaf, y.detach())[0]
+    assert torch.equal(g[-9:], torch.autograd.grad(z, alone, z.detach())[0])
+    del y, g
+    x = leaf.detach().view(-1)[:65536 * 35000].view(65536, 35000)
+    ids, top, labels = teacher_of(8, 35000, 5, 3, pad=False)
+    few, labels = x[-8:].clone().requires_grad_(), labels.clamp_min(0)
+    loss = M.distill_loss(few, top, ids, temperature=2.0, labels=labels, hard_weight=0.5)
+    want = torch.autograd.grad(loss, few)[0]
+    many = lambda t: t.repeat(8192, *[1] * (t.dim() - 1))
+    leaf = x.requires_grad_()
+    loss = M.distill_loss(leaf, many(top), many(ids), temperature=2.0, labels=many(labels), hard_weight=0.5)
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0][-8:] * 8192, want) and loss.isfinite()
+
+
 def test_distill_every_class_named():
     """Nothing is left for the others: the term is 0, not a logarithm of nothing."""
     x = rnd((3, 12), torch.float32, 1)
