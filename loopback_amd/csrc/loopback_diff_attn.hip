@@ -13,7 +13,7 @@
 // 32 x 32 result it holds column l mod 32 and, in register r, row 4 (l / 32) + r mod 4 + 8 (r / 4). Scores are formed so that
 // the next product sums over their rows: a result is then the next one's B operand as it lies in the registers, its k order
 // that of Cols32. What a wave keeps in registers are its 32 queries (forward, dq) or keys (dk, dv); the others come through
-// LDS in tiles of 64 rows, two buffers, filled by direct loads. A tile's rows are unpadded and its 16-byte pieces permuted
+// LDS in tiles of 32 or 64 rows, two buffers, filled by direct loads. A tile's rows are unpadded and its 16-byte pieces permuted
 // (swizzle), so that neither the reads of rows nor the transposing reads of columns meet in a bank.
 
 #include <hip/hip_runtime.h>
@@ -38,7 +38,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void global_void;
 
-constexpr int WG = 256, QB = 128, TILE = 64;      // lanes, rows kept per workgroup (32 a wave), rows per LDS tile
+constexpr int WG = 256, QB = 128, TILE = 64;      // lanes, rows kept per workgroup (32 a wave), rows per LDS tile of dq's kernel
 constexpr float LAZY = 8.f;                        // the maximum moves when it grows by 2^8 or more
 constexpr float NONE = -1e30f;                     // the maximum of no scores: finite, so that differences from it are
 constexpr float LOG2E = 1.4426950408889634f;
@@ -334,8 +334,11 @@ template <int DH, int DV> constexpr int waves_bwd() { return DH + DV <= 192 ? 2 
 // ---------------------------------------------------------------------------------------------------------------
 // forward: 64 queries of a head per workgroup, two waves for each 32 of them, one for each map. (Both maps in one wave read
 // the values once for both, but hold 256 registers, so two waves to a SIMD, in which the vector units, a wave's softmax, wait
-// for its products and the other way round; so it is three here.) The vector units bound it: per 32 x 32 scores of a map 16
-// exponentials of 16 cycles and some five operations of 4 for each, 580 cycles, against 384 of matrix cores.
+// for its products and the other way round; so it is three here.) Vector units and matrix cores bound it: per 32 x 32 scores of a
+// map 16 exponentials of 8 cycles and some 80 operations of 4, 490 cycles with what the issue of products costs, and 384 of
+// products; the two overlap little (counters: 0.48 and 0.37 of the time). 8 x 2048 tokens, 6 heads of 64|128 in bf16: 101 us, 77 GFLOP
+// done at 0.77 PFLOP/s; 2 x 4096, 16 heads: 235 us, 0.88. A tile's scores formed between the exponentials of the tile before, so
+// that one wave's products and softmax overlap: 107 us. Tiles of 64 keys: 111, eight waves to a workgroup: 218.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int FW = 4, FQ = 16 * FW, FT = 32, FL = 64 * FW;   // waves and queries of a workgroup, keys of a tile, lanes
 template <int DH, int DV> constexpr int waves_fwd() { return DH <= 64 && DV <= 128 ? 3 : 2; }
@@ -476,7 +479,9 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
 // few queries: the (query, head of the group) pairs of a head of keys are the 32 rows of one block (tq times the group at
 // most 32). A workgroup takes a chunk of its keys, in tiles of 64: two waves for each map, each with 32 keys of a tile. The
 // keys' and values' stream bounds it, so the probabilities enter the products as two 16-bit parts: their rounding is not added to
-// the result's. The waves' results meet in LDS, and those of the chunks in k_diff_join.
+// the result's. The waves' results meet in LDS, and those of the chunks in k_diff_join. One token each over 32 caches of up to 8192
+// keys, 8 heads on 2 of 64|128 in bf16: 40 us, 201 MB at 5.0 TB/s, and 4 for the join (a wave for each map and half of a tile's keys
+// each, not a wave for both maps and a quarter, which held too many registers: 46 to 53 us).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int FEW = 32, NT = 64;   // rows, keys of a tile
 template <int DH, int DV> constexpr int few_lds() {   // two tiles; at the end the four waves' results
@@ -683,7 +688,9 @@ template <typename T, int DV, bool SHARED> __global__ __launch_bounds__(WG) void
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// backward: dq, the deltas and dlam's parts. 128 queries of a head per workgroup, as the forward
+// backward: dq, the deltas and dlam's parts. 128 queries of a head per workgroup, both maps in a wave, which share dA. Bound as the
+// forward is, by vector units (0.39 of the time) and matrix cores (0.30) that overlap little, at two waves to a SIMD: 8 x 2048 tokens, 6
+// heads of 64|128: 122 us, 77 GFLOP at 0.63 PFLOP/s; 2 x 4096, 16 heads: 281 us, 0.73. Operands read a step ahead spill: 141.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int DH, int DV>
 __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<DH, DV>())))) void k_diff_bwd_q(const Diff a) {
@@ -862,6 +869,9 @@ template <typename T> __global__ __launch_bounds__(WG) void k_diff_dlam(const fl
 // else 1, and P2' = |lam| P2 = exp2(c s2 - (lse2 - log2 |lam|)), the numbers are lse1, lse2 - log2 |lam|, -D1 (where the product
 // for dA begins), s (D2 - D1) and -s, so that
 //   P = P1 - s P2',   dS1 = P1 (dA - D1),   dS2 = P2' (s (D2 - D1) - s (dA - D1))
+// 8 x 2048 tokens, 6 heads of 64|128: 148 us, 103 GFLOP at 0.70 PFLOP/s (vector units 0.36 of the time, matrix cores 0.32); 2 x 4096, 16
+// heads on 4: 437 us and 13 for the parts' sum. The values in LDS, not in registers, leave two waves to a SIMD without spills; 64 keys
+// to a wave at one wave took 285 us, scratch loads between the tiles' loads, which they wait for, 188 to 221.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int KVT = 32;   // queries of a tile
 template <typename T, int W> struct Kept16 {   // a wave's 32 rows as B operands: row 16 n + l mod 16, columns 32 ks + 8 (l / 16) .. + 8

@@ -247,7 +247,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
 
     A query i of batch row n sees the keys j < lengths[n] (all tk without it) and, where causal, j <= starts[n] + i: starts is the
     position of the first query among the keys, tk - tq without it (the queries are the last tokens). A query that sees no key has
-    zeros and no gradient. What k and v hold at and past lengths is not read into anything, and its gradient is zero. lengths and
+    zeros and no gradient. What k and v hold at and past lengths is not read into anything, and its gradient is zero; an infinity or
+    a NaN among the keys before that may also reach queries that do not see it yet, as a product with a probability of 0. lengths and
     starts are int32 or int64 (b,), read when a kernel runs. Differentiable in q, k, v and lam."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or not (q.is_floating_point() and k.is_floating_point() and v.is_floating_point()):
         raise ValueError(f"diff_attention takes floating point q (b, tq, 2 H, dh), k (b, tk, 2 G, dh), v (b, tk, G, dv), got {tuple(q.shape)}, "
