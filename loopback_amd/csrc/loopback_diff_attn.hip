@@ -180,8 +180,12 @@ template <template <int> class R, int W, typename O> __device__ __forceinline__ 
 
 // 16 bytes (or 4) of memory for each lane, at base + off, to LDS at `to` and what follows it in the lanes' order. In assembly:
 // the compiler would wait for it before any read of LDS, of the other buffer too. The data is there past filled().
-__device__ __forceinline__ void load_lds16(const void* base, uint32_t off, int to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+// ONCE: data that no one reads again soon, past the caches
+template <bool ONCE = false> __device__ __forceinline__ void load_lds16(const void* base, uint32_t off, int to) {
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(off), "s"(base) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void load_lds4(const void* base, uint32_t off, int to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
@@ -190,7 +194,7 @@ __device__ __forceinline__ void load_lds4(const void* base, uint32_t off, int to
 // Fills N rows of LDS from memory by LANES lanes (whole waves). MAPS rows of memory of W / MAPS elements (`width` of them
 // exist, the columns past them repeat the first piece: what they meet is zero) lie side by side in a row of LDS. Rows past
 // row `last` repeat it.
-template <typename T, int W, int MAPS, int N, int LANES> struct Fill {
+template <typename T, int W, int MAPS, int N, int LANES, bool ONCE = false> struct Fill {
   static constexpr int P = W / 8, PASSES = N * P / LANES, PM = P / MAPS, ROWS = LANES / P, VAR = ROWS >= 16 ? 1 : 16 / ROWS;
   static_assert(N * P % LANES == 0 && N % 16 == 0, "whole passes, whole turns of the swizzle");
   const T* base;      // row 0
@@ -211,12 +215,12 @@ template <typename T, int W, int MAPS, int N, int LANES> struct Fill {
     const char* b = reinterpret_cast<const char*>(base + (int64_t)row0 * stride);
     if (row0 + N - 1 <= last) {
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) load_lds16(b + 2 * i * ROWS * stride, off[i % VAR], to + 16 * i * LANES);
+      for (int i = 0; i < PASSES; ++i) load_lds16<ONCE>(b + 2 * i * ROWS * stride, off[i % VAR], to + 16 * i * LANES);
     } else {
       const int r = kept((int)(threadIdx.x % LANES) / P);   // formed here, where it is rarely needed, and not kept
 #pragma unroll
       for (int i = 0; i < PASSES; ++i)
-        load_lds16(b, off[i % VAR] + 2u * (uint32_t)(min(r + ROWS * i, last - row0) - r) * (uint32_t)stride, to + 16 * i * LANES);
+        load_lds16<ONCE>(b, off[i % VAR] + 2u * (uint32_t)(min(r + ROWS * i, last - row0) - r) * (uint32_t)stride, to + 16 * i * LANES);
     }
   }
 };
@@ -480,8 +484,8 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
 // most 32). A workgroup takes a chunk of its keys, in tiles of 64: two waves for each map, each with 32 keys of a tile. The
 // keys' and values' stream bounds it, so the probabilities enter the products as two 16-bit parts: their rounding is not added to
 // the result's. The waves' results meet in LDS, and those of the chunks in k_diff_join. One token each over 32 caches of up to 8192
-// keys, 8 heads on 2 of 64|128 in bf16: 40 us, 201 MB at 5.0 TB/s, and 4 for the join (a wave for each map and half of a tile's keys
-// each, not a wave for both maps and a quarter, which held too many registers: 46 to 53 us).
+// keys, 8 heads on 2 of 64|128 in bf16: 41 us, 201 MB at 4.9 TB/s past the caches (44 through them), and 4 for the join. (A wave for
+// both maps and a quarter of a tile's keys held too many registers: 60 where this took 44. Two and a half times as many chunks: 45.)
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int FEW = 32, NT = 64;   // rows, keys of a tile
 template <int DH, int DV> constexpr int few_lds() {   // two tiles; at the end the four waves' results
@@ -510,8 +514,8 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu(2))) void k_
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = zero16();
   Soft sm;
-  const Fill<T, 2 * DH, 2, NT, WG> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
-  const Fill<T, DV, 1, NT, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
+  const Fill<T, 2 * DH, 2, NT, WG, true> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
+  const Fill<T, DV, 1, NT, WG, true> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
   if (c0 < c1) {
     kf.fetch(c0, len - 1, K0);
     vf.fetch(c0, len - 1, V0);
