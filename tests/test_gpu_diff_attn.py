@@ -225,6 +225,24 @@ def test_a_cache_past_32_bits():
         assert torch.equal(x, y)
 
 
+def test_one_tensor_twice():
+    """The queries as the keys too, and keys that are the values' storage: the same results and gradients as from copies."""
+    q, _, _, lam = operands(2, 100, 100, 2, 2, 64, 128, torch.bfloat16)
+    far = lam.detach()[0].expand(2, 100, 2)   # one value for every query, without strides
+    def run(q, k, v, lam):
+        y = M.diff_attention(q, k, v, lam)
+        return y, torch.autograd.grad(y, [q], rnd(y.shape, torch.bfloat16, 5))[0]
+    one = q.detach().requires_grad_()
+    two = [q.detach().clone().requires_grad_() for _ in range(3)]
+    y, g = run(one, one, one.view(2, 100, 2, 128), far)
+    z = M.diff_attention(two[0], two[1], two[2].view(2, 100, 2, 128), far.contiguous())
+    grads = torch.autograd.grad(z, two, rnd(z.shape, torch.bfloat16, 5))
+    assert torch.equal(y, z)
+    # the three gradients are added in bf16, in any order
+    total, size = sum(t.double() for t in grads), sum(t.double().abs() for t in grads)
+    assert ((g.double() - total).abs() <= 2 * 2.0 ** -8 * size).all()
+
+
 def test_far_scores():
     """Scores of hundreds, rising and falling along the keys: the running maximum moves at every tile, or never."""
     for sign in (1.0, -1.0):

@@ -129,6 +129,19 @@ def test_norm_strides_and_alignment(d):
     assert x.grad.shape == x.shape and x.grad.isfinite().all()
 
 
+def test_norm_of_one_tensor_twice():
+    """A tensor added to itself, and one vector as weight and bias: both places' gradients come to it."""
+    x, w = rnd((70, 136), torch.float32, 1).requires_grad_(), rnd((136,), torch.float32, 2).requires_grad_()
+    h, y = M.add_layer_norm(x, x, w, w)
+    a, b = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    z = torch.nn.functional.layer_norm(2 * a, (136,), b, b)
+    dy, dh = rnd(y.shape, torch.float32, 3), rnd(h.shape, torch.float32, 4)
+    got = torch.autograd.grad([h, y], [x, w], [dh, dy])
+    ref = torch.autograd.grad([2 * a, z], [a, b], [dh.double(), dy.double()])
+    assert torch.equal(h, 2 * x)
+    close(y, z, 1e-5), close(got[0], ref[0], 1e-4), close(got[1], ref[1], 1e-3)   # sums of 70 terms of up to 10: 70 10 2^-24 and less
+
+
 def test_norm_gradients_that_are_asked_for():
     d = 256
     x, a, w, b = rnd((33, d), torch.bfloat16, 1), rnd((33, d), torch.bfloat16, 2), rnd((d,), torch.bfloat16, 3), rnd((d,), torch.bfloat16, 4)
