@@ -695,6 +695,9 @@ template <typename T, int DV, bool SHARED> __global__ __launch_bounds__(WG) void
 // backward: dq, the deltas and dlam's parts. 128 queries of a head per workgroup, both maps in a wave, which share dA. Bound as the
 // forward is, by vector units (0.39 of the time) and matrix cores (0.30) that overlap little, at two waves to a SIMD: 8 x 2048 tokens, 6
 // heads of 64|128: 122 us, 77 GFLOP at 0.63 PFLOP/s; 2 x 4096, 16 heads: 281 us, 0.73. Operands read a step ahead spill: 141.
+// D1 and D2 come from the rounded y and P2 v, where many keys share them; for a workgroup whose queries see at most two tiles, where
+// dA - D is a small part of both, a pass before sums P dA in fp32 (the first block of a causal sequence, short ones: no time). Of a
+// single key's probability the gradient is zero, and exactly that.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int DH, int DV>
 __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<DH, DV>())))) void k_diff_bwd_q(const Diff a) {
@@ -737,14 +740,6 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
   d1 = __builtin_fmaf(lam, d2, other_half(d1, true));
   const int64_t n = ((int64_t)b * a.h + head) * a.tq + qrow, all = (int64_t)a.b * a.h * a.tq;
   const float ls1 = a.lse[n], ls2 = a.lse[n + all];
-  if (query < a.tq && half == 0) {   // what the kernel of dk and dv reads: see there
-    const float sign = lam < 0.f ? -1.f : 1.f;
-    a.delta[n] = ls1;
-    a.delta[n + all] = ls2 - __builtin_amdgcn_logf(fabsf(lam));
-    a.delta[n + 2 * all] = -d1;
-    a.delta[n + 3 * all] = sign * (d2 - d1);
-    if (a.lam_rows) a.delta[n + 4 * all] = -sign;
-  }
   const int seen = seen_by(a, qrow, start, len);
   const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len);
   const int wmost = w0 < a.tq ? seen_by(a, min(w0 + 32, a.tq) - 1, start, len) : 0, wleast = seen_by(a, min(w0, a.tq - 1), start, len);
@@ -763,6 +758,45 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     vf.fetch(0, len - 1, V0);
   }
   filled();   // in every case: a wait for what was loaded above, left to the loop, would wait there for the tiles too
+  if (most <= 2 * TILE) {   // workgroup-uniform
+    if (ntiles > 1) {
+      kf.fetch(TILE, len - 1, K1);
+      vf.fetch(TILE, len - 1, V1);
+      filled();
+    }
+    float e[2] = {0.f, 0.f};
+    auto terms = [&](int k0, int kt, int vt) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x16 da = zero16();
+#pragma unroll
+        for (int ks = 0; ks < DV / 16; ++ks) da = Mat<T>::mfma(vrows.at(vt, 32 * i, ks), g.f[ks], da);
+        const int left = seen - k0 - 32 * i - 4 * half;
+#pragma unroll
+        for (int map = 0; map < 2; ++map) {
+          f32x16 x = zero16();
+#pragma unroll
+          for (int ks = 0; ks < DH / 16; ++ks) x = Mat<T>::mfma(krows.at(kt, 32 * i, map * (DH / 16) + ks), q[map].f[ks], x);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (row_of(r, 0) < left) e[map] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.c, map ? -ls2 : -ls1)), da[r], e[map]);
+        }
+      }
+    };
+    if (0 < wmost) terms(0, K0, V0);
+    if (TILE < wmost) terms(TILE, K1, V1);
+    d1 = other_half(e[0], true);
+    d2 = other_half(e[1], true);
+    __syncthreads();   // the second tile, which the loop fetches again, has been read
+  }
+  if (query < a.tq && half == 0) {   // what the kernel of dk and dv reads: see there
+    const float sign = lam < 0.f ? -1.f : 1.f;
+    a.delta[n] = ls1;
+    a.delta[n + all] = ls2 - __builtin_amdgcn_logf(fabsf(lam));
+    a.delta[n + 2 * all] = -d1;
+    a.delta[n + 3 * all] = seen == 1 ? 0.f : sign * (d2 - d1);
+    if (a.lam_rows) a.delta[n + 4 * all] = -sign;
+  }
   auto tile = [&](int j, auto buffer) {
     constexpr int cur = decltype(buffer)::value;   // known: the buffers' offsets go into the reads' own
     const int k0 = j * TILE;
@@ -818,7 +852,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     T* row = static_cast<T*>(a.dq) + (((int64_t)b * a.tq + query) * 2 * a.h + 2 * head) * a.dh;
 #pragma unroll
     for (int map = 0; map < 2; ++map) {
-      const float f = map ? -lam * a.scale : a.scale;
+      const float f = seen == 1 ? 0.f : map ? -lam * a.scale : a.scale;
 #pragma unroll
       for (int e = 0; e < QB_; ++e)
 #pragma unroll
@@ -1028,6 +1062,9 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (r0 + r >= left || here + r0 + r < from[n]) s1[n][r] = s2[n][r] = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)   // the probability of a query's only key does not change
+            if (seen_by(a, here + r0 + r, start, len) == 1) da[u][0][r] = da[u][1][r] = 0.f;
         }
         auto number = [&](int e) { return lds_at<f32x4>(numbers + rt + 4 * (e * KVT + r0)); };
         const f32x4 ls1 = number(0), ls2 = number(1);

@@ -225,6 +225,46 @@ def test_a_cache_past_32_bits():
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dh,dv", [(64, 128), (128, 256), (40, 80)])
+def test_a_single_key_has_no_score_gradient(dh, dv, dtype):
+    """Sequences of one key, the first query of a causal one, and one key for many queries: zeros, as the probability is 1."""
+    for t, causal, lengths in ((1, True, None), (70, True, None), (70, False, ints(1, 1)), (70, True, ints(1, 70))):
+        leaves = [x.detach().requires_grad_() for x in operands(2, t, t, 4, 2, dh, dv, dtype, "token")]
+        y = M.diff_attention(*leaves, causal=causal, lengths=lengths)
+        dq, dk, dval, _ = torch.autograd.grad(y, leaves, rnd(y.shape, dtype, 8))
+        assert (dq[:, 0] == 0).all() and dval[:, 0].abs().max() > 0
+        if t == 1 or not causal:
+            assert (dq == 0).all() and (dk == 0).all()
+        elif lengths is not None:
+            assert (dq[0] == 0).all() and (dk[0] == 0).all() and dq[1, 1:].abs().max() > 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t", [2, 3, 4, 9, 40, 100, 128])
+def test_score_gradients_of_short_sequences(t, dtype):
+    """Of up to 128 keys the sums that a score's gradient is relative to are fp32: it is rounded once to the type, and its products'
+    sum once. fp32's share: dA and D are sums of 128 products, P a score's exponential, within 64 u of |dy| |v| and of themselves."""
+    q, k, v, lam = operands(2, t, t, 1, 1, 64, 128, dtype)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, lam)]
+    y = M.diff_attention(*leaves)
+    dy = rnd(y.shape, dtype, 8)
+    dq, dk = torch.autograd.grad(y, leaves[:2], dy)
+    h, c = HALF[dtype], 64 ** -0.5
+    q, k, v, g, lam = (x.detach().double() for x in (q, k, v, dy, lam))
+    da, size = g[:, :, 0] @ v[:, :, 0].transpose(1, 2), g[:, :, 0].abs() @ v[:, :, 0].abs().transpose(1, 2)
+    for e, f in ((0, 1.0), (1, -float(lam[0]))):
+        s = q[:, :, e] @ k[:, :, e].transpose(1, 2) * c
+        p = s.masked_fill(torch.ones(t, t, device=DEV).triu(1).bool(), -math.inf).softmax(-1)
+        ds = c * f * p * (da - (p * da).sum(-1, keepdim=True))
+        fp32 = 128 * U * c * abs(f) * p * (size + (p * size).sum(-1, keepdim=True))
+        for got, other, left in ((dq[:, :, e], k[:, :, e], ds), (dk[:, :, e], q[:, :, e], ds.transpose(1, 2))):
+            more = fp32 if left is ds else fp32.transpose(1, 2)
+            bound = (h * left.abs() + (1 + h) * more) @ other.abs()
+            ref = left @ other
+            assert ((got.double() - ref).abs() <= h * (ref.abs() + bound) + bound + FLOOR[dtype] * (1 + other.abs().sum(1, keepdim=True))).all()
+
+
 def test_one_tensor_twice():
     """The queries as the keys too, and keys that are the values' storage: the same results and gradients as from copies."""
     q, _, _, lam = operands(2, 100, 100, 2, 2, 64, 128, torch.bfloat16)
