@@ -868,15 +868,19 @@ PyObject* host_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // torch_forms(dropout, join, ffn): the Python functions that the nodes call where a backward has to be torch operations
-// q [b, tq, 2 h, dh], k [b, tk, 2 hk, dh], v [b, tk, hk, dv] as the kernels take them: themselves, or contiguous copies
+// q [b, tq, 2 h, dh], k [b, tk, 2 hk, dh], v [b, tk, hk, dv] as the kernels take them: themselves, or contiguous copies. A dimension
+// of one may have any stride, which contiguous() keeps and nothing steps by: the kernels get 0 for it
 at::Tensor attn_rows(const at::Tensor& t) {
-  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(1) <= (1 << 23) && t.stride(2) <= (1 << 23);
-  for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
+  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) % 8 == 0 && (i == 0 || t.stride(i) <= (1 << 23))));
   if (ok) return t;
   at::Tensor c = t.contiguous();
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
-lmo_strides strides_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+lmo_strides strides_of(const at::Tensor& t) {
+  const auto step = [&](int i) { return t.size(i) == 1 ? 0 : t.stride(i); };
+  return {t.data_ptr(), step(0), step(1), step(2)};
+}
 lmo_strides lam_strides(const at::Tensor& t) {   // one value, one per head, or one per query and head
   return t.dim() == 3 ? lmo_strides{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}
                       : lmo_strides{t.data_ptr(), 0, 0, t.dim() == 1 ? t.stride(0) : 0};

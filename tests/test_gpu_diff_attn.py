@@ -318,6 +318,48 @@ def test_scale_strides_alignment():
         assert torch.equal(x, y)
 
 
+def test_strides_of_dimensions_of_one():
+    """A dimension of one may have any stride, which a contiguous copy keeps: one sequence and one token of a projection of an odd
+    width, one sequence cut from odd rows, one head of keys cached heads first and further than 2^23 elements apart."""
+    dt = torch.bfloat16
+    def same(ts, views, **how):
+        for n, (t, x) in enumerate(zip(ts, views)):
+            assert torch.equal(t, x), n
+        assert torch.equal(M.diff_attention(*views, **how), M.diff_attention(*ts, **how))
+        a, b = ([t.detach().requires_grad_() for t in x] for x in (views, ts))
+        ya, yb = M.diff_attention(*a, **how), M.diff_attention(*b, **how)
+        dy = rnd(ya.shape, dt, 9)
+        assert torch.equal(ya, yb)
+        for x, y in zip(torch.autograd.grad(ya, a, dy), torch.autograd.grad(yb, b, dy)):
+            assert torch.equal(x, y)
+
+    ts = operands(1, 1, 1, 4, 2, 64, 128, dt, "token")
+    row, at, views = torch.cat([t.flatten() for t in ts]), 0, []
+    for t in ts:
+        views.append(row.as_strided(t.shape, (1028, 1028, *t.stride()[2:]), at))
+        at += t.numel()
+    same(ts, views)
+    *rows, lam = operands(1, 2, 2, 2, 2, 64, 128, dt)
+    same([*rows, lam], [*(t.as_strided(t.shape, (517, *t.stride()[1:])) for t in rows), lam])
+    for tq in (1, 3):   # a kernel of few queries, and for a backward the others
+        q, k, v, lam = operands(1, tq, 70000, 2, 1, 64, 128, dt)
+        far = v.transpose(1, 2).contiguous().transpose(1, 2)
+        far = far.as_strided(far.shape, (70000 * 128, 128, 70000 * 128, 1))
+        assert far.stride(2) > 2 ** 23
+        same([q, k, v, lam], [q, k, far, lam])
+
+
+def test_rows_too_far_apart_for_the_kernels():
+    """Rows of more than 2^23 elements: torch operations."""
+    q = torch.zeros(1, 2, 2 ** 17 + 2, 64, dtype=torch.bfloat16, device=DEV)
+    k, v = rnd((1, 2, 2, 64), torch.bfloat16, 1), rnd((1, 2, 1, 128), torch.bfloat16, 2)
+    lam = torch.tensor(0.5, device=DEV)
+    assert not M.attention_native(q, k, v, lam) and M.attention_native(q[:, :1], k, v, lam) and M.attention_native(q[:, :, 2:], k, v, lam)
+    close(M.diff_attention(q, k, v, lam)[:, :, :2], *reference(q[:, :, :4], k, v, lam, None)["y"], "y")
+    one = M.diff_attention(q[:, :1], k, v, lam)
+    close(one[:, :, -2:], *reference(q[:, :1, -4:], k, v, lam, None)["y"], "y")
+
+
 def test_gradients_that_are_asked_for():
     ts = operands(2, 77, 77, 4, 2, 64, 128, torch.bfloat16)
     dy = rnd((2, 77, 4, 128), torch.bfloat16, 9)
