@@ -93,7 +93,7 @@ int lmo_diff_attn_fwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
 int64_t lmo_diff_attn_bwd_scratch(const lmo_diff_shape* shape, int lam_kind);
 
 /* The gradients, contiguous, of the forward's shapes: dq, and, where wanted (dk and dv both or neither), dk, dv and dlam. dy is
- * contiguous. Rows of dk and dv that no query sees are zeros. */
+ * contiguous, its rows H dv of up to 2^26 elements where there are several. Rows of dk and dv that no query sees are zeros. */
 int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
                       const int32_t* lengths, const int32_t* starts, const void* out, const void* second, const float* lse,
                       const void* dy, void* dq, void* dk, void* dv, void* dlam, int lam_kind, float* scratch,

@@ -1344,6 +1344,7 @@ int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
   int e = diff_args(s, q, k, v, dtype);
   if (e) return e;
   if (lam_kind < LMO_LAM_LAYER || lam_kind > LMO_LAM_TOKEN) return LDR_E_ARG;
+  if (s->tq > 1 && s->h * s->dv > (1 << 26)) return LDR_E_SHAPE;   // 32 rows of dy within 32 bits of bytes
   if (s->b * s->tq == 0) return LDR_OK;
   if (!lam || !lam->p || !out || !second || !lse || !dy || !dq || !scratch || !dk != !dv) return LDR_E_ARG;
   for (const void* p : {out, second, dy, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)scratch})

@@ -149,7 +149,7 @@ def add_layer_norm(x: torch.Tensor, add: torch.Tensor | None, weight: torch.Tens
 # differential attention
 # ---------------------------------------------------------------------------------------------------------------
 ATTN_MAX_DH, ATTN_MAX_DV, ATTN_MAX_TOKENS, ATTN_MAX_HEADS, ATTN_MAX_ROWS = 128, 256, 2 ** 30 - 1, 0x7fffff, 2 ** 29
-ATTN_MAX_STRIDE = 2 ** 23
+ATTN_MAX_STRIDE, ATTN_MAX_OUT = 2 ** 23, 2 ** 26   # between rows of q, k and v, and of y's gradient
 
 
 def _seen(b, tq, tk, causal, lengths, starts, device):
@@ -236,7 +236,8 @@ def attention_native(q, k, v, lam) -> bool:
             and 0 < v.shape[3] <= ATTN_MAX_DV and max(q.shape[1], k.shape[1]) <= ATTN_MAX_TOKENS and q.shape[0] * q.shape[2] <= ATTN_MAX_HEADS
             and q.shape[0] * q.shape[1] * q.shape[2] // 2 < ATTN_MAX_ROWS
             # a copy of rows has them that far apart
-            and all(t.shape[1] == 1 or t.shape[2] * t.shape[3] <= ATTN_MAX_STRIDE for t in (q, k, v)))
+            and all(t.shape[1] == 1 or t.shape[2] * t.shape[3] <= ATTN_MAX_STRIDE for t in (q, k, v))
+            and (q.shape[1] == 1 or q.shape[2] // 2 * v.shape[3] <= ATTN_MAX_OUT))
 
 
 def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, *, causal: bool = True,

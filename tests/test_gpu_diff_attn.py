@@ -360,6 +360,14 @@ def test_rows_too_far_apart_for_the_kernels():
     close(one[:, :, -2:], *reference(q[:, :1, -4:], k, v, lam, None)["y"], "y")
 
 
+def test_wide_results_take_torch_operations():
+    """Results of more than 2^26 elements a token, whose gradient's rows the kernels do not reach."""
+    def native(tq, h, dv):
+        one = torch.zeros(1, dtype=torch.bfloat16, device=DEV)
+        return M.attention_native(one.expand(1, tq, 2 * h, 8), one.expand(1, tq, 2, 8), one.expand(1, tq, 1, dv), one.expand(1, tq, h))
+    assert native(20, 2 ** 19, 128) and not native(20, 2 ** 19, 136) and native(1, 2 ** 19, 256)
+
+
 def test_gradients_that_are_asked_for():
     ts = operands(2, 77, 77, 4, 2, 64, 128, torch.bfloat16)
     dy = rnd((2, 77, 4, 128), torch.bfloat16, 9)

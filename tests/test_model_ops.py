@@ -291,3 +291,12 @@ def test_attention_argument_checks_before_launch():
     s = Strides(p, 1024, 128, 64)
     assert L.lmo_diff_attn_bwd(ref(s), ref(s), ref(s), ref(s), 1, None, None, p, p, p, p, p, p, None, None, 0, p, ref(few), 1, None) == -1
     assert L.lmo_diff_attn_bwd(ref(s), ref(s), ref(s), ref(s), 1, None, None, p, p, p, p, p, p, p, p, 7, p, ref(few), 1, None) == -1
+
+
+def test_attention_backward_refuses_wide_rows():
+    """Rows of dy whose distances of 32 are past 32 bits of bytes."""
+    p, ref = 4096, ctypes.byref
+    s = Strides(p, 2 ** 23, 2 ** 23, 8)
+    for h in (2 ** 18 + 1, 2 ** 19):
+        assert M.LIB.lmo_diff_attn_bwd(ref(s), ref(s), ref(s), ref(s), 1, None, None, p, p, p, p, p, p, p, p, 0, p,
+                                       ref(Shape(1, 20, 20, h, 1, 8, 256, 1, 0.125)), 1, None) == -2
