@@ -435,10 +435,11 @@ class LoopbackLM(nn.Module):
     def forward(self, ids: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
         return ops.next_token_loss(self.head(self.hidden(ids, rng)), ids)
 
-    def distill(self, ids: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.Tensor, rng: torch.Tensor | None = None, *,
-                temperature: float = 1.0, teacher_lse: torch.Tensor | None = None, hard_weight: float = 0.0) -> torch.Tensor:
+    def distill(self, ids: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.Tensor, teacher_lse: torch.Tensor | None = None, *,
+                rng: torch.Tensor | None = None, temperature: float = 1.0, hard_weight: float = 0.0) -> torch.Tensor:
         """The distillation loss (model_ops.distill_loss) towards a teacher's highest logits (B, T, k) of the classes top_ids at each
-        position of ids (teacher_top), mixed with the next tokens' cross entropy by hard_weight."""
+        position of ids, with teacher_lse the rest of its classes as one event (teacher_top gives the three, the third of its
+        temperature), mixed with the next tokens' cross entropy by hard_weight. rng: the dropout's, as forward takes it."""
         logits = self.head(self.hidden(ids, rng))
         labels = None
         if hard_weight:
@@ -454,21 +455,24 @@ class LoopbackLM(nn.Module):
 @torch.no_grad()
 def teacher_top(model: LoopbackLM, ids: torch.Tensor, k: int, temperature: float = 1.0):
     """What a teacher says of ids (B, T): its k highest logits, their classes (B, T, k), and the log of its sum of
-    exp(logit / temperature) over the vocabulary (B, T) in fp32, for LoopbackLM.distill. In evaluation, without dropout."""
-    was = model.training
+    exp(logit / temperature) over the vocabulary (B, T) in fp32: LoopbackLM.distill takes the three, or the first two, after ids. In
+    evaluation, without dropout."""
+    training = [m for m in model.modules() if m.training]
     model.eval()
     try:
         logits = model.head(model.hidden(ids))
     finally:
-        model.train(was)
+        for m in training:   # each by itself: what was kept in evaluation stays there
+            m.training = True
     top = torch.topk(logits, k, dim=-1)
     lse = torch.stack([torch.logsumexp(row.float() / temperature, -1) for row in logits])   # a sequence at a time: fp32 rows are large
     return top.values, top.indices, lse
 
 
 def train_step(model: LoopbackLM, opt: torch.optim.Optimizer, ids: torch.Tensor, teacher: tuple | None = None, **how) -> torch.Tensor:
-    """One training step: loss, backward, optimizer step, gradients released. Returns the loss (not synchronized). teacher: the
-    teacher's highest logits and their classes, and how's options, for LoopbackLM.distill."""
+    """One training step: loss, backward, optimizer step, gradients released. Returns the loss (not synchronized). teacher: what
+    LoopbackLM.distill takes after ids, the teacher's highest logits, their classes and, for the rest of its classes, its log of
+    sums; how: distill's options."""
     loss = model(ids) if teacher is None else model.distill(ids, *teacher, **how)
     loss.backward()
     opt.step()

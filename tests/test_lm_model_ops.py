@@ -155,6 +155,27 @@ def test_gradients_against_differences():
     assert abs((got[0] - got[1]) / (2 * eps) - exact) <= 1e-2 * max(1.0, abs(exact))
 
 
+def test_the_teacher_is_taken_as_it_is_given():
+    """What teacher_top gives goes into distill and train_step as a whole, the third value as the rest of the classes, not as the
+    dropout's generator; and the teacher's modules are in training or evaluation as they were."""
+    model, ids = make(**ALL), ids_of(2, 7)
+    other = make(seed=3, **ALL).train()
+    other.prelude.eval()
+    modes = [m.training for m in other.modules()]
+    top, classes, lse = teacher = lm.teacher_top(other, ids, 5, 2.0)
+    assert [m.training for m in other.modules()] == modes and True in modes and False in modes
+    tail = model.distill(ids, top, classes, teacher_lse=lse, temperature=2.0)
+    assert torch.equal(model.distill(ids, *teacher, temperature=2.0), tail)
+    assert not torch.isclose(model.distill(ids, top, classes, temperature=2.0), tail)
+    assert torch.equal(lm.train_step(model, lm.make_optimizer(model), ids, teacher, temperature=2.0), tail)
+    dropping = make(dropout=0.5, **ALL).train()
+    rng = dropping.next_rng()
+    with pytest.raises((TypeError, ValueError)):
+        dropping.distill(ids, top, classes, rng)
+    one, again = (dropping.distill(ids, *teacher, rng=rng) for _ in range(2))
+    assert torch.equal(one, again) and not torch.equal(one, dropping.distill(ids, *teacher))
+
+
 def test_training_steps():
     """train_step with a teacher runs and moves every parameter."""
     model, ids = make(**MORE), ids_of(2, 9)
