@@ -505,6 +505,7 @@ def bench(argv=None):
     ap.add_argument("--attention", default="softmax", choices=["softmax", "differential"])
     ap.add_argument("--teacher-top", type=int, default=0, metavar="K",
                     help="train towards the K highest logits of another random model, found before the steps")
+    ap.add_argument("--teacher-rest", action="store_true", help="the rest of its classes as one event, not those K alone")
     ap.add_argument("--temperature", type=float, default=1.0, help="of the distillation")
     ap.add_argument("--hard-weight", type=float, default=0.0, help="the labels' weight in the distillation")
     a = ap.parse_args(argv)
@@ -522,16 +523,16 @@ def bench(argv=None):
         ids = torch.randint(0, cfg.vocab_size, (a.batch, a.seq), device=dev, generator=gen)
         return _prefill(model, cfg, ids, a)
     print(json.dumps(time_training(a.steps, a.warmup, a.batch, a.seq, a.residual, a.teacher_top, a.temperature, a.hard_weight,
-                                   **options)), flush=True)
+                                   a.teacher_rest, **options)), flush=True)
 
 
 def time_training(steps: int = 10, warmup: int = 3, batch: int = 8, seq: int = 2048,
                   residual: str = "delta_attnres", teacher_k: int = 0, temperature: float = 1.0, hard_weight: float = 0.0,
-                  **options) -> dict:
+                  teacher_rest: bool = False, **options) -> dict:
     """Config 5's training step on cuda:0 -- the random-init LM in bf16, uniform random ids (batch, seq), AdamW --
     timed over `steps` steps after `warmup`; residual "none" is the same model as Plain Loop; teacher_k: the steps
-    distill that many of another random model's highest logits, which it gives before them; options: LMConfig's. Returns the
-    record."""
+    distill that many of another random model's highest logits, which it gives before them, and with teacher_rest the rest of its
+    classes as one event; options: LMConfig's. Returns the record."""
     dev = torch.device("cuda", 0)
     cfg = LMConfig(residual=None if residual == "none" else "delta_attnres", **options)
     torch.manual_seed(0)
@@ -542,7 +543,8 @@ def time_training(steps: int = 10, warmup: int = 3, batch: int = 8, seq: int = 2
     teacher, how = None, {}
     if teacher_k:
         other = LoopbackLM(cfg).to(device=dev, dtype=torch.bfloat16)
-        teacher, how = teacher_top(other, ids, teacher_k, temperature)[:2], {"temperature": temperature, "hard_weight": hard_weight}
+        teacher = teacher_top(other, ids, teacher_k, temperature)[:3 if teacher_rest else 2]
+        how = {"temperature": temperature, "hard_weight": hard_weight}
         del other
     for _ in range(warmup):
         train_step(model, opt, ids, teacher, **how)
@@ -562,7 +564,7 @@ def time_training(steps: int = 10, warmup: int = 3, batch: int = 8, seq: int = 2
            "optimizer": "AdamW (foreach)",
            "config": {"topology": cfg.topology(), **asdict(cfg), "batch": batch, "seq": seq}}
     if teacher_k:
-        rec["distill"] = {"teacher_top": teacher_k, **how}
+        rec["distill"] = {"teacher_top": teacher_k, "teacher_rest": teacher_rest, **how}
     del model, opt, ids
     torch.cuda.empty_cache()
     return rec

@@ -280,3 +280,17 @@ def test_checkpointed_step():
     grads = torch.autograd.grad(loss, params)
     again = checkpoint(lambda: model.distill(ids, *teacher, **HOW), use_reentrant=False)
     assert again == loss and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, params), grads))
+
+
+@pytest.mark.gpu
+def test_the_command_reaches_the_rest():
+    """A timed step towards a teacher's classes alone, and with the rest of them: two losses, each that of the same models' step."""
+    small = dict(SMALL, **ALL)
+    records = [lm.time_training(1, 0, 2, 33, "none", 5, 2.0, 0.25, rest, **small) for rest in (False, True)]
+    torch.manual_seed(0)
+    cfg = lm.LMConfig(residual=None, **small)
+    model, gen = lm.LoopbackLM(cfg).to("cuda", torch.bfloat16), torch.Generator("cuda").manual_seed(1)
+    ids = torch.randint(0, 97, (2, 33), device="cuda", generator=gen)
+    teacher = lm.teacher_top(lm.LoopbackLM(cfg).to("cuda", torch.bfloat16), ids, 5, 2.0)
+    assert [r["loss"] for r in records] == [model.distill(ids, *teacher[:n], **HOW).item() for n in (2, 3)]
+    assert records[0]["loss"] != records[1]["loss"] and [r["distill"]["teacher_rest"] for r in records] == [False, True]
