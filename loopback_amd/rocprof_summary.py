@@ -41,7 +41,8 @@ FAMILIES = [("k_read_fwd", "read_fwd"), ("k_read_online", "read_fwd_online"), ("
             ("k_pad_rows", "ffn_product"),
             ("k_join_fwd", "join_fwd"), ("k_join_bwd", "join_bwd"), ("k_join_sum", "join_bwd"), ("k_dropout", "dropout"),
             # layer norm, differential attention and the distillation loss
-            ("k_diff_bwd", "diff_attn_bwd"), ("k_diff_dlam", "diff_attn_bwd"), ("k_diff", "diff_attn_fwd"),
+            ("k_diff_bwd", "diff_attn_bwd"), ("k_diff_dlam", "diff_attn_bwd"), ("k_diff_kv_sum", "diff_attn_bwd"),
+            ("k_diff", "diff_attn_fwd"),
             ("k_layer_norm_fwd", "layer_norm_fwd"), ("k_layer_norm", "layer_norm_bwd"), ("k_distill_bwd", "distill_loss_bwd"),
             ("k_distill", "distill_loss_fwd")]
 COPY_BYTES = 1 << 30   # bench.py --copy-calibration copies 1 GiB

@@ -169,3 +169,12 @@ def test_every_kernel_has_a_family():
     for name in ("at::native::vectorized_elementwise_kernel<8, CUDAFunctor_add>", "Cijk_Ailk_Bljk_BBS_BH", "attn_fwd",
                  "void at::native::reduce_kernel<512, 1, at::native::MeanOps>"):
         assert RS.family(name) == "torch / runtime"
+
+
+def test_the_attention_backwards_kernels():
+    """Forward and backward of differential attention, and the kernels that sum their parts."""
+    name = "void (anonymous namespace)::{}<unsigned short>((anonymous namespace)::Diff)".format
+    for kernel in ("k_diff_bwd_q", "k_diff_bwd_kv", "k_diff_kv_sum", "k_diff_dlam"):
+        assert RS.family(name(kernel)) == "diff_attn_bwd", kernel
+    for kernel in ("k_diff_fwd", "k_diff_few", "k_diff_join"):
+        assert RS.family(name(kernel)) == "diff_attn_fwd", kernel
