@@ -21,12 +21,12 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "loopback_model.h"
 #include "loopback_read.h"
 #include "device_io.h"
+#include "lds_limit.h"
 
 namespace {
 
@@ -1227,20 +1227,6 @@ Diff diff_of(const lmo_diff_shape* s, const lmo_strides* q, const lmo_strides* k
   return a;
 }
 inline int64_t blocks_of(int64_t t) { return (t + QB - 1) / QB; }
-// the dynamic LDS that a kernel is allowed has to be raised past 64 KiB, once per kernel and device
-template <typename K, K KERNEL> int allow_lds(int bytes) {
-  static std::atomic<uint64_t> done{0};   // a bit per device
-  int dev = 0;
-  if (bytes <= 65536) return 0;
-  int e = (int)hipGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (e || (done.load(std::memory_order_relaxed) & bit)) return e;
-  e = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (!e && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
-  return e;
-}
-#define ALLOW_LDS(BYTES, ...) allow_lds<decltype(&__VA_ARGS__), &__VA_ARGS__>(BYTES)
-
 inline bool few(const lmo_diff_shape* s) { return s->tq * (s->h / s->hk) <= FEW; }
 // Chunks of the keys: enough workgroups for the CUs twice over, chunks of 256 keys at least. Blocks of 64 queries (not `few`: the rows
 // of the kernel of few queries) are split where that makes three chunks at least: 3 x 333 new tokens over 1001 keys, 6 heads, 26.5 us

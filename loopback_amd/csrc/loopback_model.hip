@@ -7,8 +7,11 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "loopback_model.h"
 #include "loopback_read.h"
+#include "lds_limit.h"
 #include "row_io.h"
 
 namespace {
@@ -793,15 +796,20 @@ int lmo_distill_fwd(const void* logits, const void* top, int top_dtype, const vo
   const int pow = !labels || tau == 1.f ? 0 : tau == 2.f ? 2 : tau == 4.f ? 4 : 1;
   for (; a.row0 < rows; a.row0 += MOST_GROUPS) {
     const unsigned grid = (unsigned)(rows - a.row0 < MOST_GROUPS ? rows - a.row0 : MOST_GROUPS);
+    int err = 0;
     LMO_TYPE_SWITCH(dtype, LMO_BOOL_SWITCH(teacher_lse != nullptr, TAIL, LMO_POW_SWITCH(pow, {
-      if (wide_workgroups(rows))
-        hipLaunchKernelGGL((k_distill_fwd<T, 1024, TAIL, POW, false>), dim3(grid), dim3(1024), map, st, a);
-      else if (past_caches(rows, vocab, dtype))
-        hipLaunchKernelGGL((k_distill_fwd<T, WG, TAIL, POW, true>), dim3(grid), dim3(WG), map, st, a);
-      else
-        hipLaunchKernelGGL((k_distill_fwd<T, WG, TAIL, POW, false>), dim3(grid), dim3(WG), map, st, a);
+      const auto run = [&](auto lanes, auto nt) {   // the waves' sums lie beside the map: together they can be past 64 KiB
+        constexpr int LANES = decltype(lanes)::value, BESIDE = LANES / 64 * 4;
+        constexpr bool NT = decltype(nt)::value;
+        const int most = map + BESIDE > 65536 ? LMO_DISTILL_MAX_TAIL / 8 : 0;
+        if (const int err = ALLOW_LDS_BESIDE(BESIDE, most, k_distill_fwd<T, LANES, TAIL, POW, NT>)) return err;
+        hipLaunchKernelGGL((k_distill_fwd<T, LANES, TAIL, POW, NT>), dim3(grid), dim3(LANES), map, st, a);
+        return launched();
+      };
+      if (wide_workgroups(rows)) err = run(std::integral_constant<int, 1024>(), std::false_type());
+      else if (past_caches(rows, vocab, dtype)) err = run(std::integral_constant<int, WG>(), std::true_type());
+      else err = run(std::integral_constant<int, WG>(), std::false_type());
     })))
-    const int err = launched();
     if (err) return err;
   }
   hipLaunchKernelGGL(k_distill_mean, dim3(1), dim3(MEAN_LANES), 0, st, a.terms, rows, tau, hard,

@@ -322,6 +322,17 @@ def test_distill_past_the_caches(dtype, tail, tau, hard):
         assert torch.equal(2 * grad[at], run(at)[1])
 
 
+@pytest.mark.parametrize("rows,vocab", [(3, M.DISTILL_MAX_TAIL - 512), (3, M.DISTILL_MAX_TAIL - 511), (3, M.DISTILL_MAX_TAIL),
+                                        (513, M.DISTILL_MAX_TAIL), (3, M.DISTILL_MAX_TAIL + 1)])
+def test_distill_the_largest_maps(rows, vocab):
+    """The rest of a vocabulary whose map of named classes fills the 64 KiB of LDS that a launch may take unasked, with the waves' sums
+    beside it more than fills it, and one whose map is too large for the kernels."""
+    ids, top, labels = teacher_of(rows, vocab, 9, 5)
+    ids[0, 0], ids[2, 0] = vocab - 1, vocab - 32     # the map's last word
+    x = torch.empty(rows, vocab, dtype=torch.bfloat16, device=DEV).normal_(0.0, 3.0, generator=torch.Generator(DEV).manual_seed(6))
+    check_distill(x, top, ids, lse=lse_of(top, ids, 1.0), labels=labels, hard=0.3)
+
+
 def test_rows_past_32_bits():
     """More than 2^31 elements: the last rows are what they are alone."""
     x = torch.empty(140000, 16384, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(4))
