@@ -867,7 +867,6 @@ PyObject* host_distill(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// torch_forms(dropout, join, ffn): the Python functions that the nodes call where a backward has to be torch operations
 // q [b, tq, 2 h, dh], k [b, tk, 2 hk, dh], v [b, tk, hk, dv] as the kernels take them: themselves, or contiguous copies. A dimension
 // of one may have any stride, which contiguous() keeps and nothing steps by: the kernels get 0 for it
 at::Tensor attn_rows(const at::Tensor& t) {
@@ -1017,6 +1016,7 @@ PyObject* host_diff_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// the Python functions that the nodes call where a backward has to be torch operations, `count` of them from the first's place on
 PyObject* set_forms(PyObject* const* args, Py_ssize_t n, int first, int count, const char* what) {
   bool ok = n == count;
   for (int i = 0; ok && i < count; ++i) ok = PyCallable_Check(args[i]);
@@ -1031,6 +1031,7 @@ PyObject* set_forms(PyObject* const* args, Py_ssize_t n, int first, int count, c
   }
   Py_RETURN_NONE;
 }
+// torch_forms(dropout, join, ffn): the block operators'
 PyObject* host_torch_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return set_forms(args, n, 0, BLOCK_FORMS, "torch_forms(dropout, join, ffn)");
 }

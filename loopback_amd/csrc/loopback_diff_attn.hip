@@ -340,7 +340,7 @@ template <int DH, int DV> constexpr int waves_bwd() { return DH + DV <= 192 ? 2 
 // the values once for both, but hold 256 registers, so two waves to a SIMD, in which the vector units, a wave's softmax, wait
 // for its products and the other way round; so it is three here.) Vector units and matrix cores bound it: per 32 x 32 scores of a
 // map 16 exponentials of 8 cycles and some 80 operations of 4, 490 cycles with what the issue of products costs, and 384 of
-// products; the two overlap little (counters: 0.48 and 0.37 of the time). 8 x 2048 tokens, 6 heads of 64|128 in bf16: 101 us, 77 GFLOP
+// products; the two overlap little (counters: 0.47 and 0.37 of the time). 8 x 2048 tokens, 6 heads of 64|128 in bf16: 101 us, 77 GFLOP
 // done at 0.77 PFLOP/s; 2 x 4096, 16 heads: 235 us, 0.88. A tile's scores formed between the exponentials of the tile before, so
 // that one wave's products and softmax overlap: 107 us. Tiles of 64 keys: 111, eight waves to a workgroup: 218.
 // ---------------------------------------------------------------------------------------------------------------
