@@ -183,12 +183,12 @@ template <template <int> class R, int W, typename O> __device__ __forceinline__ 
 // ONCE: data that no one reads again soon, past the caches
 template <bool ONCE = false> __device__ __forceinline__ void load_lds16(const void* base, uint32_t off, int to) {
   if constexpr (ONCE)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
 }
 __device__ __forceinline__ void load_lds4(const void* base, uint32_t off, int to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "m0", "memory");
 }
 
 // Fills N rows of LDS from memory by LANES lanes (whole waves). MAPS rows of memory of W / MAPS elements (`width` of them
