@@ -695,9 +695,9 @@ template <typename T, int DV, bool SHARED> __global__ __launch_bounds__(WG) void
 // backward: dq, the deltas and dlam's parts. 128 queries of a head per workgroup, both maps in a wave, which share dA. Bound as the
 // forward is, by vector units (0.39 of the time) and matrix cores (0.30) that overlap little, at two waves to a SIMD: 8 x 2048 tokens, 6
 // heads of 64|128: 122 us, 77 GFLOP at 0.63 PFLOP/s; 2 x 4096, 16 heads: 281 us, 0.73. Operands read a step ahead spill: 141.
-// D1 and D2 come from the rounded y and P2 v, where many keys share them; for a workgroup whose queries see at most two tiles, where
-// dA - D is a small part of both, a pass before sums P dA in fp32 (the first block of a causal sequence, short ones: no time). Of a
-// single key's probability the gradient is zero, and exactly that.
+// D1 and D2 come from the rounded y and P2 v, where many keys share them; for the queries that see at most two tiles, where dA - D is a
+// small part of both, a pass over these before sums P dA in fp32 (the first block of a causal sequence, short ones: no time). Of a single
+// key's probability the gradient is zero, and exactly that.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int DH, int DV>
 __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<DH, DV>())))) void k_diff_bwd_q(const Diff a) {
@@ -741,7 +741,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
   const int64_t n = ((int64_t)b * a.h + head) * a.tq + qrow, all = (int64_t)a.b * a.h * a.tq;
   const float ls1 = a.lse[n], ls2 = a.lse[n + all];
   const int seen = seen_by(a, qrow, start, len);
-  const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len);
+  const int most = seen_by(a, min(q0 + QB, a.tq) - 1, start, len), least = seen_by(a, q0, start, len);
   const int wmost = w0 < a.tq ? seen_by(a, min(w0 + 32, a.tq) - 1, start, len) : 0, wleast = seen_by(a, min(w0, a.tq - 1), start, len);
   const Rows32<2 * DH> krows;
   const auto vrows = of_width<Rows32, DV>(krows);
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     vf.fetch(0, len - 1, V0);
   }
   filled();   // in every case: a wait for what was loaded above, left to the loop, would wait there for the tiles too
-  if (most <= 2 * TILE) {   // workgroup-uniform
+  if (least <= 2 * TILE) {   // workgroup-uniform: some of its queries' keys all lie in the first two tiles
     if (ntiles > 1) {
       kf.fetch(TILE, len - 1, K1);
       vf.fetch(TILE, len - 1, V1);
@@ -785,8 +785,9 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     };
     if (0 < wmost) terms(0, K0, V0);
     if (TILE < wmost) terms(TILE, K1, V1);
-    d1 = other_half(e[0], true);
-    d2 = other_half(e[1], true);
+    const float sum1 = other_half(e[0], true), sum2 = other_half(e[1], true);
+    d1 = seen <= 2 * TILE ? sum1 : d1;
+    d2 = seen <= 2 * TILE ? sum2 : d2;
     __syncthreads();   // the second tile, which the loop fetches again, has been read
   }
   if (query < a.tq && half == 0) {   // what the kernel of dk and dv reads: see there

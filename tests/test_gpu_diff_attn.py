@@ -265,6 +265,36 @@ def test_score_gradients_of_short_sequences(t, dtype):
             assert ((got.double() - ref).abs() <= h * (ref.abs() + bound) + bound + FLOOR[dtype] * (1 + other.abs().sum(1, keepdim=True))).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tq,tk,starts", [(128, 129, None), (130, 131, None), (200, 201, None), (200, 280, None), (200, 264, (1, 64)),
+                                          (200, 200, (-3, -150)), (150, 300, (64, 0)), (300, 300, (-100, 2))])
+def test_score_gradients_of_queries_that_see_few_keys(tq, tk, starts, dtype):
+    """As of short sequences, whatever the other queries see: those that see more than 128 keys have no gradient here, so that dk is
+    the few ones' too."""
+    q, k, v, lam = operands(2, tq, tk, 1, 1, 64, 128, dtype)
+    start = torch.full((2,), tk - tq, device=DEV) if starts is None else ints(*starts, dtype=torch.int64)
+    keys = (start.view(2, 1) + torch.arange(tq, device=DEV) + 1).clamp(0, tk)          # that each query sees
+    dy = rnd((2, tq, 1, 128), dtype, 8) * (keys <= 128).view(2, tq, 1, 1)
+    assert (keys.amax() > 128) and ((keys >= 2) & (keys <= 128)).any()
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, lam)]
+    y = M.diff_attention(*leaves, starts=None if starts is None else start)
+    dq, dk = torch.autograd.grad(y, leaves[:2], dy)
+    h, c = HALF[dtype], 64 ** -0.5
+    q, k, v, g, lam = (x.detach().double() for x in (q, k, v, dy, lam))
+    da, size = g[:, :, 0] @ v[:, :, 0].transpose(1, 2), g[:, :, 0].abs() @ v[:, :, 0].abs().transpose(1, 2)
+    hidden = torch.arange(tk, device=DEV) >= keys.unsqueeze(-1)
+    for e, f in ((0, 1.0), (1, -float(lam[0]))):
+        s = q[:, :, e] @ k[:, :, e].transpose(1, 2) * c
+        p = torch.nan_to_num(s.masked_fill(hidden, -math.inf).softmax(-1), nan=0.0)
+        ds = c * f * p * (da - (p * da).sum(-1, keepdim=True))
+        fp32 = 128 * U * c * abs(f) * p * (size + (p * size).sum(-1, keepdim=True))
+        for got, other, left in ((dq[:, :, e], k[:, :, e], ds), (dk[:, :, e], q[:, :, e], ds.transpose(1, 2))):
+            more = fp32 if left is ds else fp32.transpose(1, 2)
+            bound = (h * left.abs() + (1 + h) * more) @ other.abs()
+            ref = left @ other
+            assert ((got.double() - ref).abs() <= h * (ref.abs() + bound) + bound + FLOOR[dtype] * (1 + other.abs().sum(1, keepdim=True))).all()
+
+
 def test_one_tensor_twice():
     """The queries as the keys too, and keys that are the values' storage: the same results and gradients as from copies."""
     q, _, _, lam = operands(2, 100, 100, 2, 2, 64, 128, torch.bfloat16)
