@@ -243,6 +243,9 @@ struct Diff {
   const void* dy;
   void *dq, *dk, *dval;
   float *delta, *dlam;           // four or, where lam has queries, five numbers [b h][tq] for k_diff_bwd_kv; dlam's parts
+  // fp16: the largest |v| of 128 keys [b hk][tk / 128], and |dy| max(1, |lam|) and max(1, |lam|) of 32 queries [b h][tq / 32]
+  float* norms;
+  float2* sizes;
   int lam_rows;                  // lam has queries; dlam is per query, else per workgroup
   // keys in chunks (few queries), or tiles of queries in parts (dk and dv)
   int splits, chunk;
@@ -334,6 +337,56 @@ __device__ __forceinline__ void soft_step(f32x16 (&s)[NB], Soft& st, f32x16 (&o)
 }
 
 template <int DH, int DV> constexpr int waves_bwd() { return DH + DV <= 192 ? 2 : 1; }   // waves to a SIMD, by their registers
+
+// ---------------------------------------------------------------------------------------------------------------
+// The score gradients P (dA - D) enter the matrix cores in 16 bits. fp16 holds 2^-14 to 2^16 in full; from upstreams of 1e-4 dq and dk
+// were 6.3e-3 and 7.2e-3 off for that (2048 tokens; their own rounding 2.0e-3 and 1.4e-3, and now no more), and from some of 1e4 infinite,
+// though both are in range. So the gradients are taken times a power of two that brings their bound, |dA - D| <= 2 |dy| |v|, to 2^LIFT,
+// and the fp32 sums by as much back: each query's own power in dq, whose columns are queries; that of all the queries that a workgroup
+// meets in dk and dv, which sum over them. What is below 2^(-24 - LIFT) of the bound is lost. dv's combined map, whose probabilities of
+// 32768 keys are about 2^-15, is lifted the same way from its bound (4.4e-4 off, now as of 4096 keys). bf16 has fp32's range. The norms of v are a
+// launch before: 8 x 2048 tokens, 6 heads of 128: 6 us of the backward's 300 (25 MB at 4 TB/s), 3 x 683 tokens, 2 of 256: 4.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T> constexpr bool LIFTED = std::is_same<T, _Float16>::value;
+constexpr int LIFT = 13;   // three binades are left for what D's own rounding adds
+__device__ __forceinline__ int lift_of(float bound) { return LIFT - __builtin_amdgcn_frexp_expf(bound); }   // bound < 2^frexp_exp; 0: any
+__device__ __forceinline__ float power_of_2(int n) { return __uint_as_float((unsigned)(127 + n) << 23); }   // within +-126, as a lift is
+__device__ __forceinline__ float finite_or_0(float x) { return x < INFINITY ? x : 0.f; }   // of x >= 0 or NaN
+// the largest |v| of the first n keys of an item, to every lane of a wave
+__device__ __forceinline__ float norm_of(const Diff& a, int item, int n) {
+  const float* of = a.norms + (int64_t)item * ((a.tk + QB - 1) / QB);
+  float most = 0.f;
+  for (int i = (int)threadIdx.x & 63; i * QB < n; i += 64) most = fmaxf(most, of[i]);
+  return lanes_reduce(most, 64, MaxOp());
+}
+// |v|, the largest of QB keys, those that are finite (a result that another one enters is not): DV / 8 lanes to a row
+template <typename T, int DV> __global__ __launch_bounds__(WG) void k_diff_bwd_norms(const Diff a) {
+  constexpr int P = DV / 8, N = QB * P / WG;
+  __shared__ float s_most[WG / 64];
+  const int tid = (int)threadIdx.x, blocks = (a.tk + QB - 1) / QB, item = (int)blockIdx.x / blocks, k0 = ((int)blockIdx.x - item * blocks) * QB;
+  const int b = item / a.hk, hk = item - b * a.hk, end = min(k0 + QB, length_of(a, b)), col = 8 * (tid % P);
+  const T* v = static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h + col;
+  typename IO<T>::Raw x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {   // all in flight at once
+    const int r = k0 + tid / P + i * (WG / P);
+    x[i] = IO<T>::zero();
+    if (r < end && col < a.dv) x[i] = IO<T>::raw(v + r * a.v.t);
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float e[8], sum = 0.f;
+    IO<T>::unpack(x[i], e);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(e[k], e[k], sum);
+    most = fmaxf(most, finite_or_0(lanes_reduce(sum, P, AddOp())));
+  }
+  most = lanes_reduce(most, 64, MaxOp());
+  if ((tid & 63) == 0) s_most[tid >> 6] = most;
+  __syncthreads();
+  if (tid == 0) a.norms[blockIdx.x] = sqrtf(fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3])));
+}
 
 // ---------------------------------------------------------------------------------------------------------------
 // forward: 64 queries of a head per workgroup, two waves for each 32 of them, one for each map. (Both maps in one wave read
@@ -750,6 +803,22 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
 #pragma unroll
   for (int d = 0; d < QB_; ++d) dq[0][d] = dq[1][d] = zero16();
   float dlam = 0.f;
+  int lift = 0;
+  if constexpr (LIFTED<T>) {
+    float sum = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DV / 16; ++ks) {
+      float u[8];
+      IO<T>::unpack(typename IO<T>::Raw{g.f[ks]}, u);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(u[k], u[k], sum);
+    }
+    const float size = finite_or_0(sqrtf(other_half(sum, true)));
+    lift = lift_of(2.f * size * norm_of(a, wk.item, most));
+    const float factor = fmaxf(1.f, finite_or_0(fabsf(lam))), largest = lanes_reduce(query < a.tq ? finite_or_0(size * factor) : 0.f, 64, MaxOp());
+    const float most_lam = lanes_reduce(factor, 64, MaxOp());
+    if (lane == 0) a.sizes[(((int64_t)b * a.h + head) * blocks + qblock) * (QB / 32) + wave] = make_float2(largest, most_lam);
+  }
   const int ntiles = (most + TILE - 1) / TILE;
   const Fill<T, 2 * DH, 2, TILE, WG> kf(static_cast<const T*>(a.k.p) + b * a.k.b + 2 * hk * a.k.h, a.k.t, a.k.h, a.dh);
   const Fill<T, DV, 1, TILE, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
@@ -798,6 +867,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     a.delta[n + 3 * all] = seen == 1 ? 0.f : sign * (d2 - d1);
     if (a.lam_rows) a.delta[n + 4 * all] = -sign;
   }
+  const float up = power_of_2(lift), d1up = d1 * up, d2up = d2 * up;
   auto tile = [&](int j, auto buffer) {
     constexpr int cur = decltype(buffer)::value;   // known: the buffers' offsets go into the reads' own
     const int k0 = j * TILE;
@@ -825,12 +895,12 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
             for (int r = 0; r < 16; ++r)
               if (32 * i + row_of(r, 0) >= left) s[r] = -INFINITY;
           }
-          const float ls = map ? ls2 : ls1, d = map ? d2 : d1;
+          const float ls = map ? ls2 : ls1, d = map ? d2 : d1, dup = map ? d2up : d1up;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -ls));
             if (map) dlam = __builtin_fmaf(p, da[r], dlam);
-            s[r] = p * (da[r] - d);
+            s[r] = p * (LIFTED<T> ? __builtin_fmaf(da[r], up, -dup) : da[r] - d);
           }
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
@@ -853,7 +923,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     T* row = static_cast<T*>(a.dq) + (((int64_t)b * a.tq + query) * 2 * a.h + 2 * head) * a.dh;
 #pragma unroll
     for (int map = 0; map < 2; ++map) {
-      const float f = seen == 1 ? 0.f : map ? -lam * a.scale : a.scale;
+      const float back = LIFTED<T> ? a.scale * power_of_2(-lift) : a.scale, f = seen == 1 ? 0.f : map ? -lam * back : back;
 #pragma unroll
       for (int e = 0; e < QB_; ++e)
 #pragma unroll
@@ -997,6 +1067,23 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(lam < 0.f ? 1.f : -1.f)));
   };
   float next_minus = minus_of(head);
+  float up = 1.f, back = 1.f, up_p = 1.f, back_p = 1.f;   // what dA - D and the combined map are multiplied by, and the results by as much back
+  if constexpr (LIFTED<T>) {
+    float size = 0.f, lam = 1.f;
+    const int tiles = (a.tq + QB - 1) / QB * (QB / KVT);
+    for (int it = it0 + lane; it < it1; it += 64) {
+      const int of = it / kv.n;
+      const float2 e = a.sizes[((int64_t)b * a.h + hk * groups + of) * tiles + kv.first + it - of * kv.n];
+      size = fmaxf(size, e.x);
+      lam = fmaxf(lam, e.y);
+    }
+    const int n = __builtin_amdgcn_readfirstlane(lift_of(2.f * lanes_reduce(size, 64, MaxOp()) * norm_of(a, wk.item, len)));
+    const int n_p = __builtin_amdgcn_readfirstlane(lift_of(2.f * lanes_reduce(lam, 64, MaxOp())));   // |P1 - lam P2| <= 2 max(1, |lam|)
+    up = power_of_2(n);
+    back = power_of_2(-n);
+    up_p = power_of_2(n_p);
+    back_p = power_of_2(-n_p);
+  }
   if (it0 < it1) {
     const Fill<T, DV, 1, QB, WG> vf(static_cast<const T*>(a.v.p) + b * a.v.b + hk * a.v.h, a.v.t, 0, a.dv);
     vf.fetch(kb, len - 1, VALUES);
@@ -1078,17 +1165,18 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
           }
         f32x4 sg;
         if (TOKEN) sg = number(NUMBERS - 1);
-        const f32x4 d = number(3);
+        f32x4 d = number(3);
+        if (LIFTED<T>) d *= up;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float q1 = s1[n][r], q2 = s2[n][r], x = da[u][n][r], m = TOKEN ? sg[r] : minus;
+            const float q1 = s1[n][r], q2 = s2[n][r], x = LIFTED<T> ? da[u][n][r] * up : da[u][n][r], m = TOKEN ? sg[r] : minus;
             da[u][n][r] = __builtin_fmaf(m, q2, q1);
             s1[n][r] = q1 * x;
             s2[n][r] = q2 * __builtin_fmaf(m, x, d[r]);
           }
-          pd[u][n] = packed4<T>(da[u][n]);
+          pd[u][n] = packed4<T>(LIFTED<T> ? da[u][n] * up_p : da[u][n]);
           p1[u][n] = packed4<T>(s1[n]);
           p2[u][n] = packed4<T>(s2[n]);
         }
@@ -1127,31 +1215,32 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
       for (int d = 0; d < KB; ++d) {
         const int col = 16 * d + 4 * grp;
         if (col < a.dh) {
-          *reinterpret_cast<f32x4*>(row + col) = dk[0][d][n];
-          *reinterpret_cast<f32x4*>(row + a.dh + col) = dk[1][d][n];
+          *reinterpret_cast<f32x4*>(row + col) = LIFTED<T> ? dk[0][d][n] * back : dk[0][d][n];
+          *reinterpret_cast<f32x4*>(row + a.dh + col) = LIFTED<T> ? dk[1][d][n] * back : dk[1][d][n];
         }
       }
 #pragma unroll
       for (int d = 0; d < VB; ++d) {
         const int col = 16 * d + 4 * grp;
-        if (col < a.dv) *reinterpret_cast<f32x4*>(row + 2 * a.dh + col) = dv[d][n];
+        if (col < a.dv) *reinterpret_cast<f32x4*>(row + 2 * a.dh + col) = LIFTED<T> ? dv[d][n] * back_p : dv[d][n];
       }
       continue;
     }
+    const float scale = LIFTED<T> ? a.scale * back : a.scale;
     T* krow = static_cast<T*>(a.dk) + (((int64_t)b * a.tk + key) * 2 * a.hk + 2 * hk) * a.dh;
     T* vrow = static_cast<T*>(a.dval) + (((int64_t)b * a.tk + key) * a.hk + hk) * a.dv;
 #pragma unroll
     for (int d = 0; d < KB; ++d) {
       const int col = 16 * d + 4 * grp;
       if (col < a.dh) {
-        *reinterpret_cast<uint2*>(krow + col) = packed4<T>(dk[0][d][n] * a.scale);
-        *reinterpret_cast<uint2*>(krow + a.dh + col) = packed4<T>(dk[1][d][n] * a.scale);
+        *reinterpret_cast<uint2*>(krow + col) = packed4<T>(dk[0][d][n] * scale);
+        *reinterpret_cast<uint2*>(krow + a.dh + col) = packed4<T>(dk[1][d][n] * scale);
       }
     }
 #pragma unroll
     for (int d = 0; d < VB; ++d) {
       const int col = 16 * d + 4 * grp;
-      if (col < a.dv) *reinterpret_cast<uint2*>(vrow + col) = packed4<T>(dv[d][n]);
+      if (col < a.dv) *reinterpret_cast<uint2*>(vrow + col) = packed4<T>(LIFTED<T> ? dv[d][n] * back_p : dv[d][n]);
     }
   }
 }
@@ -1258,6 +1347,18 @@ inline Parts kv_parts(const lmo_diff_shape* s) {
   const int64_t splits = (most + limit - 1) / limit;
   return {splits < 1 ? 1 : splits > 16 ? 16 : splits, limit};
 }
+// the backward's scratch memory, in floats from its start
+struct BwdScratch { int64_t dlam, norms, sizes, part, all; };
+inline BwdScratch bwd_scratch(const lmo_diff_shape* s, int lam_kind, const Parts& kv) {
+  const bool token = lam_kind == LMO_LAM_TOKEN;
+  BwdScratch at;
+  at.dlam = (token ? 5 : 4) * s->b * s->h * s->tq;
+  at.norms = at.dlam + s->b * s->h * (token ? s->tq : blocks_of(s->tq));
+  at.sizes = (at.norms + s->b * s->hk * blocks_of(s->tk) + 3) / 4 * 4;
+  at.part = at.sizes + s->b * s->h * blocks_of(s->tq) * (QB / KVT) * 2;   // 8 floats a block of queries
+  at.all = at.part + (kv.splits > 1 ? s->b * s->hk * blocks_of(s->tk) * kv.splits * QB * (2 * s->dh + s->dv) : 0);
+  return at;
+}
 inline int padded_dv(const lmo_diff_shape* s) { return s->dv <= 64 && s->dh <= 64 ? 64 : s->dv <= 128 ? 128 : 256; }
 
 }  // namespace
@@ -1318,10 +1419,7 @@ int lmo_diff_attn_fwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
 
 int64_t lmo_diff_attn_bwd_scratch(const lmo_diff_shape* s, int lam_kind) {
   if (!s || s->b < 1 || s->tq < 1 || s->tk < 1 || s->hk < 1 || s->h < s->hk) return 0;
-  const int64_t numbers = lam_kind == LMO_LAM_TOKEN ? 5 : 4, parts = lam_kind == LMO_LAM_TOKEN ? s->b * s->tq * s->h : s->h * s->b * blocks_of(s->tq);
-  const Parts kv = kv_parts(s);
-  return (numbers * s->b * s->h * s->tq + parts + 3) / 4 * 4 +
-         (kv.splits > 1 ? s->b * s->hk * blocks_of(s->tk) * kv.splits * QB * (2 * s->dh + s->dv) : 0);
+  return bwd_scratch(s, lam_kind, kv_parts(s)).all;
 }
 
 int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_strides* v, const lmo_strides* lam, int lam32,
@@ -1346,16 +1444,22 @@ int lmo_diff_attn_bwd(const lmo_strides* q, const lmo_strides* k, const lmo_stri
   a.dval = dv;
   a.delta = scratch;
   const Parts kv = kv_parts(s);
-  const int64_t numbers = (lam_kind == LMO_LAM_TOKEN ? 5 : 4) * s->b * s->h * s->tq;
-  a.dlam = dlam ? scratch + numbers : nullptr;
+  const BwdScratch at = bwd_scratch(s, lam_kind, kv);
+  a.dlam = dlam ? scratch + at.dlam : nullptr;
+  a.norms = scratch + at.norms;
+  a.sizes = reinterpret_cast<float2*>(scratch + at.sizes);
   a.splits = (int)kv.splits;
   a.chunk = (int)kv.limit;
-  a.part = scratch + (numbers + (lam_kind == LMO_LAM_TOKEN ? s->b * s->tq * s->h : s->h * s->b * blocks_of(s->tq)) + 3) / 4 * 4;
+  a.part = scratch + at.part;
   a.lam_rows = lam_kind == LMO_LAM_TOKEN;
   const int64_t qblocks = blocks_of(s->tq), grid_q = s->b * s->h * qblocks, grid_k = s->b * s->hk * blocks_of(s->tk) * kv.splits;
   if (grid_q > 0x7fffffff || grid_k > 0x7fffffff) return LDR_E_SHAPE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   DIFF_SWITCH(dtype, s->dh, s->dv, {
+    if constexpr (LIFTED<T>) {
+      hipLaunchKernelGGL((k_diff_bwd_norms<T, DV>), dim3((unsigned)(grid_k / kv.splits)), dim3(WG), 0, st, a);
+      if ((e = launched())) return e;
+    }
     constexpr int bytes = 2 * TILE * (2 * DH + DV) * 2;
     if ((e = ALLOW_LDS(bytes, k_diff_bwd_q<T, DH, DV>))) return e;
     hipLaunchKernelGGL((k_diff_bwd_q<T, DH, DV>), dim3((unsigned)grid_q), dim3(WG), bytes, st, a);

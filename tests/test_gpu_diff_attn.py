@@ -295,6 +295,93 @@ def test_score_gradients_of_queries_that_see_few_keys(tq, tk, starts, dtype):
             assert ((got.double() - ref).abs() <= h * (ref.abs() + bound) + bound + FLOOR[dtype] * (1 + other.abs().sum(1, keepdim=True))).all()
 
 
+def powers(shape, seed):
+    """+-1, 2 or 4: a power of two times them is exact in fp16 down to its smallest number, 2^-24."""
+    g = torch.Generator().manual_seed(seed)
+    return (torch.exp2(torch.randint(0, 3, shape, generator=g).float()) * (torch.randint(0, 2, shape, generator=g) * 2 - 1)).to(DEV)
+
+
+def gradients(ts, dy, **how):
+    leaves = [t.detach().requires_grad_() for t in ts]
+    return torch.autograd.grad(M.diff_attention(*leaves, **how), leaves, dy)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lam", ["head", "token"])
+@pytest.mark.parametrize("t,h,hk,dh,dv", [(1, 1, 1, 64, 128), (100, 2, 1, 64, 128), (300, 2, 2, 64, 128), (700, 4, 1, 40, 80), (300, 2, 1, 128, 256)])
+def test_gradients_of_small_and_large_upstreams(t, h, hk, dh, dv, lam, dtype):
+    """Gradients are linear: those of 2^k dy are 2^k times those of dy, each rounded once, from upstreams of 2^-24 to some with which
+    a score gradient before its scale is past 65504. Nothing between the two roundings depends on 2^k: an intermediate in the type
+    would, below its smallest normal number and past its largest."""
+    ts = operands(2, t, t, h, hk, dh, dv, dtype, lam)
+    ts[1], ts[2] = ts[1] * 0.25, ts[2] * 0.5      # the largest results are of some thousands
+    lengths = ints(t, (t + 1) // 2)
+    dy = powers((2, t, h, dv), 5)
+    one = gradients(ts, dy.to(dtype), lengths=lengths)
+    half, tiny = HALF[dtype], 2.0 ** -25 if dtype is torch.float16 else 2.0 ** -126
+    for k in (-24, -17, -10, 9, 12):
+        for name, got, ref in zip(("dq", "dk", "dv", "dlam"), gradients(ts, (dy * 2.0 ** k).to(dtype), lengths=lengths), one):
+            ref = ref.double() * 2.0 ** k
+            if dtype is torch.float16 and ref.abs().max() > 60000:
+                assert name in ("dv", "dlam") and k > 0   # past the range
+                continue
+            off = ((got.double() - ref).abs() - (2.1 * half * ref.abs() + tiny * (1 + 2.0 ** k))).max().item()
+            assert off <= 0, (name, k, off, ref.abs().max().item())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dh,dv", [(64, 128), (128, 256)])
+def test_gradients_of_queries_of_different_sizes(dh, dv, dtype):
+    """A query's own gradient is as near beside queries whose upstreams are 2^20 times as large; and of the keys that see only small
+    ones, those of the last block."""
+    t, half, tiny = 400, HALF[dtype], 2.0 ** -25 if dtype is torch.float16 else 2.0 ** -126
+    ts = operands(2, t, t, 2, 1, dh, dv, dtype, "token")
+    ts[1], ts[2] = ts[1] * 0.25, ts[2] * 0.5
+    dy, k = powers((2, t, 2, dv), 5), torch.full((2, t, 1, 1), -11.0, device=DEV)
+    k[:, 100:120], k[:, 7], k[:, 150] = 9.0, -24.0, -20.0
+    one, got = (gradients(ts, (dy * f).to(dtype)) for f in (1.0, torch.exp2(k)))
+    ref = one[0].double() * torch.exp2(k).double()
+    off = ((got[0].double() - ref).abs() - (2.1 * half * ref.abs() + tiny * (1 + torch.exp2(k).double()))).max().item()
+    assert off <= 0
+    for a, b in zip(got[1:3], one[1:3]):
+        a, b = a[:, 384:].double(), b[:, 384:].double() * 2.0 ** -11
+        off = ((a - b).abs() - (2.1 * half * b.abs() + tiny)).max().item()
+        assert off <= 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_lambdas_and_infinite_upstreams(dtype):
+    """Lambdas of hundreds and thousands; a query whose upstream is infinite leaves the others' gradients as they are without it."""
+    ts = operands(2, 150, 150, 2, 1, 64, 128, dtype)
+    for lam in (torch.tensor([300.0, -3000.0], device=DEV), torch.tensor([0.001, 2000.0], device=DEV).expand(2, 150, 2)):
+        check([*ts[:3], lam])
+    dy = rnd((2, 150, 2, 128), dtype, 9)
+    dy[:, 70, 1] = 0.0
+    ref = gradients(ts, dy)[0]
+    dy[:, 70, 1, 5] = math.inf
+    got = gradients(ts, dy)[0]
+    assert not got[:, 70, 2:].isfinite().any()
+    got[:, 70, 2:] = 0.0
+    assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("dtype,bound", [(torch.bfloat16, 0.75 * 2.0 ** -8), (torch.float16, 0.75 * 2.0 ** -11)])
+def test_values_gradient_of_many_keys(dtype, bound):
+    """32768 keys whose probabilities are about 2^-15: dv is a sum over the queries of P dy, whose factors' roundings are independent, of
+    half a step at most and 0.41 of it in the norm (over a binade: 1 / 3 of its square by 7 / 3 or less), and so is its own rounding:
+    together sqrt(2) 0.41 = 0.58 of half a step, here below 0.75."""
+    t = 32768
+    q, k, v, lam = operands(1, t, t, 1, 1, 64, 128, dtype, "layer")
+    dy = rnd((1, t, 1, 128), dtype, 9)
+    got = gradients([q, k, v, lam], dy, causal=False)[2][0, :, 0].double()
+    ref = torch.zeros_like(got)
+    for at in range(0, t, 4096):   # blocks of queries
+        p = [torch.softmax(q[0, at:at + 4096, m].double() @ k[0, :, m].double().T.contiguous() / 8, -1) for m in (0, 1)]
+        ref += (p[0] - lam.double() * p[1]).T.contiguous() @ dy[0, at:at + 4096, 0].double()
+    off = ((got - ref).norm() / ref.norm()).item()
+    assert off <= bound, off
+
+
 def test_one_tensor_twice():
     """The queries as the keys too, and keys that are the values' storage: the same results and gradients as from copies."""
     q, _, _, lam = operands(2, 100, 100, 2, 2, 64, 128, torch.bfloat16)
