@@ -142,9 +142,11 @@ __global__ __launch_bounds__(lanes_of(LPR)) void k_layer_norm_bwd(const NormBwd<
       IO<T>::unpack(yr[v], t[v]);
       IO<T>::unpack(hr[v], hat[v]);
       if (a.w) IO<T>::unpack(wr[v], w);
+      const int left = d - 8 * (lane + LPR * v);
+      const float rstd = left > 0 ? st.y : 0.f;   // past the row's end: -m r can be infinite, and is multiplied by a zero
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float g = t[v][k], x = (hat[v][k] - st.x) * st.y;
+        const float g = t[v][k], x = AL || k < left ? (hat[v][k] - st.x) * rstd : 0.f;
         hat[v][k] = x;
         if (there) {
           dw[v][k] = __builtin_fmaf(g, x, dw[v][k]);

@@ -322,6 +322,24 @@ def test_distill_past_the_caches(dtype, tail, tau, hard):
         assert torch.equal(2 * grad[at], run(at)[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,m,shift", [(8, 2.0 ** 121, 0), (8, 2.0 ** 121, 1), (4, 2.0 ** 122, 0), (256, 2.0 ** 116, 0), (2048, 2.0 ** 115, 0)])
+def test_norm_of_large_equal_values(d, m, shift, dtype):
+    """Rows of one large value: they lie at their mean exactly, so y is the bias and dx is r (t - mean(t)), r eps^-1/2. What a lane past the
+    row's end would form of the mean, 316 times it, is infinite."""
+    x = torch.full((5, d), m, dtype=dtype, device=DEV)
+    x = (unaligned(x) if shift else x).requires_grad_()
+    w, b = (rnd((d,), dtype, i, 0.3, 1.0).requires_grad_() for i in (1, 2))
+    y = M.layer_norm(x, w, b)
+    dy = rnd((5, d), dtype, 3)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    t = dy.double() * w.detach().double()
+    r = 1e-5 ** -0.5
+    assert torch.equal(y.detach(), b.detach().expand(5, d)) and not dw.any()
+    close(dx, r * (t - t.mean(-1, keepdim=True)), 32 * U * r * (t.abs() + t.abs().mean(-1, keepdim=True)), "dx")
+    close(db, dy.double().sum(0), 8 * U * dy.double().abs().sum(0), "db")
+
+
 @pytest.mark.parametrize("rows,vocab", [(3, M.DISTILL_MAX_TAIL - 512), (3, M.DISTILL_MAX_TAIL - 511), (3, M.DISTILL_MAX_TAIL),
                                         (513, M.DISTILL_MAX_TAIL), (3, M.DISTILL_MAX_TAIL + 1)])
 def test_distill_the_largest_maps(rows, vocab):
