@@ -15,6 +15,7 @@ Saved tensors that a hook gives back with another shape, type or device are refu
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -190,7 +191,20 @@ def _lam_of(lam, b, tq, hk, group):
     return lam.expand(b, tq, hk * group).reshape(b, tq, hk, group).permute(0, 2, 3, 1).unsqueeze(-1)
 
 
+def _own_types(t):
+    """Products of the types that they are given, where autocast would take 16 bits for them: scores keep 32, and no backward forms a
+    16-bit batched product of a transposed operand."""
+    kind = t.device.type
+    on = kind in ("cuda", "cpu") and torch.is_autocast_enabled(kind)
+    return torch.autocast(kind, enabled=False) if on else contextlib.nullcontext()
+
+
 def _diff_torch(q, k, v, lam, causal, scale, lengths, starts):
+    with _own_types(q):
+        return _diff_formula(q, k, v, lam, causal, scale, lengths, starts)
+
+
+def _diff_formula(q, k, v, lam, causal, scale, lengths, starts):
     dt, (b, tq), hk, group = q.dtype, q.shape[:2], v.shape[2], q.shape[2] // (2 * v.shape[2])
     k, v = _held(_upcast(k), lengths), _held(_upcast(v), lengths)
     p = _maps(_upcast(q), k, causal, scale, lengths, starts)
@@ -202,6 +216,11 @@ def _diff_torch(q, k, v, lam, causal, scale, lengths, starts):
 def _diff_backward(dy, q, k, v, lam, lengths, starts, causal, need, scale):
     """The torch form of differential attention's backward, for the node (csrc/host.cpp), by its formulas: the gradients of q, k, v
     and lam that need's bits ask for."""
+    with _own_types(q):
+        return _diff_gradients(dy, q, k, v, lam, lengths, starts, causal, need, scale)
+
+
+def _diff_gradients(dy, q, k, v, lam, lengths, starts, causal, need, scale):
     dt, (b, tq, h2, dh), (tk, hk, dv) = q.dtype, q.shape, v.shape[1:]
     group = h2 // (2 * hk)
     qu, ku, vu = _upcast(q), _held(_upcast(k), lengths), _held(_upcast(v), lengths)

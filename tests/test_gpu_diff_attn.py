@@ -580,3 +580,17 @@ def test_empty():
         assert y.shape == (b, tq, 2, 128) and not y.any()
         y.sum().backward()
         assert all(t.grad is not None and not t.grad.any() for t in ts)
+
+
+def test_autocast_changes_nothing():
+    """Torch operations in 32 bits, and their backward: no 16-bit products of what autocast would cast."""
+    ts = operands(2, 40, 40, 4, 2, 64, 128, torch.bfloat16)
+    dy = rnd((2, 40, 4, 128), torch.bfloat16, 9)
+    leaves = [t.requires_grad_() for t in ts]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = M.diff_attention(*leaves)
+    got = torch.autograd.grad(y, leaves, dy)
+    ref = reference(*[t.detach() for t in ts], dy)
+    close(y.detach(), *ref["y"], "y")
+    for name, g in zip(("dq", "dk", "dv", "dlam"), got):
+        close(g, *ref[name], name)

@@ -300,3 +300,26 @@ def test_attention_backward_refuses_wide_rows():
     for h in (2 ** 18 + 1, 2 ** 19):
         assert M.LIB.lmo_diff_attn_bwd(ref(s), ref(s), ref(s), ref(s), 1, None, None, p, p, p, p, p, p, p, p, 0, p,
                                        ref(Shape(1, 20, 20, h, 1, 8, 256, 1, 0.125)), 1, None) == -2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_autocast_changes_nothing(dtype):
+    """The operators compute in 32 bits and keep their input's type under autocast, whose products would be of 16."""
+    x, w, b = (rnd(*s, seed=i, dtype=dtype).requires_grad_() for i, s in enumerate(((3, 12), (12,), (12,))))
+    top, ids = rnd(3, 4, seed=5, dtype=dtype), torch.tensor([[0, 3, 7, 9]] * 3)
+    q, k, v, lam = (t.to(dtype).requires_grad_() for t in attn(dh=8))
+    calls = [(lambda: M.add_layer_norm(x, x * 0.5, w, b)[1], (x, w, b)), (lambda: M.diff_attention(q, k, v, lam), (q, k, v, lam)),
+             (lambda: M.distill_loss(x, top, ids, teacher_lse=torch.logsumexp(top.float(), -1) + 0.2, temperature=2.0), (x,))]
+    for call, leaves in calls:
+        want = call()
+        with torch.autocast("cpu", dtype=torch.bfloat16):
+            got = call()
+        assert got.dtype is want.dtype and torch.equal(got, want)
+        for a, r in zip(torch.autograd.grad(got.sum(), leaves), torch.autograd.grad(want.sum(), leaves)):
+            assert torch.equal(a, r)
+    dy = rnd(2, 5, 4, 6, seed=9, dtype=dtype)
+    leaves = [t.detach() for t in (q, k, v, lam)]
+    want = M._diff_backward(dy, *leaves, None, None, 1, 15, 8 ** -0.5)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = M._diff_backward(dy, *leaves, None, None, 1, 15, 8 ** -0.5)
+    assert all(torch.equal(a, r) for a, r in zip(got, want))
