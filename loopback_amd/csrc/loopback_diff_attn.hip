@@ -336,6 +336,24 @@ __device__ __forceinline__ void soft_step(f32x16 (&s)[NB], Soft& st, f32x16 (&o)
   }
 }
 
+// what the 16 bits of a tile's probabilities leave of them, s as soft_step left it: the products' second part, where their rounding is
+// not to be added to the result's
+template <typename T> __device__ __forceinline__ void rest_of(const f32x16& s, const uint4 (&p)[2], uint4 (&rest)[2]) {
+  typedef typename Mat<T>::Cvt C;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w[4] = {p[i].x, p[i].y, p[i].z, p[i].w};
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float u, v;
+      C::unpack2(w[k], u, v);
+      x[k] = C::pack2(s[8 * i + 2 * k] - u, s[8 * i + 2 * k + 1] - v);
+    }
+    rest[i] = make_uint4(x[0], x[1], x[2], x[3]);
+  }
+}
+
 template <int DH, int DV> constexpr int waves_bwd() { return DH + DV <= 192 ? 2 : 1; }   // waves to a SIMD, by their registers
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -396,6 +414,9 @@ template <typename T, int DV> __global__ __launch_bounds__(WG) void k_diff_bwd_n
 // products; the two overlap little (counters: 0.47 and 0.37 of the time). 8 x 2048 tokens, 6 heads of 64|128 in bf16: 101 us, 77 GFLOP
 // done at 0.77 PFLOP/s; 2 x 4096, 16 heads: 235 us, 0.88. A tile's scores formed between the exponentials of the tile before, so
 // that one wave's products and softmax overlap: 107 us. Tiles of 64 keys: 111, eight waves to a workgroup: 218.
+// The probabilities enter the products rounded to the type, which is added to the results' own rounding (1.4 to 1.5 of it in the norm):
+// as two parts, 125 us for 92 without gradients. SPLIT, few blocks of queries over long keys, takes the two parts: there they cost 20.3 ->
+// 22.7 us (3 x 333 new tokens over 1001 keys) to 75 -> 100 (500 over 16384), and the results are rounded once.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int FW = 4, FQ = 16 * FW, FT = 32, FL = 64 * FW;   // waves and queries of a workgroup, keys of a tile, lanes
 template <int DH, int DV> constexpr int waves_fwd() { return DH <= 64 && DV <= 128 ? 3 : 2; }
@@ -467,16 +488,21 @@ __global__ __launch_bounds__(FL) __attribute__((amdgpu_waves_per_eu((waves_fwd<D
         for (int r = 0; r < 16; ++r)
           if (row_of(r, 0) >= left) s[0][r] = -INFINITY;
       }
-      uint4 p[2];
+      uint4 p[2], rest[2];
       soft_step<T>(s, sm, o, p, a.c);
+      if (SPLIT) rest_of<T>(s[0], p, rest);
+      auto product = [&](int i, int d, const uint4& v) {
+        o[d] = Mat<T>::mfma(v, p[i], o[d]);
+        if (SPLIT) o[d] = Mat<T>::mfma(v, rest[i], o[d]);
+      };
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        o[d] = Mat<T>::mfma(AHEAD ? v[d] : vcols.at(vt, 32 * n, 32 * d), p[0], o[d]);
+        product(0, d, AHEAD ? v[d] : vcols.at(vt, 32 * n, 32 * d));
         if (AHEAD) v[d] = vcols.at(vt, 32 * n + 16, 32 * d);
       }
       if (AHEAD) in_order();
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] = Mat<T>::mfma(AHEAD ? v[d] : vcols.at(vt, 32 * n + 16, 32 * d), p[1], o[d]);
+      for (int d = 0; d < DB; ++d) product(1, d, AHEAD ? v[d] : vcols.at(vt, 32 * n + 16, 32 * d));
     }
     if (j + 1 < ntiles) filled();
   };
@@ -593,19 +619,8 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu(2))) void k_
           if (row_of(r, 0) >= left) s[0][r] = -INFINITY;
       }
       uint4 p[2], rest[2];
-      soft_step<T>(s, sm, o, p, a.c);   // s: the probabilities before their rounding
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t w[4] = {p[i].x, p[i].y, p[i].z, p[i].w};
-        uint32_t x[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float u, v;
-          C::unpack2(w[k], u, v);
-          x[k] = C::pack2(s[0][8 * i + 2 * k] - u, s[0][8 * i + 2 * k + 1] - v);
-        }
-        rest[i] = make_uint4(x[0], x[1], x[2], x[3]);
-      }
+      soft_step<T>(s, sm, o, p, a.c);
+      rest_of<T>(s[0], p, rest);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1320,7 +1335,7 @@ inline int64_t blocks_of(int64_t t) { return (t + QB - 1) / QB; }
 inline bool few(const lmo_diff_shape* s) { return s->tq * (s->h / s->hk) <= FEW; }
 // Chunks of the keys: enough workgroups for the CUs twice over, chunks of 256 keys at least. Blocks of 64 queries (not `few`: the rows
 // of the kernel of few queries) are split where that makes three chunks at least: 3 x 333 new tokens over 1001 keys, 6 heads, 26.5 us
-// whole and 15.7 + 5.0 for the join in three; 3 x 683 tokens, 4 heads of 128|256, 33.2 whole and 23.2 + 9.7 in two.
+// whole and 19.4 + 4.8 for the join in three; 3 x 683 tokens, 4 heads of 128|256, 33.2 whole and 23.2 + 9.7 in two (in one part).
 struct Chunks { int64_t splits, chunk; };
 inline Chunks chunks_of(const lmo_diff_shape* s, bool few) {
   const int64_t items = few ? s->b * s->hk : s->b * s->h * ((s->tq + FQ - 1) / FQ), most = s->tk / 256;

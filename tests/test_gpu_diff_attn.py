@@ -594,3 +594,15 @@ def test_autocast_changes_nothing():
     close(y.detach(), *ref["y"], "y")
     for name, g in zip(("dq", "dk", "dv", "dlam"), got):
         close(g, *ref[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,tq,tk,h,hk,dh,dv", [(3, 333, 1001, 6, 3, 40, 80), (1, 333, 2049, 4, 2, 64, 128), (1, 200, 4000, 2, 1, 128, 256),
+                                                (32, 1, 1500, 4, 4, 64, 128), (2, 8, 5000, 8, 2, 64, 64)])
+def test_results_over_a_cache_are_rounded_once(b, tq, tk, h, hk, dh, dv, dtype):
+    """Chunks of new tokens and single ones: their probabilities enter the products in two parts of 16 bits, 2^-16 (bf16) and 2^-22 of
+    them left, so the error is the result's own rounding in the norm; a single part's would make it 1.4 to 1.5 of that."""
+    ts = operands(b, tq, tk, h, hk, dh, dv, dtype, "token")
+    ref = M.diff_attention(*(t.double() for t in ts))
+    norm = lambda t: (t.double() - ref).norm().item()  # noqa: E731
+    assert norm(M.diff_attention(*ts)) <= 1.1 * norm(ref.to(dtype))
