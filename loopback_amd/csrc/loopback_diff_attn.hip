@@ -3,8 +3,8 @@
 //   y = (P1 - lam P2) v,   Pi = softmax(c qi ki^T) over the keys that a query sees
 //
 // Both maps of a head go through one pass over its keys, each with its own running maximum and sum (fp32 scores, statistics
-// and accumulators; the probabilities and score gradients enter the matrix cores in 16 bits). The difference is taken of the
-// two fp32 results. Backward, with D1 = dy . (P1 v), D2 = dy . (P2 v) and dA = dy v^T, which both maps share:
+// and accumulators; the probabilities and score gradients enter the matrix cores in 16 bits, the probabilities of few queries and
+// of chunks in two parts of 16). The difference is taken of the two fp32 results. Backward, with D1 = dy . (P1 v), D2 = dy . (P2 v) and dA = dy v^T, which both maps share:
 //
 //   dS1 = P1 (dA - D1),  dS2 = -lam P2 (dA - D2),  dqi = c dSi ki,  dki = c dSi^T qi,  dv = (P1 - lam P2)^T dy,
 //   dlam = -sum over the keys of P2 dA (from the fp32 values: D2 has the rounding of the saved P2 v)
