@@ -4,7 +4,8 @@
 //
 // Both maps of a head go through one pass over its keys, each with its own running maximum and sum (fp32 scores, statistics
 // and accumulators; the probabilities and score gradients enter the matrix cores in 16 bits, the probabilities of few queries and
-// of chunks in two parts of 16). The difference is taken of the two fp32 results. Backward, with D1 = dy . (P1 v), D2 = dy . (P2 v) and dA = dy v^T, which both maps share:
+// of chunks in two parts of 16). The difference is taken of the two fp32 results. Backward, with D1 = dy . (P1 v), D2 = dy . (P2 v)
+// and dA = dy v^T, which both maps share:
 //
 //   dS1 = P1 (dA - D1),  dS2 = -lam P2 (dA - D2),  dqi = c dSi ki,  dki = c dSi^T qi,  dv = (P1 - lam P2)^T dy,
 //   dlam = -sum over the keys of P2 dA (from the fp32 values: D2 has the rounding of the saved P2 v)
@@ -362,8 +363,8 @@ template <int DH, int DV> constexpr int waves_bwd() { return DH + DV <= 192 ? 2 
 // though both are in range. So the gradients are taken times a power of two that brings their bound, |dA - D| <= 2 |dy| |v|, to 2^LIFT,
 // and the fp32 sums by as much back: each query's own power in dq, whose columns are queries; that of all the queries that a workgroup
 // meets in dk and dv, which sum over them. What is below 2^(-24 - LIFT) of the bound is lost. dv's combined map, whose probabilities of
-// 32768 keys are about 2^-15, is lifted the same way from its bound (4.4e-4 off, now as of 4096 keys). bf16 has fp32's range. The norms of v are a
-// launch before: 8 x 2048 tokens, 6 heads of 128: 6 us of the backward's 300 (25 MB at 4 TB/s), 3 x 683 tokens, 2 of 256: 4.
+// 32768 keys are about 2^-15, is lifted the same way from its bound (4.4e-4 off, now 2.9e-4 as of 4096 keys). bf16 has fp32's range.
+// The norms of v are a launch before: 8 x 2048 tokens, 6 heads of 128: 6 us of the backward's 260 (25 MB at 4 TB/s); 3 x 683, 2 of 256: 4.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T> constexpr bool LIFTED = std::is_same<T, _Float16>::value;
 constexpr int LIFT = 13;   // three binades are left for what D's own rounding adds
@@ -830,7 +831,8 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     }
     const float size = finite_or_0(sqrtf(other_half(sum, true)));
     lift = lift_of(2.f * size * norm_of(a, wk.item, most));
-    const float factor = fmaxf(1.f, finite_or_0(fabsf(lam))), largest = lanes_reduce(query < a.tq ? finite_or_0(size * factor) : 0.f, 64, MaxOp());
+    const float factor = fmaxf(1.f, finite_or_0(fabsf(lam)));
+    const float largest = lanes_reduce(query < a.tq ? finite_or_0(size * factor) : 0.f, 64, MaxOp());
     const float most_lam = lanes_reduce(factor, 64, MaxOp());
     if (lane == 0) a.sizes[(((int64_t)b * a.h + head) * blocks + qblock) * (QB / 32) + wave] = make_float2(largest, most_lam);
   }
@@ -1082,7 +1084,7 @@ __global__ __launch_bounds__(WG) __attribute__((amdgpu_waves_per_eu((waves_bwd<D
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(lam < 0.f ? 1.f : -1.f)));
   };
   float next_minus = minus_of(head);
-  float up = 1.f, back = 1.f, up_p = 1.f, back_p = 1.f;   // what dA - D and the combined map are multiplied by, and the results by as much back
+  float up = 1.f, back = 1.f, up_p = 1.f, back_p = 1.f;   // what dA - D and the combined map are multiplied by, and the sums back
   if constexpr (LIFTED<T>) {
     float size = 0.f, lam = 1.f;
     const int tiles = (a.tq + QB - 1) / QB * (QB / KVT);

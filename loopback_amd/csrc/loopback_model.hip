@@ -540,7 +540,8 @@ __global__ __launch_bounds__(MEAN_LANES) void k_distill_mean(const DistillTerms*
     __syncthreads();
   }
   if (tid == 0) {
-    const float n = fmaxf(s[0].z, 1.f), m = fmaxf(s[0].w, 1.f);   // exact up to 2^24 rows that count; past them, as the other sums, to the tree's ten roundings
+    // exact up to 2^24 rows that count; past them, as the other sums, to the tree's ten roundings
+    const float n = fmaxf(s[0].z, 1.f), m = fmaxf(s[0].w, 1.f);
     const float soft = (1.f - hard) * tau;
     coef[0] = soft / n;
     coef[1] = hard / m;

@@ -606,3 +606,34 @@ def test_results_over_a_cache_are_rounded_once(b, tq, tk, h, hk, dh, dv, dtype):
     ref = M.diff_attention(*(t.double() for t in ts))
     norm = lambda t: (t.double() - ref).norm().item()  # noqa: E731
     assert norm(M.diff_attention(*ts)) <= 1.1 * norm(ref.to(dtype))
+
+
+def test_captured_gradients_follow_their_upstreams():
+    """A captured fp16 pass, whose powers of two come from its tensors: each replay gives the eager pass's bits, on another stream too,
+    for upstreams and values of other sizes and other lengths, eager work between the replays."""
+    ts = operands(3, 300, 300, 4, 2, 64, 128, torch.float16, "token")
+    lengths, dy = ints(300, 20, 0), rnd((3, 300, 4, 128), torch.float16, 9)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in ts]
+        y = M.diff_attention(*leaves, lengths=lengths)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(other, step()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for up, size, n in ((1.0, 1.0, (300, 20, 0)), (2.0 ** -12, 0.5, (3, 150, 64)), (2.0 ** 10, 0.25, (0, 300, 1)), (2.0 ** -3, 1.0, (129, 128, 2))):
+        lengths.copy_(ints(*n))
+        dy.copy_(rnd(dy.shape, torch.float16, 9) * up)
+        ts[2].copy_(rnd(ts[2].shape, torch.float16, 3) * size)
+        want = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for k, (a, b) in enumerate(zip(out, want)):
+            assert torch.equal(a, b), (up, k)
